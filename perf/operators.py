@@ -103,7 +103,8 @@ def _lengths(case):
 def _quantise(x, fmt):
     """[..., D] fp32 -> the codes and the fp32 scale of each row."""
     amax = x.abs().amax(-1)
-    s = (amax / (127.0 if fmt == "int8" else 448.0)).clamp_min(1e-12)
+    # the IEEE fp32 quotient: by way of 64 bits, for torch divides a GPU tensor by a number through its reciprocal
+    s = (amax.double() / (127.0 if fmt == "int8" else 448.0)).float().clamp_min(1e-12)
     y = x / s[..., None]
     if fmt == "int8":
         return torch.round(y).to(torch.int8), s
