@@ -29,6 +29,9 @@ extern "C" {
 #define RH3_DTYPE_F32 2
 #define RH3_DTYPE_F16 3
 
+#define RH3_KV_INT8 0
+#define RH3_KV_E4M3 1
+
 /* Message of the last failed call on this thread ("" if none). */
 const char* rh3_last_error(void);
 /* Library ABI version (increments when a signature changes). */
@@ -450,6 +453,58 @@ int rh3_attention_f8_prepass(const uint16_t* q, int64_t q_ss, int64_t q_sh,
 int rh3_attention_f8_forward(int64_t Sq, int64_t Sk, int64_t H, float scale, int tile,
                              uint16_t* out, int64_t o_ss, int64_t o_sh,
                              void* workspace, int64_t workspace_bytes, hipStream_t stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * Paged key / value cache: rows of keys and values kept as INT8 or e4m3 codes with one fp32 scale per row and head, and
+ * attention that reads them there. No counterpart in the reference.
+ *
+ * A cache is `pages` pages of `page` positions (16, 32, 64, 128 or 256): codes k, v [pages][heads][page][dim] (dim 64 or
+ * 128; positions contiguous, page and head strides in elements, multiples of 16) and scales k_scale, v_scale
+ * [pages][heads][page] (strides multiples of 4), all 16-byte aligned. The value of a code is code * scale.
+ *
+ * A call names `batch` sequences: position p of sequence b lies in page table[b * table_stride + p / page] (width entries; an
+ * entry outside [0, pages) is an absent page, whose positions hold nothing); lens[b] positions are cached (clamped to
+ * [0, width * page]); its rows in the call are cu[b] .. cu[b + 1] of `rows` (cu NULL: rows / batch each) and are its last
+ * positions: row i of n is position lens[b] - n + i. Rows behind cu[batch] are neither read nor written. table, lens and cu are
+ * device memory and may change between replays of a captured call; no content of theirs leads outside the buffers.
+ * Rows [rows][heads][dim]: last dim contiguous, strides multiples of 8, 16-byte aligned.
+ * ------------------------------------------------------------------------------------------- */
+typedef struct rh3_kv_cache {
+  void* k;
+  void* v;
+  float* k_scale;
+  float* v_scale;
+  int64_t page_stride, head_stride;
+  int64_t scale_page_stride, scale_head_stride;
+  int64_t pages, heads, page, dim, format;
+} rh3_kv_cache;
+
+/* Quantizes rows of k and v (bf16, fp16 or fp32) into their positions: s = max(amax / QMAX, 1e-12) (127 or 448), code =
+ * round_half_even(x / s); a row with an infinity or a NaN gets s = NaN and codes 0. Rows whose position is negative or in an
+ * absent page are skipped. A position that several rows of one call name holds codes and scale of any of them. */
+int rh3_kv_write(const rh3_kv_cache* cache, const void* k, int64_t k_st, int64_t k_sh, const void* v, int64_t v_st,
+                 int64_t v_sh, int dtype, int64_t rows, const int32_t* table, int64_t table_stride, int64_t width,
+                 const int32_t* lens, const int32_t* cu, int64_t batch, hipStream_t stream);
+
+/* The values of the same rows, code * scale rounded once to dtype; 0 where kv_write would have skipped. */
+int rh3_kv_read(const rh3_kv_cache* cache, void* k, int64_t k_st, int64_t k_sh, void* v, int64_t v_st, int64_t v_sh,
+                int dtype, int64_t rows, const int32_t* table, int64_t table_stride, int64_t width, const int32_t* lens,
+                const int32_t* cu, int64_t batch, hipStream_t stream);
+
+/* out = softmax(scale q k^T) v over a sequence's cached positions (causal: row i of n sees positions up to
+ * lens[b] - n + i), q and out [rows][q_heads][dim] bf16 or fp16, query head h reads K/V head h / (q_heads / heads); lse
+ * [rows][q_heads] fp32 or NULL: the natural log of the sum of exp(scale q.k). A row that sees no key gives 0 and -inf; one
+ * that sees a NaN key or value gives NaN. prefix_len > 0: every row also sees the first prefix_len positions of the pages
+ * prefix[], which come before the sequences' own and are read once for the batch. out may lie exactly over q.
+ * The workspace holds the parts of rows whose keys several workgroups share; how keys are split depends on the sizes, lengths
+ * and the CU count, and with it the last bits of the result; the same call gives the same bits. */
+int64_t rh3_kv_attention_workspace_bytes(const rh3_kv_cache* cache, int64_t q_heads, int64_t rows, int64_t width,
+                                         int64_t batch, int even, int64_t prefix_len);
+int rh3_kv_attention(const rh3_kv_cache* cache, const void* q, int64_t q_st, int64_t q_sh, int64_t q_heads, int dtype,
+                     int64_t rows, const int32_t* table, int64_t table_stride, int64_t width, const int32_t* lens,
+                     const int32_t* cu, int64_t batch, int causal, float scale, void* out, int64_t o_st, int64_t o_sh,
+                     float* lse, const int32_t* prefix, int64_t prefix_len, void* workspace, int64_t workspace_bytes,
+                     hipStream_t stream);
 
 #ifdef __cplusplus
 }

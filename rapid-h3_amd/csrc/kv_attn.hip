@@ -1,0 +1,287 @@
+// Attention over the paged cache: joining the parts that the token and chunk kernels leave, and the entry points.
+#include "kv_attn.hpp"
+
+namespace rh3 {
+namespace kv {
+namespace {
+
+constexpr int NT = 256;
+
+// One of up to two sources of a row's parts (a shared prefix, and the sequence's own keys)
+struct Source {
+  AttnArgs a;
+  int chunk, rows;    // kernel, rows of its tiles
+};
+
+// the parts of one query row: slot(i), i < count, and the row in each slot
+struct Parts {
+  int64_t first, next, step;
+  int count, row;
+  __device__ __forceinline__ int64_t slot(int i) const { return i == 0 ? first : next + (i - 1) * step; }
+};
+__device__ __forceinline__ Parts parts_of(const Source& s, int b, const Seq& q, int tok, int kvh, int in_group) {
+  Parts p;
+  const int64_t r = static_cast<int64_t>(tok - q.first) * s.a.group + in_group;
+  const int rt = static_cast<int>(r / s.rows);
+  p.row = static_cast<int>(r - static_cast<int64_t>(rt) * s.rows);
+  int64_t before, items;
+  if (s.chunk) {
+    int64_t tiles = 0;
+    const int lane = threadIdx.x & 63;
+    for (int at = 0; at < b; at += 64) {
+      int64_t n = at + lane < b ? (static_cast<int64_t>(seq_at(s.a.s, at + lane).n) * s.a.group + s.rows - 1) / s.rows : 0;
+#pragma unroll
+      for (int d = 32; d; d >>= 1) n += __shfl_xor(n, d);
+      tiles += n;
+    }
+    p.first = (static_cast<int64_t>(kvh) * s.a.tiles + tiles + rt) * s.a.splits;
+    p.next = p.first + 1;
+    p.step = 1;
+    p.count = tiles + rt < s.a.tiles ? s.a.splits : 0;   // (a cu that falls can count rows more than once)
+    return p;
+  }
+  const Work w = all_work(s.a, s.rows, b, before, items);
+  const SeqWork sw = work_of(s.a, q, s.rows);
+  const int64_t item = static_cast<int64_t>(kvh) * sw.row_tiles + rt;
+  const int64_t u0 = before + item * sw.key_tiles;
+  const int w0 = share_of(w, u0), w1 = share_of(w, u0 + sw.key_tiles - 1);
+  p.step = 2;
+  p.next = 2 * (static_cast<int64_t>(w0) + 1);
+  p.first = 2 * static_cast<int64_t>(w0) + 1;
+  p.count = w1 - w0 + 1;
+  if (w0 == w1) {
+    p.first = 2 * static_cast<int64_t>(s.a.wgs) + items + item;
+    p.count = s.a.keep && items + item < s.a.items ? 1 : 0;
+  }
+  return p;
+}
+
+// A query row of one head on WPR waves, each of which takes every WPR-th part: the parts' largest reference, then their sums
+// scaled to it. Bound by latency (a few KB a row).
+template <int D, int WPR>
+__global__ void __launch_bounds__(NT) join_kernel(Source own, Source prefix, int has_prefix) {
+  constexpr int EPL = D / 64;
+  __shared__ float so[NT / 64][D];
+  __shared__ float sl[NT / 64];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int heads = own.a.c.heads * own.a.group;
+  const int64_t id = static_cast<int64_t>(blockIdx.x) * (NT / 64 / WPR) + wave / WPR;
+  const int tok = static_cast<int>(id / heads), hd = static_cast<int>(id - static_cast<int64_t>(tok) * heads);
+  if (tok >= own.a.s.rows) return;             // WPR = 4: the whole workgroup, before its barrier
+  const int kvh = hd / own.a.group, ig = hd - kvh * own.a.group;
+  Seq q;
+  const int b = __builtin_amdgcn_readfirstlane(seq_of_row<64>(own.a.s, tok, q));
+  if (b < 0) return;                           // a row that no sequence has stays as it is
+  Parts p[2];
+  p[0] = parts_of(own, b, q, tok, kvh, ig);
+  p[1].count = 0;
+  if (has_prefix) {
+    const Seq all = seq_at(prefix.a.s, 0);
+    p[1] = parts_of(prefix, 0, all, tok, kvh, ig);
+  }
+  if (p[0].count + p[1].count == 0) return;    // one workgroup completed it
+  float top = -INFINITY;
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const AttnArgs& a = k ? prefix.a : own.a;
+    const int R = k ? prefix.rows : own.rows;
+    for (int i = lane; i < p[k].count; i += 64) top = fmaxf(top, a.part_ml[(p[k].slot(i) * R + p[k].row) * 2]);
+  }
+  top = wave_max(top);
+  float o[EPL] = {}, sum = 0.0f;
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const AttnArgs& a = k ? prefix.a : own.a;
+    const int R = k ? prefix.rows : own.rows;
+#pragma unroll 4
+    for (int i = wave % WPR; i < p[k].count; i += WPR) {
+      const int64_t at = p[k].slot(i) * R + p[k].row;
+      const float ref = a.part_ml[at * 2], l = a.part_ml[at * 2 + 1];
+      const float f = ref == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ref - top);
+      sum += f * l;
+      const float* po = a.part_o + at * D + EPL * lane;
+      if constexpr (EPL == 2) {
+        const float2 v = *reinterpret_cast<const float2*>(po);
+        o[0] += f * v.x;
+        o[1] += f * v.y;
+      } else {
+        o[0] += f * po[0];
+      }
+    }
+  }
+  if constexpr (WPR > 1) {
+#pragma unroll
+    for (int e = 0; e < EPL; ++e) so[wave][EPL * lane + e] = o[e];
+    if (lane == 0) sl[wave] = sum;
+    __syncthreads();
+    if (wave) return;
+#pragma unroll
+    for (int w = 1; w < WPR; ++w) {
+#pragma unroll
+      for (int e = 0; e < EPL; ++e) o[e] += so[w][EPL * lane + e];
+      sum += sl[w];
+    }
+  }
+  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+  uint16_t* dst = static_cast<uint16_t*>(own.a.out) + tok * own.a.o_st + hd * own.a.o_sh + EPL * lane;
+  if constexpr (EPL == 2) *reinterpret_cast<uint32_t*>(dst) = pack_out(own.a, o[0] * inv, o[1] * inv);
+  else *dst = static_cast<uint16_t>(pack_out(own.a, o[0] * inv, 0.0f));
+  if (own.a.lse && lane == 0)
+    own.a.lse[static_cast<int64_t>(tok) * heads + hd] = sum == 0.0f ? -INFINITY : (__builtin_amdgcn_logf(sum) + top) * 0.6931471805599453f;
+}
+
+// ---------------------------------------------------------------- host: how a call runs
+struct Plan {
+  int chunk, rows;        // kernel, query rows of its tiles
+  int wgs;                // token kernel
+  int tiles, splits;      // chunk kernel
+  int64_t items;          // token kernel: slots for items that one workgroup completes
+  int64_t slots;          // parts it may leave
+};
+
+// rows: of a call; per sequence they are counted as even. keep: a part for every item.
+Plan plan_of(int64_t rows, int64_t batch, bool even, int64_t group, int64_t heads, int64_t cap, bool keep) {
+  const int64_t cus = device_cus() > 0 ? device_cus() : 256;
+  const int64_t mean = (rows * group + batch - 1) / batch;    // query rows of a sequence's K/V head
+  Plan p{};
+  if (mean <= 32) {
+    p.rows = mean <= 16 ? 16 : 32;
+    p.wgs = static_cast<int>(2 * cus);
+    p.items = !keep ? 0 : heads * (even ? batch * ((rows / batch * group + p.rows - 1) / p.rows) : rows * group / p.rows + batch);
+    p.slots = 2 * static_cast<int64_t>(p.wgs) + p.items;
+    return p;
+  }
+  p.chunk = 1;
+  p.rows = 128;
+  const int64_t tiles = even ? batch * ((rows / batch * group + p.rows - 1) / p.rows) : rows * group / p.rows + batch;
+  const int64_t likely = batch * ((mean + p.rows - 1) / p.rows) * heads;
+  int64_t splits = (2 * cus + likely - 1) / likely;
+  const int64_t most = cap / 512;                             // 8 tiles of 64 keys to a range
+  splits = splits > most ? most : splits;
+  p.splits = static_cast<int>(splits < 1 ? 1 : splits);
+  p.tiles = static_cast<int>(tiles);
+  p.slots = p.splits > 1 || keep ? tiles * heads * p.splits : 0;
+  return p;
+}
+int64_t bytes_of(const Plan& p, int64_t dim) { return p.slots * p.rows * (dim + 2) * 4; }
+
+struct Call {
+  Plan own, prefix;
+  int64_t bytes;
+};
+Call call_of(int64_t rows, int64_t q_heads, int64_t heads, int64_t dim, int64_t page, int64_t width, int64_t batch, bool even,
+             int64_t prefix_len) {
+  Call c{};
+  const int64_t group = q_heads / heads;
+  c.own = plan_of(rows, batch, even, group, heads, width * page, prefix_len > 0);
+  c.bytes = bytes_of(c.own, dim);
+  if (prefix_len > 0) {
+    c.prefix = plan_of(rows, 1, true, group, heads, prefix_len, true);
+    c.bytes += bytes_of(c.prefix, dim);
+  }
+  return c;
+}
+
+void launch(const AttnArgs& a, const Plan& p, int fmt, int dim, hipStream_t st) {
+  if (p.chunk) launch_chunk(a, fmt, dim, p.rows, static_cast<int64_t>(p.tiles) * p.splits * a.c.heads, st);
+  else launch_token(a, fmt, dim, p.rows, st);
+}
+
+}  // namespace
+}  // namespace kv
+}  // namespace rh3
+
+using namespace rh3;
+using namespace rh3::kv;
+
+extern "C" int64_t rh3_kv_attention_workspace_bytes(const rh3_kv_cache* cache, int64_t q_heads, int64_t rows, int64_t width,
+                                                    int64_t batch, int even, int64_t prefix_len) {
+  if (!cache || cache->heads < 1 || q_heads < cache->heads || q_heads % cache->heads || rows < 1 || batch < 1 || width < 1) return 0;
+  return call_of(rows, q_heads, cache->heads, cache->dim, cache->page, width, batch, even != 0, prefix_len).bytes;
+}
+
+extern "C" int rh3_kv_attention(const rh3_kv_cache* cache, const void* q, int64_t q_st, int64_t q_sh, int64_t q_heads, int dtype,
+                                int64_t rows, const int32_t* table, int64_t table_stride, int64_t width, const int32_t* lens,
+                                const int32_t* cu, int64_t batch, int causal, float scale, void* out, int64_t o_st, int64_t o_sh,
+                                float* lse, const int32_t* prefix, int64_t prefix_len, void* workspace, int64_t workspace_bytes,
+                                hipStream_t stream) {
+  clear_error();
+  AttnArgs a{};
+  if (const int e = check_cache("kv_attention", cache, a.c)) return e;
+  if (const int e = check_seqs("kv_attention", a.c, table, table_stride, width, lens, cu, batch, rows, a.s)) return e;
+  if (rows == 0) return RH3_OK;
+  RH3_REQUIRE(dtype == RH3_DTYPE_BF16 || dtype == RH3_DTYPE_F16, "kv_attention: query type %d (bf16 or fp16)", dtype);
+  RH3_REQUIRE(q_heads >= a.c.heads && q_heads % a.c.heads == 0, "kv_attention: %lld query heads do not divide over %d K/V heads",
+              static_cast<long long>(q_heads), a.c.heads);
+  RH3_REQUIRE(rows * (q_heads / a.c.heads) <= (int64_t{1} << 30), "kv_attention: %lld rows of %lld heads", static_cast<long long>(rows),
+              static_cast<long long>(q_heads));
+  RH3_REQUIRE(q && out, "kv_attention: null q or out");
+  RH3_REQUIRE(aligned16(q) && aligned16(out) && q_st % 8 == 0 && q_sh % 8 == 0 && o_st % 8 == 0 && o_sh % 8 == 0,
+              "kv_attention: q and out must be 16-byte aligned with strides that are multiples of 8");
+  RH3_REQUIRE(prefix_len >= 0 && prefix_len <= (int64_t{1} << 30) && (prefix_len == 0 || prefix), "kv_attention: prefix of %lld positions without pages",
+              static_cast<long long>(prefix_len));
+  const int dim = static_cast<int>(cache->dim), fmt = static_cast<int>(cache->format);
+  const Call call = call_of(rows, q_heads, a.c.heads, dim, cache->page, width, batch, cu == nullptr, prefix_len);
+  RH3_REQUIRE(call.bytes == 0 || (workspace && aligned16(workspace) && workspace_bytes >= call.bytes),
+              "kv_attention: workspace of %lld bytes needed, %lld given", static_cast<long long>(call.bytes), static_cast<long long>(workspace_bytes));
+  for (const Plan* p : {&call.own, &call.prefix})
+    RH3_REQUIRE(!p->chunk || static_cast<int64_t>(p->tiles) * p->splits * a.c.heads <= MAX_GRID_256, "kv_attention: %lld rows in one call",
+                static_cast<long long>(rows));
+  a.q = q;
+  a.q_st = q_st;
+  a.q_sh = q_sh;
+  a.fp16 = dtype == RH3_DTYPE_F16;
+  a.group = static_cast<int>(q_heads / a.c.heads);
+  a.causal = causal != 0;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  a.out = out;
+  a.o_st = o_st;
+  a.o_sh = o_sh;
+  a.lse = lse;
+  a.keep = prefix_len > 0;
+
+  float* ws = static_cast<float*>(workspace);
+  auto source = [&](AttnArgs x, const Plan& p) {
+    x.items = p.items;
+    x.wgs = p.wgs;
+    x.splits = p.splits;
+    x.tiles = p.tiles;
+    x.part_o = ws;
+    x.part_ml = ws ? ws + p.slots * p.rows * dim : nullptr;
+    ws = ws ? ws + p.slots * p.rows * (dim + 2) : nullptr;
+    return Source{x, p.chunk, p.rows};
+  };
+  const Source own = source(a, call.own);
+  Source pre{};
+  if (prefix_len > 0) {
+    AttnArgs x = a;
+    x.s.table = prefix;
+    x.s.table_stride = 0;
+    x.s.lens = nullptr;
+    x.s.cu = nullptr;
+    x.s.width = static_cast<int>((prefix_len + cache->page - 1) / cache->page);
+    x.s.batch = 1;
+    x.s.per = x.s.rows;
+    x.s.fixed_len = static_cast<int>(prefix_len);
+    x.s.cap = x.s.width << x.c.log2page;
+    x.causal = 0;
+    pre = source(x, call.prefix);
+    launch(pre.a, call.prefix, fmt, dim, stream);
+    if (const int e = launch_status("kv_attention (prefix)")) return e;
+  }
+  launch(own.a, call.own, fmt, dim, stream);
+  if (const int e = launch_status("kv_attention")) return e;
+  if (call.bytes == 0) return RH3_OK;
+  // few rows with up to hundreds of parts each: a workgroup to a row; many rows with few parts: a wave
+  const int64_t ids = rows * q_heads;
+  const bool wide = !call.own.chunk && !(prefix_len > 0 && call.prefix.chunk);
+  const int64_t grid = wide ? ids : (ids + 3) / 4;
+  RH3_REQUIRE(grid <= MAX_GRID_256, "kv_attention: %lld rows in one call", static_cast<long long>(rows));
+  auto go = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(grid)), dim3(NT), 0, stream, own, pre, static_cast<int>(prefix_len > 0));
+  };
+  if (dim == 128) wide ? go(join_kernel<128, 4>) : go(join_kernel<128, 1>);
+  else wide ? go(join_kernel<64, 4>) : go(join_kernel<64, 1>);
+  return launch_status("kv_attention (join)");
+}

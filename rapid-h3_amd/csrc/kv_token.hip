@@ -1,0 +1,366 @@
+// Attention of few query rows over the paged cache: single tokens of a batch, or a few tokens each.
+//
+// Bound by the cache's bytes: 2 (dim + 4) per K/V head and position. A wave takes 32 keys at a time, for up to 32 query rows of
+// the K/V head, straight from memory to registers, and its matrix instructions' operand order is made to fit what a wide load
+// brings, so nothing passes through LDS:
+//   S^T = K Q^T: lane l holds key l % 16, two (one) 16-byte pieces of its row; the channel order this gives each MFMA step is
+//   given to Q as well. The result has the query row in l % 16 and keys 4 (l / 16) + 0 .. 3 in the registers of both 16-key tiles.
+//   O^T = V^T P^T: those keys are the ones whose P a lane now has; it loads the same keys' values, dim / 16 channels each, and
+//   turns bytes into channel-major f16 by permutes as it converts.
+// While 32 keys are computed the next 32 are on their way. A workgroup's 4 waves take a share's tiles in turn and join through LDS
+// at the end of an item; items that more than one workgroup has worked on are left as parts.
+#include "kv_attn.hpp"
+
+namespace rh3 {
+namespace kv {
+namespace {
+
+constexpr int NT = 256, WAVES = 4;
+
+template <int D>
+struct Tile {
+  uint4 k[2][D / 64];
+  uint32_t v[8][D / 64];
+  float4 ks[2], vs[2];
+};
+
+// the two pages of a 32-key tile (two 16-key halves), -1 where absent
+struct Pages {
+  int p[2];
+};
+__device__ __forceinline__ Pages pages_of(const AttnArgs& a, const int32_t* row, int tile) {
+  Pages r;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int i = min((tile * UNIT_KEYS + 16 * h) >> a.c.log2page, a.s.width - 1);
+    const int p = row[i];
+    r.p[h] = __builtin_amdgcn_readfirstlane(p >= 0 && p < a.c.pages ? p : -1);
+  }
+  return r;
+}
+
+template <int D>
+__device__ __forceinline__ void load_tile(const AttnArgs& a, int kvh, int tile, const Pages& pg, Tile<D>& t) {
+  const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int64_t p = max(pg.p[h], 0);
+    const int off = (tile * UNIT_KEYS + 16 * h) & ((1 << a.c.log2page) - 1);
+    const int64_t code = p * a.c.page_stride + kvh * a.c.head_stride + off * D;
+    const int64_t scale = p * a.c.spage_stride + kvh * a.c.shead_stride + off;
+    const uint8_t* kb = a.c.k + code;
+    const uint8_t* vb = a.c.v + code;
+#pragma unroll
+    for (int c = 0; c < D / 64; ++c) t.k[h][c] = *reinterpret_cast<const uint4*>(kb + l16 * D + 64 * c + 16 * g);
+    t.ks[h] = *reinterpret_cast<const float4*>(a.c.ks + scale + 4 * g);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint8_t* vr = vb + (4 * g + j) * D + l16 * (D / 16);
+      if constexpr (D == 128) {
+        const uint2 w = *reinterpret_cast<const uint2*>(vr);
+        t.v[4 * h + j][0] = w.x;
+        t.v[4 * h + j][1] = w.y;
+      } else {
+        t.v[4 * h + j][0] = *reinterpret_cast<const uint32_t*>(vr);
+      }
+    }
+    t.vs[h] = *reinterpret_cast<const float4*>(a.c.vs + scale + 4 * g);
+  }
+}
+
+// one wave's running state for MT x 16 query rows (row l % 16 of each)
+template <int D, int MT>
+struct State {
+  f4_t o[MT][D / 16];   // o[mt][i][r]: channel (D / 16) (4 (l / 16) + r) + i
+  float ref[MT], sum[MT], vref, ivref;
+};
+
+template <int FMT, int D, int MT>
+__device__ __forceinline__ void compute(const AttnArgs& a, Tile<D>& t, int tile, const Pages& pg, const h8_t (&q)[MT][D / 32],
+                                        const float (&qf)[MT], const int (&lim)[MT], int low, int len, State<D, MT>& st) {
+  const int lane = threadIdx.x & 63, g = lane >> 4;
+  const int kb = tile * UNIT_KEYS;
+  // low: keys that every row sees
+  const bool edge = kb + UNIT_KEYS > low || pg.p[0] < 0 || pg.p[1] < 0;
+  float ks[8] = {t.ks[0].x, t.ks[0].y, t.ks[0].z, t.ks[0].w, t.ks[1].x, t.ks[1].y, t.ks[1].z, t.ks[1].w};
+  float vs[8] = {t.vs[0].x, t.vs[0].y, t.vs[0].z, t.vs[0].w, t.vs[1].x, t.vs[1].y, t.vs[1].z, t.vs[1].w};
+#pragma unroll
+  for (int j = 0; j < 8; ++j) ks[j] = fmaf(vs[j], 0.0f, ks[j]);   // a NaN value marks the rows that see it as a NaN key does
+  int key[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) key[j] = kb + 16 * (j >> 2) + 4 * g + (j & 3);
+
+  f4_t acc[MT][2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+#pragma unroll
+    for (int m = 0; m < MT; ++m) acc[m][h] = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int c = 0; c < D / 64; ++c) {
+      const uint4 w = t.k[h][c];
+      const h8_t k0 = f16x8<FMT>(w.x, w.y), k1 = f16x8<FMT>(w.z, w.w);
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        acc[m][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, q[m][2 * c], acc[m][h], 0, 0, 0);
+        acc[m][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, q[m][2 * c + 1], acc[m][h], 0, 0, 0);
+      }
+    }
+  }
+  if (edge) {
+    // what lies behind the sequence or in an absent page may be anything: its scales and, where codes can be NaN, its values go
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if (key[j] >= len || pg.p[j >> 2] < 0) {
+        vs[j] = 0.0f;
+        if constexpr (FMT == E4M3) {
+#pragma unroll
+          for (int c = 0; c < D / 64; ++c) t.v[j][c] = 0u;
+        }
+      }
+    }
+  }
+  float x[MT][8], top[MT], vtop = 0.0f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) vtop = fmaxf(vtop, vs[j]);
+  bool move = vtop > st.vref;
+#pragma unroll
+  for (int m = 0; m < MT; ++m) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[m][j] = acc[m][j >> 2][j & 3] * (ks[j] * qf[m]);
+    if (edge) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (key[j] >= lim[m] || pg.p[j >> 2] < 0) x[m][j] = -INFINITY;
+    }
+    top[m] = x[m][0];
+#pragma unroll
+    for (int j = 1; j < 8; ++j) top[m] = fmaxf(top[m], x[m][j]);
+    move |= top[m] > st.ref[m] + REF_STALE;
+  }
+  if (__builtin_amdgcn_ballot_w64(move)) {
+    const float vt = across_max<true>(vtop);
+    float vscale = 1.0f;
+    if (vt > st.vref) {
+      const float nv = pow2_over(vt);
+      vscale = st.vref / nv;
+      st.vref = nv;
+      st.ivref = 1.0f / nv;
+    }
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      const float n = across_max<true>(top[m]);
+      float f = 1.0f;
+      if (n > st.ref[m] + REF_STALE) {
+        f = __builtin_amdgcn_exp2f(st.ref[m] - (n - REF_UNDER));   // from no keys yet: 2^-inf = 0
+        st.ref[m] = n - REF_UNDER;
+      }
+      st.sum[m] *= f;
+      f *= vscale;
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) st.o[m][i] *= f;
+    }
+  }
+  h8_t p[MT];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) vs[j] *= st.ivref;
+#pragma unroll
+  for (int m = 0; m < MT; ++m) {
+    // a row that has seen no key yet has only -inf here: any finite reference gives it zeros
+    const float ref = st.ref[m] == -INFINITY ? 0.0f : st.ref[m];
+    float y[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float e = __builtin_amdgcn_exp2f(x[m][j] - ref);
+      st.sum[m] += e;
+      y[j] = e * vs[j];
+    }
+    if (edge) {   // a key that the row does not see may hold NaN
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (key[j] >= lim[m]) y[j] = 0.0f;
+    }
+    const uint32_t w[4] = {pack_h2(y[0], y[1]), pack_h2(y[2], y[3]), pack_h2(y[4], y[5]), pack_h2(y[6], y[7])};
+    p[m] = join(__builtin_bit_cast(h2_t, w[0]), __builtin_bit_cast(h2_t, w[1]), __builtin_bit_cast(h2_t, w[2]), __builtin_bit_cast(h2_t, w[3]));
+  }
+#pragma unroll
+  for (int c = 0; c < D / 64; ++c) {
+    uint32_t w[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) w[j] = t.v[j][c];
+    h8_t v[4];
+    f16x8_across<FMT>(w, v);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+        st.o[m][4 * c + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[i], p[m], st.o[m][4 * c + i], 0, 0, 0);
+  }
+}
+
+template <int FMT, int D, int MT>
+__global__ void __launch_bounds__(NT, 2) token_kernel(AttnArgs a) {
+  constexpr int R = 16 * MT, PAD = D + 4;
+  __shared__ float so[WAVES][R][PAD];
+  __shared__ float sm[WAVES][R], sl[WAVES][R];
+  const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int64_t unused, unused2;
+  const Work work = all_work(a, R, -1, unused, unused2);
+  const int wg = blockIdx.x;
+  if (wg >= work.wgs) return;
+  int64_t u = share_begin(work, wg);
+  const int64_t end = share_begin(work, wg + 1);
+
+  while (u < end) {
+    const UnitAt at = seq_of_unit(a, R, u);
+    if (at.b < 0) return;
+    const Seq sq = seq_at(a.s, at.b);
+    const SeqWork sw = work_of(a, sq, R);
+    const int64_t local = u - at.before;
+    const int item = static_cast<int>(local / sw.key_tiles);
+    const int t0 = static_cast<int>(local - static_cast<int64_t>(item) * sw.key_tiles);
+    const int t1 = static_cast<int>(end - u < sw.key_tiles - t0 ? t0 + (end - u) : sw.key_tiles);
+    const int kvh = item / sw.row_tiles, rt = item - kvh * sw.row_tiles;
+    const int rows = sq.n * a.group;
+
+    // query rows: lane l holds row l % 16, channels 64 c + 16 (l / 16) + 0 .. 15 in steps 2 c and 2 c + 1
+    h8_t q[MT][D / 32];
+    float qf[MT];
+    int lim[MT];
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      const int row = rt * R + 16 * m + l16;
+      const bool has = row < rows;
+      const int rr = has ? row : 0;
+      const int tok = rr / a.group, hd = kvh * a.group + rr - tok * a.group;
+      float x[D / 32][8], top = 0.0f;
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c) {
+        load_q8(a, (sq.first + tok) * a.q_st + hd * a.q_sh + 64 * (c >> 1) + 16 * g + 8 * (c & 1), x[c]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          x[c][e] = has ? x[c][e] : 0.0f;
+          top = fmaxf(top, fabsf(x[c][e]));
+        }
+      }
+      const int e = q_exponent(across_max<true>(top));
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c) q[m][c] = q_f16(x[c], e);
+      qf[m] = __builtin_amdgcn_ldexpf(a.scale_log2, -e);
+      lim[m] = a.causal ? min(sq.len, sq.len - sq.n + tok + 1) : sq.len;
+    }
+    const int low = a.causal ? min(sq.len, sq.len - sq.n + (rt * R) / a.group + 1) : sq.len;
+
+    State<D, MT> st;
+    st.vref = 0.0f;
+    st.ivref = 0.0f;
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      st.ref[m] = -INFINITY;
+      st.sum[m] = 0.0f;
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) st.o[m][i] = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    const int32_t* row = a.s.table + at.b * a.s.table_stride;
+    int t = t0 + wave;
+    if (t < t1) {
+      // two tiles in registers: one computed, one loading; the pages of the one after are looked up as it begins to load
+      Tile<D> ta, tb;
+      Pages pa = pages_of(a, row, t), pb = pages_of(a, row, t + WAVES);
+      load_tile<D>(a, kvh, t, pa, ta);
+      while (t + WAVES < t1) {
+        load_tile<D>(a, kvh, t + WAVES, pb, tb);
+        const Pages pc = pages_of(a, row, t + 2 * WAVES);
+        compute<FMT, D, MT>(a, ta, t, pa, q, qf, lim, low, sq.len, st);
+        t += WAVES;
+        if (t + WAVES >= t1) {
+          compute<FMT, D, MT>(a, tb, t, pb, q, qf, lim, low, sq.len, st);
+          t += WAVES;
+          break;
+        }
+        load_tile<D>(a, kvh, t + WAVES, pc, ta);
+        const Pages pd = pages_of(a, row, t + 2 * WAVES);
+        compute<FMT, D, MT>(a, tb, t, pb, q, qf, lim, low, sq.len, st);
+        t += WAVES;
+        pa = pc;
+        pb = pd;
+      }
+      if (t < t1) compute<FMT, D, MT>(a, ta, t, pa, q, qf, lim, low, sq.len, st);
+    }
+    // join the 4 waves
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      const float sum = across_sum<true>(st.sum[m]);
+      if (g == 0) {
+        sm[wave][16 * m + l16] = st.ref[m];
+        sl[wave][16 * m + l16] = sum;
+      }
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int i = 0; i < D / 16; i += 4) {
+          float4 v = make_float4(st.o[m][i][r], st.o[m][i + 1][r], st.o[m][i + 2][r], st.o[m][i + 3][r]);
+          v.x *= st.vref; v.y *= st.vref; v.z *= st.vref; v.w *= st.vref;
+          *reinterpret_cast<float4*>(&so[wave][16 * m + l16][(D / 16) * (4 * g + r) + i]) = v;
+        }
+    }
+    __syncthreads();
+    const bool whole = t0 == 0 && t1 == sw.key_tiles;
+    constexpr int TPR = NT / R, EPT = D / TPR;   // threads to a row, channels to a thread
+    const int rl = threadIdx.x / TPR, d0 = (threadIdx.x % TPR) * EPT;
+    const int rw = rt * R + rl;
+    if (rw < rows) {
+      float top = sm[0][rl];
+#pragma unroll
+      for (int w = 1; w < WAVES; ++w) top = fmaxf(top, sm[w][rl]);
+      float f[WAVES], sum = 0.0f;
+#pragma unroll
+      for (int w = 0; w < WAVES; ++w) {
+        f[w] = sm[w][rl] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(sm[w][rl] - top);
+        sum += f[w] * sl[w][rl];
+      }
+      float o[EPT];
+#pragma unroll
+      for (int e = 0; e < EPT; ++e) {
+        o[e] = 0.0f;
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) o[e] += f[w] * so[w][rl][d0 + e];
+      }
+      if (whole && !a.keep) {
+        const int tok = rw / a.group, hd = kvh * a.group + rw - tok * a.group;
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        uint32_t w[EPT / 2];
+#pragma unroll
+        for (int e = 0; e < EPT; e += 2) w[e / 2] = pack_out(a, o[e] * inv, o[e + 1] * inv);
+        uint16_t* dst = static_cast<uint16_t*>(a.out) + (sq.first + tok) * a.o_st + hd * a.o_sh + d0;
+#pragma unroll
+        for (int e = 0; e < EPT / 2; e += 2) *reinterpret_cast<uint2*>(dst + 2 * e) = make_uint2(w[e], w[e + 1]);
+        if (a.lse && d0 == 0)
+          a.lse[static_cast<int64_t>(sq.first + tok) * a.c.heads * a.group + hd] =
+              sum == 0.0f ? -INFINITY : (__builtin_amdgcn_logf(sum) + top) * 0.6931471805599453f;
+      } else if (!whole || at.items_before + item < a.items) {   // (a cu that falls can count rows more than once)
+        // slots: two to a workgroup (the item that it goes on with, the one that it begins), then one to an item that it completes
+        const int64_t slot = whole ? 2 * static_cast<int64_t>(a.wgs) + at.items_before + item : 2 * static_cast<int64_t>(wg) + (t0 == 0);
+        float* po = a.part_o + (slot * R + rl) * D + d0;
+#pragma unroll
+        for (int e = 0; e < EPT; e += 4) *reinterpret_cast<float4*>(po + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+        if (d0 == 0) *reinterpret_cast<float2*>(a.part_ml + (slot * R + rl) * 2) = make_float2(top, sum);
+      }
+    }
+    u += t1 - t0;
+    if (u < end) __syncthreads();
+  }
+}
+
+}  // namespace
+
+void launch_token(const AttnArgs& a, int fmt, int dim, int rows, hipStream_t st) {
+  auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(a.wgs)), dim3(NT), 0, st, a); };
+  if (fmt == INT8 && dim == 128) rows == 16 ? go(token_kernel<INT8, 128, 1>) : go(token_kernel<INT8, 128, 2>);
+  else if (fmt == INT8) rows == 16 ? go(token_kernel<INT8, 64, 1>) : go(token_kernel<INT8, 64, 2>);
+  else if (dim == 128) rows == 16 ? go(token_kernel<E4M3, 128, 1>) : go(token_kernel<E4M3, 128, 2>);
+  else rows == 16 ? go(token_kernel<E4M3, 64, 1>) : go(token_kernel<E4M3, 64, 2>);
+}
+
+}  // namespace kv
+}  // namespace rh3

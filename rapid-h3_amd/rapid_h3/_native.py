@@ -18,6 +18,14 @@ _F = ctypes.c_float
 _C = ctypes.c_int
 _D = ctypes.c_double
 
+
+class KvCacheDesc(ctypes.Structure):
+    """rh3_kv_cache (include/rh3.h)."""
+    _fields_ = ([(n, _P) for n in ("k", "v", "k_scale", "v_scale")]
+                + [(n, _I) for n in ("page_stride", "head_stride", "scale_page_stride", "scale_head_stride", "pages", "heads",
+                                     "page", "dim", "format")])
+
+
 # name -> argument types, in header order (include/rh3.h)
 SIGNATURES = {
     "rh3_last_error": ([], ctypes.c_char_p),
@@ -75,11 +83,18 @@ SIGNATURES = {
     "rh3_attention_f8_prepass": ([_P, _I, _I, _P, _I, _I, _P, _I, _I, _I, _I, _I, _P, _C, _P, _P, _F, _C, _C, _C,
                                   _P, _I, ctypes.POINTER(ctypes.c_void_p), _P], _C),
     "rh3_attention_f8_forward": ([_I, _I, _I, _F, _C, _P, _I, _I, _P, _I, _P], _C),
+    "rh3_kv_write": ([_P, _P, _I, _I, _P, _I, _I, _C, _I, _P, _I, _I, _P, _P, _I, _P], _C),
+    "rh3_kv_read": ([_P, _P, _I, _I, _P, _I, _I, _C, _I, _P, _I, _I, _P, _P, _I, _P], _C),
+    "rh3_kv_attention_workspace_bytes": ([_P, _I, _I, _I, _I, _C, _I], ctypes.c_int64),
+    "rh3_kv_attention": ([_P, _P, _I, _I, _I, _C, _I, _P, _I, _I, _P, _P, _I, _C, _F, _P, _I, _I, _P, _P, _I, _P, _I,
+                          _P], _C),
 }
 
 RH3_DTYPE_BF16 = 1
 RH3_DTYPE_F32 = 2
 RH3_DTYPE_F16 = 3
+RH3_KV_INT8 = 0
+RH3_KV_E4M3 = 1
 
 _lib = None
 _FN = {}   # entry point name -> bound function, filled by lib()

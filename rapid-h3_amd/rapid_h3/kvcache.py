@@ -1,0 +1,177 @@
+"""A paged, quantised key / value cache and the attention over it, on the HIP kernels (librh3: rh3_kv_*).
+
+For programs that keep keys and values from call to call: the past frames of a video generated in chunks, a prompt's tokens
+in a text encoder in front of the DiT, a long context that many continuations share. Keys and values are quantised once, as
+they are written, by the row quantizers' rule over one head (s = max(amax / QMAX, 1e-12), round half even of x / s, QMAX 127
+or 448), and attention reads the codes where they lie. The reference has no counterpart.
+
+Every call names its sequences alike:
+  table [B, W] int32   the pages of each sequence in order; an entry outside [0, pages) is an absent page
+  lens [B] int32       cached positions of each sequence, the rows of this call included
+  cu [B + 1] int32     where each sequence's rows begin and end among the call's rows; None: the same number each
+The rows of a sequence are its last positions: row i of n is position lens[b] - n + i. The three live on the GPU and are read
+by the kernels, so a captured call follows what is written into them between replays. Rows behind cu[B] stay as they are.
+"""
+import contextlib
+import ctypes
+
+import torch
+
+from . import _native as nat
+
+FP8 = torch.float8_e4m3fn
+_ROW = {torch.bfloat16: nat.RH3_DTYPE_BF16, torch.float16: nat.RH3_DTYPE_F16, torch.float32: nat.RH3_DTYPE_F32}
+_HERE = contextlib.nullcontext()
+
+
+class KVCache:
+    """The pages of one layer: k, v [P, heads, page, dim] int8 or float8_e4m3fn codes, k_scale, v_scale [P, heads, page]
+    fp32 (page 16 to 256, a power of two; dim 64 or 128; views of larger buffers whose pages and heads lie apart are fine,
+    k like v and k_scale like v_scale). A scale is finite and not negative, or NaN. The tensors are kept and used as they are."""
+
+    __slots__ = ("k", "v", "k_scale", "v_scale", "pages", "heads", "page", "dim", "device", "_desc", "_ref")
+
+    def __init__(self, k, v, k_scale, v_scale):
+        if k.ndim != 4 or v.shape != k.shape or v.stride() != k.stride():
+            raise RuntimeError(f"KVCache: k and v must be [pages, heads, page, dim] of one layout, got {tuple(k.shape)} and {tuple(v.shape)}")
+        p, h, n, d = k.shape
+        if k.dtype not in (torch.int8, FP8) or v.dtype != k.dtype:
+            raise TypeError(f"KVCache: codes must be int8 or float8_e4m3fn, got {k.dtype} and {v.dtype}")
+        if d not in (64, 128) or n not in (16, 32, 64, 128, 256):
+            raise RuntimeError(f"KVCache: head dim 64 or 128 and pages of 16, 32, 64, 128 or 256 positions, got {d} and {n}")
+        if k.stride(3) != 1 or k.stride(2) != d:
+            raise RuntimeError("KVCache: a head's positions in a page must be contiguous")
+        for s in (k_scale, v_scale):
+            if s.shape != (p, h, n) or s.dtype != torch.float32 or s.stride(2) != 1:
+                raise RuntimeError("KVCache: scales must be fp32 [pages, heads, page] with a contiguous last dim")
+        if v_scale.stride() != k_scale.stride():
+            raise RuntimeError("KVCache: k_scale and v_scale must have one layout")
+        if not k.is_cuda or any(t.device != k.device for t in (v, k_scale, v_scale)):
+            raise RuntimeError("KVCache: the four tensors must be on one GPU (no CPU path)")
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.pages, self.heads, self.page, self.dim, self.device = p, h, n, d, k.device
+        self._desc = nat.KvCacheDesc(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), k.stride(0), k.stride(1),
+                                     k_scale.stride(0), k_scale.stride(1), p, h, n, d,
+                                     nat.RH3_KV_INT8 if k.dtype == torch.int8 else nat.RH3_KV_E4M3)
+        self._ref = ctypes.addressof(self._desc)
+
+
+def kv_cache(pages, heads, page=64, dim=128, dtype=torch.int8, device="cuda"):
+    """A new cache of zeros."""
+    def codes():
+        return torch.zeros((pages, heads, page, dim), dtype=torch.int8, device=device).view(dtype)
+
+    def scales():
+        return torch.zeros((pages, heads, page), dtype=torch.float32, device=device)
+    return KVCache(codes(), codes(), scales(), scales())
+
+
+def _on(device):
+    """The tensors' GPU as the current one for a launch, where it is another."""
+    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def _seqs(name, cache, table, lens, cu, dev):
+    """The sequences' arguments of a call after its rows: table, its stride and width, lens, cu, batch."""
+    if table.ndim != 2 or table.dtype != torch.int32 or table.stride(1) != 1:
+        raise RuntimeError(f"{name}: table must be int32 [batch, pages of a sequence] with a contiguous last dim")
+    b, w = table.shape
+    if lens.dtype != torch.int32 or lens.shape != (b,) or not lens.is_contiguous():
+        raise RuntimeError(f"{name}: lens must be contiguous int32 [{b}]")
+    if table.device != dev or lens.device != dev or cache.device != dev:
+        raise RuntimeError(f"{name}: the cache, the rows, table and lens must be on one GPU")
+    if cu is None:
+        return table.data_ptr(), table.stride(0), w, lens.data_ptr(), None, b
+    if cu.dtype != torch.int32 or cu.shape != (b + 1,) or not cu.is_contiguous() or cu.device != dev:
+        raise RuntimeError(f"{name}: cu must be contiguous int32 [{b + 1}] on the rows' GPU")
+    return table.data_ptr(), table.stride(0), w, lens.data_ptr(), cu.data_ptr(), b
+
+
+def _check_rows(name, what, x, heads, dim):
+    if x.ndim != 3 or x.shape[2] != dim or x.shape[1] != heads or x.stride(2) != 1:
+        raise RuntimeError(f"{name}: {what} must be [rows, {heads}, {dim}] with a contiguous last dim, got {tuple(x.shape)}")
+    if not x.is_cuda:
+        raise RuntimeError(f"{name}: {what} must be on a GPU (no CPU path)")
+
+
+def kv_write(cache, k, v, table, lens, cu=None):
+    """Quantise rows k, v [rows, heads, dim] (bf16, fp16 or fp32, strided ok) into their positions. Rows at a negative
+    position or in an absent page are skipped; a row that holds an infinity or a NaN is kept as NaN (its scale). Pages that
+    sequences share must not be written by more than one of them in a call."""
+    _check_rows("kv_write", "k", k, cache.heads, cache.dim)
+    _check_rows("kv_write", "v", v, cache.heads, cache.dim)
+    if k.shape != v.shape or k.dtype != v.dtype or k.dtype not in _ROW or v.device != k.device:
+        raise TypeError("kv_write: k and v must be of one shape, device and type (bf16, fp16 or fp32)")
+    seqs = _seqs("kv_write", cache, table, lens, cu, k.device)
+    with _on(k.device):
+        nat.call("rh3_kv_write", cache._ref, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
+                 _ROW[k.dtype], k.shape[0], *seqs, nat.stream(k.device))
+
+
+def kv_read(cache, table, lens, cu=None, rows=None, dtype=torch.bfloat16, out=None):
+    """The values (code * scale, rounded once to dtype) of the last cu[b + 1] - cu[b] positions of each sequence, packed as
+    kv_write takes them: k, v [rows, heads, dim]. rows: how many in all (cu[B], which only the GPU knows; without cu by
+    default one of each sequence). Positions that hold nothing read as 0. out: a pair of tensors to write into."""
+    if out is None:
+        n = table.shape[0] if rows is None else int(rows)
+        if dtype not in _ROW:
+            raise TypeError(f"kv_read: bf16, fp16 or fp32 values, got {dtype}")
+        alloc = torch.empty if cu is None else torch.zeros      # rows that no sequence has are not written
+        k, v = (alloc((n, cache.heads, cache.dim), dtype=dtype, device=cache.device) for _ in range(2))
+    else:
+        k, v = out
+        _check_rows("kv_read", "out", k, cache.heads, cache.dim)
+        _check_rows("kv_read", "out", v, cache.heads, cache.dim)
+        if k.shape != v.shape or k.dtype != v.dtype or k.dtype not in _ROW or v.device != k.device:
+            raise TypeError("kv_read: out must be two tensors of one shape, device and type (bf16, fp16 or fp32)")
+    seqs = _seqs("kv_read", cache, table, lens, cu, k.device)
+    with _on(k.device):
+        nat.call("rh3_kv_read", cache._ref, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
+                 _ROW[k.dtype], k.shape[0], *seqs, nat.stream(k.device))
+    return k, v
+
+
+def _attention(name, q, cache, prefix, prefix_len, table, lens, cu, causal, scale, out, lse):
+    if q.ndim != 3 or q.shape[2] != cache.dim or q.stride(2) != 1 or q.shape[1] % cache.heads or not q.shape[1]:
+        raise RuntimeError(f"{name}: q must be [rows, a multiple of {cache.heads} heads, {cache.dim}] with a contiguous last dim, got "
+                           f"{tuple(q.shape)}")
+    if q.dtype != torch.bfloat16 and q.dtype != torch.float16:
+        raise TypeError(f"{name}: q must be bf16 or fp16, got {q.dtype}")
+    if not q.is_cuda:
+        raise RuntimeError(f"{name}: q must be on a GPU (no CPU path)")
+    dev = q.device
+    t, hq, d = q.shape
+    seqs = _seqs(name, cache, table, lens, cu, dev)
+    alloc = torch.empty if cu is None else torch.zeros          # rows that no sequence has are not written
+    if out is None:
+        out = alloc((t, hq, d), dtype=q.dtype, device=dev)
+    elif out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1 or out.device != dev:
+        raise RuntimeError(f"{name}: out must be like q, with a contiguous last dim")
+    sums = alloc((t, hq), dtype=torch.float32, device=dev) if lse else None
+    n = nat.lib().rh3_kv_attention_workspace_bytes(cache._ref, hq, t, seqs[2], seqs[5], int(cu is None), prefix_len)
+    ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
+    with _on(dev):
+        nat.call("rh3_kv_attention", cache._ref, q.data_ptr(), q.stride(0), q.stride(1), hq, _ROW[q.dtype], t, *seqs, int(causal),
+                 d ** -0.5 if scale is None else scale, out.data_ptr(), out.stride(0), out.stride(1), nat.ptr(sums),
+                 nat.ptr(prefix), prefix_len, nat.ptr(ws), n, nat.stream(dev))
+    return (out, sums) if lse else out
+
+
+def kv_attention(q, cache, table, lens, cu=None, causal=True, scale=None, out=None, lse=False):
+    """Attention of q [rows, q heads, dim] (bf16 or fp16, strided ok) over the cached positions of each row's sequence ->
+    out like q; query head h reads K/V head h // (q heads // heads). causal: row i of n sees positions up to
+    lens[b] - n + i. scale: dim ** -0.5 by default. lse=True: also the log-sum-exp [rows, q heads] fp32 of the scaled scores.
+    A row that sees no key gives 0 and -inf."""
+    return _attention("kv_attention", q, cache, None, 0, table, lens, cu, causal, scale, out, lse)
+
+
+def kv_attention_shared(q, cache, prefix, prefix_len, table, lens, cu=None, causal=True, scale=None, out=None, lse=False):
+    """kv_attention of a batch whose sequences all begin with the first prefix_len (an int) positions of the pages `prefix`
+    (int32 [pages]): every row sees them, then its sequence's own positions (table, lens: without the prefix). The prefix is
+    read once for the whole batch."""
+    prefix_len = int(prefix_len)
+    if prefix.ndim != 1 or prefix.dtype != torch.int32 or not prefix.is_contiguous() or prefix.device != q.device:
+        raise RuntimeError("kv_attention_shared: prefix must be contiguous int32 [pages] on q's GPU")
+    if not 0 <= prefix_len <= prefix.numel() * cache.page:
+        raise RuntimeError(f"kv_attention_shared: prefix_len {prefix_len} does not fit {prefix.numel()} pages of {cache.page}")
+    return _attention("kv_attention_shared", q, cache, prefix, prefix_len, table, lens, cu, causal, scale, out, lse)

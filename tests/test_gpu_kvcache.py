@@ -1,0 +1,533 @@
+"""The paged, quantised key / value cache (rapid_h3.kvcache) on the GPU: codes and scales bit for bit against the plain
+restatement, values read back, attention (both kernels, whole and in parts, with and without a shared prefix) against float64
+over the stored values."""
+import math
+
+import pytest
+import torch
+
+from oracle import kvcache as ok
+from rapid_h3 import kvcache as kv
+
+pytestmark = pytest.mark.gpu
+
+I8, F8 = torch.int8, torch.float8_e4m3fn
+BF, HF, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+def _gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def _pool(dev, fmt, pages, heads, page, dim, seed, garbage=False):
+    """A cache full of quantised random values; garbage: full of what an unwritten pool may hold instead (NaN codes, NaN and
+    infinite scales)."""
+    if garbage:
+        k, v = (torch.full((pages, heads, page, dim), 0x7f, dtype=torch.uint8, device=dev).view(fmt) for _ in range(2))
+        ks = torch.full((pages, heads, page), math.nan, device=dev)
+        ks[:, :, ::3] = math.inf
+        return kv.KVCache(k, v, ks, ks.clone())
+    g = _gen(seed)
+    kc = 2.0 * torch.randn(1, heads, 1, dim, generator=g)
+    k, ks = ok.quantise(torch.randn(pages, heads, page, dim, generator=g) + kc, fmt)
+    v, vs = ok.quantise(torch.randn(pages, heads, page, dim, generator=g) * torch.exp(torch.randn(pages, heads, page, 1, generator=g)), fmt)
+    return kv.KVCache(*(t.to(dev) for t in (k, v, ks, vs)))
+
+
+def _tables(pages, width, batch, seed):
+    """Disjoint pages in any order, one list per sequence."""
+    p = torch.randperm(pages, generator=_gen(seed + 99)).tolist()
+    return [p[b * width:(b + 1) * width] for b in range(batch)]
+
+
+def _i32(x, dev):
+    return torch.tensor(x, dtype=torch.int32, device=dev)
+
+
+def _check(out, ref, mag, err, terms):
+    """|out - ref| within the output's rounding (half a step of its type), `terms` f16 roundings of the weights and values
+    (2^-11 each of sum p |v|), and the scores' error e (at most (exp(2 e) - 1) of the same sum)."""
+    eps = torch.finfo(out.dtype).eps / 2
+    o = out.double()
+    known = ~torch.isnan(ref)
+    assert torch.equal(torch.isnan(o), ~known)
+    tol = eps * ref.abs() * 1.01 + (terms * 2.0 ** -11 + torch.expm1(2 * err)[..., None]) * mag * 1.05 + 1e-30
+    bad = known & ((o - ref).abs() > tol)
+    assert not bad.any(), (int(bad.sum()), float(((o - ref).abs() / tol)[known].max()))
+
+
+def _check_lse(lse, ref, err):
+    known = ~torch.isnan(ref)
+    assert torch.equal(torch.isnan(lse), ~known)
+    e = lse.double()
+    inf = known & torch.isinf(ref)
+    assert torch.equal(e[inf], ref[inf])
+    fin = known & ~inf
+    tol = err + 2.0 ** -22 * ref.abs() + 2.0 ** -21
+    assert ((e - ref).abs() <= tol)[fin].all(), float(((e - ref).abs() / tol)[fin].max())
+
+
+# ---------------------------------------------------------------- writing and reading
+def _rows(n, heads, dim, dtype, seed, strided, dev):
+    g = _gen(seed)
+    x = torch.randn(n, heads, dim, generator=g) * torch.exp(2 * torch.randn(n, heads, 1, generator=g))
+    x = x.to(dtype).to(dev)
+    if strided:   # a view of a wider buffer: heads and rows apart
+        w = torch.zeros(n, heads, dim + 8, dtype=dtype, device=dev)
+        w[..., :dim] = x
+        x = w[..., :dim]
+    return x
+
+
+@pytest.mark.parametrize("fmt", [I8, F8])
+@pytest.mark.parametrize("dtype", [BF, HF, F32])
+@pytest.mark.parametrize("heads,dim,page,lens,new,strided", [
+    (3, 128, 64, [1], [1], False),
+    (1, 64, 16, [17, 5, 33], [17, 3, 16], True),
+    (2, 128, 32, [0, 40, 7, 64], [0, 33, 9, 1], False),        # a sequence without rows, one with more rows than positions
+    (5, 64, 256, [300], [300], True),
+    (8, 128, 128, [130, 1, 77], [2, 1, 0], False),
+])
+def test_write_and_read(dev, fmt, dtype, heads, dim, page, lens, new, strided):
+    b = len(lens)
+    width = max(-(-max(lens) // page), 1) + 1
+    pages = b * width + 2
+    table = _tables(pages, width, b, 5)
+    if b > 1:
+        table[1][0] = -1                                       # an absent page
+    cu = [0]
+    for n in new:
+        cu.append(cu[-1] + n)
+    rows = cu[-1] + 3                                          # three rows that no sequence has
+    even = len(set(new)) == 1
+    if even:
+        rows = cu[-1]
+    k, v = _rows(rows, heads, dim, dtype, 1, strided, dev), _rows(rows, heads, dim, dtype, 2, strided, dev)
+    c = _pool(dev, fmt, pages, heads, page, dim, 3)
+    want = [t.clone() for t in (c.k.view(torch.uint8), c.v.view(torch.uint8), c.k_scale, c.v_scale)]
+    args = (_i32(table, dev), _i32(lens, dev), None if even else _i32(cu, dev))
+    kv.kv_write(c, k, v, *args)
+    got_k, got_v = kv.kv_read(c, *args, rows=rows, dtype=dtype)
+    keep = torch.full((rows, heads, dim), 7.0, dtype=dtype, device=dev)
+    kept = (keep, keep.clone())
+    kv.kv_read(c, *args, out=kept)
+    for x, codes, scales, got, left in ((k, want[0], want[2], got_k, kept[0]), (v, want[1], want[3], got_v, kept[1])):
+        q, s = ok.quantise(x, fmt)
+        for r, where in enumerate(ok.rows_of(lens, None if even else cu, rows, b)):
+            at = where and ok.slot(table, pages, page, *where)
+            if at:
+                codes[at[0], :, at[1]] = q[r].view(torch.uint8)
+                scales[at[0], :, at[1]] = s[r]
+                value = (q[r].float() * s[r][:, None]).to(dtype)
+                assert torch.equal(got[r], value) and torch.equal(left[r], value), r
+            else:
+                assert (got[r] == 0).all(), r
+                assert (left[r] == (7.0 if where is None else 0.0)).all(), r
+    for x, y in zip(want, (c.k.view(torch.uint8), c.v.view(torch.uint8), c.k_scale, c.v_scale)):
+        assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("fmt", [I8, F8])
+@pytest.mark.parametrize("dtype", [BF, HF, F32])
+def test_write_special_rows(dev, fmt, dtype):
+    """Zeros of both signs, the smallest and largest magnitudes, halfway quotients, infinities and NaN."""
+    d, page = 128, 16
+    big = torch.finfo(dtype).max
+    rows = [torch.zeros(d), -torch.zeros(d), torch.full((d,), torch.finfo(dtype).tiny), torch.full((d,), big),
+            torch.arange(d) - 63.5, (torch.arange(d) - 64.0) * 2.0, torch.randn(d, generator=_gen(0)) * 1e-6,
+            torch.linspace(-448, 448, d), torch.randn(d, generator=_gen(1)), torch.randn(d, generator=_gen(2)),
+            torch.randn(d, generator=_gen(3))]
+    rows[8][5] = math.inf
+    rows[9][127] = math.nan
+    rows[10][0], rows[10][1] = -math.inf, math.nan
+    x = torch.stack(rows)[:, None].to(dtype).to(dev)
+    n = x.shape[0]
+    c = kv.kv_cache(1, 1, page, d, fmt, dev)
+    args = (_i32([[0]], dev), _i32([n], dev))
+    kv.kv_write(c, x, x.flip(0).contiguous(), *args)
+    for y, codes, scales in ((x, c.k, c.k_scale), (x.flip(0), c.v, c.v_scale)):
+        q, s = ok.quantise(y, fmt)
+        assert torch.equal(codes[0, 0, :n].view(torch.uint8), q[:, 0].view(torch.uint8))
+        assert torch.equal(torch.nan_to_num(scales[0, 0, :n], nan=-1.0), torch.nan_to_num(s[:, 0], nan=-1.0))
+    got, _ = kv.kv_read(c, *args, rows=n, dtype=F32)
+    # 127 * fl(max / 127) lies above the largest fp32 value: that row, and only that, may read back as infinite
+    assert torch.isnan(got[8:]).all() and torch.isfinite(got[:3]).all() and torch.isfinite(got[4:8]).all()
+    assert torch.equal(got[3], ok.quantise(x, fmt)[0][3].float() * ok.quantise(x, fmt)[1][3][:, None])
+
+
+def test_write_many_sequences(dev):
+    """More sequences than a wavefront has lanes, some of them without rows: every row finds its own."""
+    b, page, heads, dim = 1500, 16, 2, 64
+    new = [(i * 7) % 4 for i in range(b)]
+    lens = [n + i % 13 for i, n in enumerate(new)]
+    cu = [0]
+    for n in new:
+        cu.append(cu[-1] + n)
+    pages = b
+    table = [[i] for i in range(b)]
+    x = torch.randn(cu[-1], heads, dim, generator=_gen(4)).to(BF).to(dev)
+    c = kv.kv_cache(pages, heads, page, dim, I8, dev)
+    args = (_i32(table, dev), _i32(lens, dev), _i32(cu, dev))
+    kv.kv_write(c, x, -x, *args)
+    q, s = ok.quantise(x, I8)
+    where = ok.rows_of(lens, cu, cu[-1], b)
+    p = torch.tensor([w[0] for w in where], device=dev)
+    o = torch.tensor([w[1] for w in where], device=dev)
+    assert torch.equal(c.k[p, :, o], q) and torch.equal(c.v[p, :, o], -q) and torch.equal(c.k_scale[p, :, o], s)
+    assert int((c.k_scale != 0).sum()) == cu[-1] * heads
+    k, v = kv.kv_read(c, *args, rows=cu[-1])
+    assert torch.equal(k, (q.float() * s[..., None]).to(BF)) and torch.equal(v, -k)
+
+
+# ---------------------------------------------------------------- attention
+CASES = [
+    # hq, hkv, dim, page, lens, new, causal: single tokens
+    (4, 1, 128, 16, [1], [1], True),
+    (8, 8, 128, 64, [15, 16, 17, 31, 32, 33, 63, 64, 65, 127, 129], [1] * 11, True),
+    (7, 1, 64, 32, [100, 0, 1, 257], [1] * 4, True),                     # a sequence with no key
+    (16, 2, 128, 256, [1000, 3, 700], [1] * 3, False),
+    # a few tokens: ragged, more rows than positions (rows that see nothing), sequences without rows
+    (8, 2, 128, 64, [40, 2, 129, 5], [3, 4, 0, 5], True),
+    (6, 2, 64, 16, [200, 33], [5, 5], True),
+    (32, 1, 128, 128, [300, 20], [1, 1], True),                          # 32 rows to a K/V head
+    # many rows
+    (4, 4, 128, 64, [200], [200], True),
+    (6, 2, 128, 32, [300, 70, 1], [130, 70, 1], True),
+    (5, 1, 64, 64, [500, 77], [50, 77], False),
+    (3, 1, 64, 16, [130, 64], [129, 64], True),
+    (8, 1, 128, 128, [40, 400], [60, 17], True),                         # more rows than positions
+    (2, 2, 128, 256, [64, 1024, 0], [64, 65, 40], True),
+]
+
+
+@pytest.mark.parametrize("fmt", [I8, F8])
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("case", range(len(CASES)))
+def test_attention(dev, fmt, dtype, case):
+    hq, hkv, dim, page, lens, new, causal = CASES[case]
+    b = len(lens)
+    width = max(-(-max(lens) // page), 1)
+    pages = b * width + 3
+    table = _tables(pages, width, b, case)
+    cu = [0]
+    for n in new:
+        cu.append(cu[-1] + n)
+    even = len(set(new)) == 1
+    t = cu[-1]
+    c = _pool(dev, fmt, pages, hkv, page, dim, case)
+    q = (2.0 * torch.randn(t, hq, dim, generator=_gen(case + 50))).to(dtype).to(dev)
+    out, lse = kv.kv_attention(q, c, _i32(table, dev), _i32(lens, dev), None if even else _i32(cu, dev), causal=causal, lse=True)
+    ref, rl, mag, err = ok.attention(q, c, table, lens, None if even else cu, causal)
+    _check(out, ref, mag, err, 3.1)
+    _check_lse(lse, rl, err)
+
+
+@pytest.mark.parametrize("fmt", [I8, F8])
+@pytest.mark.parametrize("rows,hq,hkv,lens,page", [
+    (1, 8, 2, [20011], 64),              # one sequence on many workgroups
+    (1, 8, 8, [9000, 31, 4001, 1, 0, 2500], 16),   # uneven histories: items begin and end inside a workgroup's share
+    (2, 14, 2, [5000, 5001, 200], 128),
+    (40, 4, 1, [9001], 64),              # key ranges of the chunk kernel
+    (100, 2, 2, [3000, 20], 32),
+])
+def test_attention_in_parts(dev, fmt, rows, hq, hkv, lens, page):
+    b, dim = len(lens), 128
+    width = -(-max(lens) // page)
+    table = _tables(b * width, width, b, 1)
+    c = _pool(dev, fmt, b * width, hkv, page, dim, 8)
+    q = (2.0 * torch.randn(b * rows, hq, dim, generator=_gen(9))).to(BF).to(dev)
+    args = (_i32(table, dev), _i32(lens, dev))
+    out, lse = kv.kv_attention(q, c, *args, lse=True)
+    ref, rl, mag, err = ok.attention(q, c, table, lens)
+    _check(out, ref, mag, err, 3.1)
+    _check_lse(lse, rl, err)
+    again = kv.kv_attention(q, c, *args)
+    assert torch.equal(out.view(torch.int16), again.view(torch.int16))          # the same bits every time
+
+
+@pytest.mark.parametrize("fmt", [I8, F8])
+@pytest.mark.parametrize("rows,lens,page", [(1, [33, 5, 0], 16), (3, [70, 9], 64), (1, [1000], 32), (70, [90, 71], 16), (80, [40], 32)])
+def test_unwritten_pool_stays_out(dev, fmt, rows, lens, page):
+    """What lies behind the sequences, in absent pages and in rows that a causal limit hides (NaN codes, NaN and infinite
+    scales) reaches no row that does not see it."""
+    b, hq, hkv, dim = len(lens), 4, 2, 128
+    width = max(-(-max(lens) // page), 1) + 1
+    table = _tables(b * width, width, b, 2)
+    c = _pool(dev, fmt, b * width, hkv, page, dim, 0, garbage=True)
+    g = _gen(11)
+    total = sum(lens)
+    x = torch.randn(total, hkv, dim, generator=g).to(BF)
+    y = torch.randn(total, hkv, dim, generator=g).to(BF)
+    cu = [0]
+    for n in lens:
+        cu.append(cu[-1] + n)
+    if lens[0] > 3:        # the last position of the first sequence holds a NaN key, the one before it a NaN value
+        x[cu[1] - 1, 0, 3] = math.nan
+        y[cu[1] - 2, 1, 7] = math.inf
+    args = (_i32(table, dev), _i32(lens, dev))
+    if total:
+        kv.kv_write(c, x.to(dev), y.to(dev), *args, _i32(cu, dev))
+    if lens[0] > page:     # a page in the middle of what is visible goes away
+        table[0][0] = b * width
+    q = torch.randn(b * rows, hq, dim, generator=g).to(BF).to(dev)
+    out, lse = kv.kv_attention(q, c, _i32(table, dev), _i32(lens, dev), lse=True)
+    ref, rl, mag, err = ok.attention(q, c, table, lens)
+    _check(out, ref, mag, err, 3.1)
+    _check_lse(lse, rl, err)
+
+
+@pytest.mark.parametrize("fmt", [I8, F8])
+@pytest.mark.parametrize("b,rows,hq,hkv,prefix,lens,dim,page", [
+    (2, 1, 8, 2, 100, [5, 40], 128, 64),            # few rows on both sides
+    (3, 2, 4, 1, 1777, [0, 3, 200], 64, 16),        # a sequence with nothing of its own
+    (24, 1, 16, 2, 3000, None, 128, 64),            # many rows on the prefix, few on each sequence
+    (2, 70, 4, 2, 333, [90, 75], 128, 32),          # many on both
+    (5, 1, 4, 4, 1, [1, 2, 3, 4, 5], 64, 256),
+    (3, 1, 4, 4, 0, [7, 2, 3], 128, 64),            # no prefix after all
+])
+def test_shared_prefix(dev, fmt, b, rows, hq, hkv, prefix, lens, dim, page):
+    lens = lens or [1 + 17 * i for i in range(b)]
+    width = max(-(-max(lens) // page), 1)
+    pre = -(-prefix // page)
+    pages = b * width + pre + 1
+    table = _tables(pages, width, b, 3)
+    used = {p for t in table for p in t}
+    common = [p for p in range(pages) if p not in used][:pre]
+    c = _pool(dev, fmt, pages, hkv, page, dim, 12)
+    q = (2.0 * torch.randn(b * rows, hq, dim, generator=_gen(13))).to(HF).to(dev)
+    for causal in (True, False):
+        out, lse = kv.kv_attention_shared(q, c, _i32(common, dev), prefix, _i32(table, dev), _i32(lens, dev), causal=causal, lse=True)
+        ref, rl, mag, err = ok.attention(q, c, table, lens, None, causal, prefix=common, prefix_len=prefix)
+        _check(out, ref, mag, err, 3.1)
+        _check_lse(lse, rl, err)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("rows", [1, 50])
+def test_query_magnitudes(dev, dtype, rows):
+    """Query rows of every magnitude their type has, zero rows, and infinite or NaN ones, which change no other row."""
+    c = _pool(dev, I8, 4, 1, 64, 128, 20)
+    top = 100 if dtype == BF else 14
+    q = torch.randn(6 * rows, 1, 128, generator=_gen(21))
+    q *= torch.logspace(-top, 2, 6 * rows, base=2.0)[:, None, None]
+    q[1], q[2, 0, 5], q[3, 0, 0] = 0.0, math.nan, math.inf
+    q = q.to(dtype).to(dev)
+    table, lens = [[0, 2]] * 6, [100] * 6
+    out, lse = kv.kv_attention(q, c, _i32(table, dev), _i32(lens, dev), causal=False, lse=True)
+    ref, rl, mag, err = ok.attention(q, c, table, lens, None, False)
+    assert torch.isnan(out[2]).all() and torch.isnan(lse[2]).all()
+    keep = [i for i in range(6 * rows) if i not in (2, 3)]
+    _check(out[keep], ref[keep], mag[keep], err[keep], 3.1)
+    _check_lse(lse[keep], rl[keep], err[keep])
+
+
+@pytest.mark.parametrize("rows", [1, 60])
+def test_extreme_scores_and_scales(dev, rows):
+    """One key far above the others (their probabilities vanish), whose values are far smaller than theirs: value scales within
+    2^24 of each other keep the weights' full precision."""
+    dim, page, n = 128, 32, 200
+    g = _gen(30)
+    x, y = torch.randn(n, 1, dim, generator=g), torch.randn(n, 1, dim, generator=g)
+    x[77] *= 40.0
+    y *= torch.logspace(-6, 6, n, base=2.0)[torch.randperm(n, generator=g)][:, None, None]
+    y[77] *= 1e-3
+    c = kv.kv_cache(7, 1, page, dim, I8, dev)
+    args = (_i32([[6, 0, 3, 2, 5, 4, 1]], dev), _i32([n], dev))
+    kv.kv_write(c, x.to(dev), y.to(dev), *args)
+    q = torch.cat([3.0 * torch.randn(rows, 2, dim, generator=g) + x[77] / 8]).to(BF).to(dev)
+    out, lse = kv.kv_attention(q, c, *args, lse=True, causal=False)
+    ref, rl, mag, err = ok.attention(q, c, [[6, 0, 3, 2, 5, 4, 1]], [n], None, False)
+    _check(out, ref, mag, err, 3.1)
+    _check_lse(lse, rl, err)
+
+
+def test_layouts(dev):
+    """A cache that is a view of a buffer of several layers, strided queries and output, a wider table, out over q."""
+    pages, heads, page, dim, hq = 9, 2, 32, 128, 6
+    whole = [torch.zeros((pages, 3, heads, page, dim), dtype=torch.int8, device=dev) for _ in range(2)]
+    scale = [torch.zeros((pages, 3, heads, page), device=dev) for _ in range(2)]
+    c = kv.KVCache(whole[0][:, 1], whole[1][:, 1], scale[0][:, 1], scale[1][:, 1])
+    lens, table = [70, 33], [[8, 1, 4, 2], [0, 6, 3, 7]]
+    tab = torch.full((2, 11), -1, dtype=torch.int32, device=dev)
+    tab[:, :4] = _i32(table, dev)
+    ln = _i32(lens, dev)
+    qkv = torch.randn(103, hq + 2 * heads, dim, generator=_gen(40)).to(BF).to(dev)
+    cu = _i32([0, 70, 103], dev)
+    kv.kv_write(c, qkv[:, hq:hq + heads], qkv[:, hq + heads:], tab[:, :4], ln, cu)
+    assert not any(t[:, i].any() for t in whole + scale for i in (0, 2))
+    q = qkv[:, :hq]
+    ref, rl, mag, err = ok.attention(q, c, table, lens, [0, 70, 103])
+    wide = torch.full((103, hq, dim + 64), 5.0, dtype=BF, device=dev)
+    kv.kv_attention(q, c, tab[:, :4], ln, cu, out=wide[..., 64:])
+    _check(wide[..., 64:], ref, mag, err, 3.1)
+    assert (wide[..., :64] == 5.0).all()
+    want = wide[..., 64:].clone()
+    kv.kv_attention(q, c, tab, ln, cu, out=q)                  # the same positions by a longer table; out over q
+    _check(q, ref, mag, err, 3.1)
+    assert torch.equal(q, want)
+
+
+def test_rows_that_no_sequence_has_stay(dev):
+    c = _pool(dev, I8, 4, 1, 16, 64, 41)
+    for rows, cu in ((5, [0, 1, 3]), (90, [0, 40, 83])):
+        q = torch.randn(rows, 2, 64, generator=_gen(42)).to(BF).to(dev)
+        out = torch.full_like(q, 9.0)
+        kv.kv_attention(q, c, _i32([[0, 1], [2, 3]], dev), _i32([20, 30], dev), _i32(cu, dev), out=out)
+        assert (out[cu[-1]:] == 9.0).all() and not (out[:cu[-1]] == 9.0).all(-1).any()
+        ref, _, mag, err = ok.attention(q[:cu[-1]], c, [[0, 1], [2, 3]], [20, 30], cu)
+        _check(out[:cu[-1]], ref, mag, err, 3.1)
+
+
+def test_bad_contents_stay_inside(dev):
+    """Lengths beyond the table, negative ones, page numbers that are none, row offsets that fall or pass the end: clamped or
+    absent, and the sequences beside them keep their results."""
+    pages, page, dim = 6, 16, 64
+    c = _pool(dev, I8, pages, 2, page, dim, 43)
+    before = [t.clone() for t in (c.k, c.v, c.k_scale, c.v_scale)]
+    table = [[0, 1], [-7, 2 ** 31 - 1], [2, pages], [3, 4]]
+    lens = [10 ** 9, 20, 32, -5]
+    for rows in (1, 30):
+        q = torch.randn(4 * rows, 4, dim, generator=_gen(44)).to(BF).to(dev)
+        out = kv.kv_attention(q, c, _i32(table, dev), _i32(lens, dev), causal=False)
+        ref, _, mag, err = ok.attention(q, c, table, [32, 20, 32, 0], None, False)
+        _check(out, ref, mag, err, 3.1)
+        assert (out[rows:2 * rows] == 0).all() and (out[3 * rows:] == 0).all()
+    q = torch.randn(6, 4, dim, generator=_gen(45)).to(BF).to(dev)
+    x = torch.randn(6, 2, dim, generator=_gen(46)).to(BF).to(dev)
+    bad = _i32([2, -3, 5, 1, 99], dev)                         # rows 0 .. 5 of sequence 1 by clamping, 1 .. 5 of sequence 3 again
+    dead = _i32([[-1, pages]] * 4, dev)
+    kv.kv_write(c, x, x, dead, _i32([20] * 4, dev), bad)
+    assert all(torch.equal(a, b) for a, b in zip(before, (c.k, c.v, c.k_scale, c.v_scale)))
+    kv.kv_read(c, dead, _i32([20] * 4, dev), bad, rows=6)
+    kv.kv_attention(q, c, dead, _i32([20] * 4, dev), bad)
+    kv.kv_attention_shared(q, c, _i32([9, -1, 2], dev), 40, dead, _i32([20] * 4, dev), bad)
+    torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("fmt", [I8, F8])
+def test_offsets_past_32_bits(dev, fmt):
+    """Pages beyond 4 GiB of codes."""
+    heads, page, dim = 8, 256, 128
+    pages = (5 << 30) // (heads * page * dim)
+    k, v = (torch.empty((pages, heads, page, dim), dtype=torch.int8, device=dev).view(fmt) for _ in range(2))
+    c = kv.KVCache(k, v, *(torch.empty((pages, heads, page), device=dev) for _ in range(2)))
+    table, lens = [[pages - 1, 0, pages - 2], [1, pages - 3, 2]], [600, 700]
+    cu = [0, 600, 1300]
+    g = _gen(60)
+    x, y = (torch.randn(1300, heads, dim, generator=g).to(BF).to(dev) for _ in range(2))
+    args = (_i32(table, dev), _i32(lens, dev), _i32(cu, dev))
+    kv.kv_write(c, x, y, *args)
+    gk, gv = kv.kv_read(c, *args, rows=1300)
+    for a, b in ((x, gk), (y, gv)):
+        q, s = ok.quantise(a, fmt)
+        assert torch.equal(b, (q.float() * s[..., None]).to(BF))
+    q = torch.randn(2, 8, dim, generator=g).to(BF).to(dev)
+    out = kv.kv_attention(q, c, *args[:2])
+    ref, _, mag, err = ok.attention(q, c, table, lens)
+    _check(out, ref, mag, err, 3.1)
+    q = torch.randn(100, 8, dim, generator=g).to(BF).to(dev)
+    out = kv.kv_attention(q, c, *args[:2])
+    ref, _, mag, err = ok.attention(q, c, table, lens)
+    _check(out, ref, mag, err, 3.1)
+
+
+# ---------------------------------------------------------------- together, streams, graphs
+def test_generation(dev):
+    """A prompt is written and attended in two chunks, then tokens one by one, in a batch of uneven prompts behind a common
+    instruction: every step equals float64 attention over the stored values, and the values are the inputs' to half a step."""
+    b, hq, hkv, dim, page = 3, 8, 2, 128, 16
+    c = kv.kv_cache(40, hkv, page, dim, I8, dev)
+    prefix_len, pre = 50, [39, 38, 37, 36]
+    table = _tables(36, 9, b, 70)
+    tab, ptab = _i32(table, dev), _i32(pre, dev)
+    lens = torch.zeros(b, dtype=torch.int32, device=dev)
+    g = _gen(71)
+    kept = [torch.zeros(0, hkv, dim) for _ in range(b)]
+
+    def rows(n):
+        return (torch.randn(n, h, dim, generator=g).to(BF).to(dev) for h in (hq, hkv, hkv))
+    _, k, v = rows(prefix_len)
+    kv.kv_write(c, k, v, ptab[None], _i32([prefix_len], dev))
+    for new in ([70, 33, 1], [40, 2, 7], [1, 1, 1], [1, 1, 1], [1, 1, 1]):
+        n = _i32(new, dev)
+        cu = torch.cat([torch.zeros(1, dtype=torch.int32, device=dev), n.cumsum(0).int()])
+        lens += n
+        q, k, v = rows(sum(new))
+        kv.kv_write(c, k, v, tab, lens, cu)
+        out, lse = kv.kv_attention_shared(q, c, ptab, prefix_len, tab, lens, cu, lse=True)
+        at = lens.tolist()
+        ref, rl, mag, err = ok.attention(q, c, table, at, cu.tolist(), prefix=pre, prefix_len=prefix_len)
+        _check(out, ref, mag, err, 3.1)
+        _check_lse(lse, rl, err)
+        for i, part in enumerate(k.cpu().split(new)):
+            kept[i] = torch.cat([kept[i], part.float()])
+    whole = torch.cat([torch.zeros(1, dtype=torch.int32, device=dev), lens.cumsum(0).int()])
+    got, _ = kv.kv_read(c, tab, lens, whole, rows=int(whole[-1]), dtype=F32)
+    want = torch.cat(kept)
+    step = want.abs().amax(-1, keepdim=True) / 127
+    assert ((got.cpu() - want).abs() <= step * (0.5 + 2.0 ** -15)).all()
+
+
+def _step(c, q, k, v, tab, lens, ptab=None, prefix_len=0):
+    kv.kv_write(c, k, v, tab, lens)
+    if prefix_len:
+        return kv.kv_attention_shared(q, c, ptab, prefix_len, tab, lens)
+    return kv.kv_attention(q, c, tab, lens)
+
+
+@pytest.mark.parametrize("rows,prefix_len", [(1, 0), (1, 500), (60, 0)])
+def test_captured_steps(dev, rows, prefix_len):
+    """A step captured once follows new inputs, lengths and page tables on every replay; two captured steps run at once on two
+    streams."""
+    b, hq, hkv, dim, page = 2, 4, 2, 128, 32
+    steps = []
+    for which in range(2):
+        c = _pool(dev, I8, 80, hkv, page, dim, 80 + which)
+        g = _gen(81 + which)
+        q, k, v = (torch.randn(b * rows, h, dim, generator=g).to(BF).to(dev) for h in (hq, hkv, hkv))
+        tab, ptab = _i32(_tables(60, 30, b, which), dev), _i32(list(range(60, 76)), dev)
+        lens = _i32([700, 130], dev)
+        args = (c, q, k, v, tab, lens, ptab, prefix_len)
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            _step(*args)
+        torch.cuda.current_stream().wait_stream(s)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = _step(*args)
+        steps.append((graph, out, args, torch.cuda.Stream()))
+    for replay in range(3):
+        want = []
+        for graph, out, (c, q, k, v, tab, lens, ptab, n), _ in steps:
+            for t in (q, k, v):
+                t.copy_(torch.randn(t.shape, generator=_gen(replay + 7)).to(BF))
+            lens.copy_(torch.tensor([60 + 300 * replay, 959 - replay], dtype=torch.int32))
+            tab.copy_(tab.flip(1))
+            want.append(_step(c, q, k, v, tab, lens, ptab, n).clone())
+            out.zero_()
+        torch.cuda.synchronize()
+        for graph, _, _, stream in steps:
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        for (_, out, _, _), w in zip(steps, want):
+            assert torch.equal(out.view(torch.int16), w.view(torch.int16)), replay
+
+
+def test_two_streams(dev):
+    """Two calls at once on streams of their own."""
+    c = _pool(dev, F8, 200, 2, 64, 128, 90)
+    tab, lens = _i32(_tables(200, 100, 2, 9), dev), _i32([6400, 3001], dev)
+    qs = [torch.randn(2, 8, 128, generator=_gen(91 + i)).to(BF).to(dev) for i in range(2)]
+    want = [kv.kv_attention(q, c, tab, lens) for q in qs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in qs]
+    got = [[], []]
+    for _ in range(5):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(kv.kv_attention(qs[i], c, tab, lens))
+    torch.cuda.synchronize()
+    for w, g in zip(want, got):
+        assert all(torch.equal(w, x) for x in g)

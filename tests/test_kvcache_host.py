@@ -1,0 +1,123 @@
+"""CPU tests of the key / value cache's entry points: what they refuse, with which message, before touching the device."""
+import ctypes
+
+import pytest
+import torch
+
+from rapid_h3 import _native as nat
+from rapid_h3 import kvcache as kv
+
+FAKE = 0x1000          # never dereferenced: validation fails first
+
+
+def _desc(**kw):
+    d = dict(k=FAKE, v=FAKE, k_scale=FAKE, v_scale=FAKE, page_stride=4 * 64 * 128, head_stride=64 * 128,
+             scale_page_stride=4 * 64, scale_head_stride=64, pages=10, heads=4, page=64, dim=128, format=0)
+    d.update(kw)
+    return nat.KvCacheDesc(**d)
+
+
+def _write(desc, name="rh3_kv_write", rows=6, k=FAKE, v=FAKE, k_st=512, k_sh=128, dtype=1, table=FAKE, stride=8, width=8, lens=FAKE,
+           cu=None, batch=2):
+    return getattr(nat.lib(), name)(ctypes.addressof(desc), k, k_st, k_sh, v, 512, 128, dtype, rows, table, stride, width, lens, cu,
+                                    batch, None)
+
+
+def _attend(desc, rows=2, q=FAKE, q_st=1024, hq=8, dtype=1, table=FAKE, stride=8, width=8, lens=FAKE, cu=None, batch=2, out=FAKE,
+            prefix=None, prefix_len=0, ws=FAKE, n=1 << 40):
+    return nat.lib().rh3_kv_attention(ctypes.addressof(desc), q, q_st, 128, hq, dtype, rows, table, stride, width, lens, cu, batch, 1,
+                                      0.1, out, 1024, 128, None, prefix, prefix_len, ws, n, None)
+
+
+@pytest.mark.parametrize("change,message", [
+    (dict(k=None), "null cache array"), (dict(v_scale=None), "null cache array"), (dict(format=2), "format"),
+    (dict(dim=96), "head dim 96"), (dict(page=48), "page of 48"), (dict(page=512), "page of 512"), (dict(page=8), "page of 8"),
+    (dict(pages=0), "0 pages"), (dict(heads=0), "0 heads"), (dict(k=FAKE + 8), "16-byte aligned"),
+    (dict(head_stride=100), "16-byte aligned"), (dict(scale_page_stride=6), "16-byte aligned"),
+    (dict(page_stride=-8192), "negative stride"),
+])
+def test_cache_refusals(change, message):
+    for call in (_write, lambda d: _write(d, "rh3_kv_read"), _attend):
+        assert call(_desc(**change)) == 1 and message in nat.last_error(), nat.last_error()
+
+
+@pytest.mark.parametrize("change,message", [
+    (dict(rows=-1), "-1 rows"), (dict(table=None), "null page table"), (dict(lens=None), "null page table"),
+    (dict(batch=0), "0 sequences"), (dict(batch=70000, rows=70000), "70000 sequences"), (dict(rows=7), "do not divide"),
+    (dict(width=0), "page table of 0"), (dict(stride=7), "stride 7"), (dict(width=1 << 25, stride=1 << 25), "page table of"),
+])
+def test_sequence_refusals(change, message):
+    for call in (_write, lambda d, **kw: _write(d, "rh3_kv_read", **kw), _attend):
+        assert call(_desc(), **change) == 1 and message in nat.last_error(), nat.last_error()
+
+
+def test_row_refusals():
+    for name in ("rh3_kv_write", "rh3_kv_read"):
+        for change, message in ((dict(k=None), "null rows"), (dict(v=FAKE + 2), "16-byte aligned"), (dict(k_st=500), "multiples of 8"),
+                                (dict(k_sh=129), "multiples of 8"), (dict(dtype=4), "row type 4")):
+            assert _write(_desc(), name, **change) == 1 and message in nat.last_error(), nat.last_error()
+    for change, message in ((dict(q=None), "null q"), (dict(out=None), "null q or out"), (dict(q=FAKE + 8), "16-byte"),
+                            (dict(q_st=1028), "multiples of 8"), (dict(dtype=2), "query type 2"), (dict(hq=6), "do not divide over"),
+                            (dict(hq=0), "do not divide over"), (dict(prefix_len=5), "without pages"),
+                            (dict(prefix=FAKE, prefix_len=-1), "prefix of -1"), (dict(ws=None), "workspace"), (dict(n=64), "workspace"),
+                            (dict(ws=FAKE + 4), "workspace")):
+        assert _attend(_desc(), **change) == 1 and message in nat.last_error(), nat.last_error()
+
+
+def test_no_rows_is_no_call():
+    assert _write(_desc(), rows=0, k=None, v=None) == 0
+    assert _write(_desc(), "rh3_kv_read", rows=0, k=None, v=None) == 0
+    assert _attend(_desc(), rows=0, q=None, out=None, ws=None, n=0) == 0
+
+
+def test_workspace_holds_every_part():
+    """More rows, positions or a prefix never need less; nothing to compute needs nothing."""
+    size = nat.lib().rh3_kv_attention_workspace_bytes
+    d = ctypes.addressof(_desc())
+    assert size(d, 8, 0, 8, 2, 1, 0) == 0 and size(None, 8, 2, 8, 2, 1, 0) == 0 and size(d, 6, 2, 8, 2, 1, 0) == 0
+    for rows, batch in ((1, 1), (64, 64), (64, 2), (5000, 1)):
+        n = size(d, 8, rows, 2000, batch, 1, 0)
+        assert size(d, 8, rows, 2000, batch, 1, 3000) > n
+        assert size(d, 8, rows, 2000, batch, 0, 0) >= n
+
+
+def test_wrappers_refuse():
+    k = torch.zeros((4, 2, 64, 128), dtype=torch.int8)
+    s = torch.zeros((4, 2, 64))
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        kv.KVCache(k, k, s, s)
+    for bad, message in (((k, k[:, :1], s, s), "one layout"), ((k[..., :96], k[..., :96], s, s), "head dim"),
+                         ((k[:, :, :48], k[:, :, :48], s, s), "pages of"), ((k, k, s[:, :, :32], s), "scales must be"),
+                         ((k, k, s, s.double()), "scales must be"), ((k.transpose(1, 2), k.transpose(1, 2), s, s), "pages of"),
+                         ((k[..., ::2], k[..., ::2], s, s), "contiguous")):
+        with pytest.raises(RuntimeError, match=message):
+            kv.KVCache(*bad)
+    with pytest.raises(TypeError, match="codes"):
+        kv.KVCache(k.float(), k.float(), s, s)
+    with pytest.raises(TypeError, match="codes"):
+        kv.KVCache(k, k.view(torch.float8_e4m3fn), s, s)
+
+    class Cache:
+        heads, dim, page, device = 2, 128, 64, torch.device("cpu")
+    x = torch.zeros((3, 2, 128), dtype=torch.bfloat16)
+    t, n = torch.zeros((3, 1), dtype=torch.int32), torch.ones(3, dtype=torch.int32)
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        kv.kv_write(Cache, x, x, t, n)
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        kv.kv_attention(x, Cache, t, n)
+    with pytest.raises(RuntimeError, match="kv_write: k must be"):
+        kv.kv_write(Cache, x[..., :64], x, t, n)
+    with pytest.raises(RuntimeError, match="multiple of 2 heads"):
+        kv.kv_attention(x[:, :1], Cache, t, n)
+    with pytest.raises(TypeError, match="bf16 or fp16"):
+        kv.kv_attention(x.float(), Cache, t, n)
+    with pytest.raises(RuntimeError, match="does not fit"):
+        kv.kv_attention_shared(x, Cache, torch.zeros(2, dtype=torch.int32), 129, t, n)
+    with pytest.raises(RuntimeError, match="prefix must be"):
+        kv.kv_attention_shared(x, Cache, torch.zeros(2), 1, t, n)
+    with pytest.raises(RuntimeError, match="table must be"):
+        kv._seqs("f", Cache, t.long(), n, None, x.device)
+    with pytest.raises(RuntimeError, match="lens must be"):
+        kv._seqs("f", Cache, t, n[:2], None, x.device)
+    with pytest.raises(RuntimeError, match="cu must be"):
+        kv._seqs("f", Cache, t, n, n, x.device)
