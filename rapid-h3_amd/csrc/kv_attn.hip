@@ -24,7 +24,6 @@ __device__ __forceinline__ Parts parts_of(const Source& s, int b, const Seq& q, 
   const int64_t r = static_cast<int64_t>(tok - q.first) * s.a.group + in_group;
   const int rt = static_cast<int>(r / s.rows);
   p.row = static_cast<int>(r - static_cast<int64_t>(rt) * s.rows);
-  int64_t before, items;
   if (s.chunk) {
     int64_t tiles = 0;
     const int lane = threadIdx.x & 63;
@@ -40,18 +39,20 @@ __device__ __forceinline__ Parts parts_of(const Source& s, int b, const Seq& q, 
     p.count = tiles + rt < s.a.tiles ? s.a.splits : 0;   // (a cu that falls can count rows more than once)
     return p;
   }
-  const Work w = all_work(s.a, s.rows, b, before, items);
-  const SeqWork sw = work_of(s.a, q, s.rows);
+  Block blk;
+  const Work w = dealt(load_blocks(s.a, s.rows, blk), s.a.wgs);
+  while (b >= blk.at + 64) next_block(s.a, s.rows, blk);
+  const SeqItems sw = seq_in(s.a, blk, b - blk.at);
   const int64_t item = static_cast<int64_t>(kvh) * sw.row_tiles + rt;
-  const int64_t u0 = before + item * sw.key_tiles;
+  const int64_t u0 = sw.before + item * sw.key_tiles;
   const int w0 = share_of(w, u0), w1 = share_of(w, u0 + sw.key_tiles - 1);
   p.step = 2;
   p.next = 2 * (static_cast<int64_t>(w0) + 1);
   p.first = 2 * static_cast<int64_t>(w0) + 1;
   p.count = w1 - w0 + 1;
   if (w0 == w1) {
-    p.first = 2 * static_cast<int64_t>(s.a.wgs) + items + item;
-    p.count = s.a.keep && items + item < s.a.items ? 1 : 0;
+    p.first = 2 * static_cast<int64_t>(s.a.wgs) + sw.items_before + item;
+    p.count = s.a.keep && sw.items_before + item < s.a.items ? 1 : 0;
   }
   return p;
 }

@@ -45,13 +45,28 @@ struct AttnArgs {
 constexpr int UNIT_KEYS = 32;
 constexpr int UNIT_MIN = 4;
 
+// Units are counted in 64 bits; a division of what fits 32 bits is done there (a 64-bit one takes some hundred instructions).
+RH3_HD int64_t quotient(int64_t a, int64_t b) {
+  return ((a | b) >> 31) == 0 ? static_cast<int64_t>(static_cast<uint32_t>(a) / static_cast<uint32_t>(b)) : a / b;
+}
 struct Work {
-  int64_t units;             // of all sequences
   int wgs;                   // workgroups that have a share
+  int64_t each, more;        // the first `more` of them have each + 1 units, the others each
 };
-RH3_HD int64_t share_begin(const Work& w, int wg) { return w.units * wg / w.wgs; }
+RH3_HD Work dealt(int64_t units, int wgs) {
+  Work w;
+  const int64_t most = (units + UNIT_MIN - 1) / UNIT_MIN;
+  w.wgs = static_cast<int>(most < wgs ? (most > 0 ? most : 1) : wgs);
+  w.each = quotient(units, w.wgs);
+  w.more = units - w.each * w.wgs;
+  return w;
+}
+RH3_HD int64_t share_begin(const Work& w, int wg) { return w.each * wg + (wg < w.more ? wg : w.more); }
 // the workgroup whose share holds unit u
-RH3_HD int share_of(const Work& w, int64_t u) { return static_cast<int>(((u + 1) * w.wgs - 1) / w.units); }
+RH3_HD int share_of(const Work& w, int64_t u) {
+  const int64_t head = w.more * (w.each + 1);
+  return static_cast<int>(u < head ? quotient(u, w.each + 1) : w.more + quotient(u - head, w.each));
+}
 
 struct SeqWork {
   int row_tiles, key_tiles;
@@ -67,84 +82,84 @@ RH3_HD SeqWork work_of(const AttnArgs& a, const Seq& q, int R) {
   w.units = u < (int64_t{1} << 36) / w.key_tiles ? u * w.key_tiles : int64_t{1} << 36;
   return w;
 }
+
+// Sums over the lanes before and at each one, by lane moves within rows of 16 and two broadcasts over them
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int64_t scan_step(int64_t v) {
+  const int lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, ROWS, 0xf, true);
+  const int hi = __builtin_amdgcn_update_dpp(0, static_cast<int>(v >> 32), CTRL, ROWS, 0xf, true);
+  return v + ((static_cast<int64_t>(hi) << 32) | static_cast<uint32_t>(lo));
+}
 __device__ __forceinline__ int64_t wave_scan(int64_t v) {   // inclusive
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int64_t t = __shfl_up(v, d);
-    if (lane >= d) v += t;
-  }
+  v = scan_step<0x111, 0xf>(v);   // row_shr:1, 2, 4, 8
+  v = scan_step<0x112, 0xf>(v);
+  v = scan_step<0x114, 0xf>(v);
+  v = scan_step<0x118, 0xf>(v);
+  v = scan_step<0x142, 0xa>(v);   // row_bcast:15 into rows 1 and 3
+  v = scan_step<0x143, 0xc>(v);   // row_bcast:31 into rows 2 and 3
   return v;
 }
-__device__ __forceinline__ int64_t uniform64(int64_t v) {
-  return (static_cast<int64_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(v >> 32))) << 32) |
-         static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(v)));
+__device__ __forceinline__ int64_t lane64(int64_t v, int lane) {
+  return (static_cast<int64_t>(__builtin_amdgcn_readlane(static_cast<int>(v >> 32), lane)) << 32) |
+         static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), lane));
 }
 
-// units of all sequences; and, for the sequence b >= 0, those of the sequences before it and their items
-__device__ __forceinline__ Work all_work(const AttnArgs& a, int R, int b, int64_t& before, int64_t& items_before) {
-  const int lane = threadIdx.x & 63;
-  int64_t total = 0;
-  before = items_before = 0;
-  for (int at = 0; at < a.s.batch; at += 64) {
-    int64_t u = 0, it = 0;
-    if (at + lane < a.s.batch) {
-      const SeqWork w = work_of(a, seq_at(a.s, at + lane), R);
-      u = w.units;
-      it = static_cast<int64_t>(a.c.heads) * w.row_tiles;
-    }
-    const bool pre = at + lane < b;
-    int64_t ub = pre ? u : 0, ib = pre ? it : 0;
-#pragma unroll
-    for (int d = 32; d; d >>= 1) {
-      u += __shfl_xor(u, d);
-      if (b > at) {
-        ub += __shfl_xor(ub, d);
-        ib += __shfl_xor(ib, d);
-      }
-    }
-    total += u;
-    before += ub;
-    items_before += ib;
-  }
-  Work w;
-  w.units = uniform64(total);
-  before = uniform64(before);
-  items_before = uniform64(items_before);
-  const int64_t most = (w.units + UNIT_MIN - 1) / UNIT_MIN;
-  w.wgs = static_cast<int>(most < a.wgs ? (most > 0 ? most : 1) : a.wgs);
-  return w;
-}
-
-// the sequence that holds unit u, the units and items before it
-struct UnitAt {
-  int b;
-  int64_t before, items_before;
+// 64 sequences, one to a lane, and the units and items (row tiles of all K/V heads) up to each
+struct Block {
+  int at;                          // the first of them
+  int64_t base, items_base;        // units and items before it
+  Seq seq;
+  int64_t units, items;            // running sums within the block, this lane's included
+  int row_tiles, key_tiles;
+  __device__ __forceinline__ int64_t end() const { return base + lane64(units, 63); }
 };
-__device__ __forceinline__ UnitAt seq_of_unit(const AttnArgs& a, int R, int64_t u) {
-  const int lane = threadIdx.x & 63;
-  int64_t base = 0, ibase = 0;
-  for (int at = 0; at < a.s.batch; at += 64) {
-    int64_t n = 0, it = 0;
-    if (at + lane < a.s.batch) {
-      const SeqWork w = work_of(a, seq_at(a.s, at + lane), R);
-      n = w.units;
-      it = static_cast<int64_t>(a.c.heads) * w.row_tiles;
-    }
-    const int64_t s = wave_scan(n), si = wave_scan(it);
-    const unsigned long long m = __builtin_amdgcn_ballot_w64(base + s > u);
-    if (m) {
-      const int l = __builtin_ctzll(m);
-      UnitAt r;
-      r.b = __builtin_amdgcn_readfirstlane(at + l);
-      r.before = uniform64(base + __shfl(s - n, l));
-      r.items_before = uniform64(ibase + __shfl(si - it, l));
-      return r;
-    }
-    base += __shfl(s, 63);
-    ibase += __shfl(si, 63);
+__device__ __forceinline__ void load_block(const AttnArgs& a, int R, int at, int64_t base, int64_t items_base, Block& b) {
+  const int i = at + (threadIdx.x & 63);
+  b.at = at;
+  b.base = base;
+  b.items_base = items_base;
+  b.seq = Seq{0, 0, 0};
+  SeqWork w{0, 1, 0};
+  if (i < a.s.batch) {
+    b.seq = seq_at(a.s, i);
+    w = work_of(a, b.seq, R);
   }
-  return UnitAt{-1, 0, 0};
+  b.row_tiles = w.row_tiles;
+  b.key_tiles = w.key_tiles;
+  b.units = wave_scan(w.units);
+  b.items = a.keep ? wave_scan(static_cast<int64_t>(a.c.heads) * w.row_tiles) : 0;
+}
+// the first block, and the units of all
+__device__ __forceinline__ int64_t load_blocks(const AttnArgs& a, int R, Block& b) {
+  load_block(a, R, 0, 0, 0, b);
+  int64_t total = b.end();
+  for (int at = 64; at < a.s.batch; at += 64) {
+    Block next;
+    load_block(a, R, at, 0, 0, next);
+    total += next.end();
+  }
+  return total;
+}
+__device__ __forceinline__ void next_block(const AttnArgs& a, int R, Block& b) {
+  load_block(a, R, b.at + 64, b.end(), b.items_base + lane64(b.items, 63), b);
+}
+
+// a sequence of the block by its lane, the same in all lanes
+struct SeqItems {
+  Seq seq;
+  int row_tiles, key_tiles;
+  int64_t before, items_before;    // units, items of the sequences before it
+};
+__device__ __forceinline__ SeqItems seq_in(const AttnArgs& a, const Block& b, int l) {
+  SeqItems r;
+  r.seq.first = __builtin_amdgcn_readlane(b.seq.first, l);
+  r.seq.n = __builtin_amdgcn_readlane(b.seq.n, l);
+  r.seq.len = __builtin_amdgcn_readlane(b.seq.len, l);
+  r.row_tiles = __builtin_amdgcn_readlane(b.row_tiles, l);
+  r.key_tiles = __builtin_amdgcn_readlane(b.key_tiles, l);
+  r.before = b.base + (l ? lane64(b.units, l - 1) : 0);
+  r.items_before = b.items_base + (l ? lane64(b.items, l - 1) : 0);
+  return r;
 }
 
 // ---------------------------------------------------------------- query rows

@@ -7,7 +7,7 @@
 //   given to Q as well. The result has the query row in l % 16 and keys 4 (l / 16) + 0 .. 3 in the registers of both 16-key tiles.
 //   O^T = V^T P^T: those keys are the ones whose P a lane now has; it loads the same keys' values, dim / 16 channels each, and
 //   turns bytes into channel-major f16 by permutes as it converts.
-// While 32 keys are computed the next 32 are on their way. A workgroup's 4 waves take a share's tiles in turn and join through LDS
+// Each tile's registers take the next one as they are used up. A workgroup's 4 waves take a share's tiles in turn and join through LDS
 // at the end of an item; items that more than one workgroup has worked on are left as parts.
 #include "kv_attn.hpp"
 
@@ -20,8 +20,9 @@ constexpr int NT = 256, WAVES = 4;
 template <int D>
 struct Tile {
   uint4 k[2][D / 64];
+  float4 ks[2];
   uint32_t v[8][D / 64];
-  float4 ks[2], vs[2];
+  float4 vs[2];
 };
 
 // the two pages of a 32-key tile (two 16-key halves), -1 where absent
@@ -40,22 +41,30 @@ __device__ __forceinline__ Pages pages_of(const AttnArgs& a, const int32_t* row,
 }
 
 template <int D>
-__device__ __forceinline__ void load_tile(const AttnArgs& a, int kvh, int tile, const Pages& pg, Tile<D>& t) {
+__device__ __forceinline__ void load_keys(const AttnArgs& a, int kvh, int tile, const Pages& pg, Tile<D>& t) {
   const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     const int64_t p = max(pg.p[h], 0);
     const int off = (tile * UNIT_KEYS + 16 * h) & ((1 << a.c.log2page) - 1);
-    const int64_t code = p * a.c.page_stride + kvh * a.c.head_stride + off * D;
-    const int64_t scale = p * a.c.spage_stride + kvh * a.c.shead_stride + off;
-    const uint8_t* kb = a.c.k + code;
-    const uint8_t* vb = a.c.v + code;
+    const uint8_t* kb = a.c.k + p * a.c.page_stride + kvh * a.c.head_stride + off * D;
 #pragma unroll
-    for (int c = 0; c < D / 64; ++c) t.k[h][c] = *reinterpret_cast<const uint4*>(kb + l16 * D + 64 * c + 16 * g);
-    t.ks[h] = *reinterpret_cast<const float4*>(a.c.ks + scale + 4 * g);
+    for (int c = 0; c < D / 64; ++c) t.k[h][c] = *reinterpret_cast<const uint4*>(kb + (l16 * D + 64 * c + 16 * g));
+    t.ks[h] = *reinterpret_cast<const float4*>(a.c.ks + p * a.c.spage_stride + kvh * a.c.shead_stride + off + 4 * g);
+  }
+}
+template <int D>
+__device__ __forceinline__ void load_values(const AttnArgs& a, int kvh, int tile, const Pages& pg, Tile<D>& t) {
+  const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int64_t p = max(pg.p[h], 0);
+    const int off = (tile * UNIT_KEYS + 16 * h) & ((1 << a.c.log2page) - 1);
+    const uint8_t* vb = a.c.v + p * a.c.page_stride + kvh * a.c.head_stride + off * D;
+    t.vs[h] = *reinterpret_cast<const float4*>(a.c.vs + p * a.c.spage_stride + kvh * a.c.shead_stride + off + 4 * g);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const uint8_t* vr = vb + (4 * g + j) * D + l16 * (D / 16);
+      const uint8_t* vr = vb + ((4 * g + j) * D + l16 * (D / 16));
       if constexpr (D == 128) {
         const uint2 w = *reinterpret_cast<const uint2*>(vr);
         t.v[4 * h + j][0] = w.x;
@@ -64,7 +73,6 @@ __device__ __forceinline__ void load_tile(const AttnArgs& a, int kvh, int tile, 
         t.v[4 * h + j][0] = *reinterpret_cast<const uint32_t*>(vr);
       }
     }
-    t.vs[h] = *reinterpret_cast<const float4*>(a.c.vs + scale + 4 * g);
   }
 }
 
@@ -75,9 +83,12 @@ struct State {
   float ref[MT], sum[MT], vref, ivref;
 };
 
-template <int FMT, int D, int MT>
-__device__ __forceinline__ void compute(const AttnArgs& a, Tile<D>& t, int tile, const Pages& pg, const h8_t (&q)[MT][D / 32],
-                                        const float (&qf)[MT], const int (&lim)[MT], int low, int len, State<D, MT>& st) {
+// One tile. MORE: the wave's next tile (pages `pn`) is loaded into the same registers, its keys as soon as these are used, its
+// values at the end: a load has about half a tile's work to come in.
+template <int FMT, int D, int MT, bool MORE>
+__device__ __forceinline__ void compute(const AttnArgs& a, Tile<D>& t, int kvh, int tile, const Pages& pg, const Pages& pn,
+                                        const h8_t (&q)[MT][D / 32], const float (&qf)[MT], const int (&lim)[MT], int low, int len,
+                                        State<D, MT>& st) {
   const int lane = threadIdx.x & 63, g = lane >> 4;
   const int kb = tile * UNIT_KEYS;
   // low: keys that every row sees
@@ -106,6 +117,7 @@ __device__ __forceinline__ void compute(const AttnArgs& a, Tile<D>& t, int tile,
       }
     }
   }
+  if constexpr (MORE) load_keys<D>(a, kvh, tile + WAVES, pn, t);
   if (edge) {
     // what lies behind the sequence or in an absent page may be anything: its scales and, where codes can be NaN, its values go
 #pragma unroll
@@ -195,6 +207,7 @@ __device__ __forceinline__ void compute(const AttnArgs& a, Tile<D>& t, int tile,
       for (int m = 0; m < MT; ++m)
         st.o[m][4 * c + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[i], p[m], st.o[m][4 * c + i], 0, 0, 0);
   }
+  if constexpr (MORE) load_values<D>(a, kvh, tile + WAVES, pn, t);
 }
 
 template <int FMT, int D, int MT>
@@ -204,20 +217,23 @@ __global__ void __launch_bounds__(NT, 2) token_kernel(AttnArgs a) {
   __shared__ float sm[WAVES][R], sl[WAVES][R];
   const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  int64_t unused, unused2;
-  const Work work = all_work(a, R, -1, unused, unused2);
+  Block blk;
+  const Work work = dealt(load_blocks(a, R, blk), a.wgs);
   const int wg = blockIdx.x;
   if (wg >= work.wgs) return;
   int64_t u = share_begin(work, wg);
   const int64_t end = share_begin(work, wg + 1);
 
   while (u < end) {
-    const UnitAt at = seq_of_unit(a, R, u);
-    if (at.b < 0) return;
-    const Seq sq = seq_at(a.s, at.b);
-    const SeqWork sw = work_of(a, sq, R);
-    const int64_t local = u - at.before;
-    const int item = static_cast<int>(local / sw.key_tiles);
+    while (u >= blk.end()) {
+      if (blk.at + 64 >= a.s.batch) return;
+      next_block(a, R, blk);
+    }
+    const int l = __builtin_ctzll(__builtin_amdgcn_ballot_w64(blk.base + blk.units > u));
+    const SeqItems sw = seq_in(a, blk, l);
+    const Seq sq = sw.seq;
+    const int64_t local = u - sw.before;
+    const int item = static_cast<int>(quotient(local, sw.key_tiles));
     const int t0 = static_cast<int>(local - static_cast<int64_t>(item) * sw.key_tiles);
     const int t1 = static_cast<int>(end - u < sw.key_tiles - t0 ? t0 + (end - u) : sw.key_tiles);
     const int kvh = item / sw.row_tiles, rt = item - kvh * sw.row_tiles;
@@ -261,31 +277,20 @@ __global__ void __launch_bounds__(NT, 2) token_kernel(AttnArgs a) {
 #pragma unroll
       for (int i = 0; i < D / 16; ++i) st.o[m][i] = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
     }
-    const int32_t* row = a.s.table + at.b * a.s.table_stride;
+    const int32_t* row = a.s.table + (blk.at + l) * a.s.table_stride;
     int t = t0 + wave;
     if (t < t1) {
-      // two tiles in registers: one computed, one loading; the pages of the one after are looked up as it begins to load
-      Tile<D> ta, tb;
-      Pages pa = pages_of(a, row, t), pb = pages_of(a, row, t + WAVES);
-      load_tile<D>(a, kvh, t, pa, ta);
-      while (t + WAVES < t1) {
-        load_tile<D>(a, kvh, t + WAVES, pb, tb);
-        const Pages pc = pages_of(a, row, t + 2 * WAVES);
-        compute<FMT, D, MT>(a, ta, t, pa, q, qf, lim, low, sq.len, st);
-        t += WAVES;
-        if (t + WAVES >= t1) {
-          compute<FMT, D, MT>(a, tb, t, pb, q, qf, lim, low, sq.len, st);
-          t += WAVES;
-          break;
-        }
-        load_tile<D>(a, kvh, t + WAVES, pc, ta);
-        const Pages pd = pages_of(a, row, t + 2 * WAVES);
-        compute<FMT, D, MT>(a, tb, t, pb, q, qf, lim, low, sq.len, st);
-        t += WAVES;
-        pa = pc;
-        pb = pd;
+      Tile<D> tile;
+      Pages pg = pages_of(a, row, t), pn = pages_of(a, row, t + WAVES);
+      load_keys<D>(a, kvh, t, pg, tile);
+      load_values<D>(a, kvh, t, pg, tile);
+      for (; t + WAVES < t1; t += WAVES) {
+        const Pages p2 = pages_of(a, row, t + 2 * WAVES);
+        compute<FMT, D, MT, true>(a, tile, kvh, t, pg, pn, q, qf, lim, low, sq.len, st);
+        pg = pn;
+        pn = p2;
       }
-      if (t < t1) compute<FMT, D, MT>(a, ta, t, pa, q, qf, lim, low, sq.len, st);
+      compute<FMT, D, MT, false>(a, tile, kvh, t, pg, pn, q, qf, lim, low, sq.len, st);
     }
     // join the 4 waves
 #pragma unroll
@@ -338,9 +343,9 @@ __global__ void __launch_bounds__(NT, 2) token_kernel(AttnArgs a) {
         if (a.lse && d0 == 0)
           a.lse[static_cast<int64_t>(sq.first + tok) * a.c.heads * a.group + hd] =
               sum == 0.0f ? -INFINITY : (__builtin_amdgcn_logf(sum) + top) * 0.6931471805599453f;
-      } else if (!whole || at.items_before + item < a.items) {   // (a cu that falls can count rows more than once)
+      } else if (!whole || sw.items_before + item < a.items) {   // (a cu that falls can count rows more than once)
         // slots: two to a workgroup (the item that it goes on with, the one that it begins), then one to an item that it completes
-        const int64_t slot = whole ? 2 * static_cast<int64_t>(a.wgs) + at.items_before + item : 2 * static_cast<int64_t>(wg) + (t0 == 0);
+        const int64_t slot = whole ? 2 * static_cast<int64_t>(a.wgs) + sw.items_before + item : 2 * static_cast<int64_t>(wg) + (t0 == 0);
         float* po = a.part_o + (slot * R + rl) * D + d0;
 #pragma unroll
         for (int e = 0; e < EPT; e += 4) *reinterpret_cast<float4*>(po + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
