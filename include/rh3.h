@@ -498,8 +498,8 @@ int rh3_kv_read(const rh3_kv_cache* cache, void* k, int64_t k_st, int64_t k_sh, 
  * prefix[], which come before the sequences' own and are read once for the batch. out may lie exactly over q.
  * The workspace holds the parts of rows whose keys several workgroups share; how keys are split depends on the sizes, lengths
  * and the CU count, and with it the last bits of the result; the same call gives the same bits. */
-int64_t rh3_kv_attention_workspace_bytes(const rh3_kv_cache* cache, int64_t q_heads, int64_t rows, int64_t width,
-                                         int64_t batch, int even, int64_t prefix_len);
+int64_t rh3_kv_attention_workspace_bytes(const rh3_kv_cache* cache, int64_t q_heads, int64_t rows, int64_t batch,
+                                         int even, int64_t prefix_len);
 int rh3_kv_attention(const rh3_kv_cache* cache, const void* q, int64_t q_st, int64_t q_sh, int64_t q_heads, int dtype,
                      int64_t rows, const int32_t* table, int64_t table_stride, int64_t width, const int32_t* lens,
                      const int32_t* cu, int64_t batch, int causal, float scale, void* out, int64_t o_st, int64_t o_sh,

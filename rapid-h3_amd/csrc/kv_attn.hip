@@ -24,26 +24,12 @@ __device__ __forceinline__ Parts parts_of(const Source& s, int b, const Seq& q, 
   const int64_t r = static_cast<int64_t>(tok - q.first) * s.a.group + in_group;
   const int rt = static_cast<int>(r / s.rows);
   p.row = static_cast<int>(r - static_cast<int64_t>(rt) * s.rows);
-  if (s.chunk) {
-    int64_t tiles = 0;
-    const int lane = threadIdx.x & 63;
-    for (int at = 0; at < b; at += 64) {
-      int64_t n = at + lane < b ? (static_cast<int64_t>(seq_at(s.a.s, at + lane).n) * s.a.group + s.rows - 1) / s.rows : 0;
-#pragma unroll
-      for (int d = 32; d; d >>= 1) n += __shfl_xor(n, d);
-      tiles += n;
-    }
-    p.first = (static_cast<int64_t>(kvh) * s.a.tiles + tiles + rt) * s.a.splits;
-    p.next = p.first + 1;
-    p.step = 1;
-    p.count = tiles + rt < s.a.tiles ? s.a.splits : 0;   // (a cu that falls can count rows more than once)
-    return p;
-  }
   Block blk;
-  const Work w = dealt(load_blocks(s.a, s.rows, blk), s.a.wgs);
-  while (b >= blk.at + 64) next_block(s.a, s.rows, blk);
+  const Tiling g = tiling(s.chunk, s.rows);
+  const Work w = dealt(load_blocks(s.a, g, blk), s.a.wgs, g);
+  while (b >= blk.at + 64) next_block(s.a, g, blk);
   const SeqItems sw = seq_in(s.a, blk, b - blk.at);
-  const int64_t item = static_cast<int64_t>(kvh) * sw.row_tiles + rt;
+  const int64_t item = static_cast<int64_t>(kvh) * sw.row_tiles + (s.chunk && s.a.causal ? place_of_tile(rt, sw.row_tiles) : rt);
   const int64_t u0 = sw.before + item * sw.key_tiles;
   const int w0 = share_of(w, u0), w1 = share_of(w, u0 + sw.key_tiles - 1);
   p.step = 2;
@@ -135,34 +121,21 @@ __global__ void __launch_bounds__(NT) join_kernel(Source own, Source prefix, int
 // ---------------------------------------------------------------- host: how a call runs
 struct Plan {
   int chunk, rows;        // kernel, query rows of its tiles
-  int wgs;                // token kernel
-  int tiles, splits;      // chunk kernel
-  int64_t items;          // token kernel: slots for items that one workgroup completes
+  int wgs;
+  int64_t items;          // slots for items that one workgroup completes
   int64_t slots;          // parts it may leave
 };
 
 // rows: of a call; per sequence they are counted as even. keep: a part for every item.
-Plan plan_of(int64_t rows, int64_t batch, bool even, int64_t group, int64_t heads, int64_t cap, bool keep) {
+Plan plan_of(int64_t rows, int64_t batch, bool even, int64_t group, int64_t heads, bool keep) {
   const int64_t cus = device_cus() > 0 ? device_cus() : 256;
   const int64_t mean = (rows * group + batch - 1) / batch;    // query rows of a sequence's K/V head
   Plan p{};
-  if (mean <= 32) {
-    p.rows = mean <= 16 ? 16 : 32;
-    p.wgs = static_cast<int>(2 * cus);
-    p.items = !keep ? 0 : heads * (even ? batch * ((rows / batch * group + p.rows - 1) / p.rows) : rows * group / p.rows + batch);
-    p.slots = 2 * static_cast<int64_t>(p.wgs) + p.items;
-    return p;
-  }
-  p.chunk = 1;
-  p.rows = 128;
-  const int64_t tiles = even ? batch * ((rows / batch * group + p.rows - 1) / p.rows) : rows * group / p.rows + batch;
-  const int64_t likely = batch * ((mean + p.rows - 1) / p.rows) * heads;
-  int64_t splits = (2 * cus + likely - 1) / likely;
-  const int64_t most = cap / 512;                             // 8 tiles of 64 keys to a range
-  splits = splits > most ? most : splits;
-  p.splits = static_cast<int>(splits < 1 ? 1 : splits);
-  p.tiles = static_cast<int>(tiles);
-  p.slots = p.splits > 1 || keep ? tiles * heads * p.splits : 0;
+  p.chunk = mean > 32;
+  p.rows = mean <= 16 ? 16 : mean <= 32 ? 32 : mean <= 128 ? 128 : 256;
+  p.wgs = static_cast<int>(p.rows == 256 ? cus : 2 * cus);
+  p.items = !keep ? 0 : heads * (even ? batch * ((rows / batch * group + p.rows - 1) / p.rows) : rows * group / p.rows + batch);
+  p.slots = 2 * static_cast<int64_t>(p.wgs) + p.items;
   return p;
 }
 int64_t bytes_of(const Plan& p, int64_t dim) { return p.slots * p.rows * (dim + 2) * 4; }
@@ -171,21 +144,20 @@ struct Call {
   Plan own, prefix;
   int64_t bytes;
 };
-Call call_of(int64_t rows, int64_t q_heads, int64_t heads, int64_t dim, int64_t page, int64_t width, int64_t batch, bool even,
-             int64_t prefix_len) {
+Call call_of(int64_t rows, int64_t q_heads, int64_t heads, int64_t dim, int64_t batch, bool even, int64_t prefix_len) {
   Call c{};
   const int64_t group = q_heads / heads;
-  c.own = plan_of(rows, batch, even, group, heads, width * page, prefix_len > 0);
+  c.own = plan_of(rows, batch, even, group, heads, prefix_len > 0);
   c.bytes = bytes_of(c.own, dim);
   if (prefix_len > 0) {
-    c.prefix = plan_of(rows, 1, true, group, heads, prefix_len, true);
+    c.prefix = plan_of(rows, 1, true, group, heads, true);
     c.bytes += bytes_of(c.prefix, dim);
   }
   return c;
 }
 
 void launch(const AttnArgs& a, const Plan& p, int fmt, int dim, hipStream_t st) {
-  if (p.chunk) launch_chunk(a, fmt, dim, p.rows, static_cast<int64_t>(p.tiles) * p.splits * a.c.heads, st);
+  if (p.chunk) launch_chunk(a, fmt, dim, p.rows, st);
   else launch_token(a, fmt, dim, p.rows, st);
 }
 
@@ -196,10 +168,10 @@ void launch(const AttnArgs& a, const Plan& p, int fmt, int dim, hipStream_t st) 
 using namespace rh3;
 using namespace rh3::kv;
 
-extern "C" int64_t rh3_kv_attention_workspace_bytes(const rh3_kv_cache* cache, int64_t q_heads, int64_t rows, int64_t width,
-                                                    int64_t batch, int even, int64_t prefix_len) {
-  if (!cache || cache->heads < 1 || q_heads < cache->heads || q_heads % cache->heads || rows < 1 || batch < 1 || width < 1) return 0;
-  return call_of(rows, q_heads, cache->heads, cache->dim, cache->page, width, batch, even != 0, prefix_len).bytes;
+extern "C" int64_t rh3_kv_attention_workspace_bytes(const rh3_kv_cache* cache, int64_t q_heads, int64_t rows, int64_t batch,
+                                                    int even, int64_t prefix_len) {
+  if (!cache || cache->heads < 1 || q_heads < cache->heads || q_heads % cache->heads || rows < 1 || batch < 1) return 0;
+  return call_of(rows, q_heads, cache->heads, cache->dim, batch, even != 0, prefix_len).bytes;
 }
 
 extern "C" int rh3_kv_attention(const rh3_kv_cache* cache, const void* q, int64_t q_st, int64_t q_sh, int64_t q_heads, int dtype,
@@ -223,12 +195,9 @@ extern "C" int rh3_kv_attention(const rh3_kv_cache* cache, const void* q, int64_
   RH3_REQUIRE(prefix_len >= 0 && prefix_len <= (int64_t{1} << 30) && (prefix_len == 0 || prefix), "kv_attention: prefix of %lld positions without pages",
               static_cast<long long>(prefix_len));
   const int dim = static_cast<int>(cache->dim), fmt = static_cast<int>(cache->format);
-  const Call call = call_of(rows, q_heads, a.c.heads, dim, cache->page, width, batch, cu == nullptr, prefix_len);
-  RH3_REQUIRE(call.bytes == 0 || (workspace && aligned16(workspace) && workspace_bytes >= call.bytes),
+  const Call call = call_of(rows, q_heads, a.c.heads, dim, batch, cu == nullptr, prefix_len);
+  RH3_REQUIRE(workspace && aligned16(workspace) && workspace_bytes >= call.bytes,
               "kv_attention: workspace of %lld bytes needed, %lld given", static_cast<long long>(call.bytes), static_cast<long long>(workspace_bytes));
-  for (const Plan* p : {&call.own, &call.prefix})
-    RH3_REQUIRE(!p->chunk || static_cast<int64_t>(p->tiles) * p->splits * a.c.heads <= MAX_GRID_256, "kv_attention: %lld rows in one call",
-                static_cast<long long>(rows));
   a.q = q;
   a.q_st = q_st;
   a.q_sh = q_sh;
@@ -246,11 +215,9 @@ extern "C" int rh3_kv_attention(const rh3_kv_cache* cache, const void* q, int64_
   auto source = [&](AttnArgs x, const Plan& p) {
     x.items = p.items;
     x.wgs = p.wgs;
-    x.splits = p.splits;
-    x.tiles = p.tiles;
     x.part_o = ws;
-    x.part_ml = ws ? ws + p.slots * p.rows * dim : nullptr;
-    ws = ws ? ws + p.slots * p.rows * (dim + 2) : nullptr;
+    x.part_ml = ws + p.slots * p.rows * dim;
+    ws += p.slots * p.rows * (dim + 2);
     return Source{x, p.chunk, p.rows};
   };
   const Source own = source(a, call.own);
@@ -273,7 +240,6 @@ extern "C" int rh3_kv_attention(const rh3_kv_cache* cache, const void* q, int64_
   }
   launch(own.a, call.own, fmt, dim, stream);
   if (const int e = launch_status("kv_attention")) return e;
-  if (call.bytes == 0) return RH3_OK;
   // few rows with up to hundreds of parts each: a workgroup to a row; many rows with few parts: a wave
   const int64_t ids = rows * q_heads;
   const bool wide = !call.own.chunk && !(prefix_len > 0 && call.prefix.chunk);

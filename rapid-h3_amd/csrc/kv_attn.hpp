@@ -33,17 +33,19 @@ struct AttnArgs {
   float* part_o;
   float* part_ml;
   int64_t items;             // slots of completed items
-  int wgs;                   // token kernel: workgroups
-  int keep;                  // token kernel: leave a part for every item, also for those that one workgroup completes
-  int splits, tiles;         // chunk kernel: key ranges of an item, row tiles in the grid
+  int wgs;
+  int keep;                  // leave a part for every item, also for those that one workgroup completes
 };
 
-// ---------------------------------------------------------------- the token kernel's work, the same on every wave that asks
-// Items: (sequence, K/V head, R query rows of it). Units: 32 keys of an item. The units of all items in order (sequences, then
+// ---------------------------------------------------------------- the kernels' work, the same on every wave that asks
+// Items: (sequence, K/V head, R query rows of it). Units: KEYS keys of an item. The units of all items in order (sequences, then
 // K/V heads, then row tiles) are dealt to the workgroups in equal contiguous ranges, so that uneven histories, which only the
-// device knows, load the workgroups evenly. UNIT_MIN units at least make a workgroup worth starting: one for each of its waves.
-constexpr int UNIT_KEYS = 32;
-constexpr int UNIT_MIN = 4;
+// device knows, load the workgroups evenly. `least` units at least make a workgroup worth starting.
+struct Tiling {
+  int rows, keys, least;
+};
+constexpr int TOKEN_KEYS = 32, CHUNK_KEYS = 64;
+RH3_HD Tiling tiling(bool chunk, int rows) { return chunk ? Tiling{rows, CHUNK_KEYS, 8} : Tiling{rows, TOKEN_KEYS, 4}; }
 
 // Units are counted in 64 bits; a division of what fits 32 bits is done there (a 64-bit one takes some hundred instructions).
 RH3_HD int64_t quotient(int64_t a, int64_t b) {
@@ -53,9 +55,9 @@ struct Work {
   int wgs;                   // workgroups that have a share
   int64_t each, more;        // the first `more` of them have each + 1 units, the others each
 };
-RH3_HD Work dealt(int64_t units, int wgs) {
+RH3_HD Work dealt(int64_t units, int wgs, const Tiling& g) {
   Work w;
-  const int64_t most = (units + UNIT_MIN - 1) / UNIT_MIN;
+  const int64_t most = (units + g.least - 1) / g.least;
   w.wgs = static_cast<int>(most < wgs ? (most > 0 ? most : 1) : wgs);
   w.each = quotient(units, w.wgs);
   w.more = units - w.each * w.wgs;
@@ -72,10 +74,10 @@ struct SeqWork {
   int row_tiles, key_tiles;
   int64_t units;
 };
-RH3_HD SeqWork work_of(const AttnArgs& a, const Seq& q, int R) {
+RH3_HD SeqWork work_of(const AttnArgs& a, const Seq& q, const Tiling& g) {
   SeqWork w;
-  w.row_tiles = static_cast<int>((static_cast<int64_t>(q.n) * a.group + R - 1) / R);
-  const int kt = (q.len + UNIT_KEYS - 1) / UNIT_KEYS;
+  w.row_tiles = static_cast<int>((static_cast<int64_t>(q.n) * a.group + g.rows - 1) / g.rows);
+  const int kt = (q.len + g.keys - 1) / g.keys;
   w.key_tiles = kt < 1 ? 1 : kt;
   // no memory holds 2^36 units (2^41 keys); offsets in cu that fall can count rows many times, and must not overflow the sums
   const int64_t u = static_cast<int64_t>(a.c.heads) * w.row_tiles;
@@ -113,7 +115,7 @@ struct Block {
   int row_tiles, key_tiles;
   __device__ __forceinline__ int64_t end() const { return base + lane64(units, 63); }
 };
-__device__ __forceinline__ void load_block(const AttnArgs& a, int R, int at, int64_t base, int64_t items_base, Block& b) {
+__device__ __forceinline__ void load_block(const AttnArgs& a, const Tiling& g, int at, int64_t base, int64_t items_base, Block& b) {
   const int i = at + (threadIdx.x & 63);
   b.at = at;
   b.base = base;
@@ -122,7 +124,7 @@ __device__ __forceinline__ void load_block(const AttnArgs& a, int R, int at, int
   SeqWork w{0, 1, 0};
   if (i < a.s.batch) {
     b.seq = seq_at(a.s, i);
-    w = work_of(a, b.seq, R);
+    w = work_of(a, b.seq, g);
   }
   b.row_tiles = w.row_tiles;
   b.key_tiles = w.key_tiles;
@@ -130,18 +132,18 @@ __device__ __forceinline__ void load_block(const AttnArgs& a, int R, int at, int
   b.items = a.keep ? wave_scan(static_cast<int64_t>(a.c.heads) * w.row_tiles) : 0;
 }
 // the first block, and the units of all
-__device__ __forceinline__ int64_t load_blocks(const AttnArgs& a, int R, Block& b) {
-  load_block(a, R, 0, 0, 0, b);
+__device__ __forceinline__ int64_t load_blocks(const AttnArgs& a, const Tiling& g, Block& b) {
+  load_block(a, g, 0, 0, 0, b);
   int64_t total = b.end();
   for (int at = 64; at < a.s.batch; at += 64) {
     Block next;
-    load_block(a, R, at, 0, 0, next);
+    load_block(a, g, at, 0, 0, next);
     total += next.end();
   }
   return total;
 }
-__device__ __forceinline__ void next_block(const AttnArgs& a, int R, Block& b) {
-  load_block(a, R, b.at + 64, b.end(), b.items_base + lane64(b.items, 63), b);
+__device__ __forceinline__ void next_block(const AttnArgs& a, const Tiling& g, Block& b) {
+  load_block(a, g, b.at + 64, b.end(), b.items_base + lane64(b.items, 63), b);
 }
 
 // a sequence of the block by its lane, the same in all lanes
@@ -161,6 +163,16 @@ __device__ __forceinline__ SeqItems seq_in(const AttnArgs& a, const Block& b, in
   r.items_before = b.items_base + (l ? lane64(b.items, l - 1) : 0);
   return r;
 }
+
+// The chunk kernel's causal row tiles are taken from both ends in turn (0, n - 1, 1, n - 2, ..), so that the long and short ones
+// of a share even out: the tile at a place, and the place of a tile
+RH3_HD int tile_at_place(int at, int n) { return at & 1 ? n - 1 - (at >> 1) : at >> 1; }
+RH3_HD int place_of_tile(int rt, int n) { return rt < (n + 1) / 2 ? 2 * rt : 2 * (n - 1 - rt) + 1; }
+
+// A value that is the same in all lanes, as a scalar: a division is done by vector instructions, and what depends on its result
+// (loop bounds, addresses) would stay in vector registers
+__device__ __forceinline__ int scalar(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ int64_t scalar(int64_t v) { return lane64(v, 0); }
 
 // ---------------------------------------------------------------- query rows
 // 8 values of a query row at offset `at` as floats
@@ -205,17 +217,20 @@ __device__ __forceinline__ float across_sum(float v) {
 constexpr float REF_UNDER = 10.0f;   // a new reference lies this far under the maximum: probabilities up to 2^10
 constexpr float REF_STALE = 15.0f;   // a score this far over the reference moves it: probabilities up to 2^15
 
-// the power of two over a scale (the largest finite one for an infinity; NaN never gets here)
+// the power of two over a scale, at least 2^-111 (NaN never gets here)
 __device__ __forceinline__ float pow2_over(float v) {
   const uint32_t e = (__float_as_uint(v) >> 23) & 255u;
-  return __uint_as_float(min(e + 1u, 253u) << 23);
+  return __uint_as_float(min(max(e + 1u, 16u), 253u) << 23);
 }
+
+// 1 over a power of two given by its bits (exponents 1 to 253)
+__device__ __forceinline__ float pow2_inverse(int bits) { return __int_as_float((254 << 23) - bits); }
 
 __device__ __forceinline__ uint32_t pack_out(const AttnArgs& a, float x, float y) { return a.fp16 ? pack_h2(x, y) : pack_bf2(x, y); }
 
 // host: launches of the two kernels for their checked arguments
 void launch_token(const AttnArgs& a, int fmt, int dim, int rows, hipStream_t st);
-void launch_chunk(const AttnArgs& a, int fmt, int dim, int rows, int64_t grid, hipStream_t st);
+void launch_chunk(const AttnArgs& a, int fmt, int dim, int rows, hipStream_t st);
 
 }  // namespace kv
 }  // namespace rh3

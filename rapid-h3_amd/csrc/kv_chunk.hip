@@ -1,352 +1,407 @@
 // Attention of many query rows over the paged cache: a chunk of a prompt, the tokens of a frame, a whole batch against a prefix
 // that it shares.
 //
-// Bound by the matrix units: 4 dim flops per query row and key, while a key's 2 (dim + 4) bytes serve all rows of a tile. A
-// workgroup of 4 waves holds 4 x 32 QT query rows of one K/V head and walks its keys 64 at a time. The tile's codes come to
-// registers while the previous tile is computed, are converted to f16 once for the 4 waves and written to LDS (two buffers, one
-// barrier to a tile): K as it is, V channel-major with its keys in the order that the probabilities have. Per wave
+// Bound by the matrix units and, close behind, by the vector instructions of the softmax: 4 dim flops per query row and key,
+// while a key's 2 (dim + 4) bytes serve all rows of a tile. A workgroup of 4 or 8 waves holds 32 query rows of one K/V head on
+// each and walks its keys 64 at a time. The tile's codes come to registers while the previous tile is computed, are converted to
+// f16 once for all waves and written to LDS (two buffers, one barrier to a tile): K as it is, V channel-major with its keys in
+// the order that the probabilities have. Per wave
 //   S^T = K Q^T (32x32x16 f16): a lane has one query row (l % 32) and 16 of 32 keys, so a row's softmax is in-lane but for one
 //   exchange, and only when its reference moves; the probabilities are the B operand of
 //   O^T = V^T P^T as they stand: k-step t of 32 keys takes keys 16 t + 4 (l / 32) + 0 .. 3 and those + 8.
-// A value's scale, relative to a power of two over the largest seen, is multiplied into V as it is converted (rounded to f16,
-// 2^-12, as the probabilities are), which leaves only the key's scale to be read per score.
+// Vector work per score: one fma (key scale, softmax scale and reference at once), half a max, the exponential, the sum and half a
+// conversion. For that, the query rows of a workgroup share one power of
+// two (an element 2^22 below the tile's largest loses low bits, 2^-33 of the largest at most, which is what an absolute error
+// of a score can be); and a value's scale, relative to a power of two over the largest seen, is multiplied into V as it is
+// converted (rounded to f16, 2^-11 at most, as the probabilities are).
 #include "kv_attn.hpp"
 
 namespace rh3 {
 namespace kv {
 namespace {
 
-constexpr int NT = 256, WAVES = 4, KT = 64;
+constexpr int KT = CHUNK_KEYS;
+constexpr float NO_REF = -0x1p100f;   // reference of a row that has seen no key: any score moves it
 
-// 16-byte pieces of the LDS rows, spread so that the lanes of a read or write meet different banks
+// 16-byte pieces of the LDS rows. Each row has one piece more than it needs, so that 16 rows' pieces of one number lie in all 16
+// parts of the banks, and every read of a tile is one lane address with an immediate offset.
 template <int D>
-__device__ __forceinline__ int k_piece(int key, int piece) {   // K: [64 keys][D] f16
-  constexpr int N = D / 8;
-  return key * N + (piece ^ (D == 128 ? key & 15 : (key >> 1) & 7));
-}
-__device__ __forceinline__ int v_piece(int d, int piece) {     // V^T: [D][64 keys] f16, pieces of 8 keys
-  return d * 8 + (piece ^ (((d >> 1) ^ (d >> 4)) & 7));
-}
+constexpr int K_ROW = D / 8 + 1;                               // K: [64 keys][D] f16
+constexpr int V_ROW = KT / 8 + 1;                              // V^T: [D][64 keys] f16, pieces of 8 keys
 
-template <int D>
+// What a wave has in flight of a tile: the codes that it will convert, and of key l of the 64 its scales and table entry. With 8
+// waves a wave has keys or values, in the same registers.
+template <int D, int WAVES>
 struct Stage {
-  uint4 k[D / 64];     // the wave's 16 keys
-  uint32_t v[8];       // 8 keys x 4 channels
-  float4 vs0, vs1;     // their scales
-  float vsl, ksl;      // scales of key l of the 64
-  int page;            // page of key l, -1 where absent
+  static constexpr int KW = D / 16, VAT = WAVES == 4 ? KW : 0;
+  uint32_t raw[VAT + 8];       // words of 16 keys (KW), of 8 keys x 4 channels (8 from VAT)
+  float vs, ks;
+  int entry;
 };
 
-template <int FMT, int D, int QT>
-__global__ void __launch_bounds__(NT, QT == 1 ? 2 : 1) chunk_kernel(AttnArgs a) {
-  constexpr int R = WAVES * 32 * QT, KS = D / 16, DT = D / 32;
-  __shared__ uint4 sk[2][KT * D / 8];
-  __shared__ uint4 sv[2][KT * D / 8];
+template <int FMT, int D, int WAVES>
+__global__ void __launch_bounds__(WAVES * 64, 2) chunk_kernel(AttnArgs a) {
+  constexpr int R = WAVES * 32, KS = D / 16, DT = D / 32;
+  const Tiling TILING = tiling(true, R);
+  __shared__ uint4 sk[2][KT * K_ROW<D>];
+  __shared__ uint4 sv[2][D * V_ROW];
   __shared__ float sks[2][KT];
+  __shared__ uint4 sf[WAVES][KT / 8];   // a wave's value scales as f16, in V's key order
+  __shared__ float stop[WAVES];
   const int lane = threadIdx.x & 63, l32 = lane & 31, hi = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  // of the 64 keys, a wave converts 16 keys and 16 values (4 waves), or 16 of either (8 waves: the first four keys)
+  const int part = wave & 3;
+  const bool does_k = WAVES == 4 || wave < 4, does_v = WAVES == 4 || wave >= 4;
 
-  // the item: row tiles of all sequences in order, for each K/V head, each in `splits` key ranges. The last row tiles go first
-  // (causal: they have the most keys). A K/V head's items are 8 apart in the grid where heads allow, so that one XCD's L2 holds it.
-  const int idx = blockIdx.x;
-  const int kvh = idx % a.c.heads;
-  const int rest = idx / a.c.heads;
-  const int split = rest % a.splits;
-  const int tile = a.tiles - 1 - rest / a.splits;
-  int b = -1, rt = 0;
+  // neighbouring shares, which read the same keys, on one XCD (workgroups are dealt to the 8 XCDs in turn)
+  const int n8 = a.wgs & ~7;
+  const int wg = static_cast<int>(blockIdx.x) < n8 ? (blockIdx.x & 7) * (n8 >> 3) + (blockIdx.x >> 3) : blockIdx.x;
+  int64_t u, end;
   {
-    int64_t base = 0;
-    for (int at = 0; at < a.s.batch && b < 0; at += 64) {
-      int64_t n = 0;
-      if (at + lane < a.s.batch) n = (static_cast<int64_t>(seq_at(a.s, at + lane).n) * a.group + R - 1) / R;
-      const int64_t s = wave_scan(n);
-      const unsigned long long m = __builtin_amdgcn_ballot_w64(base + s > tile);
-      if (m) {
-        const int l = __builtin_ctzll(m);
-        b = __builtin_amdgcn_readfirstlane(at + l);
-        rt = __builtin_amdgcn_readfirstlane(static_cast<int>(tile - base - __shfl(s - n, l)));
-      }
-      base += __shfl(s, 63);
-    }
+    Block blk;
+    const Work work = dealt(load_blocks(a, TILING, blk), a.wgs, TILING);
+    if (wg >= work.wgs) return;
+    u = scalar(share_begin(work, wg));
+    end = scalar(share_begin(work, wg + 1));
   }
-  if (b < 0) return;
-  const Seq sq = seq_at(a.s, b);
-  const int rows = sq.n * a.group;
-  const int tok_last = min(rows - 1, rt * R + R - 1) / a.group;
-  const int seen = a.causal ? min(sq.len, max(0, sq.len - sq.n + tok_last + 1)) : sq.len;   // keys that some row sees
-  const int nkt = (seen + KT - 1) / KT;
-  const int per = (nkt + a.splits - 1) / a.splits;
-  const int t0 = min(nkt, split * per), t1 = min(nkt, t0 + per);
 
-  h8_t q[QT][KS];
-  float qf[QT];
-  int lim[QT], row_of[QT];
-#pragma unroll
-  for (int m = 0; m < QT; ++m) {
-    const int row = rt * R + wave * 32 * QT + 32 * m + l32;
+  while (u < end) {
+    // the sequences are looked up again for every item: kept, they would take registers from the loop below
+    Block blk;
+    load_block(a, TILING, 0, 0, 0, blk);
+    while (u >= blk.end()) {
+      if (blk.at + 64 >= a.s.batch) return;
+      next_block(a, TILING, blk);
+    }
+    const int in_block = __builtin_ctzll(__builtin_amdgcn_ballot_w64(blk.base + blk.units > u));
+    const int seq = blk.at + in_block;
+    const SeqItems sw = seq_in(a, blk, in_block);
+    const Seq sq = sw.seq;
+    const int64_t local = u - sw.before;
+    const int item = scalar(static_cast<int>(quotient(local, sw.key_tiles)));
+    const int t0 = static_cast<int>(local - static_cast<int64_t>(item) * sw.key_tiles);
+    const int share_t1 = static_cast<int>(end - u < sw.key_tiles - t0 ? t0 + (end - u) : sw.key_tiles);
+    const bool whole = t0 == 0 && share_t1 == sw.key_tiles;
+    const int kvh = scalar(item / sw.row_tiles), at = item - kvh * sw.row_tiles;
+    const int rt = a.causal ? tile_at_place(at, sw.row_tiles) : at;
+    const int rows = sq.n * a.group;
+    const int tok_last = scalar(min(rows - 1, rt * R + R - 1) / a.group);
+    const int seen = a.causal ? min(sq.len, max(0, sq.len - sq.n + tok_last + 1)) : sq.len;   // keys that some row sees
+    const int t1 = min(share_t1, (seen + KT - 1) / KT);
+
+    const int row = rt * R + wave * 32 + l32;
     const bool has = row < rows;
     const int rr = has ? row : rows - 1;
     const int tok = rr / a.group, hd = kvh * a.group + rr - tok * a.group;
-    const int64_t at = (sq.first + tok) * a.q_st + hd * a.q_sh + 8 * hi;
-    float top = 0.0f;
+    h8_t q[KS];
+    float qf;
+    {
+      const int64_t qat = (sq.first + tok) * a.q_st + hd * a.q_sh + 8 * hi;
+      float top = 0.0f;
 #pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      float x[8];
-      load_q8(a, at + 16 * s, x);
+      for (int s = 0; s < KS; ++s) {
+        float x[8];
+        load_q8(a, qat + 16 * s, x);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[e]));
+        for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[e]) < INFINITY ? fabsf(x[e]) : 0.0f);
+      }
+      top = wave_max(top);
+      if (lane == 0) stop[wave] = top;
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < WAVES; ++w) top = fmaxf(top, stop[w]);
+      const int e = q_exponent(top);
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        float x[8];
+        load_q8(a, qat + 16 * s, x);
+        q[s] = q_f16(x, e);
+      }
+      qf = __builtin_amdgcn_ldexpf(a.scale_log2, -e);
     }
-    const int e = q_exponent(across_max<false>(top));
-#pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      float x[8];
-      load_q8(a, at + 16 * s, x);
-      q[m][s] = q_f16(x, e);
-    }
-    qf[m] = __builtin_amdgcn_ldexpf(a.scale_log2, -e);
-    lim[m] = a.causal ? min(sq.len, sq.len - sq.n + tok + 1) : sq.len;
-    row_of[m] = has ? row : -1;
-  }
-  // of the wave's rows: keys that all see, keys that some see
-  const int r0 = rt * R + wave * 32 * QT, r1 = min(rows - 1, r0 + 32 * QT - 1);
-  const bool idle = r0 >= rows;
-  const int low = a.causal ? min(sq.len, sq.len - sq.n + r0 / a.group + 1) : sq.len;
-  const int top_key = idle ? 0 : a.causal ? min(sq.len, sq.len - sq.n + r1 / a.group + 1) : sq.len;
+    const int lim = a.causal ? min(sq.len, sq.len - sq.n + tok + 1) : sq.len;
+    // of the wave's rows: keys that all see, keys that some see
+    const int r0 = rt * R + wave * 32, r1 = min(rows - 1, r0 + 31);
+    const int low = a.causal ? min(sq.len, sq.len - sq.n + scalar(r0 / a.group) + 1) : sq.len;
+    const int top_key = r0 >= rows ? 0 : a.causal ? min(sq.len, sq.len - sq.n + scalar(r1 / a.group) + 1) : sq.len;
 
-  f16_t o[QT][DT];
-  float ref[QT], sum[QT], vref = 0.0f, ivref = 0.0f;
-#pragma unroll
-  for (int m = 0; m < QT; ++m) {
-    ref[m] = -INFINITY;
-    sum[m] = 0.0f;
+    f16_t o[DT];
+    float ref = NO_REF, sum = 0.0f;
+    int vref = -1;   // bits of the values' reference, the same in all lanes; no tile has that of -1: the first one is never fast
 #pragma unroll
     for (int d = 0; d < DT; ++d)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) o[m][d][i] = 0.0f;
-  }
+      for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
 
-  const int32_t* table = a.s.table + b * a.s.table_stride;
-  const int mask = (1 << a.c.log2page) - 1;
-  auto lookup = [&](int t) {   // page of key l of tile t
-    const int p = table[min((t * KT + lane) >> a.c.log2page, a.s.width - 1)];
-    return p >= 0 && p < a.c.pages ? p : -1;
-  };
-  // V: a thread takes 4 channels of the 8 keys of one piece; D 64: the first 16 lanes of each half
-  const int vq = lane & (D / 4 - 1);
-  const bool vmine = D == 128 || (lane & 16) == 0;
-  auto load = [&](Stage<D>& s, int t, int page) {
-    s.page = page;
-    const int64_t pl = max(page, 0);
-    const int offl = (t * KT + lane) & mask;
-    const int64_t sl = pl * a.c.spage_stride + kvh * a.c.shead_stride + offl;
-    s.vsl = a.c.vs[sl];
-    s.ksl = a.c.ks[sl];
-    const int64_t p = max(__builtin_amdgcn_readlane(page, 16 * wave), 0);
-    const int off = (t * KT + 16 * wave) & mask;
-    const int64_t code = p * a.c.page_stride + kvh * a.c.head_stride + off * D;
-    const uint8_t* kb = a.c.k + code;
-    const uint8_t* vb = a.c.v + code;
+    const int32_t* table = a.s.table + seq * a.s.table_stride;
+    const int mask = (1 << a.c.log2page) - 1;
+    auto lookup = [&](int t) {   // table entry of key l of tile t
+      return table[min((t * KT + lane) >> a.c.log2page, a.s.width - 1)];
+    };
+    // V: a thread takes 4 channels of the 8 keys of one piece; D 64: the first 16 lanes of each half
+    const int vq = lane & (D / 4 - 1);
+    const bool vmine = D == 128 || (lane & 16) == 0;
+    using St = Stage<D, WAVES>;
+    auto page_in = [&](int entry) { return entry >= 0 && entry < a.c.pages ? entry : -1; };
+    auto load = [&](St& s, int t) {   // s.entry: of this tile
+      const int page = page_in(s.entry);
+      const int64_t pl = max(page, 0);
+      const int64_t at = pl * a.c.spage_stride + kvh * a.c.shead_stride + ((t * KT + lane) & mask);
+      s.vs = a.c.vs[at];
+      s.ks = a.c.ks[at];
+      const int64_t p = max(__builtin_amdgcn_readlane(page, 16 * part), 0);
+      const int64_t code = p * a.c.page_stride + kvh * a.c.head_stride + ((t * KT + 16 * part) & mask) * D;
+      if (does_k) {
+        const uint8_t* kb = a.c.k + code;
 #pragma unroll
-    for (int c = 0; c < D / 64; ++c) s.k[c] = *reinterpret_cast<const uint4*>(kb + (64 * c + lane) * 16);
-    const float* sb = a.c.vs + p * a.c.spage_stride + kvh * a.c.shead_stride + off + 4 * hi;
-    s.vs0 = *reinterpret_cast<const float4*>(sb);
-    s.vs1 = *reinterpret_cast<const float4*>(sb + 8);
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      s.v[j] = *reinterpret_cast<const uint32_t*>(vb + (4 * hi + (j & 3) + 8 * (j >> 2)) * D + 4 * vq);
-  };
-  // codes to f16 in LDS; returns the values' reference of this tile and whether a page is absent
-  float nvref = 0.0f;
-  bool absent = false;
-  auto store = [&](Stage<D>& s, int t, int buf) {
-    const bool here = t * KT + lane < sq.len && s.page >= 0;
-    absent = __builtin_amdgcn_ballot_w64(s.page < 0) != 0;
-    const float vt = wave_max(here && s.vsl < INFINITY ? s.vsl : 0.0f);
-    // so that the largest code times its scale comes to 2^14 to 2^15: f16's range down from there is the smaller scales'
-    const float over = pow2_over(vt) * (FMT == INT8 ? 0x1p-8f : 0x1p-6f);
-    nvref = vt > 0.0f && nvref < over ? over : nvref;
-    const float iv = nvref > 0.0f ? 1.0f / nvref : 0.0f;
-    // a NaN value would reach rows that do not see its key (0 x NaN): its key is made NaN, its codes 0
-    if (wave == 0) sks[buf][lane] = fmaf(s.vsl, 0.0f, s.ksl);
-    float vs[8] = {s.vs0.x, s.vs0.y, s.vs0.z, s.vs0.w, s.vs1.x, s.vs1.y, s.vs1.z, s.vs1.w};
-    const int page = __builtin_amdgcn_readlane(s.page, 16 * wave);
-    if (t * KT + 16 * wave + 16 > sq.len || page < 0) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (page < 0 || t * KT + 16 * wave + 4 * hi + (j & 3) + 8 * (j >> 2) >= sq.len) {
-          vs[j] = 0.0f;
-          s.v[j] = 0u;
+        for (int c = 0; c < D / 64; ++c) {
+          const uint4 w = *reinterpret_cast<const uint4*>(kb + (64 * c + lane) * 16);
+          s.raw[4 * c] = w.x; s.raw[4 * c + 1] = w.y; s.raw[4 * c + 2] = w.z; s.raw[4 * c + 3] = w.w;
         }
-    }
-#pragma unroll
-    for (int c = 0; c < D / 64; ++c) {
-      const int e = 64 * c + lane;                      // 16-byte piece of the wave's 16 keys
-      const int key = 16 * wave + e / (D / 16), piece = 2 * (e % (D / 16));
-      sk[buf][k_piece<D>(key, piece)] = __builtin_bit_cast(uint4, f16x8<FMT>(s.k[c].x, s.k[c].y));
-      sk[buf][k_piece<D>(key, piece + 1)] = __builtin_bit_cast(uint4, f16x8<FMT>(s.k[c].z, s.k[c].w));
-    }
-    if (vmine) {
-      h8_t v[4], f;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) f[j] = static_cast<_Float16>(fmaxf(vs[j] * iv, 0.0f));
-      f16x8_across<FMT>(s.v, v);
-#pragma unroll
-      for (int c = 0; c < 4; ++c) sv[buf][v_piece(4 * vq + c, 2 * wave + hi)] = __builtin_bit_cast(uint4, v[c] * f);
-    }
-  };
-
-  Stage<D> stage;
-  int page_next = 0;
-  if (t0 < t1) {
-    load(stage, t0, lookup(t0));
-    page_next = lookup(t0 + 1);
-    store(stage, t0, 0);
-  }
-  __syncthreads();
-  for (int t = t0; t < t1; ++t) {
-    const int buf = (t - t0) & 1;
-    const bool more = t + 1 < t1;
-    const float tile_vref = nvref;
-    const bool tile_absent = absent;
-    const int pages_now = stage.page;
-    if (more) {
-      load(stage, t + 1, page_next);
-      page_next = lookup(t + 2);
-    }
-    if (t * KT < top_key) {
-      const bool edge = t * KT + KT > low || tile_absent;
-      if (tile_vref != vref) {
-        const float f = vref / tile_vref;
-#pragma unroll
-        for (int m = 0; m < QT; ++m)
-#pragma unroll
-          for (int d = 0; d < DT; ++d) o[m][d] *= f;
-        vref = tile_vref;
       }
-      unsigned long long gone = 0;
-      if (edge) gone = __builtin_amdgcn_ballot_w64(pages_now < 0);
+      if (does_v) {
+        const uint8_t* vb = a.c.v + code;
 #pragma unroll
+        for (int j = 0; j < 8; ++j)
+          s.raw[St::VAT + j] = *reinterpret_cast<const uint32_t*>(vb + (4 * hi + (j & 3) + 8 * (j >> 2)) * D + 4 * vq);
+      }
+    };
+    int nvref = 0;   // that of the tile converted last
+    bool absent = false;
+    auto store = [&](St& s, int t, int buf) {
+      const int page = page_in(s.entry);
+      const bool here = t * KT + lane < sq.len && page >= 0;
+      absent = __builtin_amdgcn_ballot_w64(page < 0) != 0;
+      // a NaN value would reach rows that do not see its key (0 x NaN): its key is made NaN, its codes 0
+      if (wave == 0) sks[buf][lane] = fmaf(s.vs, 0.0f, s.ks * qf);
+      const float vs = here && s.vs < INFINITY ? s.vs : 0.0f;
+      // The reference is such that the largest code times its scale comes to 2^14 to 2^15: f16's range down from there is the
+      // smaller scales'. A float that is not negative is ordered like its bits.
+      constexpr int HEAD = (FMT == INT8 ? 8 : 6) << 23;
+      if (__builtin_amdgcn_ballot_w64(__float_as_int(vs) > (nvref ? nvref + HEAD : 0)))
+        nvref = max(nvref, scalar(__float_as_int(pow2_over(wave_max(vs)))) - HEAD);
+      if (does_k) {
+#pragma unroll
+        for (int c = 0; c < D / 64; ++c) {
+          const int e = 64 * c + lane;                      // 16-byte piece of the 16 keys
+          const int key = 16 * part + e / (D / 16), piece = 2 * (e % (D / 16));
+          sk[buf][key * K_ROW<D> + piece] = __builtin_bit_cast(uint4, f16x8<FMT>(s.raw[4 * c], s.raw[4 * c + 1]));
+          sk[buf][key * K_ROW<D> + piece + 1] = __builtin_bit_cast(uint4, f16x8<FMT>(s.raw[4 * c + 2], s.raw[4 * c + 3]));
+        }
+      }
+      if (does_v) {
+        // scales through LDS from a key to a lane to the 8 keys of a piece
+        reinterpret_cast<_Float16*>(sf[wave])[(lane >> 4) * 16 + ((lane >> 2) & 1) * 8 + (lane & 3) + ((lane >> 3) & 1) * 4] =
+            static_cast<_Float16>(nvref > 0 ? vs * pow2_inverse(nvref) : 0.0f);
+        asm volatile("" ::: "memory");   // a wave's LDS accesses are in order; the compiler keeps this one
+        uint32_t w[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) w[j] = s.raw[St::VAT + j];
+        if constexpr (FMT == E4M3) {   // behind the sequence there may be NaN codes
+          if (t * KT + 16 * part + 16 > sq.len || __builtin_amdgcn_readlane(page, 16 * part) < 0) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              if (__builtin_amdgcn_readlane(page, 16 * part) < 0 || t * KT + 16 * part + 4 * hi + (j & 3) + 8 * (j >> 2) >= sq.len) w[j] = 0u;
+          }
+        }
+        h8_t v[4];
+        f16x8_across<FMT>(w, v);
+        const h8_t f = __builtin_bit_cast(h8_t, sf[wave][2 * part + hi]);
+        if (vmine) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) sv[buf][(4 * vq + c) * V_ROW + 2 * part + hi] = __builtin_bit_cast(uint4, v[c] * f);
+        }
+      }
+    };
+
+    St stage;
+    int entry_next = 0;   // looked at a tile later, when the load has come
+    if (t0 < t1) {
+      stage.entry = lookup(t0);
+      load(stage, t0);
+      entry_next = lookup(t0 + 1);
+      store(stage, t0, 0);
+    }
+
+    const f16_t zero = {};
+    auto qk = [&](const uint4* kp) __attribute__((always_inline)) {   // 32 keys against the wave's rows
+      f16_t s;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+        s = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8_t, kp[2 * ks]), q[ks], ks ? s : zero, 0, 0, 0);
+      return s;
+    };
+    // scores less a reference, base 2
+    auto scores = [&](const f16_t& s, const float4* sp, float r, float (&y)[16]) __attribute__((always_inline)) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float4 kv = sp[2 * i];
+        y[4 * i] = fmaf(s[4 * i], kv.x, -r);
+        y[4 * i + 1] = fmaf(s[4 * i + 1], kv.y, -r);
+        y[4 * i + 2] = fmaf(s[4 * i + 2], kv.z, -r);
+        y[4 * i + 3] = fmaf(s[4 * i + 3], kv.w, -r);
+      }
+    };
+    auto pv = [&](const float (&y)[16], const uint4* vp) __attribute__((always_inline)) {
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        h2_t w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float p0 = __builtin_amdgcn_exp2f(y[8 * c + 2 * e]), p1 = __builtin_amdgcn_exp2f(y[8 * c + 2 * e + 1]);
+          sum += p0 + p1;
+          w[e] = __builtin_bit_cast(h2_t, pack_h2(p0, p1));
+        }
+        const h8_t p = join(w[0], w[1], w[2], w[3]);
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+          o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8_t, vp[32 * d * V_ROW + 2 * c]), p, o[d], 0, 0, 0);
+      }
+    };
+    // Any tile: keys that a row does not see (from `most` on, or absent: gone) hidden, the reference moved where it must be
+    auto slow = [&](int buf, int most, unsigned long long gone) {
+#pragma unroll 1
       for (int h = 0; h < 2; ++h) {
-        f16_t s[QT];
+        float y[16];
+        scores(qk(&sk[buf][(32 * h + l32) * K_ROW<D> + hi]), reinterpret_cast<const float4*>(&sks[buf][32 * h + 4 * hi]), 0.0f, y);
+        const int m = most - 32 * h - 4 * hi;
+        const uint32_t g = static_cast<uint32_t>(gone >> (32 * h + 4 * hi));
+        float top = -INFINITY;
 #pragma unroll
-        for (int m = 0; m < QT; ++m)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) s[m][i] = 0.0f;
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-          const h8_t k = __builtin_bit_cast(h8_t, sk[buf][k_piece<D>(32 * h + l32, 2 * ks + hi)]);
-#pragma unroll
-          for (int m = 0; m < QT; ++m) s[m] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, q[m][ks], s[m], 0, 0, 0);
+        for (int i = 0; i < 16; ++i) {
+          const int key = 8 * (i >> 2) + (i & 3);
+          y[i] = (key >= m) | ((g >> key) & 1) ? -INFINITY : y[i];
+          top = fmax_nc(top, y[i]);
         }
-        float top[QT];
-        bool move = false;
+        top = across_max<false>(top);
+        const float now = top > ref + REF_STALE ? top - REF_UNDER : ref;
+        const float f = __builtin_amdgcn_exp2f(ref - now);
+        ref = now;
+        sum *= f;
 #pragma unroll
-        for (int m = 0; m < QT; ++m) top[m] = -INFINITY;
+        for (int d = 0; d < DT; ++d) o[d] *= f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float4 kv = *reinterpret_cast<const float4*>(&sks[buf][32 * h + 8 * i + 4 * hi]);
-          const float ks4[4] = {kv.x, kv.y, kv.z, kv.w};
-#pragma unroll
-          for (int m = 0; m < QT; ++m)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              float x = s[m][4 * i + j] * (ks4[j] * qf[m]);
-              if (edge) {
-                const int key = 32 * h + 8 * i + 4 * hi + j;
-                if (t * KT + key >= lim[m] || ((gone >> key) & 1)) x = -INFINITY;
-              }
-              s[m][4 * i + j] = x;
-              top[m] = fmaxf(top[m], x);
-            }
+        for (int i = 0; i < 16; ++i) y[i] -= now;
+        pv(y, &sv[buf][l32 * V_ROW + 4 * h + hi]);
+      }
+    };
+    // Each wave meets one barrier to a tile, whichever way it takes through it. The fast tiles are a loop of their own, which
+    // keeps the accumulators in place.
+    __syncthreads();
+    int t = t0;
+    while (t < t1) {
+      bool loaded = false;
+      auto ahead = [&]() __attribute__((always_inline)) {
+        if (t + 1 < t1) {
+          stage.entry = entry_next;
+          entry_next = lookup(t + 2);
+          load(stage, t + 1);
         }
+      };
+      // tiles whose every key every row sees
+      while (t + 1 < t1 && t * KT + KT <= low && nvref == vref && !absent) {
+        ahead();
+        const int buf = (t - t0) & 1;
+        const uint4* kp = &sk[buf][l32 * K_ROW<D> + hi];
+        const uint4* vp = &sv[buf][l32 * V_ROW + hi];
+        const float4* sp = reinterpret_cast<const float4*>(&sks[buf][4 * hi]);
+        float y0[16], y1[16];
+        const f16_t s0 = qk(kp), s1 = qk(kp + 32 * K_ROW<D>);
+        scores(s0, sp, ref, y0);
+        scores(s1, sp + 8, ref, y1);
+        float top = fmax_nc(y0[0], y1[0]);
 #pragma unroll
-        for (int m = 0; m < QT; ++m) move |= top[m] > ref[m] + REF_STALE;
-        if (__builtin_amdgcn_ballot_w64(move)) {
+        for (int i = 1; i < 16; ++i) top = max3(top, y0[i], y1[i]);
+        // issue order: the first half's key scales and 4 keys' pieces, then a read ahead of each MFMA, the first half's scores
+        // among the second's products
+        __builtin_amdgcn_sched_group_barrier(0x100, 8, 0);
 #pragma unroll
-          for (int m = 0; m < QT; ++m) {
-            const float n = across_max<false>(top[m]);
-            if (n > ref[m] + REF_STALE) {
-              const float f = __builtin_amdgcn_exp2f(ref[m] - (n - REF_UNDER));
-              ref[m] = n - REF_UNDER;
-              sum[m] *= f;
-#pragma unroll
-              for (int d = 0; d < DT; ++d) o[m][d] *= f;
-            }
-          }
-        }
-        h8_t p[QT][2];
-#pragma unroll
-        for (int m = 0; m < QT; ++m) {
-          const float r = ref[m] == -INFINITY ? 0.0f : ref[m];
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            s[m][i] = __builtin_amdgcn_exp2f(s[m][i] - r);
-            sum[m] += s[m][i];
-          }
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            uint32_t w[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) w[e] = pack_h2(s[m][8 * c + 2 * e], s[m][8 * c + 2 * e + 1]);
-            p[m][c] = join(__builtin_bit_cast(h2_t, w[0]), __builtin_bit_cast(h2_t, w[1]), __builtin_bit_cast(h2_t, w[2]),
-                           __builtin_bit_cast(h2_t, w[3]));
-          }
+        for (int i = 0; i < KS; ++i) {
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
         }
 #pragma unroll
-        for (int c = 0; c < 2; ++c)
+        for (int i = 0; i < KS; ++i) {
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(0x002, 2, 0);
+        }
+        if (__builtin_amdgcn_ballot_w64(top > REF_STALE)) {   // a reference has to move: the slow way
+          loaded = true;
+          break;
+        }
+        pv(y0, vp);
+        pv(y1, vp + 4);
+        __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
 #pragma unroll
-          for (int d = 0; d < DT; ++d) {
-            const h8_t v = __builtin_bit_cast(h8_t, sv[buf][v_piece(32 * d + l32, 4 * h + 2 * c + hi)]);
+        for (int i = 0; i < 4 * DT - 4; ++i) {
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
+        store(stage, t + 1, (t - t0 + 1) & 1);
+        __syncthreads();
+        ++t;
+      }
+      if (!loaded) ahead();
+      if (t * KT < top_key) {
+        if (nvref != vref) {
+          const float f = vref > 0 ? __int_as_float(vref) * pow2_inverse(nvref) : 0.0f;
 #pragma unroll
-            for (int m = 0; m < QT; ++m) o[m][d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, p[m][c], o[m][d], 0, 0, 0);
-          }
+          for (int d = 0; d < DT; ++d) o[d] *= f;
+          vref = nvref;
+        }
+        slow((t - t0) & 1, lim - t * KT, absent ? __builtin_amdgcn_ballot_w64(page_in(lookup(t)) < 0) : 0ull);
+      }
+      if (t + 1 < t1) store(stage, t + 1, (t - t0 + 1) & 1);
+      __syncthreads();
+      ++t;
+    }
+
+    // lane: query row l % 32, channels 32 d + 8 i + 4 (l / 32) + 0 .. 3
+    const float total = across_sum<false>(sum);
+    if (has) {
+      if (whole && !a.keep) {
+        const int tok = row / a.group, hd = kvh * a.group + row - tok * a.group;
+        const float inv = total == 0.0f ? 0.0f : __int_as_float(max(vref, 0)) / total;
+        uint16_t* dst = static_cast<uint16_t*>(a.out) + (sq.first + tok) * a.o_st + hd * a.o_sh + 4 * hi;
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            *reinterpret_cast<uint2*>(dst + 32 * d + 8 * i) = make_uint2(pack_out(a, o[d][4 * i] * inv, o[d][4 * i + 1] * inv),
+                                                                      pack_out(a, o[d][4 * i + 2] * inv, o[d][4 * i + 3] * inv));
+        if (a.lse && hi == 0)
+          a.lse[static_cast<int64_t>(sq.first + tok) * a.c.heads * a.group + hd] =
+              total == 0.0f ? -INFINITY : (__builtin_amdgcn_logf(total) + ref) * 0.6931471805599453f;
+      } else if (!whole || sw.items_before + item < a.items) {   // (a cu that falls can count rows more than once)
+        // slots: two to a workgroup (the item that it goes on with, the one that it begins), then one to an item that it completes
+        const int64_t slot = whole ? 2 * static_cast<int64_t>(a.wgs) + sw.items_before + item : 2 * static_cast<int64_t>(wg) + (t0 == 0);
+        const int rl = wave * 32 + l32;
+        const float vf = __int_as_float(max(vref, 0));
+        float* po = a.part_o + (slot * R + rl) * D + 4 * hi;
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            *reinterpret_cast<float4*>(po + 32 * d + 8 * i) =
+                make_float4(o[d][4 * i] * vf, o[d][4 * i + 1] * vf, o[d][4 * i + 2] * vf, o[d][4 * i + 3] * vf);
+        if (hi == 0) *reinterpret_cast<float2*>(a.part_ml + (slot * R + rl) * 2) = make_float2(total == 0.0f ? -INFINITY : ref, total);
       }
     }
-    if (more) store(stage, t + 1, buf ^ 1);
-    __syncthreads();
-  }
-
-  // lane: query row l % 32, channels 32 d + 8 i + 4 (l / 32) + 0 .. 3
-#pragma unroll
-  for (int m = 0; m < QT; ++m) {
-    const float total = across_sum<false>(sum[m]);
-    if (row_of[m] < 0) continue;
-    if (a.splits == 1 && !a.keep) {
-      const int tok = row_of[m] / a.group, hd = kvh * a.group + row_of[m] - tok * a.group;
-      const float inv = total == 0.0f ? 0.0f : vref / total;
-      uint16_t* dst = static_cast<uint16_t*>(a.out) + (sq.first + tok) * a.o_st + hd * a.o_sh + 4 * hi;
-#pragma unroll
-      for (int d = 0; d < DT; ++d)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          *reinterpret_cast<uint2*>(dst + 32 * d + 8 * i) = make_uint2(pack_out(a, o[m][d][4 * i] * inv, o[m][d][4 * i + 1] * inv),
-                                                                    pack_out(a, o[m][d][4 * i + 2] * inv, o[m][d][4 * i + 3] * inv));
-      if (a.lse && hi == 0)
-        a.lse[static_cast<int64_t>(sq.first + tok) * a.c.heads * a.group + hd] =
-            total == 0.0f ? -INFINITY : (__builtin_amdgcn_logf(total) + ref[m]) * 0.6931471805599453f;
-    } else {
-      const int64_t slot = (static_cast<int64_t>(kvh) * a.tiles + tile) * a.splits + split;
-      const int rl = row_of[m] - rt * R;
-      float* po = a.part_o + (slot * R + rl) * D + 4 * hi;
-#pragma unroll
-      for (int d = 0; d < DT; ++d)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          *reinterpret_cast<float4*>(po + 32 * d + 8 * i) = make_float4(o[m][d][4 * i] * vref, o[m][d][4 * i + 1] * vref,
-                                                                     o[m][d][4 * i + 2] * vref, o[m][d][4 * i + 3] * vref);
-      if (hi == 0) *reinterpret_cast<float2*>(a.part_ml + (slot * R + rl) * 2) = make_float2(ref[m], total);
-    }
+    u += share_t1 - t0;
   }
 }
 
 }  // namespace
 
-void launch_chunk(const AttnArgs& a, int fmt, int dim, int rows, int64_t grid, hipStream_t st) {
-  auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(grid)), dim3(NT), 0, st, a); };
-  if (fmt == INT8 && dim == 128) rows == 128 ? go(chunk_kernel<INT8, 128, 1>) : go(chunk_kernel<INT8, 128, 2>);
-  else if (fmt == INT8) rows == 128 ? go(chunk_kernel<INT8, 64, 1>) : go(chunk_kernel<INT8, 64, 2>);
-  else if (dim == 128) rows == 128 ? go(chunk_kernel<E4M3, 128, 1>) : go(chunk_kernel<E4M3, 128, 2>);
-  else rows == 128 ? go(chunk_kernel<E4M3, 64, 1>) : go(chunk_kernel<E4M3, 64, 2>);
+void launch_chunk(const AttnArgs& a, int fmt, int dim, int rows, hipStream_t st) {
+  auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(a.wgs)), dim3(static_cast<uint32_t>(2 * rows)), 0, st, a); };
+  if (fmt == INT8 && dim == 128) rows == 128 ? go(chunk_kernel<INT8, 128, 4>) : go(chunk_kernel<INT8, 128, 8>);
+  else if (fmt == INT8) rows == 128 ? go(chunk_kernel<INT8, 64, 4>) : go(chunk_kernel<INT8, 64, 8>);
+  else if (dim == 128) rows == 128 ? go(chunk_kernel<E4M3, 128, 4>) : go(chunk_kernel<E4M3, 128, 8>);
+  else rows == 128 ? go(chunk_kernel<E4M3, 64, 4>) : go(chunk_kernel<E4M3, 64, 8>);
 }
 
 }  // namespace kv

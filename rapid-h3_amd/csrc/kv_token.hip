@@ -33,7 +33,7 @@ __device__ __forceinline__ Pages pages_of(const AttnArgs& a, const int32_t* row,
   Pages r;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    const int i = min((tile * UNIT_KEYS + 16 * h) >> a.c.log2page, a.s.width - 1);
+    const int i = min((tile * TOKEN_KEYS + 16 * h) >> a.c.log2page, a.s.width - 1);
     const int p = row[i];
     r.p[h] = __builtin_amdgcn_readfirstlane(p >= 0 && p < a.c.pages ? p : -1);
   }
@@ -46,7 +46,7 @@ __device__ __forceinline__ void load_keys(const AttnArgs& a, int kvh, int tile, 
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     const int64_t p = max(pg.p[h], 0);
-    const int off = (tile * UNIT_KEYS + 16 * h) & ((1 << a.c.log2page) - 1);
+    const int off = (tile * TOKEN_KEYS + 16 * h) & ((1 << a.c.log2page) - 1);
     const uint8_t* kb = a.c.k + p * a.c.page_stride + kvh * a.c.head_stride + off * D;
 #pragma unroll
     for (int c = 0; c < D / 64; ++c) t.k[h][c] = *reinterpret_cast<const uint4*>(kb + (l16 * D + 64 * c + 16 * g));
@@ -59,7 +59,7 @@ __device__ __forceinline__ void load_values(const AttnArgs& a, int kvh, int tile
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     const int64_t p = max(pg.p[h], 0);
-    const int off = (tile * UNIT_KEYS + 16 * h) & ((1 << a.c.log2page) - 1);
+    const int off = (tile * TOKEN_KEYS + 16 * h) & ((1 << a.c.log2page) - 1);
     const uint8_t* vb = a.c.v + p * a.c.page_stride + kvh * a.c.head_stride + off * D;
     t.vs[h] = *reinterpret_cast<const float4*>(a.c.vs + p * a.c.spage_stride + kvh * a.c.shead_stride + off + 4 * g);
 #pragma unroll
@@ -90,9 +90,9 @@ __device__ __forceinline__ void compute(const AttnArgs& a, Tile<D>& t, int kvh, 
                                         const h8_t (&q)[MT][D / 32], const float (&qf)[MT], const int (&lim)[MT], int low, int len,
                                         State<D, MT>& st) {
   const int lane = threadIdx.x & 63, g = lane >> 4;
-  const int kb = tile * UNIT_KEYS;
+  const int kb = tile * TOKEN_KEYS;
   // low: keys that every row sees
-  const bool edge = kb + UNIT_KEYS > low || pg.p[0] < 0 || pg.p[1] < 0;
+  const bool edge = kb + TOKEN_KEYS > low || pg.p[0] < 0 || pg.p[1] < 0;
   float ks[8] = {t.ks[0].x, t.ks[0].y, t.ks[0].z, t.ks[0].w, t.ks[1].x, t.ks[1].y, t.ks[1].z, t.ks[1].w};
   float vs[8] = {t.vs[0].x, t.vs[0].y, t.vs[0].z, t.vs[0].w, t.vs[1].x, t.vs[1].y, t.vs[1].z, t.vs[1].w};
 #pragma unroll
@@ -213,30 +213,31 @@ __device__ __forceinline__ void compute(const AttnArgs& a, Tile<D>& t, int kvh, 
 template <int FMT, int D, int MT>
 __global__ void __launch_bounds__(NT, 2) token_kernel(AttnArgs a) {
   constexpr int R = 16 * MT, PAD = D + 4;
+  const Tiling TILING = tiling(false, R);
   __shared__ float so[WAVES][R][PAD];
   __shared__ float sm[WAVES][R], sl[WAVES][R];
   const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   Block blk;
-  const Work work = dealt(load_blocks(a, R, blk), a.wgs);
+  const Work work = dealt(load_blocks(a, TILING, blk), a.wgs, TILING);
   const int wg = blockIdx.x;
   if (wg >= work.wgs) return;
-  int64_t u = share_begin(work, wg);
-  const int64_t end = share_begin(work, wg + 1);
+  int64_t u = scalar(share_begin(work, wg));
+  const int64_t end = scalar(share_begin(work, wg + 1));
 
   while (u < end) {
     while (u >= blk.end()) {
       if (blk.at + 64 >= a.s.batch) return;
-      next_block(a, R, blk);
+      next_block(a, TILING, blk);
     }
     const int l = __builtin_ctzll(__builtin_amdgcn_ballot_w64(blk.base + blk.units > u));
     const SeqItems sw = seq_in(a, blk, l);
     const Seq sq = sw.seq;
     const int64_t local = u - sw.before;
-    const int item = static_cast<int>(quotient(local, sw.key_tiles));
+    const int item = scalar(static_cast<int>(quotient(local, sw.key_tiles)));
     const int t0 = static_cast<int>(local - static_cast<int64_t>(item) * sw.key_tiles);
     const int t1 = static_cast<int>(end - u < sw.key_tiles - t0 ? t0 + (end - u) : sw.key_tiles);
-    const int kvh = item / sw.row_tiles, rt = item - kvh * sw.row_tiles;
+    const int kvh = scalar(item / sw.row_tiles), rt = item - kvh * sw.row_tiles;
     const int rows = sq.n * a.group;
 
     // query rows: lane l holds row l % 16, channels 64 c + 16 (l / 16) + 0 .. 15 in steps 2 c and 2 c + 1
@@ -265,7 +266,7 @@ __global__ void __launch_bounds__(NT, 2) token_kernel(AttnArgs a) {
       qf[m] = __builtin_amdgcn_ldexpf(a.scale_log2, -e);
       lim[m] = a.causal ? min(sq.len, sq.len - sq.n + tok + 1) : sq.len;
     }
-    const int low = a.causal ? min(sq.len, sq.len - sq.n + (rt * R) / a.group + 1) : sq.len;
+    const int low = a.causal ? min(sq.len, sq.len - sq.n + scalar((rt * R) / a.group) + 1) : sq.len;
 
     State<D, MT> st;
     st.vref = 0.0f;

@@ -148,12 +148,12 @@ def _attention(name, q, cache, prefix, prefix_len, table, lens, cu, causal, scal
     elif out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1 or out.device != dev:
         raise RuntimeError(f"{name}: out must be like q, with a contiguous last dim")
     sums = alloc((t, hq), dtype=torch.float32, device=dev) if lse else None
-    n = nat.lib().rh3_kv_attention_workspace_bytes(cache._ref, hq, t, seqs[2], seqs[5], int(cu is None), prefix_len)
-    ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
+    n = nat.lib().rh3_kv_attention_workspace_bytes(cache._ref, hq, t, seqs[5], cu is None, prefix_len)
+    ws = torch.empty(n, dtype=torch.uint8, device=dev)
     with _on(dev):
         nat.call("rh3_kv_attention", cache._ref, q.data_ptr(), q.stride(0), q.stride(1), hq, _ROW[q.dtype], t, *seqs, int(causal),
                  d ** -0.5 if scale is None else scale, out.data_ptr(), out.stride(0), out.stride(1), nat.ptr(sums),
-                 nat.ptr(prefix), prefix_len, nat.ptr(ws), n, nat.stream(dev))
+                 nat.ptr(prefix), prefix_len, ws.data_ptr(), n, nat.stream(dev))
     return (out, sums) if lse else out
 
 
