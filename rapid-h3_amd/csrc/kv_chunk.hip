@@ -225,46 +225,28 @@ __global__ void __launch_bounds__(WAVES * 64, 2) chunk_kernel(AttnArgs a) {
     }
 
     const f16_t zero = {};
-    auto qk = [&](const uint4* kp) __attribute__((always_inline)) {   // 32 keys against the wave's rows
-      f16_t s;
+    auto probabilities = [&](const float* y) __attribute__((always_inline)) {   // of 8 keys, added to the sum
+      h2_t w[4];
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks)
-        s = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8_t, kp[2 * ks]), q[ks], ks ? s : zero, 0, 0, 0);
-      return s;
-    };
-    // scores less a reference, base 2
-    auto scores = [&](const f16_t& s, const float4* sp, float r, float (&y)[16]) __attribute__((always_inline)) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float4 kv = sp[2 * i];
-        y[4 * i] = fmaf(s[4 * i], kv.x, -r);
-        y[4 * i + 1] = fmaf(s[4 * i + 1], kv.y, -r);
-        y[4 * i + 2] = fmaf(s[4 * i + 2], kv.z, -r);
-        y[4 * i + 3] = fmaf(s[4 * i + 3], kv.w, -r);
+      for (int e = 0; e < 4; ++e) {
+        const float p0 = __builtin_amdgcn_exp2f(y[2 * e]), p1 = __builtin_amdgcn_exp2f(y[2 * e + 1]);
+        sum += p0 + p1;
+        w[e] = __builtin_bit_cast(h2_t, pack_h2(p0, p1));
       }
-    };
-    auto pv = [&](const float (&y)[16], const uint4* vp) __attribute__((always_inline)) {
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        h2_t w[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float p0 = __builtin_amdgcn_exp2f(y[8 * c + 2 * e]), p1 = __builtin_amdgcn_exp2f(y[8 * c + 2 * e + 1]);
-          sum += p0 + p1;
-          w[e] = __builtin_bit_cast(h2_t, pack_h2(p0, p1));
-        }
-        const h8_t p = join(w[0], w[1], w[2], w[3]);
-#pragma unroll
-        for (int d = 0; d < DT; ++d)
-          o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8_t, vp[32 * d * V_ROW + 2 * c]), p, o[d], 0, 0, 0);
-      }
+      return join(w[0], w[1], w[2], w[3]);
     };
     // Any tile: keys that a row does not see (from `most` on, or absent: gone) hidden, the reference moved where it must be
     auto slow = [&](int buf, int most, unsigned long long gone) {
 #pragma unroll 1
       for (int h = 0; h < 2; ++h) {
         float y[16];
-        scores(qk(&sk[buf][(32 * h + l32) * K_ROW<D> + hi]), reinterpret_cast<const float4*>(&sks[buf][32 * h + 4 * hi]), 0.0f, y);
+        const uint4* kp = &sk[buf][(32 * h + l32) * K_ROW<D> + hi];
+        const uint4* vp = &sv[buf][l32 * V_ROW + 4 * h + hi];
+        f16_t s = zero;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) s = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8_t, kp[2 * ks]), q[ks], s, 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) y[i] = s[i] * sks[buf][32 * h + 8 * (i >> 2) + 4 * hi + (i & 3)];
         const int m = most - 32 * h - 4 * hi;
         const uint32_t g = static_cast<uint32_t>(gone >> (32 * h + 4 * hi));
         float top = -INFINITY;
@@ -283,7 +265,13 @@ __global__ void __launch_bounds__(WAVES * 64, 2) chunk_kernel(AttnArgs a) {
         for (int d = 0; d < DT; ++d) o[d] *= f;
 #pragma unroll
         for (int i = 0; i < 16; ++i) y[i] -= now;
-        pv(y, &sv[buf][l32 * V_ROW + 4 * h + hi]);
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const h8_t p = probabilities(y + 8 * c);
+#pragma unroll
+          for (int d = 0; d < DT; ++d)
+            o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8_t, vp[32 * d * V_ROW + 2 * c]), p, o[d], 0, 0, 0);
+        }
       }
     };
     // Each wave meets one barrier to a tile, whichever way it takes through it. The fast tiles are a loop of their own, which
@@ -306,40 +294,49 @@ __global__ void __launch_bounds__(WAVES * 64, 2) chunk_kernel(AttnArgs a) {
         const uint4* kp = &sk[buf][l32 * K_ROW<D> + hi];
         const uint4* vp = &sv[buf][l32 * V_ROW + hi];
         const float4* sp = reinterpret_cast<const float4*>(&sks[buf][4 * hi]);
-        float y0[16], y1[16];
-        const f16_t s0 = qk(kp), s1 = qk(kp + 32 * K_ROW<D>);
-        scores(s0, sp, ref, y0);
-        scores(s1, sp + 8, ref, y1);
-        float top = fmax_nc(y0[0], y1[0]);
+        // Each MFMA's operand is read four MFMAs (128 cycles) before it; left alone, the compiler puts every read right before its
+        // use. Only vector and scalar arithmetic moves past a step's end.
+        constexpr int AHEAD = 4, ARITH = 0x2 | 0x4 | 0x400;
+        float4 kv[8];
+        h8_t f[AHEAD];
+        f16_t s[2];
 #pragma unroll
-        for (int i = 1; i < 16; ++i) top = max3(top, y0[i], y1[i]);
-        // issue order: the first half's key scales and 4 keys' pieces, then a read ahead of each MFMA, the first half's scores
-        // among the second's products
-        __builtin_amdgcn_sched_group_barrier(0x100, 8, 0);
+        for (int i = 0; i < 4; ++i) kv[i] = sp[2 * i];
 #pragma unroll
-        for (int i = 0; i < KS; ++i) {
-          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-          __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        for (int i = 0; i < AHEAD; ++i) f[i] = __builtin_bit_cast(h8_t, kp[2 * i]);
+        __builtin_amdgcn_sched_barrier(ARITH);
+#pragma unroll
+        for (int i = 0; i < 2 * KS; ++i) {
+          const int h = i / KS, ks = i % KS, n = i + AHEAD;
+          s[h] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[i % AHEAD], q[ks], ks ? s[h] : zero, 0, 0, 0);
+          if (n < 2 * KS) f[i % AHEAD] = __builtin_bit_cast(h8_t, kp[32 * (n / KS) * K_ROW<D> + 2 * (n % KS)]);
+          else kv[4 + n - 2 * KS] = sp[8 + 2 * (n - 2 * KS)];
+          __builtin_amdgcn_sched_barrier(ARITH);
         }
 #pragma unroll
-        for (int i = 0; i < KS; ++i) {
-          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-          __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-          __builtin_amdgcn_sched_group_barrier(0x002, 2, 0);
+        for (int i = 0; i < AHEAD; ++i) f[i] = __builtin_bit_cast(h8_t, vp[32 * (i % DT) * V_ROW + 2 * (i / DT)]);
+        float y[32], top = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          y[4 * i] = fmaf(s[i / 4][4 * (i % 4)], kv[i].x, -ref);
+          y[4 * i + 1] = fmaf(s[i / 4][4 * (i % 4) + 1], kv[i].y, -ref);
+          y[4 * i + 2] = fmaf(s[i / 4][4 * (i % 4) + 2], kv[i].z, -ref);
+          y[4 * i + 3] = fmaf(s[i / 4][4 * (i % 4) + 3], kv[i].w, -ref);
+          top = max3(max3(top, y[4 * i], y[4 * i + 1]), y[4 * i + 2], y[4 * i + 3]);
         }
         if (__builtin_amdgcn_ballot_w64(top > REF_STALE)) {   // a reference has to move: the slow way
           loaded = true;
           break;
         }
-        pv(y0, vp);
-        pv(y1, vp + 4);
-        __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+        h8_t p;
 #pragma unroll
-        for (int i = 0; i < 4 * DT - 4; ++i) {
-          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-          __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        for (int i = 0; i < 4 * DT; ++i) {
+          const int c = i / DT, d = i % DT, n = i + AHEAD;
+          if (d == 0) p = probabilities(y + 8 * c);
+          o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[i % AHEAD], p, o[d], 0, 0, 0);
+          if (n < 4 * DT) f[i % AHEAD] = __builtin_bit_cast(h8_t, vp[32 * (n % DT) * V_ROW + 2 * (n / DT)]);
+          __builtin_amdgcn_sched_barrier(ARITH);
         }
-        __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
         store(stage, t + 1, (t - t0 + 1) & 1);
         __syncthreads();
         ++t;
