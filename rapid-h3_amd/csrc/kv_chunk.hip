@@ -27,32 +27,32 @@ constexpr float NO_REF = -0x1p100f;   // reference of a row that has seen no key
 // parts of the banks, and every read of a tile is one lane address with an immediate offset.
 template <int D>
 constexpr int K_ROW = D / 8 + 1;                               // K: [64 keys][D] f16
-constexpr int V_ROW = KT / 8 + 1;                              // V^T: [D][64 keys] f16, pieces of 8 keys
+// V: the same, but read by transposing loads (8 bytes a lane, 4 rows x 32 channels to 32 lanes): rows 64 bytes apart in the banks
+template <int D>
+constexpr int V_ROW = D / 8 + 4;
 
-// What a wave has in flight of a tile: the codes that it will convert, and of key l of the 64 its scales and table entry. With 8
-// waves a wave has keys or values, in the same registers.
-template <int D, int WAVES>
-struct Stage {
-  static constexpr int KW = D / 16, VAT = WAVES == 4 ? KW : 0;
-  uint32_t raw[VAT + 8];       // words of 16 keys (KW), of 8 keys x 4 channels (8 from VAT)
-  float vs, ks;
-  int entry;
-};
+// 4 rows x 16 channels to 16 lanes: lane i gives the address of row i / 4, channels 4 (i % 4) + 0 .. 3, and gets channel i's 4 rows
+typedef __fp16 g4_t __attribute__((__vector_size__(4 * sizeof(__fp16))));
+typedef _Float16 h4_t __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ h4_t lds_read_tr(const uint8_t* p) {
+  return __builtin_bit_cast(h4_t, __builtin_amdgcn_ds_read_tr16_b64_v4f16((__attribute__((address_space(3))) g4_t*)p));
+}
+// a table entry by the scalar cache: the same address in all lanes, and nothing that a kernel writes
+__device__ __forceinline__ int scalar_load(const int32_t* p) {
+  return *(const __attribute__((address_space(4))) int32_t*)(p);
+}
 
 template <int FMT, int D, int WAVES>
 __global__ void __launch_bounds__(WAVES * 64, 2) chunk_kernel(AttnArgs a) {
   constexpr int R = WAVES * 32, KS = D / 16, DT = D / 32;
   const Tiling TILING = tiling(true, R);
   __shared__ uint4 sk[2][KT * K_ROW<D>];
-  __shared__ uint4 sv[2][D * V_ROW];
-  __shared__ float sks[2][KT];
-  __shared__ uint4 sf[WAVES][KT / 8];   // a wave's value scales as f16, in V's key order
-  __shared__ float stop[WAVES];
+  __shared__ uint4 sv[2][KT * V_ROW<D>];
+  __shared__ float sks[8][32];            // key scales of 8 half tiles in turn
+  __shared__ float stop[WAVES], sscale[WAVES];
   const int lane = threadIdx.x & 63, l32 = lane & 31, hi = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  // of the 64 keys, a wave converts 16 keys and 16 values (4 waves), or 16 of either (8 waves: the first four keys)
-  const int part = wave & 3;
-  const bool does_k = WAVES == 4 || wave < 4, does_v = WAVES == 4 || wave >= 4;
+  constexpr int NP = 8 / WAVES;           // pieces of 8 keys that a wave converts
 
   // neighbouring shares, which read the same keys, on one XCD (workgroups are dealt to the 8 XCDs in turn)
   const int n8 = a.wgs & ~7;
@@ -94,8 +94,12 @@ __global__ void __launch_bounds__(WAVES * 64, 2) chunk_kernel(AttnArgs a) {
     const bool has = row < rows;
     const int rr = has ? row : rows - 1;
     const int tok = rr / a.group, hd = kvh * a.group + rr - tok * a.group;
+    const int32_t* table = a.s.table + seq * a.s.table_stride;
+    const int mask = (1 << a.c.log2page) - 1;
+    auto page_in = [&](int entry) { return entry >= 0 && entry < a.c.pages ? entry : -1; };
     h8_t q[KS];
     float qf;
+    int vref;   // bits of a power of two, the same in all lanes
     {
       const int64_t qat = (sq.first + tok) * a.q_st + hd * a.q_sh + 8 * hi;
       float top = 0.0f;
@@ -107,10 +111,29 @@ __global__ void __launch_bounds__(WAVES * 64, 2) chunk_kernel(AttnArgs a) {
         for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[e]) < INFINITY ? fabsf(x[e]) : 0.0f);
       }
       top = wave_max(top);
-      if (lane == 0) stop[wave] = top;
+      // the largest finite scale of the share's values, 4 keys (of one page) to a thread at a time
+      float big = 0.0f;
+#pragma unroll 4
+      for (int key = t0 * KT + 4 * static_cast<int>(threadIdx.x); key < min(t1 * KT, sq.len); key += 4 * WAVES * 64) {
+        const int page = page_in(table[min(key >> a.c.log2page, a.s.width - 1)]);
+        const float4 v = *reinterpret_cast<const float4*>(a.c.vs + max(page, 0) * a.c.spage_stride + kvh * a.c.shead_stride + (key & mask));
+        const float x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) big = fmaxf(big, page >= 0 && key + e < sq.len && x[e] < INFINITY ? x[e] : 0.0f);
+      }
+      big = wave_max(big);
+      if (lane == 0) {
+        stop[wave] = top;
+        sscale[wave] = big;
+      }
       __syncthreads();
 #pragma unroll
-      for (int w = 0; w < WAVES; ++w) top = fmaxf(top, stop[w]);
+      for (int w = 0; w < WAVES; ++w) {
+        top = fmaxf(top, stop[w]);
+        big = fmaxf(big, sscale[w]);
+      }
+      // V's reference: the largest code times its scale comes to 2^14 to 2^15; f16's range down from there is the smaller scales'
+      vref = scalar(__float_as_int(pow2_over(big))) - ((FMT == INT8 ? 8 : 6) << 23);
       const int e = q_exponent(top);
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
@@ -128,103 +151,103 @@ __global__ void __launch_bounds__(WAVES * 64, 2) chunk_kernel(AttnArgs a) {
 
     f16_t o[DT];
     float ref = NO_REF, sum = 0.0f;
-    int vref = -1;   // bits of the values' reference, the same in all lanes; no tile has that of -1: the first one is never fast
 #pragma unroll
     for (int d = 0; d < DT; ++d)
 #pragma unroll
       for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
 
-    const int32_t* table = a.s.table + seq * a.s.table_stride;
-    const int mask = (1 << a.c.log2page) - 1;
-    auto lookup = [&](int t) {   // table entry of key l of tile t
-      return table[min((t * KT + lane) >> a.c.log2page, a.s.width - 1)];
+    // Window w: keys [64 w - 32, 64 w + 32). Stage x in LDS (buffer x & 1) has K of window x + 1 and V of window x. A wave brings 8
+    // NP keys of a window, which lie in one page; lane l has 1 / 8 of key l / 8 of each 8.
+    const int first = 8 * NP * wave;
+    auto lookup = [&](int w) {   // the entry of the wave's page; the first window begins before the sequence
+      return scalar_load(table + min(max(w * KT - 32 + first, 0) >> a.c.log2page, a.s.width - 1));
     };
-    // V: a thread takes 4 channels of the 8 keys of one piece; D 64: the first 16 lanes of each half
-    const int vq = lane & (D / 4 - 1);
-    const bool vmine = D == 128 || (lane & 16) == 0;
-    using St = Stage<D, WAVES>;
-    auto page_in = [&](int entry) { return entry >= 0 && entry < a.c.pages ? entry : -1; };
-    auto load = [&](St& s, int t) {   // s.entry: of this tile
-      const int page = page_in(s.entry);
-      const int64_t pl = max(page, 0);
-      const int64_t at = pl * a.c.spage_stride + kvh * a.c.shead_stride + ((t * KT + lane) & mask);
-      s.vs = a.c.vs[at];
-      s.ks = a.c.ks[at];
-      const int64_t p = max(__builtin_amdgcn_readlane(page, 16 * part), 0);
-      const int64_t code = p * a.c.page_stride + kvh * a.c.head_stride + ((t * KT + 16 * part) & mask) * D;
-      if (does_k) {
-        const uint8_t* kb = a.c.k + code;
+    auto all_there = [&](int s) {   // no key of step s in an absent page
+      int bad = 0;
 #pragma unroll
-        for (int c = 0; c < D / 64; ++c) {
-          const uint4 w = *reinterpret_cast<const uint4*>(kb + (64 * c + lane) * 16);
-          s.raw[4 * c] = w.x; s.raw[4 * c + 1] = w.y; s.raw[4 * c + 2] = w.z; s.raw[4 * c + 3] = w.w;
-        }
+      for (int i = 0; i < 4; ++i) {
+        const int e = scalar_load(table + min((s * KT + 16 * i) >> a.c.log2page, a.s.width - 1));
+        bad |= e < 0 || e >= a.c.pages;
       }
-      if (does_v) {
-        const uint8_t* vb = a.c.v + code;
+      return bad == 0;
+    };
+    uint32_t kraw[NP][D / 32], vraw[NP][D / 32];
+    float ks[NP], kvs[NP], vs[NP];         // scales of the lane's keys: key and value of K's window, value of V's
+    int kpage, vpage, entry;               // the wave's pages in the two windows; the entry for K's next one
+    auto load_codes = [&](const uint8_t* base, int page, int w, uint32_t (&raw)[NP][D / 32]) __attribute__((always_inline)) {
+      const uint8_t* at = base + (max(page, 0) * a.c.page_stride + kvh * a.c.head_stride + ((w * KT - 32 + first) & mask) * D);
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-          s.raw[St::VAT + j] = *reinterpret_cast<const uint32_t*>(vb + (4 * hi + (j & 3) + 8 * (j >> 2)) * D + 4 * vq);
+      for (int i = 0; i < NP; ++i) {
+        if constexpr (D == 128) {
+          const uint4 r = *reinterpret_cast<const uint4*>(at + (16 * lane + 8 * D * i));
+          raw[i][0] = r.x; raw[i][1] = r.y; raw[i][2] = r.z; raw[i][3] = r.w;
+        } else {
+          const uint2 r = *reinterpret_cast<const uint2*>(at + (8 * lane + 8 * D * i));
+          raw[i][0] = r.x; raw[i][1] = r.y;
+        }
       }
     };
-    int nvref = 0;   // that of the tile converted last
-    bool absent = false;
-    auto store = [&](St& s, int t, int buf) {
-      const int page = page_in(s.entry);
-      const bool here = t * KT + lane < sq.len && page >= 0;
-      absent = __builtin_amdgcn_ballot_w64(page < 0) != 0;
-      // a NaN value would reach rows that do not see its key (0 x NaN): its key is made NaN, its codes 0
-      if (wave == 0) sks[buf][lane] = fmaf(s.vs, 0.0f, s.ks * qf);
-      const float vs = here && s.vs < INFINITY ? s.vs : 0.0f;
-      // The reference is such that the largest code times its scale comes to 2^14 to 2^15: f16's range down from there is the
-      // smaller scales'. A float that is not negative is ordered like its bits.
-      constexpr int HEAD = (FMT == INT8 ? 8 : 6) << 23;
-      if (__builtin_amdgcn_ballot_w64(__float_as_int(vs) > (nvref ? nvref + HEAD : 0)))
-        nvref = max(nvref, scalar(__float_as_int(pow2_over(wave_max(vs)))) - HEAD);
-      if (does_k) {
+    auto load_k = [&](int w) __attribute__((always_inline)) {
+      const int64_t at = max(kpage, 0) * a.c.spage_stride + kvh * a.c.shead_stride + ((w * KT - 32 + first) & mask);
 #pragma unroll
-        for (int c = 0; c < D / 64; ++c) {
-          const int e = 64 * c + lane;                      // 16-byte piece of the 16 keys
-          const int key = 16 * part + e / (D / 16), piece = 2 * (e % (D / 16));
-          sk[buf][key * K_ROW<D> + piece] = __builtin_bit_cast(uint4, f16x8<FMT>(s.raw[4 * c], s.raw[4 * c + 1]));
-          sk[buf][key * K_ROW<D> + piece + 1] = __builtin_bit_cast(uint4, f16x8<FMT>(s.raw[4 * c + 2], s.raw[4 * c + 3]));
-        }
+      for (int i = 0; i < NP; ++i) {
+        ks[i] = (a.c.ks + at)[8 * i + (lane >> 3)];
+        kvs[i] = (a.c.vs + at)[8 * i + (lane >> 3)];
       }
-      if (does_v) {
-        // scales through LDS from a key to a lane to the 8 keys of a piece
-        reinterpret_cast<_Float16*>(sf[wave])[(lane >> 4) * 16 + ((lane >> 2) & 1) * 8 + (lane & 3) + ((lane >> 3) & 1) * 4] =
-            static_cast<_Float16>(nvref > 0 ? vs * pow2_inverse(nvref) : 0.0f);
-        asm volatile("" ::: "memory");   // a wave's LDS accesses are in order; the compiler keeps this one
-        uint32_t w[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) w[j] = s.raw[St::VAT + j];
-        if constexpr (FMT == E4M3) {   // behind the sequence there may be NaN codes
-          if (t * KT + 16 * part + 16 > sq.len || __builtin_amdgcn_readlane(page, 16 * part) < 0) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-              if (__builtin_amdgcn_readlane(page, 16 * part) < 0 || t * KT + 16 * part + 4 * hi + (j & 3) + 8 * (j >> 2) >= sq.len) w[j] = 0u;
-          }
-        }
-        h8_t v[4];
-        f16x8_across<FMT>(w, v);
-        const h8_t f = __builtin_bit_cast(h8_t, sf[wave][2 * part + hi]);
-        if (vmine) {
-#pragma unroll
-          for (int c = 0; c < 4; ++c) sv[buf][(4 * vq + c) * V_ROW + 2 * part + hi] = __builtin_bit_cast(uint4, v[c] * f);
-        }
+      load_codes(a.c.k, kpage, w, kraw);
+    };
+    // Stage x (loaded) to LDS in 2 NP parts of K and 2 NP of V; the loads of stage x + 1
+    auto put_k = [&](int x, int part) __attribute__((always_inline)) {
+      const int i = part / 2, c = part % 2, key = first + 8 * i + (lane >> 3);
+      // a NaN value would reach rows that do not see its key (0 x NaN): its key is made NaN
+      if (c == 0) sks[(2 * x + 1 + (key >> 5)) & 7][key & 31] = fmaf(kvs[i], 0.0f, ks[i] * qf);
+      if (c < D / 64)
+        sk[x & 1][key * K_ROW<D> + (lane & 7) * (D / 64) + c] = __builtin_bit_cast(uint4, f16x8<FMT>(kraw[i][2 * c], kraw[i][2 * c + 1]));
+    };
+    const float vinv = pow2_inverse(vref);
+    auto put_v = [&](int x, int part) __attribute__((always_inline)) {
+      const int i = part / 2, c = part % 2, key = first + 8 * i + (lane >> 3);
+      // outside the share's keys and in an absent page there may be anything: 0 (and codes that can be NaN go)
+      const int pos = x * KT - 32 + key;
+      const bool here = vpage >= 0 && pos >= t0 * KT && pos < min(sq.len, t1 * KT);
+      const _Float16 f = static_cast<_Float16>(here && vs[i] < INFINITY ? vs[i] * vinv : 0.0f);
+      if (c < D / 64) {
+        const bool keep = FMT == INT8 || here;
+        const h8_t v = f16x8<FMT>(keep ? vraw[i][2 * c] : 0u, keep ? vraw[i][2 * c + 1] : 0u);
+        sv[x & 1][key * V_ROW<D> + (lane & 7) * (D / 64) + c] = __builtin_bit_cast(uint4, v * f);
       }
+    };
+    auto load_next = [&](int x) __attribute__((always_inline)) {
+#pragma unroll
+      for (int i = 0; i < NP; ++i) vs[i] = kvs[i];
+      vpage = kpage;
+      kpage = page_in(entry);
+      entry = lookup(x + 3);
+      load_k(x + 2);
+      load_codes(a.c.v, vpage, x + 1, vraw);
+    };
+    auto stage = [&](int x) __attribute__((always_inline)) {
+#pragma unroll
+      for (int i = 0; i < 2 * NP; ++i) put_k(x, i);
+#pragma unroll
+      for (int i = 0; i < 2 * NP; ++i) put_v(x, i);
+      load_next(x);
     };
 
-    St stage;
-    int entry_next = 0;   // looked at a tile later, when the load has come
-    if (t0 < t1) {
-      stage.entry = lookup(t0);
-      load(stage, t0);
-      entry_next = lookup(t0 + 1);
-      store(stage, t0, 0);
-    }
-
+    // The products of a half tile's keys with the wave's rows, of values with probabilities, and in between a half tile's softmax:
+    // half h is scored while half h - 1's values are summed and half h + 1's products run, so that matrix and vector
+    // instructions always have each other's company. Step s does halves 2 s and 2 s + 1 with stage s.
     const f16_t zero = {};
+    f16_t sa = zero, sb = zero;            // products of the next even and odd half
+    h8_t p[2] = {};                        // probabilities of the last half
+    constexpr int AHEAD = 4;
+    auto k_at = [&](int b, int half, int ks) { return __builtin_bit_cast(h8_t, sk[b][(32 * half + l32) * K_ROW<D> + hi + 2 * ks]); };
+    const uint8_t* v_lane = reinterpret_cast<const uint8_t*>(sv) + (4 * hi + ((lane & 15) >> 2)) * V_ROW<D> * 16 + ((lane >> 4) & 1) * 32 + (lane & 3) * 8;
+    auto v_at = [&](int b, int half, int i) {   // i: k-step * DT + channel tile
+      const uint8_t* at = v_lane + ((b * KT + 32 * half + 16 * (i / DT)) * V_ROW<D> * 16 + 64 * (i % DT));
+      const h4_t lo = lds_read_tr(at), up = lds_read_tr(at + 8 * V_ROW<D> * 16);
+      return __builtin_shufflevector(lo, up, 0, 1, 2, 3, 4, 5, 6, 7);
+    };
     auto probabilities = [&](const float* y) __attribute__((always_inline)) {   // of 8 keys, added to the sum
       h2_t w[4];
 #pragma unroll
@@ -235,133 +258,174 @@ __global__ void __launch_bounds__(WAVES * 64, 2) chunk_kernel(AttnArgs a) {
       }
       return join(w[0], w[1], w[2], w[3]);
     };
-    // Any tile: keys that a row does not see (from `most` on, or absent: gone) hidden, the reference moved where it must be
-    auto slow = [&](int buf, int most, unsigned long long gone) {
-#pragma unroll 1
-      for (int h = 0; h < 2; ++h) {
-        float y[16];
-        const uint4* kp = &sk[buf][(32 * h + l32) * K_ROW<D> + hi];
-        const uint4* vp = &sv[buf][l32 * V_ROW + 4 * h + hi];
-        f16_t s = zero;
+    // a KS-th of a half tile's scores less the row's reference, and their largest; a 2 DT-th of its probabilities
+    auto score = [&](const f16_t& s, const float4 (&kv)[4], int i, float (&y)[16], float& top) __attribute__((always_inline)) {
+      constexpr int N = 16 / KS;
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) s = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8_t, kp[2 * ks]), q[ks], s, 0, 0, 0);
+      for (int e = N * i; e < N * i + N; ++e) {
+        const float4 k = kv[e / 4];
+        y[e] = fmaf(s[e], e % 4 == 0 ? k.x : e % 4 == 1 ? k.y : e % 4 == 2 ? k.z : k.w, -ref);
+      }
 #pragma unroll
-        for (int i = 0; i < 16; ++i) y[i] = s[i] * sks[buf][32 * h + 8 * (i >> 2) + 4 * hi + (i & 3)];
-        const int m = most - 32 * h - 4 * hi;
-        const uint32_t g = static_cast<uint32_t>(gone >> (32 * h + 4 * hi));
-        float top = -INFINITY;
+      for (int e = N * i; e < N * i + N; e += 2) top = max3(top, y[e], y[e + 1]);
+    };
+    auto probability = [&](float (&y)[16], int i, h8_t (&n)[2]) __attribute__((always_inline)) {
+      constexpr int N = 8 / DT;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int key = 8 * (i >> 2) + (i & 3);
-          y[i] = (key >= m) | ((g >> key) & 1) ? -INFINITY : y[i];
-          top = fmax_nc(top, y[i]);
-        }
-        top = across_max<false>(top);
-        const float now = top > ref + REF_STALE ? top - REF_UNDER : ref;
-        const float f = __builtin_amdgcn_exp2f(ref - now);
-        ref = now;
-        sum *= f;
-#pragma unroll
-        for (int d = 0; d < DT; ++d) o[d] *= f;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) y[i] -= now;
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const h8_t p = probabilities(y + 8 * c);
-#pragma unroll
-          for (int d = 0; d < DT; ++d)
-            o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8_t, vp[32 * d * V_ROW + 2 * c]), p, o[d], 0, 0, 0);
-        }
+      for (int e = N * i; e < N * i + N; e += 2) {
+        const float p0 = __builtin_amdgcn_exp2f(y[e]), p1 = __builtin_amdgcn_exp2f(y[e + 1]);
+        sum += p0 + p1;
+        const h2_t w = __builtin_bit_cast(h2_t, pack_h2(p0, p1));
+        n[e / 8][e % 8] = w[0];
+        n[e / 8][e % 8 + 1] = w[1];
       }
     };
-    // Each wave meets one barrier to a tile, whichever way it takes through it. The fast tiles are a loop of their own, which
-    // keeps the accumulators in place.
-    __syncthreads();
-    int t = t0;
-    while (t < t1) {
-      bool loaded = false;
-      auto ahead = [&]() __attribute__((always_inline)) {
-        if (t + 1 < t1) {
-          stage.entry = entry_next;
-          entry_next = lookup(t + 2);
-          load(stage, t + 1);
-        }
-      };
-      // tiles whose every key every row sees
-      while (t + 1 < t1 && t * KT + KT <= low && nvref == vref && !absent) {
-        ahead();
-        const int buf = (t - t0) & 1;
-        const uint4* kp = &sk[buf][l32 * K_ROW<D> + hi];
-        const uint4* vp = &sv[buf][l32 * V_ROW + hi];
-        const float4* sp = reinterpret_cast<const float4*>(&sks[buf][4 * hi]);
-        // Each MFMA's operand is read four MFMAs (128 cycles) before it; left alone, the compiler puts every read right before its
-        // use. Only vector and scalar arithmetic moves past a step's end.
-        constexpr int AHEAD = 4, ARITH = 0x2 | 0x4 | 0x400;
-        float4 kv[8];
-        h8_t f[AHEAD];
-        f16_t s[2];
+    bool there = all_there(t0);   // of the step at hand
+    bool begun = false;           // the first step sets the references
+    // Any half: keys that a row does not see hidden, the reference moved where it must be
+    auto slow = [&](int b, int s, int half, f16_t& now, f16_t& next) __attribute__((always_inline)) {
+      const int h = 2 * s + half;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) kv[i] = sp[2 * i];
+      for (int i = 0; i < 2 * DT; ++i) o[i % DT] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v_at(b, half, i), p[i / DT], o[i % DT], 0, 0, 0);
+      next = zero;
 #pragma unroll
-        for (int i = 0; i < AHEAD; ++i) f[i] = __builtin_bit_cast(h8_t, kp[2 * i]);
-        __builtin_amdgcn_sched_barrier(ARITH);
+      for (int ks = 0; ks < KS; ++ks) next = __builtin_amdgcn_mfma_f32_32x32x16_f16(k_at(b, half, ks), q[ks], next, 0, 0, 0);
+      const int key0 = 32 * h + 4 * hi, m = lim - key0;
+      uint32_t gone = 0;
+      if (!there)
+        gone = static_cast<uint32_t>(__builtin_amdgcn_ballot_w64(page_in(table[min((32 * h + l32) >> a.c.log2page, a.s.width - 1)]) < 0) >> (4 * hi));
+      float y[16], top = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < 2 * KS; ++i) {
-          const int h = i / KS, ks = i % KS, n = i + AHEAD;
-          s[h] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[i % AHEAD], q[ks], ks ? s[h] : zero, 0, 0, 0);
-          if (n < 2 * KS) f[i % AHEAD] = __builtin_bit_cast(h8_t, kp[32 * (n / KS) * K_ROW<D> + 2 * (n % KS)]);
-          else kv[4 + n - 2 * KS] = sp[8 + 2 * (n - 2 * KS)];
-          __builtin_amdgcn_sched_barrier(ARITH);
-        }
-#pragma unroll
-        for (int i = 0; i < AHEAD; ++i) f[i] = __builtin_bit_cast(h8_t, vp[32 * (i % DT) * V_ROW + 2 * (i / DT)]);
-        float y[32], top = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          y[4 * i] = fmaf(s[i / 4][4 * (i % 4)], kv[i].x, -ref);
-          y[4 * i + 1] = fmaf(s[i / 4][4 * (i % 4) + 1], kv[i].y, -ref);
-          y[4 * i + 2] = fmaf(s[i / 4][4 * (i % 4) + 2], kv[i].z, -ref);
-          y[4 * i + 3] = fmaf(s[i / 4][4 * (i % 4) + 3], kv[i].w, -ref);
-          top = max3(max3(top, y[4 * i], y[4 * i + 1]), y[4 * i + 2], y[4 * i + 3]);
-        }
-        if (__builtin_amdgcn_ballot_w64(top > REF_STALE)) {   // a reference has to move: the slow way
-          loaded = true;
-          break;
-        }
-        h8_t p;
-#pragma unroll
-        for (int i = 0; i < 4 * DT; ++i) {
-          const int c = i / DT, d = i % DT, n = i + AHEAD;
-          if (d == 0) p = probabilities(y + 8 * c);
-          o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[i % AHEAD], p, o[d], 0, 0, 0);
-          if (n < 4 * DT) f[i % AHEAD] = __builtin_bit_cast(h8_t, vp[32 * (n % DT) * V_ROW + 2 * (n / DT)]);
-          __builtin_amdgcn_sched_barrier(ARITH);
-        }
-        store(stage, t + 1, (t - t0 + 1) & 1);
-        __syncthreads();
-        ++t;
+      for (int i = 0; i < 16; ++i) {
+        const int key = 8 * (i >> 2) + (i & 3);
+        y[i] = now[i] * sks[h & 7][4 * hi + key];
+        y[i] = (key >= m) | ((gone >> key) & 1) ? -INFINITY : y[i];
+        top = fmax_nc(top, y[i]);
       }
-      if (!loaded) ahead();
-      if (t * KT < top_key) {
-        if (nvref != vref) {
-          const float f = vref > 0 ? __int_as_float(vref) * pow2_inverse(nvref) : 0.0f;
+      top = across_max<false>(top);
+      const float to = top > ref + REF_STALE ? top - REF_UNDER : ref;
+      const float f = __builtin_amdgcn_exp2f(ref - to);
+      ref = to;
+      sum *= f;
 #pragma unroll
-          for (int d = 0; d < DT; ++d) o[d] *= f;
-          vref = nvref;
-        }
-        slow((t - t0) & 1, lim - t * KT, absent ? __builtin_amdgcn_ballot_w64(page_in(lookup(t)) < 0) : 0ull);
-      }
-      if (t + 1 < t1) store(stage, t + 1, (t - t0 + 1) & 1);
+      for (int d = 0; d < DT; ++d) o[d] *= f;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) y[i] -= to;
+      p[0] = probabilities(y);
+      p[1] = probabilities(y + 8);
+    };
+
+    if (t0 < t1) {
+      // stage t0 - 1 is only K of window t0
+      kpage = page_in(lookup(t0));
+      load_k(t0);
+      entry = lookup(t0 + 1);
+#pragma unroll
+      for (int i = 0; i < 2 * NP; ++i) put_k(t0 - 1, i);
+      load_next(t0 - 1);
       __syncthreads();
-      ++t;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) sa = __builtin_amdgcn_mfma_f32_32x32x16_f16(k_at((t0 - 1) & 1, 1, ks), q[ks], sa, 0, 0, 0);
+      stage(t0);
     }
+    __syncthreads();
+    int s = t0;
+    while (s < t1) {
+      bool staged = false, odd = false;
+      // Steps whose every key every row sees. The accumulators stay in place in a loop of their own; a step's instructions stay
+      // in the order written: behind each MFMA an operand's read for the one after next but two, and vector work that it covers.
+      while (begun && there && s * KT + KT <= low) {
+        const int b = s & 1;
+        h8_t f[AHEAD], n[2];
+        float4 kv[4];
+        float y[16], top;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) kv[i] = *reinterpret_cast<const float4*>(&sks[(2 * s) & 7][8 * i + 4 * hi]);
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) f[i] = k_at(b, 0, i);
+        __builtin_amdgcn_sched_barrier(0);
+        // the products of half 2 s + 1, the scores of half 2 s
+        top = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < KS; ++i) {
+          sb = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[i % AHEAD], q[i], i ? sb : zero, 0, 0, 0);
+          f[i % AHEAD] = i + AHEAD < KS ? k_at(b, 0, i + AHEAD) : v_at(b, 0, i + AHEAD - KS);
+          score(sa, kv, i, y, top);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        if (__builtin_amdgcn_ballot_w64(top > REF_STALE)) break;   // a reference has to move
+        // the values of half 2 s - 1, the probabilities of half 2 s
+#pragma unroll
+        for (int i = 0; i < 2 * DT; ++i) {
+          o[i % DT] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[i % AHEAD], p[i / DT], o[i % DT], 0, 0, 0);
+          f[i % AHEAD] = i + AHEAD < 2 * DT ? v_at(b, 0, i + AHEAD) : k_at(b, 1, i + AHEAD - 2 * DT);
+          probability(y, i, n);
+          if (i == 0) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) kv[j] = *reinterpret_cast<const float4*>(&sks[(2 * s + 1) & 7][8 * j + 4 * hi]);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        p[0] = n[0];
+        p[1] = n[1];
+        odd = true;
+        // the products of half 2 s + 2, the scores of half 2 s + 1, the next stage
+        top = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < KS; ++i) {
+          sa = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[i % AHEAD], q[i], i ? sa : zero, 0, 0, 0);
+          f[i % AHEAD] = i + AHEAD < KS ? k_at(b, 1, i + AHEAD) : v_at(b, 1, i + AHEAD - KS);
+          score(sb, kv, i, y, top);
+          if constexpr (D == 128) {   // (dim 64 has half as many MFMAs to a step: two parts to each)
+            if (i < 2 * NP) put_k(s + 1, i);
+            else if (i < 4 * NP) put_v(s + 1, i - 2 * NP);
+          } else {
+            if (2 * i < 2 * NP) { put_k(s + 1, 2 * i); put_k(s + 1, 2 * i + 1); }
+            else if (2 * i < 4 * NP) { put_v(s + 1, 2 * i - 2 * NP); put_v(s + 1, 2 * i + 1 - 2 * NP); }
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        load_next(s + 1);
+        staged = true;
+        if (__builtin_amdgcn_ballot_w64(top > REF_STALE)) break;
+        // the values of half 2 s, the probabilities of half 2 s + 1
+#pragma unroll
+        for (int i = 0; i < 2 * DT; ++i) {
+          o[i % DT] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[i % AHEAD], p[i / DT], o[i % DT], 0, 0, 0);
+          if (i + AHEAD < 2 * DT) f[i % AHEAD] = v_at(b, 1, i + AHEAD);
+          probability(y, i, n);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        p[0] = n[0];
+        p[1] = n[1];
+        __syncthreads();
+        staged = odd = false;
+        there = all_there(++s);
+        if (s >= t1) break;
+      }
+      if (s >= t1) break;
+      const int b = s & 1;
+      if ((s - 1) * KT < top_key) {   // (a step past the last key that a row sees sums its last values)
+        if (!odd) slow(b, s, 0, sa, sb);
+        slow(b, s, 1, sb, sa);
+      }
+      if (!staged) stage(s + 1);
+      begun = true;
+      __syncthreads();
+      there = all_there(++s);
+    }
+    if (t0 < t1) {   // the last half's values
+#pragma unroll
+      for (int i = 0; i < 2 * DT; ++i) o[i % DT] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v_at(t1 & 1, 0, i), p[i / DT], o[i % DT], 0, 0, 0);
+    }
+    __syncthreads();   // the next item's tiles go where these are read
 
     // lane: query row l % 32, channels 32 d + 8 i + 4 (l / 32) + 0 .. 3
     const float total = across_sum<false>(sum);
     if (has) {
       if (whole && !a.keep) {
         const int tok = row / a.group, hd = kvh * a.group + row - tok * a.group;
-        const float inv = total == 0.0f ? 0.0f : __int_as_float(max(vref, 0)) / total;
+        const float inv = total == 0.0f ? 0.0f : __int_as_float(vref) / total;
         uint16_t* dst = static_cast<uint16_t*>(a.out) + (sq.first + tok) * a.o_st + hd * a.o_sh + 4 * hi;
 #pragma unroll
         for (int d = 0; d < DT; ++d)
@@ -376,7 +440,7 @@ __global__ void __launch_bounds__(WAVES * 64, 2) chunk_kernel(AttnArgs a) {
         // slots: two to a workgroup (the item that it goes on with, the one that it begins), then one to an item that it completes
         const int64_t slot = whole ? 2 * static_cast<int64_t>(a.wgs) + sw.items_before + item : 2 * static_cast<int64_t>(wg) + (t0 == 0);
         const int rl = wave * 32 + l32;
-        const float vf = __int_as_float(max(vref, 0));
+        const float vf = __int_as_float(vref);
         float* po = a.part_o + (slot * R + rl) * D + 4 * hi;
 #pragma unroll
         for (int d = 0; d < DT; ++d)
