@@ -5,8 +5,6 @@ namespace rh3 {
 namespace kv {
 namespace {
 
-constexpr int NT = 256;
-
 // One of up to two sources of a row's parts (a shared prefix, and the sequence's own keys)
 struct Source {
   AttnArgs a;
@@ -43,79 +41,129 @@ __device__ __forceinline__ Parts parts_of(const Source& s, int b, const Seq& q, 
   return p;
 }
 
-// A query row of one head on WPR waves, each of which takes every WPR-th part: the parts' largest reference, then their sums
-// scaled to it. Bound by latency (a few KB a row).
+// Sums of a row's parts on WPR waves, each of which takes every WPR-th part: lane l has channels EPL l .. of them
+template <int D>
+struct Sums {
+  static constexpr int EPL = D / 64;
+  float o[EPL], sum;
+  __device__ __forceinline__ void add(const AttnArgs& a, int64_t at, float top) {
+    const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + 2 * at);
+    const float f = ml.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml.x - top);
+    sum += f * ml.y;
+    const float* po = a.part_o + at * D + EPL * (threadIdx.x & 63);
+#pragma unroll
+    for (int e = 0; e < EPL; ++e) o[e] += f * po[e];
+  }
+  __device__ __forceinline__ void store(const AttnArgs& a, int tok, int hd, float top) const {
+    const int lane = threadIdx.x & 63;
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    uint16_t* dst = static_cast<uint16_t*>(a.out) + tok * a.o_st + hd * a.o_sh + EPL * lane;
+    if constexpr (EPL == 2) *reinterpret_cast<uint32_t*>(dst) = pack_out(a, o[0] * inv, o[1] * inv);
+    else *dst = static_cast<uint16_t>(pack_out(a, o[0] * inv, 0.0f));
+    if (a.lse && lane == 0)
+      a.lse[static_cast<int64_t>(tok) * a.c.heads * a.group + hd] = sum == 0.0f ? -INFINITY : (__builtin_amdgcn_logf(sum) + top) * 0.6931471805599453f;
+  }
+};
+
+// Every query row of the call, WPR waves to one: where a row has many parts (few items on all workgroups), or parts of two
+// sources. Bound by latency: a row's parts are a few KB to some hundred.
 template <int D, int WPR>
-__global__ void __launch_bounds__(NT) join_kernel(Source own, Source prefix, int has_prefix) {
-  constexpr int EPL = D / 64;
-  __shared__ float so[NT / 64][D];
-  __shared__ float sl[NT / 64];
+__global__ void __launch_bounds__(WPR > 4 ? WPR * 64 : 256) join_rows_kernel(Source own, Source prefix, int has_prefix) {
+  constexpr int WAVES = WPR > 4 ? WPR : 4, EPL = D / 64;
+  __shared__ float so[WAVES][D];
+  __shared__ float sl[WAVES];
   const int lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wave = scalar(static_cast<int>(threadIdx.x >> 6));
   const int heads = own.a.c.heads * own.a.group;
-  const int64_t id = static_cast<int64_t>(blockIdx.x) * (NT / 64 / WPR) + wave / WPR;
-  const int tok = static_cast<int>(id / heads), hd = static_cast<int>(id - static_cast<int64_t>(tok) * heads);
-  if (tok >= own.a.s.rows) return;             // WPR = 4: the whole workgroup, before its barrier
-  const int kvh = hd / own.a.group, ig = hd - kvh * own.a.group;
+  const int64_t id = static_cast<int64_t>(blockIdx.x) * (WAVES / WPR) + wave / WPR;
+  const int tok = scalar(static_cast<int>(quotient(id, heads))), hd = static_cast<int>(id - static_cast<int64_t>(tok) * heads);
+  if (tok >= own.a.s.rows) return;             // WPR > 1: the whole workgroup, before its barrier
+  const int kvh = scalar(hd / own.a.group), ig = hd - kvh * own.a.group;
   Seq q;
-  const int b = __builtin_amdgcn_readfirstlane(seq_of_row<64>(own.a.s, tok, q));
+  const int b = scalar(seq_of_row<64>(own.a.s, tok, q));
   if (b < 0) return;                           // a row that no sequence has stays as it is
   Parts p[2];
   p[0] = parts_of(own, b, q, tok, kvh, ig);
   p[1].count = 0;
-  if (has_prefix) {
-    const Seq all = seq_at(prefix.a.s, 0);
-    p[1] = parts_of(prefix, 0, all, tok, kvh, ig);
-  }
+  if (has_prefix) p[1] = parts_of(prefix, 0, seq_at(prefix.a.s, 0), tok, kvh, ig);
   if (p[0].count + p[1].count == 0) return;    // one workgroup completed it
   float top = -INFINITY;
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
-    const AttnArgs& a = k ? prefix.a : own.a;
-    const int R = k ? prefix.rows : own.rows;
-    for (int i = lane; i < p[k].count; i += 64) top = fmaxf(top, a.part_ml[(p[k].slot(i) * R + p[k].row) * 2]);
+    const Source& s = k ? prefix : own;
+    for (int i = lane; i < p[k].count; i += 64) top = fmaxf(top, s.a.part_ml[(p[k].slot(i) * s.rows + p[k].row) * 2]);
   }
   top = wave_max(top);
-  float o[EPL] = {}, sum = 0.0f;
+  Sums<D> r{};
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
-    const AttnArgs& a = k ? prefix.a : own.a;
-    const int R = k ? prefix.rows : own.rows;
+    const Source& s = k ? prefix : own;
 #pragma unroll 4
-    for (int i = wave % WPR; i < p[k].count; i += WPR) {
-      const int64_t at = p[k].slot(i) * R + p[k].row;
-      const float ref = a.part_ml[at * 2], l = a.part_ml[at * 2 + 1];
-      const float f = ref == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ref - top);
-      sum += f * l;
-      const float* po = a.part_o + at * D + EPL * lane;
-      if constexpr (EPL == 2) {
-        const float2 v = *reinterpret_cast<const float2*>(po);
-        o[0] += f * v.x;
-        o[1] += f * v.y;
-      } else {
-        o[0] += f * po[0];
-      }
-    }
+    for (int i = wave % WPR; i < p[k].count; i += WPR) r.add(s.a, p[k].slot(i) * s.rows + p[k].row, top);
   }
   if constexpr (WPR > 1) {
 #pragma unroll
-    for (int e = 0; e < EPL; ++e) so[wave][EPL * lane + e] = o[e];
-    if (lane == 0) sl[wave] = sum;
+    for (int e = 0; e < EPL; ++e) so[wave][EPL * lane + e] = r.o[e];
+    if (lane == 0) sl[wave] = r.sum;
     __syncthreads();
     if (wave) return;
 #pragma unroll
     for (int w = 1; w < WPR; ++w) {
 #pragma unroll
-      for (int e = 0; e < EPL; ++e) o[e] += so[w][EPL * lane + e];
-      sum += sl[w];
+      for (int e = 0; e < EPL; ++e) r.o[e] += so[w][EPL * lane + e];
+      r.sum += sl[w];
     }
   }
-  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-  uint16_t* dst = static_cast<uint16_t*>(own.a.out) + tok * own.a.o_st + hd * own.a.o_sh + EPL * lane;
-  if constexpr (EPL == 2) *reinterpret_cast<uint32_t*>(dst) = pack_out(own.a, o[0] * inv, o[1] * inv);
-  else *dst = static_cast<uint16_t>(pack_out(own.a, o[0] * inv, 0.0f));
-  if (own.a.lse && lane == 0)
-    own.a.lse[static_cast<int64_t>(tok) * heads + hd] = sum == 0.0f ? -INFINITY : (__builtin_amdgcn_logf(sum) + top) * 0.6931471805599453f;
+  r.store(own.a, tok, hd, top);
+}
+
+// Only the items that shares divide, at most one to a boundary of two shares: workgroup (w, y) joins rows 16 y .. of the item that
+// begins in share w and goes on behind it, if there is one.
+template <int D>
+__global__ void __launch_bounds__(256) join_shares_kernel(Source own) {
+  const AttnArgs& a = own.a;
+  const Tiling g = tiling(own.chunk, own.rows);
+  Block blk;
+  const Work work = dealt(load_blocks(a, g, blk), a.wgs, g);
+  const int w = blockIdx.x;
+  if (w + 1 >= work.wgs) return;
+  const int64_t end = scalar(share_begin(work, w + 1));
+  while (end > blk.end()) {
+    if (blk.at + 64 >= a.s.batch) return;
+    next_block(a, g, blk);
+  }
+  const int l = __builtin_ctzll(__builtin_amdgcn_ballot_w64(blk.base + blk.units >= end));   // the share's last unit is its
+  const SeqItems sw = seq_in(a, blk, l);
+  const int item = scalar(static_cast<int>(quotient(end - 1 - sw.before, sw.key_tiles)));
+  const int64_t last = sw.before + (static_cast<int64_t>(item) + 1) * sw.key_tiles;          // end of the item
+  if (last == end || last - sw.key_tiles < share_begin(work, w)) return;
+  const int parts = scalar(share_of(work, last - 1)) - w + 1;
+  const int kvh = scalar(item / sw.row_tiles), at = item - kvh * sw.row_tiles;
+  const int rt = own.chunk && a.causal ? tile_at_place(at, sw.row_tiles) : at;
+  const int wave = scalar(static_cast<int>(threadIdx.x >> 6)), lane = threadIdx.x & 63;
+  const int rows = sw.seq.n * a.group;
+  // a wave's 4 rows side by side: their loads do not wait for each other
+  const int row0 = 16 * blockIdx.y + 4 * wave;
+  if (rt * own.rows + row0 >= rows) return;
+  auto slot = [&](int j) { return (2 * static_cast<int64_t>(w + j) + (j == 0)) * own.rows + row0; };
+  float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+  for (int j = lane; j < parts; j += 64)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) top[i] = fmaxf(top[i], a.part_ml[2 * (slot(j) + i)]);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) top[i] = wave_max(top[i]);
+  Sums<D> r[4] = {};
+#pragma unroll 2
+  for (int j = 0; j < parts; ++j)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i].add(a, slot(j) + i, top[i]);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int rw = rt * own.rows + row0 + i;
+    if (rw >= rows) return;
+    const int tok = scalar(rw / a.group);
+    r[i].store(a, sw.seq.first + tok, kvh * a.group + rw - tok * a.group, top[i]);
+  }
 }
 
 // ---------------------------------------------------------------- host: how a call runs
@@ -240,15 +288,24 @@ extern "C" int rh3_kv_attention(const rh3_kv_cache* cache, const void* q, int64_
   }
   launch(own.a, call.own, fmt, dim, stream);
   if (const int e = launch_status("kv_attention")) return e;
-  // few rows with up to hundreds of parts each: a workgroup to a row; many rows with few parts: a wave
-  const int64_t ids = rows * q_heads;
-  const bool wide = !call.own.chunk && !(prefix_len > 0 && call.prefix.chunk);
-  const int64_t grid = wide ? ids : (ids + 3) / 4;
-  RH3_REQUIRE(grid <= MAX_GRID_256, "kv_attention: %lld rows in one call", static_cast<long long>(rows));
+  // Parts that a row may have: the workgroups over the least count of items, no more than the keys make. Measured (kernel us, by
+  // shares / rows on 4 waves / on 16): 8 parts of 32 rows 4.2 / 4.7 / 5.7, 16 of 224 rows - / 6.2 / 7.7.
+  const int64_t ids = rows * q_heads, cap = width * cache->page + prefix_len;
+  const int64_t shared = call.own.wgs / (batch * a.c.heads), parts = shared < cap / 128 ? shared : cap / 128;
+  const int has = prefix_len > 0;
+  if (!has && (call.own.chunk || parts <= 8)) {
+    const dim3 grid(static_cast<uint32_t>(call.own.wgs), static_cast<uint32_t>(call.own.rows / 16));
+    if (dim == 128) hipLaunchKernelGGL((join_shares_kernel<128>), grid, dim3(256), 0, stream, own);
+    else hipLaunchKernelGGL((join_shares_kernel<64>), grid, dim3(256), 0, stream, own);
+    return launch_status("kv_attention (join)");
+  }
+  const int wpr = !call.own.chunk && parts > 32 ? 16 : !call.own.chunk && !call.prefix.chunk ? 4 : 1;
+  const int64_t grid = wpr == 1 ? (ids + 3) / 4 : ids;
+  RH3_REQUIRE(grid * (wpr == 16 ? 4 : 1) <= MAX_GRID_256, "kv_attention: %lld rows in one call", static_cast<long long>(rows));
   auto go = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(grid)), dim3(NT), 0, stream, own, pre, static_cast<int>(prefix_len > 0));
+    hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(grid)), dim3(wpr == 16 ? 1024 : 256), 0, stream, own, pre, has);
   };
-  if (dim == 128) wide ? go(join_kernel<128, 4>) : go(join_kernel<128, 1>);
-  else wide ? go(join_kernel<64, 4>) : go(join_kernel<64, 1>);
+  if (dim == 128) wpr == 16 ? go(join_rows_kernel<128, 16>) : wpr == 4 ? go(join_rows_kernel<128, 4>) : go(join_rows_kernel<128, 1>);
+  else wpr == 16 ? go(join_rows_kernel<64, 16>) : wpr == 4 ? go(join_rows_kernel<64, 4>) : go(join_rows_kernel<64, 1>);
   return launch_status("kv_attention (join)");
 }
