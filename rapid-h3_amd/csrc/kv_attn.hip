@@ -5,7 +5,7 @@ namespace rh3 {
 namespace kv {
 namespace {
 
-// One of up to two sources of a row's parts (a shared prefix, and the sequence's own keys)
+// A launch that has left parts
 struct Source {
   AttnArgs a;
   int chunk, rows;    // kernel, rows of its tiles
@@ -13,30 +13,24 @@ struct Source {
 
 // the parts of one query row: slot(i), i < count, and the row in each slot
 struct Parts {
-  int64_t first, next, step;
+  int64_t first, next;
   int count, row;
-  __device__ __forceinline__ int64_t slot(int i) const { return i == 0 ? first : next + (i - 1) * step; }
+  __device__ __forceinline__ int64_t slot(int i) const { return i == 0 ? first : next + 2 * (i - 1); }
 };
-__device__ __forceinline__ Parts parts_of(const Source& s, int b, const Seq& q, int tok, int kvh, int in_group) {
+// of row r of a K/V head of the launch's sequence b
+__device__ __forceinline__ Parts parts_of(const Source& s, const Work& w, const SeqItems& sw, const Tiling& g, bool causal, int64_t r, int kvh) {
   Parts p;
-  const int64_t r = static_cast<int64_t>(tok - q.first) * s.a.group + in_group;
-  const int rt = static_cast<int>(r / s.rows);
+  const int rt = scalar(static_cast<int>(quotient(r, s.rows)));
   p.row = static_cast<int>(r - static_cast<int64_t>(rt) * s.rows);
-  Block blk;
-  const Tiling g = tiling(s.chunk, s.rows);
-  const Work w = dealt(load_blocks(s.a, g, blk), s.a.wgs, g);
-  while (b >= blk.at + 64) next_block(s.a, g, blk);
-  const SeqItems sw = seq_in(s.a, blk, b - blk.at);
-  const int64_t item = static_cast<int64_t>(kvh) * sw.row_tiles + (s.chunk && s.a.causal ? place_of_tile(rt, sw.row_tiles) : rt);
-  const int64_t u0 = sw.before + item * sw.key_tiles;
-  const int w0 = share_of(w, u0), w1 = share_of(w, u0 + sw.key_tiles - 1);
-  p.step = 2;
+  const int64_t item = static_cast<int64_t>(kvh) * sw.row_tiles + (s.chunk && causal ? place_of_tile(rt, sw.row_tiles) : rt);
+  const int64_t u = sw.before + item * sw.span;
+  const int w0 = share_of(w, u + g.extra), w1 = share_of(w, u + sw.span - 1);
   p.next = 2 * (static_cast<int64_t>(w0) + 1);
   p.first = 2 * static_cast<int64_t>(w0) + 1;
   p.count = w1 - w0 + 1;
   if (w0 == w1) {
     p.first = 2 * static_cast<int64_t>(s.a.wgs) + sw.items_before + item;
-    p.count = s.a.keep && sw.items_before + item < s.a.items ? 1 : 0;
+    p.count = s.a.keep && sw.items_before + item < s.a.items ? 1 : 0;   // (a cu that falls can count rows more than once)
   }
   return p;
 }
@@ -65,8 +59,8 @@ struct Sums {
   }
 };
 
-// Every query row of the call, WPR waves to one: where a row has many parts (few items on all workgroups), or parts of two
-// sources. Bound by latency: a row's parts are a few KB to some hundred.
+// Every query row of the call, WPR waves to one: where a row has many parts (few items on all workgroups), or a prefix's beside its
+// own (of the same launch, or of `prefix`). Bound by latency: a row's parts are a few KB to some hundred.
 template <int D, int WPR>
 __global__ void __launch_bounds__(WPR > 4 ? WPR * 64 : 256) join_rows_kernel(Source own, Source prefix, int has_prefix) {
   constexpr int WAVES = WPR > 4 ? WPR : 4, EPL = D / 64;
@@ -83,21 +77,37 @@ __global__ void __launch_bounds__(WPR > 4 ? WPR * 64 : 256) join_rows_kernel(Sou
   const int b = scalar(seq_of_row<64>(own.a.s, tok, q));
   if (b < 0) return;                           // a row that no sequence has stays as it is
   Parts p[2];
-  p[0] = parts_of(own, b, q, tok, kvh, ig);
   p[1].count = 0;
-  if (has_prefix) p[1] = parts_of(prefix, 0, seq_at(prefix.a.s, 0), tok, kvh, ig);
+  {
+    Block blk;
+    const Tiling g = tiling(own.chunk, own.rows);
+    const Work w = dealt(load_blocks(own.a, g, blk), own.a.wgs, g);
+    const int64_t all = static_cast<int64_t>(tok) * own.a.group + ig;
+    int at = b;
+    if (own.a.prefix) {
+      p[1] = parts_of(own, w, seq_in(own.a, blk, 0), g, false, all, kvh);
+      ++at;
+    }
+    while (at >= blk.at + 64) next_block(own.a, g, blk);
+    p[0] = parts_of(own, w, seq_in(own.a, blk, at - blk.at), g, own.a.causal, all - static_cast<int64_t>(q.first) * own.a.group, kvh);
+    if (has_prefix) {
+      const Tiling gp = tiling(prefix.chunk, prefix.rows);
+      const Work wp = dealt(load_blocks(prefix.a, gp, blk), prefix.a.wgs, gp);
+      p[1] = parts_of(prefix, wp, seq_in(prefix.a, blk, 0), gp, false, all, kvh);
+    }
+  }
   if (p[0].count + p[1].count == 0) return;    // one workgroup completed it
   float top = -INFINITY;
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
-    const Source& s = k ? prefix : own;
+    const Source& s = k && has_prefix ? prefix : own;
     for (int i = lane; i < p[k].count; i += 64) top = fmaxf(top, s.a.part_ml[(p[k].slot(i) * s.rows + p[k].row) * 2]);
   }
   top = wave_max(top);
   Sums<D> r{};
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
-    const Source& s = k ? prefix : own;
+    const Source& s = k && has_prefix ? prefix : own;
 #pragma unroll 4
     for (int i = wave % WPR; i < p[k].count; i += WPR) r.add(s.a, p[k].slot(i) * s.rows + p[k].row, top);
   }
@@ -129,14 +139,15 @@ __global__ void __launch_bounds__(256) join_shares_kernel(Source own) {
   if (w + 1 >= work.wgs) return;
   const int64_t end = scalar(share_begin(work, w + 1));
   while (end > blk.end()) {
-    if (blk.at + 64 >= a.s.batch) return;
+    if (blk.at + 64 >= sequences(a)) return;
     next_block(a, g, blk);
   }
   const int l = __builtin_ctzll(__builtin_amdgcn_ballot_w64(blk.base + blk.units >= end));   // the share's last unit is its
   const SeqItems sw = seq_in(a, blk, l);
-  const int item = scalar(static_cast<int>(quotient(end - 1 - sw.before, sw.key_tiles)));
-  const int64_t last = sw.before + (static_cast<int64_t>(item) + 1) * sw.key_tiles;          // end of the item
-  if (last == end || last - sw.key_tiles < share_begin(work, w)) return;
+  const int item = scalar(static_cast<int>(quotient(end - 1 - sw.before, sw.span)));
+  const int64_t last = sw.before + (static_cast<int64_t>(item) + 1) * sw.span;               // end of the item
+  const int64_t begin = last - sw.span + g.extra;                                            // its first key's unit
+  if (last == end || begin >= end || begin < share_begin(work, w)) return;
   const int parts = scalar(share_of(work, last - 1)) - w + 1;
   const int kvh = scalar(item / sw.row_tiles), at = item - kvh * sw.row_tiles;
   const int rt = own.chunk && a.causal ? tile_at_place(at, sw.row_tiles) : at;
@@ -190,17 +201,25 @@ int64_t bytes_of(const Plan& p, int64_t dim) { return p.slots * p.rows * (dim + 
 
 struct Call {
   Plan own, prefix;
+  bool joined;            // the prefix is a sequence of the one launch
   int64_t bytes;
 };
 Call call_of(int64_t rows, int64_t q_heads, int64_t heads, int64_t dim, int64_t batch, bool even, int64_t prefix_len) {
   Call c{};
   const int64_t group = q_heads / heads;
   c.own = plan_of(rows, batch, even, group, heads, prefix_len > 0);
-  c.bytes = bytes_of(c.own, dim);
   if (prefix_len > 0) {
     c.prefix = plan_of(rows, 1, true, group, heads, true);
-    c.bytes += bytes_of(c.prefix, dim);
+    c.joined = c.own.chunk == c.prefix.chunk;   // the prefix's rows then go by the sequences' tiles
+    if (c.joined) {
+      const int64_t items = heads * ((rows * group + c.own.rows - 1) / c.own.rows);
+      c.own.items += items;
+      c.own.slots += items;
+    } else {
+      c.bytes += bytes_of(c.prefix, dim);
+    }
   }
+  c.bytes += bytes_of(c.own, dim);
   return c;
 }
 
@@ -268,15 +287,21 @@ extern "C" int rh3_kv_attention(const rh3_kv_cache* cache, const void* q, int64_
     ws += p.slots * p.rows * (dim + 2);
     return Source{x, p.chunk, p.rows};
   };
+  const int prefix_width = static_cast<int>((prefix_len + cache->page - 1) / cache->page);
+  if (call.joined) {
+    a.prefix = prefix;
+    a.prefix_len = static_cast<int>(prefix_len);
+    a.prefix_width = prefix_width;
+  }
   const Source own = source(a, call.own);
   Source pre{};
-  if (prefix_len > 0) {
+  if (prefix_len > 0 && !call.joined) {
     AttnArgs x = a;
     x.s.table = prefix;
     x.s.table_stride = 0;
     x.s.lens = nullptr;
     x.s.cu = nullptr;
-    x.s.width = static_cast<int>((prefix_len + cache->page - 1) / cache->page);
+    x.s.width = prefix_width;
     x.s.batch = 1;
     x.s.per = x.s.rows;
     x.s.fixed_len = static_cast<int>(prefix_len);
@@ -292,14 +317,14 @@ extern "C" int rh3_kv_attention(const rh3_kv_cache* cache, const void* q, int64_
   // shares / rows on 4 waves / on 16): 8 parts of 32 rows 4.2 / 4.7 / 5.7, 16 of 224 rows - / 6.2 / 7.7.
   const int64_t ids = rows * q_heads, cap = width * cache->page + prefix_len;
   const int64_t shared = call.own.wgs / (batch * a.c.heads), parts = shared < cap / 128 ? shared : cap / 128;
-  const int has = prefix_len > 0;
-  if (!has && (call.own.chunk || parts <= 8)) {
+  const int has = prefix_len > 0 && !call.joined;
+  if (prefix_len == 0 && (call.own.chunk || parts <= 8)) {
     const dim3 grid(static_cast<uint32_t>(call.own.wgs), static_cast<uint32_t>(call.own.rows / 16));
     if (dim == 128) hipLaunchKernelGGL((join_shares_kernel<128>), grid, dim3(256), 0, stream, own);
     else hipLaunchKernelGGL((join_shares_kernel<64>), grid, dim3(256), 0, stream, own);
     return launch_status("kv_attention (join)");
   }
-  const int wpr = !call.own.chunk && parts > 32 ? 16 : !call.own.chunk && !call.prefix.chunk ? 4 : 1;
+  const int wpr = !call.own.chunk && parts > 32 ? 16 : !call.own.chunk && !has ? 4 : 1;
   const int64_t grid = wpr == 1 ? (ids + 3) / 4 : ids;
   RH3_REQUIRE(grid * (wpr == 16 ? 4 : 1) <= MAX_GRID_256, "kv_attention: %lld rows in one call", static_cast<long long>(rows));
   auto go = [&](auto kernel) {

@@ -32,6 +32,10 @@ struct AttnArgs {
   float* lse;                // [rows][q heads] or null
   float* part_o;
   float* part_ml;
+  // A prefix that all rows see, taken as the first sequence (all rows its own, no causal limit) by the launch that also does the
+  // others; or null
+  const int32_t* prefix;
+  int prefix_len, prefix_width;
   int64_t items;             // slots of completed items
   int wgs;
   int keep;                  // leave a part for every item, also for those that one workgroup completes
@@ -41,11 +45,13 @@ struct AttnArgs {
 // Items: (sequence, K/V head, R query rows of it). Units: KEYS keys of an item. The units of all items in order (sequences, then
 // K/V heads, then row tiles) are dealt to the workgroups in equal contiguous ranges, so that uneven histories, which only the
 // device knows, load the workgroups evenly. `least` units at least make a workgroup worth starting.
+// An item counts `extra` units before its keys, about what beginning one takes: without them a workgroup with several short items
+// would have as many keys as one with a long one, and take longer.
 struct Tiling {
-  int rows, keys, least;
+  int rows, keys, extra, least;
 };
 constexpr int TOKEN_KEYS = 32, CHUNK_KEYS = 64;
-RH3_HD Tiling tiling(bool chunk, int rows) { return chunk ? Tiling{rows, CHUNK_KEYS, 8} : Tiling{rows, TOKEN_KEYS, 4}; }
+RH3_HD Tiling tiling(bool chunk, int rows) { return chunk ? Tiling{rows, CHUNK_KEYS, 4, 8} : Tiling{rows, TOKEN_KEYS, 4, 4}; }
 
 // Units are counted in 64 bits; a division of what fits 32 bits is done there (a 64-bit one takes some hundred instructions).
 RH3_HD int64_t quotient(int64_t a, int64_t b) {
@@ -70,18 +76,28 @@ RH3_HD int share_of(const Work& w, int64_t u) {
   return static_cast<int>(u < head ? quotient(u, w.each + 1) : w.more + quotient(u - head, w.each));
 }
 
+// a sequence of the launch: the prefix, if there is one, before the batch's
+RH3_HD int sequences(const AttnArgs& a) { return a.s.batch + (a.prefix != nullptr); }
+RH3_HD Seq sequence(const AttnArgs& a, int i) {
+  if (a.prefix) {
+    if (i == 0) return Seq{0, a.s.rows, a.prefix_len};
+    --i;
+  }
+  return seq_at(a.s, i);
+}
+
 struct SeqWork {
-  int row_tiles, key_tiles;
+  int row_tiles, span;       // span: units of an item
   int64_t units;
 };
 RH3_HD SeqWork work_of(const AttnArgs& a, const Seq& q, const Tiling& g) {
   SeqWork w;
   w.row_tiles = static_cast<int>((static_cast<int64_t>(q.n) * a.group + g.rows - 1) / g.rows);
   const int kt = (q.len + g.keys - 1) / g.keys;
-  w.key_tiles = kt < 1 ? 1 : kt;
+  w.span = (kt < 1 ? 1 : kt) + g.extra;
   // no memory holds 2^36 units (2^41 keys); offsets in cu that fall can count rows many times, and must not overflow the sums
   const int64_t u = static_cast<int64_t>(a.c.heads) * w.row_tiles;
-  w.units = u < (int64_t{1} << 36) / w.key_tiles ? u * w.key_tiles : int64_t{1} << 36;
+  w.units = u < (int64_t{1} << 36) / w.span ? u * w.span : int64_t{1} << 36;
   return w;
 }
 
@@ -112,7 +128,7 @@ struct Block {
   int64_t base, items_base;        // units and items before it
   Seq seq;
   int64_t units, items;            // running sums within the block, this lane's included
-  int row_tiles, key_tiles;
+  int row_tiles, span;
   __device__ __forceinline__ int64_t end() const { return base + lane64(units, 63); }
 };
 __device__ __forceinline__ void load_block(const AttnArgs& a, const Tiling& g, int at, int64_t base, int64_t items_base, Block& b) {
@@ -122,12 +138,12 @@ __device__ __forceinline__ void load_block(const AttnArgs& a, const Tiling& g, i
   b.items_base = items_base;
   b.seq = Seq{0, 0, 0};
   SeqWork w{0, 1, 0};
-  if (i < a.s.batch) {
-    b.seq = seq_at(a.s, i);
+  if (i < sequences(a)) {
+    b.seq = sequence(a, i);
     w = work_of(a, b.seq, g);
   }
   b.row_tiles = w.row_tiles;
-  b.key_tiles = w.key_tiles;
+  b.span = w.span;
   b.units = wave_scan(w.units);
   b.items = a.keep ? wave_scan(static_cast<int64_t>(a.c.heads) * w.row_tiles) : 0;
 }
@@ -135,7 +151,7 @@ __device__ __forceinline__ void load_block(const AttnArgs& a, const Tiling& g, i
 __device__ __forceinline__ int64_t load_blocks(const AttnArgs& a, const Tiling& g, Block& b) {
   load_block(a, g, 0, 0, 0, b);
   int64_t total = b.end();
-  for (int at = 64; at < a.s.batch; at += 64) {
+  for (int at = 64; at < sequences(a); at += 64) {
     Block next;
     load_block(a, g, at, 0, 0, next);
     total += next.end();
@@ -149,7 +165,7 @@ __device__ __forceinline__ void next_block(const AttnArgs& a, const Tiling& g, B
 // a sequence of the block by its lane, the same in all lanes
 struct SeqItems {
   Seq seq;
-  int row_tiles, key_tiles;
+  int row_tiles, span;
   int64_t before, items_before;    // units, items of the sequences before it
 };
 __device__ __forceinline__ SeqItems seq_in(const AttnArgs& a, const Block& b, int l) {
@@ -158,7 +174,7 @@ __device__ __forceinline__ SeqItems seq_in(const AttnArgs& a, const Block& b, in
   r.seq.n = __builtin_amdgcn_readlane(b.seq.n, l);
   r.seq.len = __builtin_amdgcn_readlane(b.seq.len, l);
   r.row_tiles = __builtin_amdgcn_readlane(b.row_tiles, l);
-  r.key_tiles = __builtin_amdgcn_readlane(b.key_tiles, l);
+  r.span = __builtin_amdgcn_readlane(b.span, l);
   r.before = b.base + (l ? lane64(b.units, l - 1) : 0);
   r.items_before = b.items_base + (l ? lane64(b.items, l - 1) : 0);
   return r;

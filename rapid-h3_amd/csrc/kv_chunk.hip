@@ -37,10 +37,6 @@ typedef _Float16 h4_t __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ h4_t lds_read_tr(const uint8_t* p) {
   return __builtin_bit_cast(h4_t, __builtin_amdgcn_ds_read_tr16_b64_v4f16((__attribute__((address_space(3))) g4_t*)p));
 }
-// a table entry by the scalar cache: the same address in all lanes, and nothing that a kernel writes
-__device__ __forceinline__ int scalar_load(const int32_t* p) {
-  return *(const __attribute__((address_space(4))) int32_t*)(p);
-}
 
 template <int FMT, int D, int WAVES>
 __global__ void __launch_bounds__(WAVES * 64, 2) chunk_kernel(AttnArgs a) {
@@ -71,7 +67,7 @@ __global__ void __launch_bounds__(WAVES * 64, 2) chunk_kernel(AttnArgs a) {
     Block blk;
     load_block(a, TILING, 0, 0, 0, blk);
     while (u >= blk.end()) {
-      if (blk.at + 64 >= a.s.batch) return;
+      if (blk.at + 64 >= sequences(a)) return;
       next_block(a, TILING, blk);
     }
     const int in_block = __builtin_ctzll(__builtin_amdgcn_ballot_w64(blk.base + blk.units > u));
@@ -79,22 +75,27 @@ __global__ void __launch_bounds__(WAVES * 64, 2) chunk_kernel(AttnArgs a) {
     const SeqItems sw = seq_in(a, blk, in_block);
     const Seq sq = sw.seq;
     const int64_t local = u - sw.before;
-    const int item = scalar(static_cast<int>(quotient(local, sw.key_tiles)));
-    const int t0 = static_cast<int>(local - static_cast<int64_t>(item) * sw.key_tiles);
-    const int share_t1 = static_cast<int>(end - u < sw.key_tiles - t0 ? t0 + (end - u) : sw.key_tiles);
-    const bool whole = t0 == 0 && share_t1 == sw.key_tiles;
+    const int item = scalar(static_cast<int>(quotient(local, sw.span)));
+    const int u0 = static_cast<int>(local - static_cast<int64_t>(item) * sw.span);
+    const int u1 = static_cast<int>(end - u < sw.span - u0 ? u0 + (end - u) : sw.span);
+    u += u1 - u0;
+    const int t0 = max(u0 - TILING.extra, 0), share_t1 = u1 - TILING.extra;
+    if (share_t1 <= 0) continue;
+    const bool whole = t0 == 0 && u1 == sw.span;
+    const bool pre = a.prefix && seq == 0, causal = a.causal && !pre;
+    const int32_t* table = pre ? a.prefix : a.s.table + (seq - (a.prefix != nullptr)) * a.s.table_stride;
+    const int width = pre ? a.prefix_width : a.s.width;
     const int kvh = scalar(item / sw.row_tiles), at = item - kvh * sw.row_tiles;
-    const int rt = a.causal ? tile_at_place(at, sw.row_tiles) : at;
+    const int rt = causal ? tile_at_place(at, sw.row_tiles) : at;
     const int rows = sq.n * a.group;
     const int tok_last = scalar(min(rows - 1, rt * R + R - 1) / a.group);
-    const int seen = a.causal ? min(sq.len, max(0, sq.len - sq.n + tok_last + 1)) : sq.len;   // keys that some row sees
+    const int seen = causal ? min(sq.len, max(0, sq.len - sq.n + tok_last + 1)) : sq.len;   // keys that some row sees
     const int t1 = min(share_t1, (seen + KT - 1) / KT);
 
     const int row = rt * R + wave * 32 + l32;
     const bool has = row < rows;
     const int rr = has ? row : rows - 1;
     const int tok = rr / a.group, hd = kvh * a.group + rr - tok * a.group;
-    const int32_t* table = a.s.table + seq * a.s.table_stride;
     const int mask = (1 << a.c.log2page) - 1;
     auto page_in = [&](int entry) { return entry >= 0 && entry < a.c.pages ? entry : -1; };
     h8_t q[KS];
@@ -115,7 +116,7 @@ __global__ void __launch_bounds__(WAVES * 64, 2) chunk_kernel(AttnArgs a) {
       float big = 0.0f;
 #pragma unroll 4
       for (int key = t0 * KT + 4 * static_cast<int>(threadIdx.x); key < min(t1 * KT, sq.len); key += 4 * WAVES * 64) {
-        const int page = page_in(table[min(key >> a.c.log2page, a.s.width - 1)]);
+        const int page = page_in(table[min(key >> a.c.log2page, width - 1)]);
         const float4 v = *reinterpret_cast<const float4*>(a.c.vs + max(page, 0) * a.c.spage_stride + kvh * a.c.shead_stride + (key & mask));
         const float x[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
@@ -143,11 +144,11 @@ __global__ void __launch_bounds__(WAVES * 64, 2) chunk_kernel(AttnArgs a) {
       }
       qf = __builtin_amdgcn_ldexpf(a.scale_log2, -e);
     }
-    const int lim = a.causal ? min(sq.len, sq.len - sq.n + tok + 1) : sq.len;
+    const int lim = causal ? min(sq.len, sq.len - sq.n + tok + 1) : sq.len;
     // of the wave's rows: keys that all see, keys that some see
     const int r0 = rt * R + wave * 32, r1 = min(rows - 1, r0 + 31);
-    const int low = a.causal ? min(sq.len, sq.len - sq.n + scalar(r0 / a.group) + 1) : sq.len;
-    const int top_key = r0 >= rows ? 0 : a.causal ? min(sq.len, sq.len - sq.n + scalar(r1 / a.group) + 1) : sq.len;
+    const int low = causal ? min(sq.len, sq.len - sq.n + scalar(r0 / a.group) + 1) : sq.len;
+    const int top_key = r0 >= rows ? 0 : causal ? min(sq.len, sq.len - sq.n + scalar(r1 / a.group) + 1) : sq.len;
 
     f16_t o[DT];
     float ref = NO_REF, sum = 0.0f;
@@ -160,13 +161,13 @@ __global__ void __launch_bounds__(WAVES * 64, 2) chunk_kernel(AttnArgs a) {
     // NP keys of a window, which lie in one page; lane l has 1 / 8 of key l / 8 of each 8.
     const int first = 8 * NP * wave;
     auto lookup = [&](int w) {   // the entry of the wave's page; the first window begins before the sequence
-      return scalar_load(table + min(max(w * KT - 32 + first, 0) >> a.c.log2page, a.s.width - 1));
+      return scalar_load(table + min(max(w * KT - 32 + first, 0) >> a.c.log2page, width - 1));
     };
     auto all_there = [&](int s) {   // no key of step s in an absent page
       int bad = 0;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int e = scalar_load(table + min((s * KT + 16 * i) >> a.c.log2page, a.s.width - 1));
+        const int e = scalar_load(table + min((s * KT + 16 * i) >> a.c.log2page, width - 1));
         bad |= e < 0 || e >= a.c.pages;
       }
       return bad == 0;
@@ -293,7 +294,7 @@ __global__ void __launch_bounds__(WAVES * 64, 2) chunk_kernel(AttnArgs a) {
       const int key0 = 32 * h + 4 * hi, m = lim - key0;
       uint32_t gone = 0;
       if (!there)
-        gone = static_cast<uint32_t>(__builtin_amdgcn_ballot_w64(page_in(table[min((32 * h + l32) >> a.c.log2page, a.s.width - 1)]) < 0) >> (4 * hi));
+        gone = static_cast<uint32_t>(__builtin_amdgcn_ballot_w64(page_in(table[min((32 * h + l32) >> a.c.log2page, width - 1)]) < 0) >> (4 * hi));
       float y[16], top = -INFINITY;
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
@@ -451,7 +452,6 @@ __global__ void __launch_bounds__(WAVES * 64, 2) chunk_kernel(AttnArgs a) {
         if (hi == 0) *reinterpret_cast<float2*>(a.part_ml + (slot * R + rl) * 2) = make_float2(total == 0.0f ? -INFINITY : ref, total);
       }
     }
-    u += share_t1 - t0;
   }
 }
 

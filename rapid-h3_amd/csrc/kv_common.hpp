@@ -92,6 +92,11 @@ RH3_HD int page_of(const Seqs& s, const Cache& c, int b, int pos) {
   return p >= 0 && p < c.pages ? p : -1;
 }
 
+// a table entry by the scalar cache: the same address in all lanes, and nothing that a kernel of this call writes
+__device__ __forceinline__ int scalar_load(const int32_t* p) {
+  return *(const __attribute__((address_space(4))) int32_t*)(p);
+}
+
 // ---------------------------------------------------------------- codes to f16, exact
 // int8: the byte c + 128 beside 0x64 is the f16 1024 + (c + 128), from which one packed subtraction takes 1152
 // (a permute, an xor and a packed add per two codes). e4m3: the hardware conversion (its scale operand 1).

@@ -29,13 +29,13 @@ struct Tile {
 struct Pages {
   int p[2];
 };
-__device__ __forceinline__ Pages pages_of(const AttnArgs& a, const int32_t* row, int tile) {
+__device__ __forceinline__ Pages pages_of(const AttnArgs& a, const int32_t* row, int width, int tile) {
   Pages r;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    const int i = min((tile * TOKEN_KEYS + 16 * h) >> a.c.log2page, a.s.width - 1);
-    const int p = row[i];
-    r.p[h] = __builtin_amdgcn_readfirstlane(p >= 0 && p < a.c.pages ? p : -1);
+    const int i = min((tile * TOKEN_KEYS + 16 * h) >> a.c.log2page, width - 1);
+    const int p = scalar_load(row + i);
+    r.p[h] = p >= 0 && p < a.c.pages ? p : -1;
   }
   return r;
 }
@@ -227,16 +227,22 @@ __global__ void __launch_bounds__(NT, 2) token_kernel(AttnArgs a) {
 
   while (u < end) {
     while (u >= blk.end()) {
-      if (blk.at + 64 >= a.s.batch) return;
+      if (blk.at + 64 >= sequences(a)) return;
       next_block(a, TILING, blk);
     }
     const int l = __builtin_ctzll(__builtin_amdgcn_ballot_w64(blk.base + blk.units > u));
     const SeqItems sw = seq_in(a, blk, l);
     const Seq sq = sw.seq;
     const int64_t local = u - sw.before;
-    const int item = scalar(static_cast<int>(quotient(local, sw.key_tiles)));
-    const int t0 = static_cast<int>(local - static_cast<int64_t>(item) * sw.key_tiles);
-    const int t1 = static_cast<int>(end - u < sw.key_tiles - t0 ? t0 + (end - u) : sw.key_tiles);
+    const int item = scalar(static_cast<int>(quotient(local, sw.span)));
+    const int u0 = static_cast<int>(local - static_cast<int64_t>(item) * sw.span);
+    const int u1 = static_cast<int>(end - u < sw.span - u0 ? u0 + (end - u) : sw.span);
+    u += u1 - u0;
+    const int t0 = max(u0 - TILING.extra, 0), t1 = u1 - TILING.extra;
+    if (t1 <= 0) continue;
+    const bool pre = a.prefix && blk.at + l == 0, causal = a.causal && !pre;
+    const int32_t* row = pre ? a.prefix : a.s.table + (blk.at + l - (a.prefix != nullptr)) * a.s.table_stride;
+    const int width = pre ? a.prefix_width : a.s.width;
     const int kvh = scalar(item / sw.row_tiles), rt = item - kvh * sw.row_tiles;
     const int rows = sq.n * a.group;
 
@@ -264,9 +270,9 @@ __global__ void __launch_bounds__(NT, 2) token_kernel(AttnArgs a) {
 #pragma unroll
       for (int c = 0; c < D / 32; ++c) q[m][c] = q_f16(x[c], e);
       qf[m] = __builtin_amdgcn_ldexpf(a.scale_log2, -e);
-      lim[m] = a.causal ? min(sq.len, sq.len - sq.n + tok + 1) : sq.len;
+      lim[m] = causal ? min(sq.len, sq.len - sq.n + tok + 1) : sq.len;
     }
-    const int low = a.causal ? min(sq.len, sq.len - sq.n + scalar((rt * R) / a.group) + 1) : sq.len;
+    const int low = causal ? min(sq.len, sq.len - sq.n + scalar((rt * R) / a.group) + 1) : sq.len;
 
     State<D, MT> st;
     st.vref = 0.0f;
@@ -278,15 +284,14 @@ __global__ void __launch_bounds__(NT, 2) token_kernel(AttnArgs a) {
 #pragma unroll
       for (int i = 0; i < D / 16; ++i) st.o[m][i] = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
     }
-    const int32_t* row = a.s.table + (blk.at + l) * a.s.table_stride;
     int t = t0 + wave;
     if (t < t1) {
       Tile<D> tile;
-      Pages pg = pages_of(a, row, t), pn = pages_of(a, row, t + WAVES);
+      Pages pg = pages_of(a, row, width, t), pn = pages_of(a, row, width, t + WAVES);
       load_keys<D>(a, kvh, t, pg, tile);
       load_values<D>(a, kvh, t, pg, tile);
       for (; t + WAVES < t1; t += WAVES) {
-        const Pages p2 = pages_of(a, row, t + 2 * WAVES);
+        const Pages p2 = pages_of(a, row, width, t + 2 * WAVES);
         compute<FMT, D, MT, true>(a, tile, kvh, t, pg, pn, q, qf, lim, low, sq.len, st);
         pg = pn;
         pn = p2;
@@ -311,7 +316,7 @@ __global__ void __launch_bounds__(NT, 2) token_kernel(AttnArgs a) {
         }
     }
     __syncthreads();
-    const bool whole = t0 == 0 && t1 == sw.key_tiles;
+    const bool whole = t0 == 0 && u1 == sw.span;
     constexpr int TPR = NT / R, EPT = D / TPR;   // threads to a row, channels to a thread
     const int rl = threadIdx.x / TPR, d0 = (threadIdx.x % TPR) * EPT;
     const int rw = rt * R + rl;
@@ -353,7 +358,6 @@ __global__ void __launch_bounds__(NT, 2) token_kernel(AttnArgs a) {
         if (d0 == 0) *reinterpret_cast<float2*>(a.part_ml + (slot * R + rl) * 2) = make_float2(top, sum);
       }
     }
-    u += t1 - t0;
     if (u < end) __syncthreads();
   }
 }
