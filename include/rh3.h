@@ -31,6 +31,9 @@ extern "C" {
 
 #define RH3_KV_INT8 0
 #define RH3_KV_E4M3 1
+#define RH3_KV_BY_SIZE 0
+#define RH3_KV_TOKEN 1
+#define RH3_KV_CHUNK 2
 
 /* Message of the last failed call on this thread ("" if none). */
 const char* rh3_last_error(void);
@@ -495,16 +498,18 @@ int rh3_kv_read(const rh3_kv_cache* cache, void* k, int64_t k_st, int64_t k_sh, 
  * lens[b] - n + i), q and out [rows][q_heads][dim] bf16 or fp16, query head h reads K/V head h / (q_heads / heads); lse
  * [rows][q_heads] fp32 or NULL: the natural log of the sum of exp(scale q.k). A row that sees no key gives 0 and -inf; one
  * that sees a NaN key or value gives NaN. prefix_len > 0: every row also sees the first prefix_len positions of the pages
- * prefix[], which come before the sequences' own and are read once for the batch. out may lie exactly over q.
+ * prefix[], which come before the sequences' own and are read once for the batch. out may lie exactly over q. form: the
+ * kernel for few query rows to a K/V head (RH3_KV_TOKEN) or for many (RH3_KV_CHUNK), or by the sizes, where the table's width
+ * stands for the lengths, which only the device knows.
  * The workspace holds the parts of rows whose keys several workgroups share; how keys are split depends on the sizes, lengths
  * and the CU count, and with it the last bits of the result; the same call gives the same bits. */
-int64_t rh3_kv_attention_workspace_bytes(const rh3_kv_cache* cache, int64_t q_heads, int64_t rows, int64_t batch,
-                                         int even, int64_t prefix_len);
+int64_t rh3_kv_attention_workspace_bytes(const rh3_kv_cache* cache, int64_t q_heads, int64_t rows, int64_t width,
+                                         int64_t batch, int even, int64_t prefix_len, int form);
 int rh3_kv_attention(const rh3_kv_cache* cache, const void* q, int64_t q_st, int64_t q_sh, int64_t q_heads, int dtype,
                      int64_t rows, const int32_t* table, int64_t table_stride, int64_t width, const int32_t* lens,
                      const int32_t* cu, int64_t batch, int causal, float scale, void* out, int64_t o_st, int64_t o_sh,
-                     float* lse, const int32_t* prefix, int64_t prefix_len, void* workspace, int64_t workspace_bytes,
-                     hipStream_t stream);
+                     float* lse, const int32_t* prefix, int64_t prefix_len, int form, void* workspace,
+                     int64_t workspace_bytes, hipStream_t stream);
 
 #ifdef __cplusplus
 }

@@ -186,12 +186,19 @@ struct Plan {
 };
 
 // rows: of a call; per sequence they are counted as even. keep: a part for every item.
-Plan plan_of(int64_t rows, int64_t batch, bool even, int64_t group, int64_t heads, bool keep) {
+// The token kernel reads the keys once for every 16 (dim 64: 32) query rows of a K/V head, at some 6.8 TB/s, mostly from L2 from
+// the second time on; the chunk kernel once for 128 or 256, as 3 TB/s at most (it is bound by its arithmetic), after some 40 us
+// that its longer beginning, end and joins take. The lengths are the device's: the table's width stands for them. Measured (us,
+// token / chunk, 8 K/V heads of 128): 28 rows of 8 sequences x 32,768 keys 164 / 222, 49 rows of them 304 / 217, 49 rows of 8 x up
+// to 2,048 24 / 51, 96 rows of 2 x 16,384 61 / 83.
+Plan plan_of(int64_t rows, int64_t batch, bool even, int64_t group, int64_t heads, int64_t dim, int64_t cap, bool keep, int form) {
   const int64_t cus = device_cus() > 0 ? device_cus() : 256;
   const int64_t mean = (rows * group + batch - 1) / batch;    // query rows of a sequence's K/V head
+  const int small = dim == 64 && mean > 16 ? 32 : 16;
+  const double mb = 2e-6 * static_cast<double>(dim + 4) * static_cast<double>(batch * heads) * static_cast<double>(cap);
   Plan p{};
-  p.chunk = mean > 32;
-  p.rows = mean <= 16 ? 16 : mean <= 32 ? 32 : mean <= 128 ? 128 : 256;
+  p.chunk = form != RH3_KV_BY_SIZE ? form == RH3_KV_CHUNK : static_cast<double>((mean + small - 1) / small) * mb / 6.8 > 40.0 + static_cast<double>((mean + 127) / 128) * mb / 3.0;
+  p.rows = !p.chunk ? small : mean <= 128 ? 128 : 256;
   p.wgs = static_cast<int>(p.rows == 256 ? cus : 2 * cus);
   p.items = !keep ? 0 : heads * (even ? batch * ((rows / batch * group + p.rows - 1) / p.rows) : rows * group / p.rows + batch);
   p.slots = 2 * static_cast<int64_t>(p.wgs) + p.items;
@@ -204,12 +211,12 @@ struct Call {
   bool joined;            // the prefix is a sequence of the one launch
   int64_t bytes;
 };
-Call call_of(int64_t rows, int64_t q_heads, int64_t heads, int64_t dim, int64_t batch, bool even, int64_t prefix_len) {
+Call call_of(int64_t rows, int64_t q_heads, int64_t heads, int64_t dim, int64_t cap, int64_t batch, bool even, int64_t prefix_len, int form) {
   Call c{};
   const int64_t group = q_heads / heads;
-  c.own = plan_of(rows, batch, even, group, heads, prefix_len > 0);
+  c.own = plan_of(rows, batch, even, group, heads, dim, cap, prefix_len > 0, form);
   if (prefix_len > 0) {
-    c.prefix = plan_of(rows, 1, true, group, heads, true);
+    c.prefix = plan_of(rows, 1, true, group, heads, dim, prefix_len, true, form);
     c.joined = c.own.chunk == c.prefix.chunk;   // the prefix's rows then go by the sequences' tiles
     if (c.joined) {
       const int64_t items = heads * ((rows * group + c.own.rows - 1) / c.own.rows);
@@ -235,17 +242,17 @@ void launch(const AttnArgs& a, const Plan& p, int fmt, int dim, hipStream_t st) 
 using namespace rh3;
 using namespace rh3::kv;
 
-extern "C" int64_t rh3_kv_attention_workspace_bytes(const rh3_kv_cache* cache, int64_t q_heads, int64_t rows, int64_t batch,
-                                                    int even, int64_t prefix_len) {
-  if (!cache || cache->heads < 1 || q_heads < cache->heads || q_heads % cache->heads || rows < 1 || batch < 1) return 0;
-  return call_of(rows, q_heads, cache->heads, cache->dim, batch, even != 0, prefix_len).bytes;
+extern "C" int64_t rh3_kv_attention_workspace_bytes(const rh3_kv_cache* cache, int64_t q_heads, int64_t rows, int64_t width,
+                                                    int64_t batch, int even, int64_t prefix_len, int form) {
+  if (!cache || cache->heads < 1 || q_heads < cache->heads || q_heads % cache->heads || rows < 1 || batch < 1 || width < 1) return 0;
+  return call_of(rows, q_heads, cache->heads, cache->dim, width * cache->page, batch, even != 0, prefix_len, form).bytes;
 }
 
 extern "C" int rh3_kv_attention(const rh3_kv_cache* cache, const void* q, int64_t q_st, int64_t q_sh, int64_t q_heads, int dtype,
                                 int64_t rows, const int32_t* table, int64_t table_stride, int64_t width, const int32_t* lens,
                                 const int32_t* cu, int64_t batch, int causal, float scale, void* out, int64_t o_st, int64_t o_sh,
-                                float* lse, const int32_t* prefix, int64_t prefix_len, void* workspace, int64_t workspace_bytes,
-                                hipStream_t stream) {
+                                float* lse, const int32_t* prefix, int64_t prefix_len, int form, void* workspace,
+                                int64_t workspace_bytes, hipStream_t stream) {
   clear_error();
   AttnArgs a{};
   if (const int e = check_cache("kv_attention", cache, a.c)) return e;
@@ -261,8 +268,9 @@ extern "C" int rh3_kv_attention(const rh3_kv_cache* cache, const void* q, int64_
               "kv_attention: q and out must be 16-byte aligned with strides that are multiples of 8");
   RH3_REQUIRE(prefix_len >= 0 && prefix_len <= (int64_t{1} << 30) && (prefix_len == 0 || prefix), "kv_attention: prefix of %lld positions without pages",
               static_cast<long long>(prefix_len));
+  RH3_REQUIRE(form >= RH3_KV_BY_SIZE && form <= RH3_KV_CHUNK, "kv_attention: form %d", form);
   const int dim = static_cast<int>(cache->dim), fmt = static_cast<int>(cache->format);
-  const Call call = call_of(rows, q_heads, a.c.heads, dim, batch, cu == nullptr, prefix_len);
+  const Call call = call_of(rows, q_heads, a.c.heads, dim, width * cache->page, batch, cu == nullptr, prefix_len, form);
   RH3_REQUIRE(workspace && aligned16(workspace) && workspace_bytes >= call.bytes,
               "kv_attention: workspace of %lld bytes needed, %lld given", static_cast<long long>(call.bytes), static_cast<long long>(workspace_bytes));
   a.q = q;
@@ -314,17 +322,19 @@ extern "C" int rh3_kv_attention(const rh3_kv_cache* cache, const void* q, int64_
   launch(own.a, call.own, fmt, dim, stream);
   if (const int e = launch_status("kv_attention")) return e;
   // Parts that a row may have: the workgroups over the least count of items, no more than the keys make. Measured (kernel us, by
-  // shares / rows on 4 waves / on 16): 8 parts of 32 rows 4.2 / 4.7 / 5.7, 16 of 224 rows - / 6.2 / 7.7.
+  // shares / rows on 4 waves / on 16): 8 parts of 32 rows 5.1 / 4.7 / 5.7, 16 of 224 rows - / 6.3 / 7.7.
   const int64_t ids = rows * q_heads, cap = width * cache->page + prefix_len;
-  const int64_t shared = call.own.wgs / (batch * a.c.heads), parts = shared < cap / 128 ? shared : cap / 128;
+  const int64_t tiles = (rows * a.group / batch + call.own.rows - 1) / call.own.rows;
+  const int64_t shared = call.own.wgs / (batch * a.c.heads * (tiles > 0 ? tiles : 1));
+  const int64_t most = cap / (call.own.chunk ? 8 * CHUNK_KEYS : 4 * TOKEN_KEYS), parts = shared < most ? shared : most;
   const int has = prefix_len > 0 && !call.joined;
-  if (prefix_len == 0 && (call.own.chunk || parts <= 8)) {
+  if (prefix_len == 0 && parts <= 8) {
     const dim3 grid(static_cast<uint32_t>(call.own.wgs), static_cast<uint32_t>(call.own.rows / 16));
     if (dim == 128) hipLaunchKernelGGL((join_shares_kernel<128>), grid, dim3(256), 0, stream, own);
     else hipLaunchKernelGGL((join_shares_kernel<64>), grid, dim3(256), 0, stream, own);
     return launch_status("kv_attention (join)");
   }
-  const int wpr = !call.own.chunk && parts > 32 ? 16 : !call.own.chunk && !has ? 4 : 1;
+  const int wpr = parts > 32 ? 16 : ids <= 16384 ? 4 : 1;
   const int64_t grid = wpr == 1 ? (ids + 3) / 4 : ids;
   RH3_REQUIRE(grid * (wpr == 16 ? 4 : 1) <= MAX_GRID_256, "kv_attention: %lld rows in one call", static_cast<long long>(rows));
   auto go = [&](auto kernel) {

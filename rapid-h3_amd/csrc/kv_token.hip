@@ -1,7 +1,8 @@
 // Attention of few query rows over the paged cache: single tokens of a batch, or a few tokens each.
 //
-// Bound by the cache's bytes: 2 (dim + 4) per K/V head and position. A wave takes 32 keys at a time, for up to 32 query rows of
-// the K/V head, straight from memory to registers, and its matrix instructions' operand order is made to fit what a wide load
+// Bound by the cache's bytes: 2 (dim + 4) per K/V head and position. A wave takes 32 keys at a time, for 16 query rows of the K/V
+// head (32 at dim 64: at 128 their accumulators leave no registers for the loads, and 2 x 16 rows, the second time mostly from
+// L2, took 164 us where 32 took 230: 8 sequences of 4 tokens x 56 / 8 heads x 32,768 keys), straight from memory to registers, and its matrix instructions' operand order is made to fit what a wide load
 // brings, so nothing passes through LDS:
 //   S^T = K Q^T: lane l holds key l % 16, two (one) 16-byte pieces of its row; the channel order this gives each MFMA step is
 //   given to Q as well. The result has the query row in l % 16 and keys 4 (l / 16) + 0 .. 3 in the registers of both 16-key tiles.
@@ -366,9 +367,8 @@ __global__ void __launch_bounds__(NT, 2) token_kernel(AttnArgs a) {
 
 void launch_token(const AttnArgs& a, int fmt, int dim, int rows, hipStream_t st) {
   auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(a.wgs)), dim3(NT), 0, st, a); };
-  if (fmt == INT8 && dim == 128) rows == 16 ? go(token_kernel<INT8, 128, 1>) : go(token_kernel<INT8, 128, 2>);
+  if (dim == 128) fmt == INT8 ? go(token_kernel<INT8, 128, 1>) : go(token_kernel<E4M3, 128, 1>);
   else if (fmt == INT8) rows == 16 ? go(token_kernel<INT8, 64, 1>) : go(token_kernel<INT8, 64, 2>);
-  else if (dim == 128) rows == 16 ? go(token_kernel<E4M3, 128, 1>) : go(token_kernel<E4M3, 128, 2>);
   else rows == 16 ? go(token_kernel<E4M3, 64, 1>) : go(token_kernel<E4M3, 64, 2>);
 }
 

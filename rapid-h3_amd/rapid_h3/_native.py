@@ -85,9 +85,9 @@ SIGNATURES = {
     "rh3_attention_f8_forward": ([_I, _I, _I, _F, _C, _P, _I, _I, _P, _I, _P], _C),
     "rh3_kv_write": ([_P, _P, _I, _I, _P, _I, _I, _C, _I, _P, _I, _I, _P, _P, _I, _P], _C),
     "rh3_kv_read": ([_P, _P, _I, _I, _P, _I, _I, _C, _I, _P, _I, _I, _P, _P, _I, _P], _C),
-    "rh3_kv_attention_workspace_bytes": ([_P, _I, _I, _I, _C, _I], ctypes.c_int64),
-    "rh3_kv_attention": ([_P, _P, _I, _I, _I, _C, _I, _P, _I, _I, _P, _P, _I, _C, _F, _P, _I, _I, _P, _P, _I, _P, _I,
-                          _P], _C),
+    "rh3_kv_attention_workspace_bytes": ([_P, _I, _I, _I, _I, _C, _I, _C], ctypes.c_int64),
+    "rh3_kv_attention": ([_P, _P, _I, _I, _I, _C, _I, _P, _I, _I, _P, _P, _I, _C, _F, _P, _I, _I, _P, _P, _I, _C, _P,
+                          _I, _P], _C),
 }
 
 RH3_DTYPE_BF16 = 1
@@ -95,6 +95,7 @@ RH3_DTYPE_F32 = 2
 RH3_DTYPE_F16 = 3
 RH3_KV_INT8 = 0
 RH3_KV_E4M3 = 1
+RH3_KV_BY_SIZE, RH3_KV_TOKEN, RH3_KV_CHUNK = 0, 1, 2
 
 _lib = None
 _FN = {}   # entry point name -> bound function, filled by lib()

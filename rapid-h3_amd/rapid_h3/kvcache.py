@@ -21,6 +21,7 @@ from . import _native as nat
 
 FP8 = torch.float8_e4m3fn
 _ROW = {torch.bfloat16: nat.RH3_DTYPE_BF16, torch.float16: nat.RH3_DTYPE_F16, torch.float32: nat.RH3_DTYPE_F32}
+_FORM = {None: nat.RH3_KV_BY_SIZE, "token": nat.RH3_KV_TOKEN, "chunk": nat.RH3_KV_CHUNK}
 _HERE = contextlib.nullcontext()
 
 
@@ -131,7 +132,10 @@ def kv_read(cache, table, lens, cu=None, rows=None, dtype=torch.bfloat16, out=No
     return k, v
 
 
-def _attention(name, q, cache, prefix, prefix_len, table, lens, cu, causal, scale, out, lse):
+def _attention(name, q, cache, prefix, prefix_len, table, lens, cu, causal, scale, out, lse, form):
+    f = _FORM.get(form)
+    if f is None:
+        raise ValueError(f"{name}: form {form!r} (None, 'token' or 'chunk')")
     if q.ndim != 3 or q.shape[2] != cache.dim or q.stride(2) != 1 or q.shape[1] % cache.heads or not q.shape[1]:
         raise RuntimeError(f"{name}: q must be [rows, a multiple of {cache.heads} heads, {cache.dim}] with a contiguous last dim, got "
                            f"{tuple(q.shape)}")
@@ -148,24 +152,26 @@ def _attention(name, q, cache, prefix, prefix_len, table, lens, cu, causal, scal
     elif out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1 or out.device != dev:
         raise RuntimeError(f"{name}: out must be like q, with a contiguous last dim")
     sums = alloc((t, hq), dtype=torch.float32, device=dev) if lse else None
-    n = nat.lib().rh3_kv_attention_workspace_bytes(cache._ref, hq, t, seqs[5], cu is None, prefix_len)
+    n = nat.lib().rh3_kv_attention_workspace_bytes(cache._ref, hq, t, seqs[2], seqs[5], cu is None, prefix_len, f)
     ws = torch.empty(n, dtype=torch.uint8, device=dev)
     with _on(dev):
         nat.call("rh3_kv_attention", cache._ref, q.data_ptr(), q.stride(0), q.stride(1), hq, _ROW[q.dtype], t, *seqs, int(causal),
                  d ** -0.5 if scale is None else scale, out.data_ptr(), out.stride(0), out.stride(1), nat.ptr(sums),
-                 nat.ptr(prefix), prefix_len, ws.data_ptr(), n, nat.stream(dev))
+                 nat.ptr(prefix), prefix_len, f, ws.data_ptr(), n, nat.stream(dev))
     return (out, sums) if lse else out
 
 
-def kv_attention(q, cache, table, lens, cu=None, causal=True, scale=None, out=None, lse=False):
+def kv_attention(q, cache, table, lens, cu=None, causal=True, scale=None, out=None, lse=False, form=None):
     """Attention of q [rows, q heads, dim] (bf16 or fp16, strided ok) over the cached positions of each row's sequence ->
     out like q; query head h reads K/V head h // (q heads // heads). causal: row i of n sees positions up to
     lens[b] - n + i. scale: dim ** -0.5 by default. lse=True: also the log-sum-exp [rows, q heads] fp32 of the scaled scores.
-    A row that sees no key gives 0 and -inf."""
-    return _attention("kv_attention", q, cache, None, 0, table, lens, cu, causal, scale, out, lse)
+    A row that sees no key gives 0 and -inf. form: "token" or "chunk", the kernel for few or for many query rows to a K/V head;
+    by default the sizes decide, with the table's width in the place of the lengths, which only the GPU knows."""
+    return _attention("kv_attention", q, cache, None, 0, table, lens, cu, causal, scale, out, lse, form)
 
 
-def kv_attention_shared(q, cache, prefix, prefix_len, table, lens, cu=None, causal=True, scale=None, out=None, lse=False):
+def kv_attention_shared(q, cache, prefix, prefix_len, table, lens, cu=None, causal=True, scale=None, out=None, lse=False,
+                        form=None):
     """kv_attention of a batch whose sequences all begin with the first prefix_len (an int) positions of the pages `prefix`
     (int32 [pages]): every row sees them, then its sequence's own positions (table, lens: without the prefix). The prefix is
     read once for the whole batch."""
@@ -174,4 +180,4 @@ def kv_attention_shared(q, cache, prefix, prefix_len, table, lens, cu=None, caus
         raise RuntimeError("kv_attention_shared: prefix must be contiguous int32 [pages] on q's GPU")
     if not 0 <= prefix_len <= prefix.numel() * cache.page:
         raise RuntimeError(f"kv_attention_shared: prefix_len {prefix_len} does not fit {prefix.numel()} pages of {cache.page}")
-    return _attention("kv_attention_shared", q, cache, prefix, prefix_len, table, lens, cu, causal, scale, out, lse)
+    return _attention("kv_attention_shared", q, cache, prefix, prefix_len, table, lens, cu, causal, scale, out, lse, form)

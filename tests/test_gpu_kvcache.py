@@ -12,6 +12,7 @@ from rapid_h3 import kvcache as kv
 pytestmark = pytest.mark.gpu
 
 I8, F8 = torch.int8, torch.float8_e4m3fn
+FORMS = ["token", "chunk"]          # both kernels, whichever the sizes would choose
 BF, HF, F32 = torch.bfloat16, torch.float16, torch.float32
 
 
@@ -202,8 +203,9 @@ CASES = [
 
 @pytest.mark.parametrize("fmt", [I8, F8])
 @pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("form", FORMS)
 @pytest.mark.parametrize("case", range(len(CASES)))
-def test_attention(dev, fmt, dtype, case):
+def test_attention(dev, fmt, dtype, form, case):
     hq, hkv, dim, page, lens, new, causal = CASES[case]
     b = len(lens)
     width = max(-(-max(lens) // page), 1)
@@ -216,7 +218,8 @@ def test_attention(dev, fmt, dtype, case):
     t = cu[-1]
     c = _pool(dev, fmt, pages, hkv, page, dim, case)
     q = (2.0 * torch.randn(t, hq, dim, generator=_gen(case + 50))).to(dtype).to(dev)
-    out, lse = kv.kv_attention(q, c, _i32(table, dev), _i32(lens, dev), None if even else _i32(cu, dev), causal=causal, lse=True)
+    out, lse = kv.kv_attention(q, c, _i32(table, dev), _i32(lens, dev), None if even else _i32(cu, dev), causal=causal, lse=True,
+                               form=form)
     ref, rl, mag, err = ok.attention(q, c, table, lens, None if even else cu, causal)
     _check(out, ref, mag, err, 3.1)
     _check_lse(lse, rl, err)
@@ -230,24 +233,26 @@ def test_attention(dev, fmt, dtype, case):
     (40, 4, 1, [9001], 64),              # key ranges of the chunk kernel
     (100, 2, 2, [3000, 20], 32),
 ])
-def test_attention_in_parts(dev, fmt, rows, hq, hkv, lens, page):
+@pytest.mark.parametrize("form", FORMS)
+def test_attention_in_parts(dev, fmt, form, rows, hq, hkv, lens, page):
     b, dim = len(lens), 128
     width = -(-max(lens) // page)
     table = _tables(b * width, width, b, 1)
     c = _pool(dev, fmt, b * width, hkv, page, dim, 8)
     q = (2.0 * torch.randn(b * rows, hq, dim, generator=_gen(9))).to(BF).to(dev)
     args = (_i32(table, dev), _i32(lens, dev))
-    out, lse = kv.kv_attention(q, c, *args, lse=True)
+    out, lse = kv.kv_attention(q, c, *args, lse=True, form=form)
     ref, rl, mag, err = ok.attention(q, c, table, lens)
     _check(out, ref, mag, err, 3.1)
     _check_lse(lse, rl, err)
-    again = kv.kv_attention(q, c, *args)
+    again = kv.kv_attention(q, c, *args, form=form)
     assert torch.equal(out.view(torch.int16), again.view(torch.int16))          # the same bits every time
 
 
 @pytest.mark.parametrize("fmt", [I8, F8])
 @pytest.mark.parametrize("rows,lens,page", [(1, [33, 5, 0], 16), (3, [70, 9], 64), (1, [1000], 32), (70, [90, 71], 16), (80, [40], 32)])
-def test_unwritten_pool_stays_out(dev, fmt, rows, lens, page):
+@pytest.mark.parametrize("form", FORMS)
+def test_unwritten_pool_stays_out(dev, fmt, form, rows, lens, page):
     """What lies behind the sequences, in absent pages and in rows that a causal limit hides (NaN codes, NaN and infinite
     scales) reaches no row that does not see it."""
     b, hq, hkv, dim = len(lens), 4, 2, 128
@@ -270,7 +275,7 @@ def test_unwritten_pool_stays_out(dev, fmt, rows, lens, page):
     if lens[0] > page:     # a page in the middle of what is visible goes away
         table[0][0] = b * width
     q = torch.randn(b * rows, hq, dim, generator=g).to(BF).to(dev)
-    out, lse = kv.kv_attention(q, c, _i32(table, dev), _i32(lens, dev), lse=True)
+    out, lse = kv.kv_attention(q, c, _i32(table, dev), _i32(lens, dev), lse=True, form=form)
     ref, rl, mag, err = ok.attention(q, c, table, lens)
     _check(out, ref, mag, err, 3.1)
     _check_lse(lse, rl, err)
@@ -285,7 +290,8 @@ def test_unwritten_pool_stays_out(dev, fmt, rows, lens, page):
     (5, 1, 4, 4, 1, [1, 2, 3, 4, 5], 64, 256),
     (3, 1, 4, 4, 0, [7, 2, 3], 128, 64),            # no prefix after all
 ])
-def test_shared_prefix(dev, fmt, b, rows, hq, hkv, prefix, lens, dim, page):
+@pytest.mark.parametrize("form", [None] + FORMS)
+def test_shared_prefix(dev, fmt, form, b, rows, hq, hkv, prefix, lens, dim, page):
     lens = lens or [1 + 17 * i for i in range(b)]
     width = max(-(-max(lens) // page), 1)
     pre = -(-prefix // page)
@@ -296,15 +302,17 @@ def test_shared_prefix(dev, fmt, b, rows, hq, hkv, prefix, lens, dim, page):
     c = _pool(dev, fmt, pages, hkv, page, dim, 12)
     q = (2.0 * torch.randn(b * rows, hq, dim, generator=_gen(13))).to(HF).to(dev)
     for causal in (True, False):
-        out, lse = kv.kv_attention_shared(q, c, _i32(common, dev), prefix, _i32(table, dev), _i32(lens, dev), causal=causal, lse=True)
+        out, lse = kv.kv_attention_shared(q, c, _i32(common, dev), prefix, _i32(table, dev), _i32(lens, dev), causal=causal, lse=True,
+                                         form=form)
         ref, rl, mag, err = ok.attention(q, c, table, lens, None, causal, prefix=common, prefix_len=prefix)
         _check(out, ref, mag, err, 3.1)
         _check_lse(lse, rl, err)
 
 
 @pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("form", FORMS)
 @pytest.mark.parametrize("rows", [1, 50])
-def test_query_magnitudes(dev, dtype, rows):
+def test_query_magnitudes(dev, dtype, form, rows):
     """Query rows of every magnitude their type has, zero rows, and infinite or NaN ones, which change no other row."""
     c = _pool(dev, I8, 4, 1, 64, 128, 20)
     top = 100 if dtype == BF else 14
@@ -313,7 +321,7 @@ def test_query_magnitudes(dev, dtype, rows):
     q[1], q[2, 0, 5], q[3, 0, 0] = 0.0, math.nan, math.inf
     q = q.to(dtype).to(dev)
     table, lens = [[0, 2]] * 6, [100] * 6
-    out, lse = kv.kv_attention(q, c, _i32(table, dev), _i32(lens, dev), causal=False, lse=True)
+    out, lse = kv.kv_attention(q, c, _i32(table, dev), _i32(lens, dev), causal=False, lse=True, form=form)
     ref, rl, mag, err = ok.attention(q, c, table, lens, None, False)
     assert torch.isnan(out[2]).all() and torch.isnan(lse[2]).all()
     keep = [i for i in range(6 * rows) if i not in (2, 3)]
@@ -321,8 +329,9 @@ def test_query_magnitudes(dev, dtype, rows):
     _check_lse(lse[keep], rl[keep], err[keep])
 
 
+@pytest.mark.parametrize("form", FORMS)
 @pytest.mark.parametrize("rows", [1, 60])
-def test_extreme_scores_and_scales(dev, rows):
+def test_extreme_scores_and_scales(dev, form, rows):
     """One key far above the others (their probabilities vanish), whose values are far smaller than theirs: value scales within
     2^24 of each other keep the weights' full precision."""
     dim, page, n = 128, 32, 200
@@ -335,7 +344,7 @@ def test_extreme_scores_and_scales(dev, rows):
     args = (_i32([[6, 0, 3, 2, 5, 4, 1]], dev), _i32([n], dev))
     kv.kv_write(c, x.to(dev), y.to(dev), *args)
     q = torch.cat([3.0 * torch.randn(rows, 2, dim, generator=g) + x[77] / 8]).to(BF).to(dev)
-    out, lse = kv.kv_attention(q, c, *args, lse=True, causal=False)
+    out, lse = kv.kv_attention(q, c, *args, lse=True, causal=False, form=form)
     ref, rl, mag, err = ok.attention(q, c, [[6, 0, 3, 2, 5, 4, 1]], [n], None, False)
     _check(out, ref, mag, err, 3.1)
     _check_lse(lse, rl, err)
@@ -369,10 +378,10 @@ def test_layouts(dev):
 
 def test_rows_that_no_sequence_has_stay(dev):
     c = _pool(dev, I8, 4, 1, 16, 64, 41)
-    for rows, cu in ((5, [0, 1, 3]), (90, [0, 40, 83])):
+    for rows, cu, form in ((5, [0, 1, 3], "token"), (90, [0, 40, 83], "chunk"), (90, [0, 40, 83], "token")):
         q = torch.randn(rows, 2, 64, generator=_gen(42)).to(BF).to(dev)
         out = torch.full_like(q, 9.0)
-        kv.kv_attention(q, c, _i32([[0, 1], [2, 3]], dev), _i32([20, 30], dev), _i32(cu, dev), out=out)
+        kv.kv_attention(q, c, _i32([[0, 1], [2, 3]], dev), _i32([20, 30], dev), _i32(cu, dev), out=out, form=form)
         assert (out[cu[-1]:] == 9.0).all() and not (out[:cu[-1]] == 9.0).all(-1).any()
         ref, _, mag, err = ok.attention(q[:cu[-1]], c, [[0, 1], [2, 3]], [20, 30], cu)
         _check(out[:cu[-1]], ref, mag, err, 3.1)
@@ -386,9 +395,9 @@ def test_bad_contents_stay_inside(dev):
     before = [t.clone() for t in (c.k, c.v, c.k_scale, c.v_scale)]
     table = [[0, 1], [-7, 2 ** 31 - 1], [2, pages], [3, 4]]
     lens = [10 ** 9, 20, 32, -5]
-    for rows in (1, 30):
+    for rows, form in ((1, "token"), (30, "token"), (1, "chunk"), (30, "chunk")):
         q = torch.randn(4 * rows, 4, dim, generator=_gen(44)).to(BF).to(dev)
-        out = kv.kv_attention(q, c, _i32(table, dev), _i32(lens, dev), causal=False)
+        out = kv.kv_attention(q, c, _i32(table, dev), _i32(lens, dev), causal=False, form=form)
         ref, _, mag, err = ok.attention(q, c, table, [32, 20, 32, 0], None, False)
         _check(out, ref, mag, err, 3.1)
         assert (out[rows:2 * rows] == 0).all() and (out[3 * rows:] == 0).all()
@@ -399,8 +408,9 @@ def test_bad_contents_stay_inside(dev):
     kv.kv_write(c, x, x, dead, _i32([20] * 4, dev), bad)
     assert all(torch.equal(a, b) for a, b in zip(before, (c.k, c.v, c.k_scale, c.v_scale)))
     kv.kv_read(c, dead, _i32([20] * 4, dev), bad, rows=6)
-    kv.kv_attention(q, c, dead, _i32([20] * 4, dev), bad)
-    kv.kv_attention_shared(q, c, _i32([9, -1, 2], dev), 40, dead, _i32([20] * 4, dev), bad)
+    for form in FORMS:
+        kv.kv_attention(q, c, dead, _i32([20] * 4, dev), bad, form=form)
+        kv.kv_attention_shared(q, c, _i32([9, -1, 2], dev), 40, dead, _i32([20] * 4, dev), bad, form=form)
     torch.cuda.synchronize()
 
 
@@ -426,7 +436,7 @@ def test_offsets_past_32_bits(dev, fmt):
     ref, _, mag, err = ok.attention(q, c, table, lens)
     _check(out, ref, mag, err, 3.1)
     q = torch.randn(100, 8, dim, generator=g).to(BF).to(dev)
-    out = kv.kv_attention(q, c, *args[:2])
+    out = kv.kv_attention(q, c, *args[:2], form="chunk")
     ref, _, mag, err = ok.attention(q, c, table, lens)
     _check(out, ref, mag, err, 3.1)
 
@@ -468,15 +478,16 @@ def test_generation(dev):
     assert ((got.cpu() - want).abs() <= step * (0.5 + 2.0 ** -15)).all()
 
 
-def _step(c, q, k, v, tab, lens, ptab=None, prefix_len=0):
+def _step(c, q, k, v, tab, lens, ptab=None, prefix_len=0, form=None):
     kv.kv_write(c, k, v, tab, lens)
     if prefix_len:
-        return kv.kv_attention_shared(q, c, ptab, prefix_len, tab, lens)
-    return kv.kv_attention(q, c, tab, lens)
+        return kv.kv_attention_shared(q, c, ptab, prefix_len, tab, lens, form=form)
+    return kv.kv_attention(q, c, tab, lens, form=form)
 
 
+@pytest.mark.parametrize("form", FORMS)
 @pytest.mark.parametrize("rows,prefix_len", [(1, 0), (1, 500), (60, 0)])
-def test_captured_steps(dev, rows, prefix_len):
+def test_captured_steps(dev, form, rows, prefix_len):
     """A step captured once follows new inputs, lengths and page tables on every replay; two captured steps run at once on two
     streams."""
     b, hq, hkv, dim, page = 2, 4, 2, 128, 32
@@ -487,7 +498,7 @@ def test_captured_steps(dev, rows, prefix_len):
         q, k, v = (torch.randn(b * rows, h, dim, generator=g).to(BF).to(dev) for h in (hq, hkv, hkv))
         tab, ptab = _i32(_tables(60, 30, b, which), dev), _i32(list(range(60, 76)), dev)
         lens = _i32([700, 130], dev)
-        args = (c, q, k, v, tab, lens, ptab, prefix_len)
+        args = (c, q, k, v, tab, lens, ptab, prefix_len, form)
         s = torch.cuda.Stream()
         s.wait_stream(torch.cuda.current_stream())
         with torch.cuda.stream(s):
@@ -499,12 +510,12 @@ def test_captured_steps(dev, rows, prefix_len):
         steps.append((graph, out, args, torch.cuda.Stream()))
     for replay in range(3):
         want = []
-        for graph, out, (c, q, k, v, tab, lens, ptab, n), _ in steps:
+        for graph, out, (c, q, k, v, tab, lens, ptab, n, _), _ in steps:
             for t in (q, k, v):
                 t.copy_(torch.randn(t.shape, generator=_gen(replay + 7)).to(BF))
             lens.copy_(torch.tensor([60 + 300 * replay, 959 - replay], dtype=torch.int32))
             tab.copy_(tab.flip(1))
-            want.append(_step(c, q, k, v, tab, lens, ptab, n).clone())
+            want.append(_step(c, q, k, v, tab, lens, ptab, n, form).clone())
             out.zero_()
         torch.cuda.synchronize()
         for graph, _, _, stream in steps:

@@ -24,9 +24,9 @@ def _write(desc, name="rh3_kv_write", rows=6, k=FAKE, v=FAKE, k_st=512, k_sh=128
 
 
 def _attend(desc, rows=2, q=FAKE, q_st=1024, hq=8, dtype=1, table=FAKE, stride=8, width=8, lens=FAKE, cu=None, batch=2, out=FAKE,
-            prefix=None, prefix_len=0, ws=FAKE, n=1 << 40):
+            prefix=None, prefix_len=0, form=0, ws=FAKE, n=1 << 40):
     return nat.lib().rh3_kv_attention(ctypes.addressof(desc), q, q_st, 128, hq, dtype, rows, table, stride, width, lens, cu, batch, 1,
-                                      0.1, out, 1024, 128, None, prefix, prefix_len, ws, n, None)
+                                      0.1, out, 1024, 128, None, prefix, prefix_len, form, ws, n, None)
 
 
 @pytest.mark.parametrize("change,message", [
@@ -60,7 +60,7 @@ def test_row_refusals():
                             (dict(q_st=1028), "multiples of 8"), (dict(dtype=2), "query type 2"), (dict(hq=6), "do not divide over"),
                             (dict(hq=0), "do not divide over"), (dict(prefix_len=5), "without pages"),
                             (dict(prefix=FAKE, prefix_len=-1), "prefix of -1"), (dict(ws=None), "workspace"), (dict(n=64), "workspace"),
-                            (dict(ws=FAKE + 4), "workspace")):
+                            (dict(ws=FAKE + 4), "workspace"), (dict(form=3), "form 3"), (dict(form=-1), "form -1")):
         assert _attend(_desc(), **change) == 1 and message in nat.last_error(), nat.last_error()
 
 
@@ -74,11 +74,11 @@ def test_workspace_holds_every_part():
     """More rows, positions or a prefix never need less; nothing to compute needs nothing."""
     size = nat.lib().rh3_kv_attention_workspace_bytes
     d = ctypes.addressof(_desc())
-    assert size(d, 8, 0, 2, 1, 0) == 0 and size(None, 8, 2, 2, 1, 0) == 0 and size(d, 6, 2, 2, 1, 0) == 0
-    for rows, batch in ((1, 1), (64, 64), (64, 2), (5000, 1)):
-        n = size(d, 8, rows, batch, 1, 0)
-        assert size(d, 8, rows, batch, 1, 3000) > n
-        assert size(d, 8, rows, batch, 0, 0) >= n
+    assert size(d, 8, 0, 8, 2, 1, 0, 0) == 0 and size(None, 8, 2, 8, 2, 1, 0, 0) == 0 and size(d, 6, 2, 8, 2, 1, 0, 0) == 0
+    for rows, batch, form in ((1, 1, 0), (64, 64, 0), (64, 2, 1), (64, 2, 2), (5000, 1, 0)):
+        n = size(d, 8, rows, 2000, batch, 1, 0, form)
+        assert size(d, 8, rows, 2000, batch, 1, 3000, form) > n
+        assert size(d, 8, rows, 2000, batch, 0, 0, form) >= n
 
 
 def test_wrappers_refuse():
@@ -111,6 +111,8 @@ def test_wrappers_refuse():
         kv.kv_attention(x[:, :1], Cache, t, n)
     with pytest.raises(TypeError, match="bf16 or fp16"):
         kv.kv_attention(x.float(), Cache, t, n)
+    with pytest.raises(ValueError, match="form 'both'"):
+        kv.kv_attention(x, Cache, t, n, form="both")
     with pytest.raises(RuntimeError, match="does not fit"):
         kv.kv_attention_shared(x, Cache, torch.zeros(2, dtype=torch.int32), 129, t, n)
     with pytest.raises(RuntimeError, match="prefix must be"):
