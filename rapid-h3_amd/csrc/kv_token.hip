@@ -84,9 +84,14 @@ struct State {
   float ref[MT], sum[MT], vref, ivref;
 };
 
-// One tile. MORE: the wave's next tile (pages `pn`) is loaded into the same registers, its keys as soon as these are used, its
+__device__ __forceinline__ h8_t to_f16(const float (&y)[8]) {
+  return join(__builtin_bit_cast(h2_t, pack_h2(y[0], y[1])), __builtin_bit_cast(h2_t, pack_h2(y[2], y[3])),
+              __builtin_bit_cast(h2_t, pack_h2(y[4], y[5])), __builtin_bit_cast(h2_t, pack_h2(y[6], y[7])));
+}
+
+// One tile. FINE (fp16 results, whose own rounding is no coarser than that of the weights): the weights in two f16 terms. MORE: the wave's next tile (pages `pn`) is loaded into the same registers, its keys as soon as these are used, its
 // values at the end: a load has about half a tile's work to come in.
-template <int FMT, int D, int MT, bool MORE>
+template <int FMT, int D, int MT, bool FINE, bool MORE>
 __device__ __forceinline__ void compute(const AttnArgs& a, Tile<D>& t, int kvh, int tile, const Pages& pg, const Pages& pn,
                                         const h8_t (&q)[MT][D / 32], const float (&qf)[MT], const int (&lim)[MT], int low, int len,
                                         State<D, MT>& st) {
@@ -173,7 +178,7 @@ __device__ __forceinline__ void compute(const AttnArgs& a, Tile<D>& t, int kvh, 
       for (int i = 0; i < D / 16; ++i) st.o[m][i] *= f;
     }
   }
-  h8_t p[MT];
+  h8_t p[MT], rest[FINE ? MT : 1];
 #pragma unroll
   for (int j = 0; j < 8; ++j) vs[j] *= st.ivref;
 #pragma unroll
@@ -192,8 +197,12 @@ __device__ __forceinline__ void compute(const AttnArgs& a, Tile<D>& t, int kvh, 
       for (int j = 0; j < 8; ++j)
         if (key[j] >= lim[m]) y[j] = 0.0f;
     }
-    const uint32_t w[4] = {pack_h2(y[0], y[1]), pack_h2(y[2], y[3]), pack_h2(y[4], y[5]), pack_h2(y[6], y[7])};
-    p[m] = join(__builtin_bit_cast(h2_t, w[0]), __builtin_bit_cast(h2_t, w[1]), __builtin_bit_cast(h2_t, w[2]), __builtin_bit_cast(h2_t, w[3]));
+    p[m] = to_f16(y);
+    if constexpr (FINE) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) y[j] -= static_cast<float>(p[m][j]);
+      rest[m] = to_f16(y);
+    }
   }
 #pragma unroll
   for (int c = 0; c < D / 64; ++c) {
@@ -205,13 +214,15 @@ __device__ __forceinline__ void compute(const AttnArgs& a, Tile<D>& t, int kvh, 
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int m = 0; m < MT; ++m)
+      for (int m = 0; m < MT; ++m) {
         st.o[m][4 * c + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[i], p[m], st.o[m][4 * c + i], 0, 0, 0);
+        if constexpr (FINE) st.o[m][4 * c + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[i], rest[m], st.o[m][4 * c + i], 0, 0, 0);
+      }
   }
   if constexpr (MORE) load_values<D>(a, kvh, tile + WAVES, pn, t);
 }
 
-template <int FMT, int D, int MT>
+template <int FMT, int D, int MT, bool FINE>
 __global__ void __launch_bounds__(NT, 2) token_kernel(AttnArgs a) {
   constexpr int R = 16 * MT, PAD = D + 4;
   const Tiling TILING = tiling(false, R);
@@ -293,11 +304,11 @@ __global__ void __launch_bounds__(NT, 2) token_kernel(AttnArgs a) {
       load_values<D>(a, kvh, t, pg, tile);
       for (; t + WAVES < t1; t += WAVES) {
         const Pages p2 = pages_of(a, row, width, t + 2 * WAVES);
-        compute<FMT, D, MT, true>(a, tile, kvh, t, pg, pn, q, qf, lim, low, sq.len, st);
+        compute<FMT, D, MT, FINE, true>(a, tile, kvh, t, pg, pn, q, qf, lim, low, sq.len, st);
         pg = pn;
         pn = p2;
       }
-      compute<FMT, D, MT, false>(a, tile, kvh, t, pg, pn, q, qf, lim, low, sq.len, st);
+      compute<FMT, D, MT, FINE, false>(a, tile, kvh, t, pg, pn, q, qf, lim, low, sq.len, st);
     }
     // join the 4 waves
 #pragma unroll
@@ -367,9 +378,13 @@ __global__ void __launch_bounds__(NT, 2) token_kernel(AttnArgs a) {
 
 void launch_token(const AttnArgs& a, int fmt, int dim, int rows, hipStream_t st) {
   auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(a.wgs)), dim3(NT), 0, st, a); };
-  if (dim == 128) fmt == INT8 ? go(token_kernel<INT8, 128, 1>) : go(token_kernel<E4M3, 128, 1>);
-  else if (fmt == INT8) rows == 16 ? go(token_kernel<INT8, 64, 1>) : go(token_kernel<INT8, 64, 2>);
-  else rows == 16 ? go(token_kernel<E4M3, 64, 1>) : go(token_kernel<E4M3, 64, 2>);
+  auto by_type = [&](auto bf16, auto fp16) { a.fp16 ? go(fp16) : go(bf16); };
+  if (dim == 128 && fmt == INT8) by_type(token_kernel<INT8, 128, 1, false>, token_kernel<INT8, 128, 1, true>);
+  else if (dim == 128) by_type(token_kernel<E4M3, 128, 1, false>, token_kernel<E4M3, 128, 1, true>);
+  else if (fmt == INT8 && rows == 16) by_type(token_kernel<INT8, 64, 1, false>, token_kernel<INT8, 64, 1, true>);
+  else if (fmt == INT8) by_type(token_kernel<INT8, 64, 2, false>, token_kernel<INT8, 64, 2, true>);
+  else if (rows == 16) by_type(token_kernel<E4M3, 64, 1, false>, token_kernel<E4M3, 64, 1, true>);
+  else by_type(token_kernel<E4M3, 64, 2, false>, token_kernel<E4M3, 64, 2, true>);
 }
 
 }  // namespace kv

@@ -309,6 +309,48 @@ def test_shared_prefix(dev, fmt, form, b, rows, hq, hkv, prefix, lens, dim, page
         _check_lse(lse, rl, err)
 
 
+@pytest.mark.parametrize("form", FORMS)
+def test_many_sequences(dev, form):
+    """More sequences than a wavefront has lanes, uneven, some without rows or without keys, alone and behind a prefix."""
+    b, hq, hkv, dim, page = 200, 4, 2, 64, 16
+    new = [(i * 7) % 4 for i in range(b)]
+    lens = [(i * i) % 97 for i in range(b)]
+    cu = [0]
+    for n in new:
+        cu.append(cu[-1] + n)
+    width = 7
+    table = _tables(b * width + 10, width, b, 21)
+    used = {p for t in table for p in t}
+    common = [p for p in range(b * width + 10) if p not in used]
+    c = _pool(dev, F8, b * width + 10, hkv, page, dim, 22)
+    q = torch.randn(cu[-1], hq, dim, generator=_gen(23)).to(BF).to(dev)
+    args = (_i32(table, dev), _i32(lens, dev), _i32(cu, dev))
+    out, lse = kv.kv_attention(q, c, *args, lse=True, form=form)
+    ref, rl, mag, err = ok.attention(q, c, table, lens, cu)
+    _check(out, ref, mag, err, 3.1)
+    _check_lse(lse, rl, err)
+    out, lse = kv.kv_attention_shared(q, c, _i32(common, dev), 155, *args, lse=True, form=form)
+    ref, rl, mag, err = ok.attention(q, c, table, lens, cu, prefix=common, prefix_len=155)
+    _check(out, ref, mag, err, 3.1)
+    _check_lse(lse, rl, err)
+
+
+def test_prefix_and_sequences_on_their_own_kernels(dev):
+    """A prefix long enough for the chunk kernel before sequences that take the token kernel."""
+    b, hq, hkv, dim, page, prefix = 64, 8, 2, 128, 256, 60001
+    lens = [1 + 5 * i for i in range(b)]
+    pre = -(-prefix // page)
+    table = _tables(2 * b + pre, 2, b, 24)
+    used = {p for t in table for p in t}
+    common = [p for p in range(2 * b + pre) if p not in used]
+    c = _pool(dev, I8, 2 * b + pre, hkv, page, dim, 25)
+    q = torch.randn(b, hq, dim, generator=_gen(26)).to(BF).to(dev)
+    out, lse = kv.kv_attention_shared(q, c, _i32(common, dev), prefix, _i32(table, dev), _i32(lens, dev), lse=True)
+    ref, rl, mag, err = ok.attention(q, c, table, lens, prefix=common, prefix_len=prefix)
+    _check(out, ref, mag, err, 3.1)
+    _check_lse(lse, rl, err)
+
+
 @pytest.mark.parametrize("dtype", [BF, HF])
 @pytest.mark.parametrize("form", FORMS)
 @pytest.mark.parametrize("rows", [1, 50])
