@@ -501,9 +501,9 @@ int rh3_kv_read(const rh3_kv_cache* cache, void* k, int64_t k_st, int64_t k_sh, 
  * prefix[], which come before the sequences' own and are read once for the batch. out may lie exactly over q. form: the
  * kernel for few query rows to a K/V head (RH3_KV_TOKEN) or for many (RH3_KV_CHUNK), or by the sizes, where the table's width
  * stands for the lengths, which only the device knows.
- * The workspace holds the parts of rows whose keys several workgroups share; how keys are split depends on the sizes, lengths
+ * The workspace (capacity: width * page; even: 1 where cu is NULL) holds the parts of rows whose keys several workgroups share; how keys are split depends on the sizes, lengths
  * and the CU count, and with it the last bits of the result; the same call gives the same bits. */
-int64_t rh3_kv_attention_workspace_bytes(const rh3_kv_cache* cache, int64_t q_heads, int64_t rows, int64_t width,
+int64_t rh3_kv_attention_workspace_bytes(int64_t q_heads, int64_t heads, int64_t dim, int64_t rows, int64_t capacity,
                                          int64_t batch, int even, int64_t prefix_len, int form);
 int rh3_kv_attention(const rh3_kv_cache* cache, const void* q, int64_t q_st, int64_t q_sh, int64_t q_heads, int dtype,
                      int64_t rows, const int32_t* table, int64_t table_stride, int64_t width, const int32_t* lens,

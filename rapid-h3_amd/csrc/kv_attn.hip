@@ -242,10 +242,10 @@ void launch(const AttnArgs& a, const Plan& p, int fmt, int dim, hipStream_t st) 
 using namespace rh3;
 using namespace rh3::kv;
 
-extern "C" int64_t rh3_kv_attention_workspace_bytes(const rh3_kv_cache* cache, int64_t q_heads, int64_t rows, int64_t width,
+extern "C" int64_t rh3_kv_attention_workspace_bytes(int64_t q_heads, int64_t heads, int64_t dim, int64_t rows, int64_t capacity,
                                                     int64_t batch, int even, int64_t prefix_len, int form) {
-  if (!cache || cache->heads < 1 || q_heads < cache->heads || q_heads % cache->heads || rows < 1 || batch < 1 || width < 1) return 0;
-  return call_of(rows, q_heads, cache->heads, cache->dim, width * cache->page, batch, even != 0, prefix_len, form).bytes;
+  if (heads < 1 || q_heads < heads || q_heads % heads || rows < 1 || batch < 1 || capacity < 1) return 0;
+  return call_of(rows, q_heads, heads, dim, capacity, batch, even != 0, prefix_len, form).bytes;
 }
 
 extern "C" int rh3_kv_attention(const rh3_kv_cache* cache, const void* q, int64_t q_st, int64_t q_sh, int64_t q_heads, int dtype,

@@ -85,7 +85,7 @@ SIGNATURES = {
     "rh3_attention_f8_forward": ([_I, _I, _I, _F, _C, _P, _I, _I, _P, _I, _P], _C),
     "rh3_kv_write": ([_P, _P, _I, _I, _P, _I, _I, _C, _I, _P, _I, _I, _P, _P, _I, _P], _C),
     "rh3_kv_read": ([_P, _P, _I, _I, _P, _I, _I, _C, _I, _P, _I, _I, _P, _P, _I, _P], _C),
-    "rh3_kv_attention_workspace_bytes": ([_P, _I, _I, _I, _I, _C, _I, _C], ctypes.c_int64),
+    "rh3_kv_attention_workspace_bytes": ([_I, _I, _I, _I, _I, _I, _C, _I, _C], ctypes.c_int64),
     "rh3_kv_attention": ([_P, _P, _I, _I, _I, _C, _I, _P, _I, _I, _P, _P, _I, _C, _F, _P, _I, _I, _P, _P, _I, _C, _P,
                           _I, _P], _C),
 }

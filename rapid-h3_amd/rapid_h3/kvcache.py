@@ -14,6 +14,7 @@ by the kernels, so a captured call follows what is written into them between rep
 """
 import contextlib
 import ctypes
+import functools
 
 import torch
 
@@ -30,7 +31,7 @@ class KVCache:
     fp32 (page 16 to 256, a power of two; dim 64 or 128; views of larger buffers whose pages and heads lie apart are fine,
     k like v and k_scale like v_scale). A scale is finite and not negative, or NaN. The tensors are kept and used as they are."""
 
-    __slots__ = ("k", "v", "k_scale", "v_scale", "pages", "heads", "page", "dim", "device", "_desc", "_ref")
+    __slots__ = ("k", "v", "k_scale", "v_scale", "pages", "heads", "page", "dim", "device", "gpu", "_desc", "_ref")
 
     def __init__(self, k, v, k_scale, v_scale):
         if k.ndim != 4 or v.shape != k.shape or v.stride() != k.stride():
@@ -51,6 +52,7 @@ class KVCache:
             raise RuntimeError("KVCache: the four tensors must be on one GPU (no CPU path)")
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.pages, self.heads, self.page, self.dim, self.device = p, h, n, d, k.device
+        self.gpu = k.get_device()
         self._desc = nat.KvCacheDesc(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), k.stride(0), k.stride(1),
                                      k_scale.stride(0), k_scale.stride(1), p, h, n, d,
                                      nat.RH3_KV_INT8 if k.dtype == torch.int8 else nat.RH3_KV_E4M3)
@@ -67,46 +69,60 @@ def kv_cache(pages, heads, page=64, dim=128, dtype=torch.int8, device="cuda"):
     return KVCache(codes(), codes(), scales(), scales())
 
 
-def _on(device):
+# The small calls (a token of one sequence is 12 us of GPU work in two launches) are bound by what the host does: shapes, strides
+# and devices are asked for once a call, devices as numbers, and the workspace's size once for each set of sizes.
+def _on(index):
     """The tensors' GPU as the current one for a launch, where it is another."""
-    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    return _HERE if index == torch._C._cuda_getDevice() else torch.cuda.device(index)
 
 
-def _seqs(name, cache, table, lens, cu, dev):
+_stream = torch._C._cuda_getCurrentRawStream
+
+
+def _seqs(name, cache, table, lens, cu, gpu):
     """The sequences' arguments of a call after its rows: table, its stride and width, lens, cu, batch."""
     if table.ndim != 2 or table.dtype != torch.int32 or table.stride(1) != 1:
         raise RuntimeError(f"{name}: table must be int32 [batch, pages of a sequence] with a contiguous last dim")
     b, w = table.shape
-    if lens.dtype != torch.int32 or lens.shape != (b,) or not lens.is_contiguous():
+    if lens.dtype != torch.int32 or lens.ndim != 1 or lens.numel() != b or not lens.is_contiguous():
         raise RuntimeError(f"{name}: lens must be contiguous int32 [{b}]")
-    if table.device != dev or lens.device != dev or cache.device != dev:
+    if table.get_device() != gpu or lens.get_device() != gpu or cache.gpu != gpu:
         raise RuntimeError(f"{name}: the cache, the rows, table and lens must be on one GPU")
     if cu is None:
         return table.data_ptr(), table.stride(0), w, lens.data_ptr(), None, b
-    if cu.dtype != torch.int32 or cu.shape != (b + 1,) or not cu.is_contiguous() or cu.device != dev:
+    if cu.dtype != torch.int32 or cu.ndim != 1 or cu.numel() != b + 1 or not cu.is_contiguous() or cu.get_device() != gpu:
         raise RuntimeError(f"{name}: cu must be contiguous int32 [{b + 1}] on the rows' GPU")
     return table.data_ptr(), table.stride(0), w, lens.data_ptr(), cu.data_ptr(), b
 
 
-def _check_rows(name, what, x, heads, dim):
-    if x.ndim != 3 or x.shape[2] != dim or x.shape[1] != heads or x.stride(2) != 1:
-        raise RuntimeError(f"{name}: {what} must be [rows, {heads}, {dim}] with a contiguous last dim, got {tuple(x.shape)}")
-    if not x.is_cuda:
-        raise RuntimeError(f"{name}: {what} must be on a GPU (no CPU path)")
+def _rows(name, what, x, cache):
+    """Rows of keys or values: their number and strides."""
+    if x.ndim == 3:
+        t, h, d = x.shape
+        st, sh, sd = x.stride()
+        if h == cache.heads and d == cache.dim and sd == 1:
+            if not x.is_cuda:
+                raise RuntimeError(f"{name}: {what} must be on a GPU (no CPU path)")
+            return t, st, sh
+    raise RuntimeError(f"{name}: {what} must be [rows, {cache.heads}, {cache.dim}] with a contiguous last dim, got {tuple(x.shape)}")
+
+
+def _rows_call(name, entry, what, cache, k, v, table, lens, cu):
+    t, k_st, k_sh = _rows(name, what[0], k, cache)
+    tv, v_st, v_sh = _rows(name, what[1], v, cache)
+    dt, gpu = _ROW.get(k.dtype), k.get_device()
+    if tv != t or v.dtype != k.dtype or dt is None or v.get_device() != gpu:
+        raise TypeError(f"{name}: {what[0]} and {what[1]} must be of one shape, device and type (bf16, fp16 or fp32)")
+    seqs = _seqs(name, cache, table, lens, cu, gpu)
+    with _on(gpu):
+        nat.call(entry, cache._ref, k.data_ptr(), k_st, k_sh, v.data_ptr(), v_st, v_sh, dt, t, *seqs, _stream(gpu))
 
 
 def kv_write(cache, k, v, table, lens, cu=None):
     """Quantise rows k, v [rows, heads, dim] (bf16, fp16 or fp32, strided ok) into their positions. Rows at a negative
     position or in an absent page are skipped; a row that holds an infinity or a NaN is kept as NaN (its scale). Pages that
     sequences share must not be written by more than one of them in a call."""
-    _check_rows("kv_write", "k", k, cache.heads, cache.dim)
-    _check_rows("kv_write", "v", v, cache.heads, cache.dim)
-    if k.shape != v.shape or k.dtype != v.dtype or k.dtype not in _ROW or v.device != k.device:
-        raise TypeError("kv_write: k and v must be of one shape, device and type (bf16, fp16 or fp32)")
-    seqs = _seqs("kv_write", cache, table, lens, cu, k.device)
-    with _on(k.device):
-        nat.call("rh3_kv_write", cache._ref, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
-                 _ROW[k.dtype], k.shape[0], *seqs, nat.stream(k.device))
+    _rows_call("kv_write", "rh3_kv_write", ("k", "v"), cache, k, v, table, lens, cu)
 
 
 def kv_read(cache, table, lens, cu=None, rows=None, dtype=torch.bfloat16, out=None):
@@ -118,18 +134,15 @@ def kv_read(cache, table, lens, cu=None, rows=None, dtype=torch.bfloat16, out=No
         if dtype not in _ROW:
             raise TypeError(f"kv_read: bf16, fp16 or fp32 values, got {dtype}")
         alloc = torch.empty if cu is None else torch.zeros      # rows that no sequence has are not written
-        k, v = (alloc((n, cache.heads, cache.dim), dtype=dtype, device=cache.device) for _ in range(2))
-    else:
-        k, v = out
-        _check_rows("kv_read", "out", k, cache.heads, cache.dim)
-        _check_rows("kv_read", "out", v, cache.heads, cache.dim)
-        if k.shape != v.shape or k.dtype != v.dtype or k.dtype not in _ROW or v.device != k.device:
-            raise TypeError("kv_read: out must be two tensors of one shape, device and type (bf16, fp16 or fp32)")
-    seqs = _seqs("kv_read", cache, table, lens, cu, k.device)
-    with _on(k.device):
-        nat.call("rh3_kv_read", cache._ref, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
-                 _ROW[k.dtype], k.shape[0], *seqs, nat.stream(k.device))
+        out = alloc((2, n, cache.heads, cache.dim), dtype=dtype, device=cache.device).unbind(0)
+    k, v = out
+    _rows_call("kv_read", "rh3_kv_read", ("out[0]", "out[1]"), cache, k, v, table, lens, cu)
     return k, v
+
+
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(*sizes):
+    return nat.lib().rh3_kv_attention_workspace_bytes(*sizes)
 
 
 def _attention(name, q, cache, prefix, prefix_len, table, lens, cu, causal, scale, out, lse, form):
@@ -139,25 +152,30 @@ def _attention(name, q, cache, prefix, prefix_len, table, lens, cu, causal, scal
     if q.ndim != 3 or q.shape[2] != cache.dim or q.stride(2) != 1 or q.shape[1] % cache.heads or not q.shape[1]:
         raise RuntimeError(f"{name}: q must be [rows, a multiple of {cache.heads} heads, {cache.dim}] with a contiguous last dim, got "
                            f"{tuple(q.shape)}")
-    if q.dtype != torch.bfloat16 and q.dtype != torch.float16:
+    dt = _ROW.get(q.dtype)
+    if dt is None or dt == nat.RH3_DTYPE_F32:
         raise TypeError(f"{name}: q must be bf16 or fp16, got {q.dtype}")
     if not q.is_cuda:
         raise RuntimeError(f"{name}: q must be on a GPU (no CPU path)")
-    dev = q.device
+    gpu, dev = q.get_device(), cache.device
     t, hq, d = q.shape
-    seqs = _seqs(name, cache, table, lens, cu, dev)
+    q_st, q_sh, _ = q.stride()
+    seqs = _seqs(name, cache, table, lens, cu, gpu)
     alloc = torch.empty if cu is None else torch.zeros          # rows that no sequence has are not written
     if out is None:
         out = alloc((t, hq, d), dtype=q.dtype, device=dev)
-    elif out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1 or out.device != dev:
-        raise RuntimeError(f"{name}: out must be like q, with a contiguous last dim")
+        o_st, o_sh = hq * d, d
+    else:
+        if out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1 or out.get_device() != gpu:
+            raise RuntimeError(f"{name}: out must be like q, with a contiguous last dim")
+        o_st, o_sh, _ = out.stride()
     sums = alloc((t, hq), dtype=torch.float32, device=dev) if lse else None
-    n = nat.lib().rh3_kv_attention_workspace_bytes(cache._ref, hq, t, seqs[2], seqs[5], cu is None, prefix_len, f)
+    n = _workspace_bytes(hq, cache.heads, d, t, seqs[2] * cache.page, seqs[5], cu is None, prefix_len, f)
     ws = torch.empty(n, dtype=torch.uint8, device=dev)
-    with _on(dev):
-        nat.call("rh3_kv_attention", cache._ref, q.data_ptr(), q.stride(0), q.stride(1), hq, _ROW[q.dtype], t, *seqs, int(causal),
-                 d ** -0.5 if scale is None else scale, out.data_ptr(), out.stride(0), out.stride(1), nat.ptr(sums),
-                 nat.ptr(prefix), prefix_len, f, ws.data_ptr(), n, nat.stream(dev))
+    with _on(gpu):
+        nat.call("rh3_kv_attention", cache._ref, q.data_ptr(), q_st, q_sh, hq, dt, t, *seqs, causal, d ** -0.5 if scale is None else scale,
+                 out.data_ptr(), o_st, o_sh, None if sums is None else sums.data_ptr(), None if prefix is None else prefix.data_ptr(),
+                 prefix_len, f, ws.data_ptr(), n, _stream(gpu))
     return (out, sums) if lse else out
 
 
@@ -176,7 +194,7 @@ def kv_attention_shared(q, cache, prefix, prefix_len, table, lens, cu=None, caus
     (int32 [pages]): every row sees them, then its sequence's own positions (table, lens: without the prefix). The prefix is
     read once for the whole batch."""
     prefix_len = int(prefix_len)
-    if prefix.ndim != 1 or prefix.dtype != torch.int32 or not prefix.is_contiguous() or prefix.device != q.device:
+    if prefix.ndim != 1 or prefix.dtype != torch.int32 or not prefix.is_contiguous() or prefix.get_device() != q.get_device():
         raise RuntimeError("kv_attention_shared: prefix must be contiguous int32 [pages] on q's GPU")
     if not 0 <= prefix_len <= prefix.numel() * cache.page:
         raise RuntimeError(f"kv_attention_shared: prefix_len {prefix_len} does not fit {prefix.numel()} pages of {cache.page}")

@@ -73,12 +73,11 @@ def test_no_rows_is_no_call():
 def test_workspace_holds_every_part():
     """More rows, positions or a prefix never need less; nothing to compute needs nothing."""
     size = nat.lib().rh3_kv_attention_workspace_bytes
-    d = ctypes.addressof(_desc())
-    assert size(d, 8, 0, 8, 2, 1, 0, 0) == 0 and size(None, 8, 2, 8, 2, 1, 0, 0) == 0 and size(d, 6, 2, 8, 2, 1, 0, 0) == 0
+    assert size(8, 4, 128, 0, 512, 2, 1, 0, 0) == 0 and size(6, 4, 128, 2, 512, 2, 1, 0, 0) == 0 and size(8, 0, 128, 2, 512, 2, 1, 0, 0) == 0
     for rows, batch, form in ((1, 1, 0), (64, 64, 0), (64, 2, 1), (64, 2, 2), (5000, 1, 0)):
-        n = size(d, 8, rows, 2000, batch, 1, 0, form)
-        assert size(d, 8, rows, 2000, batch, 1, 3000, form) > n
-        assert size(d, 8, rows, 2000, batch, 0, 0, form) >= n
+        n = size(8, 4, 128, rows, 128000, batch, 1, 0, form)
+        assert size(8, 4, 128, rows, 128000, batch, 1, 3000, form) > n
+        assert size(8, 4, 128, rows, 128000, batch, 0, 0, form) >= n
 
 
 def test_wrappers_refuse():
@@ -98,7 +97,7 @@ def test_wrappers_refuse():
         kv.KVCache(k, k.view(torch.float8_e4m3fn), s, s)
 
     class Cache:
-        heads, dim, page, device = 2, 128, 64, torch.device("cpu")
+        heads, dim, page, device, gpu = 2, 128, 64, torch.device("cpu"), -1
     x = torch.zeros((3, 2, 128), dtype=torch.bfloat16)
     t, n = torch.zeros((3, 1), dtype=torch.int32), torch.ones(3, dtype=torch.int32)
     with pytest.raises(RuntimeError, match="no CPU path"):
@@ -118,8 +117,8 @@ def test_wrappers_refuse():
     with pytest.raises(RuntimeError, match="prefix must be"):
         kv.kv_attention_shared(x, Cache, torch.zeros(2), 1, t, n)
     with pytest.raises(RuntimeError, match="table must be"):
-        kv._seqs("f", Cache, t.long(), n, None, x.device)
+        kv._seqs("f", Cache, t.long(), n, None, -1)
     with pytest.raises(RuntimeError, match="lens must be"):
-        kv._seqs("f", Cache, t, n[:2], None, x.device)
+        kv._seqs("f", Cache, t, n[:2], None, -1)
     with pytest.raises(RuntimeError, match="cu must be"):
-        kv._seqs("f", Cache, t, n, n, x.device)
+        kv._seqs("f", Cache, t, n, n, -1)
