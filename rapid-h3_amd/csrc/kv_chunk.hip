@@ -1,19 +1,31 @@
 // Attention of many query rows over the paged cache: a chunk of a prompt, the tokens of a frame, a whole batch against a prefix
 // that it shares.
 //
-// Bound by the matrix units and, close behind, by the vector instructions of the softmax: 4 dim flops per query row and key,
-// while a key's 2 (dim + 4) bytes serve all rows of a tile. A workgroup of 4 or 8 waves holds 32 query rows of one K/V head on
-// each and walks its keys 64 at a time. The tile's codes come to registers while the previous tile is computed, are converted to
-// f16 once for all waves and written to LDS (two buffers, one barrier to a tile): K as it is, V channel-major with its keys in
-// the order that the probabilities have. Per wave
+// 4 dim flops per query row and key, while a key's 2 (dim + 4) bytes serve all rows of a tile: bound by the matrix units and the
+// vector instructions of the softmax together, which share the card's power (both some 40 % busy at 1.7 GHz: 800 TFLOP/s at 2,048
+// rows x 32 heads on 8,192 + 2,048 keys, 710 at 1,560 rows x 56 heads on 22,332; a large f16 matrix product reaches 1,485).
+//
+// A workgroup of 4 or 8 waves holds 32 query rows of one K/V head on each and walks its keys 64 at a time. The keys' codes come
+// to registers a step ahead, are converted to f16 once for all waves and written to LDS (two buffers, one barrier to a step), K
+// and V alike. Per wave
 //   S^T = K Q^T (32x32x16 f16): a lane has one query row (l % 32) and 16 of 32 keys, so a row's softmax is in-lane but for one
 //   exchange, and only when its reference moves; the probabilities are the B operand of
-//   O^T = V^T P^T as they stand: k-step t of 32 keys takes keys 16 t + 4 (l / 32) + 0 .. 3 and those + 8.
-// Vector work per score: one fma (key scale, softmax scale and reference at once), half a max, the exponential, the sum and half a
-// conversion. For that, the query rows of a workgroup share one power of
-// two (an element 2^22 below the tile's largest loses low bits, 2^-33 of the largest at most, which is what an absolute error
-// of a score can be); and a value's scale, relative to a power of two over the largest seen, is multiplied into V as it is
-// converted (rounded to f16, 2^-11 at most, as the probabilities are).
+//   O^T = V^T P^T as they stand: k-step t of 32 keys takes keys 16 t + 4 (l / 32) + 0 .. 3 and those + 8, and V's operand comes
+//   from LDS by transposing loads.
+// The keys are taken by halves of 32: while one half's softmax runs, so do the MFMAs of the next half's scores and of the half
+// before's values, one MFMA to every one (dim 64: two) of the lane's 16 scores. Where keys are masked, a page is absent or a
+// reference has to move, a plain path does the half.
+// Vector work per score: one fma (key scale, softmax scale and reference at once), the exponential, the sum and half a
+// conversion. For that, the query rows of a workgroup share one power of two (an element 2^22 below the tile's largest loses low
+// bits, 2^-33 of the largest at most, which is what an absolute error of a score can be); a value's scale, relative to a power of
+// two over the largest of the share's keys (a scan of the scales before the first step), is multiplied into V as it is converted.
+// Roundings to f16: the probability, and the value times its scale; 2^-11 relative at most each, with fp32 sums.
+//
+// Tried and slower, or no faster: exponentials only beside the values' MFMAs (703 against 688 us for the first size above), the
+// next step's page entries looked up one by one behind the barrier (688 against 670), a load two steps ahead of the next one that
+// brings its lines to the L2 (723), the largest score in place of the probabilities' sum to find that a reference must move.
+#include <type_traits>
+
 #include "kv_attn.hpp"
 
 namespace rh3 {
@@ -21,6 +33,7 @@ namespace kv {
 namespace {
 
 constexpr int KT = CHUNK_KEYS;
+constexpr float SUM_STALE = 0x1p15f;  // up to this sum of a half's probabilities none of them is over 2^REF_STALE
 constexpr float NO_REF = -0x1p100f;   // reference of a row that has seen no key: any score moves it
 
 // 16-byte pieces of the LDS rows. Each row has one piece more than it needs, so that 16 rows' pieces of one number lie in all 16
@@ -46,6 +59,7 @@ __global__ void __launch_bounds__(WAVES * 64, 2) chunk_kernel(AttnArgs a) {
   __shared__ uint4 sv[2][KT * V_ROW<D>];
   __shared__ float sks[8][32];            // key scales of 8 half tiles in turn
   __shared__ float stop[WAVES], sscale[WAVES];
+  __shared__ int sgone[WAVES];
   const int lane = threadIdx.x & 63, l32 = lane & 31, hi = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   constexpr int NP = 8 / WAVES;           // pieces of 8 keys that a wave converts
@@ -101,6 +115,7 @@ __global__ void __launch_bounds__(WAVES * 64, 2) chunk_kernel(AttnArgs a) {
     h8_t q[KS];
     float qf;
     int vref;   // bits of a power of two, the same in all lanes
+    bool full;  // no key of the share in an absent page
     {
       const int64_t qat = (sq.first + tok) * a.q_st + hd * a.q_sh + 8 * hi;
       float top = 0.0f;
@@ -114,25 +129,31 @@ __global__ void __launch_bounds__(WAVES * 64, 2) chunk_kernel(AttnArgs a) {
       top = wave_max(top);
       // the largest finite scale of the share's values, 4 keys (of one page) to a thread at a time
       float big = 0.0f;
+      bool gone = false;
 #pragma unroll 4
       for (int key = t0 * KT + 4 * static_cast<int>(threadIdx.x); key < min(t1 * KT, sq.len); key += 4 * WAVES * 64) {
         const int page = page_in(table[min(key >> a.c.log2page, width - 1)]);
         const float4 v = *reinterpret_cast<const float4*>(a.c.vs + max(page, 0) * a.c.spage_stride + kvh * a.c.shead_stride + (key & mask));
         const float x[4] = {v.x, v.y, v.z, v.w};
+        gone |= page < 0;
 #pragma unroll
         for (int e = 0; e < 4; ++e) big = fmaxf(big, page >= 0 && key + e < sq.len && x[e] < INFINITY ? x[e] : 0.0f);
       }
       big = wave_max(big);
+      const int any = __builtin_amdgcn_ballot_w64(gone) != 0;
       if (lane == 0) {
         stop[wave] = top;
         sscale[wave] = big;
+        sgone[wave] = any;
       }
       __syncthreads();
 #pragma unroll
       for (int w = 0; w < WAVES; ++w) {
         top = fmaxf(top, stop[w]);
         big = fmaxf(big, sscale[w]);
+        gone |= sgone[w] != 0;
       }
+      full = __builtin_amdgcn_ballot_w64(gone) == 0;
       // V's reference: the largest code times its scale comes to 2^14 to 2^15; f16's range down from there is the smaller scales'
       vref = scalar(__float_as_int(pow2_over(big))) - ((FMT == INT8 ? 8 : 6) << 23);
       const int e = q_exponent(top);
@@ -161,9 +182,11 @@ __global__ void __launch_bounds__(WAVES * 64, 2) chunk_kernel(AttnArgs a) {
     // NP keys of a window, which lie in one page; lane l has 1 / 8 of key l / 8 of each 8.
     const int first = 8 * NP * wave;
     auto lookup = [&](int w) {   // the entry of the wave's page; the first window begins before the sequence
-      return scalar_load(table + min(max(w * KT - 32 + first, 0) >> a.c.log2page, width - 1));
+      // not by a scalar load: that, on its way, would make every wait for an LDS read a wait for all of them
+      return table[min(max(w * KT - 32 + first, 0) >> a.c.log2page, width - 1)];
     };
     auto all_there = [&](int s) {   // no key of step s in an absent page
+      if (full) return true;
       int bad = 0;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -218,26 +241,30 @@ __global__ void __launch_bounds__(WAVES * 64, 2) chunk_kernel(AttnArgs a) {
         sv[x & 1][key * V_ROW<D> + (lane & 7) * (D / 64) + c] = __builtin_bit_cast(uint4, v * f);
       }
     };
-    auto load_next = [&](int x) __attribute__((always_inline)) {
+    auto next_v = [&](int x) __attribute__((always_inline)) {   // (before next_k: the window's scales and page are K's of stage x)
 #pragma unroll
       for (int i = 0; i < NP; ++i) vs[i] = kvs[i];
       vpage = kpage;
-      kpage = page_in(entry);
-      entry = lookup(x + 3);
-      load_k(x + 2);
       load_codes(a.c.v, vpage, x + 1, vraw);
     };
-    auto stage = [&](int x) __attribute__((always_inline)) {
-#pragma unroll
-      for (int i = 0; i < 2 * NP; ++i) put_k(x, i);
+    auto next_k = [&](int x) __attribute__((always_inline)) {
+      kpage = page_in(scalar(entry));
+      entry = lookup(x + 3);
+      load_k(x + 2);
+    };
+    auto stage_v = [&](int x) __attribute__((always_inline)) {
 #pragma unroll
       for (int i = 0; i < 2 * NP; ++i) put_v(x, i);
-      load_next(x);
+      next_v(x);
+    };
+    auto stage_k = [&](int x) __attribute__((always_inline)) {
+#pragma unroll
+      for (int i = 0; i < 2 * NP; ++i) put_k(x, i);
+      next_k(x);
     };
 
-    // The products of a half tile's keys with the wave's rows, of values with probabilities, and in between a half tile's softmax:
-    // half h is scored while half h - 1's values are summed and half h + 1's products run, so that matrix and vector
-    // instructions always have each other's company. Step s does halves 2 s and 2 s + 1 with stage s.
+    // Half h's softmax runs beside the products of half h + 1 and the values of half h - 1. Step s does halves 2 s and 2 s + 1 with
+    // stage s.
     const f16_t zero = {};
     f16_t sa = zero, sb = zero;            // products of the next even and odd half
     h8_t p[2] = {};                        // probabilities of the last half
@@ -259,38 +286,68 @@ __global__ void __launch_bounds__(WAVES * 64, 2) chunk_kernel(AttnArgs a) {
       }
       return join(w[0], w[1], w[2], w[3]);
     };
-    // a KS-th of a half tile's scores less the row's reference, and their largest; a 2 DT-th of its probabilities
-    auto score = [&](const f16_t& s, const float4 (&kv)[4], int i, float (&y)[16], float& top) __attribute__((always_inline)) {
-      constexpr int N = 16 / KS;
+    // Half H of step s, its softmax spread evenly over the half's MFMAs; the sum of its probabilities. `side(i)` goes with MFMA i.
+    auto fast = [&](auto H, int b, int s, f16_t& now, f16_t& next, h8_t (&f)[AHEAD], float4 (&k0)[2], h8_t (&n)[2], auto side)
+                    __attribute__((always_inline)) {
+      constexpr int HALF = decltype(H)::value, MM = KS + 2 * DT, N = 16 / MM;
+      float4 k1[2];
+      float y[N], w[16], more = 0.0f;
+      auto score = [&](int e) __attribute__((always_inline)) {
+        const float4 k = e < 8 ? k0[e / 4] : k1[e / 4 - 2];
+        y[e % N] = fmaf(now[e], e % 4 == 0 ? k.x : e % 4 == 1 ? k.y : e % 4 == 2 ? k.z : k.w, -ref);
+      };
+      auto pair = [&](int e) __attribute__((always_inline)) {
+        more = e == 0 ? w[0] + w[1] : more + (w[e] + w[e + 1]);
+        const h2_t r = __builtin_bit_cast(h2_t, pack_h2(w[e], w[e + 1]));
+        uint32_t bits = __builtin_bit_cast(uint32_t, r);
+        asm volatile("" : "+v"(bits), "+v"(more));   // done here, not behind the last MFMA
+        const h2_t r2 = __builtin_bit_cast(h2_t, bits);
+        n[e / 8][e % 8] = r2[0];
+        n[e / 8][e % 8 + 1] = r2[1];
+      };
 #pragma unroll
-      for (int e = N * i; e < N * i + N; ++e) {
-        const float4 k = kv[e / 4];
-        y[e] = fmaf(s[e], e % 4 == 0 ? k.x : e % 4 == 1 ? k.y : e % 4 == 2 ? k.z : k.w, -ref);
+      for (int e = 0; e < N; ++e) score(e);
+#pragma unroll
+      for (int i = 0; i < MM; ++i) {
+        const int j = i - KS, r = i + AHEAD;
+        if (i < KS) next = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[i % AHEAD], q[i < KS ? i : 0], i ? next : zero, 0, 0, 0);
+        else o[j & (DT - 1)] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[i % AHEAD], p[(j < 0 ? 0 : j) / DT], o[j & (DT - 1)], 0, 0, 0);
+        if (r < KS) f[i % AHEAD] = k_at(b, HALF, r);
+        else if (r < MM) f[i % AHEAD] = v_at(b, HALF, r - KS);
+        else if (HALF == 0) f[i % AHEAD] = k_at(b, 1, r - MM);
+        if (i == MM / 8) {
+#pragma unroll
+          for (int c = 0; c < 2; ++c) k1[c] = *reinterpret_cast<const float4*>(&sks[(2 * s + HALF) & 7][8 * (c + 2) + 4 * hi]);
+        }
+        if (HALF == 0 && i == 5 * MM / 8) {
+#pragma unroll
+          for (int c = 0; c < 2; ++c) k0[c] = *reinterpret_cast<const float4*>(&sks[(2 * s + 1) & 7][8 * c + 4 * hi]);
+        }
+#pragma unroll
+        for (int e = i * N; e < i * N + N; ++e) w[e] = __builtin_amdgcn_exp2f(y[e % N]);
+        if (i + 1 < MM) {
+#pragma unroll
+          for (int e = (i + 1) * N; e < (i + 1) * N + N; ++e) score(e);
+        }
+        if (i * N >= 2 && (i * N) % 2 == 0) pair(i * N - 2);
+        side(i);
+        __builtin_amdgcn_sched_barrier(0);
       }
-#pragma unroll
-      for (int e = N * i; e < N * i + N; e += 2) top = max3(top, y[e], y[e + 1]);
-    };
-    auto probability = [&](float (&y)[16], int i, h8_t (&n)[2]) __attribute__((always_inline)) {
-      constexpr int N = 8 / DT;
-#pragma unroll
-      for (int e = N * i; e < N * i + N; e += 2) {
-        const float p0 = __builtin_amdgcn_exp2f(y[e]), p1 = __builtin_amdgcn_exp2f(y[e + 1]);
-        sum += p0 + p1;
-        const h2_t w = __builtin_bit_cast(h2_t, pack_h2(p0, p1));
-        n[e / 8][e % 8] = w[0];
-        n[e / 8][e % 8 + 1] = w[1];
-      }
+      pair(14);
+      return more;
     };
     bool there = all_there(t0);   // of the step at hand
     bool begun = false;           // the first step sets the references
     // Any half: keys that a row does not see hidden, the reference moved where it must be
-    auto slow = [&](int b, int s, int half, f16_t& now, f16_t& next) __attribute__((always_inline)) {
+    auto slow = [&](int b, int s, int half, bool made, f16_t& now, f16_t& next) __attribute__((always_inline)) {
       const int h = 2 * s + half;
+      if (!made) {
 #pragma unroll
-      for (int i = 0; i < 2 * DT; ++i) o[i % DT] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v_at(b, half, i), p[i / DT], o[i % DT], 0, 0, 0);
-      next = zero;
+        for (int i = 0; i < 2 * DT; ++i) o[i % DT] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v_at(b, half, i), p[i / DT], o[i % DT], 0, 0, 0);
+        next = zero;
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) next = __builtin_amdgcn_mfma_f32_32x32x16_f16(k_at(b, half, ks), q[ks], next, 0, 0, 0);
+        for (int ks = 0; ks < KS; ++ks) next = __builtin_amdgcn_mfma_f32_32x32x16_f16(k_at(b, half, ks), q[ks], next, 0, 0, 0);
+      }
       const int key0 = 32 * h + 4 * hi, m = lim - key0;
       uint32_t gone = 0;
       if (!there)
@@ -318,99 +375,68 @@ __global__ void __launch_bounds__(WAVES * 64, 2) chunk_kernel(AttnArgs a) {
 
     if (t0 < t1) {
       // stage t0 - 1 is only K of window t0
-      kpage = page_in(lookup(t0));
+      kpage = page_in(scalar(lookup(t0)));
       load_k(t0);
       entry = lookup(t0 + 1);
 #pragma unroll
       for (int i = 0; i < 2 * NP; ++i) put_k(t0 - 1, i);
-      load_next(t0 - 1);
+      next_v(t0 - 1);
+      next_k(t0 - 1);
       __syncthreads();
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) sa = __builtin_amdgcn_mfma_f32_32x32x16_f16(k_at((t0 - 1) & 1, 1, ks), q[ks], sa, 0, 0, 0);
-      stage(t0);
+      stage_v(t0);
+      stage_k(t0);
     }
     __syncthreads();
     int s = t0;
     while (s < t1) {
-      bool staged = false, odd = false;
+      // of the step at hand: V's and K's stage, the even half, the products of the half at hand
+      bool staged_v = false, staged_k = false, odd = false, made = false;
       // Steps whose every key every row sees. The accumulators stay in place in a loop of their own; a step's instructions stay
       // in the order written: behind each MFMA an operand's read for the one after next but two, and vector work that it covers.
       while (begun && there && s * KT + KT <= low) {
         const int b = s & 1;
+        constexpr int MM = KS + 2 * DT, EACH = MM / (4 * NP);
         h8_t f[AHEAD], n[2];
-        float4 kv[4];
-        float y[16], top;
+        float4 k0[2];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) kv[i] = *reinterpret_cast<const float4*>(&sks[(2 * s) & 7][8 * i + 4 * hi]);
+        for (int c = 0; c < 2; ++c) k0[c] = *reinterpret_cast<const float4*>(&sks[(2 * s) & 7][8 * c + 4 * hi]);
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i) f[i] = k_at(b, 0, i);
         __builtin_amdgcn_sched_barrier(0);
-        // the products of half 2 s + 1, the scores of half 2 s
-        top = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < KS; ++i) {
-          sb = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[i % AHEAD], q[i], i ? sb : zero, 0, 0, 0);
-          f[i % AHEAD] = i + AHEAD < KS ? k_at(b, 0, i + AHEAD) : v_at(b, 0, i + AHEAD - KS);
-          score(sa, kv, i, y, top);
-          __builtin_amdgcn_sched_barrier(0);
-        }
-        if (__builtin_amdgcn_ballot_w64(top > REF_STALE)) break;   // a reference has to move
-        // the values of half 2 s - 1, the probabilities of half 2 s
-#pragma unroll
-        for (int i = 0; i < 2 * DT; ++i) {
-          o[i % DT] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[i % AHEAD], p[i / DT], o[i % DT], 0, 0, 0);
-          f[i % AHEAD] = i + AHEAD < 2 * DT ? v_at(b, 0, i + AHEAD) : k_at(b, 1, i + AHEAD - 2 * DT);
-          probability(y, i, n);
-          if (i == 0) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) kv[j] = *reinterpret_cast<const float4*>(&sks[(2 * s + 1) & 7][8 * j + 4 * hi]);
-          }
-          __builtin_amdgcn_sched_barrier(0);
-        }
+        float more = fast(std::integral_constant<int, 0>(), b, s, sa, sb, f, k0, n, [&](int i) __attribute__((always_inline)) {
+          if (i >= MM / 2 && i % EACH == 0) put_v(s + 1, (i - MM / 2) / EACH);
+          if (i == MM - 1) next_v(s + 1);
+        });
+        staged_v = made = true;
+        if (__builtin_amdgcn_ballot_w64(more > SUM_STALE)) break;   // a reference has to move
+        sum += more;
         p[0] = n[0];
         p[1] = n[1];
         odd = true;
-        // the products of half 2 s + 2, the scores of half 2 s + 1, the next stage
-        top = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < KS; ++i) {
-          sa = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[i % AHEAD], q[i], i ? sa : zero, 0, 0, 0);
-          f[i % AHEAD] = i + AHEAD < KS ? k_at(b, 1, i + AHEAD) : v_at(b, 1, i + AHEAD - KS);
-          score(sb, kv, i, y, top);
-          if constexpr (D == 128) {   // (dim 64 has half as many MFMAs to a step: two parts to each)
-            if (i < 2 * NP) put_k(s + 1, i);
-            else if (i < 4 * NP) put_v(s + 1, i - 2 * NP);
-          } else {
-            if (2 * i < 2 * NP) { put_k(s + 1, 2 * i); put_k(s + 1, 2 * i + 1); }
-            else if (2 * i < 4 * NP) { put_v(s + 1, 2 * i - 2 * NP); put_v(s + 1, 2 * i + 1 - 2 * NP); }
-          }
-          __builtin_amdgcn_sched_barrier(0);
-        }
-        load_next(s + 1);
-        staged = true;
-        if (__builtin_amdgcn_ballot_w64(top > REF_STALE)) break;
-        // the values of half 2 s, the probabilities of half 2 s + 1
-#pragma unroll
-        for (int i = 0; i < 2 * DT; ++i) {
-          o[i % DT] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[i % AHEAD], p[i / DT], o[i % DT], 0, 0, 0);
-          if (i + AHEAD < 2 * DT) f[i % AHEAD] = v_at(b, 1, i + AHEAD);
-          probability(y, i, n);
-          __builtin_amdgcn_sched_barrier(0);
-        }
+        more = fast(std::integral_constant<int, 1>(), b, s, sb, sa, f, k0, n, [&](int i) __attribute__((always_inline)) {
+          if (i >= MM / 2 && i % EACH == 0) put_k(s + 1, (i - MM / 2) / EACH);
+          if (i == MM - 1) next_k(s + 1);
+        });
+        staged_k = true;
+        if (__builtin_amdgcn_ballot_w64(more > SUM_STALE)) break;
+        sum += more;
         p[0] = n[0];
         p[1] = n[1];
         __syncthreads();
-        staged = odd = false;
+        staged_v = staged_k = odd = made = false;
         there = all_there(++s);
         if (s >= t1) break;
       }
       if (s >= t1) break;
       const int b = s & 1;
       if ((s - 1) * KT < top_key) {   // (a step past the last key that a row sees sums its last values)
-        if (!odd) slow(b, s, 0, sa, sb);
-        slow(b, s, 1, sb, sa);
+        if (!odd) slow(b, s, 0, made, sa, sb);
+        slow(b, s, 1, made && odd, sb, sa);
       }
-      if (!staged) stage(s + 1);
+      if (!staged_v) stage_v(s + 1);
+      if (!staged_k) stage_k(s + 1);
       begun = true;
       __syncthreads();
       there = all_there(++s);

@@ -109,11 +109,6 @@ __device__ __forceinline__ float fmax_nc(float a, float b) {
   asm("v_max_f32 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
   return r;
 }
-__device__ __forceinline__ float max3(float a, float b, float c) {
-  float r;
-  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
-  return r;
-}
 __device__ __forceinline__ float max3_abs(float m, float a, float b) {
   float r;
   asm("v_max3_f32 %0, %1, |%2|, |%3|" : "=v"(r) : "v"(m), "v"(a), "v"(b));
@@ -280,21 +275,6 @@ __device__ __forceinline__ void lds_dma16_s(const void* sbase, uint32_t voff, ui
                : "=&s"(saved)
                : "v"(voff), "s"(sbase), "s"(lds_base)
                : "memory");
-}
-
-// ---------------------------------------------------------------- device: instruction order
-// Issue order of a run of N (LDS read, MFMA) pairs: the first A reads, then each MFMA followed by the next read,
-// then the last A MFMAs, so that every operand is read A MFMAs (>= 32 A pipe cycles) before its use. Left alone,
-// the scheduler places each read right before its MFMA and waits for it there.
-template <int N, int A>
-__device__ __forceinline__ void read_ahead() {
-  __builtin_amdgcn_sched_group_barrier(0x100, A, 0);  // 0x100: LDS reads
-#pragma unroll
-  for (int i = 0; i < N - A; ++i) {
-    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // 0x008: MFMA
-    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-  }
-  __builtin_amdgcn_sched_group_barrier(0x008, A, 0);
 }
 
 }  // namespace rh3

@@ -392,6 +392,33 @@ def test_extreme_scores_and_scales(dev, form, rows):
     _check_lse(lse, rl, err)
 
 
+@pytest.mark.parametrize("fmt", [I8, F8])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("rows,hkv,gap", [(600, 4, 70), (600, 4, 23), (100, 2, 45), (2, 2, 40)])
+def test_rising_scores(dev, fmt, dim, form, rows, hkv, gap):
+    """Scores that rise again and again along the keys, for some rows by far more than the weights' range, for others downwards or
+    not at all, and a page that is not there."""
+    page, n = 64, 1500
+    g = _gen(41)
+    u = torch.randn(dim, generator=g)
+    u = u / u.norm() * 8.0
+    rise = torch.cumsum((torch.rand(n, generator=g) < 1.0 / gap).float(), 0)
+    k = rise[:, None, None] * u + 0.3 * torch.randn(n, hkv, dim, generator=g)
+    v = torch.randn(n, hkv, dim, generator=g)
+    width = -(-n // page)
+    table = _tables(width, width, 1, 5)
+    c = kv.kv_cache(width, hkv, page, dim, fmt, dev)
+    kv.kv_write(c, k.to(dev), v.to(dev), _i32(table, dev), _i32([n], dev))
+    table[0][9] = -1
+    share = torch.tensor([0.3, 2.0, -1.0, 0.0])[torch.randint(0, 4, (rows, hkv), generator=g)]
+    q = (share[..., None] * u + 0.3 * torch.randn(rows, hkv, dim, generator=g)).to(BF).to(dev)
+    out, lse = kv.kv_attention(q, c, _i32(table, dev), _i32([n], dev), lse=True, causal=False, form=form)
+    ref, rl, mag, err = ok.attention(q, c, table, [n], None, False)
+    _check(out, ref, mag, err, 3.1)
+    _check_lse(lse, rl, err)
+
+
 def test_layouts(dev):
     """A cache that is a view of a buffer of several layers, strided queries and output, a wider table, out over q."""
     pages, heads, page, dim, hq = 9, 2, 32, 128, 6
