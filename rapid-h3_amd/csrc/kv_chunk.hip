@@ -23,7 +23,8 @@
 //
 // Tried and slower, or no faster: exponentials only beside the values' MFMAs (703 against 688 us for the first size above), the
 // next step's page entries looked up one by one behind the barrier (688 against 670), a load two steps ahead of the next one that
-// brings its lines to the L2 (723), the largest score in place of the probabilities' sum to find that a reference must move.
+// brings its lines to the L2 (723), the largest score in place of the probabilities' sum to find that a reference must move, 64
+// rows to each of 4 waves, which halves the reads of LDS but leaves one wave to a SIMD (915 against 670).
 #include <type_traits>
 
 #include "kv_attn.hpp"
@@ -116,55 +117,6 @@ __global__ void __launch_bounds__(WAVES * 64, 2) chunk_kernel(AttnArgs a) {
     float qf;
     int vref;   // bits of a power of two, the same in all lanes
     bool full;  // no key of the share in an absent page
-    {
-      const int64_t qat = (sq.first + tok) * a.q_st + hd * a.q_sh + 8 * hi;
-      float top = 0.0f;
-#pragma unroll
-      for (int s = 0; s < KS; ++s) {
-        float x[8];
-        load_q8(a, qat + 16 * s, x);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[e]) < INFINITY ? fabsf(x[e]) : 0.0f);
-      }
-      top = wave_max(top);
-      // the largest finite scale of the share's values, 4 keys (of one page) to a thread at a time
-      float big = 0.0f;
-      bool gone = false;
-#pragma unroll 4
-      for (int key = t0 * KT + 4 * static_cast<int>(threadIdx.x); key < min(t1 * KT, sq.len); key += 4 * WAVES * 64) {
-        const int page = page_in(table[min(key >> a.c.log2page, width - 1)]);
-        const float4 v = *reinterpret_cast<const float4*>(a.c.vs + max(page, 0) * a.c.spage_stride + kvh * a.c.shead_stride + (key & mask));
-        const float x[4] = {v.x, v.y, v.z, v.w};
-        gone |= page < 0;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) big = fmaxf(big, page >= 0 && key + e < sq.len && x[e] < INFINITY ? x[e] : 0.0f);
-      }
-      big = wave_max(big);
-      const int any = __builtin_amdgcn_ballot_w64(gone) != 0;
-      if (lane == 0) {
-        stop[wave] = top;
-        sscale[wave] = big;
-        sgone[wave] = any;
-      }
-      __syncthreads();
-#pragma unroll
-      for (int w = 0; w < WAVES; ++w) {
-        top = fmaxf(top, stop[w]);
-        big = fmaxf(big, sscale[w]);
-        gone |= sgone[w] != 0;
-      }
-      full = __builtin_amdgcn_ballot_w64(gone) == 0;
-      // V's reference: the largest code times its scale comes to 2^14 to 2^15; f16's range down from there is the smaller scales'
-      vref = scalar(__float_as_int(pow2_over(big))) - ((FMT == INT8 ? 8 : 6) << 23);
-      const int e = q_exponent(top);
-#pragma unroll
-      for (int s = 0; s < KS; ++s) {
-        float x[8];
-        load_q8(a, qat + 16 * s, x);
-        q[s] = q_f16(x, e);
-      }
-      qf = __builtin_amdgcn_ldexpf(a.scale_log2, -e);
-    }
     const int lim = causal ? min(sq.len, sq.len - sq.n + tok + 1) : sq.len;
     // of the wave's rows: keys that all see, keys that some see
     const int r0 = rt * R + wave * 32, r1 = min(rows - 1, r0 + 31);
@@ -220,6 +172,57 @@ __global__ void __launch_bounds__(WAVES * 64, 2) chunk_kernel(AttnArgs a) {
       }
       load_codes(a.c.k, kpage, w, kraw);
     };
+    if (t0 < t1) {   // the first loads, beside those of the query rows and the scales
+      kpage = page_in(scalar(lookup(t0)));
+      load_k(t0);
+      entry = lookup(t0 + 1);
+    }
+    {
+      const int64_t qat = (sq.first + tok) * a.q_st + hd * a.q_sh + 8 * hi;
+      float x[KS][8], top = 0.0f;
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        load_q8(a, qat + 16 * s, x[s]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[s][e]) < INFINITY ? fabsf(x[s][e]) : 0.0f);
+      }
+      top = wave_max(top);
+      // the largest finite scale of the share's values, 4 keys (of one page) to a thread at a time
+      float big = 0.0f;
+      bool gone = false;
+#pragma unroll 4
+      for (int key = t0 * KT + 4 * static_cast<int>(threadIdx.x); key < min(t1 * KT, sq.len); key += 4 * WAVES * 64) {
+        const int page = page_in(table[min(key >> a.c.log2page, width - 1)]);
+        const float4 v = *reinterpret_cast<const float4*>(a.c.vs + max(page, 0) * a.c.spage_stride + kvh * a.c.shead_stride + (key & mask));
+        const float x[4] = {v.x, v.y, v.z, v.w};
+        gone |= page < 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) big = fmaxf(big, page >= 0 && key + e < sq.len && x[e] < INFINITY ? x[e] : 0.0f);
+      }
+      big = wave_max(big);
+      const int any = __builtin_amdgcn_ballot_w64(gone) != 0;
+      if (lane == 0) {
+        stop[wave] = top;
+        sscale[wave] = big;
+        sgone[wave] = any;
+      }
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < WAVES; ++w) {
+        top = fmaxf(top, stop[w]);
+        big = fmaxf(big, sscale[w]);
+        gone |= sgone[w] != 0;
+      }
+      full = __builtin_amdgcn_ballot_w64(gone) == 0;
+      // V's reference: the largest code times its scale comes to 2^14 to 2^15; f16's range down from there is the smaller scales'
+      vref = scalar(__float_as_int(pow2_over(big))) - ((FMT == INT8 ? 8 : 6) << 23);
+      const int e = q_exponent(top);
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        q[s] = q_f16(x[s], e);
+      }
+      qf = __builtin_amdgcn_ldexpf(a.scale_log2, -e);
+    }
     // Stage x (loaded) to LDS in 2 NP parts of K and 2 NP of V; the loads of stage x + 1
     auto put_k = [&](int x, int part) __attribute__((always_inline)) {
       const int i = part / 2, c = part % 2, key = first + 8 * i + (lane >> 3);
@@ -375,9 +378,6 @@ __global__ void __launch_bounds__(WAVES * 64, 2) chunk_kernel(AttnArgs a) {
 
     if (t0 < t1) {
       // stage t0 - 1 is only K of window t0
-      kpage = page_in(scalar(lookup(t0)));
-      load_k(t0);
-      entry = lookup(t0 + 1);
 #pragma unroll
       for (int i = 0; i < 2 * NP; ++i) put_k(t0 - 1, i);
       next_v(t0 - 1);
