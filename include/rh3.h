@@ -484,7 +484,8 @@ typedef struct rh3_kv_cache {
 
 /* Quantizes rows of k and v (bf16, fp16 or fp32) into their positions: s = max(amax / QMAX, 1e-12) (127 or 448), code =
  * round_half_even(x / s); a row with an infinity or a NaN gets s = NaN and codes 0. Rows whose position is negative or in an
- * absent page are skipped. A position that several rows of one call name holds codes and scale of any of them. */
+ * absent page are skipped. A position that several rows of one call name (a page that two sequences share, or that a table
+ * names twice) ends with a mixture of them: name each position written once. */
 int rh3_kv_write(const rh3_kv_cache* cache, const void* k, int64_t k_st, int64_t k_sh, const void* v, int64_t v_st,
                  int64_t v_sh, int dtype, int64_t rows, const int32_t* table, int64_t table_stride, int64_t width,
                  const int32_t* lens, const int32_t* cu, int64_t batch, hipStream_t stream);
@@ -501,8 +502,9 @@ int rh3_kv_read(const rh3_kv_cache* cache, void* k, int64_t k_st, int64_t k_sh, 
  * prefix[], which come before the sequences' own and are read once for the batch. out may lie exactly over q. form: the
  * kernel for few query rows to a K/V head (RH3_KV_TOKEN) or for many (RH3_KV_CHUNK), or by the sizes, where the table's width
  * stands for the lengths, which only the device knows.
- * The workspace (capacity: width * page; even: 1 where cu is NULL) holds the parts of rows whose keys several workgroups share; how keys are split depends on the sizes, lengths
- * and the CU count, and with it the last bits of the result; the same call gives the same bits. */
+ * The workspace (capacity: width * page; even: 1 where cu is NULL) holds the parts of rows whose keys several workgroups share;
+ * how keys are split depends on the sizes, lengths and the CU count, and with it the last bits of the result; the same call
+ * gives the same bits. */
 int64_t rh3_kv_attention_workspace_bytes(int64_t q_heads, int64_t heads, int64_t dim, int64_t rows, int64_t capacity,
                                          int64_t batch, int even, int64_t prefix_len, int form);
 int rh3_kv_attention(const rh3_kv_cache* cache, const void* q, int64_t q_st, int64_t q_sh, int64_t q_heads, int dtype,

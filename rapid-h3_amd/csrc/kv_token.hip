@@ -1,15 +1,18 @@
 // Attention of few query rows over the paged cache: single tokens of a batch, or a few tokens each.
 //
-// Bound by the cache's bytes: 2 (dim + 4) per K/V head and position. A wave takes 32 keys at a time, for 16 query rows of the K/V
-// head (32 at dim 64: at 128 their accumulators leave no registers for the loads, and 2 x 16 rows, the second time mostly from
-// L2, took 164 us where 32 took 230: 8 sequences of 4 tokens x 56 / 8 heads x 32,768 keys), straight from memory to registers, and its matrix instructions' operand order is made to fit what a wide load
+// Bound by the cache's bytes: 2 (dim + 4) per K/V head and position. Measured: 64 sequences of up to 8,190 keys x 8 K/V heads of
+// 128 (0.37 GB) in 77 us, 4.9 TB/s; 4 of 131,071 keys (1.1 GB) in 190 us, 5.8 TB/s; a large copy moves 4.8, a fill 6.8.
+//
+// A wave takes 32 keys at a time, for 16 query rows of the K/V head (32 at dim 64: at 128 their accumulators leave no registers for
+// the loads, and 2 x 16 rows, the second time mostly from L2, took 164 us where 32 took 230: 8 sequences of 4 tokens x 56 / 8 heads
+// x 32,768 keys), straight from memory to registers, and its matrix instructions' operand order is made to fit what a wide load
 // brings, so nothing passes through LDS:
 //   S^T = K Q^T: lane l holds key l % 16, two (one) 16-byte pieces of its row; the channel order this gives each MFMA step is
 //   given to Q as well. The result has the query row in l % 16 and keys 4 (l / 16) + 0 .. 3 in the registers of both 16-key tiles.
 //   O^T = V^T P^T: those keys are the ones whose P a lane now has; it loads the same keys' values, dim / 16 channels each, and
 //   turns bytes into channel-major f16 by permutes as it converts.
-// Each tile's registers take the next one as they are used up. A workgroup's 4 waves take a share's tiles in turn and join through LDS
-// at the end of an item; items that more than one workgroup has worked on are left as parts.
+// Each tile's registers take the next one as they are used up. A workgroup's 4 waves take a share's tiles in turn and join through
+// LDS at the end of an item; items that more than one workgroup has worked on are left as parts.
 #include "kv_attn.hpp"
 
 namespace rh3 {
@@ -89,8 +92,10 @@ __device__ __forceinline__ h8_t to_f16(const float (&y)[8]) {
               __builtin_bit_cast(h2_t, pack_h2(y[4], y[5])), __builtin_bit_cast(h2_t, pack_h2(y[6], y[7])));
 }
 
-// One tile. FINE (fp16 results, whose own rounding is no coarser than that of the weights): the weights in two f16 terms. MORE: the wave's next tile (pages `pn`) is loaded into the same registers, its keys as soon as these are used, its
-// values at the end: a load has about half a tile's work to come in.
+// One tile. The weights are rounded to f16 (2^-11 at most), or, FINE, to two f16 terms: for fp16 results, whose own rounding is no
+// coarser than one (error 4.0e-4 -> 2.1e-4 of the largest, that of the result's rounding; bf16 results round by up to 2^-8). MORE: the
+// wave's next tile (pages `pn`) is loaded into the same registers, its keys as soon as these are used, its values at the end: a load
+// has about half a tile's work to come in.
 template <int FMT, int D, int MT, bool FINE, bool MORE>
 __device__ __forceinline__ void compute(const AttnArgs& a, Tile<D>& t, int kvh, int tile, const Pages& pg, const Pages& pn,
                                         const h8_t (&q)[MT][D / 32], const float (&qf)[MT], const int (&lim)[MT], int low, int len,

@@ -29,7 +29,8 @@ _HERE = contextlib.nullcontext()
 class KVCache:
     """The pages of one layer: k, v [P, heads, page, dim] int8 or float8_e4m3fn codes, k_scale, v_scale [P, heads, page]
     fp32 (page 16 to 256, a power of two; dim 64 or 128; views of larger buffers whose pages and heads lie apart are fine,
-    k like v and k_scale like v_scale). A scale is finite and not negative, or NaN. The tensors are kept and used as they are."""
+    k like v and k_scale like v_scale). Where a position holds something, no code is NaN and a scale is finite and not
+    negative, or NaN for a row that is (as kv_write leaves them). The tensors are kept and used as they are."""
 
     __slots__ = ("k", "v", "k_scale", "v_scale", "pages", "heads", "page", "dim", "device", "gpu", "_desc", "_ref")
 
@@ -120,8 +121,8 @@ def _rows_call(name, entry, what, cache, k, v, table, lens, cu):
 
 def kv_write(cache, k, v, table, lens, cu=None):
     """Quantise rows k, v [rows, heads, dim] (bf16, fp16 or fp32, strided ok) into their positions. Rows at a negative
-    position or in an absent page are skipped; a row that holds an infinity or a NaN is kept as NaN (its scale). Pages that
-    sequences share must not be written by more than one of them in a call."""
+    position or in an absent page are skipped; a row that holds an infinity or a NaN is kept as NaN (its scale). A position
+    that two rows of a call name (a page that sequences share, or that a table names twice) ends with a mixture of them."""
     _rows_call("kv_write", "rh3_kv_write", ("k", "v"), cache, k, v, table, lens, cu)
 
 
