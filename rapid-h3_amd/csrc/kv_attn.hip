@@ -60,8 +60,8 @@ struct Sums {
 };
 
 // Every query row of the call, WPR waves to one: where a row has many parts (few items on all workgroups), or a prefix's beside its
-// own (of the same launch, or of `prefix`). Bound by latency: a row's parts are a few KB to some hundred (4 rows x 56 heads in 256
-// parts each 5.5 us; 64 x 32 with a prefix's 33 parts each, 38 MB, 19).
+// own (of the same launch, or of `prefix`). Bound by latency: a row's parts are a few KB to some hundred (4 rows x 56 heads in 16
+// parts 5.5 us; 64 x 32 with a prefix's 33 parts each, 38 MB, 13).
 template <int D, int WPR>
 __global__ void __launch_bounds__(WPR > 4 ? WPR * 64 : 256) join_rows_kernel(Source own, Source prefix, int has_prefix) {
   constexpr int WAVES = WPR > 4 ? WPR : 4, EPL = D / 64;
@@ -188,17 +188,18 @@ struct Plan {
 
 // rows: of a call; per sequence they are counted as even. keep: a part for every item.
 // The token kernel reads the keys once for every 16 (dim 64: 32) query rows of a K/V head, at some 6.8 TB/s, mostly from L2 from
-// the second time on; the chunk kernel once for 128 or 256, as 3 TB/s at most (it is bound by its arithmetic), after some 40 us
-// that its longer beginning, end and joins take. The lengths are the device's: the table's width stands for them. Measured (us,
-// token / chunk, 8 K/V heads of 128): 28 rows of 8 sequences x 32,768 keys 164 / 222, 49 rows of them 304 / 217, 49 rows of 8 x up
-// to 2,048 24 / 51, 96 rows of 2 x 16,384 61 / 83.
+// the second time on; the chunk kernel once for 128 or 256, as 3 TB/s at most (it is bound by its arithmetic), after some 34 us
+// that its longer beginning, end and joins take. The lengths are the device's: the table's width stands for them. Measured (us a
+// call, token / chunk, 8 K/V heads of 128, rows of a K/V head): 1 sequence of 16,384 keys: 32 rows 24 / 39, 96 41 / 49, 128 45 / 53,
+// 192 58 / 47, 256 67 / 53; 16 of 4,096: 32 50 / 66, 48 68 / 71, 64 82 / 73, 96 121 / 80; 4 of 65,536: 32 140 / 188, 48 285 / 197;
+// 4 of 1,024: 16 16 / 37, 256 24 / 49. Heads of 64: 1 of 65,536: 128 60 / 70, 192 81 / 80, 256 103 / 87; 4: 96 150 / 158, 128 186 / 169.
 Plan plan_of(int64_t rows, int64_t batch, bool even, int64_t group, int64_t heads, int64_t dim, int64_t cap, bool keep, int form) {
   const int64_t cus = device_cus() > 0 ? device_cus() : 256;
   const int64_t mean = (rows * group + batch - 1) / batch;    // query rows of a sequence's K/V head
   const int small = dim == 64 && mean > 16 ? 32 : 16;
   const double mb = 2e-6 * static_cast<double>(dim + 4) * static_cast<double>(batch * heads) * static_cast<double>(cap);
   Plan p{};
-  p.chunk = form != RH3_KV_BY_SIZE ? form == RH3_KV_CHUNK : static_cast<double>((mean + small - 1) / small) * mb / 6.8 > 40.0 + static_cast<double>((mean + 127) / 128) * mb / 3.0;
+  p.chunk = form != RH3_KV_BY_SIZE ? form == RH3_KV_CHUNK : static_cast<double>((mean + small - 1) / small) * mb / 6.8 > 34.0 + static_cast<double>((mean + 127) / 128) * mb / 3.0;
   p.rows = !p.chunk ? small : mean <= 128 ? 128 : 256;
   p.wgs = static_cast<int>(p.rows == 256 ? cus : 2 * cus);
   p.items = !keep ? 0 : heads * (even ? batch * ((rows / batch * group + p.rows - 1) / p.rows) : rows * group / p.rows + batch);
@@ -323,7 +324,10 @@ extern "C" int rh3_kv_attention(const rh3_kv_cache* cache, const void* q, int64_
   launch(own.a, call.own, fmt, dim, stream);
   if (const int e = launch_status("kv_attention")) return e;
   // Parts that a row may have: the workgroups over the least count of items, no more than the keys make. Measured (kernel us, by
-  // shares / rows on 4 waves / on 16): 8 parts of 32 rows 5.1 / 4.7 / 5.7, 16 of 224 rows - / 6.3 / 7.7.
+  // shares / rows on 4 waves / on 16): 8 parts of 32 rows 5.1 / 4.7 / 5.7, 16 of 224 rows - / 6.3 / 7.7. Waves of one row each find
+  // their way through the shares themselves, so many rows, which fill the chip, have one (us, rows on 1 wave / on 4): 192 rows
+  // behind a prefix 7.9 / 6.1, 512 21.2 / 20.8 (whole calls, as those that follow), 768 21.6 / 22.1, 1,024 24.8 / 26.2, 1,536 29.5 /
+  // 32.4; 2,048 of 33 parts 13.5 / 19.2; 4,096 of 16 parts 72 / 78 (whole calls).
   const int64_t ids = rows * q_heads, cap = width * cache->page + prefix_len;
   const int64_t tiles = (rows * a.group / batch + call.own.rows - 1) / call.own.rows;
   const int64_t shared = call.own.wgs / (batch * a.c.heads * (tiles > 0 ? tiles : 1));
@@ -335,7 +339,7 @@ extern "C" int rh3_kv_attention(const rh3_kv_cache* cache, const void* q, int64_
     else hipLaunchKernelGGL((join_shares_kernel<64>), grid, dim3(256), 0, stream, own);
     return launch_status("kv_attention (join)");
   }
-  const int wpr = parts > 32 ? 16 : ids <= 16384 ? 4 : 1;
+  const int wpr = parts > 32 ? 16 : ids <= 2 * device_cus() ? 4 : 1;
   const int64_t grid = wpr == 1 ? (ids + 3) / 4 : ids;
   RH3_REQUIRE(grid * (wpr == 16 ? 4 : 1) <= MAX_GRID_256, "kv_attention: %lld rows in one call", static_cast<long long>(rows));
   auto go = [&](auto kernel) {

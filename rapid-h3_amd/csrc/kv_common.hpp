@@ -144,6 +144,20 @@ __device__ __forceinline__ void f16x8_across(const uint32_t (&w)[8], h8_t (&o)[N
 }
 
 // ---------------------------------------------------------------- rows of bf16 / fp16 / fp32
+template <int DT>   // bf16 or fp16
+__device__ __forceinline__ void row8(const uint4 r, float* v) {
+  if constexpr (DT == RH3_DTYPE_BF16) {
+    unpack8(r, v);
+  } else {
+    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const h2_t h = __builtin_bit_cast(h2_t, w[i]);
+      v[2 * i] = static_cast<float>(h[0]);
+      v[2 * i + 1] = static_cast<float>(h[1]);
+    }
+  }
+}
 template <int DT>
 __device__ __forceinline__ void load_row8(const void* p, int64_t at, float* v) {
   if constexpr (DT == RH3_DTYPE_F32) {
@@ -151,18 +165,7 @@ __device__ __forceinline__ void load_row8(const void* p, int64_t at, float* v) {
     const float4 b = reinterpret_cast<const float4*>(static_cast<const float*>(p) + at)[1];
     v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
   } else {
-    const uint4 r = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + at);
-    if constexpr (DT == RH3_DTYPE_BF16) {
-      unpack8(r, v);
-    } else {
-      const uint32_t w[4] = {r.x, r.y, r.z, r.w};
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const h2_t h = __builtin_bit_cast(h2_t, w[i]);
-        v[2 * i] = static_cast<float>(h[0]);
-        v[2 * i + 1] = static_cast<float>(h[1]);
-      }
-    }
+    row8<DT>(*reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + at), v);
   }
 }
 __device__ __forceinline__ uint32_t pack_h2(float a, float b) {   // round to nearest even

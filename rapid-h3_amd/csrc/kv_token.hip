@@ -1,7 +1,7 @@
 // Attention of few query rows over the paged cache: single tokens of a batch, or a few tokens each.
 //
 // Bound by the cache's bytes: 2 (dim + 4) per K/V head and position. Measured: 64 sequences of up to 8,190 keys x 8 K/V heads of
-// 128 (0.37 GB) in 77 us, 4.9 TB/s; 4 of 131,071 keys (1.1 GB) in 190 us, 5.8 TB/s; a large copy moves 4.8, a fill 6.8.
+// 128 (0.37 GB) in 74 us, 5.0 TB/s; 4 of 131,071 keys (1.1 GB) in 188 us, 5.9 TB/s; a large copy moves 4.8, a fill 6.8.
 //
 // A wave takes 32 keys at a time, for 16 query rows of the K/V head (32 at dim 64: at 128 their accumulators leave no registers for
 // the loads, and 2 x 16 rows, the second time mostly from L2, took 164 us where 32 took 230: 8 sequences of 4 tokens x 56 / 8 heads
@@ -264,19 +264,35 @@ __global__ void __launch_bounds__(NT, 2) token_kernel(AttnArgs a) {
     const int rows = sq.n * a.group;
 
     // query rows: lane l holds row l % 16, channels 64 c + 16 (l / 16) + 0 .. 15 in steps 2 c and 2 c + 1
-    h8_t q[MT][D / 32];
-    float qf[MT];
+    uint4 raw[MT][D / 32];
     int lim[MT];
+    int t = t0 + wave;
+    Pages pg = pages_of(a, row, width, t), pn = pages_of(a, row, width, t + WAVES);
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
       const int row = rt * R + 16 * m + l16;
-      const bool has = row < rows;
-      const int rr = has ? row : 0;
+      const int rr = row < rows ? row : 0;
       const int tok = rr / a.group, hd = kvh * a.group + rr - tok * a.group;
+      const uint16_t* src = static_cast<const uint16_t*>(a.q) + (sq.first + tok) * a.q_st + hd * a.q_sh + 16 * g;
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c) raw[m][c] = *reinterpret_cast<const uint4*>(src + 64 * (c >> 1) + 8 * (c & 1));
+      lim[m] = causal ? min(sq.len, sq.len - sq.n + tok + 1) : sq.len;
+    }
+    // the first keys and values are on their way while the query rows come in
+    Tile<D> tile;
+    if (t < t1) {
+      load_keys<D>(a, kvh, t, pg, tile);
+      load_values<D>(a, kvh, t, pg, tile);
+    }
+    h8_t q[MT][D / 32];
+    float qf[MT];
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      const bool has = rt * R + 16 * m + l16 < rows;
       float x[D / 32][8], top = 0.0f;
 #pragma unroll
       for (int c = 0; c < D / 32; ++c) {
-        load_q8(a, (sq.first + tok) * a.q_st + hd * a.q_sh + 64 * (c >> 1) + 16 * g + 8 * (c & 1), x[c]);
+        row8<FINE ? RH3_DTYPE_F16 : RH3_DTYPE_BF16>(raw[m][c], x[c]);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           x[c][e] = has ? x[c][e] : 0.0f;
@@ -287,7 +303,6 @@ __global__ void __launch_bounds__(NT, 2) token_kernel(AttnArgs a) {
 #pragma unroll
       for (int c = 0; c < D / 32; ++c) q[m][c] = q_f16(x[c], e);
       qf[m] = __builtin_amdgcn_ldexpf(a.scale_log2, -e);
-      lim[m] = causal ? min(sq.len, sq.len - sq.n + tok + 1) : sq.len;
     }
     const int low = causal ? min(sq.len, sq.len - sq.n + scalar((rt * R) / a.group) + 1) : sq.len;
 
@@ -301,12 +316,7 @@ __global__ void __launch_bounds__(NT, 2) token_kernel(AttnArgs a) {
 #pragma unroll
       for (int i = 0; i < D / 16; ++i) st.o[m][i] = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
     }
-    int t = t0 + wave;
     if (t < t1) {
-      Tile<D> tile;
-      Pages pg = pages_of(a, row, width, t), pn = pages_of(a, row, width, t + WAVES);
-      load_keys<D>(a, kvh, t, pg, tile);
-      load_values<D>(a, kvh, t, pg, tile);
       for (; t + WAVES < t1; t += WAVES) {
         const Pages p2 = pages_of(a, row, width, t + 2 * WAVES);
         compute<FMT, D, MT, FINE, true>(a, tile, kvh, t, pg, pn, q, qf, lim, low, sq.len, st);
