@@ -21,7 +21,10 @@
 // conversion. For that, the query rows of a workgroup share one power of two (an element 2^22 below the tile's largest loses low
 // bits, 2^-33 of the largest at most, which is what an absolute error of a score can be); a value's scale, relative to a power of
 // two over the largest of the share's keys (a scan of the scales before the first step), is multiplied into V as it is converted.
-// Roundings to f16: the probability, and the value times its scale; 2^-11 relative at most each, with fp32 sums.
+// Roundings to f16: the probability, and the value times its scale; 2^-11 relative at most each, with fp32 sums, beside a bf16
+// result's own 2^-8. FINE, for fp16 results, whose own rounding is no coarser: the scale is multiplied into the probability, which
+// is kept in two f16 terms (error of 300 rows on 3,000 keys 4.0e-4 -> 2.1e-4, that of the result's rounding; the first size
+// above 545 -> 730 us, the last 67 -> 79).
 //
 // Tried and slower, or no faster: exponentials only beside the values' MFMAs (703 against 688 us for the first size above), the
 // next step's page entries looked up one by one behind the barrier (688 against 670), a load two steps ahead of the next one that
@@ -54,13 +57,14 @@ __device__ __forceinline__ h4_t lds_read_tr(const uint8_t* p) {
   return __builtin_bit_cast(h4_t, __builtin_amdgcn_ds_read_tr16_b64_v4f16((__attribute__((address_space(3))) g4_t*)p));
 }
 
-template <int FMT, int D, int WAVES>
+template <int FMT, int D, int WAVES, bool FINE>
 __global__ void __launch_bounds__(WAVES * 64, 2) chunk_kernel(AttnArgs a) {
   constexpr int R = WAVES * 32, KS = D / 16, DT = D / 32;
   const Tiling TILING = tiling(true, R);
   __shared__ uint4 sk[2][KT * K_ROW<D>];
   __shared__ uint4 sv[2][KT * V_ROW<D>];
   __shared__ float sks[8][32];            // key scales of 8 half tiles in turn
+  __shared__ float svs[FINE ? 8 : 1][32]; // value scales of them
   __shared__ float stop[WAVES], sscale[WAVES];
   __shared__ int sgone[WAVES];
   const int lane = threadIdx.x & 63, l32 = lane & 31, hi = lane >> 5;
@@ -217,7 +221,7 @@ __global__ void __launch_bounds__(WAVES * 64, 2) chunk_kernel(AttnArgs a) {
       }
       full = __builtin_amdgcn_ballot_w64(gone) == 0;
       // V's reference: the largest code times its scale comes to 2^14 to 2^15; f16's range down from there is the smaller scales'
-      vref = scalar(__float_as_int(pow2_over(big))) - ((FMT == INT8 ? 8 : 6) << 23);
+      vref = scalar(__float_as_int(pow2_over(big))) - (FINE ? 0 : (FMT == INT8 ? 8 : 6) << 23);
       const int e = q_exponent(top);
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
@@ -226,24 +230,28 @@ __global__ void __launch_bounds__(WAVES * 64, 2) chunk_kernel(AttnArgs a) {
       qf = __builtin_amdgcn_ldexpf(a.scale_log2, -e);
     }
     // Stage x (loaded) to LDS in 2 NP parts of K and 2 NP of V; the loads of stage x + 1
+    const float vinv = pow2_inverse(vref);
     auto put_k = [&](int x, int part) __attribute__((always_inline)) {
-      const int i = part / 2, c = part % 2, key = first + 8 * i + (lane >> 3);
+      const int i = part / 2, c = part % 2, key = first + 8 * i + (lane >> 3), h = (2 * x + 1 + (key >> 5)) & 7;
+      if constexpr (FINE) {
+        if (c == 0) svs[h][key & 31] = kvs[i] < INFINITY ? kvs[i] * vinv : 0.0f;
+      }
       // a NaN value would reach rows that do not see its key (0 x NaN): its key is made NaN
-      if (c == 0) sks[(2 * x + 1 + (key >> 5)) & 7][key & 31] = fmaf(kvs[i], 0.0f, ks[i] * qf);
+      if (c == 0) sks[h][key & 31] = fmaf(kvs[i], 0.0f, ks[i] * qf);
       if (c < D / 64)
         sk[x & 1][key * K_ROW<D> + (lane & 7) * (D / 64) + c] = __builtin_bit_cast(uint4, f16x8<FMT>(kraw[i][2 * c], kraw[i][2 * c + 1]));
     };
-    const float vinv = pow2_inverse(vref);
     auto put_v = [&](int x, int part) __attribute__((always_inline)) {
       const int i = part / 2, c = part % 2, key = first + 8 * i + (lane >> 3);
       // outside the share's keys and in an absent page there may be anything: 0 (and codes that can be NaN go)
       const int pos = x * KT - 32 + key;
       const bool here = vpage >= 0 && pos >= t0 * KT && pos < min(sq.len, t1 * KT);
-      const _Float16 f = static_cast<_Float16>(here && vs[i] < INFINITY ? vs[i] * vinv : 0.0f);
+      [[maybe_unused]] const _Float16 f = static_cast<_Float16>(here && vs[i] < INFINITY ? vs[i] * vinv : 0.0f);
       if (c < D / 64) {
         const bool keep = FMT == INT8 || here;
         const h8_t v = f16x8<FMT>(keep ? vraw[i][2 * c] : 0u, keep ? vraw[i][2 * c + 1] : 0u);
-        sv[x & 1][key * V_ROW<D> + (lane & 7) * (D / 64) + c] = __builtin_bit_cast(uint4, v * f);
+        if constexpr (FINE) sv[x & 1][key * V_ROW<D> + (lane & 7) * (D / 64) + c] = __builtin_bit_cast(uint4, v);
+        else sv[x & 1][key * V_ROW<D> + (lane & 7) * (D / 64) + c] = __builtin_bit_cast(uint4, v * f);
       }
     };
     auto next_v = [&](int x) __attribute__((always_inline)) {   // (before next_k: the window's scales and page are K's of stage x)
@@ -272,7 +280,7 @@ __global__ void __launch_bounds__(WAVES * 64, 2) chunk_kernel(AttnArgs a) {
     // stage s.
     const f16_t zero = {};
     f16_t sa = zero, sb = zero;            // products of the next even and odd half
-    h8_t p[2] = {};                        // probabilities of the last half
+    h8_t p[2] = {}, pr[2] = {};   // weights of the last half, what their rounding left
     constexpr int AHEAD = 4;
     auto k_at = [&](int b, int half, int ks) { return __builtin_bit_cast(h8_t, sk[b][(32 * half + l32) * K_ROW<D> + hi + 2 * ks]); };
     const uint8_t* v_lane = reinterpret_cast<const uint8_t*>(sv) + (4 * hi + ((lane & 15) >> 2)) * V_ROW<D> * 16 + ((lane >> 4) & 1) * 32 + (lane & 3) * 8;
@@ -281,21 +289,30 @@ __global__ void __launch_bounds__(WAVES * 64, 2) chunk_kernel(AttnArgs a) {
       const h4_t lo = lds_read_tr(at), up = lds_read_tr(at + 8 * V_ROW<D> * 16);
       return __builtin_shufflevector(lo, up, 0, 1, 2, 3, 4, 5, 6, 7);
     };
-    auto probabilities = [&](const float* y) __attribute__((always_inline)) {   // of 8 keys, added to the sum
-      h2_t w[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float p0 = __builtin_amdgcn_exp2f(y[2 * e]), p1 = __builtin_amdgcn_exp2f(y[2 * e + 1]);
-        sum += p0 + p1;
-        w[e] = __builtin_bit_cast(h2_t, pack_h2(p0, p1));
+    // Weights of two keys to f16; FINE: times their values' scales, in two terms
+    auto weights = [&](float w0, float w1, float v0, float v1, uint32_t& rest) __attribute__((always_inline)) {
+      if constexpr (FINE) {
+        w0 *= v0;
+        w1 *= v1;
       }
-      return join(w[0], w[1], w[2], w[3]);
+      const uint32_t w = pack_h2(w0, w1);
+      if constexpr (FINE) {
+        const h2_t r = __builtin_bit_cast(h2_t, w);
+        rest = pack_h2(w0 - static_cast<float>(r[0]), w1 - static_cast<float>(r[1]));
+      }
+      return w;
+    };
+    auto set2 = [](h8_t (&x)[2], int e, uint32_t w) __attribute__((always_inline)) {
+      const h2_t r = __builtin_bit_cast(h2_t, w);
+      x[e / 8][e % 8] = r[0];
+      x[e / 8][e % 8 + 1] = r[1];
     };
     // Half H of step s, its softmax spread evenly over the half's MFMAs; the sum of its probabilities. `side(i)` goes with MFMA i.
-    auto fast = [&](auto H, int b, int s, f16_t& now, f16_t& next, h8_t (&f)[AHEAD], float4 (&k0)[2], h8_t (&n)[2], auto side)
-                    __attribute__((always_inline)) {
+    auto fast = [&](auto H, int b, int s, f16_t& now, f16_t& next, h8_t (&f)[AHEAD], float4 (&k0)[2], h8_t (&n)[2], h8_t (&nr)[2],
+                    auto side) __attribute__((always_inline)) {
       constexpr int HALF = decltype(H)::value, MM = KS + 2 * DT, N = 16 / MM;
       float4 k1[2];
+      [[maybe_unused]] float4 v4;   // value scales of the 4 keys at hand
       float y[N], w[16], more = 0.0f;
       auto score = [&](int e) __attribute__((always_inline)) {
         const float4 k = e < 8 ? k0[e / 4] : k1[e / 4 - 2];
@@ -303,12 +320,17 @@ __global__ void __launch_bounds__(WAVES * 64, 2) chunk_kernel(AttnArgs a) {
       };
       auto pair = [&](int e) __attribute__((always_inline)) {
         more = e == 0 ? w[0] + w[1] : more + (w[e] + w[e + 1]);
-        const h2_t r = __builtin_bit_cast(h2_t, pack_h2(w[e], w[e + 1]));
-        uint32_t bits = __builtin_bit_cast(uint32_t, r);
+        uint32_t rest = 0;
+        if constexpr (FINE) {
+          if (e % 4 == 0) v4 = *reinterpret_cast<const float4*>(&svs[(2 * s + HALF) & 7][2 * e + 4 * hi]);
+        }
+        uint32_t bits = weights(w[e], w[e + 1], FINE ? e % 4 ? v4.z : v4.x : 0.0f, FINE ? e % 4 ? v4.w : v4.y : 0.0f, rest);
+        if constexpr (FINE) {
+          asm volatile("" : "+v"(rest));
+          set2(nr, e, rest);
+        }
         asm volatile("" : "+v"(bits), "+v"(more));   // done here, not behind the last MFMA
-        const h2_t r2 = __builtin_bit_cast(h2_t, bits);
-        n[e / 8][e % 8] = r2[0];
-        n[e / 8][e % 8 + 1] = r2[1];
+        set2(n, e, bits);
       };
 #pragma unroll
       for (int e = 0; e < N; ++e) score(e);
@@ -317,6 +339,10 @@ __global__ void __launch_bounds__(WAVES * 64, 2) chunk_kernel(AttnArgs a) {
         const int j = i - KS, r = i + AHEAD;
         if (i < KS) next = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[i % AHEAD], q[i < KS ? i : 0], i ? next : zero, 0, 0, 0);
         else o[j & (DT - 1)] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[i % AHEAD], p[(j < 0 ? 0 : j) / DT], o[j & (DT - 1)], 0, 0, 0);
+        if constexpr (FINE) {
+          if (i >= KS)
+            o[j & (DT - 1)] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[i % AHEAD], pr[(j < 0 ? 0 : j) / DT], o[j & (DT - 1)], 0, 0, 0);
+        }
         if (r < KS) f[i % AHEAD] = k_at(b, HALF, r);
         else if (r < MM) f[i % AHEAD] = v_at(b, HALF, r - KS);
         else if (HALF == 0) f[i % AHEAD] = k_at(b, 1, r - MM);
@@ -343,12 +369,19 @@ __global__ void __launch_bounds__(WAVES * 64, 2) chunk_kernel(AttnArgs a) {
     };
     bool there = all_there(t0);   // of the step at hand
     bool begun = false;           // the first step sets the references
+    auto values = [&](int b, int half) __attribute__((always_inline)) {
+#pragma unroll
+      for (int i = 0; i < 2 * DT; ++i) {
+        const h8_t v = v_at(b, half, i);
+        o[i % DT] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, p[i / DT], o[i % DT], 0, 0, 0);
+        if constexpr (FINE) o[i % DT] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pr[i / DT], o[i % DT], 0, 0, 0);
+      }
+    };
     // Any half: keys that a row does not see hidden, the reference moved where it must be
     auto slow = [&](int b, int s, int half, bool made, f16_t& now, f16_t& next) __attribute__((always_inline)) {
       const int h = 2 * s + half;
       if (!made) {
-#pragma unroll
-        for (int i = 0; i < 2 * DT; ++i) o[i % DT] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v_at(b, half, i), p[i / DT], o[i % DT], 0, 0, 0);
+        values(b, half);
         next = zero;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) next = __builtin_amdgcn_mfma_f32_32x32x16_f16(k_at(b, half, ks), q[ks], next, 0, 0, 0);
@@ -373,11 +406,28 @@ __global__ void __launch_bounds__(WAVES * 64, 2) chunk_kernel(AttnArgs a) {
 #pragma unroll
       for (int d = 0; d < DT; ++d) o[d] *= f;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) y[i] -= to;
-      p[0] = probabilities(y);
-      p[1] = probabilities(y + 8);
+      for (int i = 0; i < 16; i += 2) {
+        const float p0 = __builtin_amdgcn_exp2f(y[i] - to), p1 = __builtin_amdgcn_exp2f(y[i + 1] - to);
+        sum += p0 + p1;
+        uint32_t rest = 0;
+        if constexpr (FINE) {
+          // a scale behind the sequence may be anything
+          const float* v = &svs[h & 7][4 * hi + 8 * (i >> 2) + (i & 3)];
+          set2(p, i, weights(p0, p1, y[i] == -INFINITY ? 0.0f : v[0], y[i + 1] == -INFINITY ? 0.0f : v[1], rest));
+          set2(pr, i, rest);
+        } else {
+          set2(p, i, weights(p0, p1, 0.0f, 0.0f, rest));
+        }
+      }
     };
 
+    auto take = [&](const h8_t (&n)[2], const h8_t (&nr)[2]) __attribute__((always_inline)) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        p[i] = n[i];
+        if constexpr (FINE) pr[i] = nr[i];
+      }
+    };
     if (t0 < t1) {
       // stage t0 - 1 is only K of window t0
 #pragma unroll
@@ -400,32 +450,30 @@ __global__ void __launch_bounds__(WAVES * 64, 2) chunk_kernel(AttnArgs a) {
       while (begun && there && s * KT + KT <= low) {
         const int b = s & 1;
         constexpr int MM = KS + 2 * DT, EACH = MM / (4 * NP);
-        h8_t f[AHEAD], n[2];
+        h8_t f[AHEAD], n[2], nr[2];
         float4 k0[2];
 #pragma unroll
         for (int c = 0; c < 2; ++c) k0[c] = *reinterpret_cast<const float4*>(&sks[(2 * s) & 7][8 * c + 4 * hi]);
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i) f[i] = k_at(b, 0, i);
         __builtin_amdgcn_sched_barrier(0);
-        float more = fast(std::integral_constant<int, 0>(), b, s, sa, sb, f, k0, n, [&](int i) __attribute__((always_inline)) {
+        float more = fast(std::integral_constant<int, 0>(), b, s, sa, sb, f, k0, n, nr, [&](int i) __attribute__((always_inline)) {
           if (i >= MM / 2 && i % EACH == 0) put_v(s + 1, (i - MM / 2) / EACH);
           if (i == MM - 1) next_v(s + 1);
         });
         staged_v = made = true;
         if (__builtin_amdgcn_ballot_w64(more > SUM_STALE)) break;   // a reference has to move
         sum += more;
-        p[0] = n[0];
-        p[1] = n[1];
+        take(n, nr);
         odd = true;
-        more = fast(std::integral_constant<int, 1>(), b, s, sb, sa, f, k0, n, [&](int i) __attribute__((always_inline)) {
+        more = fast(std::integral_constant<int, 1>(), b, s, sb, sa, f, k0, n, nr, [&](int i) __attribute__((always_inline)) {
           if (i >= MM / 2 && i % EACH == 0) put_k(s + 1, (i - MM / 2) / EACH);
           if (i == MM - 1) next_k(s + 1);
         });
         staged_k = true;
         if (__builtin_amdgcn_ballot_w64(more > SUM_STALE)) break;
         sum += more;
-        p[0] = n[0];
-        p[1] = n[1];
+        take(n, nr);
         __syncthreads();
         staged_v = staged_k = odd = made = false;
         there = all_there(++s);
@@ -444,8 +492,7 @@ __global__ void __launch_bounds__(WAVES * 64, 2) chunk_kernel(AttnArgs a) {
       there = all_there(++s);
     }
     if (t0 < t1) {   // the last half's values
-#pragma unroll
-      for (int i = 0; i < 2 * DT; ++i) o[i % DT] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v_at(t1 & 1, 0, i), p[i / DT], o[i % DT], 0, 0, 0);
+      values(t1 & 1, 0);
     }
     __syncthreads();   // the next item's tiles go where these are read
 
@@ -487,10 +534,18 @@ __global__ void __launch_bounds__(WAVES * 64, 2) chunk_kernel(AttnArgs a) {
 
 void launch_chunk(const AttnArgs& a, int fmt, int dim, int rows, hipStream_t st) {
   auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(a.wgs)), dim3(static_cast<uint32_t>(2 * rows)), 0, st, a); };
-  if (fmt == INT8 && dim == 128) rows == 128 ? go(chunk_kernel<INT8, 128, 4>) : go(chunk_kernel<INT8, 128, 8>);
-  else if (fmt == INT8) rows == 128 ? go(chunk_kernel<INT8, 64, 4>) : go(chunk_kernel<INT8, 64, 8>);
-  else if (dim == 128) rows == 128 ? go(chunk_kernel<E4M3, 128, 4>) : go(chunk_kernel<E4M3, 128, 8>);
-  else rows == 128 ? go(chunk_kernel<E4M3, 64, 4>) : go(chunk_kernel<E4M3, 64, 8>);
+  auto by = [&](auto four, auto eight, auto four_fine, auto eight_fine) {
+    if (rows == 128) a.fp16 ? go(four_fine) : go(four);
+    else a.fp16 ? go(eight_fine) : go(eight);
+  };
+  if (fmt == INT8 && dim == 128)
+    by(chunk_kernel<INT8, 128, 4, false>, chunk_kernel<INT8, 128, 8, false>, chunk_kernel<INT8, 128, 4, true>, chunk_kernel<INT8, 128, 8, true>);
+  else if (fmt == INT8)
+    by(chunk_kernel<INT8, 64, 4, false>, chunk_kernel<INT8, 64, 8, false>, chunk_kernel<INT8, 64, 4, true>, chunk_kernel<INT8, 64, 8, true>);
+  else if (dim == 128)
+    by(chunk_kernel<E4M3, 128, 4, false>, chunk_kernel<E4M3, 128, 8, false>, chunk_kernel<E4M3, 128, 4, true>, chunk_kernel<E4M3, 128, 8, true>);
+  else
+    by(chunk_kernel<E4M3, 64, 4, false>, chunk_kernel<E4M3, 64, 8, false>, chunk_kernel<E4M3, 64, 4, true>, chunk_kernel<E4M3, 64, 8, true>);
 }
 
 }  // namespace kv

@@ -351,6 +351,23 @@ def test_prefix_and_sequences_on_their_own_kernels(dev):
     _check_lse(lse, rl, err)
 
 
+@pytest.mark.parametrize("fmt", [I8, F8])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("rows,hkv", [(1, 1), (9, 2), (70, 2), (400, 1)])
+def test_fp16_results_are_rounded_once(dev, fmt, dim, form, rows, hkv):
+    """fp16 results: the weights in two f16 terms (2^-22 of each, and sums in fp32: with 2^-20 of sum p |v| for both) leave little
+    beside the rounding of the result."""
+    n, page = 777, 32
+    width = -(-n // page)
+    table = _tables(2 * width, width, 2, 3)
+    c = _pool(dev, fmt, 2 * width, hkv, page, dim, 6)
+    q = torch.randn(2 * rows, 2 * hkv, dim, generator=_gen(7)).to(HF).to(dev)
+    out = kv.kv_attention(q, c, _i32(table, dev), _i32([n, n - 300], dev), form=form)
+    ref, _, mag, err = ok.attention(q, c, table, [n, n - 300])
+    _check(out, ref, mag, err, 2.0 ** -9)
+
+
 @pytest.mark.parametrize("dtype", [BF, HF])
 @pytest.mark.parametrize("form", FORMS)
 @pytest.mark.parametrize("rows", [1, 50])
