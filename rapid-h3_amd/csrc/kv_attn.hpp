@@ -191,11 +191,6 @@ __device__ __forceinline__ int scalar(int v) { return __builtin_amdgcn_readfirst
 __device__ __forceinline__ int64_t scalar(int64_t v) { return lane64(v, 0); }
 
 // ---------------------------------------------------------------- query rows
-// 8 values of a query row at offset `at` as floats
-__device__ __forceinline__ void load_q8(const AttnArgs& a, int64_t at, float* v) {
-  if (a.fp16) load_row8<RH3_DTYPE_F16>(a.q, at, v);
-  else load_row8<RH3_DTYPE_BF16>(a.q, at, v);
-}
 // the exponent that brings a magnitude to [2^7, 2^8) (zero, infinite or NaN: none)
 __device__ __forceinline__ int q_exponent(float amax) {
   const int e = static_cast<int>(__float_as_uint(amax) >> 23) & 255;

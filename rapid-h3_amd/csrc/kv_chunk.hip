@@ -188,7 +188,7 @@ __global__ void __launch_bounds__(WAVES * 64, 2) chunk_kernel(AttnArgs a) {
       float x[KS][8], top = 0.0f;
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
-        load_q8(a, qat + 16 * s, x[s]);
+        load_row8<FINE ? RH3_DTYPE_F16 : RH3_DTYPE_BF16>(a.q, qat + 16 * s, x[s]);
 #pragma unroll
         for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[s][e]) < INFINITY ? fabsf(x[s][e]) : 0.0f);
       }

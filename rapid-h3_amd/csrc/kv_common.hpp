@@ -59,7 +59,7 @@ RH3_HD Seq seq_at(const Seqs& s, int b) {
   return r;
 }
 
-// The sequence of a row: the last b with cu[b] <= row, by a search over `lanes` (16 or 64) lanes at a time that hold the same
+// The sequence of a row: the last b with cu[b] <= row, by a search over LANES (8, 16 or 64) lanes that hold the same
 // row, or -1 for a row that no sequence has (behind the last one, or in a cu that does not rise).
 template <int LANES>
 __device__ __forceinline__ int seq_of_row(const Seqs& s, int row, Seq& q) {
@@ -121,19 +121,19 @@ __device__ __forceinline__ h8_t f16x8(uint32_t lo, uint32_t hi) {
                 __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, false), __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, true));
   }
 }
-// w[0 .. 7]: words of N (2 or 4) channels at 8 positions -> for each of the channels, its 8 positions as f16
-template <int FMT, int N>
-__device__ __forceinline__ void f16x8_across(const uint32_t (&w)[8], h8_t (&o)[N]) {
+// w[0 .. 7]: words of 4 channels at 8 positions -> for each of the channels, its 8 positions as f16
+template <int FMT>
+__device__ __forceinline__ void f16x8_across(const uint32_t (&w)[8], h8_t (&o)[4]) {
   if constexpr (FMT == INT8) {
 #pragma unroll
-    for (int c = 0; c < N; ++c) {
+    for (int c = 0; c < 4; ++c) {
       const uint32_t sel = 0x0c040c00u + static_cast<uint32_t>(c) * 0x00010001u;
       o[c] = join(f16_of_spread(__builtin_amdgcn_perm(w[1], w[0], sel)), f16_of_spread(__builtin_amdgcn_perm(w[3], w[2], sel)),
                   f16_of_spread(__builtin_amdgcn_perm(w[5], w[4], sel)), f16_of_spread(__builtin_amdgcn_perm(w[7], w[6], sel)));
     }
   } else {
 #pragma unroll
-    for (int p = 0; p < N / 2; ++p) {      // channels 2p and 2p + 1
+    for (int p = 0; p < 2; ++p) {      // channels 2p and 2p + 1
       const uint32_t sel = p ? 0x07030602u : 0x05010400u;
       const uint32_t a = __builtin_amdgcn_perm(w[1], w[0], sel), b = __builtin_amdgcn_perm(w[3], w[2], sel);
       const uint32_t c = __builtin_amdgcn_perm(w[5], w[4], sel), d = __builtin_amdgcn_perm(w[7], w[6], sel);

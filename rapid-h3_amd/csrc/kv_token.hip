@@ -215,7 +215,7 @@ __device__ __forceinline__ void compute(const AttnArgs& a, Tile<D>& t, int kvh, 
 #pragma unroll
     for (int j = 0; j < 8; ++j) w[j] = t.v[j][c];
     h8_t v[4];
-    f16x8_across<FMT, 4>(w, v);
+    f16x8_across<FMT>(w, v);
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
