@@ -462,6 +462,27 @@ def test_layouts(dev):
     assert torch.equal(q, want)
 
 
+@pytest.mark.parametrize("form", [None] + FORMS)
+@pytest.mark.parametrize("rows", [1, 21, 300])
+@pytest.mark.parametrize("prefix_len", [0, 333])
+def test_out_over_q_and_repeated_rows(dev, form, rows, prefix_len):
+    """The result written over q, and q given as one row repeated without memory of its own (stride 0): the same bits as apart."""
+    b, hq, hkv, dim, page = 3, 6, 2, 128, 64
+    c = _pool(dev, I8, 40, hkv, page, dim, 60)
+    table, lens, prefix = _i32([[1, 2, 3], [30, 5, 6], [7, 8, 39]], dev), _i32([190, 64, 5], dev), _i32([9, 20, 11, 12, 13, 14], dev)
+
+    def call(q, out=None):
+        if prefix_len:
+            return kv.kv_attention_shared(q, c, prefix, prefix_len, table, lens, out=out, form=form)
+        return kv.kv_attention(q, c, table, lens, out=out, form=form)
+    q = torch.randn(b * rows, hq, dim, generator=_gen(61)).to(BF).to(dev)
+    want = call(q)
+    same = q.clone()
+    assert call(same, out=same) is same and torch.equal(same.view(torch.int16), want.view(torch.int16))
+    one = q[:1].expand(b * rows, hq, dim)
+    assert torch.equal(call(one).view(torch.int16), call(one.contiguous()).view(torch.int16))
+
+
 def test_rows_that_no_sequence_has_stay(dev):
     c = _pool(dev, I8, 4, 1, 16, 64, 41)
     for rows, cu, form in ((5, [0, 1, 3], "token"), (90, [0, 40, 83], "chunk"), (90, [0, 40, 83], "token")):
