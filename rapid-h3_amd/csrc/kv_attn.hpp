@@ -6,8 +6,8 @@
 // token of the sequence, numbered token * group + head in the group, so that the group shares each key and value that is read.
 //
 // Arithmetic. Codes are small integers (int8) or 4-bit significands (e4m3): exact in f16. A query row is scaled by the power of
-// two that brings its largest magnitude to [2^7, 2^8): bf16 and fp16 values are exact in f16 after it (those 2^21 below the row's
-// largest lose low bits, 2^-33 of it at most). So q.k is a sum of exact products in fp32 on the f16 MFMA, times the key's scale,
+// two that brings its largest magnitude to [2^14, 2^15) (the chunk kernel: the largest of all rows of its tile, where none is far
+// below it): bf16 and fp16 values are exact in f16 after it (those 2^28 below lose low bits, 2^-40 of it at most). So q.k is a sum of exact products in fp32 on the f16 MFMA, times the key's scale,
 // in fp32. Probabilities are taken against a reference 10 to 15 under the row's running maximum (base 2), so that in f16 they use
 // its range from 2^15 down, rounded to nearest (2^-11 relative at most); products of probability and value scale keep that
 // precision down to 2^-24 of the largest. Their sum is fp32.
@@ -191,10 +191,10 @@ __device__ __forceinline__ int scalar(int v) { return __builtin_amdgcn_readfirst
 __device__ __forceinline__ int64_t scalar(int64_t v) { return lane64(v, 0); }
 
 // ---------------------------------------------------------------- query rows
-// the exponent that brings a magnitude to [2^7, 2^8) (zero, infinite or NaN: none)
+// the exponent that brings a magnitude to [2^14, 2^15) (zero, infinite or NaN: none)
 __device__ __forceinline__ int q_exponent(float amax) {
   const int e = static_cast<int>(__float_as_uint(amax) >> 23) & 255;
-  return e == 0 || e == 255 ? 0 : 134 - e;
+  return e == 0 || e == 255 ? 0 : 141 - e;
 }
 __device__ __forceinline__ h8_t q_f16(const float* v, int e) {
   h8_t r;

@@ -18,8 +18,9 @@
 // before's values, one MFMA to every one (dim 64: two) of the lane's 16 scores. Where keys are masked, a page is absent or a
 // reference has to move, a plain path does the half.
 // Vector work per score: one fma (key scale, softmax scale and reference at once), the exponential, the sum and half a
-// conversion. For that, the query rows of a workgroup share one power of two (an element 2^22 below the tile's largest loses low
-// bits, 2^-33 of the largest at most, which is what an absolute error of a score can be); a value's scale, relative to a power of
+// conversion. For that, the query rows of a workgroup share one power of two, if each row's largest is within 2^15 of the tile's (an
+// element is then off by 2^-24 of its own row's largest at most); rows further apart, as of an idle slot of a batch beside the
+// others, have one each, and the plain path does the whole item with a row's own factor in its scores. A value's scale, relative to a power of
 // two over the largest of the share's keys (a scan of the scales before the first step), is multiplied into V as it is converted.
 // Roundings to f16: the probability, and the value times its scale; 2^-11 relative at most each, with fp32 sums, beside a bf16
 // result's own 2^-8. FINE, for fp16 results, whose own rounding is no coarser: the scale is multiplied into the probability, which
@@ -40,6 +41,7 @@ namespace {
 
 constexpr int KT = CHUNK_KEYS;
 constexpr float SUM_STALE = 0x1p15f;  // up to this sum of a half's probabilities none of them is over 2^REF_STALE
+constexpr float ROWS_APART = 0x1p-15f;  // query rows whose largest is this far below the tile's do not share its power of two
 constexpr float NO_REF = -0x1p100f;   // reference of a row that has seen no key: any score moves it
 
 // 16-byte pieces of the LDS rows. Each row has one piece more than it needs, so that 16 rows' pieces of one number lie in all 16
@@ -65,7 +67,8 @@ __global__ void __launch_bounds__(WAVES * 64, 2) chunk_kernel(AttnArgs a) {
   __shared__ uint4 sv[2][KT * V_ROW<D>];
   __shared__ float sks[8][32];            // key scales of 8 half tiles in turn
   __shared__ float svs[FINE ? 8 : 1][32]; // value scales of them
-  __shared__ float stop[WAVES], sscale[WAVES];
+  __shared__ float stop[WAVES], sleast[WAVES], sscale[WAVES];
+  __shared__ float srow[WAVES * 32];      // rows far apart: what a row's scores are multiplied by
   __shared__ int sgone[WAVES];
   const int lane = threadIdx.x & 63, l32 = lane & 31, hi = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -123,6 +126,7 @@ __global__ void __launch_bounds__(WAVES * 64, 2) chunk_kernel(AttnArgs a) {
     float qf;
     int vref;   // bits of a power of two, the same in all lanes
     bool full;  // no key of the share in an absent page
+    bool apart; // query rows with a power of two each
     const int lim = causal ? min(sq.len, sq.len - sq.n + tok + 1) : sq.len;
     // of the wave's rows: keys that all see, keys that some see
     const int r0 = rt * R + wave * 32, r1 = min(rows - 1, r0 + 31);
@@ -192,7 +196,9 @@ __global__ void __launch_bounds__(WAVES * 64, 2) chunk_kernel(AttnArgs a) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[s][e]) < INFINITY ? fabsf(x[s][e]) : 0.0f);
       }
-      top = wave_max(top);
+      const float mine = across_max<false>(top);   // of the lane's row
+      float least = -wave_max(mine > 0.0f ? -mine : -INFINITY);
+      top = wave_max(mine);
       // the largest finite scale of the share's values, 4 keys (of one page) to a thread at a time
       float big = 0.0f;
       bool gone = false;
@@ -209,6 +215,7 @@ __global__ void __launch_bounds__(WAVES * 64, 2) chunk_kernel(AttnArgs a) {
       const int any = __builtin_amdgcn_ballot_w64(gone) != 0;
       if (lane == 0) {
         stop[wave] = top;
+        sleast[wave] = least;
         sscale[wave] = big;
         sgone[wave] = any;
       }
@@ -216,18 +223,21 @@ __global__ void __launch_bounds__(WAVES * 64, 2) chunk_kernel(AttnArgs a) {
 #pragma unroll
       for (int w = 0; w < WAVES; ++w) {
         top = fmaxf(top, stop[w]);
+        least = fminf(least, sleast[w]);
         big = fmaxf(big, sscale[w]);
         gone |= sgone[w] != 0;
       }
       full = __builtin_amdgcn_ballot_w64(gone) == 0;
       // V's reference: the largest code times its scale comes to 2^14 to 2^15; f16's range down from there is the smaller scales'
       vref = scalar(__float_as_int(pow2_over(big))) - (FINE ? 0 : (FMT == INT8 ? 8 : 6) << 23);
-      const int e = q_exponent(top);
+      apart = __builtin_amdgcn_ballot_w64(least < top * ROWS_APART) != 0;
+      const int e = q_exponent(apart ? mine : top);
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
         q[s] = q_f16(x[s], e);
       }
-      qf = __builtin_amdgcn_ldexpf(a.scale_log2, -e);
+      qf = __builtin_amdgcn_ldexpf(a.scale_log2, apart ? 0 : -e);
+      if (apart) srow[wave * 32 + l32] = __builtin_amdgcn_ldexpf(1.0f, -e);
     }
     // Stage x (loaded) to LDS in 2 NP parts of K and 2 NP of V; the loads of stage x + 1
     const float vinv = pow2_inverse(vref);
@@ -368,7 +378,7 @@ __global__ void __launch_bounds__(WAVES * 64, 2) chunk_kernel(AttnArgs a) {
       return more;
     };
     bool there = all_there(t0);   // of the step at hand
-    bool begun = false;           // the first step sets the references
+    bool begun = false;           // the first step sets the references (rows far apart: all steps go the plain way)
     auto values = [&](int b, int half) __attribute__((always_inline)) {
 #pragma unroll
       for (int i = 0; i < 2 * DT; ++i) {
@@ -391,6 +401,7 @@ __global__ void __launch_bounds__(WAVES * 64, 2) chunk_kernel(AttnArgs a) {
       if (!there)
         gone = static_cast<uint32_t>(__builtin_amdgcn_ballot_w64(page_in(table[min((32 * h + l32) >> a.c.log2page, width - 1)]) < 0) >> (4 * hi));
       float y[16], top = -INFINITY;
+      if (apart) now *= srow[wave * 32 + l32];
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const int key = 8 * (i >> 2) + (i & 3);
@@ -487,7 +498,7 @@ __global__ void __launch_bounds__(WAVES * 64, 2) chunk_kernel(AttnArgs a) {
       }
       if (!staged_v) stage_v(s + 1);
       if (!staged_k) stage_k(s + 1);
-      begun = true;
+      begun = !apart;
       __syncthreads();
       there = all_there(++s);
     }

@@ -436,6 +436,60 @@ def test_rising_scores(dev, fmt, dim, form, rows, hkv, gap):
     _check_lse(lse, rl, err)
 
 
+# ---------------------------------------------------------------- neighbours of another magnitude
+def _call(q, c, table, lens, cu, prefix, prefix_len, dev, **kw):
+    """kv_attention or, with a prefix, kv_attention_shared, by lists."""
+    args = (_i32(table, dev), _i32(lens, dev), None if cu is None else _i32(cu, dev))
+    if prefix_len:
+        return kv.kv_attention_shared(q, c, _i32(prefix, dev), prefix_len, *args, **kw)
+    return kv.kv_attention(q, c, *args, **kw)
+
+
+@pytest.mark.parametrize("fmt", [I8, F8])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("big", [2.0 ** 13, 2.0 ** 17, 2.0 ** 30, 1e12, 1e30])
+@pytest.mark.parametrize("b,rows,prefix_len", [(1, 60, 0), (2, 300, 0), (6, 1, 333), (5, 40, 700)])
+def test_rows_beside_far_larger_ones(dev, fmt, dim, form, big, b, rows, prefix_len):
+    """A query row's result is its own, however large a finite row beside it is: of its sequence, or of another that shares the
+    prefix."""
+    hq, hkv, page = 4, 2, 32
+    lens = [350 - 7 * i for i in range(b)]
+    width, pre = 11, -(-prefix_len // page)
+    table = _tables(b * width, width, b, 31)
+    common = list(range(b * width, b * width + pre))
+    c = _pool(dev, fmt, b * width + pre, hkv, page, dim, 32)
+    q = 2.0 * torch.randn(b * rows, hq, dim, generator=_gen(33))
+    at = [0, 3 * (b * rows) // 4]
+    q[at] *= big
+    q = q.to(BF).to(dev)
+    out, lse = _call(q, c, table, lens, None, common, prefix_len, dev, lse=True, form=form)
+    ref, rl, mag, err = ok.attention(q, c, table, lens, prefix=common, prefix_len=prefix_len)
+    rest = [i for i in range(b * rows) if i not in at]
+    _check(out[rest], ref[rest], mag[rest], err[rest], 3.1)
+    _check_lse(lse[rest], rl[rest], err[rest])
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("rows", [1, 90])
+def test_small_rows_beside_a_large_one_fp16(dev, form, rows):
+    """The same for fp16 rows over the whole of that type's range, with scores that matter from large keys."""
+    c = kv.kv_cache(5, 1, 64, 128, I8, dev)
+    g = _gen(34)
+    x, y = 2000.0 * torch.randn(300, 1, 128, generator=g), torch.randn(300, 1, 128, generator=g)
+    args = (_i32([[0, 1, 2, 3, 4]], dev), _i32([300], dev))
+    kv.kv_write(c, x.to(dev), y.to(dev), *args)
+    q = 1e-3 * torch.randn(rows, 3, 128, generator=g)
+    q[:, 0] *= 2.0 ** -8
+    q[rows // 2, 1] = 30000.0 * torch.sign(q[rows // 2, 1])
+    q = q.to(HF).to(dev)
+    out = kv.kv_attention(q, c, *args, causal=False, form=form)
+    ref, _, mag, err = ok.attention(q, c, [[0, 1, 2, 3, 4]], [300], None, False)
+    keep = torch.ones(rows, 3, dtype=torch.bool, device=dev)
+    keep[rows // 2, 1] = False
+    _check(out[keep], ref[keep], mag[keep], err[keep], 2.0 ** -9)
+
+
 def test_layouts(dev):
     """A cache that is a view of a buffer of several layers, strided queries and output, a wider table, out over q."""
     pages, heads, page, dim, hq = 9, 2, 32, 128, 6
