@@ -227,6 +227,11 @@ __device__ __forceinline__ float across_sum(float v) {
 // ---------------------------------------------------------------- the softmax reference and the values' scale
 constexpr float REF_UNDER = 10.0f;   // a new reference lies this far under the maximum: probabilities up to 2^10
 constexpr float REF_STALE = 15.0f;   // a score this far over the reference moves it: probabilities up to 2^15
+// (from 2^27 on a score's last place is 16: a reference that would come to lie that far under the maximum is the maximum itself)
+__device__ __forceinline__ float reference_under(float top) {
+  const float r = top - REF_UNDER;
+  return top - r > REF_STALE ? top : r;
+}
 
 // the power of two over a scale, at least 2^-111 (NaN never gets here)
 __device__ __forceinline__ float pow2_over(float v) {

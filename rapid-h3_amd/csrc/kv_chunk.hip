@@ -42,7 +42,7 @@ namespace {
 constexpr int KT = CHUNK_KEYS;
 constexpr float SUM_STALE = 0x1p15f;  // up to this sum of a half's probabilities none of them is over 2^REF_STALE
 constexpr float ROWS_APART = 0x1p-15f;  // query rows whose largest is this far below the tile's do not share its power of two
-constexpr float NO_REF = -0x1p100f;   // reference of a row that has seen no key: any score moves it
+constexpr float NO_REF = -0x1.fffffep127f;   // reference of a row that has seen no key: any score moves it
 
 // 16-byte pieces of the LDS rows. Each row has one piece more than it needs, so that 16 rows' pieces of one number lie in all 16
 // parts of the banks, and every read of a tile is one lane address with an immediate offset.
@@ -410,7 +410,7 @@ __global__ void __launch_bounds__(WAVES * 64, 2) chunk_kernel(AttnArgs a) {
         top = fmax_nc(top, y[i]);
       }
       top = across_max<false>(top);
-      const float to = top > ref + REF_STALE ? top - REF_UNDER : ref;
+      const float to = top - ref > REF_STALE ? reference_under(top) : ref;
       const float f = __builtin_amdgcn_exp2f(ref - to);
       ref = to;
       sum *= f;

@@ -158,7 +158,7 @@ __device__ __forceinline__ void compute(const AttnArgs& a, Tile<D>& t, int kvh, 
     top[m] = x[m][0];
 #pragma unroll
     for (int j = 1; j < 8; ++j) top[m] = fmaxf(top[m], x[m][j]);
-    move |= top[m] > st.ref[m] + REF_STALE;
+    move |= top[m] - st.ref[m] > REF_STALE;
   }
   if (__builtin_amdgcn_ballot_w64(move)) {
     const float vt = across_max<true>(vtop);
@@ -173,9 +173,10 @@ __device__ __forceinline__ void compute(const AttnArgs& a, Tile<D>& t, int kvh, 
     for (int m = 0; m < MT; ++m) {
       const float n = across_max<true>(top[m]);
       float f = 1.0f;
-      if (n > st.ref[m] + REF_STALE) {
-        f = __builtin_amdgcn_exp2f(st.ref[m] - (n - REF_UNDER));   // from no keys yet: 2^-inf = 0
-        st.ref[m] = n - REF_UNDER;
+      if (n - st.ref[m] > REF_STALE) {
+        const float to = reference_under(n);
+        f = __builtin_amdgcn_exp2f(st.ref[m] - to);   // from no keys yet: 2^-inf = 0
+        st.ref[m] = to;
       }
       st.sum[m] *= f;
       f *= vscale;

@@ -468,6 +468,7 @@ def test_rows_beside_far_larger_ones(dev, fmt, dim, form, big, b, rows, prefix_l
     rest = [i for i in range(b * rows) if i not in at]
     _check(out[rest], ref[rest], mag[rest], err[rest], 3.1)
     _check_lse(lse[rest], rl[rest], err[rest])
+    assert bool(torch.isfinite(out[at]).all()) and bool(torch.isfinite(lse[at]).all())
 
 
 @pytest.mark.parametrize("form", FORMS)
@@ -488,6 +489,38 @@ def test_small_rows_beside_a_large_one_fp16(dev, form, rows):
     keep = torch.ones(rows, 3, dtype=torch.bool, device=dev)
     keep[rows // 2, 1] = False
     _check(out[keep], ref[keep], mag[keep], err[keep], 2.0 ** -9)
+
+
+@pytest.mark.parametrize("fmt", [I8, F8])
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("rows", [1, 90])
+def test_scores_of_every_size(dev, fmt, dtype, form, sign, rows):
+    """Scores c 2^e (base 2, c of 1 to 16, or all negative) up to the largest of fp32: the row is the mean of its largest keys'
+    values, also where a score's last place is more than the distance between a maximum and its reference."""
+    n, dim, page = 200, 64, 32
+    g = _gen(35)
+    code = sign * torch.randint(1, 17, (n,), generator=g)
+    k = torch.zeros(n, dim)
+    k[:, 0] = code
+    k = torch.cat([k, torch.zeros(24, dim)]).reshape(7, 1, page, dim).to(fmt)
+    v, vs = ok.quantise(torch.randn(7, 1, page, dim, generator=g), fmt)
+    c = kv.KVCache(k.to(dev), v.to(dev), torch.ones(7, 1, page, device=dev), vs.to(dev))
+    values = (v.double() * vs.double()[..., None]).reshape(224, dim)[:n]
+    see = torch.arange(n) <= n - rows + torch.arange(rows)[:, None]
+    top = torch.where(see, code, -99).amax(1, keepdim=True)
+    w = (see & (code == top)).double()
+    ref = ((w @ values) / w.sum(1, keepdim=True)).to(dev)[:, None]
+    mag = ((w @ values.abs()) / w.sum(1, keepdim=True)).to(dev)[:, None]
+    for e in [*range(6, 15)] + ([*range(15, 48), 60, 90, 99, 101, 110, 120, 123] if dtype == BF else []):
+        q = torch.zeros(rows, 1, dim)
+        q[:, :, 0] = 2.0 ** e
+        out, lse = kv.kv_attention(q.to(dtype).to(dev), c, _i32([list(range(7))], dev), _i32([n], dev), scale=math.log(2.0), lse=True,
+                                   form=form)
+        _check(out, ref, mag, torch.zeros(rows, 1, dtype=torch.float64, device=dev), 3.1)
+        rl = (math.log(2.0) * top.double() * 2.0 ** e + torch.log(w.sum(1, keepdim=True))).to(dev)
+        assert ((lse.double() - rl).abs() <= 2.0 ** -21 * rl.abs() + 2.0 ** -20).all(), e
 
 
 def test_layouts(dev):
