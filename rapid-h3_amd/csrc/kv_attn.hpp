@@ -239,6 +239,14 @@ __device__ __forceinline__ float pow2_over(float v) {
   return __uint_as_float(min(max(e + 1u, 16u), 253u) << 23);
 }
 
+// The unit of a row's weights (probability times value scale, in f16) where its probabilities so far are scaled by f (at most 1)
+// and the largest weight of the next keys is w base: a power of two. The weights so far are in fp32 sums and may lie under it.
+constexpr float WEIGHT_MOST = 0x1p15f;
+__device__ __forceinline__ float weight_unit(float unit, float f, float w, float base) {
+  const float kept = unit * __uint_as_float(__float_as_uint(f) & 0x7f800000u);
+  return fmaxf(fmaxf(kept, base * (pow2_over(w) * 0x1p-11f)), 0x1p-120f);
+}
+
 // 1 over a power of two given by its bits (exponents 1 to 253)
 __device__ __forceinline__ float pow2_inverse(int bits) { return __int_as_float((254 << 23) - bits); }
 

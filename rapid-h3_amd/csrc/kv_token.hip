@@ -84,7 +84,7 @@ __device__ __forceinline__ void load_values(const AttnArgs& a, int kvh, int tile
 template <int D, int MT>
 struct State {
   f4_t o[MT][D / 16];   // o[mt][i][r]: channel (D / 16) (4 (l / 16) + r) + i
-  float ref[MT], sum[MT], vref, ivref;
+  float ref[MT], sum[MT], vref[MT], ivref[MT];   // o is in units of vref, a power of two
 };
 
 __device__ __forceinline__ h8_t to_f16(const float (&y)[8]) {
@@ -96,6 +96,8 @@ __device__ __forceinline__ h8_t to_f16(const float (&y)[8]) {
 // coarser than one (error 4.0e-4 -> 2.1e-4 of the largest, that of the result's rounding; bf16 results round by up to 2^-8). MORE: the
 // wave's next tile (pages `pn`) is loaded into the same registers, its keys as soon as these are used, its values at the end: a load
 // has about half a tile's work to come in.
+// A row's weights are in units of its own, which follow the largest of them as the reference follows the scores: neither values that
+// the row does not see nor large values of small probability take bits from the others, down to 2^-24 of the largest product.
 template <int FMT, int D, int MT, bool FINE, bool MORE>
 __device__ __forceinline__ void compute(const AttnArgs& a, Tile<D>& t, int kvh, int tile, const Pages& pg, const Pages& pn,
                                         const h8_t (&q)[MT][D / 32], const float (&qf)[MT], const int (&lim)[MT], int low, int len,
@@ -142,33 +144,34 @@ __device__ __forceinline__ void compute(const AttnArgs& a, Tile<D>& t, int kvh, 
       }
     }
   }
-  float x[MT][8], top[MT], vtop = 0.0f;
+  // a row's largest score and value scale, of the keys that it sees
+  float x[MT][8], top[MT], vtop[MT];
+  vtop[0] = vs[0];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) vtop = fmaxf(vtop, vs[j]);
-  bool move = vtop > st.vref;
+  for (int j = 1; j < 8; ++j) vtop[0] = fmaxf(vtop[0], vs[j]);
+  bool move = false;
 #pragma unroll
-  for (int m = 0; m < MT; ++m) {
+  for (int m = MT - 1; m >= 0; --m) {
+    vtop[m] = vtop[0];
 #pragma unroll
     for (int j = 0; j < 8; ++j) x[m][j] = acc[m][j >> 2][j & 3] * (ks[j] * qf[m]);
     if (edge) {
+      vtop[m] = 0.0f;
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (key[j] >= lim[m] || pg.p[j >> 2] < 0) x[m][j] = -INFINITY;
+      for (int j = 0; j < 8; ++j) {
+        const bool hidden = key[j] >= lim[m] || pg.p[j >> 2] < 0;
+        x[m][j] = hidden ? -INFINITY : x[m][j];
+        vtop[m] = fmaxf(vtop[m], hidden ? 0.0f : vs[j]);
+      }
     }
     top[m] = x[m][0];
 #pragma unroll
     for (int j = 1; j < 8; ++j) top[m] = fmaxf(top[m], x[m][j]);
-    move |= top[m] - st.ref[m] > REF_STALE;
+    // over 2^15: a probability, or what its product with a value's scale can be
+    const float most = __builtin_amdgcn_exp2f(top[m] - (st.ref[m] == -INFINITY ? 0.0f : st.ref[m])) * (vtop[m] * st.ivref[m]);
+    move |= top[m] - st.ref[m] > REF_STALE || !(most <= WEIGHT_MOST);
   }
   if (__builtin_amdgcn_ballot_w64(move)) {
-    const float vt = across_max<true>(vtop);
-    float vscale = 1.0f;
-    if (vt > st.vref) {
-      const float nv = pow2_over(vt);
-      vscale = st.vref / nv;
-      st.vref = nv;
-      st.ivref = 1.0f / nv;
-    }
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
       const float n = across_max<true>(top[m]);
@@ -179,14 +182,21 @@ __device__ __forceinline__ void compute(const AttnArgs& a, Tile<D>& t, int kvh, 
         st.ref[m] = to;
       }
       st.sum[m] *= f;
-      f *= vscale;
+      // the weights' unit: down with the probabilities so far, up to where the largest weight of these keys is 2^10 to 2^11
+      const float base = pow2_over(across_max<true>(vtop[m]));
+      const float ibase = pow2_inverse(__float_as_int(base));
+      float w = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) w = fmaxf(w, __builtin_amdgcn_exp2f(x[m][j] - (st.ref[m] == -INFINITY ? 0.0f : st.ref[m])) * (vs[j] * ibase));
+      const float unit = weight_unit(st.vref[m], f, across_max<true>(w), base);
+      st.ivref[m] = pow2_inverse(__float_as_int(unit));
+      f *= st.vref[m] * st.ivref[m];
+      st.vref[m] = unit;
 #pragma unroll
       for (int i = 0; i < D / 16; ++i) st.o[m][i] *= f;
     }
   }
   h8_t p[MT], rest[FINE ? MT : 1];
-#pragma unroll
-  for (int j = 0; j < 8; ++j) vs[j] *= st.ivref;
 #pragma unroll
   for (int m = 0; m < MT; ++m) {
     // a row that has seen no key yet has only -inf here: any finite reference gives it zeros
@@ -196,7 +206,7 @@ __device__ __forceinline__ void compute(const AttnArgs& a, Tile<D>& t, int kvh, 
     for (int j = 0; j < 8; ++j) {
       const float e = __builtin_amdgcn_exp2f(x[m][j] - ref);
       st.sum[m] += e;
-      y[j] = e * vs[j];
+      y[j] = e * (vs[j] * st.ivref[m]);
     }
     if (edge) {   // a key that the row does not see may hold NaN
 #pragma unroll
@@ -308,12 +318,12 @@ __global__ void __launch_bounds__(NT, 2) token_kernel(AttnArgs a) {
     const int low = causal ? min(sq.len, sq.len - sq.n + scalar((rt * R) / a.group) + 1) : sq.len;
 
     State<D, MT> st;
-    st.vref = 0.0f;
-    st.ivref = 0.0f;
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
       st.ref[m] = -INFINITY;
       st.sum[m] = 0.0f;
+      st.vref[m] = 0.0f;
+      st.ivref[m] = 0.0f;
 #pragma unroll
       for (int i = 0; i < D / 16; ++i) st.o[m][i] = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
     }
@@ -339,7 +349,7 @@ __global__ void __launch_bounds__(NT, 2) token_kernel(AttnArgs a) {
 #pragma unroll
         for (int i = 0; i < D / 16; i += 4) {
           float4 v = make_float4(st.o[m][i][r], st.o[m][i + 1][r], st.o[m][i + 2][r], st.o[m][i + 3][r]);
-          v.x *= st.vref; v.y *= st.vref; v.z *= st.vref; v.w *= st.vref;
+          v.x *= st.vref[m]; v.y *= st.vref[m]; v.z *= st.vref[m]; v.w *= st.vref[m];
           *reinterpret_cast<float4*>(&so[wave][16 * m + l16][(D / 16) * (4 * g + r) + i]) = v;
         }
     }

@@ -523,6 +523,83 @@ def test_scores_of_every_size(dev, fmt, dtype, form, sign, rows):
         assert ((lse.double() - rl).abs() <= 2.0 ** -21 * rl.abs() + 2.0 ** -20).all(), e
 
 
+def _outlier_values(dev, fmt, dim, n, rows, factor, at, hidden, seed, slack=0.0):
+    """A cache of one sequence whose value at position `at` is `factor` times the others, with queries that either may not see it
+    (hidden) or see it with about 1 / factor of the other keys' probability (or 2^-slack of that)."""
+    page, hkv = 32, 2
+    g = _gen(seed)
+    width = -(-n // page)
+    u = torch.randn(dim, generator=g)
+    u = u / u.norm()
+    x = torch.randn(n, hkv, dim, generator=g)
+    y = torch.randn(n, hkv, dim, generator=g) * torch.exp(0.5 * torch.randn(n, hkv, 1, generator=g))
+    y[at] *= factor
+    if not hidden:
+        x[at] = -u * (math.log(factor) + slack * math.log(2.0)) / 8.0 * dim ** 0.5
+    q = 0.5 * torch.randn(rows, 2 * hkv, dim, generator=g)
+    q = q - (q @ u)[..., None] * u + 8.0 * u
+    if not hidden:
+        others = torch.arange(n) != at
+        x[others] -= (x[others] @ u)[..., None] * u
+    table = _tables(width, width, 1, seed)
+    c = kv.kv_cache(width, hkv, page, dim, fmt, dev)
+    kv.kv_write(c, x.to(dev), y.to(dev), _i32(table, dev), _i32([n], dev))
+    return c, table, q
+
+
+@pytest.mark.parametrize("fmt", [I8, F8])
+@pytest.mark.parametrize("form", ["token"])
+@pytest.mark.parametrize("factor", [2.0 ** 18, 2.0 ** 24, 2.0 ** 60, 1e30])
+@pytest.mark.parametrize("rows,dim,dtype", [(4, 128, BF), (4, 64, HF), (90, 64, BF), (90, 128, HF)])
+def test_values_beside_far_larger_hidden_ones(dev, fmt, form, factor, rows, dim, dtype):
+    """What a causal row may not see does not touch its result: the last position's value is larger by any factor."""
+    n = 300
+    c, table, q = _outlier_values(dev, fmt, dim, n, rows, factor, n - 1, True, 36)
+    q = q.to(dtype).to(dev)
+    out, lse = kv.kv_attention(q, c, _i32(table, dev), _i32([n], dev), lse=True, form=form)
+    ref, rl, mag, err = ok.attention(q, c, table, [n])
+    _check(out[:-1], ref[:-1], mag[:-1], err[:-1], 3.1)
+    _check_lse(lse, rl, err)
+
+
+@pytest.mark.parametrize("fmt", [I8, F8])
+@pytest.mark.parametrize("form", ["token"])
+@pytest.mark.parametrize("factor", [2.0 ** 24, 2.0 ** 60])
+@pytest.mark.parametrize("at", [0, 150, 299])
+@pytest.mark.parametrize("slack", [0.0, -6.0])
+@pytest.mark.parametrize("rows,dim,dtype", [(4, 128, BF), (90, 64, BF), (90, 128, HF)])
+def test_values_beside_far_larger_unlikely_ones(dev, fmt, form, factor, at, slack, rows, dim, dtype):
+    """A value larger by a factor that its probability is smaller by: it and the others count as much as they do."""
+    n = 300
+    c, table, q = _outlier_values(dev, fmt, dim, n, rows, factor, at, False, 37, slack)
+    q = q.to(dtype).to(dev)
+    out, lse = kv.kv_attention(q, c, _i32(table, dev), _i32([n], dev), causal=False, lse=True, form=form)
+    ref, rl, mag, err = ok.attention(q, c, table, [n], None, False)
+    _check(out, ref, mag, err, 3.1)
+    _check_lse(lse, rl, err)
+
+
+@pytest.mark.parametrize("fmt", [I8, F8])
+@pytest.mark.parametrize("form", ["token"])
+@pytest.mark.parametrize("rows", [2, 70])
+def test_values_of_every_size_and_zero_ones(dev, fmt, form, rows):
+    """Values that grow from key to key through all of their type's range, and rows of zeros between them, whose scale is the
+    quantiser's least: each causal row has its own largest."""
+    n, dim, page = 90, 128, 16
+    g = _gen(38)
+    x = 0.3 * torch.randn(n, 1, dim, generator=g)
+    y = torch.randn(n, 1, dim, generator=g) * torch.logspace(-30, 60, n, base=2.0)[:, None, None]
+    y[::7] = 0.0
+    c = kv.kv_cache(6, 1, page, dim, fmt, dev)
+    args = (_i32([[5, 3, 0, 1, 2, 4]], dev), _i32([n], dev))
+    kv.kv_write(c, x.to(dev), y.to(dev), *args)
+    q = torch.randn(rows, 3, dim, generator=g).to(BF).to(dev)
+    out, lse = kv.kv_attention(q, c, *args, lse=True, form=form)
+    ref, rl, mag, err = ok.attention(q, c, [[5, 3, 0, 1, 2, 4]], [n])
+    _check(out, ref, mag, err, 3.1)
+    _check_lse(lse, rl, err)
+
+
 def test_layouts(dev):
     """A cache that is a view of a buffer of several layers, strided queries and output, a wider table, out over q."""
     pages, heads, page, dim, hq = 9, 2, 32, 128, 6
