@@ -7,10 +7,11 @@
 //
 // Arithmetic. Codes are small integers (int8) or 4-bit significands (e4m3): exact in f16. A query row is scaled by the power of
 // two that brings its largest magnitude to [2^14, 2^15) (the chunk kernel: the largest of all rows of its tile, where none is far
-// below it): bf16 and fp16 values are exact in f16 after it (those 2^28 below lose low bits, 2^-40 of it at most). So q.k is a sum of exact products in fp32 on the f16 MFMA, times the key's scale,
-// in fp32. Probabilities are taken against a reference 10 to 15 under the row's running maximum (base 2), so that in f16 they use
-// its range from 2^15 down, rounded to nearest (2^-11 relative at most); products of probability and value scale keep that
-// precision down to 2^-24 of the largest. Their sum is fp32.
+// below it): bf16 and fp16 values are exact in f16 after it (those 2^28 below lose low bits, 2^-40 of it at most). So q.k is a sum
+// of exact products in fp32 on the f16 MFMA, times the key's scale, in fp32. Probabilities are taken against a reference 10 to 15
+// under the row's running maximum (base 2), so that in f16 they use its range from 2^15 down, rounded to nearest (2^-11 relative at
+// most); where they are multiplied by value scales first, the products keep that precision down to 2^-24 of the row's largest.
+// Their sum is fp32.
 #pragma once
 
 #include "kv_common.hpp"

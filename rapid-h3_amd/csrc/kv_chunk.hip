@@ -20,12 +20,15 @@
 // Vector work per score: one fma (key scale, softmax scale and reference at once), the exponential, the sum and half a
 // conversion. For that, the query rows of a workgroup share one power of two, if each row's largest is within 2^15 of the tile's (an
 // element is then off by 2^-24 of its own row's largest at most); rows further apart, as of an idle slot of a batch beside the
-// others, have one each, and the plain path does the whole item with a row's own factor in its scores. A value's scale, relative to a power of
-// two over the largest of the share's keys (a scan of the scales before the first step), is multiplied into V as it is converted.
-// Roundings to f16: the probability, and the value times its scale; 2^-11 relative at most each, with fp32 sums, beside a bf16
-// result's own 2^-8. FINE, for fp16 results, whose own rounding is no coarser: the scale is multiplied into the probability, which
-// is kept in two f16 terms (error of 300 rows on 3,000 keys 4.0e-4 -> 2.1e-4, that of the result's rounding; the first size
-// above 545 -> 730 us, the last 67 -> 79).
+// others, have one each, and the plain path does the whole item with a row's own factor in its scores. A value's scale, relative
+// to a power of two over the largest of the share's keys (a scan of the scales before the first step), is multiplied into V as it
+// is converted, if those scales are within 2^18 of each other (rows of zeros aside). Else a large value would take bits from rows
+// that do not see it, or hardly: the plain path takes that item, too, and multiplies the scales into the probabilities, in a unit
+// of each row's own.
+// Roundings to f16: the probability, the value's scale, and the product of that with the code; 2^-11 relative at most each, with
+// fp32 sums, beside a bf16 result's own 2^-8. FINE, for fp16 results, whose own rounding is no coarser: the scale (within 2^14 of
+// the others) is multiplied into the probability, which is kept in two f16 terms (error of 300 rows on 3,000 keys 4.0e-4 ->
+// 2.1e-4, that of the result's rounding; the first size above 545 -> 730 us, the last 67 -> 79).
 //
 // Tried and slower, or no faster: exponentials only beside the values' MFMAs (703 against 688 us for the first size above), the
 // next step's page entries looked up one by one behind the barrier (688 against 670), a load two steps ahead of the next one that
@@ -52,6 +55,18 @@ constexpr int K_ROW = D / 8 + 1;                               // K: [64 keys][D
 template <int D>
 constexpr int V_ROW = D / 8 + 4;
 
+// whether a row of codes has one that is not zero
+template <int FMT, int D>
+__device__ __forceinline__ bool codes_in(const uint8_t* row) {
+  uint32_t any = 0;
+#pragma unroll 1
+  for (int i = 0; i < D / 16; ++i) {
+    const uint4 r = reinterpret_cast<const uint4*>(row)[i];
+    any |= r.x | r.y | r.z | r.w;
+  }
+  return (any & (FMT == INT8 ? 0xffffffffu : 0x7f7f7f7fu)) != 0;
+}
+
 // 4 rows x 16 channels to 16 lanes: lane i gives the address of row i / 4, channels 4 (i % 4) + 0 .. 3, and gets channel i's 4 rows
 typedef __fp16 g4_t __attribute__((__vector_size__(4 * sizeof(__fp16))));
 typedef _Float16 h4_t __attribute__((ext_vector_type(4)));
@@ -66,9 +81,9 @@ __global__ void __launch_bounds__(WAVES * 64, 2) chunk_kernel(AttnArgs a) {
   __shared__ uint4 sk[2][KT * K_ROW<D>];
   __shared__ uint4 sv[2][KT * V_ROW<D>];
   __shared__ float sks[8][32];            // key scales of 8 half tiles in turn
-  __shared__ float svs[FINE ? 8 : 1][32]; // value scales of them
-  __shared__ float stop[WAVES], sleast[WAVES], sscale[WAVES];
-  __shared__ float srow[WAVES * 32];      // rows far apart: what a row's scores are multiplied by
+  __shared__ float svs[8][32];            // value scales of them (where they go to the weights)
+  __shared__ float stop[WAVES], sleast[WAVES], sscale[WAVES], ssmall[WAVES];
+  __shared__ float srow[WAVES * 32], sunit[WAVES * 32];   // rows or values far apart: a row's factor of its scores, unit of its weights
   __shared__ int sgone[WAVES];
   const int lane = threadIdx.x & 63, l32 = lane & 31, hi = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -126,7 +141,7 @@ __global__ void __launch_bounds__(WAVES * 64, 2) chunk_kernel(AttnArgs a) {
     float qf;
     int vref;   // bits of a power of two, the same in all lanes
     bool full;  // no key of the share in an absent page
-    bool apart; // query rows with a power of two each
+    bool apart; // query rows with a power of two each, weights with a unit to each row
     const int lim = causal ? min(sq.len, sq.len - sq.n + tok + 1) : sq.len;
     // of the wave's rows: keys that all see, keys that some see
     const int r0 = rt * R + wave * 32, r1 = min(rows - 1, r0 + 31);
@@ -200,7 +215,7 @@ __global__ void __launch_bounds__(WAVES * 64, 2) chunk_kernel(AttnArgs a) {
       float least = -wave_max(mine > 0.0f ? -mine : -INFINITY);
       top = wave_max(mine);
       // the largest finite scale of the share's values, 4 keys (of one page) to a thread at a time
-      float big = 0.0f;
+      float big = 0.0f, small = INFINITY;
       bool gone = false;
 #pragma unroll 4
       for (int key = t0 * KT + 4 * static_cast<int>(threadIdx.x); key < min(t1 * KT, sq.len); key += 4 * WAVES * 64) {
@@ -209,14 +224,22 @@ __global__ void __launch_bounds__(WAVES * 64, 2) chunk_kernel(AttnArgs a) {
         const float x[4] = {v.x, v.y, v.z, v.w};
         gone |= page < 0;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) big = fmaxf(big, page >= 0 && key + e < sq.len && x[e] < INFINITY ? x[e] : 0.0f);
+        for (int e = 0; e < 4; ++e) {
+          const float y = page >= 0 && key + e < sq.len && x[e] < INFINITY ? x[e] : 0.0f;
+          big = fmaxf(big, y);
+          // (a row of zeros has the quantizers' least scale and takes no part)
+          if (y > 0.0f && (y > 1e-12f || codes_in<FMT, D>(a.c.v + page * a.c.page_stride + kvh * a.c.head_stride + ((key + e) & mask) * D)))
+            small = fminf(small, y);
+        }
       }
       big = wave_max(big);
+      small = -wave_max(-small);
       const int any = __builtin_amdgcn_ballot_w64(gone) != 0;
       if (lane == 0) {
         stop[wave] = top;
         sleast[wave] = least;
         sscale[wave] = big;
+        ssmall[wave] = small;
         sgone[wave] = any;
       }
       __syncthreads();
@@ -225,27 +248,29 @@ __global__ void __launch_bounds__(WAVES * 64, 2) chunk_kernel(AttnArgs a) {
         top = fmaxf(top, stop[w]);
         least = fminf(least, sleast[w]);
         big = fmaxf(big, sscale[w]);
+        small = fminf(small, ssmall[w]);
         gone |= sgone[w] != 0;
       }
       full = __builtin_amdgcn_ballot_w64(gone) == 0;
       // V's reference: the largest code times its scale comes to 2^14 to 2^15; f16's range down from there is the smaller scales'
       vref = scalar(__float_as_int(pow2_over(big))) - (FINE ? 0 : (FMT == INT8 ? 8 : 6) << 23);
-      apart = __builtin_amdgcn_ballot_w64(least < top * ROWS_APART) != 0;
+      apart = __builtin_amdgcn_ballot_w64(least < top * ROWS_APART || small < big * (FINE ? 0x1p-14f : 0x1p-18f)) != 0;
       const int e = q_exponent(apart ? mine : top);
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
         q[s] = q_f16(x[s], e);
       }
       qf = __builtin_amdgcn_ldexpf(a.scale_log2, apart ? 0 : -e);
-      if (apart) srow[wave * 32 + l32] = __builtin_amdgcn_ldexpf(1.0f, -e);
+      if (apart) {
+        srow[wave * 32 + l32] = __builtin_amdgcn_ldexpf(1.0f, -e);
+        sunit[wave * 32 + l32] = 0.0f;
+      }
     }
     // Stage x (loaded) to LDS in 2 NP parts of K and 2 NP of V; the loads of stage x + 1
-    const float vinv = pow2_inverse(vref);
+    const float vinv = apart ? 1.0f : pow2_inverse(vref);
     auto put_k = [&](int x, int part) __attribute__((always_inline)) {
       const int i = part / 2, c = part % 2, key = first + 8 * i + (lane >> 3), h = (2 * x + 1 + (key >> 5)) & 7;
-      if constexpr (FINE) {
-        if (c == 0) svs[h][key & 31] = kvs[i] < INFINITY ? kvs[i] * vinv : 0.0f;
-      }
+      if (c == 0 && (FINE || apart)) svs[h][key & 31] = kvs[i] < INFINITY ? kvs[i] * vinv : 0.0f;
       // a NaN value would reach rows that do not see its key (0 x NaN): its key is made NaN
       if (c == 0) sks[h][key & 31] = fmaf(kvs[i], 0.0f, ks[i] * qf);
       if (c < D / 64)
@@ -256,7 +281,7 @@ __global__ void __launch_bounds__(WAVES * 64, 2) chunk_kernel(AttnArgs a) {
       // outside the share's keys and in an absent page there may be anything: 0 (and codes that can be NaN go)
       const int pos = x * KT - 32 + key;
       const bool here = vpage >= 0 && pos >= t0 * KT && pos < min(sq.len, t1 * KT);
-      [[maybe_unused]] const _Float16 f = static_cast<_Float16>(here && vs[i] < INFINITY ? vs[i] * vinv : 0.0f);
+      [[maybe_unused]] const _Float16 f = static_cast<_Float16>(here && vs[i] < INFINITY ? (apart ? 1.0f : vs[i] * vinv) : 0.0f);
       if (c < D / 64) {
         const bool keep = FMT == INT8 || here;
         const h8_t v = f16x8<FMT>(keep ? vraw[i][2 * c] : 0u, keep ? vraw[i][2 * c + 1] : 0u);
@@ -299,12 +324,8 @@ __global__ void __launch_bounds__(WAVES * 64, 2) chunk_kernel(AttnArgs a) {
       const h4_t lo = lds_read_tr(at), up = lds_read_tr(at + 8 * V_ROW<D> * 16);
       return __builtin_shufflevector(lo, up, 0, 1, 2, 3, 4, 5, 6, 7);
     };
-    // Weights of two keys to f16; FINE: times their values' scales, in two terms
-    auto weights = [&](float w0, float w1, float v0, float v1, uint32_t& rest) __attribute__((always_inline)) {
-      if constexpr (FINE) {
-        w0 *= v0;
-        w1 *= v1;
-      }
+    // Weights of two keys to f16; FINE: in two terms
+    auto weights = [&](float w0, float w1, uint32_t& rest) __attribute__((always_inline)) {
       const uint32_t w = pack_h2(w0, w1);
       if constexpr (FINE) {
         const h2_t r = __builtin_bit_cast(h2_t, w);
@@ -334,7 +355,7 @@ __global__ void __launch_bounds__(WAVES * 64, 2) chunk_kernel(AttnArgs a) {
         if constexpr (FINE) {
           if (e % 4 == 0) v4 = *reinterpret_cast<const float4*>(&svs[(2 * s + HALF) & 7][2 * e + 4 * hi]);
         }
-        uint32_t bits = weights(w[e], w[e + 1], FINE ? e % 4 ? v4.z : v4.x : 0.0f, FINE ? e % 4 ? v4.w : v4.y : 0.0f, rest);
+        uint32_t bits = FINE ? weights(w[e] * (e % 4 ? v4.z : v4.x), w[e + 1] * (e % 4 ? v4.w : v4.y), rest) : weights(w[e], w[e + 1], rest);
         if constexpr (FINE) {
           asm volatile("" : "+v"(rest));
           set2(nr, e, rest);
@@ -411,24 +432,46 @@ __global__ void __launch_bounds__(WAVES * 64, 2) chunk_kernel(AttnArgs a) {
       }
       top = across_max<false>(top);
       const float to = top - ref > REF_STALE ? reference_under(top) : ref;
-      const float f = __builtin_amdgcn_exp2f(ref - to);
+      float f = __builtin_amdgcn_exp2f(ref - to);
       ref = to;
       sum *= f;
+      // to weights; FINE or rows apart: times their values' scales (one that the row does not see may be anything)
+      const float* scale = &svs[h & 7][4 * hi];
+      if (apart) {
+        float vtop = 0.0f, w = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) vtop = fmaxf(vtop, y[i] == -INFINITY ? 0.0f : scale[8 * (i >> 2) + (i & 3)]);
+        const float base = pow2_over(across_max<false>(vtop)), ibase = pow2_inverse(__float_as_int(base));
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const float e = __builtin_amdgcn_exp2f(y[i] - to);
+          sum += e;
+          y[i] = e * ((y[i] == -INFINITY ? 0.0f : scale[8 * (i >> 2) + (i & 3)]) * ibase);
+          w = fmaxf(w, y[i]);
+        }
+        float* unit = &sunit[wave * 32 + l32];
+        const float now_in = weight_unit(*unit, f, across_max<false>(w), base), inv = pow2_inverse(__float_as_int(now_in));
+        f *= *unit * inv;
+        *unit = now_in;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) y[i] *= base * inv;
+      } else {
+#pragma unroll
+        for (int i = 0; i < 16; i += 2) {
+          const float e0 = __builtin_amdgcn_exp2f(y[i] - to), e1 = __builtin_amdgcn_exp2f(y[i + 1] - to);
+          const float* v = scale + 8 * (i >> 2) + (i & 3);
+          sum += e0 + e1;
+          y[i] = FINE ? e0 * (y[i] == -INFINITY ? 0.0f : v[0]) : e0;
+          y[i + 1] = FINE ? e1 * (y[i + 1] == -INFINITY ? 0.0f : v[1]) : e1;
+        }
+      }
 #pragma unroll
       for (int d = 0; d < DT; ++d) o[d] *= f;
 #pragma unroll
       for (int i = 0; i < 16; i += 2) {
-        const float p0 = __builtin_amdgcn_exp2f(y[i] - to), p1 = __builtin_amdgcn_exp2f(y[i + 1] - to);
-        sum += p0 + p1;
         uint32_t rest = 0;
-        if constexpr (FINE) {
-          // a scale behind the sequence may be anything
-          const float* v = &svs[h & 7][4 * hi + 8 * (i >> 2) + (i & 3)];
-          set2(p, i, weights(p0, p1, y[i] == -INFINITY ? 0.0f : v[0], y[i + 1] == -INFINITY ? 0.0f : v[1], rest));
-          set2(pr, i, rest);
-        } else {
-          set2(p, i, weights(p0, p1, 0.0f, 0.0f, rest));
-        }
+        set2(p, i, weights(y[i], y[i + 1], rest));
+        if constexpr (FINE) set2(pr, i, rest);
       }
     };
 
@@ -509,10 +552,11 @@ __global__ void __launch_bounds__(WAVES * 64, 2) chunk_kernel(AttnArgs a) {
 
     // lane: query row l % 32, channels 32 d + 8 i + 4 (l / 32) + 0 .. 3
     const float total = across_sum<false>(sum);
+    const float unit = apart ? sunit[wave * 32 + l32] : __int_as_float(vref);
     if (has) {
       if (whole && !a.keep) {
         const int tok = row / a.group, hd = kvh * a.group + row - tok * a.group;
-        const float inv = total == 0.0f ? 0.0f : __int_as_float(vref) / total;
+        const float inv = total == 0.0f ? 0.0f : unit / total;
         uint16_t* dst = static_cast<uint16_t*>(a.out) + (sq.first + tok) * a.o_st + hd * a.o_sh + 4 * hi;
 #pragma unroll
         for (int d = 0; d < DT; ++d)
@@ -527,14 +571,13 @@ __global__ void __launch_bounds__(WAVES * 64, 2) chunk_kernel(AttnArgs a) {
         // slots: two to a workgroup (the item that it goes on with, the one that it begins), then one to an item that it completes
         const int64_t slot = whole ? 2 * static_cast<int64_t>(a.wgs) + sw.items_before + item : 2 * static_cast<int64_t>(wg) + (t0 == 0);
         const int rl = wave * 32 + l32;
-        const float vf = __int_as_float(vref);
         float* po = a.part_o + (slot * R + rl) * D + 4 * hi;
 #pragma unroll
         for (int d = 0; d < DT; ++d)
 #pragma unroll
           for (int i = 0; i < 4; ++i)
             *reinterpret_cast<float4*>(po + 32 * d + 8 * i) =
-                make_float4(o[d][4 * i] * vf, o[d][4 * i + 1] * vf, o[d][4 * i + 2] * vf, o[d][4 * i + 3] * vf);
+                make_float4(o[d][4 * i] * unit, o[d][4 * i + 1] * unit, o[d][4 * i + 2] * unit, o[d][4 * i + 3] * unit);
         if (hi == 0) *reinterpret_cast<float2*>(a.part_ml + (slot * R + rl) * 2) = make_float2(total == 0.0f ? -INFINITY : ref, total);
       }
     }

@@ -548,7 +548,7 @@ def _outlier_values(dev, fmt, dim, n, rows, factor, at, hidden, seed, slack=0.0)
 
 
 @pytest.mark.parametrize("fmt", [I8, F8])
-@pytest.mark.parametrize("form", ["token"])
+@pytest.mark.parametrize("form", FORMS)
 @pytest.mark.parametrize("factor", [2.0 ** 18, 2.0 ** 24, 2.0 ** 60, 1e30])
 @pytest.mark.parametrize("rows,dim,dtype", [(4, 128, BF), (4, 64, HF), (90, 64, BF), (90, 128, HF)])
 def test_values_beside_far_larger_hidden_ones(dev, fmt, form, factor, rows, dim, dtype):
@@ -563,7 +563,7 @@ def test_values_beside_far_larger_hidden_ones(dev, fmt, form, factor, rows, dim,
 
 
 @pytest.mark.parametrize("fmt", [I8, F8])
-@pytest.mark.parametrize("form", ["token"])
+@pytest.mark.parametrize("form", FORMS)
 @pytest.mark.parametrize("factor", [2.0 ** 24, 2.0 ** 60])
 @pytest.mark.parametrize("at", [0, 150, 299])
 @pytest.mark.parametrize("slack", [0.0, -6.0])
@@ -580,7 +580,7 @@ def test_values_beside_far_larger_unlikely_ones(dev, fmt, form, factor, at, slac
 
 
 @pytest.mark.parametrize("fmt", [I8, F8])
-@pytest.mark.parametrize("form", ["token"])
+@pytest.mark.parametrize("form", FORMS)
 @pytest.mark.parametrize("rows", [2, 70])
 def test_values_of_every_size_and_zero_ones(dev, fmt, form, rows):
     """Values that grow from key to key through all of their type's range, and rows of zeros between them, whose scale is the
