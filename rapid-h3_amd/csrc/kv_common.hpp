@@ -76,7 +76,7 @@ __device__ __forceinline__ int seq_of_row(const Seqs& s, int row, Seq& q) {
       const bool le = at < lo + n && s.cu[at] <= row;
       unsigned long long m = __builtin_amdgcn_ballot_w64(le);
       if constexpr (LANES < 64) m = (m >> (lane & ~(LANES - 1))) & ((1ull << LANES) - 1);
-      const int c = max(__popcll(m) - 1, 0);
+      const int c = max(static_cast<int>(__popcll(m)), 1) - 1;   // none: a row in front of cu[lo]
       n = min(step, lo + n - (lo + c * step));
       lo += c * step;
     }

@@ -600,6 +600,40 @@ def test_values_of_every_size_and_zero_ones(dev, fmt, form, rows):
     _check_lse(lse, rl, err)
 
 
+@pytest.mark.parametrize("b,first", [(1, 1), (5, 2), (70, 3), (300, 40)])
+def test_rows_in_front_of_the_first_sequence(dev, b, first):
+    """cu[0] > 0: the rows in front of it are no sequence's; nor is any row where all offsets lie behind the rows."""
+    hq, hkv, dim, page = 4, 2, 64, 16
+    new = [1 + i % 3 for i in range(b)]
+    lens = [n + i % 11 for i, n in enumerate(new)]
+    cu = [first]
+    for n in new:
+        cu.append(cu[-1] + n)
+    rows = cu[-1] + 2
+    table = [[i] for i in range(b)]
+    x = torch.randn(rows, hkv, dim, generator=_gen(50)).to(BF).to(dev)
+    c = kv.kv_cache(b, hkv, page, dim, I8, dev)
+    args = (_i32(table, dev), _i32(lens, dev), _i32(cu, dev))
+    kv.kv_write(c, x, -x, *args)
+    assert int((c.k_scale != 0).sum()) == (cu[-1] - first) * hkv
+    k, v = kv.kv_read(c, *args, rows=rows)
+    q, s = ok.quantise(x, I8)
+    want = (q.float() * s[..., None]).to(BF)
+    mine = slice(first, cu[-1])
+    assert torch.equal(k[mine], want[mine]) and torch.equal(v[mine], -want[mine])
+    assert not k[:first].any() and not k[cu[-1]:].any()
+    q = torch.randn(rows, hq, dim, generator=_gen(51)).to(BF).to(dev)
+    for form in FORMS:
+        out = torch.full_like(q, 5.0)
+        kv.kv_attention(q, c, *args, out=out, form=form)
+        assert bool((out[:first] == 5.0).all()) and bool((out[cu[-1]:] == 5.0).all())
+        ref, _, mag, err = ok.attention(q[mine], c, table, lens, [i - first for i in cu])
+        _check(out[mine], ref, mag, err, 3.1)
+        out.fill_(5.0)
+        kv.kv_attention(q, c, args[0], args[1], args[2] + rows, out=out, form=form)
+        assert bool((out == 5.0).all())
+
+
 def test_layouts(dev):
     """A cache that is a view of a buffer of several layers, strided queries and output, a wider table, out over q."""
     pages, heads, page, dim, hq = 9, 2, 32, 128, 6
