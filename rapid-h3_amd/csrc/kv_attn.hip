@@ -85,8 +85,13 @@ __global__ void __launch_bounds__(WPR > 4 ? WPR * 64 : 256) join_rows_kernel(Sou
     const Work w = dealt(load_blocks(own.a, g, blk), own.a.wgs, g);
     const int64_t all = static_cast<int64_t>(tok) * own.a.group + ig;
     int at = b;
+    auto of_prefix = [&](const Source& s, const Work& w, const Tiling& g) {
+      const SeqItems sw = seq_in(s.a, blk, 0);
+      const int64_t r = all - static_cast<int64_t>(sw.seq.first) * own.a.group;
+      if (r >= 0 && tok < sw.seq.first + sw.seq.n) p[1] = parts_of(s, w, sw, g, false, r, kvh);   // (not so where a cu falls)
+    };
     if (own.a.prefix) {
-      p[1] = parts_of(own, w, seq_in(own.a, blk, 0), g, false, all, kvh);
+      of_prefix(own, w, g);
       ++at;
     }
     while (at >= blk.at + 64) next_block(own.a, g, blk);
@@ -94,7 +99,7 @@ __global__ void __launch_bounds__(WPR > 4 ? WPR * 64 : 256) join_rows_kernel(Sou
     if (has_prefix) {
       const Tiling gp = tiling(prefix.chunk, prefix.rows);
       const Work wp = dealt(load_blocks(prefix.a, gp, blk), prefix.a.wgs, gp);
-      p[1] = parts_of(prefix, wp, seq_in(prefix.a, blk, 0), gp, false, all, kvh);
+      of_prefix(prefix, wp, gp);
     }
   }
   if (p[0].count + p[1].count == 0) return;    // one workgroup completed it
@@ -297,26 +302,17 @@ extern "C" int rh3_kv_attention(const rh3_kv_cache* cache, const void* q, int64_
     ws += p.slots * p.rows * (dim + 2);
     return Source{x, p.chunk, p.rows};
   };
-  const int prefix_width = static_cast<int>((prefix_len + cache->page - 1) / cache->page);
-  if (call.joined) {
-    a.prefix = prefix;
-    a.prefix_len = static_cast<int>(prefix_len);
-    a.prefix_width = prefix_width;
-  }
-  const Source own = source(a, call.own);
+  auto with_prefix = [&](AttnArgs x) {
+    x.prefix = prefix;
+    x.prefix_len = static_cast<int>(prefix_len);
+    x.prefix_width = static_cast<int>((prefix_len + cache->page - 1) / cache->page);
+    return x;
+  };
+  const Source own = source(call.joined ? with_prefix(a) : a, call.own);
   Source pre{};
   if (prefix_len > 0 && !call.joined) {
-    AttnArgs x = a;
-    x.s.table = prefix;
-    x.s.table_stride = 0;
-    x.s.lens = nullptr;
-    x.s.cu = nullptr;
-    x.s.width = prefix_width;
-    x.s.batch = 1;
-    x.s.per = x.s.rows;
-    x.s.fixed_len = static_cast<int>(prefix_len);
-    x.s.cap = x.s.width << x.c.log2page;
-    x.causal = 0;
+    AttnArgs x = with_prefix(a);
+    x.alone = 1;
     pre = source(x, call.prefix);
     launch(pre.a, call.prefix, fmt, dim, stream);
     if (const int e = launch_status("kv_attention (prefix)")) return e;

@@ -33,10 +33,10 @@ struct AttnArgs {
   float* lse;                // [rows][q heads] or null
   float* part_o;
   float* part_ml;
-  // A prefix that all rows see, taken as the first sequence (all rows its own, no causal limit) by the launch that also does the
-  // others; or null
+  // A prefix that all sequences' rows see, taken as the first sequence (those rows its own, no causal limit) by the launch that
+  // also does the others, or by one for it alone; or null
   const int32_t* prefix;
-  int prefix_len, prefix_width;
+  int prefix_len, prefix_width, alone;
   int64_t items;             // slots of completed items
   int wgs;
   int keep;                  // leave a part for every item, also for those that one workgroup completes
@@ -78,10 +78,13 @@ RH3_HD int share_of(const Work& w, int64_t u) {
 }
 
 // a sequence of the launch: the prefix, if there is one, before the batch's
-RH3_HD int sequences(const AttnArgs& a) { return a.s.batch + (a.prefix != nullptr); }
+RH3_HD int sequences(const AttnArgs& a) { return (a.alone ? 0 : a.s.batch) + (a.prefix != nullptr); }
 RH3_HD Seq sequence(const AttnArgs& a, int i) {
   if (a.prefix) {
-    if (i == 0) return Seq{0, a.s.rows, a.prefix_len};
+    if (i == 0) {
+      const int first = a.s.cu ? clamped(a.s.cu[0], 0, a.s.rows) : 0;
+      return Seq{first, (a.s.cu ? clamped(a.s.cu[a.s.batch], first, a.s.rows) : a.s.rows) - first, a.prefix_len};
+    }
     --i;
   }
   return seq_at(a.s, i);

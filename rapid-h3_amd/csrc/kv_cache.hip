@@ -223,7 +223,6 @@ int check_seqs(const char* name, const Cache& c, const int32_t* table, int64_t t
   s.batch = static_cast<int>(batch);
   s.rows = static_cast<int>(rows);
   s.per = cu ? 0 : static_cast<int>(rows / batch);
-  s.fixed_len = 0;
   s.cap = static_cast<int>(width << c.log2page);
   return RH3_OK;
 }

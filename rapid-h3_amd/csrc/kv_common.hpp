@@ -32,13 +32,13 @@ struct Cache {
 };
 
 // batch sequences: `rows` packed rows, those of sequence b at cu[b] .. cu[b + 1] (cu null: `per` each); lens[b] cached
-// positions (lens null: fixed_len). The last rows of a sequence are its last positions.
+// positions. The last rows of a sequence are its last positions.
 struct Seqs {
   const int32_t* table;
   int64_t table_stride;
   const int32_t* lens;
   const int32_t* cu;
-  int width, batch, rows, per, fixed_len, cap;   // cap: width * page
+  int width, batch, rows, per, cap;   // cap: width * page
 };
 
 struct Seq {
@@ -55,7 +55,7 @@ RH3_HD Seq seq_at(const Seqs& s, int b) {
     r.first = b * s.per;
     r.n = s.per;
   }
-  r.len = clamped(s.lens ? s.lens[b] : s.fixed_len, 0, s.cap);
+  r.len = clamped(s.lens[b], 0, s.cap);
   return r;
 }
 

@@ -634,6 +634,35 @@ def test_rows_in_front_of_the_first_sequence(dev, b, first):
         assert bool((out == 5.0).all())
 
 
+@pytest.mark.parametrize("form,b,new,prefix_len", [("token", 5, 3, 333), ("chunk", 5, 3, 333), ("chunk", 3, 50, 90), (None, 5, 3, 333),
+                                                   (None, 64, 1, 60001)])
+@pytest.mark.parametrize("first", [0, 2])
+def test_shared_rows_that_no_sequence_has(dev, form, b, new, prefix_len, first):
+    """Rows in front of cu[0] and behind cu[B] of a call with a prefix: neither their results nor, whatever they hold, those of the
+    other rows are touched."""
+    hq, hkv, dim, page = 8, 2, 128, 256
+    lens = [1 + 5 * i for i in range(b)]
+    pre = -(-prefix_len // page)
+    table = _tables(2 * b + pre, 2, b, 24)
+    used = {p for t in table for p in t}
+    common = [p for p in range(2 * b + pre) if p not in used]
+    c = _pool(dev, I8, 2 * b + pre, hkv, page, dim, 25)
+    cu = [first + new * i for i in range(b + 1)]
+    mine = slice(cu[0], cu[-1])
+    q = torch.randn(cu[-1] + 9, hq, dim, generator=_gen(26)).to(BF).to(dev)
+    got = []
+    for other in (1.0, 1e30, math.nan, math.inf):
+        q[:cu[0]], q[cu[-1]:] = other, other
+        out = torch.full_like(q, 5.0)
+        _call(q, c, table, lens, cu, common, prefix_len, dev, out=out, form=form)
+        assert bool((out[:cu[0]] == 5.0).all()) and bool((out[cu[-1]:] == 5.0).all())
+        got.append(out[mine].clone())
+    assert all(torch.equal(got[0].view(torch.int16), x.view(torch.int16)) for x in got[1:])
+    cu0 = [x - first for x in cu]
+    ref, _, mag, err = ok.attention(q[mine], c, table, lens, cu0, prefix=common, prefix_len=prefix_len)
+    _check(got[0], ref, mag, err, 3.1)
+
+
 def test_layouts(dev):
     """A cache that is a view of a buffer of several layers, strided queries and output, a wider table, out over q."""
     pages, heads, page, dim, hq = 9, 2, 32, 128, 6
