@@ -466,10 +466,11 @@ int rh3_attention_f8_forward(int64_t Sq, int64_t Sk, int64_t H, float scale, int
  * [pages][heads][page] (strides multiples of 4), all 16-byte aligned. The value of a code is code * scale.
  *
  * A call names `batch` sequences: position p of sequence b lies in page table[b * table_stride + p / page] (width entries; an
- * entry outside [0, pages) is an absent page, whose positions hold nothing); lens[b] positions are cached (clamped to
- * [0, width * page]); its rows in the call are cu[b] .. cu[b + 1] of `rows` (cu NULL: rows / batch each) and are its last
- * positions: row i of n is position lens[b] - n + i. Rows behind cu[batch] are neither read nor written. table, lens and cu are
- * device memory and may change between replays of a captured call; no content of theirs leads outside the buffers.
+ * entry outside [0, pages) is an absent page, whose positions hold nothing, and neither do those past the table); lens[b]
+ * positions are cached; its rows in the call are cu[b] .. cu[b + 1] of `rows` (cu NULL: rows / batch each) and are its last
+ * positions: row i of n = cu[b + 1] - cu[b] is position lens[b] - n + i, also where some of the n lie outside 0 .. rows, which the
+ * call does not have. Rows in front of cu[0] and behind cu[batch] are neither read nor written. table, lens and cu are device
+ * memory and may change between replays of a captured call; no content of theirs leads outside the buffers.
  * Rows [rows][heads][dim]: last dim contiguous, strides multiples of 8, 16-byte aligned.
  * ------------------------------------------------------------------------------------------- */
 typedef struct rh3_kv_cache {
@@ -483,8 +484,8 @@ typedef struct rh3_kv_cache {
 } rh3_kv_cache;
 
 /* Quantizes rows of k and v (bf16, fp16 or fp32) into their positions: s = max(amax / QMAX, 1e-12) (127 or 448), code =
- * round_half_even(x / s); a row with an infinity or a NaN gets s = NaN and codes 0. Rows whose position is negative or in an
- * absent page are skipped. A position that several rows of one call name (a page that two sequences share, or that a table
+ * round_half_even(x / s); a row with an infinity or a NaN gets s = NaN and codes 0. Rows whose position is negative, past the
+ * table or in an absent page are skipped. A position that several rows of one call name (a page that two sequences share, or that a table
  * names twice) ends with a mixture of them: name each position written once. */
 int rh3_kv_write(const rh3_kv_cache* cache, const void* k, int64_t k_st, int64_t k_sh, const void* v, int64_t v_st,
                  int64_t v_sh, int dtype, int64_t rows, const int32_t* table, int64_t table_stride, int64_t width,

@@ -2,7 +2,7 @@
 // bytes), kv_chunk.hip many (bound by the matrix units), kv_attn.hip joins the parts that either leaves and holds the entry points.
 //
 // For a query row i of a sequence of n rows and `len` cached positions: o_i = sum_j p_ij v_j / sum_j p_ij with
-// p_ij = exp(scale q_i.k_j) over j < len, and j <= len - n + i if causal. A K/V head's query rows are its group's heads of every
+// p_ij = exp(scale q_i.k_j) over j < len, and j <= pos + i (pos = len - n) if causal. A K/V head's query rows are its group's heads of every
 // token of the sequence, numbered token * group + head in the group, so that the group shares each key and value that is read.
 //
 // Arithmetic. Codes are small integers (int8) or 4-bit significands (e4m3): exact in f16. A query row is scaled by the power of
@@ -83,7 +83,7 @@ RH3_HD Seq sequence(const AttnArgs& a, int i) {
   if (a.prefix) {
     if (i == 0) {
       const int first = a.s.cu ? clamped(a.s.cu[0], 0, a.s.rows) : 0;
-      return Seq{first, (a.s.cu ? clamped(a.s.cu[a.s.batch], first, a.s.rows) : a.s.rows) - first, a.prefix_len};
+      return Seq{first, (a.s.cu ? clamped(a.s.cu[a.s.batch], first, a.s.rows) : a.s.rows) - first, a.prefix_len, 0};
     }
     --i;
   }
@@ -140,7 +140,7 @@ __device__ __forceinline__ void load_block(const AttnArgs& a, const Tiling& g, i
   b.at = at;
   b.base = base;
   b.items_base = items_base;
-  b.seq = Seq{0, 0, 0};
+  b.seq = Seq{0, 0, 0, 0};
   SeqWork w{0, 1, 0};
   if (i < sequences(a)) {
     b.seq = sequence(a, i);
@@ -177,6 +177,7 @@ __device__ __forceinline__ SeqItems seq_in(const AttnArgs& a, const Block& b, in
   r.seq.first = __builtin_amdgcn_readlane(b.seq.first, l);
   r.seq.n = __builtin_amdgcn_readlane(b.seq.n, l);
   r.seq.len = __builtin_amdgcn_readlane(b.seq.len, l);
+  r.seq.pos = __builtin_amdgcn_readlane(b.seq.pos, l);
   r.row_tiles = __builtin_amdgcn_readlane(b.row_tiles, l);
   r.span = __builtin_amdgcn_readlane(b.span, l);
   r.before = b.base + (l ? lane64(b.units, l - 1) : 0);

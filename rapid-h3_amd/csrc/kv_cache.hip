@@ -20,7 +20,7 @@ namespace {
 constexpr int NT = 256;
 
 // where a row of the call lies in the cache: offsets of its codes and scale without the head's part; false if it lies nowhere
-// (no sequence has the row, its position is before the first, its page is absent). `mine`: a sequence has the row.
+// (no sequence has the row, its position is before the first or past the table, its page is absent). `mine`: a sequence has the row.
 struct Place {
   int64_t code, scale;
   bool mine, there;
@@ -32,11 +32,11 @@ __device__ __forceinline__ Place place_of(const Seqs& s, const Cache& c, int row
   const int b = seq_of_row<D / 8 == 16 ? 16 : 8>(s, min(row, s.rows - 1), q);
   if (b < 0 || row >= s.rows) return p;
   p.mine = true;
-  const int64_t pos = static_cast<int64_t>(q.len) - q.n + (row - q.first);
-  if (pos < 0) return p;
-  const int pg = page_of(s, c, b, static_cast<int>(pos));
+  const int pos = q.pos + (row - q.first);
+  if (pos < 0 || pos >= s.cap) return p;
+  const int pg = page_of(s, c, b, pos);
   if (pg < 0) return p;
-  const int64_t off = pos & ((1 << c.log2page) - 1);
+  const int off = pos & ((1 << c.log2page) - 1);
   p.code = pg * c.page_stride + off * D;
   p.scale = pg * c.spage_stride + off;
   p.there = true;
@@ -208,10 +208,10 @@ int check_cache(const char* name, const rh3_kv_cache* x, Cache& c) {
 
 int check_seqs(const char* name, const Cache& c, const int32_t* table, int64_t table_stride, int64_t width, const int32_t* lens,
                const int32_t* cu, int64_t batch, int64_t rows, Seqs& s) {
-  RH3_REQUIRE(rows >= 0 && rows <= (int64_t{1} << 30), "%s: %lld rows", name, static_cast<long long>(rows));
+  RH3_REQUIRE(rows >= 0 && rows <= MAX_ROWS, "%s: %lld rows", name, static_cast<long long>(rows));
   RH3_REQUIRE(batch >= 1 && batch <= 65536, "%s: %lld sequences (1 to 65536)", name, static_cast<long long>(batch));
   RH3_REQUIRE(table && lens, "%s: null page table or lengths", name);
-  RH3_REQUIRE(width >= 1 && table_stride >= (batch > 1 ? width : 0) && (width << c.log2page) <= (int64_t{1} << 30),
+  RH3_REQUIRE(width >= 1 && table_stride >= (batch > 1 ? width : 0) && (width << c.log2page) <= MAX_ROWS,
               "%s: page table of %lld entries per sequence, stride %lld", name, static_cast<long long>(width), static_cast<long long>(table_stride));
   RH3_REQUIRE(cu || rows % batch == 0, "%s: %lld rows do not divide over %lld sequences (give their offsets)", name,
               static_cast<long long>(rows), static_cast<long long>(batch));

@@ -128,7 +128,7 @@ __global__ void __launch_bounds__(WAVES * 64, 2) chunk_kernel(AttnArgs a) {
     const int rt = causal ? tile_at_place(at, sw.row_tiles) : at;
     const int rows = sq.n * a.group;
     const int tok_last = scalar(min(rows - 1, rt * R + R - 1) / a.group);
-    const int seen = causal ? min(sq.len, max(0, sq.len - sq.n + tok_last + 1)) : sq.len;   // keys that some row sees
+    const int seen = causal ? min(sq.len, max(0, sq.pos + tok_last + 1)) : sq.len;   // keys that some row sees
     const int t1 = min(share_t1, (seen + KT - 1) / KT);
 
     const int row = rt * R + wave * 32 + l32;
@@ -142,11 +142,11 @@ __global__ void __launch_bounds__(WAVES * 64, 2) chunk_kernel(AttnArgs a) {
     int vref;   // bits of a power of two, the same in all lanes
     bool full;  // no key of the share in an absent page
     bool apart; // query rows with a power of two each, weights with a unit to each row
-    const int lim = causal ? min(sq.len, sq.len - sq.n + tok + 1) : sq.len;
+    const int lim = causal ? min(sq.len, sq.pos + tok + 1) : sq.len;
     // of the wave's rows: keys that all see, keys that some see
     const int r0 = rt * R + wave * 32, r1 = min(rows - 1, r0 + 31);
-    const int low = causal ? min(sq.len, sq.len - sq.n + scalar(r0 / a.group) + 1) : sq.len;
-    const int top_key = r0 >= rows ? 0 : causal ? min(sq.len, sq.len - sq.n + scalar(r1 / a.group) + 1) : sq.len;
+    const int low = causal ? min(sq.len, sq.pos + scalar(r0 / a.group) + 1) : sq.len;
+    const int top_key = r0 >= rows ? 0 : causal ? min(sq.len, sq.pos + scalar(r1 / a.group) + 1) : sq.len;
 
     f16_t o[DT];
     float ref = NO_REF, sum = 0.0f;

@@ -32,7 +32,7 @@ struct Cache {
 };
 
 // batch sequences: `rows` packed rows, those of sequence b at cu[b] .. cu[b + 1] (cu null: `per` each); lens[b] cached
-// positions. The last rows of a sequence are its last positions.
+// positions. The rows of a sequence are its last positions, row cu[b + 1] - 1 the last of all, whether the call has that row or not.
 struct Seqs {
   const int32_t* table;
   int64_t table_stride;
@@ -42,20 +42,28 @@ struct Seqs {
 };
 
 struct Seq {
-  int first, n, len;   // rows [first, first + n), cached positions
+  int first, n, len;   // rows [first, first + n), cached positions that the table has
+  int pos;             // of row `first`: negative or past len where it has no place
 };
+
+constexpr int64_t MAX_ROWS = int64_t{1} << 30;   // of a call, and positions of a table
 
 RH3_HD int clamped(int v, int lo, int hi) { return v < lo ? lo : v > hi ? hi : v; }
 RH3_HD Seq seq_at(const Seqs& s, int b) {
   Seq r;
+  int64_t end;
   if (s.cu) {
+    end = s.cu[b + 1];
     r.first = clamped(s.cu[b], 0, s.rows);
-    r.n = clamped(s.cu[b + 1], r.first, s.rows) - r.first;
+    r.n = clamped(static_cast<int>(end), r.first, s.rows) - r.first;
   } else {
     r.first = b * s.per;
     r.n = s.per;
+    end = r.first + r.n;
   }
-  r.len = clamped(s.lens[b], 0, s.cap);
+  const int64_t len = s.lens[b], pos = len - end + r.first;
+  r.len = clamped(static_cast<int>(len), 0, s.cap);
+  r.pos = static_cast<int>(pos < -MAX_ROWS ? -MAX_ROWS : pos > s.cap ? s.cap : pos);
   return r;
 }
 

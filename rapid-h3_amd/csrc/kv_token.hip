@@ -287,7 +287,7 @@ __global__ void __launch_bounds__(NT, 2) token_kernel(AttnArgs a) {
       const uint16_t* src = static_cast<const uint16_t*>(a.q) + (sq.first + tok) * a.q_st + hd * a.q_sh + 16 * g;
 #pragma unroll
       for (int c = 0; c < D / 32; ++c) raw[m][c] = *reinterpret_cast<const uint4*>(src + 64 * (c >> 1) + 8 * (c & 1));
-      lim[m] = causal ? min(sq.len, sq.len - sq.n + tok + 1) : sq.len;
+      lim[m] = causal ? min(sq.len, sq.pos + tok + 1) : sq.len;
     }
     // the first keys and values are on their way while the query rows come in
     Tile<D> tile;
@@ -315,7 +315,7 @@ __global__ void __launch_bounds__(NT, 2) token_kernel(AttnArgs a) {
       for (int c = 0; c < D / 32; ++c) q[m][c] = q_f16(x[c], e);
       qf[m] = __builtin_amdgcn_ldexpf(a.scale_log2, -e);
     }
-    const int low = causal ? min(sq.len, sq.len - sq.n + scalar((rt * R) / a.group) + 1) : sq.len;
+    const int low = causal ? min(sq.len, sq.pos + scalar((rt * R) / a.group) + 1) : sq.len;
 
     State<D, MT> st;
 #pragma unroll

@@ -6,11 +6,13 @@ they are written, by the row quantizers' rule over one head (s = max(amax / QMAX
 or 448), and attention reads the codes where they lie. The reference has no counterpart.
 
 Every call names its sequences alike:
-  table [B, W] int32   the pages of each sequence in order; an entry outside [0, pages) is an absent page
+  table [B, W] int32   the pages of each sequence in order; an entry outside [0, pages) is an absent page, and so is what lies
+                       past the table
   lens [B] int32       cached positions of each sequence, the rows of this call included
   cu [B + 1] int32     where each sequence's rows begin and end among the call's rows; None: the same number each
 The rows of a sequence are its last positions: row i of n is position lens[b] - n + i. The three live on the GPU and are read
-by the kernels, so a captured call follows what is written into them between replays. Rows behind cu[B] stay as they are.
+by the kernels, so a captured call follows what is written into them between replays. Rows in front of cu[0] and behind cu[B]
+are not read and stay as they are; of rows that cu names but the call does not have, it takes none.
 """
 import contextlib
 import ctypes
@@ -121,7 +123,7 @@ def _rows_call(name, entry, what, cache, k, v, table, lens, cu):
 
 def kv_write(cache, k, v, table, lens, cu=None):
     """Quantise rows k, v [rows, heads, dim] (bf16, fp16 or fp32, strided ok) into their positions. Rows at a negative
-    position or in an absent page are skipped; a row that holds an infinity or a NaN is kept as NaN (its scale). A position
+    position, past the table or in an absent page are skipped; a row that holds an infinity or a NaN is kept as NaN (its scale). A position
     that two rows of a call name (a page that sequences share, or that a table names twice) ends with a mixture of them."""
     _rows_call("kv_write", "rh3_kv_write", ("k", "v"), cache, k, v, table, lens, cu)
 

@@ -663,6 +663,62 @@ def test_shared_rows_that_no_sequence_has(dev, form, b, new, prefix_len, first):
     _check(got[0], ref, mag, err, 3.1)
 
 
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("fmt,dim", [(I8, 64), (F8, 128)])
+@pytest.mark.parametrize("lens,cu,rows", [
+    ([40, 25, 33], [0, 5, 12, 30], 20),           # the last sequence's rows end behind the call's
+    ([40, 25, 33], [-7, 5, 12, 20], 20),          # the first one's begin in front of them
+    ([40, 25, 33], [-300, -4, 2, 400], 20),
+    ([60, 48, 33], [0, 12, 24, 30], 30),          # sequences that have outgrown their tables
+    ([90, 47, 33], [0, 12, 24, 30], 30),
+    ([60, 100, 90], None, 30),
+])
+def test_rows_outside_the_call_or_the_table(dev, fmt, dim, form, lens, cu, rows):
+    """A row's position is lens[b] - (cu[b + 1] - cu[b]) + i also where the call has only some of the sequence's rows, or the table
+    not all of its positions: what it does not have is skipped, read as 0 and not seen, and nothing else is written or read in its
+    place."""
+    b, hq, hkv, page = 3, 4, 2, 16
+    table = [[4, 7, 1], [0, 3, 8], [2, 6, 5]]                    # 48 positions
+    longer = [t + [-1] * 4 for t in table]                       # the oracle's: absent pages behind them
+    whole = [rows // b * i for i in range(b + 1)] if cu is None else cu
+    c = _pool(dev, fmt, 9, hkv, page, dim, 52)
+    before = [t.clone() for t in (c.k.view(torch.uint8), c.v.view(torch.uint8), c.k_scale, c.v_scale)]
+    args = (_i32(table, dev), _i32(lens, dev), None if cu is None else _i32(cu, dev))
+    x, y = _rows(rows, hkv, dim, BF, 53, False, dev), _rows(rows, hkv, dim, BF, 54, False, dev)
+    place = {}                                                   # row -> (page, offset) or None, of rows that a sequence has
+    for i in range(b):
+        for r in range(max(whole[i], 0), min(whole[i + 1], rows)):
+            place[r] = ok.slot(longer, 9, page, i, lens[i] - whole[i + 1] + r)
+    got = kv.kv_read(c, *args, rows=rows, dtype=F32)
+    for t, codes, scales in ((got[0], before[0], before[2]), (got[1], before[1], before[3])):
+        for r in range(rows):
+            at = place.get(r)
+            want = codes[at[0], :, at[1]].view(fmt).float() * scales[at[0], :, at[1]][:, None] if at else torch.zeros_like(t[r])
+            assert torch.equal(t[r], want), r
+    kv.kv_write(c, x, y, *args)
+    for t, codes, scales in ((x, before[0], before[2]), (y, before[1], before[3])):
+        q, s = ok.quantise(t, fmt)
+        for r, at in place.items():
+            if at:
+                codes[at[0], :, at[1]], scales[at[0], :, at[1]] = q[r].view(torch.uint8), s[r]
+    for t, u in zip(before, (c.k.view(torch.uint8), c.v.view(torch.uint8), c.k_scale, c.v_scale)):
+        assert torch.equal(t, u)
+    # attention: the oracle over all rows that the offsets name, of which the call has some
+    q = torch.randn(max(whole[-1], rows) - whole[0], hq, dim, generator=_gen(55)).to(BF).to(dev)
+    mine = slice(-whole[0], -whole[0] + rows)
+    for causal in (True, False):
+        out, lse = kv.kv_attention(q[mine], c, *args, causal=causal, lse=True, form=form)
+        ref, rl, mag, err = (t[mine] for t in ok.attention(q, c, longer, [min(n, 48) if not causal else n for n in lens],
+                                                           [i - whole[0] for i in whole], causal))
+        # Value rows here differ by up to e^+-6 and some weights vanish beside others. A weight is at least 2^10 for the row's largest
+        # (in the units that f16 has it in), and off by half of f16's last place, 2^-25, where it is small: 2^-35 of the largest
+        # value for each of a row's up to 48 keys, also in a channel where the large ones hold 0.
+        most = max(float(t.max()) for t in ok.gather(c, sum(table, []), 144)[1].abs())
+        far = (out.double() - ref).abs() <= 48 * 2.0 ** -35 * most
+        _check(torch.where(far, ref.to(BF), out), ref, mag, err, 3.1)
+        _check_lse(lse, rl, err)
+
+
 def test_layouts(dev):
     """A cache that is a view of a buffer of several layers, strided queries and output, a wider table, out over q."""
     pages, heads, page, dim, hq = 9, 2, 32, 128, 6
