@@ -130,9 +130,11 @@ def kv_write(cache, k, v, table, lens, cu=None):
 
 def kv_read(cache, table, lens, cu=None, rows=None, dtype=torch.bfloat16, out=None):
     """The values (code * scale, rounded once to dtype) of the last cu[b + 1] - cu[b] positions of each sequence, packed as
-    kv_write takes them: k, v [rows, heads, dim]. rows: how many in all (cu[B], which only the GPU knows; without cu by
-    default one of each sequence). Positions that hold nothing read as 0. out: a pair of tensors to write into."""
+    kv_write takes them: k, v [rows, heads, dim]. rows: how many in all (cu[B], which only the GPU knows and has to be given
+    with cu; without cu by default one of each sequence). Positions that hold nothing read as 0. out: a pair of tensors to write into."""
     if out is None:
+        if rows is None and cu is not None:
+            raise ValueError("kv_read: with cu, rows (cu[B], how many in all) or out must be given")
         n = table.shape[0] if rows is None else int(rows)
         if dtype not in _ROW:
             raise TypeError(f"kv_read: bf16, fp16 or fp32 values, got {dtype}")

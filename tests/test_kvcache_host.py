@@ -122,3 +122,12 @@ def test_wrappers_refuse():
         kv._seqs("f", Cache, t, n[:2], None, -1)
     with pytest.raises(RuntimeError, match="cu must be"):
         kv._seqs("f", Cache, t, n, n, -1)
+
+
+def test_read_needs_its_number_of_rows():
+    """With offsets, whose last only the GPU knows, kv_read takes no number of its own choice."""
+    class Cache:
+        heads, dim, page, device, gpu = 2, 128, 64, torch.device("cpu"), -1
+    t, n = torch.zeros((3, 1), dtype=torch.int32), torch.ones(3, dtype=torch.int32)
+    with pytest.raises(ValueError, match="rows .* must be given"):
+        kv.kv_read(Cache, t, n, torch.tensor([0, 2, 3, 9], dtype=torch.int32))
