@@ -280,6 +280,20 @@ extern "C" int rh3_kv_attention(const rh3_kv_cache* cache, const void* q, int64_
   const Call call = call_of(rows, q_heads, a.c.heads, dim, width * cache->page, batch, cu == nullptr, prefix_len, form);
   RH3_REQUIRE(workspace && aligned16(workspace) && workspace_bytes >= call.bytes,
               "kv_attention: workspace of %lld bytes needed, %lld given", static_cast<long long>(call.bytes), static_cast<long long>(workspace_bytes));
+  // Parts that a row may have: the workgroups over the least count of items, no more than the keys make. Measured (kernel us, by
+  // shares / rows on 4 waves / on 16): 8 parts of 32 rows 5.1 / 4.7 / 5.7, 16 of 224 rows - / 6.3 / 7.7. Waves of one row each find
+  // their way through the shares themselves, so many rows, which fill the chip, have one (us, rows on 1 wave / on 4): 192 rows
+  // behind a prefix 7.9 / 6.1, 512 21.2 / 20.8 (whole calls, as those that follow), 768 21.6 / 22.1, 1,024 24.8 / 26.2, 1,536 29.5 /
+  // 32.4; 2,048 of 33 parts 13.5 / 19.2; 4,096 of 16 parts 72 / 78 (whole calls).
+  const int64_t ids = rows * q_heads, cap = width * cache->page + prefix_len;
+  const int64_t tiles = (rows * (q_heads / a.c.heads) / batch + call.own.rows - 1) / call.own.rows;
+  const int64_t shared = call.own.wgs / (batch * a.c.heads * (tiles > 0 ? tiles : 1));
+  const int64_t most = cap / (call.own.chunk ? 8 * CHUNK_KEYS : 4 * TOKEN_KEYS), parts = shared < most ? shared : most;
+  const bool by_shares = prefix_len == 0 && parts <= 8;
+  const int wpr = parts > 32 ? 16 : ids <= 2 * device_cus() ? 4 : 1;
+  const int64_t waves = wpr == 1 ? (ids + 3) / 4 : ids;   // workgroups of the join by rows
+  RH3_REQUIRE(by_shares || waves * (wpr == 16 ? 4 : 1) <= MAX_GRID_256, "kv_attention: %lld rows of %lld heads behind a prefix in one call",
+              static_cast<long long>(rows), static_cast<long long>(q_heads));
   a.q = q;
   a.q_st = q_st;
   a.q_sh = q_sh;
@@ -319,27 +333,15 @@ extern "C" int rh3_kv_attention(const rh3_kv_cache* cache, const void* q, int64_
   }
   launch(own.a, call.own, fmt, dim, stream);
   if (const int e = launch_status("kv_attention")) return e;
-  // Parts that a row may have: the workgroups over the least count of items, no more than the keys make. Measured (kernel us, by
-  // shares / rows on 4 waves / on 16): 8 parts of 32 rows 5.1 / 4.7 / 5.7, 16 of 224 rows - / 6.3 / 7.7. Waves of one row each find
-  // their way through the shares themselves, so many rows, which fill the chip, have one (us, rows on 1 wave / on 4): 192 rows
-  // behind a prefix 7.9 / 6.1, 512 21.2 / 20.8 (whole calls, as those that follow), 768 21.6 / 22.1, 1,024 24.8 / 26.2, 1,536 29.5 /
-  // 32.4; 2,048 of 33 parts 13.5 / 19.2; 4,096 of 16 parts 72 / 78 (whole calls).
-  const int64_t ids = rows * q_heads, cap = width * cache->page + prefix_len;
-  const int64_t tiles = (rows * a.group / batch + call.own.rows - 1) / call.own.rows;
-  const int64_t shared = call.own.wgs / (batch * a.c.heads * (tiles > 0 ? tiles : 1));
-  const int64_t most = cap / (call.own.chunk ? 8 * CHUNK_KEYS : 4 * TOKEN_KEYS), parts = shared < most ? shared : most;
   const int has = prefix_len > 0 && !call.joined;
-  if (prefix_len == 0 && parts <= 8) {
+  if (by_shares) {
     const dim3 grid(static_cast<uint32_t>(call.own.wgs), static_cast<uint32_t>(call.own.rows / 16));
     if (dim == 128) hipLaunchKernelGGL((join_shares_kernel<128>), grid, dim3(256), 0, stream, own);
     else hipLaunchKernelGGL((join_shares_kernel<64>), grid, dim3(256), 0, stream, own);
     return launch_status("kv_attention (join)");
   }
-  const int wpr = parts > 32 ? 16 : ids <= 2 * device_cus() ? 4 : 1;
-  const int64_t grid = wpr == 1 ? (ids + 3) / 4 : ids;
-  RH3_REQUIRE(grid * (wpr == 16 ? 4 : 1) <= MAX_GRID_256, "kv_attention: %lld rows in one call", static_cast<long long>(rows));
   auto go = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(grid)), dim3(wpr == 16 ? 1024 : 256), 0, stream, own, pre, has);
+    hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(waves)), dim3(wpr == 16 ? 1024 : 256), 0, stream, own, pre, has);
   };
   if (dim == 128) wpr == 16 ? go(join_rows_kernel<128, 16>) : wpr == 4 ? go(join_rows_kernel<128, 4>) : go(join_rows_kernel<128, 1>);
   else wpr == 16 ? go(join_rows_kernel<64, 16>) : wpr == 4 ? go(join_rows_kernel<64, 4>) : go(join_rows_kernel<64, 1>);

@@ -131,3 +131,11 @@ def test_read_needs_its_number_of_rows():
     t, n = torch.zeros((3, 1), dtype=torch.int32), torch.ones(3, dtype=torch.int32)
     with pytest.raises(ValueError, match="rows .* must be given"):
         kv.kv_read(Cache, t, n, torch.tensor([0, 2, 3, 9], dtype=torch.int32))
+
+
+def test_join_refusal_comes_before_any_launch():
+    """More (row, head) pairs behind a prefix than the join's grid holds: refused as an argument, with nothing launched (on a machine
+    without a GPU a launch would be another error)."""
+    rows = 1 << 21
+    assert _attend(_desc(), rows=rows, hq=64, prefix=FAKE, prefix_len=100, n=1 << 62) == 1
+    assert f"{rows} rows of 64 heads" in nat.last_error()
