@@ -505,7 +505,7 @@ int rh3_kv_read(const rh3_kv_cache* cache, void* k, int64_t k_st, int64_t k_sh, 
  * stands for the lengths, which only the device knows.
  * The workspace (capacity: width * page; even: 1 where cu is NULL) holds the parts of rows whose keys several workgroups share;
  * how keys are split depends on the sizes, lengths and the CU count, and with it the last bits of the result; the same call
- * gives the same bits. */
+ * gives the same bits. The size is 0 for sizes that attention refuses or that leave nothing to do. */
 int64_t rh3_kv_attention_workspace_bytes(int64_t q_heads, int64_t heads, int64_t dim, int64_t rows, int64_t capacity,
                                          int64_t batch, int even, int64_t prefix_len, int form);
 int rh3_kv_attention(const rh3_kv_cache* cache, const void* q, int64_t q_st, int64_t q_sh, int64_t q_heads, int dtype,

@@ -251,7 +251,9 @@ using namespace rh3::kv;
 
 extern "C" int64_t rh3_kv_attention_workspace_bytes(int64_t q_heads, int64_t heads, int64_t dim, int64_t rows, int64_t capacity,
                                                     int64_t batch, int even, int64_t prefix_len, int form) {
-  if (heads < 1 || q_heads < heads || q_heads % heads || rows < 1 || batch < 1 || capacity < 1) return 0;
+  if (heads < 1 || heads > 65535 || q_heads < heads || q_heads % heads || rows < 1 || rows > MAX_ROWS || q_heads / heads > MAX_ROWS / rows ||
+      batch < 1 || batch > 65536 || capacity < 1 || capacity > MAX_ROWS || prefix_len < 0 || prefix_len > MAX_ROWS || (dim != 64 && dim != 128))
+    return 0;
   return call_of(rows, q_heads, heads, dim, capacity, batch, even != 0, prefix_len, form).bytes;
 }
 
@@ -268,12 +270,12 @@ extern "C" int rh3_kv_attention(const rh3_kv_cache* cache, const void* q, int64_
   RH3_REQUIRE(dtype == RH3_DTYPE_BF16 || dtype == RH3_DTYPE_F16, "kv_attention: query type %d (bf16 or fp16)", dtype);
   RH3_REQUIRE(q_heads >= a.c.heads && q_heads % a.c.heads == 0, "kv_attention: %lld query heads do not divide over %d K/V heads",
               static_cast<long long>(q_heads), a.c.heads);
-  RH3_REQUIRE(rows * (q_heads / a.c.heads) <= (int64_t{1} << 30), "kv_attention: %lld rows of %lld heads", static_cast<long long>(rows),
+  RH3_REQUIRE(q_heads / a.c.heads <= MAX_ROWS / rows, "kv_attention: %lld rows of %lld heads", static_cast<long long>(rows),
               static_cast<long long>(q_heads));
   RH3_REQUIRE(q && out, "kv_attention: null q or out");
   RH3_REQUIRE(aligned16(q) && aligned16(out) && q_st % 8 == 0 && q_sh % 8 == 0 && o_st % 8 == 0 && o_sh % 8 == 0,
               "kv_attention: q and out must be 16-byte aligned with strides that are multiples of 8");
-  RH3_REQUIRE(prefix_len >= 0 && prefix_len <= (int64_t{1} << 30) && (prefix_len == 0 || prefix), "kv_attention: prefix of %lld positions without pages",
+  RH3_REQUIRE(prefix_len >= 0 && prefix_len <= MAX_ROWS && (prefix_len == 0 || prefix), "kv_attention: prefix of %lld positions without pages",
               static_cast<long long>(prefix_len));
   RH3_REQUIRE(form >= RH3_KV_BY_SIZE && form <= RH3_KV_CHUNK, "kv_attention: form %d", form);
   const int dim = static_cast<int>(cache->dim), fmt = static_cast<int>(cache->format);

@@ -211,7 +211,7 @@ int check_seqs(const char* name, const Cache& c, const int32_t* table, int64_t t
   RH3_REQUIRE(rows >= 0 && rows <= MAX_ROWS, "%s: %lld rows", name, static_cast<long long>(rows));
   RH3_REQUIRE(batch >= 1 && batch <= 65536, "%s: %lld sequences (1 to 65536)", name, static_cast<long long>(batch));
   RH3_REQUIRE(table && lens, "%s: null page table or lengths", name);
-  RH3_REQUIRE(width >= 1 && table_stride >= (batch > 1 ? width : 0) && (width << c.log2page) <= MAX_ROWS,
+  RH3_REQUIRE(width >= 1 && table_stride >= (batch > 1 ? width : 0) && width <= (MAX_ROWS >> c.log2page),
               "%s: page table of %lld entries per sequence, stride %lld", name, static_cast<long long>(width), static_cast<long long>(table_stride));
   RH3_REQUIRE(cu || rows % batch == 0, "%s: %lld rows do not divide over %lld sequences (give their offsets)", name,
               static_cast<long long>(rows), static_cast<long long>(batch));

@@ -139,3 +139,17 @@ def test_join_refusal_comes_before_any_launch():
     rows = 1 << 21
     assert _attend(_desc(), rows=rows, hq=64, prefix=FAKE, prefix_len=100, n=1 << 62) == 1
     assert f"{rows} rows of 64 heads" in nat.last_error()
+
+
+def test_sizes_past_64_bits_are_refused():
+    """Widths and head counts whose products with the page or the rows would not fit 64 bits; the workspace has no size for them."""
+    for call in (_write, lambda d, **kw: _write(d, "rh3_kv_read", **kw), _attend):
+        for width in (1 << 58, 1 << 60, (1 << 62) + 8):
+            assert call(_desc(), width=width, stride=width) == 1 and "page table of" in nat.last_error()
+    for rows, hq in ((8, 1 << 62), (1 << 20, 1 << 46), (1 << 30, 8)):
+        assert _attend(_desc(), rows=rows, hq=hq, n=(1 << 63) - 1) == 1 and f"{rows} rows of {hq} heads" in nat.last_error()
+    size = nat.lib().rh3_kv_attention_workspace_bytes
+    good = dict(hq=8, heads=4, dim=128, rows=2, cap=512, batch=2, even=1, prefix=0, form=0)
+    assert size(*good.values()) > 0
+    for bad in (dict(hq=1 << 62), dict(dim=96), dict(rows=1 << 40), dict(cap=1 << 40), dict(batch=1 << 20), dict(prefix=-1), dict(prefix=1 << 40)):
+        assert size(*{**good, **bad}.values()) == 0, bad
