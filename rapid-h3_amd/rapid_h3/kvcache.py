@@ -28,6 +28,11 @@ _FORM = {None: nat.RH3_KV_BY_SIZE, "token": nat.RH3_KV_TOKEN, "chunk": nat.RH3_K
 _HERE = contextlib.nullcontext()
 
 
+def _st(t, axis):
+    """The stride of an axis; 0 for one of length 1, whose stride may be any number and is not used."""
+    return t.stride(axis) if t.shape[axis] > 1 else 0
+
+
 class KVCache:
     """The pages of one layer: k, v [P, heads, page, dim] int8 or float8_e4m3fn codes, k_scale, v_scale [P, heads, page]
     fp32 (page 16 to 256, a power of two; dim 64 or 128; views of larger buffers whose pages and heads lie apart are fine,
@@ -37,7 +42,7 @@ class KVCache:
     __slots__ = ("k", "v", "k_scale", "v_scale", "pages", "heads", "page", "dim", "device", "gpu", "_desc", "_ref")
 
     def __init__(self, k, v, k_scale, v_scale):
-        if k.ndim != 4 or v.shape != k.shape or v.stride() != k.stride():
+        if k.ndim != 4 or v.shape != k.shape or any(_st(v, i) != _st(k, i) for i in range(4)):
             raise RuntimeError(f"KVCache: k and v must be [pages, heads, page, dim] of one layout, got {tuple(k.shape)} and {tuple(v.shape)}")
         p, h, n, d = k.shape
         if k.dtype not in (torch.int8, FP8) or v.dtype != k.dtype:
@@ -49,15 +54,15 @@ class KVCache:
         for s in (k_scale, v_scale):
             if s.shape != (p, h, n) or s.dtype != torch.float32 or s.stride(2) != 1:
                 raise RuntimeError("KVCache: scales must be fp32 [pages, heads, page] with a contiguous last dim")
-        if v_scale.stride() != k_scale.stride():
+        if any(_st(v_scale, i) != _st(k_scale, i) for i in range(2)):
             raise RuntimeError("KVCache: k_scale and v_scale must have one layout")
         if not k.is_cuda or any(t.device != k.device for t in (v, k_scale, v_scale)):
             raise RuntimeError("KVCache: the four tensors must be on one GPU (no CPU path)")
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.pages, self.heads, self.page, self.dim, self.device = p, h, n, d, k.device
         self.gpu = k.get_device()
-        self._desc = nat.KvCacheDesc(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), k.stride(0), k.stride(1),
-                                     k_scale.stride(0), k_scale.stride(1), p, h, n, d,
+        self._desc = nat.KvCacheDesc(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), _st(k, 0), _st(k, 1),
+                                     _st(k_scale, 0), _st(k_scale, 1), p, h, n, d,
                                      nat.RH3_KV_INT8 if k.dtype == torch.int8 else nat.RH3_KV_E4M3)
         self._ref = ctypes.addressof(self._desc)
 
@@ -84,7 +89,7 @@ _stream = torch._C._cuda_getCurrentRawStream
 
 def _seqs(name, cache, table, lens, cu, gpu):
     """The sequences' arguments of a call after its rows: table, its stride and width, lens, cu, batch."""
-    if table.ndim != 2 or table.dtype != torch.int32 or table.stride(1) != 1:
+    if table.ndim != 2 or table.dtype != torch.int32 or (table.stride(1) != 1 and table.shape[1] > 1):
         raise RuntimeError(f"{name}: table must be int32 [batch, pages of a sequence] with a contiguous last dim")
     b, w = table.shape
     if lens.dtype != torch.int32 or lens.ndim != 1 or lens.numel() != b or not lens.is_contiguous():
@@ -106,7 +111,7 @@ def _rows(name, what, x, cache):
         if h == cache.heads and d == cache.dim and sd == 1:
             if not x.is_cuda:
                 raise RuntimeError(f"{name}: {what} must be on a GPU (no CPU path)")
-            return t, st, sh
+            return t, st if t > 1 else 0, sh if h > 1 else 0
     raise RuntimeError(f"{name}: {what} must be [rows, {cache.heads}, {cache.dim}] with a contiguous last dim, got {tuple(x.shape)}")
 
 
@@ -164,7 +169,7 @@ def _attention(name, q, cache, prefix, prefix_len, table, lens, cu, causal, scal
         raise RuntimeError(f"{name}: q must be on a GPU (no CPU path)")
     gpu, dev = q.get_device(), cache.device
     t, hq, d = q.shape
-    q_st, q_sh, _ = q.stride()
+    q_st, q_sh = _st(q, 0), _st(q, 1)
     seqs = _seqs(name, cache, table, lens, cu, gpu)
     alloc = torch.empty if cu is None else torch.zeros          # rows that no sequence has are not written
     if out is None:
@@ -173,7 +178,7 @@ def _attention(name, q, cache, prefix, prefix_len, table, lens, cu, causal, scal
     else:
         if out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1 or out.get_device() != gpu:
             raise RuntimeError(f"{name}: out must be like q, with a contiguous last dim")
-        o_st, o_sh, _ = out.stride()
+        o_st, o_sh = _st(out, 0), _st(out, 1)
     sums = alloc((t, hq), dtype=torch.float32, device=dev) if lse else None
     n = _workspace_bytes(hq, cache.heads, d, t, seqs[2] * cache.page, seqs[5], cu is None, prefix_len, f)
     ws = torch.empty(n, dtype=torch.uint8, device=dev)

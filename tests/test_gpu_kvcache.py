@@ -719,6 +719,28 @@ def test_rows_outside_the_call_or_the_table(dev, fmt, dim, form, lens, cu, rows)
         _check_lse(lse, rl, err)
 
 
+@pytest.mark.parametrize("form", FORMS)
+def test_axes_of_length_one(dev, form):
+    """One head, one row, one page and one table entry: the stride of such an axis is no one's, whatever number it is."""
+    def odd(t):   # the same tensor with other strides at its axes of length 1
+        return t.as_strided(t.shape, [s if n > 1 else 12345 + 7 * i for i, (n, s) in enumerate(zip(t.shape, t.stride()))])
+    c = _pool(dev, I8, 1, 1, 64, 128, 56)
+    d = kv.KVCache(odd(c.k), c.v, odd(c.k_scale), c.v_scale)
+    x, y = (torch.randn(1, 1, 128, generator=_gen(57 + i)).to(BF).to(dev) for i in range(2))
+    table, lens = _i32([[0]], dev), _i32([50], dev)
+    kv.kv_write(c, x, y, table, lens)
+    want = [t.clone() for t in (c.k, c.v, c.k_scale, c.v_scale)]
+    kv.kv_write(d, odd(x), y, odd(table), lens)
+    assert all(torch.equal(t, u) for t, u in zip(want, (d.k, d.v, d.k_scale, d.v_scale)))
+    got = (odd(torch.zeros_like(x)), odd(torch.zeros_like(y)))
+    kv.kv_read(d, odd(table), lens, out=got)
+    assert all(torch.equal(t, u) for t, u in zip(got, kv.kv_read(c, table, lens)))
+    q = torch.randn(1, 1, 128, generator=_gen(59)).to(BF).to(dev)
+    out = odd(torch.zeros_like(q))
+    kv.kv_attention(odd(q), d, odd(table), lens, out=out, form=form)
+    assert torch.equal(out, kv.kv_attention(q, c, table, lens, form=form))
+
+
 def test_layouts(dev):
     """A cache that is a view of a buffer of several layers, strided queries and output, a wider table, out over q."""
     pages, heads, page, dim, hq = 9, 2, 32, 128, 6
