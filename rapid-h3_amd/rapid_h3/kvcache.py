@@ -151,7 +151,8 @@ def kv_read(cache, table, lens, cu=None, rows=None, dtype=torch.bfloat16, out=No
 
 
 @functools.lru_cache(maxsize=1024)
-def _workspace_bytes(*sizes):
+def _workspace_bytes(gpu, *sizes):
+    """Of a call on this GPU, which is the current one: the number of its CUs counts."""
     return nat.lib().rh3_kv_attention_workspace_bytes(*sizes)
 
 
@@ -180,9 +181,9 @@ def _attention(name, q, cache, prefix, prefix_len, table, lens, cu, causal, scal
             raise RuntimeError(f"{name}: out must be like q, with a contiguous last dim")
         o_st, o_sh = _st(out, 0), _st(out, 1)
     sums = alloc((t, hq), dtype=torch.float32, device=dev) if lse else None
-    n = _workspace_bytes(hq, cache.heads, d, t, seqs[2] * cache.page, seqs[5], cu is None, prefix_len, f)
-    ws = torch.empty(n, dtype=torch.uint8, device=dev)
     with _on(gpu):
+        n = _workspace_bytes(gpu, hq, cache.heads, d, t, seqs[2] * cache.page, seqs[5], cu is None, prefix_len, f)
+        ws = torch.empty(n, dtype=torch.uint8, device=dev)
         nat.call("rh3_kv_attention", cache._ref, q.data_ptr(), q_st, q_sh, hq, dt, t, *seqs, causal, d ** -0.5 if scale is None else scale,
                  out.data_ptr(), o_st, o_sh, None if sums is None else sums.data_ptr(), None if prefix is None else prefix.data_ptr(),
                  prefix_len, f, ws.data_ptr(), n, _stream(gpu))

@@ -153,3 +153,52 @@ def test_sizes_past_64_bits_are_refused():
     assert size(*good.values()) > 0
     for bad in (dict(hq=1 << 62), dict(dim=96), dict(rows=1 << 40), dict(cap=1 << 40), dict(batch=1 << 20), dict(prefix=-1), dict(prefix=1 << 40)):
         assert size(*{**good, **bad}.values()) == 0, bad
+
+
+def test_workspace_size_is_of_the_calls_gpu(monkeypatch):
+    """The size depends on the GPU's number of CUs: kept per GPU, and asked for with the call's GPU as the current one."""
+    now = [0]
+
+    class On:
+        def __init__(self, gpu):
+            self.gpu = gpu
+
+        def __enter__(self):
+            self.before, now[0] = now[0], self.gpu
+
+        def __exit__(self, *_):
+            now[0] = self.before
+
+    class Lib:
+        @staticmethod
+        def rh3_kv_attention_workspace_bytes(*sizes):
+            return 1000 * (1 + now[0])
+
+    class Row:          # a tensor of a GPU, as far as the wrapper looks
+        ndim, shape, dtype, is_cuda = 3, (2, 4, 128), torch.bfloat16, True
+
+        def __init__(self, gpu):
+            self.gpu = gpu
+
+        def stride(self, i=None):
+            return (512, 128, 1) if i is None else (512, 128, 1)[i]
+
+        def get_device(self):
+            return self.gpu
+
+        def data_ptr(self):
+            return FAKE
+    sizes = []
+    monkeypatch.setattr(kv, "_on", On)
+    monkeypatch.setattr(kv, "_stream", lambda gpu: None)
+    monkeypatch.setattr(kv, "_seqs", lambda *a: (FAKE, 1, 1, FAKE, None, 2))
+    monkeypatch.setattr(nat, "lib", lambda: Lib)
+    monkeypatch.setattr(nat, "call", lambda name, *args: sizes.append(args[-2]))
+
+    class Cache:
+        heads, dim, page, device, _ref = 2, 128, 64, torch.device("cpu"), None
+    kv._workspace_bytes.cache_clear()
+    for gpu in (0, 1, 0):
+        kv.kv_attention(Row(gpu), Cache, None, None, out=Row(gpu))
+    kv._workspace_bytes.cache_clear()
+    assert sizes == [1000, 2000, 1000]
