@@ -37,7 +37,8 @@ class KVCache:
     """The pages of one layer: k, v [P, heads, page, dim] int8 or float8_e4m3fn codes, k_scale, v_scale [P, heads, page]
     fp32 (page 16 to 256, a power of two; dim 64 or 128; views of larger buffers whose pages and heads lie apart are fine,
     k like v and k_scale like v_scale). Where a position holds something, no code is NaN and a scale is finite and not
-    negative, or NaN for a row that is (as kv_write leaves them). The tensors are kept and used as they are."""
+    negative, or NaN for a row that is (as kv_write leaves them). The tensors are kept and used as they are; the attributes
+    cannot be changed."""
 
     __slots__ = ("k", "v", "k_scale", "v_scale", "pages", "heads", "page", "dim", "device", "gpu", "_desc", "_ref")
 
@@ -65,6 +66,11 @@ class KVCache:
                                      _st(k_scale, 0), _st(k_scale, 1), p, h, n, d,
                                      nat.RH3_KV_INT8 if k.dtype == torch.int8 else nat.RH3_KV_E4M3)
         self._ref = ctypes.addressof(self._desc)
+
+    def __setattr__(self, name, value):
+        if hasattr(self, "_ref"):   # the kernels would go on with the addresses taken at first
+            raise AttributeError(f"KVCache: {name} cannot be changed; make a new KVCache")
+        object.__setattr__(self, name, value)
 
 
 def kv_cache(pages, heads, page=64, dim=128, dtype=torch.int8, device="cuda"):

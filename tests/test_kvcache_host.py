@@ -202,3 +202,15 @@ def test_workspace_size_is_of_the_calls_gpu(monkeypatch):
         kv.kv_attention(Row(gpu), Cache, None, None, out=Row(gpu))
     kv._workspace_bytes.cache_clear()
     assert sizes == [1000, 2000, 1000]
+
+
+def test_cache_attributes_stay(monkeypatch):
+    """The kernels read the addresses that a KVCache was made with, so its tensors cannot be exchanged."""
+    k, s = torch.zeros((4, 2, 64, 128), dtype=torch.int8), torch.zeros((4, 2, 64))
+    monkeypatch.setattr(torch.Tensor, "is_cuda", True)
+    c = kv.KVCache(k, k.clone(), s, s.clone())
+    monkeypatch.undo()
+    for name in ("k", "v", "k_scale", "v_scale", "page", "heads"):
+        with pytest.raises(AttributeError, match="cannot be changed"):
+            setattr(c, name, getattr(c, name))
+    assert c.k is k and c.k_scale is s
