@@ -50,7 +50,7 @@ struct Sums {
   }
   __device__ __forceinline__ void store(const AttnArgs& a, int tok, int hd, float top) const {
     const int lane = threadIdx.x & 63;
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    const float inv = sum == 0.0f ? 0.0f : (1.0f / PART) / sum;
     uint16_t* dst = static_cast<uint16_t*>(a.out) + tok * a.o_st + hd * a.o_sh + EPL * lane;
     if constexpr (EPL == 2) *reinterpret_cast<uint32_t*>(dst) = pack_out(a, o[0] * inv, o[1] * inv);
     else *dst = static_cast<uint16_t>(pack_out(a, o[0] * inv, 0.0f));

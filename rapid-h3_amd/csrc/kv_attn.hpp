@@ -19,8 +19,10 @@
 namespace rh3 {
 namespace kv {
 
-// A part: the unnormalised sum of a query row over some of its keys, with the fp32 sum of its probabilities and their reference
-// (base 2). Slots of parts hold R rows each: part_o [slot][R][dim], part_ml [slot][R][2] (reference, sum).
+// A part: the unnormalised sum of a query row over some of its keys, times PART (probabilities of up to 2^15 of very many keys with
+// values near fp32's largest), with the fp32 sum of its probabilities and their reference (base 2). Slots of parts hold R rows each: part_o [slot][R][dim], part_ml [slot][R][2] (reference, sum).
+constexpr float PART = 0x1p-32f;
+
 struct AttnArgs {
   Cache c;
   Seqs s;

@@ -349,7 +349,10 @@ __global__ void __launch_bounds__(NT, 2) token_kernel(AttnArgs a) {
 #pragma unroll
         for (int i = 0; i < D / 16; i += 4) {
           float4 v = make_float4(st.o[m][i][r], st.o[m][i + 1][r], st.o[m][i + 2][r], st.o[m][i + 3][r]);
-          v.x *= st.vref[m]; v.y *= st.vref[m]; v.z *= st.vref[m]; v.w *= st.vref[m];
+          v.x = v.x * PART * st.vref[m];
+          v.y = v.y * PART * st.vref[m];
+          v.z = v.z * PART * st.vref[m];
+          v.w = v.w * PART * st.vref[m];
           *reinterpret_cast<float4*>(&so[wave][16 * m + l16][(D / 16) * (4 * g + r) + i]) = v;
         }
     }
@@ -377,7 +380,7 @@ __global__ void __launch_bounds__(NT, 2) token_kernel(AttnArgs a) {
       }
       if (whole && !a.keep) {
         const int tok = rw / a.group, hd = kvh * a.group + rw - tok * a.group;
-        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        const float inv = sum == 0.0f ? 0.0f : (1.0f / PART) / sum;
         uint32_t w[EPT / 2];
 #pragma unroll
         for (int e = 0; e < EPT; e += 2) w[e / 2] = pack_out(a, o[e] * inv, o[e + 1] * inv);

@@ -741,6 +741,25 @@ def test_axes_of_length_one(dev, form):
     assert torch.equal(out, kv.kv_attention(q, c, table, lens, form=form))
 
 
+@pytest.mark.parametrize("fmt", [I8, F8])
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("rows,n,prefix_len", [(1, 200, 0), (1, 20011, 0), (100, 3000, 0), (3, 100, 9000), (200, 90, 700)])
+def test_values_near_the_largest(dev, fmt, form, rows, n, prefix_len):
+    """Values of 2^126 at most, which many keys' weights times them, before the division by the weights' sum, are far past fp32."""
+    hq, hkv, dim, page = 4, 2, 128, 64
+    width, pre = -(-n // page), -(-prefix_len // page)
+    g = _gen(43)
+    k, ks = ok.quantise(0.2 * torch.randn(width + pre, hkv, page, dim, generator=g), fmt)
+    v, vs = ok.quantise((torch.rand(width + pre, hkv, page, dim, generator=g) - 0.3) * 2.0 ** 126, fmt)
+    c = kv.KVCache(*(t.to(dev) for t in (k, v, ks, vs)))
+    table, common = [list(range(pre, pre + width))], list(range(pre))
+    q = torch.randn(rows, hq, dim, generator=g).to(BF).to(dev)
+    out, lse = _call(q, c, table, [n], None, common, prefix_len, dev, lse=True, form=form)
+    ref, rl, mag, err = ok.attention(q, c, table, [n], prefix=common, prefix_len=prefix_len)
+    _check(out, ref, mag, err, 3.1)
+    _check_lse(lse, rl, err)
+
+
 def test_layouts(dev):
     """A cache that is a view of a buffer of several layers, strided queries and output, a wider table, out over q."""
     pages, heads, page, dim, hq = 9, 2, 32, 128, 6
