@@ -471,7 +471,8 @@ int rh3_attention_f8_forward(int64_t Sq, int64_t Sk, int64_t H, float scale, int
  * positions: row i of n = cu[b + 1] - cu[b] is position lens[b] - n + i, also where some of the n lie outside 0 .. rows, which the
  * call does not have. Rows in front of cu[0] and behind cu[batch] are neither read nor written. table, lens and cu are device
  * memory and may change between replays of a captured call; no content of theirs leads outside the buffers.
- * Rows [rows][heads][dim]: last dim contiguous, strides multiples of 8, 16-byte aligned.
+ * Rows [rows][heads][dim]: last dim contiguous, strides multiples of 8 (0 for rows or heads that are one, in what is read),
+ * 16-byte aligned.
  * ------------------------------------------------------------------------------------------- */
 typedef struct rh3_kv_cache {
   void* k;

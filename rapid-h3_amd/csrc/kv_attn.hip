@@ -275,6 +275,7 @@ extern "C" int rh3_kv_attention(const rh3_kv_cache* cache, const void* q, int64_
   RH3_REQUIRE(q && out, "kv_attention: null q or out");
   RH3_REQUIRE(aligned16(q) && aligned16(out) && q_st % 8 == 0 && q_sh % 8 == 0 && o_st % 8 == 0 && o_sh % 8 == 0,
               "kv_attention: q and out must be 16-byte aligned with strides that are multiples of 8");
+  RH3_REQUIRE((rows == 1 || o_st != 0) && (q_heads == 1 || o_sh != 0), "kv_attention: rows or heads of out share memory");
   RH3_REQUIRE(prefix_len >= 0 && prefix_len <= MAX_ROWS && (prefix_len == 0 || prefix), "kv_attention: prefix of %lld positions without pages",
               static_cast<long long>(prefix_len));
   RH3_REQUIRE(form >= RH3_KV_BY_SIZE && form <= RH3_KV_CHUNK, "kv_attention: form %d", form);
