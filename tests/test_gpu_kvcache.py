@@ -760,6 +760,25 @@ def test_values_near_the_largest(dev, fmt, form, rows, n, prefix_len):
     _check_lse(lse, rl, err)
 
 
+@pytest.mark.parametrize("fmt", [I8, F8])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("form,dtype,terms", [("token", BF, 1), ("chunk", BF, 3), ("token", HF, 2.0 ** -10), ("chunk", HF, 2.0 ** -10)])
+@pytest.mark.parametrize("rows,prefix_len", [(3, 0), (90, 0), (90, 300)])
+def test_roundings_of_each_kernel(dev, fmt, dim, form, dtype, terms, rows, prefix_len):
+    """No more than each kernel's own f16 roundings, 2^-11 of a product each, before that of the result: one of the weight in the
+    token kernel, three (weight, value scale, scaled value) in the chunk kernel, for fp16 results two terms of the weight (2^-22,
+    and 2^-22 for fp32 sums)."""
+    n, page = 777, 32
+    width, pre = -(-n // page), -(-prefix_len // page)
+    c = _pool(dev, fmt, 2 * width + pre, 2, page, dim, 62)
+    table, common = _tables(2 * width, width, 2, 63), list(range(2 * width, 2 * width + pre))
+    lens = [n, n - 300]
+    q = torch.randn(2 * rows, 4, dim, generator=_gen(64)).to(dtype).to(dev)
+    out = _call(q, c, table, lens, None, common, prefix_len, dev, form=form)
+    ref, _, mag, err = ok.attention(q, c, table, lens, prefix=common, prefix_len=prefix_len)
+    _check(out, ref, mag, err, terms)
+
+
 def test_layouts(dev):
     """A cache that is a view of a buffer of several layers, strided queries and output, a wider table, out over q."""
     pages, heads, page, dim, hq = 9, 2, 32, 128, 6
