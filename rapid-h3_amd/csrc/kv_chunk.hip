@@ -45,6 +45,7 @@ namespace {
 constexpr int KT = CHUNK_KEYS;
 constexpr float SUM_STALE = 0x1p15f;  // up to this sum of a half's probabilities none of them is over 2^REF_STALE
 constexpr float ROWS_APART = 0x1p-15f;  // query rows whose largest is this far below the tile's do not share its power of two
+constexpr float LEAST_SCALE = 1e-12f;   // the quantizers' least, that of a row of zeros
 constexpr float NO_REF = -0x1.fffffep127f;   // reference of a row that has seen no key: any score moves it
 
 // 16-byte pieces of the LDS rows. Each row has one piece more than it needs, so that 16 rows' pieces of one number lie in all 16
@@ -216,7 +217,7 @@ __global__ void __launch_bounds__(WAVES * 64, 2) chunk_kernel(AttnArgs a) {
       top = wave_max(mine);
       // the largest finite scale of the share's values, 4 keys (of one page) to a thread at a time
       float big = 0.0f, small = INFINITY;
-      bool gone = false;
+      bool gone = false, zeros = false;
 #pragma unroll 4
       for (int key = t0 * KT + 4 * static_cast<int>(threadIdx.x); key < min(t1 * KT, sq.len); key += 4 * WAVES * 64) {
         const int page = page_in(table[min(key >> a.c.log2page, width - 1)]);
@@ -227,9 +228,18 @@ __global__ void __launch_bounds__(WAVES * 64, 2) chunk_kernel(AttnArgs a) {
         for (int e = 0; e < 4; ++e) {
           const float y = page >= 0 && key + e < sq.len && x[e] < INFINITY ? x[e] : 0.0f;
           big = fmaxf(big, y);
-          // (a row of zeros has the quantizers' least scale and takes no part)
-          if (y > 0.0f && (y > 1e-12f || codes_in<FMT, D>(a.c.v + page * a.c.page_stride + kvh * a.c.head_stride + ((key + e) & mask) * D)))
-            small = fminf(small, y);
+          small = fminf(small, y > LEAST_SCALE ? y : INFINITY);
+          zeros |= y > 0.0f && y <= LEAST_SCALE;
+        }
+      }
+      if (__builtin_amdgcn_ballot_w64(zeros)) {   // rows of zeros take no part
+#pragma unroll 1
+        for (int key = t0 * KT + static_cast<int>(threadIdx.x); key < min(t1 * KT, sq.len); key += WAVES * 64) {
+          const int page = page_in(table[min(key >> a.c.log2page, width - 1)]);
+          if (page < 0) continue;
+          const float x = a.c.vs[page * a.c.spage_stride + kvh * a.c.shead_stride + (key & mask)];
+          if (x > 0.0f && x <= LEAST_SCALE && codes_in<FMT, D>(a.c.v + page * a.c.page_stride + kvh * a.c.head_stride + (key & mask) * D))
+            small = fminf(small, x);
         }
       }
       big = wave_max(big);
@@ -268,7 +278,7 @@ __global__ void __launch_bounds__(WAVES * 64, 2) chunk_kernel(AttnArgs a) {
     }
     // Stage x (loaded) to LDS in 2 NP parts of K and 2 NP of V; the loads of stage x + 1
     const float vinv = apart ? 1.0f : pow2_inverse(vref);
-    auto put_k = [&](int x, int part) __attribute__((always_inline)) {
+    auto put_k = [&](int x, int part, bool apart) __attribute__((always_inline)) {
       const int i = part / 2, c = part % 2, key = first + 8 * i + (lane >> 3), h = (2 * x + 1 + (key >> 5)) & 7;
       if (c == 0 && (FINE || apart)) svs[h][key & 31] = kvs[i] < INFINITY ? kvs[i] * vinv : 0.0f;
       // a NaN value would reach rows that do not see its key (0 x NaN): its key is made NaN
@@ -276,7 +286,7 @@ __global__ void __launch_bounds__(WAVES * 64, 2) chunk_kernel(AttnArgs a) {
       if (c < D / 64)
         sk[x & 1][key * K_ROW<D> + (lane & 7) * (D / 64) + c] = __builtin_bit_cast(uint4, f16x8<FMT>(kraw[i][2 * c], kraw[i][2 * c + 1]));
     };
-    auto put_v = [&](int x, int part) __attribute__((always_inline)) {
+    auto put_v = [&](int x, int part, bool apart) __attribute__((always_inline)) {
       const int i = part / 2, c = part % 2, key = first + 8 * i + (lane >> 3);
       // outside the share's keys and in an absent page there may be anything: 0 (and codes that can be NaN go)
       const int pos = x * KT - 32 + key;
@@ -302,12 +312,12 @@ __global__ void __launch_bounds__(WAVES * 64, 2) chunk_kernel(AttnArgs a) {
     };
     auto stage_v = [&](int x) __attribute__((always_inline)) {
 #pragma unroll
-      for (int i = 0; i < 2 * NP; ++i) put_v(x, i);
+      for (int i = 0; i < 2 * NP; ++i) put_v(x, i, apart);
       next_v(x);
     };
     auto stage_k = [&](int x) __attribute__((always_inline)) {
 #pragma unroll
-      for (int i = 0; i < 2 * NP; ++i) put_k(x, i);
+      for (int i = 0; i < 2 * NP; ++i) put_k(x, i, apart);
       next_k(x);
     };
 
@@ -485,7 +495,7 @@ __global__ void __launch_bounds__(WAVES * 64, 2) chunk_kernel(AttnArgs a) {
     if (t0 < t1) {
       // stage t0 - 1 is only K of window t0
 #pragma unroll
-      for (int i = 0; i < 2 * NP; ++i) put_k(t0 - 1, i);
+      for (int i = 0; i < 2 * NP; ++i) put_k(t0 - 1, i, apart);
       next_v(t0 - 1);
       next_k(t0 - 1);
       __syncthreads();
@@ -512,7 +522,7 @@ __global__ void __launch_bounds__(WAVES * 64, 2) chunk_kernel(AttnArgs a) {
         for (int i = 0; i < AHEAD; ++i) f[i] = k_at(b, 0, i);
         __builtin_amdgcn_sched_barrier(0);
         float more = fast(std::integral_constant<int, 0>(), b, s, sa, sb, f, k0, n, nr, [&](int i) __attribute__((always_inline)) {
-          if (i >= MM / 2 && i % EACH == 0) put_v(s + 1, (i - MM / 2) / EACH);
+          if (i >= MM / 2 && i % EACH == 0) put_v(s + 1, (i - MM / 2) / EACH, false);
           if (i == MM - 1) next_v(s + 1);
         });
         staged_v = made = true;
@@ -521,7 +531,7 @@ __global__ void __launch_bounds__(WAVES * 64, 2) chunk_kernel(AttnArgs a) {
         take(n, nr);
         odd = true;
         more = fast(std::integral_constant<int, 1>(), b, s, sb, sa, f, k0, n, nr, [&](int i) __attribute__((always_inline)) {
-          if (i >= MM / 2 && i % EACH == 0) put_k(s + 1, (i - MM / 2) / EACH);
+          if (i >= MM / 2 && i % EACH == 0) put_k(s + 1, (i - MM / 2) / EACH, false);
           if (i == MM - 1) next_k(s + 1);
         });
         staged_k = true;
