@@ -211,6 +211,7 @@ int check_cache(const char* name, const rh3_kv_cache* x, Cache& c) {
 int check_seqs(const char* name, const Cache& c, const int32_t* table, int64_t table_stride, int64_t width, const int32_t* lens,
                const int32_t* cu, int64_t batch, int64_t rows, Seqs& s) {
   RH3_REQUIRE(rows >= 0 && rows <= MAX_ROWS, "%s: %lld rows", name, static_cast<long long>(rows));
+  if (rows == 0 && batch == 0) return RH3_OK;   // the callers have nothing to do
   RH3_REQUIRE(batch >= 1 && batch <= 65536, "%s: %lld sequences (1 to 65536)", name, static_cast<long long>(batch));
   RH3_REQUIRE(table && lens, "%s: null page table or lengths", name);
   RH3_REQUIRE(width >= 1 && table_stride >= (batch > 1 ? width : 0) && width <= (MAX_ROWS >> c.log2page),

@@ -227,3 +227,11 @@ def test_results_do_not_share_memory():
 def _attend_out(o_st=1024, o_sh=128):
     return nat.lib().rh3_kv_attention(ctypes.addressof(_desc()), FAKE, 1024, 128, 8, 1, 2, FAKE, 8, 8, FAKE, None, 2, 1, 0.1, FAKE, o_st,
                                       o_sh, None, None, 0, 0, FAKE, 1 << 40, None)
+
+
+def test_no_sequences_is_no_call():
+    """An empty batch: no rows of no sequences."""
+    for name in ("rh3_kv_write", "rh3_kv_read"):
+        assert _write(_desc(), name, rows=0, batch=0, k=None, v=None, table=None, lens=None) == 0
+        assert _write(_desc(), name, rows=3, batch=0) == 1 and "0 sequences" in nat.last_error()
+    assert _attend(_desc(), rows=0, batch=0, q=None, out=None, ws=None, n=0, table=None, lens=None) == 0
