@@ -61,7 +61,7 @@ struct Sums {
 
 // Every query row of the call, WPR waves to one: where a row has many parts (few items on all workgroups), or a prefix's beside its
 // own (of the same launch, or of `prefix`). Bound by latency: a row's parts are a few KB to some hundred (4 rows x 56 heads in 16
-// parts 5.5 us; 64 x 32 with a prefix's 33 parts each, 38 MB, 13).
+// parts 5.7 us; 64 x 32 with a prefix's 33 parts each, 38 MB, 14.5).
 template <int D, int WPR>
 __global__ void __launch_bounds__(WPR > 4 ? WPR * 64 : 256) join_rows_kernel(Source own, Source prefix, int has_prefix) {
   constexpr int WAVES = WPR > 4 ? WPR : 4, EPL = D / 64;

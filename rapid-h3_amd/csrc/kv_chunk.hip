@@ -1,11 +1,13 @@
 // Attention of many query rows over the paged cache: a chunk of a prompt, the tokens of a frame, a whole batch against a prefix
 // that it shares.
 //
-// 4 dim flops per query row and key, while a key's 2 (dim + 4) bytes serve all rows of a tile: bound by the matrix units and the
-// vector instructions of the softmax together, which share the card's power. Measured: 2,048 rows x 32 / 8 heads at the end of
-// 16,384 keys, int8, 570 to 660 us (780 to 900 TFLOP/s by how long the card has been busy; matrix units 38 %, vector units 44 % at
-// 2.0 GHz, waves waiting 35 %); 1,560 rows x 56 heads on 22,332 keys, e4m3, 1,265 to 1,400 us (710 to 790; 39 % and 42 % at 1.73
-// GHz); 64 x 4 rows x 8 heads on 32,768 keys 70 us (490). A large f16 matrix product reaches 1,485.
+// 4 dim flops per query row and key, while a key's 2 (dim + 4) bytes serve all rows of a tile. Measured: 2,048 rows x 32 / 8 heads
+// at the end of 16,384 keys, int8, 590 to 660 us (780 to 870 TFLOP/s by how long the card has been busy); 1,560 rows x 56 heads on
+// 22,332 keys, e4m3, 1,280 to 1,400 us (710 to 780); 64 x 4 rows x 8 heads on 32,768 keys 71 us (480). A large f16 matrix product
+// reaches 1,485. Of the first's cycles, at 2.0 GHz, the matrix units are busy in 37 %, the vector units in 42 %, LDS in 34 %, and the
+// waves wait for 37 % of their time: no unit is full, but two waves to a SIMD do not cover each other's way from scores over
+// weights to values, and the clock falls as the units fill. The next limit is LDS: 64 keys at dim 128 are 288 KB of reads and
+// writes for 8 waves, 2,300 cycles, beside 2,048 of MFMA.
 //
 // A workgroup of 4 or 8 waves holds 32 query rows of one K/V head on each and walks its keys 64 at a time. The keys' codes come
 // to registers a step ahead, are converted to f16 once for all waves and written to LDS (two buffers, one barrier to a step), K
@@ -24,11 +26,12 @@
 // to a power of two over the largest of the share's keys (a scan of the scales before the first step), is multiplied into V as it
 // is converted, if those scales are within 2^18 of each other (rows of zeros aside). Else a large value would take bits from rows
 // that do not see it, or hardly: the plain path takes that item, too, and multiplies the scales into the probabilities, in a unit
-// of each row's own.
+// of each row's own (the first size with one query row of 10^12, or values of 10^9, in every tile: 1,290 us; a tile alone as much
+// longer). With rows of zeros on every page 617.
 // Roundings to f16: the probability, the value's scale, and the product of that with the code; 2^-11 relative at most each, with
 // fp32 sums, beside a bf16 result's own 2^-8. FINE, for fp16 results, whose own rounding is no coarser: the scale (within 2^14 of
 // the others) is multiplied into the probability, which is kept in two f16 terms (error of 300 rows on 3,000 keys 4.0e-4 ->
-// 2.1e-4, that of the result's rounding; the first size above 545 -> 730 us, the last 67 -> 79).
+// 2.1e-4, that of the result's rounding; the first size above 590 -> 810 us, the last 80 -> 97 with its join).
 //
 // Tried and slower, or no faster: exponentials only beside the values' MFMAs (703 against 688 us for the first size above), the
 // next step's page entries looked up one by one behind the barrier (688 against 670), a load two steps ahead of the next one that

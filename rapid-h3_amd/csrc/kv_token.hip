@@ -1,7 +1,7 @@
 // Attention of few query rows over the paged cache: single tokens of a batch, or a few tokens each.
 //
 // Bound by the cache's bytes: 2 (dim + 4) per K/V head and position. Measured: 64 sequences of up to 8,190 keys x 8 K/V heads of
-// 128 (0.37 GB) in 74 us, 5.0 TB/s; 4 of 131,071 keys (1.1 GB) in 188 us, 5.9 TB/s; a large copy moves 4.8, a fill 6.8.
+// 128 (0.37 GB) in 74 us, 5.0 TB/s; 4 of 131,071 keys (1.1 GB) in 190 us, 5.8 TB/s; a large copy moves 4.8, a fill 6.8.
 //
 // A wave takes 32 keys at a time, for 16 query rows of the K/V head (32 at dim 64: at 128 their accumulators leave no registers for
 // the loads, and 2 x 16 rows, the second time mostly from L2, took 164 us where 32 took 230: 8 sequences of 4 tokens x 56 / 8 heads

@@ -176,7 +176,7 @@ def _attention(name, q, cache, prefix, prefix_len, table, lens, cu, causal, scal
         raise RuntimeError(f"{name}: q must be on a GPU (no CPU path)")
     gpu, dev = q.get_device(), cache.device
     t, hq, d = q.shape
-    q_st, q_sh = _st(q, 0), _st(q, 1)
+    q_st, q_sh, _ = q.stride()
     seqs = _seqs(name, cache, table, lens, cu, gpu)
     alloc = torch.empty if cu is None else torch.zeros          # rows that no sequence has are not written
     if out is None:
@@ -185,7 +185,11 @@ def _attention(name, q, cache, prefix, prefix_len, table, lens, cu, causal, scal
     else:
         if out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1 or out.get_device() != gpu:
             raise RuntimeError(f"{name}: out must be like q, with a contiguous last dim")
-        o_st, o_sh = _st(out, 0), _st(out, 1)
+        o_st, o_sh, _ = out.stride()
+    if t == 1:
+        q_st = o_st = 0
+    if hq == 1:
+        q_sh = o_sh = 0
     sums = alloc((t, hq), dtype=torch.float32, device=dev) if lse else None
     with _on(gpu):
         n = _workspace_bytes(gpu, hq, cache.heads, d, t, seqs[2] * cache.page, seqs[5], cu is None, prefix_len, f)

@@ -221,11 +221,11 @@ def test_results_do_not_share_memory():
     for change in (dict(k_st=0), dict(k_sh=0)):
         assert _write(_desc(), "rh3_kv_read", **change) == 1 and "share memory" in nat.last_error()
     for change in (dict(o_st=0), dict(o_sh=0)):
-        assert _attend_out(**change) == 1 and "out share memory" in nat.last_error()
+        assert _attend_out(_desc(), **change) == 1 and "out share memory" in nat.last_error()
 
 
-def _attend_out(o_st=1024, o_sh=128):
-    return nat.lib().rh3_kv_attention(ctypes.addressof(_desc()), FAKE, 1024, 128, 8, 1, 2, FAKE, 8, 8, FAKE, None, 2, 1, 0.1, FAKE, o_st,
+def _attend_out(desc, o_st=1024, o_sh=128):
+    return nat.lib().rh3_kv_attention(ctypes.addressof(desc), FAKE, 1024, 128, 8, 1, 2, FAKE, 8, 8, FAKE, None, 2, 1, 0.1, FAKE, o_st,
                                       o_sh, None, None, 0, 0, FAKE, 1 << 40, None)
 
 
