@@ -500,7 +500,8 @@ int rh3_kv_read(const rh3_kv_cache* cache, void* k, int64_t k_st, int64_t k_sh, 
 /* out = softmax(scale q k^T) v over a sequence's cached positions (causal: row i of n sees positions up to
  * lens[b] - n + i), q and out [rows][q_heads][dim] bf16 or fp16, query head h reads K/V head h / (q_heads / heads); lse
  * [rows][q_heads] fp32 or NULL: the natural log of the sum of exp(scale q.k). A row that sees no key gives 0 and -inf; one
- * that sees a NaN key or value gives NaN. prefix_len > 0: every row also sees the first prefix_len positions of the pages
+ * that sees a NaN key or value gives NaN; what the other rows, positions that it does not see and memory that holds nothing contain
+ * is of no account for a row, but for its last bits. prefix_len > 0: every row also sees the first prefix_len positions of the pages
  * prefix[], which come before the sequences' own and are read once for the batch. out may lie exactly over q. form: the
  * kernel for few query rows to a K/V head (RH3_KV_TOKEN) or for many (RH3_KV_CHUNK), or by the sizes, where the table's width
  * stands for the lengths, which only the device knows.
