@@ -2,8 +2,9 @@
 // bytes), kv_chunk.hip many (bound by the matrix units), kv_attn.hip joins the parts that either leaves and holds the entry points.
 //
 // For a query row i of a sequence of n rows and `len` cached positions: o_i = sum_j p_ij v_j / sum_j p_ij with
-// p_ij = exp(scale q_i.k_j) over j < len, and j <= pos + i (pos = len - n) if causal. A K/V head's query rows are its group's heads of every
-// token of the sequence, numbered token * group + head in the group, so that the group shares each key and value that is read.
+// p_ij = exp(scale q_i.k_j) over j < len, and j <= pos + i (pos = len - n) if causal. A K/V head's query rows are its group's heads
+// of every token of the sequence, numbered token * group + head in the group, so that the group shares each key and value that is
+// read.
 //
 // Arithmetic. Codes are small integers (int8) or 4-bit significands (e4m3): exact in f16. A query row is scaled by the power of
 // two that brings its largest magnitude to [2^14, 2^15) (the chunk kernel: the largest of all rows of its tile, where none is far
@@ -20,7 +21,8 @@ namespace rh3 {
 namespace kv {
 
 // A part: the unnormalised sum of a query row over some of its keys, times PART (probabilities of up to 2^15 of very many keys with
-// values near fp32's largest), with the fp32 sum of its probabilities and their reference (base 2). Slots of parts hold R rows each: part_o [slot][R][dim], part_ml [slot][R][2] (reference, sum).
+// values near fp32's largest), with the fp32 sum of its probabilities and their reference (base 2). Slots of parts hold R rows
+// each: part_o [slot][R][dim], part_ml [slot][R][2] (reference, sum).
 constexpr float PART = 0x1p-32f;
 
 struct AttnArgs {

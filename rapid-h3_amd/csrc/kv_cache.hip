@@ -167,7 +167,8 @@ int rows_call(const char* name, const rh3_kv_cache* cache, void* k, int64_t k_st
   RH3_REQUIRE(aligned16(k) && aligned16(v) && k_st % 8 == 0 && k_sh % 8 == 0 && v_st % 8 == 0 && v_sh % 8 == 0,
               "%s: rows must be 16-byte aligned with strides that are multiples of 8", name);
   if constexpr (!WRITE)
-    RH3_REQUIRE((rows == 1 || (k_st != 0 && v_st != 0)) && (c.heads == 1 || (k_sh != 0 && v_sh != 0)), "%s: rows or heads of the result share memory", name);
+    RH3_REQUIRE((rows == 1 || (k_st != 0 && v_st != 0)) && (c.heads == 1 || (k_sh != 0 && v_sh != 0)),
+                "%s: rows or heads of the result share memory", name);
   const int dim = static_cast<int>(cache->dim), fmt = static_cast<int>(cache->format);
   const dim3 g = grid_of(rows, c.heads, dim);
   RH3_REQUIRE(g.x <= MAX_GRID_256, "%s: %lld rows in one call", name, static_cast<long long>(rows));

@@ -590,7 +590,8 @@ __global__ void __launch_bounds__(WAVES * 64, 2) chunk_kernel(AttnArgs a) {
 #pragma unroll
           for (int i = 0; i < 4; ++i)
             *reinterpret_cast<float4*>(po + 32 * d + 8 * i) =
-                make_float4(o[d][4 * i] * PART * unit, o[d][4 * i + 1] * PART * unit, o[d][4 * i + 2] * PART * unit, o[d][4 * i + 3] * PART * unit);
+                make_float4(o[d][4 * i] * PART * unit, o[d][4 * i + 1] * PART * unit, o[d][4 * i + 2] * PART * unit,
+                            o[d][4 * i + 3] * PART * unit);
         if (hi == 0) *reinterpret_cast<float2*>(a.part_ml + (slot * R + rl) * 2) = make_float2(total == 0.0f ? -INFINITY : ref, total);
       }
     }

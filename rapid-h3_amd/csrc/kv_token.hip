@@ -187,7 +187,8 @@ __device__ __forceinline__ void compute(const AttnArgs& a, Tile<D>& t, int kvh, 
       const float ibase = pow2_inverse(__float_as_int(base));
       float w = 0.0f;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) w = fmaxf(w, __builtin_amdgcn_exp2f(x[m][j] - (st.ref[m] == -INFINITY ? 0.0f : st.ref[m])) * (vs[j] * ibase));
+      for (int j = 0; j < 8; ++j)
+        w = fmaxf(w, __builtin_amdgcn_exp2f(x[m][j] - (st.ref[m] == -INFINITY ? 0.0f : st.ref[m])) * (vs[j] * ibase));
       const float unit = weight_unit(st.vref[m], f, across_max<true>(w), base);
       st.ivref[m] = pow2_inverse(__float_as_int(unit));
       f *= st.vref[m] * st.ivref[m];

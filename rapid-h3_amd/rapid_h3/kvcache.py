@@ -134,8 +134,9 @@ def _rows_call(name, entry, what, cache, k, v, table, lens, cu):
 
 def kv_write(cache, k, v, table, lens, cu=None):
     """Quantise rows k, v [rows, heads, dim] (bf16, fp16 or fp32, strided ok) into their positions. Rows at a negative
-    position, past the table or in an absent page are skipped; a row that holds an infinity or a NaN is kept as NaN (its scale). A position
-    that two rows of a call name (a page that sequences share, or that a table names twice) ends with a mixture of them."""
+    position, past the table or in an absent page are skipped; a row that holds an infinity or a NaN is kept as NaN (its scale).
+    A position that two rows of a call name (a page that sequences share, or that a table names twice) ends with a mixture of
+    them."""
     _rows_call("kv_write", "rh3_kv_write", ("k", "v"), cache, k, v, table, lens, cu)
 
 
