@@ -499,22 +499,27 @@ def _plain_attention(s):
 
 
 # ---------------------------------------------------------------- the result in 64 bits
+def _pow2_64(e):
+    """2^e in float64, by its bits."""
+    return ((e.long() + 1023) << 52).view(F64)
+
+
 def _decoded(codes, scale):
     """Float64 values of codes with their scales, without a table: sign, exponent and mantissa of each code."""
     if codes.dtype != torch.uint8:
         return codes.to(F64) * scale.to(F64)[..., None]
     c = torch.stack([codes.int() & 15, codes.int() >> 4], -1).flatten(-2)
     e, m = (c >> 1) & 3, (c & 1).to(F64)
-    mag = torch.where(e == 0, 0.5 * m, torch.ldexp(1.0 + 0.5 * m, e - 1))
+    mag = torch.where(e == 0, 0.5 * m, (1.0 + 0.5 * m) * _pow2_64(e - 1))
     x = torch.where(c >= 8, -mag, mag).unflatten(-1, (-1, GROUP))
-    return torch.ldexp(x, scale.to(F64)[..., None] - 127).flatten(-2)
+    return (x * _pow2_64(scale.int() - 127)[..., None]).flatten(-2)
 
 
 def _nearest(y, bits, least, most):
     """Float64 values to the nearest with `bits` bits behind the leading one, from the exponent `least` on, halves to even."""
     y = y.clamp(-most, most)
     _, e = torch.frexp(y)
-    grid = torch.ldexp(torch.ones_like(y), (e - 1).clamp_min(least) - bits)
+    grid = _pow2_64((e - 1).clamp_min(least) - bits)
     return torch.round(y / grid) * grid
 
 
@@ -524,7 +529,7 @@ def _stored(x, fmt):
     if fmt == "fp4":
         y = x.unflatten(-1, (-1, GROUP))
         e = torch.ceil(torch.log2(y.abs().amax(-1, keepdim=True) / 7.0)).clamp(-125, 125)
-        f = torch.ldexp(torch.ones_like(e), e)
+        f = _pow2_64(e)
         return (_nearest(y / f, 1, 0, 6.0) * f).flatten(-2)
     f = (x.abs().amax(-1, keepdim=True) / (127 if fmt == "int8" else 448)).clamp_min(1e-12).to(F32).to(F64)
     y = (x / f).to(F32).to(F64)   # the quotient that is rounded to a code is the fp32 one, by definition
