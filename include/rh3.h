@@ -31,6 +31,7 @@ extern "C" {
 
 #define RH3_KV_INT8 0
 #define RH3_KV_E4M3 1
+#define RH3_KV_FP4 4
 #define RH3_KV_BY_SIZE 0
 #define RH3_KV_TOKEN 1
 #define RH3_KV_CHUNK 2
@@ -463,7 +464,11 @@ int rh3_attention_f8_forward(int64_t Sq, int64_t Sk, int64_t H, float scale, int
  *
  * A cache is `pages` pages of `page` positions (16, 32, 64, 128 or 256): codes k, v [pages][heads][page][dim] (dim 64 or
  * 128; positions contiguous, page and head strides in elements, multiples of 16) and scales k_scale, v_scale
- * [pages][heads][page] (strides multiples of 4), all 16-byte aligned. The value of a code is code * scale.
+ * [pages][heads][page] (strides multiples of 4), all 16-byte aligned. The value of a code is code * scale. Format RH3_KV_FP4: codes
+ * are e2m1, two to a byte (the lower channel in the low half), [pages][heads][page][dim / 2], and a scale is the byte e + 127 of a
+ * power of two 2^e that 32 channels share, [pages][heads][page][dim / 32] (positions contiguous); strides of both in bytes,
+ * multiples of 16. Bytes of positions that hold something are at most 252, or 255 in all of a position's key scales where its key
+ * or value is not finite (NaN in both then).
  *
  * A call names `batch` sequences: position p of sequence b lies in page table[b * table_stride + p / page] (width entries; an
  * entry outside [0, pages) is an absent page, whose positions hold nothing, and neither do those past the table); lens[b]
@@ -485,7 +490,9 @@ typedef struct rh3_kv_cache {
 } rh3_kv_cache;
 
 /* Quantizes rows of k and v (bf16, fp16 or fp32) into their positions: s = max(amax / QMAX, 1e-12) (127 or 448), code =
- * round_half_even(x / s); a row with an infinity or a NaN gets s = NaN and codes 0. Rows whose position is negative, past the
+ * round_half_even(x / s); a row with an infinity or a NaN gets s = NaN and codes 0. RH3_KV_FP4: e the least with amax <= 7 * 2^e of
+ * the 32 channels, within +-125, code the nearest to x / 2^e, ties to the even one, past 6 to 6; a position whose key or value has
+ * an infinity or a NaN gets key scales 255, all else 0. Rows whose position is negative, past the
  * table or in an absent page are skipped. A position that several rows of one call name (a page that two sequences share, or that a table
  * names twice) ends with a mixture of them: name each position written once. */
 int rh3_kv_write(const rh3_kv_cache* cache, const void* k, int64_t k_st, int64_t k_sh, const void* v, int64_t v_st,

@@ -22,6 +22,43 @@ def quantise(x, code):
     return q, s
 
 
+E2M1 = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
+
+
+def _pow2(e):
+    """2^e in float64 by its bits (torch's ldexp goes through a power that need not be exact)."""
+    return ((e.long() + 1023) << 52).view(torch.float64)
+
+
+def quantise4(x):
+    """[..., D] finite values -> the bytes of two e2m1 codes [..., D / 2] (the lower channel in the low half) and the scale bytes
+    [..., D / 32]: e the least with amax <= 7 * 2^e of a group of 32, within +-125, kept as e + 127; the nearest code to x / 2^e, ties
+    to the even one, past 6 to 6."""
+    y = x.double().unflatten(-1, (-1, 32))
+    amax = y.abs().amax(-1)
+    m, e = torch.frexp(amax)                     # amax = m * 2^e, m in [0.5, 1): 7 = 0.875 * 2^3
+    e = torch.where(m > 0.875, e - 2, e - 3).clamp(-125, 125)
+    e = torch.where(amax == 0, -125, e)
+    a = (y * _pow2(-e)[..., None]).flatten(-2)
+    grid = torch.tensor(E2M1, dtype=torch.float64, device=x.device)
+    mid = (grid[1:] + grid[:-1]) / 2
+    code = torch.zeros(a.shape, dtype=torch.int32, device=x.device)
+    for i, t in enumerate(mid.tolist()):         # between codes i and i + 1: the middle goes to the even one
+        code += (a.abs() > t) if i % 2 == 0 else (a.abs() >= t)
+    code += 8 * torch.signbit(a)
+    c = code.unflatten(-1, (-1, 2))
+    return (c[..., 0] + 16 * c[..., 1]).to(torch.uint8), (e + 127).to(torch.uint8)
+
+
+def values4(codes, scale):
+    """Float64 values of 4-bit codes [..., D / 2] and their scale bytes [..., D / 32]; a byte of 255 is NaN."""
+    c, s = codes.view(torch.uint8).int(), scale.view(torch.uint8).int()
+    c = torch.stack([c & 15, c >> 4], -1).flatten(-2)
+    grid = torch.tensor(E2M1 + tuple(-v for v in E2M1), dtype=torch.float64, device=codes.device)
+    f = torch.where(s == 255, math.nan, _pow2(s - 127))
+    return (grid[c.long()].unflatten(-1, (-1, 32)) * f[..., None]).flatten(-2)
+
+
 def rows_of(lens, cu, rows, batch):
     """(sequence, position) of each row, None where no sequence has it; position may be negative."""
     if cu is None:
@@ -51,7 +88,10 @@ def gather(cache, table, n):
     at = torch.where(here, at, 0)
     out = []
     for codes, scale in ((cache.k, cache.k_scale), (cache.v, cache.v_scale)):
-        x = codes.view(torch.uint8)[at, :, off].view(codes.dtype).double() * scale[at, :, off].double()[..., None]
+        if scale.dim() == 4:      # 4-bit codes
+            x = values4(codes.view(torch.uint8)[at, :, off], scale.view(torch.uint8)[at, :, off])
+        else:
+            x = codes.view(torch.uint8)[at, :, off].view(codes.dtype).double() * scale[at, :, off].double()[..., None]
         out.append(x.transpose(0, 1))
     return out[0], out[1], here
 

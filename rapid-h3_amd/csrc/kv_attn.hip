@@ -1,5 +1,5 @@
 // Attention over the paged cache: joining the parts that the token and chunk kernels leave, and the entry points.
-#include "kv_attn.hpp"
+#include "kv_four.hpp"
 
 namespace rh3 {
 namespace kv {
@@ -198,10 +198,10 @@ struct Plan {
 // call, token / chunk, 8 K/V heads of 128, rows of a K/V head): 1 sequence of 16,384 keys: 32 rows 24 / 39, 96 41 / 49, 128 45 / 53,
 // 192 58 / 47, 256 67 / 53; 16 of 4,096: 32 50 / 66, 48 68 / 71, 64 82 / 73, 96 121 / 80; 4 of 65,536: 32 140 / 188, 48 285 / 197;
 // 4 of 1,024: 16 16 / 37, 256 24 / 49. Heads of 64: 1 of 65,536: 128 60 / 70, 192 81 / 80, 256 103 / 87; 4: 96 150 / 158, 128 186 / 169.
-Plan plan_of(int64_t rows, int64_t batch, bool even, int64_t group, int64_t heads, int64_t dim, int64_t cap, bool keep, int form) {
+Plan plan_of(int fmt, int64_t rows, int64_t batch, bool even, int64_t group, int64_t heads, int64_t dim, int64_t cap, bool keep, int form) {
   const int64_t cus = device_cus() > 0 ? device_cus() : 256;
   const int64_t mean = (rows * group + batch - 1) / batch;    // query rows of a sequence's K/V head
-  const int small = dim == 64 && mean > 16 ? 32 : 16;
+  const int small = fmt != FP4 && dim == 64 && mean > 16 ? 32 : 16;
   const double mb = 2e-6 * static_cast<double>(dim + 4) * static_cast<double>(batch * heads) * static_cast<double>(cap);
   Plan p{};
   p.chunk = form != RH3_KV_BY_SIZE ? form == RH3_KV_CHUNK : static_cast<double>((mean + small - 1) / small) * mb / 6.8 > 34.0 + static_cast<double>((mean + 127) / 128) * mb / 3.0;
@@ -218,12 +218,12 @@ struct Call {
   bool joined;            // the prefix is a sequence of the one launch
   int64_t bytes;
 };
-Call call_of(int64_t rows, int64_t q_heads, int64_t heads, int64_t dim, int64_t cap, int64_t batch, bool even, int64_t prefix_len, int form) {
+Call call_of(int fmt, int64_t rows, int64_t q_heads, int64_t heads, int64_t dim, int64_t cap, int64_t batch, bool even, int64_t prefix_len, int form) {
   Call c{};
   const int64_t group = q_heads / heads;
-  c.own = plan_of(rows, batch, even, group, heads, dim, cap, prefix_len > 0, form);
+  c.own = plan_of(fmt, rows, batch, even, group, heads, dim, cap, prefix_len > 0, form);
   if (prefix_len > 0) {
-    c.prefix = plan_of(rows, 1, true, group, heads, dim, prefix_len, true, form);
+    c.prefix = plan_of(fmt, rows, 1, true, group, heads, dim, prefix_len, true, form);
     c.joined = c.own.chunk == c.prefix.chunk;   // the prefix's rows then go by the sequences' tiles
     if (c.joined) {
       const int64_t items = heads * ((rows * group + c.own.rows - 1) / c.own.rows);
@@ -238,7 +238,8 @@ Call call_of(int64_t rows, int64_t q_heads, int64_t heads, int64_t dim, int64_t 
 }
 
 void launch(const AttnArgs& a, const Plan& p, int fmt, int dim, hipStream_t st) {
-  if (p.chunk) launch_chunk(a, fmt, dim, p.rows, st);
+  if (fmt == FP4) p.chunk ? launch_chunk4(a, dim, p.rows, st) : launch_token4(a, dim, st);
+  else if (p.chunk) launch_chunk(a, fmt, dim, p.rows, st);
   else launch_token(a, fmt, dim, p.rows, st);
 }
 
@@ -254,7 +255,10 @@ extern "C" int64_t rh3_kv_attention_workspace_bytes(int64_t q_heads, int64_t hea
   if (heads < 1 || heads > 65535 || q_heads < heads || q_heads % heads || rows < 1 || rows > MAX_ROWS || q_heads / heads > MAX_ROWS / rows ||
       batch < 1 || batch > 65536 || capacity < 1 || capacity > MAX_ROWS || prefix_len < 0 || prefix_len > MAX_ROWS || (dim != 64 && dim != 128))
     return 0;
-  return call_of(rows, q_heads, heads, dim, capacity, batch, even != 0, prefix_len, form).bytes;
+  // enough for a cache of either width of codes
+  const int64_t eight = call_of(INT8, rows, q_heads, heads, dim, capacity, batch, even != 0, prefix_len, form).bytes;
+  const int64_t four = call_of(FP4, rows, q_heads, heads, dim, capacity, batch, even != 0, prefix_len, form).bytes;
+  return eight > four ? eight : four;
 }
 
 extern "C" int rh3_kv_attention(const rh3_kv_cache* cache, const void* q, int64_t q_st, int64_t q_sh, int64_t q_heads, int dtype,
@@ -280,7 +284,7 @@ extern "C" int rh3_kv_attention(const rh3_kv_cache* cache, const void* q, int64_
               static_cast<long long>(prefix_len));
   RH3_REQUIRE(form >= RH3_KV_BY_SIZE && form <= RH3_KV_CHUNK, "kv_attention: form %d", form);
   const int dim = static_cast<int>(cache->dim), fmt = static_cast<int>(cache->format);
-  const Call call = call_of(rows, q_heads, a.c.heads, dim, width * cache->page, batch, cu == nullptr, prefix_len, form);
+  const Call call = call_of(fmt, rows, q_heads, a.c.heads, dim, width * cache->page, batch, cu == nullptr, prefix_len, form);
   RH3_REQUIRE(workspace && aligned16(workspace) && workspace_bytes >= call.bytes,
               "kv_attention: workspace of %lld bytes needed, %lld given", static_cast<long long>(call.bytes), static_cast<long long>(workspace_bytes));
   // Parts that a row may have: the workgroups over the least count of items, no more than the keys make. Measured (kernel us, by

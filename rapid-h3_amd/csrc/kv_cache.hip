@@ -11,67 +11,11 @@
 // Measured, K and V of 22,332 rows x 56 heads of 128, bf16 and e4m3 (0.97 GB each way; a large copy moves 4.8 TB/s): written in
 // 237 us (4.1 TB/s, the vector units 55 % busy), read back in 184 us (5.3 TB/s); 8 x 7,919 rows x 16 heads int8 (0.79 GB)
 // read back in 160 to 187 us. 16 rows of 8 heads: 3.9 and 2.8 us, the length of a few dependent loads.
-#include "kv_common.hpp"
+#include "kv_rows.hpp"
 
 namespace rh3 {
 namespace kv {
 namespace {
-
-constexpr int NT = 256;
-
-// where a row of the call lies in the cache: offsets of its codes and scale without the head's part; false if it lies nowhere
-// (no sequence has the row, its position is before the first or past the table, its page is absent). `mine`: a sequence has the row.
-struct Place {
-  int64_t code, scale;
-  bool mine, there;
-};
-template <int D>
-__device__ __forceinline__ Place place_of(const Seqs& s, const Cache& c, int row) {
-  Place p{0, 0, false, false};
-  Seq q;
-  const int b = seq_of_row<D / 8 == 16 ? 16 : 8>(s, min(row, s.rows - 1), q);
-  if (b < 0 || row >= s.rows) return p;
-  p.mine = true;
-  const int pos = q.pos + (row - q.first);
-  if (pos < 0 || pos >= s.cap) return p;
-  const int pg = page_of(s, c, b, pos);
-  if (pg < 0) return p;
-  const int off = pos & ((1 << c.log2page) - 1);
-  p.code = pg * c.page_stride + off * D;
-  p.scale = pg * c.spage_stride + off;
-  p.there = true;
-  return p;
-}
-
-// max over the D / 8 lanes of a row
-template <int D>
-__device__ __forceinline__ uint32_t row_max(uint32_t v) {
-  v = max(v, static_cast<uint32_t>(__shfl_xor(static_cast<int>(v), 1)));
-  v = max(v, static_cast<uint32_t>(__shfl_xor(static_cast<int>(v), 2)));
-  v = max(v, static_cast<uint32_t>(__shfl_xor(static_cast<int>(v), 4)));
-  if constexpr (D == 128) v = max(v, static_cast<uint32_t>(__shfl_xor(static_cast<int>(v), 8)));
-  return v;
-}
-
-template <int FMT, int D>
-__device__ __forceinline__ void put(const float* x, uint8_t* codes, float* scale, bool first) {
-  uint32_t m = 0;   // magnitudes order like their bits, infinities and NaN last
-#pragma unroll
-  for (int e = 0; e < 8; ++e) m = max(m, __float_as_uint(x[e]) & 0x7fffffffu);
-  m = row_max<D>(m);
-  uint2 q = make_uint2(0u, 0u);
-  float s = __uint_as_float(0x7fc00000u);
-  if (m < 0x7f800000u) {
-    s = fmaxf(__uint_as_float(m) / (FMT == INT8 ? 127.0f : 448.0f), 1e-12f);
-    const float inv = 1.0f / s;
-    if constexpr (FMT == INT8)
-      q = quant8_i8(x, s, inv);
-    else
-      q = quant8_fp8(x, s, inv, fp8_odd(__uint_as_float(m), 0.0f, s));
-  }
-  *reinterpret_cast<uint2*>(codes) = q;
-  if (first) *scale = s;
-}
 
 template <int FMT, int D, int DT>
 __global__ void __launch_bounds__(NT) write_kernel(Cache c, Seqs s, const void* __restrict__ k, int64_t k_st, int64_t k_sh,
@@ -79,15 +23,13 @@ __global__ void __launch_bounds__(NT) write_kernel(Cache c, Seqs s, const void* 
   constexpr int LPR = D / 8;
   const int l = threadIdx.x % LPR;
   const int row = blockIdx.x * (NT / LPR) + threadIdx.x / LPR;
-  const Place p = place_of<D>(s, c, row);
+  const Place p = place_of<FMT, D>(s, c, row);
   if (!p.there) return;   // whole rows of lanes leave together
   for (int h = blockIdx.y; h < c.heads; h += gridDim.y) {
     float x[8], y[8];
     load_row8<DT>(k, row * k_st + h * k_sh + 8 * l, x);
     load_row8<DT>(v, row * v_st + h * v_sh + 8 * l, y);
-    const int64_t code = p.code + h * c.head_stride + 8 * l, scale = p.scale + h * c.shead_stride;
-    put<FMT, D>(x, c.k + code, c.ks + scale, l == 0);
-    put<FMT, D>(y, c.v + code, c.vs + scale, l == 0);
+    put<FMT, D>(c, p, h, l, x, y);
   }
 }
 
@@ -107,34 +49,39 @@ __device__ __forceinline__ void values(uint2 w, float s, float* x) {
   }
 }
 
+__device__ __forceinline__ void values4(uint32_t w, uint32_t byte, float* x) {   // 255: NaN
+  const float s = __uint_as_float(byte << 23);
+  const f2_t a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 1);
+  const f2_t d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 2), e = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 3);
+  x[0] = a[0]; x[1] = a[1]; x[2] = b[0]; x[3] = b[1];
+  x[4] = d[0]; x[5] = d[1]; x[6] = e[0]; x[7] = e[1];
+}
+
 template <int FMT, int D, int DT>
 __global__ void __launch_bounds__(NT) read_kernel(Cache c, Seqs s, void* __restrict__ k, int64_t k_st, int64_t k_sh,
                                                   void* __restrict__ v, int64_t v_st, int64_t v_sh) {
   constexpr int LPR = D / 8;
   const int l = threadIdx.x % LPR;
   const int row = blockIdx.x * (NT / LPR) + threadIdx.x / LPR;
-  const Place p = place_of<D>(s, c, row);
+  const Place p = place_of<FMT, D>(s, c, row);
   if (!p.mine) return;
   for (int h = blockIdx.y; h < c.heads; h += gridDim.y) {
     float x[8] = {}, y[8] = {};
     if (p.there) {
-      const int64_t code = p.code + h * c.head_stride + 8 * l, scale = p.scale + h * c.shead_stride;
-      values<FMT>(*reinterpret_cast<const uint2*>(c.k + code), c.ks[scale], x);
-      values<FMT>(*reinterpret_cast<const uint2*>(c.v + code), c.vs[scale], y);
+      if constexpr (FMT == FP4) {
+        const int64_t code = p.code + h * c.head_stride + 4 * l, scale = p.scale + h * c.shead_stride + l / 4;
+        const uint32_t sk = reinterpret_cast<const uint8_t*>(c.ks)[scale], sv = reinterpret_cast<const uint8_t*>(c.vs)[scale];
+        values4(*reinterpret_cast<const uint32_t*>(c.k + code), sk, x);
+        values4(*reinterpret_cast<const uint32_t*>(c.v + code), sk == 255 ? sk : sv, y);   // (a marked position is NaN in both)
+      } else {
+        const int64_t code = p.code + h * c.head_stride + 8 * l, scale = p.scale + h * c.shead_stride;
+        values<FMT>(*reinterpret_cast<const uint2*>(c.k + code), c.ks[scale], x);
+        values<FMT>(*reinterpret_cast<const uint2*>(c.v + code), c.vs[scale], y);
+      }
     }
     store_row8<DT>(k, row * k_st + h * k_sh + 8 * l, x);
     store_row8<DT>(v, row * v_st + h * v_sh + 8 * l, y);
   }
-}
-
-// Workgroups for `rows` rows: along x the rows, along y as many heads side by side as it takes for 8 workgroups to a CU; the
-// other heads are the workgroup's loop, which resolves a row's page once for all of them.
-dim3 grid_of(int64_t rows, int heads, int dim) {
-  const int64_t gx = (rows + NT / (dim / 8) - 1) / (NT / (dim / 8));
-  const int64_t want = 8 * static_cast<int64_t>(device_cus() > 0 ? device_cus() : 256);
-  int64_t gy = (want + gx - 1) / gx;
-  gy = gy < 1 ? 1 : gy > heads ? heads : gy;
-  return dim3(static_cast<uint32_t>(gx), static_cast<uint32_t>(gy));
 }
 
 template <bool WRITE, int FMT, int D>
@@ -174,6 +121,8 @@ int rows_call(const char* name, const rh3_kv_cache* cache, void* k, int64_t k_st
   RH3_REQUIRE(g.x <= MAX_GRID_256, "%s: %lld rows in one call", name, static_cast<long long>(rows));
   if (fmt == INT8 && dim == 128) launch_rows<WRITE, INT8, 128>(dtype, g, st, c, s, k, k_st, k_sh, v, v_st, v_sh);
   else if (fmt == INT8) launch_rows<WRITE, INT8, 64>(dtype, g, st, c, s, k, k_st, k_sh, v, v_st, v_sh);
+  else if (fmt == FP4 && dim == 128) launch_rows<WRITE, FP4, 128>(dtype, g, st, c, s, k, k_st, k_sh, v, v_st, v_sh);
+  else if (fmt == FP4) launch_rows<WRITE, FP4, 64>(dtype, g, st, c, s, k, k_st, k_sh, v, v_st, v_sh);
   else if (dim == 128) launch_rows<WRITE, E4M3, 128>(dtype, g, st, c, s, k, k_st, k_sh, v, v_st, v_sh);
   else launch_rows<WRITE, E4M3, 64>(dtype, g, st, c, s, k, k_st, k_sh, v, v_st, v_sh);
   return launch_status(name);
@@ -184,14 +133,15 @@ int rows_call(const char* name, const rh3_kv_cache* cache, void* k, int64_t k_st
 int check_cache(const char* name, const rh3_kv_cache* x, Cache& c) {
   RH3_REQUIRE(x, "%s: null cache", name);
   RH3_REQUIRE(x->k && x->v && x->k_scale && x->v_scale, "%s: null cache array", name);
-  RH3_REQUIRE(x->format == RH3_KV_INT8 || x->format == RH3_KV_E4M3, "%s: cache format %lld", name, static_cast<long long>(x->format));
+  RH3_REQUIRE(x->format == RH3_KV_INT8 || x->format == RH3_KV_E4M3 || x->format == RH3_KV_FP4, "%s: cache format %lld", name, static_cast<long long>(x->format));
   RH3_REQUIRE(x->dim == 64 || x->dim == 128, "%s: head dim %lld (64 or 128)", name, static_cast<long long>(x->dim));
   RH3_REQUIRE(x->page >= 16 && x->page <= 256 && (x->page & (x->page - 1)) == 0, "%s: page of %lld positions (16, 32, 64, 128 or 256)",
               name, static_cast<long long>(x->page));
   RH3_REQUIRE(x->pages >= 1 && x->pages <= INT32_MAX, "%s: %lld pages", name, static_cast<long long>(x->pages));
   RH3_REQUIRE(x->heads >= 1 && x->heads <= 65535, "%s: %lld heads", name, static_cast<long long>(x->heads));
+  const int64_t scales = x->format == RH3_KV_FP4 ? 16 : 4;   // in 16 bytes
   RH3_REQUIRE(aligned16(x->k) && aligned16(x->v) && aligned16(x->k_scale) && aligned16(x->v_scale) && x->page_stride % 16 == 0 &&
-                  x->head_stride % 16 == 0 && x->scale_page_stride % 4 == 0 && x->scale_head_stride % 4 == 0,
+                  x->head_stride % 16 == 0 && x->scale_page_stride % scales == 0 && x->scale_head_stride % scales == 0,
               "%s: pages and heads of the cache must be 16-byte aligned", name);
   RH3_REQUIRE(x->page_stride >= 0 && x->head_stride >= 0 && x->scale_page_stride >= 0 && x->scale_head_stride >= 0,
               "%s: negative stride in the cache", name);

@@ -1,8 +1,9 @@
-// Shared by the kernels of the paged key / value cache (kv_cache.hip, kv_token.hip, kv_chunk.hip, kv_attn.hip): where a
-// sequence's rows and positions lie, page lookups, and the conversion of 8-bit codes to f16.
+// Shared by the kernels of the paged key / value cache (kv_cache.hip, kv_token.hip, kv_chunk.hip, their 4-bit forms,
+// kv_attn.hip): where a sequence's rows and positions lie, page lookups, and the conversion of 8-bit codes to f16.
 //
-// A cache is pages of `page` positions: codes [P][heads][page][dim], one fp32 scale per code row [P][heads][page]. Position p
-// of sequence b lies in page table[b][p / page]; an entry outside [0, P) is an absent page, whose positions hold nothing.
+// A cache is pages of `page` positions: codes [P][heads][page][dim], one fp32 scale per code row [P][heads][page] (4-bit format:
+// bytes of two codes [..][dim / 2], scale bytes [..][dim / 32], kv_four.hpp). Position p of sequence b lies in page
+// table[b][p / page]; an entry outside [0, P) is an absent page, whose positions hold nothing.
 // Everything that comes from device memory (lengths, row offsets, page numbers) is clamped before it addresses anything, so no
 // content of these arrays can make an access leave the caller's buffers.
 #pragma once
@@ -16,6 +17,7 @@ namespace kv {
 
 constexpr int INT8 = RH3_KV_INT8;
 constexpr int E4M3 = RH3_KV_E4M3;
+constexpr int FP4 = RH3_KV_FP4;
 
 typedef _Float16 h2_t __attribute__((ext_vector_type(2)));
 typedef _Float16 h8_t __attribute__((ext_vector_type(8)));
@@ -27,7 +29,7 @@ struct Cache {
   uint8_t *k, *v;
   float *ks, *vs;
   int64_t page_stride, head_stride;     // of codes, in bytes
-  int64_t spage_stride, shead_stride;   // of scales, in floats
+  int64_t spage_stride, shead_stride;   // of scales, in floats (4-bit format: in bytes)
   int pages, heads, log2page;
 };
 

@@ -1,0 +1,110 @@
+// Rows of keys and values on their way into the paged cache: where a row of a call lies, and its codes and scales (kv_cache.hip,
+// kv_rope.hip).
+#pragma once
+
+#include "kv_four.hpp"
+
+namespace rh3 {
+namespace kv {
+
+constexpr int NT = 256;
+
+// where a row of the call lies in the cache: offsets of its codes and scale without the head's part; false if it lies nowhere
+// (no sequence has the row, its position is before the first or past the table, its page is absent). `mine`: a sequence has the row.
+struct Place {
+  int64_t code, scale;
+  int pos;          // of a row that is `mine`
+  bool mine, there;
+};
+template <int FMT, int D>
+__device__ __forceinline__ Place place_of(const Seqs& s, const Cache& c, int row) {
+  Place p{0, 0, 0, false, false};
+  Seq q;
+  const int b = seq_of_row<D / 8 == 16 ? 16 : 8>(s, min(row, s.rows - 1), q);
+  if (b < 0 || row >= s.rows) return p;
+  p.mine = true;
+  p.pos = q.pos + (row - q.first);
+  if (p.pos < 0 || p.pos >= s.cap) return p;
+  const int pg = page_of(s, c, b, p.pos);
+  if (pg < 0) return p;
+  const int off = p.pos & ((1 << c.log2page) - 1);
+  p.code = pg * c.page_stride + off * (FMT == FP4 ? D / 2 : D);
+  p.scale = pg * c.spage_stride + off * (FMT == FP4 ? D / GROUP4 : 1);
+  p.there = true;
+  return p;
+}
+
+__device__ __forceinline__ uint32_t max_with(uint32_t v, int lane_xor) { return max(v, static_cast<uint32_t>(__shfl_xor(static_cast<int>(v), lane_xor))); }
+// the largest magnitude of 8 values by its bits: they order like the values, infinities and NaN last
+__device__ __forceinline__ uint32_t magnitude8(const float* x) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) m = max(m, __float_as_uint(x[e]) & 0x7fffffffu);
+  return m;
+}
+// max over the D / 8 lanes of a row
+template <int D>
+__device__ __forceinline__ uint32_t row_max(uint32_t v) {
+  v = max_with(max_with(max_with(v, 1), 2), 4);
+  if constexpr (D == 128) v = max_with(v, 8);
+  return v;
+}
+
+template <int FMT, int D>
+__device__ __forceinline__ void put8(const float* x, uint8_t* codes, float* scale, bool first) {
+  const uint32_t m = row_max<D>(magnitude8(x));
+  uint2 q = make_uint2(0u, 0u);
+  float s = __uint_as_float(0x7fc00000u);
+  if (m < 0x7f800000u) {
+    s = fmaxf(__uint_as_float(m) / (FMT == INT8 ? 127.0f : 448.0f), 1e-12f);
+    const float inv = 1.0f / s;
+    if constexpr (FMT == INT8)
+      q = quant8_i8(x, s, inv);
+    else
+      q = quant8_fp8(x, s, inv, fp8_odd(__uint_as_float(m), 0.0f, s));
+  }
+  *reinterpret_cast<uint2*>(codes) = q;
+  if (first) *scale = s;
+}
+
+// lane l of a row's D / 8: its 8 values of a key (x) and value (y) of head h to their codes
+template <int FMT, int D>
+__device__ __forceinline__ void put(const Cache& c, const Place& p, int h, int l, const float* x, const float* y) {
+  if constexpr (FMT != FP4) {
+    const int64_t code = p.code + h * c.head_stride + 8 * l, scale = p.scale + h * c.shead_stride;
+    put8<FMT, D>(x, c.k + code, c.ks + scale, l == 0);
+    put8<FMT, D>(y, c.v + code, c.vs + scale, l == 0);
+  } else {
+    // 4 lanes are a group. An infinity or a NaN anywhere in the two rows marks the position: key scales 255, all else 0
+    const uint32_t mk = max_with(max_with(magnitude8(x), 1), 2), mv = max_with(max_with(magnitude8(y), 1), 2);
+    uint32_t all = max_with(max(mk, mv), 4);
+    if constexpr (D == 128) all = max_with(all, 8);
+    uint32_t sk = 255, sv = 0, wk = 0, wv = 0;
+    if (all < 0x7f800000u) {
+      sk = scale4(mk);
+      sv = scale4(mv);
+      wk = codes4(x, sk);
+      wv = codes4(y, sv);
+    }
+    const int64_t code = p.code + h * c.head_stride + 4 * l, scale = p.scale + h * c.shead_stride + l / 4;
+    *reinterpret_cast<uint32_t*>(c.k + code) = wk;
+    *reinterpret_cast<uint32_t*>(c.v + code) = wv;
+    if (l % 4 == 0) {
+      reinterpret_cast<uint8_t*>(c.ks)[scale] = static_cast<uint8_t>(sk);
+      reinterpret_cast<uint8_t*>(c.vs)[scale] = static_cast<uint8_t>(sv);
+    }
+  }
+}
+
+// Workgroups for `rows` rows: along x the rows, along y as many heads side by side as it takes for 8 workgroups to a CU; the
+// other heads are the workgroup's loop, which resolves a row's page once for all of them.
+inline dim3 grid_of(int64_t rows, int heads, int dim) {
+  const int64_t gx = (rows + NT / (dim / 8) - 1) / (NT / (dim / 8));
+  const int64_t want = 8 * static_cast<int64_t>(device_cus() > 0 ? device_cus() : 256);
+  int64_t gy = (want + gx - 1) / gx;
+  gy = gy < 1 ? 1 : gy > heads ? heads : gy;
+  return dim3(static_cast<uint32_t>(gx), static_cast<uint32_t>(gy));
+}
+
+}  // namespace kv
+}  // namespace rh3

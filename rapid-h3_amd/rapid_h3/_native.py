@@ -95,6 +95,7 @@ RH3_DTYPE_F32 = 2
 RH3_DTYPE_F16 = 3
 RH3_KV_INT8 = 0
 RH3_KV_E4M3 = 1
+RH3_KV_FP4 = 4
 RH3_KV_BY_SIZE, RH3_KV_TOKEN, RH3_KV_CHUNK = 0, 1, 2
 
 _lib = None

@@ -23,6 +23,10 @@ import torch
 from . import _native as nat
 
 FP8 = torch.float8_e4m3fn
+FP4 = torch.float4_e2m1fn_x2          # two codes to a byte
+GROUP4 = 32                           # channels of a 4-bit row that share a scale
+_BYTES = (torch.uint8, FP4)
+_SCALE4 = (torch.uint8, torch.float8_e8m0fnu)
 _ROW = {torch.bfloat16: nat.RH3_DTYPE_BF16, torch.float16: nat.RH3_DTYPE_F16, torch.float32: nat.RH3_DTYPE_F32}
 _FORM = {None: nat.RH3_KV_BY_SIZE, "token": nat.RH3_KV_TOKEN, "chunk": nat.RH3_KV_CHUNK}
 _HERE = contextlib.nullcontext()
@@ -36,8 +40,10 @@ def _st(t, axis):
 class KVCache:
     """The pages of one layer: k, v [P, heads, page, dim] int8 or float8_e4m3fn codes, k_scale, v_scale [P, heads, page]
     fp32 (page 16 to 256, a power of two; dim 64 or 128; views of larger buffers whose pages and heads lie apart are fine,
-    k like v and k_scale like v_scale). Where a position holds something, no code is NaN and a scale is finite and not
-    negative, or NaN for a row that is (as kv_write leaves them). The tensors are kept and used as they are; the attributes
+    k like v and k_scale like v_scale). 4-bit codes: k, v [P, heads, page, dim / 2] float4_e2m1fn_x2 or uint8, two codes to a byte, the
+    lower channel in the low half; k_scale, v_scale [P, heads, page, dim / 32] float8_e8m0fnu or uint8, e + 127. Where a position holds something, no code is NaN and a scale is finite and not
+    negative, or NaN for a row that is (as kv_write leaves them); of 4-bit codes, a scale byte is at most 252, or 255 in all of
+    k_scale's at a position whose key or value is not finite (NaN in both). The tensors are kept and used as they are; the attributes
     cannot be changed."""
 
     __slots__ = ("k", "v", "k_scale", "v_scale", "pages", "heads", "page", "dim", "device", "gpu", "_desc", "_ref")
@@ -46,25 +52,31 @@ class KVCache:
         if k.ndim != 4 or v.shape != k.shape or any(_st(v, i) != _st(k, i) for i in range(4)):
             raise RuntimeError(f"KVCache: k and v must be [pages, heads, page, dim] of one layout, got {tuple(k.shape)} and {tuple(v.shape)}")
         p, h, n, d = k.shape
-        if k.dtype not in (torch.int8, FP8) or v.dtype != k.dtype:
-            raise TypeError(f"KVCache: codes must be int8 or float8_e4m3fn, got {k.dtype} and {v.dtype}")
-        if d not in (64, 128) or n not in (16, 32, 64, 128, 256):
-            raise RuntimeError(f"KVCache: head dim 64 or 128 and pages of 16, 32, 64, 128 or 256 positions, got {d} and {n}")
+        four = k.dtype in _BYTES and v.dtype in _BYTES
+        if not four and (k.dtype not in (torch.int8, FP8) or v.dtype != k.dtype):
+            raise TypeError(f"KVCache: codes must be int8 or float8_e4m3fn, or pairs of 4-bit ones (float4_e2m1fn_x2 or uint8), got {k.dtype} and {v.dtype}")
+        dim = 2 * d if four else d
+        if dim not in (64, 128) or n not in (16, 32, 64, 128, 256):
+            raise RuntimeError(f"KVCache: head dim 64 or 128 and pages of 16, 32, 64, 128 or 256 positions, got {dim} and {n}")
         if k.stride(3) != 1 or k.stride(2) != d:
             raise RuntimeError("KVCache: a head's positions in a page must be contiguous")
         for s in (k_scale, v_scale):
-            if s.shape != (p, h, n) or s.dtype != torch.float32 or s.stride(2) != 1:
+            if four:
+                if s.shape != (p, h, n, dim // GROUP4) or s.dtype not in _SCALE4 or s.stride(3) != 1 or s.stride(2) != dim // GROUP4:
+                    raise RuntimeError("KVCache: scales of 4-bit codes must be float8_e8m0fnu or uint8 [pages, heads, page, dim / 32] with a "
+                                       "head's positions in a page contiguous")
+            elif s.shape != (p, h, n) or s.dtype != torch.float32 or s.stride(2) != 1:
                 raise RuntimeError("KVCache: scales must be fp32 [pages, heads, page] with a contiguous last dim")
         if any(_st(v_scale, i) != _st(k_scale, i) for i in range(2)):
             raise RuntimeError("KVCache: k_scale and v_scale must have one layout")
         if not k.is_cuda or any(t.device != k.device for t in (v, k_scale, v_scale)):
             raise RuntimeError("KVCache: the four tensors must be on one GPU (no CPU path)")
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
-        self.pages, self.heads, self.page, self.dim, self.device = p, h, n, d, k.device
+        self.pages, self.heads, self.page, self.dim, self.device = p, h, n, dim, k.device
         self.gpu = k.get_device()
         self._desc = nat.KvCacheDesc(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), _st(k, 0), _st(k, 1),
-                                     _st(k_scale, 0), _st(k_scale, 1), p, h, n, d,
-                                     nat.RH3_KV_INT8 if k.dtype == torch.int8 else nat.RH3_KV_E4M3)
+                                     _st(k_scale, 0), _st(k_scale, 1), p, h, n, dim,
+                                     nat.RH3_KV_FP4 if four else nat.RH3_KV_INT8 if k.dtype == torch.int8 else nat.RH3_KV_E4M3)
         self._ref = ctypes.addressof(self._desc)
 
     def __setattr__(self, name, value):
@@ -74,11 +86,15 @@ class KVCache:
 
 
 def kv_cache(pages, heads, page=64, dim=128, dtype=torch.int8, device="cuda"):
-    """A new cache of zeros."""
+    """A new cache of zeros: dtype int8, float8_e4m3fn or float4_e2m1fn_x2."""
+    four = dtype == FP4
+
     def codes():
-        return torch.zeros((pages, heads, page, dim), dtype=torch.int8, device=device).view(dtype)
+        return torch.zeros((pages, heads, page, dim // 2 if four else dim), dtype=torch.uint8, device=device).view(dtype)
 
     def scales():
+        if four:
+            return torch.zeros((pages, heads, page, dim // GROUP4), dtype=torch.uint8, device=device).view(torch.float8_e8m0fnu)
         return torch.zeros((pages, heads, page), dtype=torch.float32, device=device)
     return KVCache(codes(), codes(), scales(), scales())
 
@@ -134,7 +150,8 @@ def _rows_call(name, entry, what, cache, k, v, table, lens, cu):
 
 def kv_write(cache, k, v, table, lens, cu=None):
     """Quantise rows k, v [rows, heads, dim] (bf16, fp16 or fp32, strided ok) into their positions. Rows at a negative
-    position, past the table or in an absent page are skipped; a row that holds an infinity or a NaN is kept as NaN (its scale).
+    position, past the table or in an absent page are skipped; a row that holds an infinity or a NaN is kept as NaN (its scale; in 4 bits, key and value
+    of that head's position alike).
     A position that two rows of a call name (a page that sequences share, or that a table names twice) ends with a mixture of
     them."""
     _rows_call("kv_write", "rh3_kv_write", ("k", "v"), cache, k, v, table, lens, cu)
