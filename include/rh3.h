@@ -504,6 +504,26 @@ int rh3_kv_read(const rh3_kv_cache* cache, void* k, int64_t k_st, int64_t k_sh, 
                 int dtype, int64_t rows, const int32_t* table, int64_t table_stride, int64_t width, const int32_t* lens,
                 const int32_t* cu, int64_t batch, hipStream_t stream);
 
+/* The RMS norm (norm != 0: y = (x / sqrt(mean x^2 + eps)) * w, qw and kw [dim] of the rows' type, or fp32 where wide_weights, or
+ * NULL) and rotation (rot > 0 channels, a multiple of 16) of each head's row of q [rows][q_heads][dim] and k [rows][k_heads][dim]
+ * (dim 64 or 128; either may have 0 heads; strides as above): pairs (a, b) of channels i and i + rot / 2 (interleaved: 2 i and
+ * 2 i + 1) become (a cos - b sin, b cos + a sin) of the angle positions[row] * freq[i] (freq [rot / 2], 64 bits, as the product is),
+ * cosine and sine times factor; rounded to the rows' type once. The results may lie exactly over q and k. */
+int rh3_qk_norm_rope(const void* q, int64_t q_st, int64_t q_sh, void* q_out, int64_t qo_st, int64_t qo_sh, int64_t q_heads,
+                     const void* k, int64_t k_st, int64_t k_sh, void* k_out, int64_t ko_st, int64_t ko_sh, int64_t k_heads,
+                     int64_t rows, int64_t dim, int dtype, const int32_t* positions, const double* freq, int64_t rot,
+                     int interleaved, double factor, int norm, double eps, const void* qw, const void* kw, int wide_weights,
+                     hipStream_t stream);
+
+/* rh3_qk_norm_rope at the rows' positions in their sequences (plus first) and rh3_kv_write of its k (rounded to the rows' type) and of
+ * v, in one pass. Rows that no sequence has are not touched; of rows whose position is nowhere in the cache only q is done. */
+int rh3_kv_write_rope(const rh3_kv_cache* cache, const void* q, int64_t q_st, int64_t q_sh, void* q_out, int64_t qo_st,
+                      int64_t qo_sh, int64_t q_heads, const void* k, int64_t k_st, int64_t k_sh, const void* v, int64_t v_st,
+                      int64_t v_sh, int dtype, int64_t rows, const int32_t* table, int64_t table_stride, int64_t width,
+                      const int32_t* lens, const int32_t* cu, int64_t batch, int64_t first, const double* freq, int64_t rot,
+                      int interleaved, double factor, int norm, double eps, const void* qw, const void* kw, int wide_weights,
+                      hipStream_t stream);
+
 /* out = softmax(scale q k^T) v over a sequence's cached positions (causal: row i of n sees positions up to
  * lens[b] - n + i), q and out [rows][q_heads][dim] bf16 or fp16, query head h reads K/V head h / (q_heads / heads); lse
  * [rows][q_heads] fp32 or NULL: the natural log of the sum of exp(scale q.k). A row that sees no key gives 0 and -inf; one

@@ -1,0 +1,380 @@
+// The RMS norm of each query and key head with its position rotation, in one pass over the rows; and the same on the way into the
+// paged cache, with the keys and values quantised where they lie: no key is written and read in between.
+//
+// A row x of a head (dim channels): y = (x * r) * w, r = 1 / sqrt(mean x^2 + eps); then pairs (a, b) of the first `rot` channels turn by
+// the angle position * f_i: (a cos - b sin, b cos + a sin), the pairs being channels (i, i + rot / 2) or (2 i, 2 i + 1). One rounding to
+// the rows' type at the end. What is quantised afterwards may lie next to a code's border, so every step is defined to the last
+// bit or nearly so: the squares are summed and r is made in 64 bits and rounded to fp32 once, angles are 64-bit products (a far
+// position times a frequency), their cosines and sines are made in 64 bits (good to some 2^-52) and rounded to fp32 once, the rest
+// are single fp32 operations in the order written. The vector units do as many 64-bit fused multiply-adds as 32-bit ones, and an
+// angle's are shared by all heads of a token.
+//
+// Bound by memory. A workgroup takes 4 tokens (few rows: 1), makes their cosines and sines in LDS, one angle to a thread, and walks
+// the heads, 16 rows of 128 at a time (64: 32); a row is 8 channels in each of dim / 8 lanes, which keep their token and so the
+// cosines and sines of their channels in registers. The other channels of a lane's pairs, where they lie rot / 2 apart, are loaded
+// a second time (from L1) and normed again, which needs no exchange between lanes.
+#include "kv_rows.hpp"
+
+namespace rh3 {
+namespace kv {
+namespace {
+
+constexpr int NONE = -1;             // FMT of the rows that go to no cache
+constexpr int MOST_PAIRS = 64;       // of a head
+
+struct Turn {
+  const double* freq;                // [rot / 2] radians to a position, or null
+  double factor;                     // of the cosines and sines
+  int rot, interleaved;
+  int norm, wide;                    // wide: fp32 weights (else of the rows' type)
+  double eps;
+  const void *qw, *kw;               // [dim] or null
+};
+struct Rows {
+  const void* x;
+  int64_t st, sh;
+};
+struct Out {
+  void* x;
+  int64_t st, sh;
+};
+struct RopeArgs {
+  Turn t;
+  Rows q, k, v;
+  Out qo, ko;                        // ko: FMT NONE
+  int q_heads, k_heads, rows, log2tt;
+  int first;                         // added to the positions of the cache's rows
+  const int32_t* positions;          // FMT NONE
+  Cache c;
+  Seqs s;
+};
+
+// cosine and sine of a (64 bits): a less the nearest multiple of pi / 2 (in two parts of 53 bits), then the Taylor series, whose next
+// terms are under 2^-54 on +-pi / 4
+__device__ __forceinline__ float2 cos_sin(double a, double factor) {
+  const double n = __builtin_rint(a * 0.63661977236758134308);
+  double r = __builtin_fma(n, -1.57079632679489655800, a);
+  r = __builtin_fma(n, -6.12323399573676603587e-17, r);
+  const double z = r * r;
+  double s = -1.0 / 1307674368000.0, c = 1.0 / 20922789888000.0;
+  s = __builtin_fma(s, z, 1.0 / 6227020800.0);
+  s = __builtin_fma(s, z, -1.0 / 39916800.0);
+  s = __builtin_fma(s, z, 1.0 / 362880.0);
+  s = __builtin_fma(s, z, -1.0 / 5040.0);
+  s = __builtin_fma(s, z, 1.0 / 120.0);
+  s = __builtin_fma(s, z, -1.0 / 6.0);
+  s = __builtin_fma(s * z, r, r);
+  c = __builtin_fma(c, z, -1.0 / 87178291200.0);
+  c = __builtin_fma(c, z, 1.0 / 479001600.0);
+  c = __builtin_fma(c, z, -1.0 / 3628800.0);
+  c = __builtin_fma(c, z, 1.0 / 40320.0);
+  c = __builtin_fma(c, z, -1.0 / 720.0);
+  c = __builtin_fma(c, z, 1.0 / 24.0);
+  c = __builtin_fma(c, z, -0.5);
+  c = __builtin_fma(c, z, 1.0);
+  const int quarter = static_cast<int>(n - 4.0 * __builtin_floor(n * 0.25));   // 0 .. 3 quarters of a turn
+  const double x = quarter & 1 ? s : c, y = quarter & 1 ? c : s;
+  return make_float2(static_cast<float>((quarter == 1 || quarter == 2 ? -x : x) * factor), static_cast<float>((quarter >= 2 ? -y : y) * factor));
+}
+
+// a lane's 64-bit value from lane l ^ 8, 4, 2 or 1 of its 16
+template <int CTRL>
+__device__ __forceinline__ double moved(double v) {
+  const int64_t b = __builtin_bit_cast(int64_t, v);
+  const int lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(b), CTRL, 0xf, 0xf, true);
+  const int hi = __builtin_amdgcn_update_dpp(0, static_cast<int>(b >> 32), CTRL, 0xf, 0xf, true);
+  return __builtin_bit_cast(double, (static_cast<int64_t>(hi) << 32) | static_cast<uint32_t>(lo));
+}
+// 1 / sqrt(mean x^2 + eps) of a row in dim / 8 lanes
+template <int D>
+__device__ __forceinline__ float inverse_rms(const float* x, double eps) {
+  double s = 0.0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) s = __builtin_fma(static_cast<double>(x[e]), static_cast<double>(x[e]), s);
+  s += moved<0xB1>(s);                      // quad_perm [1,0,3,2]
+  s += moved<0x4E>(s);                      // quad_perm [2,3,0,1]
+  s += moved<0x1B>(moved<0x141>(s));        // row_half_mirror, quad_perm [3,2,1,0]: lane ^ 4
+  if constexpr (D == 128) s += moved<0x128>(s);   // row_ror:8
+  const double m = __builtin_fma(s, 1.0 / D, eps);
+  double y = __builtin_amdgcn_rsq(m);
+  if (m > 0.0 && m < static_cast<double>(INFINITY)) {   // two steps of Newton's method on the hardware's first 2^-24 or so
+    const double h = 0.5 * m;
+    y = __builtin_fma(y, __builtin_fma(-h * y, y, 0.5), y);
+    y = __builtin_fma(y, __builtin_fma(-h * y, y, 0.5), y);
+  }
+  return static_cast<float>(y);
+}
+
+template <int DT>
+struct Raw {
+  uint4 w[DT == RH3_DTYPE_F32 ? 2 : 1];
+};
+template <int DT>
+__device__ __forceinline__ Raw<DT> load_raw(const void* p, int64_t at) {
+  Raw<DT> r;
+  const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p) + at * (DT == RH3_DTYPE_F32 ? 4 : 2));
+  r.w[0] = src[0];
+  if constexpr (DT == RH3_DTYPE_F32) r.w[1] = src[1];
+  return r;
+}
+template <int DT>
+__device__ __forceinline__ void values_of(const Raw<DT>& r, float* x) {
+  if constexpr (DT == RH3_DTYPE_F32) {
+    const uint32_t w[8] = {r.w[0].x, r.w[0].y, r.w[0].z, r.w[0].w, r.w[1].x, r.w[1].y, r.w[1].z, r.w[1].w};
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = __uint_as_float(w[e]);
+  } else {
+    row8<DT>(r.w[0], x);
+  }
+}
+template <int DT>
+__device__ __forceinline__ void weights8(const Turn& t, const void* w, int at, float* x) {
+  if (!w) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = 1.0f;
+  } else if (t.wide) {
+    load_row8<RH3_DTYPE_F32>(w, at, x);
+  } else {
+    load_row8<DT>(w, at, x);
+  }
+}
+// rounded to the rows' type
+template <int DT>
+__device__ __forceinline__ void rounded8(float* x) {
+  if constexpr (DT == RH3_DTYPE_BF16) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = round_bf(x[e]);
+  } else if constexpr (DT == RH3_DTYPE_F16) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = static_cast<float>(static_cast<_Float16>(x[e]));
+  }
+}
+
+template <int FMT, int D, int DT>
+__global__ void __launch_bounds__(NT) rope_kernel(RopeArgs a) {
+  constexpr int LPR = D / 8, SLOTS = NT / LPR;
+  __shared__ float2 turns[4][MOST_PAIRS];
+  const int l = threadIdx.x % LPR, slot = threadIdx.x / LPR;
+  const int tt = 1 << a.log2tt, heads_at_once = SLOTS >> a.log2tt;
+  const int tok = slot & (tt - 1), row = (blockIdx.x << a.log2tt) + tok, hs = slot >> a.log2tt;
+  const Turn& t = a.t;
+  const int half = t.rot >> 1, c0 = 8 * l;
+  const bool turned = c0 < t.rot;
+  // the other half's channels of the lane's pairs
+  const int p0 = t.interleaved || !turned ? c0 : c0 < half ? c0 + half : c0 - half;
+
+  Place place{0, 0, 0, true, false};
+  if constexpr (FMT != NONE) place = place_of<FMT, D>(a.s, a.c, row);
+  const bool mine = row < a.rows && place.mine;
+  const int q_groups = (a.q_heads + heads_at_once - 1) / heads_at_once, k_groups = (a.k_heads + heads_at_once - 1) / heads_at_once;
+  int g = blockIdx.y;
+  auto load = [&](int g, Raw<DT>& own, Raw<DT>& other) __attribute__((always_inline)) {
+    const bool key = g >= q_groups;
+    const int h = (key ? g - q_groups : g) * heads_at_once + hs;
+    if (mine && g < q_groups + k_groups && h < (key ? a.k_heads : a.q_heads)) {
+      const Rows& r = key ? a.k : a.q;
+      own = load_raw<DT>(r.x, row * r.st + h * r.sh + c0);
+      other = load_raw<DT>(r.x, row * r.st + h * r.sh + p0);
+    }
+  };
+  Raw<DT> own{}, other{};
+  load(g, own, other);
+
+  if (half) {
+    for (int i = threadIdx.x; i < half << a.log2tt; i += NT) {
+      const int r = i / half, f = i - r * half;
+      const int at = (blockIdx.x << a.log2tt) + r;
+      int pos = 0;
+      if constexpr (FMT == NONE) {
+        if (at < a.rows) pos = a.positions[at];
+        turns[r][f] = cos_sin(static_cast<double>(pos) * t.freq[f], t.factor);
+      }
+    }
+    if constexpr (FMT != NONE) {
+      // a token's position is known to its own lanes: LPR of them and, with other heads of it, those of other slots
+      const double pos = static_cast<double>(static_cast<int64_t>(place.pos) + a.first);
+      for (int f = hs * LPR + l; f < half; f += heads_at_once * LPR) turns[tok][f] = cos_sin(pos * t.freq[f], t.factor);
+    }
+    __syncthreads();
+  }
+  float cs[8], sn[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    cs[e] = 1.0f;
+    sn[e] = 0.0f;
+  }
+  if (turned) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float2 v = turns[tok][t.interleaved ? (c0 + e) >> 1 : (c0 < half ? c0 : c0 - half) + e];
+      cs[e] = v.x;
+      sn[e] = (t.interleaved ? (e & 1) == 0 : c0 < half) ? -v.y : v.y;
+    }
+  }
+  float w[8], wo[8];
+  bool loaded_q = false, loaded_k = false;
+  for (; g < q_groups + k_groups; g += gridDim.y) {
+    const bool key = g >= q_groups;
+    const int h = (key ? g - q_groups : g) * heads_at_once + hs;
+    const bool here = mine && h < (key ? a.k_heads : a.q_heads);
+    Raw<DT> next_own{}, next_other{};
+    load(g + gridDim.y, next_own, next_other);
+    if (t.norm && !(key ? loaded_k : loaded_q)) {
+      weights8<DT>(t, key ? t.kw : t.qw, c0, w);
+      weights8<DT>(t, key ? t.kw : t.qw, p0, wo);
+      loaded_q = !key;
+      loaded_k = key;
+    }
+    if (here) {   // whole rows of lanes
+      float x[8], o[8];
+      values_of<DT>(own, x);
+      values_of<DT>(other, o);
+      if (t.norm) {
+        const float r = inverse_rms<D>(x, t.eps);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          x[e] = (x[e] * r) * w[e];
+          o[e] = (o[e] * r) * wo[e];
+        }
+      }
+      if (turned) {
+        if (t.interleaved) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) o[e] = x[e ^ 1];
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = x[e] * cs[e] + o[e] * sn[e];
+      }
+      if (!key) {
+        store_row8<DT>(a.qo.x, row * a.qo.st + h * a.qo.sh + c0, x);
+      } else if constexpr (FMT == NONE) {
+        store_row8<DT>(a.ko.x, row * a.ko.st + h * a.ko.sh + c0, x);
+      } else if (place.there) {
+        float y[8];
+        values_of<DT>(load_raw<DT>(a.v.x, row * a.v.st + h * a.v.sh + c0), y);
+        rounded8<DT>(x);
+        put<FMT, D>(a.c, place, h, l, x, y);
+      }
+    }
+    own = next_own;
+    other = next_other;
+  }
+}
+
+int check_turn(const char* name, const Turn& t, int64_t rot, int64_t dim) {
+  RH3_REQUIRE(dim == 64 || dim == 128, "%s: head dim %lld (64 or 128)", name, static_cast<long long>(dim));
+  RH3_REQUIRE(rot >= 0 && rot <= dim && rot % 16 == 0, "%s: %lld rotated channels of %lld (a multiple of 16)", name, static_cast<long long>(rot),
+              static_cast<long long>(dim));
+  RH3_REQUIRE(rot == 0 || t.freq, "%s: no frequencies for %lld rotated channels", name, static_cast<long long>(rot));
+  RH3_REQUIRE(rot || t.norm, "%s: neither a norm nor a rotation", name);
+  RH3_REQUIRE(aligned16(t.qw) && aligned16(t.kw) && (reinterpret_cast<uintptr_t>(t.freq) & 7) == 0, "%s: weights must be 16-byte aligned, frequencies 8-byte", name);
+  return RH3_OK;
+}
+int check_rows(const char* name, const char* what, const void* x, int64_t st, int64_t sh) {
+  RH3_REQUIRE(x, "%s: null %s", name, what);
+  RH3_REQUIRE(aligned16(x) && st % 8 == 0 && sh % 8 == 0, "%s: %s must be 16-byte aligned with strides that are multiples of 8", name, what);
+  return RH3_OK;
+}
+int check_out(const char* name, const char* what, const Out& o, int64_t rows, int64_t heads) {
+  if (const int e = check_rows(name, what, o.x, o.st, o.sh)) return e;
+  RH3_REQUIRE((rows == 1 || o.st != 0) && (heads == 1 || o.sh != 0), "%s: rows or heads of %s share memory", name, what);
+  return RH3_OK;
+}
+
+// Few tokens go one to a workgroup, whose heads then take fewer turns; heads are spread over workgroups until there are 8 to a CU.
+template <int FMT, int D>
+int launch_rope(const char* name, RopeArgs& a, int dtype, hipStream_t st) {
+  const int64_t cus = device_cus() > 0 ? device_cus() : 256;
+  a.log2tt = a.rows < 4 * cus ? 0 : 2;
+  const int at_once = NT / (D / 8) >> a.log2tt;
+  const int64_t gx = (static_cast<int64_t>(a.rows) + (1 << a.log2tt) - 1) >> a.log2tt;
+  const int64_t groups = (a.q_heads + at_once - 1) / at_once + (a.k_heads + at_once - 1) / at_once;
+  int64_t gy = (8 * cus + gx - 1) / gx;
+  gy = gy < 1 ? 1 : gy > groups ? groups : gy;
+  RH3_REQUIRE(gx <= MAX_GRID_256, "%s: %d rows in one call", name, a.rows);
+  const dim3 grid(static_cast<uint32_t>(gx), static_cast<uint32_t>(gy));
+  auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(NT), 0, st, a); };
+  if (dtype == RH3_DTYPE_BF16) go(rope_kernel<FMT, D, RH3_DTYPE_BF16>);
+  else if (dtype == RH3_DTYPE_F16) go(rope_kernel<FMT, D, RH3_DTYPE_F16>);
+  else go(rope_kernel<FMT, D, RH3_DTYPE_F32>);
+  return launch_status(name);
+}
+
+}  // namespace
+}  // namespace kv
+}  // namespace rh3
+
+using namespace rh3;
+using namespace rh3::kv;
+
+extern "C" int rh3_qk_norm_rope(const void* q, int64_t q_st, int64_t q_sh, void* q_out, int64_t qo_st, int64_t qo_sh, int64_t q_heads,
+                                const void* k, int64_t k_st, int64_t k_sh, void* k_out, int64_t ko_st, int64_t ko_sh, int64_t k_heads,
+                                int64_t rows, int64_t dim, int dtype, const int32_t* positions, const double* freq, int64_t rot,
+                                int interleaved, double factor, int norm, double eps, const void* qw, const void* kw, int wide_weights,
+                                hipStream_t stream) {
+  const char* name = "qk_norm_rope";
+  clear_error();
+  RopeArgs a{};
+  a.t = Turn{freq, factor, static_cast<int>(rot), interleaved != 0, norm != 0, wide_weights != 0, eps, qw, kw};
+  if (const int e = check_turn(name, a.t, rot, dim)) return e;
+  RH3_REQUIRE(rows >= 0 && rows <= MAX_ROWS, "%s: %lld rows", name, static_cast<long long>(rows));
+  RH3_REQUIRE(q_heads >= 0 && q_heads <= 65535 && k_heads >= 0 && k_heads <= 65535, "%s: %lld and %lld heads", name, static_cast<long long>(q_heads),
+              static_cast<long long>(k_heads));
+  RH3_REQUIRE(dtype == RH3_DTYPE_BF16 || dtype == RH3_DTYPE_F16 || dtype == RH3_DTYPE_F32, "%s: row type %d (bf16, fp16 or fp32)", name, dtype);
+  if (rows == 0 || q_heads + k_heads == 0) return RH3_OK;
+  RH3_REQUIRE(rot == 0 || positions, "%s: no positions", name);
+  a.q = Rows{q, q_st, q_sh};
+  a.k = Rows{k, k_st, k_sh};
+  a.qo = Out{q_out, qo_st, qo_sh};
+  a.ko = Out{k_out, ko_st, ko_sh};
+  if (q_heads) {
+    if (const int e = check_rows(name, "q", q, q_st, q_sh)) return e;
+    if (const int e = check_out(name, "q's result", a.qo, rows, q_heads)) return e;
+  }
+  if (k_heads) {
+    if (const int e = check_rows(name, "k", k, k_st, k_sh)) return e;
+    if (const int e = check_out(name, "k's result", a.ko, rows, k_heads)) return e;
+  }
+  a.q_heads = static_cast<int>(q_heads);
+  a.k_heads = static_cast<int>(k_heads);
+  a.rows = static_cast<int>(rows);
+  a.positions = positions;
+  return dim == 128 ? launch_rope<NONE, 128>(name, a, dtype, stream) : launch_rope<NONE, 64>(name, a, dtype, stream);
+}
+
+extern "C" int rh3_kv_write_rope(const rh3_kv_cache* cache, const void* q, int64_t q_st, int64_t q_sh, void* q_out, int64_t qo_st,
+                                 int64_t qo_sh, int64_t q_heads, const void* k, int64_t k_st, int64_t k_sh, const void* v, int64_t v_st,
+                                 int64_t v_sh, int dtype, int64_t rows, const int32_t* table, int64_t table_stride, int64_t width,
+                                 const int32_t* lens, const int32_t* cu, int64_t batch, int64_t first, const double* freq, int64_t rot,
+                                 int interleaved, double factor, int norm, double eps, const void* qw, const void* kw, int wide_weights,
+                                 hipStream_t stream) {
+  const char* name = "kv_write_rope";
+  clear_error();
+  RopeArgs a{};
+  if (const int e = check_cache(name, cache, a.c)) return e;
+  if (const int e = check_seqs(name, a.c, table, table_stride, width, lens, cu, batch, rows, a.s)) return e;
+  a.t = Turn{freq, factor, static_cast<int>(rot), interleaved != 0, norm != 0, wide_weights != 0, eps, qw, kw};
+  if (const int e = check_turn(name, a.t, rot, cache->dim)) return e;
+  RH3_REQUIRE(q_heads >= 1 && q_heads <= 65535, "%s: %lld query heads", name, static_cast<long long>(q_heads));
+  RH3_REQUIRE(first >= -MAX_ROWS && first <= MAX_ROWS, "%s: first position %lld", name, static_cast<long long>(first));
+  RH3_REQUIRE(dtype == RH3_DTYPE_BF16 || dtype == RH3_DTYPE_F16 || dtype == RH3_DTYPE_F32, "%s: row type %d (bf16, fp16 or fp32)", name, dtype);
+  if (rows == 0) return RH3_OK;
+  a.q = Rows{q, q_st, q_sh};
+  a.k = Rows{k, k_st, k_sh};
+  a.v = Rows{v, v_st, v_sh};
+  a.qo = Out{q_out, qo_st, qo_sh};
+  if (const int e = check_rows(name, "q", q, q_st, q_sh)) return e;
+  if (const int e = check_rows(name, "k", k, k_st, k_sh)) return e;
+  if (const int e = check_rows(name, "v", v, v_st, v_sh)) return e;
+  if (const int e = check_out(name, "q's result", a.qo, rows, q_heads)) return e;
+  a.q_heads = static_cast<int>(q_heads);
+  a.k_heads = a.c.heads;
+  a.rows = static_cast<int>(rows);
+  a.first = static_cast<int>(first);
+  const int64_t fmt = cache->format;
+  if (cache->dim == 128)
+    return fmt == INT8 ? launch_rope<INT8, 128>(name, a, dtype, stream)
+                       : fmt == E4M3 ? launch_rope<E4M3, 128>(name, a, dtype, stream) : launch_rope<FP4, 128>(name, a, dtype, stream);
+  return fmt == INT8 ? launch_rope<INT8, 64>(name, a, dtype, stream)
+                     : fmt == E4M3 ? launch_rope<E4M3, 64>(name, a, dtype, stream) : launch_rope<FP4, 64>(name, a, dtype, stream);
+}

@@ -14,22 +14,21 @@ The rows of a sequence are its last positions: row i of n is position lens[b] - 
 by the kernels, so a captured call follows what is written into them between replays. Rows in front of cu[0] and behind cu[B]
 are not read and stay as they are; of rows that cu names but the call does not have, it takes none.
 """
-import contextlib
 import ctypes
 import functools
 
 import torch
 
 from . import _native as nat
+from . import rope
+from ._rows import _ROW, _on, _stream
 
 FP8 = torch.float8_e4m3fn
 FP4 = torch.float4_e2m1fn_x2          # two codes to a byte
 GROUP4 = 32                           # channels of a 4-bit row that share a scale
 _BYTES = (torch.uint8, FP4)
 _SCALE4 = (torch.uint8, torch.float8_e8m0fnu)
-_ROW = {torch.bfloat16: nat.RH3_DTYPE_BF16, torch.float16: nat.RH3_DTYPE_F16, torch.float32: nat.RH3_DTYPE_F32}
 _FORM = {None: nat.RH3_KV_BY_SIZE, "token": nat.RH3_KV_TOKEN, "chunk": nat.RH3_KV_CHUNK}
-_HERE = contextlib.nullcontext()
 
 
 def _st(t, axis):
@@ -99,16 +98,6 @@ def kv_cache(pages, heads, page=64, dim=128, dtype=torch.int8, device="cuda"):
     return KVCache(codes(), codes(), scales(), scales())
 
 
-# The small calls (a token of one sequence is 12 us of GPU work in two launches) are bound by what the host does: shapes, strides
-# and devices are asked for once a call, devices as numbers, and the workspace's size once for each set of sizes.
-def _on(index):
-    """The tensors' GPU as the current one for a launch, where it is another."""
-    return _HERE if index == torch._C._cuda_getDevice() else torch.cuda.device(index)
-
-
-_stream = torch._C._cuda_getCurrentRawStream
-
-
 def _seqs(name, cache, table, lens, cu, gpu):
     """The sequences' arguments of a call after its rows: table, its stride and width, lens, cu, batch."""
     if table.ndim != 2 or table.dtype != torch.int32 or (table.stride(1) != 1 and table.shape[1] > 1):
@@ -155,6 +144,29 @@ def kv_write(cache, k, v, table, lens, cu=None):
     A position that two rows of a call name (a page that sequences share, or that a table names twice) ends with a mixture of
     them."""
     _rows_call("kv_write", "rh3_kv_write", ("k", "v"), cache, k, v, table, lens, cu)
+
+
+def kv_write_rope(cache, q, k, v, table, lens, cu=None, rotary=None, q_weight=None, k_weight=None, eps=None, first=0, out=None):
+    """rope.qk_norm_rope of the rows q [rows, q heads, dim] and k [rows, heads, dim] at their positions in their sequences (`first` more
+    than in the cache: what a shared prefix holds), with k, rounded to its type, and v written into the cache as kv_write does. ->
+    the new q (`out`, which may lie exactly over q). Rows that no sequence has are left out (0 in a new q)."""
+    name = "kv_write_rope"
+    t, k_st, k_sh = _rows(name, "k", k, cache)
+    tv, v_st, v_sh = _rows(name, "v", v, cache)
+    q_st, q_sh = rope._heads(name, "q", q)
+    gpu = q.get_device()
+    if tv != t or q.shape[0] != t or q.shape[2] != cache.dim or k.dtype != q.dtype or v.dtype != q.dtype or k.get_device() != gpu or v.get_device() != gpu:
+        raise TypeError(f"{name}: q, k and v must be of one number of rows, dim, device and type (bf16, fp16 or fp32)")
+    turn = rope._turn(name, rotary, q_weight, k_weight, eps, cache.dim, q.dtype, gpu)
+    seqs = _seqs(name, cache, table, lens, cu, gpu)
+    if out is None:
+        out = (torch.empty if cu is None else torch.zeros)(q.shape, dtype=q.dtype, device=q.device)
+    else:
+        rope._result(name, "q", q, out)
+    with _on(gpu):
+        nat.call("rh3_kv_write_rope", cache._ref, q.data_ptr(), q_st, q_sh, out.data_ptr(), *rope._heads(name, "out", out), q.shape[1],
+                 k.data_ptr(), k_st, k_sh, v.data_ptr(), v_st, v_sh, _ROW[q.dtype], t, *seqs, int(first), *turn, _stream(gpu))
+    return out
 
 
 def kv_read(cache, table, lens, cu=None, rows=None, dtype=torch.bfloat16, out=None):
