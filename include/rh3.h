@@ -489,6 +489,18 @@ typedef struct rh3_kv_cache {
   int64_t pages, heads, page, dim, format;
 } rh3_kv_cache;
 
+/* The page tables of a batch from one step to the next. A pool: free_pages [pages], of which the first state[0] are free, taken and
+ * given back at the end; state[1]: how many pages this call lacked. In the order of the sequences: the pages of those with done[b] != 0
+ * (done NULL: none) go back, in the order of the table, which then holds -1; each sequence's length becomes (done ? 0 : lens[b]) +
+ * more[b], and the entries of its row of the table that this adds (as far as width) are the next pages off the list, -1 where it is
+ * empty. cu [batch + 1]: where each one's new rows begin; of each of `rows` (a capacity) its position in its sequence and its slot, page *
+ * page size + offset; slots -1 where it has no place, both -1 behind cu[batch]. Negative lens and more count as 0; a length is at most
+ * 2^30. batch * width at most 2^30. Everything is device memory; nothing is read back. The workspace holds sums for a call. */
+int64_t rh3_kv_extend_workspace_bytes(int64_t batch);
+int rh3_kv_extend(int32_t* free_pages, int64_t pages, int32_t* state, int64_t page, int32_t* table, int64_t table_stride,
+                  int64_t width, int32_t* lens, const int32_t* more, const uint8_t* done, int64_t batch, int32_t* cu,
+                  int32_t* positions, int64_t* slots, int64_t rows, void* workspace, int64_t workspace_bytes, hipStream_t stream);
+
 /* Quantizes rows of k and v (bf16, fp16 or fp32) into their positions: s = max(amax / QMAX, 1e-12) (127 or 448), code =
  * round_half_even(x / s); a row with an infinity or a NaN gets s = NaN and codes 0. RH3_KV_FP4: e the least with amax <= 7 * 2^e of
  * the 32 channels, within +-125, code the nearest to x / 2^e, ties to the even one, past 6 to 6; a position whose key or value has

@@ -1,0 +1,286 @@
+// The page tables of a batch from one step to the next, kept on the GPU: sequences that have ended give their pages back, every
+// sequence takes the pages that its new rows need, and of each new row the position and the slot in the cache are written down.
+//
+// A pool is a list of free pages, taken and given back at its end, and how many there are. In the order of the sequences, and of each
+// one's table: the pages of those that have ended go on the list, then those that the others need come off it. With start = 0 for a
+// sequence that has ended and its length else, end = start + its new rows, P positions to a page: the entries
+// [ceil(start / P), ceil(end / P)) of its row of the table are the next pages off the list, as far as the row and the list reach.
+// All of it is prefix sums over the sequences and searches in them, so the result is the same in every run.
+//
+// Bound by latency: a step moves 9 bytes a sequence, 12 a row and 8 a page. The sums need one workgroup: it makes them, walks the
+// pages that come back (4 entries to a thread at a time, in order) and, of small calls, does the rest too; of large ones a second
+// launch spreads the pages taken and the rows over the chip. A page that is taken is looked up in the list, not in the table, which
+// the same launch is writing.
+#include "kv_common.hpp"
+
+namespace rh3 {
+namespace kv {
+namespace {
+
+constexpr int NT = 1024, WAVES = NT / 64, ROW_NT = 256;
+constexpr int NEAR = 2048;             // sequences whose sums are kept in LDS
+constexpr int MOST = 1 << 30;          // positions of a sequence
+
+struct PagesArgs {
+  int32_t* free;
+  int32_t* state;                      // pages in the list; what the last call lacked
+  int32_t* table;
+  int64_t table_stride;
+  int32_t* lens;
+  const int32_t* more;                 // new rows
+  const uint8_t* done;
+  int32_t* cu;
+  int32_t* positions;
+  int64_t* slots;
+  int32_t *back, *taken, *start;       // workspace: pages given back and taken before each sequence [batch + 1], starts [batch + 1]
+  int pages, width, batch, rows, log2page, alone;
+};
+
+// the last i in [0, n) with at[i] <= v, where at[0] <= v < at[n]
+template <typename Array>
+__device__ __forceinline__ int search(const Array at, int n, int v) {
+  int lo = 0;
+  while (n > 1) {
+    const int half = n >> 1;
+    if (at[lo + half] <= v) {
+      lo += half;
+      n -= half;
+    } else {
+      n = half;
+    }
+  }
+  return lo;
+}
+
+__device__ __forceinline__ int pages_for(const PagesArgs& a, int positions) {
+  return min((positions + (1 << a.log2page) - 1) >> a.log2page, a.width);
+}
+
+// sum of v over the threads before this one, and of all
+template <typename T>
+__device__ __forceinline__ T scan(T v, T* waves, T& all) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  T s = v;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const T up = __shfl_up(s, d);
+    if (lane >= d) s += up;
+  }
+  if (lane == 63) waves[wave] = s;
+  __syncthreads();
+  T before = 0, total = 0;
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) {
+    const T x = waves[w];
+    before += w < wave ? x : 0;
+    total += x;
+  }
+  __syncthreads();
+  all = total;
+  return before + s - v;
+}
+
+// page i of those taken: sequence s, with `first` the number taken before it and p0 its first entry that is filled
+__device__ __forceinline__ int taken_page(const PagesArgs& a, int held, int i) { return i < held ? a.free[held - 1 - i] : -1; }
+
+template <typename Array>
+__device__ __forceinline__ void take(const PagesArgs& a, const Array taken, int held, int i) {
+  const int s = search(taken, a.batch, i);
+  const int p0 = pages_for(a, a.start[s]);
+  a.table[s * a.table_stride + p0 + i - taken[s]] = taken_page(a, held, i);
+}
+
+template <typename Cu, typename Array>
+__device__ __forceinline__ void row(const PagesArgs& a, const Cu cu, const Array taken, int held, int r, int& pos, int64_t& slot) {
+  pos = -1;
+  slot = -1;
+  if (r >= cu[a.batch]) return;
+  const int s = search(cu, a.batch, r);
+  const int start = a.start[s];
+  pos = static_cast<int>(min(static_cast<int64_t>(start) + (r - cu[s]), static_cast<int64_t>(MOST)));
+  const int p = pos >> a.log2page, p0 = pages_for(a, start);
+  if (p >= a.width) return;
+  const int page = p < p0 ? a.table[s * a.table_stride + p] : taken_page(a, held, taken[s] + p - p0);
+  if (page >= 0) slot = (static_cast<int64_t>(page) << a.log2page) + (pos & ((1 << a.log2page) - 1));
+}
+
+__global__ void __launch_bounds__(NT) plan_kernel(PagesArgs a) {
+  __shared__ int near_back[NEAR + 1], near_taken[NEAR + 1], near_cu[NEAR + 1];
+  __shared__ int waves[WAVES];
+  __shared__ int64_t waves64[WAVES];
+  const int tid = threadIdx.x;
+  const bool near = a.batch <= NEAR;
+  const int held0 = min(max(a.state[0], 0), a.pages);
+  int back = 0, taken = 0;
+  int64_t rows = 0;
+  for (int at = 0; at < a.batch; at += NT) {
+    const int b = at + tid;
+    int start = 0, end = 0, more = 0, gone = 0;
+    if (b < a.batch) {
+      const int len = min(max(a.lens[b], 0), MOST);
+      more = min(max(a.more[b], 0), MOST);
+      const bool over = a.done && a.done[b];
+      gone = over ? pages_for(a, len) : 0;
+      start = over ? 0 : len;
+      end = min(start + more, MOST);
+    }
+    const int need = max(pages_for(a, end) - pages_for(a, start), 0);
+    int all_back, all_taken;
+    int64_t all_rows;
+    const int x = back + scan(gone, waves, all_back), y = taken + scan(need, waves, all_taken);
+    const int64_t z = rows + scan(static_cast<int64_t>(more), waves64, all_rows);
+    if (b < a.batch) {
+      const int c = static_cast<int>(min(z, static_cast<int64_t>(INT32_MAX)));
+      a.lens[b] = end;
+      a.cu[b] = c;
+      a.start[b] = start;
+      a.taken[b] = y;
+      if (near) {
+        near_back[b] = x;
+        near_taken[b] = y;
+        near_cu[b] = c;
+      } else {
+        a.back[b] = x;
+      }
+    }
+    back += all_back;
+    taken += all_taken;
+    rows += all_rows;
+  }
+  if (tid == 0) {
+    const int c = static_cast<int>(min(rows, static_cast<int64_t>(INT32_MAX)));
+    a.cu[a.batch] = c;
+    a.taken[a.batch] = taken;
+    if (near) {
+      near_back[a.batch] = back;
+      near_taken[a.batch] = taken;
+      near_cu[a.batch] = c;
+    } else {
+      a.back[a.batch] = back;
+    }
+  }
+  __syncthreads();
+
+  int held = held0;
+  constexpr int EACH = 4;
+  for (int at = 0; at < back; at += NT * EACH) {
+    int entry[EACH], n = 0;
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+      const int f = at + EACH * tid + i;
+      entry[i] = -1;
+      if (f < back) {
+        const int s = near ? search(near_back, a.batch, f) : search(a.back, a.batch, f);
+        int32_t* e = a.table + s * a.table_stride + (f - (near ? near_back[s] : a.back[s]));
+        entry[i] = *e;
+        *e = -1;
+      }
+      if (entry[i] < 0 || entry[i] >= a.pages) entry[i] = -1;
+      n += entry[i] >= 0;
+    }
+    int all;
+    int to = held + scan(n, waves, all);
+#pragma unroll
+    for (int i = 0; i < EACH; ++i)
+      if (entry[i] >= 0) {
+        if (to < a.pages) a.free[to] = entry[i];
+        ++to;
+      }
+    held = min(held + all, a.pages);
+  }
+  if (tid == 0) {
+    a.state[0] = max(held - taken, 0);
+    a.state[1] = max(taken - held, 0);
+    a.start[a.batch] = held;           // for the second launch
+  }
+  if (!a.alone) return;
+  __syncthreads();
+  for (int i = tid; i < taken; i += NT) near ? take(a, near_taken, held, i) : take(a, a.taken, held, i);
+  for (int r = tid; r < a.rows; r += NT) {
+    int pos;
+    int64_t slot;
+    if (near) row(a, near_cu, near_taken, held, r, pos, slot);
+    else row(a, a.cu, a.taken, held, r, pos, slot);
+    a.positions[r] = pos;
+    a.slots[r] = slot;
+  }
+}
+
+__global__ void __launch_bounds__(ROW_NT) rows_kernel(PagesArgs a) {
+  __shared__ int near_taken[NEAR + 1], near_cu[NEAR + 1];
+  const bool near = a.batch <= NEAR;
+  if (near) {
+    for (int i = threadIdx.x; i <= a.batch; i += ROW_NT) {
+      near_taken[i] = a.taken[i];
+      near_cu[i] = a.cu[i];
+    }
+    __syncthreads();
+  }
+  const int held = a.start[a.batch], taken = near ? near_taken[a.batch] : a.taken[a.batch];
+  const int first = blockIdx.x * ROW_NT + threadIdx.x, step = gridDim.x * ROW_NT;
+  for (int i = first; i < taken; i += step) near ? take(a, near_taken, held, i) : take(a, a.taken, held, i);
+  for (int64_t r = first; r < a.rows; r += step) {
+    int pos;
+    int64_t slot;
+    if (near) row(a, near_cu, near_taken, held, static_cast<int>(r), pos, slot);
+    else row(a, a.cu, a.taken, held, static_cast<int>(r), pos, slot);
+    a.positions[r] = pos;
+    a.slots[r] = slot;
+  }
+}
+
+}  // namespace
+}  // namespace kv
+}  // namespace rh3
+
+using namespace rh3;
+using namespace rh3::kv;
+
+extern "C" int64_t rh3_kv_extend_workspace_bytes(int64_t batch) { return batch < 1 || batch > 65536 ? 0 : 3 * (batch + 1) * 4; }
+
+extern "C" int rh3_kv_extend(int32_t* free_pages, int64_t pages, int32_t* state, int64_t page, int32_t* table, int64_t table_stride,
+                             int64_t width, int32_t* lens, const int32_t* more, const uint8_t* done, int64_t batch, int32_t* cu,
+                             int32_t* positions, int64_t* slots, int64_t rows, void* workspace, int64_t workspace_bytes,
+                             hipStream_t stream) {
+  const char* name = "kv_extend";
+  clear_error();
+  RH3_REQUIRE(pages >= 1 && pages <= INT32_MAX, "%s: %lld pages", name, static_cast<long long>(pages));
+  RH3_REQUIRE(page >= 16 && page <= 256 && (page & (page - 1)) == 0, "%s: page of %lld positions (16, 32, 64, 128 or 256)", name,
+              static_cast<long long>(page));
+  RH3_REQUIRE(rows >= 0 && rows <= MAX_ROWS, "%s: %lld rows", name, static_cast<long long>(rows));
+  RH3_REQUIRE(batch >= 1 && batch <= 65536, "%s: %lld sequences (1 to 65536)", name, static_cast<long long>(batch));
+  PagesArgs a{};
+  a.log2page = __builtin_ctzll(static_cast<unsigned long long>(page));
+  RH3_REQUIRE(width >= 1 && width <= (MAX_ROWS >> a.log2page) && table_stride >= (batch > 1 ? width : 0) && batch * width <= MAX_ROWS,
+              "%s: page table of %lld entries per sequence, stride %lld", name, static_cast<long long>(width), static_cast<long long>(table_stride));
+  RH3_REQUIRE(free_pages && state && table && lens && more && cu, "%s: null pool, page table, lengths, new rows or offsets", name);
+  RH3_REQUIRE(rows == 0 || (positions && slots), "%s: null positions or slots", name);
+  RH3_REQUIRE(workspace && aligned16(workspace) && workspace_bytes >= rh3_kv_extend_workspace_bytes(batch),
+              "%s: workspace of %lld bytes needed, %lld given", name, static_cast<long long>(rh3_kv_extend_workspace_bytes(batch)),
+              static_cast<long long>(workspace_bytes));
+  a.free = free_pages;
+  a.state = state;
+  a.table = table;
+  a.table_stride = table_stride;
+  a.lens = lens;
+  a.more = more;
+  a.done = done;
+  a.cu = cu;
+  a.positions = positions;
+  a.slots = slots;
+  a.back = static_cast<int32_t*>(workspace);
+  a.taken = a.back + batch + 1;
+  a.start = a.taken + batch + 1;
+  a.pages = static_cast<int>(pages);
+  a.width = static_cast<int>(width);
+  a.batch = static_cast<int>(batch);
+  a.rows = static_cast<int>(rows);
+  a.alone = rows <= 4 * NT && batch <= NEAR;
+  hipLaunchKernelGGL(plan_kernel, dim3(1), dim3(NT), 0, stream, a);
+  if (const int e = launch_status(name)) return e;
+  if (a.alone) return RH3_OK;
+  const int64_t all = rows + rows / page + batch, most = 8 * static_cast<int64_t>(device_cus() > 0 ? device_cus() : 256);
+  const int64_t grid = (all + ROW_NT - 1) / ROW_NT;
+  hipLaunchKernelGGL(rows_kernel, dim3(static_cast<uint32_t>(grid < most ? grid : most)), dim3(ROW_NT), 0, stream, a);
+  return launch_status("kv_extend (rows)");
+}

@@ -83,6 +83,8 @@ SIGNATURES = {
     "rh3_attention_f8_prepass": ([_P, _I, _I, _P, _I, _I, _P, _I, _I, _I, _I, _I, _P, _C, _P, _P, _F, _C, _C, _C,
                                   _P, _I, ctypes.POINTER(ctypes.c_void_p), _P], _C),
     "rh3_attention_f8_forward": ([_I, _I, _I, _F, _C, _P, _I, _I, _P, _I, _P], _C),
+    "rh3_kv_extend_workspace_bytes": ([_I], ctypes.c_int64),
+    "rh3_kv_extend": ([_P, _I, _P, _I, _P, _I, _I, _P, _P, _P, _I, _P, _P, _P, _I, _P, _I, _P], _C),
     "rh3_kv_write": ([_P, _P, _I, _I, _P, _I, _I, _C, _I, _P, _I, _I, _P, _P, _I, _P], _C),
     "rh3_kv_read": ([_P, _P, _I, _I, _P, _I, _I, _C, _I, _P, _I, _I, _P, _P, _I, _P], _C),
     "rh3_qk_norm_rope": ([_P, _I, _I, _P, _I, _I, _I, _P, _I, _I, _P, _I, _I, _I, _I, _I, _C, _P, _P, _I, _C, _D, _C, _D, _P, _P, _C, _P], _C),

@@ -98,6 +98,69 @@ def kv_cache(pages, heads, page=64, dim=128, dtype=torch.int8, device="cuda"):
     return KVCache(codes(), codes(), scales(), scales())
 
 
+class KVPages:
+    """The free pages of a cache: free [pages] int32, of which the first state[0] are free; state [2] int32: how many, and how many
+    pages the last kv_extend lacked. On the GPU, and changed there; page: positions to a page. The tensors are kept and used as they
+    are; the attributes cannot be changed."""
+
+    __slots__ = ("free", "state", "page", "pages", "gpu", "_args")
+
+    def __init__(self, free, state, page):
+        if free.ndim != 1 or free.dtype != torch.int32 or not free.is_contiguous() or not free.numel():
+            raise RuntimeError("KVPages: free must be contiguous int32 [pages]")
+        if state.shape != (2,) or state.dtype != torch.int32 or not state.is_contiguous() or state.get_device() != free.get_device():
+            raise RuntimeError("KVPages: state must be contiguous int32 [2] on free's GPU")
+        if page not in (16, 32, 64, 128, 256):
+            raise RuntimeError(f"KVPages: pages of 16, 32, 64, 128 or 256 positions, got {page}")
+        if not free.is_cuda:
+            raise RuntimeError("KVPages: free must be on a GPU (no CPU path)")
+        self.free, self.state, self.page, self.pages, self.gpu = free, state, page, free.numel(), free.get_device()
+        self._args = (free.data_ptr(), self.pages, state.data_ptr(), page)
+
+    def __setattr__(self, name, value):
+        if hasattr(self, "_args"):
+            raise AttributeError(f"KVPages: {name} cannot be changed; make a new KVPages")
+        object.__setattr__(self, name, value)
+
+
+def kv_pages(pages, page=64, device="cuda"):
+    """A pool of all pages, 0 taken first."""
+    free = torch.arange(pages - 1, -1, -1, dtype=torch.int32, device=device)
+    return KVPages(free, torch.tensor([pages, 0], dtype=torch.int32, device=device), page)
+
+
+def kv_extend(pool, table, lens, new, rows, done=None):
+    """A step's page table, made on the GPU: sequences with done [B] (bool) give their pages back to the pool and begin again at
+    length 0; lens grows by new [B] int32, the rows that each sequence gets in this step; the pages that takes are put into table
+    [B, W] (entries past W are left out; -1 where the pool is empty: pool.state[1] says how many those are). table and lens change in
+    place. -> cu [B + 1], positions [rows] int32 and slots [rows] int64 of the new rows, packed sequence by sequence: the position in the
+    sequence, and page * pool.page + offset, where k.transpose(1, 2) of the cache has it (-1: nowhere). rows: how many the call has room
+    for; behind the last row both are -1. cu, lens and table are what the other calls take."""
+    name = "kv_extend"
+    gpu = pool.gpu
+    if table.ndim != 2 or table.dtype != torch.int32 or (table.stride(1) != 1 and table.shape[1] > 1) or table.get_device() != gpu:
+        raise RuntimeError(f"{name}: table must be int32 [batch, pages of a sequence] with a contiguous last dim, on the pool's GPU")
+    b, w = table.shape
+    for what, x in (("lens", lens), ("new", new)):
+        if x.shape != (b,) or x.dtype != torch.int32 or not x.is_contiguous() or x.get_device() != gpu:
+            raise RuntimeError(f"{name}: {what} must be contiguous int32 [{b}] on the pool's GPU")
+    if done is not None and (done.shape != (b,) or done.dtype not in (torch.bool, torch.uint8) or not done.is_contiguous() or done.get_device() != gpu):
+        raise RuntimeError(f"{name}: done must be contiguous bool [{b}] on the pool's GPU")
+    rows = int(rows)
+    if rows < 0:
+        raise ValueError(f"{name}: {rows} rows")
+    dev = table.device
+    cu = torch.empty(b + 1, dtype=torch.int32, device=dev)
+    positions = torch.empty(rows, dtype=torch.int32, device=dev)
+    slots = torch.empty(rows, dtype=torch.int64, device=dev)
+    with _on(gpu):
+        n = 12 * (b + 1)
+        ws = torch.empty(n, dtype=torch.uint8, device=dev)
+        nat.call("rh3_kv_extend", *pool._args, table.data_ptr(), _st(table, 0), w, lens.data_ptr(), new.data_ptr(), nat.ptr(done), b,
+                 cu.data_ptr(), positions.data_ptr() if rows else None, slots.data_ptr() if rows else None, rows, ws.data_ptr(), n, _stream(gpu))
+    return cu, positions, slots
+
+
 def _seqs(name, cache, table, lens, cu, gpu):
     """The sequences' arguments of a call after its rows: table, its stride and width, lens, cu, batch."""
     if table.ndim != 2 or table.dtype != torch.int32 or (table.stride(1) != 1 and table.shape[1] > 1):
