@@ -206,7 +206,7 @@ Plan plan_of(int fmt, int64_t rows, int64_t batch, bool even, int64_t group, int
   Plan p{};
   p.chunk = form != RH3_KV_BY_SIZE ? form == RH3_KV_CHUNK : static_cast<double>((mean + small - 1) / small) * mb / 6.8 > 34.0 + static_cast<double>((mean + 127) / 128) * mb / 3.0;
   p.rows = !p.chunk ? small : mean <= 128 ? 128 : 256;
-  p.wgs = static_cast<int>(p.rows == 256 ? cus : 2 * cus);
+  p.wgs = static_cast<int>(p.rows == 256 ? cus : fmt == FP4 && !p.chunk ? 3 * cus : 2 * cus);
   p.items = !keep ? 0 : heads * (even ? batch * ((rows / batch * group + p.rows - 1) / p.rows) : rows * group / p.rows + batch);
   p.slots = 2 * static_cast<int64_t>(p.wgs) + p.items;
   return p;

@@ -22,7 +22,6 @@ namespace {
 
 constexpr int KT = CHUNK_KEYS;
 constexpr float SUM_STALE = 0x1p-12f;        // up to this sum of a half's probabilities none of them is over 2^STALE
-constexpr float NO_REF = -0x1.fffffep127f;   // reference of a row that has seen no key: any score moves it
 
 // 16-byte pieces of the LDS rows. Each row has one piece more than it needs, so that 16 rows' pieces of one number lie in all 16
 // parts of the banks, and every read of a tile is one lane address with an immediate offset.

@@ -70,6 +70,7 @@ __device__ __forceinline__ void query8(const uint4 raw, b8_t& hi, b8_t& lo) {
 // reference is then the maximum itself, or the next number.)
 constexpr float OVER = 24.0f;
 constexpr float STALE = -12.0f;
+constexpr float NO_REF = -0x1.fffffep127f;   // reference of a row that has seen no key: any score moves it
 __device__ __forceinline__ float reference_over(float top) { return top + OVER; }
 // parts are kept against a reference 2^24 lower (their sums times PART, as the join takes them)
 constexpr float PART_UP = 0x1p24f;

@@ -14,24 +14,27 @@ namespace rh3 {
 namespace kv {
 namespace {
 
-constexpr int WAVES = 8, NT = WAVES * 64, R = 16;
+constexpr int WAVES = 4, NT = WAVES * 64, R = 16;
 
 template <int D>
 struct Tile {
   uint32_t k[2][D / 32];      // of key l % 16 of each half
   uint32_t ks[2];             // its scale byte
-  uint32_t v[8];              // dim / 16 codes of keys 4 (l / 16) + 0 .. 3 of each half
+  uint2 v[2][D / 64];         // 16 codes of one of keys 4 (l / 16) + 0 .. 3, at 128 of one of the first two and of the others (values())
   uint32_t vs[2][D / 32];     // scale bytes of 4 keys
 };
 
-// the two pages of a 32-key tile (two 16-key halves), -1 where absent
+// The page of a 32-key tile, -1 where absent; with pages of 16 (SMALL) the two of its 16-key halves
+template <bool SMALL>
 struct Pages {
-  int p[2];
+  int p[SMALL ? 2 : 1];
+  __device__ __forceinline__ int of(int half) const { return p[SMALL ? half : 0]; }
 };
-__device__ __forceinline__ Pages pages_of(const AttnArgs& a, const int32_t* row, int width, int tile) {
-  Pages r;
+template <bool SMALL>
+__device__ __forceinline__ Pages<SMALL> pages_of(const AttnArgs& a, const int32_t* row, int width, int tile) {
+  Pages<SMALL> r;
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
+  for (int h = 0; h < (SMALL ? 2 : 1); ++h) {
     const int i = min((tile * TOKEN_KEYS + 16 * h) >> a.c.log2page, width - 1);
     const int p = scalar_load(row + i);
     r.p[h] = p >= 0 && p < a.c.pages ? p : -1;
@@ -39,65 +42,110 @@ __device__ __forceinline__ Pages pages_of(const AttnArgs& a, const int32_t* row,
   return r;
 }
 
-template <int D>
-__device__ __forceinline__ void load_keys(const AttnArgs& a, int kvh, int tile, const Pages& pg, Tile<D>& t) {
-  const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
-  const uint8_t* scales = reinterpret_cast<const uint8_t*>(a.c.ks);
+// A tile's loads: scalar bases (a buffer's, which takes them without vector arithmetic), and offsets that the lane keeps. head: the
+// K/V head's codes and scales of keys and of values in page 0.
+template <int D, bool SMALL>
+struct Bases {
+  __amdgpu_buffer_rsrc_t codes[SMALL ? 2 : 1], scales[SMALL ? 2 : 1];
+};
+template <int D, bool SMALL>
+__device__ __forceinline__ Bases<D, SMALL> bases_of(const AttnArgs& a, const uint8_t* codes, const uint8_t* scales, int tile, const Pages<SMALL>& pg) {
+  auto buffer = [](const uint8_t* p) { return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(p), 0, 0x7fffffff, BUF_RSRC_WORD3); };
+  const int off = (tile * TOKEN_KEYS) & ((1 << a.c.log2page) - 1);
+  Bases<D, SMALL> b;
+#pragma unroll
+  for (int h = 0; h < (SMALL ? 2 : 1); ++h) {
+    const int64_t p = max(pg.p[h], 0);
+    b.codes[h] = buffer(codes + (p * a.c.page_stride + off * (D / 2)));
+    b.scales[h] = buffer(scales + (p * a.c.spage_stride + off * (D / 32)));
+  }
+  return b;
+}
+template <int D, bool SMALL>
+__device__ __forceinline__ void load_keys(const AttnArgs& a, const uint8_t* const (&head)[4], int tile, const Pages<SMALL>& pg, Tile<D>& t) {
+  const uint32_t lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
+  const Bases<D, SMALL> b = bases_of<D, SMALL>(a, head[0], head[1], tile, pg);
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    const int64_t p = max(pg.p[h], 0);
-    const int off = (tile * TOKEN_KEYS + 16 * h) & ((1 << a.c.log2page) - 1);
-    const uint8_t* kb = a.c.k + p * a.c.page_stride + kvh * a.c.head_stride + off * (D / 2) + l16 * (D / 2) + g * (D / 8);
+    const int w = SMALL ? h : 0, key = SMALL ? 0 : 16 * h;
+    const uint32_t codes = l16 * (D / 2) + g * (D / 8) + key * (D / 2);
     if constexpr (D == 128) {
-      const uint4 w = *reinterpret_cast<const uint4*>(kb);
-      t.k[h][0] = w.x; t.k[h][1] = w.y; t.k[h][2] = w.z; t.k[h][3] = w.w;
+      const u32x4_t x = __builtin_amdgcn_raw_buffer_load_b128(b.codes[w], codes, 0, 0);
+      t.k[h][0] = x[0]; t.k[h][1] = x[1]; t.k[h][2] = x[2]; t.k[h][3] = x[3];
     } else {
-      const uint2 w = *reinterpret_cast<const uint2*>(kb);
-      t.k[h][0] = w.x; t.k[h][1] = w.y;
+      const u32x2_t x = __builtin_amdgcn_raw_buffer_load_b64(b.codes[w], codes, 0, 0);
+      t.k[h][0] = x[0]; t.k[h][1] = x[1];
     }
-    t.ks[h] = scales[p * a.c.spage_stride + kvh * a.c.shead_stride + off * (D / 32) + l16 * (D / 32) + (g * D / 4) / GROUP4];
+    t.ks[h] = __builtin_amdgcn_raw_buffer_load_b8(b.scales[w], l16 * (D / 32) + (g * D / 4) / GROUP4 + key * (D / 32), 0, 0);
   }
 }
-template <int D>
-__device__ __forceinline__ void load_values(const AttnArgs& a, int kvh, int tile, const Pages& pg, Tile<D>& t) {
-  const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
-  const uint8_t* scales = reinterpret_cast<const uint8_t*>(a.c.vs);
+template <int D, bool SMALL>
+__device__ __forceinline__ void load_values(const AttnArgs& a, const uint8_t* const (&head)[4], int tile, const Pages<SMALL>& pg, Tile<D>& t) {
+  const uint32_t lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
+  const Bases<D, SMALL> b = bases_of<D, SMALL>(a, head[2], head[3], tile, pg);
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    const int64_t p = max(pg.p[h], 0);
-    const int off = (tile * TOKEN_KEYS + 16 * h) & ((1 << a.c.log2page) - 1);
-    const uint8_t* vb = a.c.v + p * a.c.page_stride + kvh * a.c.head_stride + off * (D / 2) + 4 * g * (D / 2) + l16 * (D / 32);
-    const uint8_t* sb = scales + p * a.c.spage_stride + kvh * a.c.shead_stride + off * (D / 32) + 4 * g * (D / 32);
+    const int w = SMALL ? h : 0, key = SMALL ? 0 : 16 * h;
+    const uint32_t scales = 4 * g * (D / 32) + key * (D / 32);
     if constexpr (D == 128) {
-      const uint4 s = *reinterpret_cast<const uint4*>(sb);
-      t.vs[h][0] = s.x; t.vs[h][1] = s.y; t.vs[h][2] = s.z; t.vs[h][3] = s.w;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) t.v[4 * h + j] = *reinterpret_cast<const uint32_t*>(vb + j * (D / 2));
+      const u32x4_t x = __builtin_amdgcn_raw_buffer_load_b128(b.scales[w], scales, 0, 0);
+      t.vs[h][0] = x[0]; t.vs[h][1] = x[1]; t.vs[h][2] = x[2]; t.vs[h][3] = x[3];
     } else {
-      const uint2 s = *reinterpret_cast<const uint2*>(sb);
-      t.vs[h][0] = s.x; t.vs[h][1] = s.y;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) t.v[4 * h + j] = *reinterpret_cast<const uint16_t*>(vb + j * (D / 2));
+      const u32x2_t x = __builtin_amdgcn_raw_buffer_load_b64(b.scales[w], scales, 0, 0);
+      t.vs[h][0] = x[0]; t.vs[h][1] = x[1];
     }
+#pragma unroll
+    for (int i = 0; i < D / 64; ++i) {
+      const u32x2_t x = __builtin_amdgcn_raw_buffer_load_b64(b.codes[w], 128 * (D / 64) * g + 8 * l16 + (128 * i + key * (D / 2)), 0, 0);
+      t.v[h][i] = make_uint2(x[0], x[1]);
+    }
+  }
+}
+
+// The loads of values are whole lines of 128 bytes to 16 lanes: a load brings a lane 16 channels of one key, and lanes 8 apart (at 64
+// also 4 apart) exchange what the other one's channels are. A lane then has, of each of its 4 keys, the dim / 16 channels that begin
+// at channel_of(l % 16).
+template <int D>
+RH3_HD int channel_of(int m) { return D == 128 ? 16 * (m & 7) + 8 * (m >> 3) : 16 * (m & 3) + 8 * (m >> 3) + 4 * ((m >> 2) & 1); }
+template <int CTRL>
+__device__ __forceinline__ uint32_t moved(uint32_t v) {
+  return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, 0xf, 0xf, true));
+}
+// codes of 4 keys: 128: a word each; 64: a half word each, in two words
+template <int D>
+__device__ __forceinline__ void exchange(const uint2 (&v)[D / 64], uint32_t (&w)[D / 32]) {
+  const uint32_t lane = threadIdx.x & 63;
+  const bool up = lane & 8;
+#pragma unroll
+  for (int i = 0; i < D / 64; ++i) {
+    const uint32_t got = moved<0x128>(up ? v[i].x : v[i].y);   // row_ror:8: from lane ^ 8
+    w[2 * i] = up ? got : v[i].x;
+    w[2 * i + 1] = up ? v[i].y : got;
+  }
+  if constexpr (D == 64) {
+    const uint32_t sel = lane & 4 ? 0x03020706u : 0x05040100u;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) w[i] = __builtin_amdgcn_perm(moved<0x1B>(moved<0x141>(w[i])), w[i], sel);   // from lane ^ 4
   }
 }
 
 // one wave's running state for 16 query rows (row l % 16)
 template <int D>
 struct State {
-  f4_t o[D / 16];   // o[i][r]: channel (D / 16) (4 (l / 16) + r) + i
+  f4_t o[D / 16];   // o[i][r]: channel channel_of(4 (l / 16) + r) + i
   float ref, sum;
 };
 
-// One tile. FINE: fp16 queries, in two terms. MORE: the wave's next tile (pages `pn`) is loaded into the same registers, its keys as
-// soon as these are used, its values at the end.
-template <int D, bool FINE, bool MORE>
-__device__ __forceinline__ void compute(const AttnArgs& a, Tile<D>& t, int kvh, int tile, const Pages& pg, const Pages& pn,
-                                        const b8_t (&q)[D / 32], const b8_t (&ql)[D / 32], int lim, int low, int len, State<D>& st) {
+// One tile. FINE: fp16 queries, in two terms. The wave's next tile (nt, pages pn) is loaded into the same registers, its keys as soon
+// as these are used, its values as soon as theirs are. (The last turn loads its own tile again: loads that are only sometimes there
+// would be waited for at once.)
+template <int D, bool FINE, bool SMALL>
+__device__ __forceinline__ void compute(const AttnArgs& a, Tile<D>& t, int tile, const Pages<SMALL>& pg, const b8_t (&q)[D / 32],
+                                        const b8_t (&ql)[D / 32], int lim, int low, int len, const uint8_t* const (&head)[4], int nt, const Pages<SMALL>& pn, State<D>& st) {
   const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
   const int kb = tile * TOKEN_KEYS;
   // low: keys that every row sees
-  const bool edge = kb + TOKEN_KEYS > low || pg.p[0] < 0 || pg.p[1] < 0;
+  const bool edge = kb + TOKEN_KEYS > low || pg.of(0) < 0 || pg.of(1) < 0;
   f4_t acc[2];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
@@ -110,36 +158,41 @@ __device__ __forceinline__ void compute(const AttnArgs& a, Tile<D>& t, int kvh, 
       if constexpr (FINE) acc[h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, ql[c], acc[h], 0, 0, 0);
     }
   }
-  if constexpr (MORE) load_keys<D>(a, kvh, tile + WAVES, pn, t);
+  load_keys<D, SMALL>(a, head, nt, pn, t);
   auto key = [&](int j) { return kb + 16 * (j >> 2) + 4 * g + (j & 3); };
-  float x[8], top = -INFINITY;
+  auto hidden = [&](int j, int end) { return key(j) >= end || pg.of(j >> 2) < 0; };
+  // scores less the reference, which is finite: before a row's first key it is the lowest number
+  float y[8];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) x[j] = acc[j >> 2][j & 3] * a.scale_log2;
+  for (int j = 0; j < 8; ++j) y[j] = fmaf(acc[j >> 2][j & 3], a.scale_log2, -st.ref);
   if (edge) {
 #pragma unroll
+    for (int j = 0; j < 8; ++j) y[j] = hidden(j, lim) ? -INFINITY : y[j];
+  }
+  float top = y[0];
+#pragma unroll
+  for (int j = 1; j < 8; ++j) top = fmaxf(top, y[j]);
+  if (__builtin_amdgcn_ballot_w64(top > STALE)) {
+    float n = -INFINITY;
+#pragma unroll
     for (int j = 0; j < 8; ++j) {
-      x[j] = key(j) >= lim || pg.p[j >> 2] < 0 ? -INFINITY : x[j];
+      y[j] = edge && hidden(j, lim) ? -INFINITY : acc[j >> 2][j & 3] * a.scale_log2;
+      n = fmaxf(n, y[j]);
     }
-  }
+    n = across_max<true>(n);
+    const float to = n - st.ref > STALE ? reference_over(n) : st.ref;
+    const float f = __builtin_amdgcn_exp2f(st.ref - to);
+    st.ref = to;
+    st.sum *= f;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) top = fmaxf(top, x[j]);
-  if (__builtin_amdgcn_ballot_w64(top - st.ref > STALE)) {
-    const float n = across_max<true>(top);
-    if (n - st.ref > STALE) {
-      const float to = reference_over(n);
-      const float f = __builtin_amdgcn_exp2f(st.ref - to);   // from no keys yet: 2^-inf = 0
-      st.ref = to;
-      st.sum *= f;
+    for (int i = 0; i < D / 16; ++i) st.o[i] *= f;
 #pragma unroll
-      for (int i = 0; i < D / 16; ++i) st.o[i] *= f;
-    }
+    for (int j = 0; j < 8; ++j) y[j] -= to;
   }
-  // a row that has seen no key yet has only -inf here: any finite reference gives it zeros
-  const float ref = st.ref == -INFINITY ? 0.0f : st.ref;
   uint32_t hi[4], lo[4];
 #pragma unroll
   for (int j = 0; j < 8; j += 2) {
-    const float e0 = __builtin_amdgcn_exp2f(x[j] - ref), e1 = __builtin_amdgcn_exp2f(x[j + 1] - ref);
+    const float e0 = __builtin_amdgcn_exp2f(y[j]), e1 = __builtin_amdgcn_exp2f(y[j + 1]);
     st.sum += e0 + e1;
     hi[j / 2] = pack_bf2(e0, e1);
     lo[j / 2] = pack_bf2(e0 - __uint_as_float(hi[j / 2] << 16), e1 - __uint_as_float(hi[j / 2] & 0xffff0000u));
@@ -147,7 +200,7 @@ __device__ __forceinline__ void compute(const AttnArgs& a, Tile<D>& t, int kvh, 
   const b8_t p = bf16x8(hi[0], hi[1], hi[2], hi[3]), rest = bf16x8(lo[0], lo[1], lo[2], lo[3]);
 
   // the scale byte of the lane's group to where a float's exponent is; what lies beside it is not looked at
-  const int group = (l16 * (D / 16)) / GROUP4;
+  const int group = channel_of<D>(l16) / GROUP4;
   float s[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
@@ -155,11 +208,15 @@ __device__ __forceinline__ void compute(const AttnArgs& a, Tile<D>& t, int kvh, 
     const int byte = D == 128 ? group : 2 * (j & 1) + group;
     s[j] = __uint_as_float(__builtin_amdgcn_alignbit(w, w, (8 * byte + 9) & 31));
   }
+  uint32_t v[2][D / 32];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) exchange<D>(t.v[h], v[h]);
   if (edge) {   // what lies behind the sequence or in an absent page may be anything
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      if (key(j) >= len || pg.p[j >> 2] < 0) {
-        t.v[j] = 0;
+      if (hidden(j, len)) {
+        if constexpr (D == 128) v[j >> 2][j & 3] = 0;
+        else v[j >> 2][(j & 3) >> 1] &= j & 1 ? 0x0000ffffu : 0xffff0000u;
         s[j] = 1.0f;
       }
     }
@@ -168,47 +225,103 @@ __device__ __forceinline__ void compute(const AttnArgs& a, Tile<D>& t, int kvh, 
     constexpr int c = decltype(C)::value;
     uint32_t w[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) w[j] = pair4<c>(t.v[j], s[j]);
+    for (int j = 0; j < 8; ++j) {
+      if constexpr (D == 128) w[j] = pair4<c>(v[j >> 2][j & 3], s[j]);
+      else w[j] = j & 1 ? pair4<(c + 2) & 3>(v[j >> 2][(j & 3) >> 1], s[j]) : pair4<c>(v[j >> 2][(j & 3) >> 1], s[j]);
+    }
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       const uint32_t sel = e ? 0x07060302u : 0x05040100u;
-      const b8_t v = bf16x8(__builtin_amdgcn_perm(w[1], w[0], sel), __builtin_amdgcn_perm(w[3], w[2], sel),
+      const b8_t x = bf16x8(__builtin_amdgcn_perm(w[1], w[0], sel), __builtin_amdgcn_perm(w[3], w[2], sel),
                             __builtin_amdgcn_perm(w[5], w[4], sel), __builtin_amdgcn_perm(w[7], w[6], sel));
-      st.o[2 * c + e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, p, st.o[2 * c + e], 0, 0, 0);
-      st.o[2 * c + e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, rest, st.o[2 * c + e], 0, 0, 0);
+      st.o[2 * c + e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, p, st.o[2 * c + e], 0, 0, 0);
+      st.o[2 * c + e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, rest, st.o[2 * c + e], 0, 0, 0);
     }
   };
+  load_values<D, SMALL>(a, head, nt, pn, t);
   channels(std::integral_constant<int, 0>());
   channels(std::integral_constant<int, 1>());
   if constexpr (D == 128) {
     channels(std::integral_constant<int, 2>());
     channels(std::integral_constant<int, 3>());
   }
-  if constexpr (MORE) load_values<D>(a, kvh, tile + WAVES, pn, t);
 }
 
-template <int D, bool FINE>
-__global__ void __launch_bounds__(NT, 4) token_kernel(AttnArgs a) {
+// The block of 64 sequences at hand (kv_attn.hpp), kept in LDS: in registers it would take what the loop's loads need
+struct SharedList {
+  int first[64], n[64], len[64], pos[64], row_tiles[64], span[64];
+  int64_t units[64], items[64];
+};
+struct Listed {
+  int at;
+  int64_t base, items_base, end;
+  __device__ __forceinline__ void put(const Block& b, SharedList& s) {
+    const int lane = threadIdx.x & 63;
+    at = b.at;
+    base = scalar(b.base);
+    items_base = scalar(b.items_base);
+    end = b.end();
+    __syncthreads();
+    if (threadIdx.x < 64) {
+      s.first[lane] = b.seq.first;
+      s.n[lane] = b.seq.n;
+      s.len[lane] = b.seq.len;
+      s.pos[lane] = b.seq.pos;
+      s.row_tiles[lane] = b.row_tiles;
+      s.span[lane] = b.span;
+      s.units[lane] = b.units;
+      s.items[lane] = b.items;
+    }
+    __syncthreads();
+  }
+  __device__ __forceinline__ Work begin(const AttnArgs& a, const Tiling& g, SharedList& s) {
+    Block b;
+    const Work w = dealt(load_blocks(a, g, b), a.wgs, g);
+    put(b, s);
+    return w;
+  }
+  __device__ __forceinline__ void next(const AttnArgs& a, const Tiling& g, SharedList& s) {
+    Block b;
+    load_block(a, g, at + 64, end, items_base + scalar(s.items[63]), b);
+    put(b, s);
+  }
+  __device__ __forceinline__ int lane_of(const SharedList& s, int64_t u) const {
+    return __builtin_ctzll(__builtin_amdgcn_ballot_w64(base + s.units[threadIdx.x & 63] > u));
+  }
+  __device__ __forceinline__ SeqItems sequence(const SharedList& s, int l) const {
+    SeqItems r;
+    r.seq = Seq{scalar(s.first[l]), scalar(s.n[l]), scalar(s.len[l]), scalar(s.pos[l])};
+    r.row_tiles = scalar(s.row_tiles[l]);
+    r.span = scalar(s.span[l]);
+    r.before = base + (l ? scalar(s.units[l - 1]) : 0);
+    r.items_before = items_base + (l ? scalar(s.items[l - 1]) : 0);
+    return r;
+  }
+};
+
+template <int D, bool FINE, bool SMALL>
+__global__ void __launch_bounds__(NT, 3) token_kernel(AttnArgs a) {
   constexpr int PAD = D + 4;
   const Tiling TILING = tiling(false, R);
   __shared__ float so[WAVES][R][PAD];
   __shared__ float sm[WAVES][R], sl[WAVES][R];
+  __shared__ SharedList shared_list;
   const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  Block blk;
-  const Work work = dealt(load_blocks(a, TILING, blk), a.wgs, TILING);
+  Listed list;
+  const Work work = list.begin(a, TILING, shared_list);
   const int wg = blockIdx.x;
   if (wg >= work.wgs) return;
   int64_t u = scalar(share_begin(work, wg));
   const int64_t end = scalar(share_begin(work, wg + 1));
 
   while (u < end) {
-    while (u >= blk.end()) {
-      if (blk.at + 64 >= sequences(a)) return;
-      next_block(a, TILING, blk);
+    while (u >= list.end) {
+      if (list.at + 64 >= sequences(a)) return;
+      list.next(a, TILING, shared_list);
     }
-    const int l = __builtin_ctzll(__builtin_amdgcn_ballot_w64(blk.base + blk.units > u));
-    const SeqItems sw = seq_in(a, blk, l);
+    const int l = list.lane_of(shared_list, u);
+    const SeqItems sw = list.sequence(shared_list, l);
     const Seq sq = sw.seq;
     const int64_t local = u - sw.before;
     const int item = scalar(static_cast<int>(quotient(local, sw.span)));
@@ -217,15 +330,15 @@ __global__ void __launch_bounds__(NT, 4) token_kernel(AttnArgs a) {
     u += u1 - u0;
     const int t0 = max(u0 - TILING.extra, 0), t1 = u1 - TILING.extra;
     if (t1 <= 0) continue;
-    const bool pre = a.prefix && blk.at + l == 0, causal = a.causal && !pre;
-    const int32_t* row = pre ? a.prefix : a.s.table + (blk.at + l - (a.prefix != nullptr)) * a.s.table_stride;
+    const bool pre = a.prefix && list.at + l == 0, causal = a.causal && !pre;
+    const int32_t* row = pre ? a.prefix : a.s.table + (list.at + l - (a.prefix != nullptr)) * a.s.table_stride;
     const int width = pre ? a.prefix_width : a.s.width;
     const int kvh = scalar(item / sw.row_tiles), rt = item - kvh * sw.row_tiles;
     const int rows = sq.n * a.group;
 
     // query rows: lane l holds row l % 16, channels (dim / 4) (l / 16) + 8 c + 0 .. 7 in step c
     int t = t0 + wave;
-    Pages pg = pages_of(a, row, width, t), pn = pages_of(a, row, width, t + WAVES);
+    Pages<SMALL> pg = pages_of<SMALL>(a, row, width, t), pn = pages_of<SMALL>(a, row, width, t + WAVES);
     const int mine = rt * R + l16, rr = mine < rows ? mine : 0;
     const int tok = rr / a.group, hd = kvh * a.group + rr - tok * a.group;
     uint4 raw[D / 32];
@@ -235,9 +348,12 @@ __global__ void __launch_bounds__(NT, 4) token_kernel(AttnArgs a) {
     const int lim = causal ? min(sq.len, sq.pos + tok + 1) : sq.len;
     // the first keys and values are on their way while the query rows come in
     Tile<D> tile;
+    const int64_t codes = kvh * a.c.head_stride, scales = kvh * a.c.shead_stride;
+    const uint8_t* const head[4] = {a.c.k + codes, reinterpret_cast<const uint8_t*>(a.c.ks) + scales, a.c.v + codes,
+                                    reinterpret_cast<const uint8_t*>(a.c.vs) + scales};
     if (t < t1) {
-      load_keys<D>(a, kvh, t, pg, tile);
-      load_values<D>(a, kvh, t, pg, tile);
+      load_keys<D, SMALL>(a, head, t, pg, tile);
+      load_values<D, SMALL>(a, head, t, pg, tile);
     }
     b8_t q[D / 32], ql[D / 32];
 #pragma unroll
@@ -245,18 +361,17 @@ __global__ void __launch_bounds__(NT, 4) token_kernel(AttnArgs a) {
     const int low = causal ? min(sq.len, sq.pos + scalar((rt * R) / a.group) + 1) : sq.len;
 
     State<D> st;
-    st.ref = -INFINITY;
+    st.ref = NO_REF;
     st.sum = 0.0f;
 #pragma unroll
     for (int i = 0; i < D / 16; ++i) st.o[i] = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
-    if (t < t1) {
-      for (; t + WAVES < t1; t += WAVES) {
-        const Pages p2 = pages_of(a, row, width, t + 2 * WAVES);
-        compute<D, FINE, true>(a, tile, kvh, t, pg, pn, q, ql, lim, low, sq.len, st);
-        pg = pn;
-        pn = p2;
-      }
-      compute<D, FINE, false>(a, tile, kvh, t, pg, pn, q, ql, lim, low, sq.len, st);
+    while (t < t1) {
+      const Pages<SMALL> p2 = pages_of<SMALL>(a, row, width, t + 2 * WAVES);
+      const bool more = t + WAVES < t1;
+      compute<D, FINE, SMALL>(a, tile, t, pg, q, ql, lim, low, sq.len, head, more ? t + WAVES : t, more ? pn : pg, st);
+      pg = pn;
+      pn = p2;
+      t += WAVES;
     }
     // join the waves
     const float mysum = across_sum<true>(st.sum);
@@ -268,7 +383,7 @@ __global__ void __launch_bounds__(NT, 4) token_kernel(AttnArgs a) {
     for (int r = 0; r < 4; ++r)
 #pragma unroll
       for (int i = 0; i < D / 16; i += 4)
-        *reinterpret_cast<float4*>(&so[wave][l16][(D / 16) * (4 * g + r) + i]) = make_float4(st.o[i][r], st.o[i + 1][r], st.o[i + 2][r], st.o[i + 3][r]);
+        *reinterpret_cast<float4*>(&so[wave][l16][channel_of<D>(4 * g + r) + i]) = make_float4(st.o[i][r], st.o[i + 1][r], st.o[i + 2][r], st.o[i + 3][r]);
     __syncthreads();
     const bool whole = t0 == 0 && u1 == sw.span;
     constexpr int TPR = NT / R, EPT = D / TPR;   // threads to a row, channels to a thread
@@ -281,8 +396,7 @@ __global__ void __launch_bounds__(NT, 4) token_kernel(AttnArgs a) {
       float sum = 0.0f, o[EPT] = {};
 #pragma unroll
       for (int w = 0; w < WAVES; ++w) {
-        // (a wave that has seen nothing but NaN has its sums under no reference)
-        const float f = sm[w][rl] == -INFINITY ? (sl[w][rl] == 0.0f ? 0.0f : sl[w][rl]) : __builtin_amdgcn_exp2f(sm[w][rl] - top);
+        const float f = __builtin_amdgcn_exp2f(sm[w][rl] - top);
         sum += f * sl[w][rl];
 #pragma unroll
         for (int e = 0; e < EPT; ++e) o[e] += f * so[w][rl][d0 + e];
@@ -291,11 +405,11 @@ __global__ void __launch_bounds__(NT, 4) token_kernel(AttnArgs a) {
         const int tok = rw / a.group, hd = kvh * a.group + rw - tok * a.group;
         const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
         uint16_t* dst = static_cast<uint16_t*>(a.out) + (sq.first + tok) * a.o_st + hd * a.o_sh + d0;
-        if constexpr (EPT == 4) {
-          *reinterpret_cast<uint2*>(dst) = make_uint2(pack_out(a, o[0] * inv, o[1] * inv), pack_out(a, o[2] * inv, o[3] * inv));
-        } else {
-          *reinterpret_cast<uint32_t*>(dst) = pack_out(a, o[0] * inv, o[1] * inv);
-        }
+        uint32_t w[EPT / 2];
+#pragma unroll
+        for (int e = 0; e < EPT; e += 2) w[e / 2] = pack_out(a, o[e] * inv, o[e + 1] * inv);
+#pragma unroll
+        for (int e = 0; e < EPT / 2; e += 2) *reinterpret_cast<uint2*>(dst + 2 * e) = make_uint2(w[e], w[e + 1]);
         if (a.lse && d0 == 0)
           a.lse[static_cast<int64_t>(sq.first + tok) * a.c.heads * a.group + hd] =
               sum == 0.0f ? -INFINITY : (__builtin_amdgcn_logf(sum) + top) * 0.6931471805599453f;
@@ -304,8 +418,9 @@ __global__ void __launch_bounds__(NT, 4) token_kernel(AttnArgs a) {
         const int64_t slot = whole ? 2 * static_cast<int64_t>(a.wgs) + sw.items_before + item : 2 * static_cast<int64_t>(wg) + (t0 == 0);
         float* po = a.part_o + (slot * R + rl) * D + d0;
 #pragma unroll
-        for (int e = 0; e < EPT; ++e) po[e] = o[e] * (PART * PART_UP);
-        if (d0 == 0) *reinterpret_cast<float2*>(a.part_ml + (slot * R + rl) * 2) = make_float2(sum == sum ? top - OVER : 0.0f, sum * PART_UP);
+        for (int e = 0; e < EPT; e += 4)
+          *reinterpret_cast<float4*>(po + e) = make_float4(o[e] * (PART * PART_UP), o[e + 1] * (PART * PART_UP), o[e + 2] * (PART * PART_UP), o[e + 3] * (PART * PART_UP));
+        if (d0 == 0) *reinterpret_cast<float2*>(a.part_ml + (slot * R + rl) * 2) = make_float2(sum == 0.0f ? -INFINITY : sum == sum ? top - OVER : 0.0f, sum * PART_UP);
       }
     }
     if (u < end) __syncthreads();
@@ -316,8 +431,9 @@ __global__ void __launch_bounds__(NT, 4) token_kernel(AttnArgs a) {
 
 void launch_token4(const AttnArgs& a, int dim, hipStream_t st) {
   auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(a.wgs)), dim3(NT), 0, st, a); };
-  if (dim == 128) a.fp16 ? go(token_kernel<128, true>) : go(token_kernel<128, false>);
-  else a.fp16 ? go(token_kernel<64, true>) : go(token_kernel<64, false>);
+  auto by = [&](auto small, auto large) { a.c.log2page == 4 ? go(small) : go(large); };
+  if (dim == 128) a.fp16 ? by(token_kernel<128, true, true>, token_kernel<128, true, false>) : by(token_kernel<128, false, true>, token_kernel<128, false, false>);
+  else a.fp16 ? by(token_kernel<64, true, true>, token_kernel<64, true, false>) : by(token_kernel<64, false, true>, token_kernel<64, false, false>);
 }
 
 }  // namespace kv
