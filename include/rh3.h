@@ -497,9 +497,24 @@ typedef struct rh3_kv_cache {
  * page size + offset; slots -1 where it has no place, both -1 behind cu[batch]. Negative lens and more count as 0; a length is at most
  * 2^30. batch * width at most 2^30. Everything is device memory; nothing is read back. The workspace holds sums for a call. */
 int64_t rh3_kv_extend_workspace_bytes(int64_t batch);
-int rh3_kv_extend(int32_t* free_pages, int64_t pages, int32_t* state, int64_t page, int32_t* table, int64_t table_stride,
-                  int64_t width, int32_t* lens, const int32_t* more, const uint8_t* done, int64_t batch, int32_t* cu,
-                  int32_t* positions, int64_t* slots, int64_t rows, void* workspace, int64_t workspace_bytes, hipStream_t stream);
+typedef struct rh3_kv_extend_args {
+  int32_t* free_pages;
+  int64_t pages;
+  int32_t* state;
+  int64_t page;
+  int32_t* table;
+  int64_t table_stride, width;
+  int32_t* lens;
+  const int32_t* more;
+  const uint8_t* done;
+  int64_t batch;
+  int32_t *cu, *positions;
+  int64_t* slots;
+  int64_t rows;
+  void* workspace;
+  int64_t workspace_bytes;
+} rh3_kv_extend_args;
+int rh3_kv_extend(const rh3_kv_extend_args* args, hipStream_t stream);
 
 /* Quantizes rows of k and v (bf16, fp16 or fp32) into their positions: s = max(amax / QMAX, 1e-12) (127 or 448), code =
  * round_half_even(x / s); a row with an infinity or a NaN gets s = NaN and codes 0. RH3_KV_FP4: e the least with amax <= 7 * 2^e of
@@ -521,20 +536,39 @@ int rh3_kv_read(const rh3_kv_cache* cache, void* k, int64_t k_st, int64_t k_sh, 
  * (dim 64 or 128; either may have 0 heads; strides as above): pairs (a, b) of channels i and i + rot / 2 (interleaved: 2 i and
  * 2 i + 1) become (a cos - b sin, b cos + a sin) of the angle positions[row] * freq[i] (freq [rot / 2], 64 bits, as the product is),
  * cosine and sine times factor; rounded to the rows' type once. The results may lie exactly over q and k. */
-int rh3_qk_norm_rope(const void* q, int64_t q_st, int64_t q_sh, void* q_out, int64_t qo_st, int64_t qo_sh, int64_t q_heads,
-                     const void* k, int64_t k_st, int64_t k_sh, void* k_out, int64_t ko_st, int64_t ko_sh, int64_t k_heads,
-                     int64_t rows, int64_t dim, int dtype, const int32_t* positions, const double* freq, int64_t rot,
-                     int interleaved, double factor, int norm, double eps, const void* qw, const void* kw, int wide_weights,
-                     hipStream_t stream);
+typedef struct rh3_head_rows {
+  void* x;               /* [rows][heads][dim] */
+  int64_t st, sh;
+} rh3_head_rows;
+typedef struct rh3_turn {
+  const double* freq;
+  int64_t rot, interleaved;
+  double factor;
+  int64_t norm;
+  double eps;
+  const void *qw, *kw;
+  int64_t wide_weights;
+} rh3_turn;
+typedef struct rh3_rope_args {
+  rh3_head_rows q, q_out, k, k_out;
+  int64_t q_heads, k_heads, rows, dim, dtype;
+  const int32_t* positions;
+  rh3_turn turn;
+} rh3_rope_args;
+int rh3_qk_norm_rope(const rh3_rope_args* args, hipStream_t stream);
 
 /* rh3_qk_norm_rope at the rows' positions in their sequences (plus first) and rh3_kv_write of its k (rounded to the rows' type) and of
  * v, in one pass. Rows that no sequence has are not touched; of rows whose position is nowhere in the cache only q is done. */
-int rh3_kv_write_rope(const rh3_kv_cache* cache, const void* q, int64_t q_st, int64_t q_sh, void* q_out, int64_t qo_st,
-                      int64_t qo_sh, int64_t q_heads, const void* k, int64_t k_st, int64_t k_sh, const void* v, int64_t v_st,
-                      int64_t v_sh, int dtype, int64_t rows, const int32_t* table, int64_t table_stride, int64_t width,
-                      const int32_t* lens, const int32_t* cu, int64_t batch, int64_t first, const double* freq, int64_t rot,
-                      int interleaved, double factor, int norm, double eps, const void* qw, const void* kw, int wide_weights,
-                      hipStream_t stream);
+typedef struct rh3_kv_rope_args {
+  rh3_head_rows q, q_out, k, v;
+  int64_t q_heads, dtype, rows;
+  const int32_t* table;
+  int64_t table_stride, width;
+  const int32_t *lens, *cu;
+  int64_t batch, first;
+  rh3_turn turn;
+} rh3_kv_rope_args;
+int rh3_kv_write_rope(const rh3_kv_cache* cache, const rh3_kv_rope_args* args, hipStream_t stream);
 
 /* out = softmax(scale q k^T) v over a sequence's cached positions (causal: row i of n sees positions up to
  * lens[b] - n + i), q and out [rows][q_heads][dim] bf16 or fp16, query head h reads K/V head h / (q_heads / heads); lse

@@ -238,40 +238,41 @@ using namespace rh3::kv;
 
 extern "C" int64_t rh3_kv_extend_workspace_bytes(int64_t batch) { return batch < 1 || batch > 65536 ? 0 : 3 * (batch + 1) * 4; }
 
-extern "C" int rh3_kv_extend(int32_t* free_pages, int64_t pages, int32_t* state, int64_t page, int32_t* table, int64_t table_stride,
-                             int64_t width, int32_t* lens, const int32_t* more, const uint8_t* done, int64_t batch, int32_t* cu,
-                             int32_t* positions, int64_t* slots, int64_t rows, void* workspace, int64_t workspace_bytes,
-                             hipStream_t stream) {
+extern "C" int rh3_kv_extend(const rh3_kv_extend_args* x, hipStream_t stream) {
   const char* name = "kv_extend";
   clear_error();
-  RH3_REQUIRE(pages >= 1 && pages <= INT32_MAX, "%s: %lld pages", name, static_cast<long long>(pages));
+  RH3_REQUIRE(x, "%s: null arguments", name);
+  const int64_t page = x->page, width = x->width, batch = x->batch, rows = x->rows;
+  RH3_REQUIRE(x->pages >= 1 && x->pages <= INT32_MAX, "%s: %lld pages", name, static_cast<long long>(x->pages));
   RH3_REQUIRE(page >= 16 && page <= 256 && (page & (page - 1)) == 0, "%s: page of %lld positions (16, 32, 64, 128 or 256)", name,
               static_cast<long long>(page));
   RH3_REQUIRE(rows >= 0 && rows <= MAX_ROWS, "%s: %lld rows", name, static_cast<long long>(rows));
+  if (rows == 0 && batch == 0) return RH3_OK;
   RH3_REQUIRE(batch >= 1 && batch <= 65536, "%s: %lld sequences (1 to 65536)", name, static_cast<long long>(batch));
   PagesArgs a{};
   a.log2page = __builtin_ctzll(static_cast<unsigned long long>(page));
-  RH3_REQUIRE(width >= 1 && width <= (MAX_ROWS >> a.log2page) && table_stride >= (batch > 1 ? width : 0) && batch * width <= MAX_ROWS,
-              "%s: page table of %lld entries per sequence, stride %lld", name, static_cast<long long>(width), static_cast<long long>(table_stride));
-  RH3_REQUIRE(free_pages && state && table && lens && more && cu, "%s: null pool, page table, lengths, new rows or offsets", name);
-  RH3_REQUIRE(rows == 0 || (positions && slots), "%s: null positions or slots", name);
-  RH3_REQUIRE(workspace && aligned16(workspace) && workspace_bytes >= rh3_kv_extend_workspace_bytes(batch),
+  RH3_REQUIRE(width >= 1 && width <= (MAX_ROWS >> a.log2page) && x->table_stride >= (batch > 1 ? width : 0) && batch * width <= MAX_ROWS,
+              "%s: page table of %lld entries per sequence, stride %lld", name, static_cast<long long>(width),
+              static_cast<long long>(x->table_stride));
+  RH3_REQUIRE(x->free_pages && x->state && x->table && x->lens && x->more && x->cu, "%s: null pool, page table, lengths, new rows or offsets", name);
+  RH3_REQUIRE(rows == 0 || (x->positions && x->slots), "%s: null positions or slots", name);
+  RH3_REQUIRE(x->workspace && aligned16(x->workspace) && x->workspace_bytes >= rh3_kv_extend_workspace_bytes(batch),
               "%s: workspace of %lld bytes needed, %lld given", name, static_cast<long long>(rh3_kv_extend_workspace_bytes(batch)),
-              static_cast<long long>(workspace_bytes));
-  a.free = free_pages;
-  a.state = state;
-  a.table = table;
-  a.table_stride = table_stride;
-  a.lens = lens;
-  a.more = more;
-  a.done = done;
-  a.cu = cu;
-  a.positions = positions;
-  a.slots = slots;
-  a.back = static_cast<int32_t*>(workspace);
+              static_cast<long long>(x->workspace_bytes));
+  a.free = x->free_pages;
+  a.state = x->state;
+  a.table = x->table;
+  a.table_stride = x->table_stride;
+  a.lens = x->lens;
+  a.more = x->more;
+  a.done = x->done;
+  a.cu = x->cu;
+  a.positions = x->positions;
+  a.slots = x->slots;
+  a.back = static_cast<int32_t*>(x->workspace);
   a.taken = a.back + batch + 1;
   a.start = a.taken + batch + 1;
-  a.pages = static_cast<int>(pages);
+  a.pages = static_cast<int>(x->pages);
   a.width = static_cast<int>(width);
   a.batch = static_cast<int>(batch);
   a.rows = static_cast<int>(rows);

@@ -30,18 +30,10 @@ struct Turn {
   double eps;
   const void *qw, *kw;               // [dim] or null
 };
-struct Rows {
-  const void* x;
-  int64_t st, sh;
-};
-struct Out {
-  void* x;
-  int64_t st, sh;
-};
 struct RopeArgs {
   Turn t;
-  Rows q, k, v;
-  Out qo, ko;                        // ko: FMT NONE
+  rh3_head_rows q, k, v;             // v: not of FMT NONE
+  rh3_head_rows qo, ko;              // ko: of FMT NONE
   int q_heads, k_heads, rows, log2tt;
   int first;                         // added to the positions of the cache's rows
   const int32_t* positions;          // FMT NONE
@@ -172,7 +164,7 @@ __global__ void __launch_bounds__(NT) rope_kernel(RopeArgs a) {
     const bool key = g >= q_groups;
     const int h = (key ? g - q_groups : g) * heads_at_once + hs;
     if (mine && g < q_groups + k_groups && h < (key ? a.k_heads : a.q_heads)) {
-      const Rows& r = key ? a.k : a.q;
+      const rh3_head_rows& r = key ? a.k : a.q;
       own = load_raw<DT>(r.x, row * r.st + h * r.sh + c0);
       other = load_raw<DT>(r.x, row * r.st + h * r.sh + p0);
     }
@@ -261,29 +253,36 @@ __global__ void __launch_bounds__(NT) rope_kernel(RopeArgs a) {
   }
 }
 
-int check_turn(const char* name, const Turn& t, int64_t rot, int64_t dim) {
+int check_turn(const char* name, const rh3_turn& x, int64_t dim, Turn& t) {
   RH3_REQUIRE(dim == 64 || dim == 128, "%s: head dim %lld (64 or 128)", name, static_cast<long long>(dim));
-  RH3_REQUIRE(rot >= 0 && rot <= dim && rot % 16 == 0, "%s: %lld rotated channels of %lld (a multiple of 16)", name, static_cast<long long>(rot),
-              static_cast<long long>(dim));
-  RH3_REQUIRE(rot == 0 || t.freq, "%s: no frequencies for %lld rotated channels", name, static_cast<long long>(rot));
-  RH3_REQUIRE(rot || t.norm, "%s: neither a norm nor a rotation", name);
-  RH3_REQUIRE(aligned16(t.qw) && aligned16(t.kw) && (reinterpret_cast<uintptr_t>(t.freq) & 7) == 0, "%s: weights must be 16-byte aligned, frequencies 8-byte", name);
+  RH3_REQUIRE(x.rot >= 0 && x.rot <= dim && x.rot % 16 == 0, "%s: %lld rotated channels of %lld (a multiple of 16)", name,
+              static_cast<long long>(x.rot), static_cast<long long>(dim));
+  RH3_REQUIRE(x.rot == 0 || x.freq, "%s: no frequencies for %lld rotated channels", name, static_cast<long long>(x.rot));
+  RH3_REQUIRE(x.rot || x.norm, "%s: neither a norm nor a rotation", name);
+  RH3_REQUIRE(aligned16(x.qw) && aligned16(x.kw) && (reinterpret_cast<uintptr_t>(x.freq) & 7) == 0,
+              "%s: weights must be 16-byte aligned, frequencies 8-byte", name);
+  t = Turn{x.freq, x.factor, static_cast<int>(x.rot), x.interleaved != 0, x.norm != 0, x.wide_weights != 0, x.eps, x.qw, x.kw};
   return RH3_OK;
 }
-int check_rows(const char* name, const char* what, const void* x, int64_t st, int64_t sh) {
-  RH3_REQUIRE(x, "%s: null %s", name, what);
-  RH3_REQUIRE(aligned16(x) && st % 8 == 0 && sh % 8 == 0, "%s: %s must be 16-byte aligned with strides that are multiples of 8", name, what);
+int check_type(const char* name, int64_t dtype) {
+  RH3_REQUIRE(dtype == RH3_DTYPE_BF16 || dtype == RH3_DTYPE_F16 || dtype == RH3_DTYPE_F32, "%s: row type %lld (bf16, fp16 or fp32)", name,
+              static_cast<long long>(dtype));
   return RH3_OK;
 }
-int check_out(const char* name, const char* what, const Out& o, int64_t rows, int64_t heads) {
-  if (const int e = check_rows(name, what, o.x, o.st, o.sh)) return e;
-  RH3_REQUIRE((rows == 1 || o.st != 0) && (heads == 1 || o.sh != 0), "%s: rows or heads of %s share memory", name, what);
+int check_rows(const char* name, const char* what, const rh3_head_rows& r) {
+  RH3_REQUIRE(r.x, "%s: null %s", name, what);
+  RH3_REQUIRE(aligned16(r.x) && r.st % 8 == 0 && r.sh % 8 == 0, "%s: %s must be 16-byte aligned with strides that are multiples of 8", name, what);
+  return RH3_OK;
+}
+int check_out(const char* name, const char* what, const rh3_head_rows& r, int64_t rows, int64_t heads) {
+  if (const int e = check_rows(name, what, r)) return e;
+  RH3_REQUIRE((rows == 1 || r.st != 0) && (heads == 1 || r.sh != 0), "%s: rows or heads of %s share memory", name, what);
   return RH3_OK;
 }
 
 // Few tokens go one to a workgroup, whose heads then take fewer turns; heads are spread over workgroups until there are 8 to a CU.
 template <int FMT, int D>
-int launch_rope(const char* name, RopeArgs& a, int dtype, hipStream_t st) {
+int launch_rope(const char* name, RopeArgs& a, int64_t dtype, hipStream_t st) {
   const int64_t cus = device_cus() > 0 ? device_cus() : 256;
   a.log2tt = a.rows < 4 * cus ? 0 : 2;
   const int at_once = NT / (D / 8) >> a.log2tt;
@@ -307,74 +306,65 @@ int launch_rope(const char* name, RopeArgs& a, int dtype, hipStream_t st) {
 using namespace rh3;
 using namespace rh3::kv;
 
-extern "C" int rh3_qk_norm_rope(const void* q, int64_t q_st, int64_t q_sh, void* q_out, int64_t qo_st, int64_t qo_sh, int64_t q_heads,
-                                const void* k, int64_t k_st, int64_t k_sh, void* k_out, int64_t ko_st, int64_t ko_sh, int64_t k_heads,
-                                int64_t rows, int64_t dim, int dtype, const int32_t* positions, const double* freq, int64_t rot,
-                                int interleaved, double factor, int norm, double eps, const void* qw, const void* kw, int wide_weights,
-                                hipStream_t stream) {
+extern "C" int rh3_qk_norm_rope(const rh3_rope_args* x, hipStream_t stream) {
   const char* name = "qk_norm_rope";
   clear_error();
+  RH3_REQUIRE(x, "%s: null arguments", name);
   RopeArgs a{};
-  a.t = Turn{freq, factor, static_cast<int>(rot), interleaved != 0, norm != 0, wide_weights != 0, eps, qw, kw};
-  if (const int e = check_turn(name, a.t, rot, dim)) return e;
-  RH3_REQUIRE(rows >= 0 && rows <= MAX_ROWS, "%s: %lld rows", name, static_cast<long long>(rows));
-  RH3_REQUIRE(q_heads >= 0 && q_heads <= 65535 && k_heads >= 0 && k_heads <= 65535, "%s: %lld and %lld heads", name, static_cast<long long>(q_heads),
-              static_cast<long long>(k_heads));
-  RH3_REQUIRE(dtype == RH3_DTYPE_BF16 || dtype == RH3_DTYPE_F16 || dtype == RH3_DTYPE_F32, "%s: row type %d (bf16, fp16 or fp32)", name, dtype);
-  if (rows == 0 || q_heads + k_heads == 0) return RH3_OK;
-  RH3_REQUIRE(rot == 0 || positions, "%s: no positions", name);
-  a.q = Rows{q, q_st, q_sh};
-  a.k = Rows{k, k_st, k_sh};
-  a.qo = Out{q_out, qo_st, qo_sh};
-  a.ko = Out{k_out, ko_st, ko_sh};
-  if (q_heads) {
-    if (const int e = check_rows(name, "q", q, q_st, q_sh)) return e;
-    if (const int e = check_out(name, "q's result", a.qo, rows, q_heads)) return e;
+  if (const int e = check_turn(name, x->turn, x->dim, a.t)) return e;
+  RH3_REQUIRE(x->rows >= 0 && x->rows <= MAX_ROWS, "%s: %lld rows", name, static_cast<long long>(x->rows));
+  RH3_REQUIRE(x->q_heads >= 0 && x->q_heads <= 65535 && x->k_heads >= 0 && x->k_heads <= 65535, "%s: %lld and %lld heads", name,
+              static_cast<long long>(x->q_heads), static_cast<long long>(x->k_heads));
+  if (const int e = check_type(name, x->dtype)) return e;
+  if (x->rows == 0 || x->q_heads + x->k_heads == 0) return RH3_OK;
+  RH3_REQUIRE(x->turn.rot == 0 || x->positions, "%s: no positions", name);
+  if (x->q_heads) {
+    if (const int e = check_rows(name, "q", x->q)) return e;
+    if (const int e = check_out(name, "q's result", x->q_out, x->rows, x->q_heads)) return e;
   }
-  if (k_heads) {
-    if (const int e = check_rows(name, "k", k, k_st, k_sh)) return e;
-    if (const int e = check_out(name, "k's result", a.ko, rows, k_heads)) return e;
+  if (x->k_heads) {
+    if (const int e = check_rows(name, "k", x->k)) return e;
+    if (const int e = check_out(name, "k's result", x->k_out, x->rows, x->k_heads)) return e;
   }
-  a.q_heads = static_cast<int>(q_heads);
-  a.k_heads = static_cast<int>(k_heads);
-  a.rows = static_cast<int>(rows);
-  a.positions = positions;
-  return dim == 128 ? launch_rope<NONE, 128>(name, a, dtype, stream) : launch_rope<NONE, 64>(name, a, dtype, stream);
+  a.q = x->q;
+  a.k = x->k;
+  a.qo = x->q_out;
+  a.ko = x->k_out;
+  a.q_heads = static_cast<int>(x->q_heads);
+  a.k_heads = static_cast<int>(x->k_heads);
+  a.rows = static_cast<int>(x->rows);
+  a.positions = x->positions;
+  return x->dim == 128 ? launch_rope<NONE, 128>(name, a, x->dtype, stream) : launch_rope<NONE, 64>(name, a, x->dtype, stream);
 }
 
-extern "C" int rh3_kv_write_rope(const rh3_kv_cache* cache, const void* q, int64_t q_st, int64_t q_sh, void* q_out, int64_t qo_st,
-                                 int64_t qo_sh, int64_t q_heads, const void* k, int64_t k_st, int64_t k_sh, const void* v, int64_t v_st,
-                                 int64_t v_sh, int dtype, int64_t rows, const int32_t* table, int64_t table_stride, int64_t width,
-                                 const int32_t* lens, const int32_t* cu, int64_t batch, int64_t first, const double* freq, int64_t rot,
-                                 int interleaved, double factor, int norm, double eps, const void* qw, const void* kw, int wide_weights,
-                                 hipStream_t stream) {
+extern "C" int rh3_kv_write_rope(const rh3_kv_cache* cache, const rh3_kv_rope_args* x, hipStream_t stream) {
   const char* name = "kv_write_rope";
   clear_error();
+  RH3_REQUIRE(x, "%s: null arguments", name);
   RopeArgs a{};
   if (const int e = check_cache(name, cache, a.c)) return e;
-  if (const int e = check_seqs(name, a.c, table, table_stride, width, lens, cu, batch, rows, a.s)) return e;
-  a.t = Turn{freq, factor, static_cast<int>(rot), interleaved != 0, norm != 0, wide_weights != 0, eps, qw, kw};
-  if (const int e = check_turn(name, a.t, rot, cache->dim)) return e;
-  RH3_REQUIRE(q_heads >= 1 && q_heads <= 65535, "%s: %lld query heads", name, static_cast<long long>(q_heads));
-  RH3_REQUIRE(first >= -MAX_ROWS && first <= MAX_ROWS, "%s: first position %lld", name, static_cast<long long>(first));
-  RH3_REQUIRE(dtype == RH3_DTYPE_BF16 || dtype == RH3_DTYPE_F16 || dtype == RH3_DTYPE_F32, "%s: row type %d (bf16, fp16 or fp32)", name, dtype);
-  if (rows == 0) return RH3_OK;
-  a.q = Rows{q, q_st, q_sh};
-  a.k = Rows{k, k_st, k_sh};
-  a.v = Rows{v, v_st, v_sh};
-  a.qo = Out{q_out, qo_st, qo_sh};
-  if (const int e = check_rows(name, "q", q, q_st, q_sh)) return e;
-  if (const int e = check_rows(name, "k", k, k_st, k_sh)) return e;
-  if (const int e = check_rows(name, "v", v, v_st, v_sh)) return e;
-  if (const int e = check_out(name, "q's result", a.qo, rows, q_heads)) return e;
-  a.q_heads = static_cast<int>(q_heads);
+  if (const int e = check_seqs(name, a.c, x->table, x->table_stride, x->width, x->lens, x->cu, x->batch, x->rows, a.s)) return e;
+  if (const int e = check_turn(name, x->turn, cache->dim, a.t)) return e;
+  RH3_REQUIRE(x->q_heads >= 1 && x->q_heads <= 65535, "%s: %lld query heads", name, static_cast<long long>(x->q_heads));
+  RH3_REQUIRE(x->first >= -MAX_ROWS && x->first <= MAX_ROWS, "%s: first position %lld", name, static_cast<long long>(x->first));
+  if (const int e = check_type(name, x->dtype)) return e;
+  if (x->rows == 0) return RH3_OK;
+  if (const int e = check_rows(name, "q", x->q)) return e;
+  if (const int e = check_rows(name, "k", x->k)) return e;
+  if (const int e = check_rows(name, "v", x->v)) return e;
+  if (const int e = check_out(name, "q's result", x->q_out, x->rows, x->q_heads)) return e;
+  a.q = x->q;
+  a.k = x->k;
+  a.v = x->v;
+  a.qo = x->q_out;
+  a.q_heads = static_cast<int>(x->q_heads);
   a.k_heads = a.c.heads;
-  a.rows = static_cast<int>(rows);
-  a.first = static_cast<int>(first);
+  a.rows = static_cast<int>(x->rows);
+  a.first = static_cast<int>(x->first);
   const int64_t fmt = cache->format;
   if (cache->dim == 128)
-    return fmt == INT8 ? launch_rope<INT8, 128>(name, a, dtype, stream)
-                       : fmt == E4M3 ? launch_rope<E4M3, 128>(name, a, dtype, stream) : launch_rope<FP4, 128>(name, a, dtype, stream);
-  return fmt == INT8 ? launch_rope<INT8, 64>(name, a, dtype, stream)
-                     : fmt == E4M3 ? launch_rope<E4M3, 64>(name, a, dtype, stream) : launch_rope<FP4, 64>(name, a, dtype, stream);
+    return fmt == INT8 ? launch_rope<INT8, 128>(name, a, x->dtype, stream)
+                       : fmt == E4M3 ? launch_rope<E4M3, 128>(name, a, x->dtype, stream) : launch_rope<FP4, 128>(name, a, x->dtype, stream);
+  return fmt == INT8 ? launch_rope<INT8, 64>(name, a, x->dtype, stream)
+                     : fmt == E4M3 ? launch_rope<E4M3, 64>(name, a, x->dtype, stream) : launch_rope<FP4, 64>(name, a, x->dtype, stream);
 }

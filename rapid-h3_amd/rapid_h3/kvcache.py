@@ -16,6 +16,7 @@ are not read and stay as they are; of rows that cu names but the call does not h
 """
 import ctypes
 import functools
+import struct
 
 import torch
 
@@ -29,6 +30,10 @@ GROUP4 = 32                           # channels of a 4-bit row that share a sca
 _BYTES = (torch.uint8, FP4)
 _SCALE4 = (torch.uint8, torch.float8_e8m0fnu)
 _FORM = {None: nat.RH3_KV_BY_SIZE, "token": nat.RH3_KV_TOKEN, "chunk": nat.RH3_KV_CHUNK}
+
+
+_EXTEND = struct.Struct("=17q")                        # rh3_kv_extend_args
+_WRITE_ROPE = struct.Struct("=22q" + rope._TURN)       # rh3_kv_rope_args
 
 
 def _st(t, axis):
@@ -152,12 +157,15 @@ def kv_extend(pool, table, lens, new, rows, done=None):
     dev = table.device
     cu = torch.empty(b + 1, dtype=torch.int32, device=dev)
     positions = torch.empty(rows, dtype=torch.int32, device=dev)
-    slots = torch.empty(rows, dtype=torch.int64, device=dev)
+    # the slots, with the workspace of 3 (b + 1) words behind them (16-byte aligned)
+    even = rows + rows % 2
+    both = torch.empty(even + (3 * b + 4) // 2, dtype=torch.int64, device=dev)
+    at = both.data_ptr()
+    args = _EXTEND.pack(*pool._args, table.data_ptr(), _st(table, 0), w, lens.data_ptr(), new.data_ptr(), 0 if done is None else done.data_ptr(), b,
+                        cu.data_ptr(), positions.data_ptr(), at, rows, at + 8 * even, 12 * (b + 1))
     with _on(gpu):
-        n = 12 * (b + 1)
-        ws = torch.empty(n, dtype=torch.uint8, device=dev)
-        nat.call("rh3_kv_extend", *pool._args, table.data_ptr(), _st(table, 0), w, lens.data_ptr(), new.data_ptr(), nat.ptr(done), b,
-                 cu.data_ptr(), positions.data_ptr() if rows else None, slots.data_ptr() if rows else None, rows, ws.data_ptr(), n, _stream(gpu))
+        nat.call("rh3_kv_extend", args, _stream(gpu))
+    slots = both[:rows]
     return cu, positions, slots
 
 
@@ -216,19 +224,19 @@ def kv_write_rope(cache, q, k, v, table, lens, cu=None, rotary=None, q_weight=No
     name = "kv_write_rope"
     t, k_st, k_sh = _rows(name, "k", k, cache)
     tv, v_st, v_sh = _rows(name, "v", v, cache)
-    q_st, q_sh = rope._heads(name, "q", q)
-    gpu = q.get_device()
-    if tv != t or q.shape[0] != t or q.shape[2] != cache.dim or k.dtype != q.dtype or v.dtype != q.dtype or k.get_device() != gpu or v.get_device() != gpu:
+    qr, tq, hq, d = rope._rows_of(name, "q", q)
+    dtype, gpu = q.dtype, q.get_device()
+    if tv != t or tq != t or d != cache.dim or k.dtype != dtype or v.dtype != dtype or k.get_device() != gpu or v.get_device() != gpu:
         raise TypeError(f"{name}: q, k and v must be of one number of rows, dim, device and type (bf16, fp16 or fp32)")
-    turn = rope._turn(name, rotary, q_weight, k_weight, eps, cache.dim, q.dtype, gpu)
-    seqs = _seqs(name, cache, table, lens, cu, gpu)
-    if out is None:
-        out = (torch.empty if cu is None else torch.zeros)(q.shape, dtype=q.dtype, device=q.device)
-    else:
-        rope._result(name, "q", q, out)
+    turn = rope._turn(name, rotary, q_weight, k_weight, eps, d, dtype, gpu)
+    table_at, table_st, width, lens_at, cu_at, b = _seqs(name, cache, table, lens, cu, gpu)
+    if out is None and cu is not None:
+        out = torch.zeros((t, hq, d), dtype=dtype, device=q.device)      # rows that no sequence has are not written
+    out, outr = rope._result(name, "q", q, t, hq, d, out)
+    args = _WRITE_ROPE.pack(*qr, *outr, k.data_ptr(), k_st, k_sh, v.data_ptr(), v_st, v_sh, hq, _ROW[dtype], t, table_at, table_st, width, lens_at,
+                            cu_at or 0, b, int(first), *turn)
     with _on(gpu):
-        nat.call("rh3_kv_write_rope", cache._ref, q.data_ptr(), q_st, q_sh, out.data_ptr(), *rope._heads(name, "out", out), q.shape[1],
-                 k.data_ptr(), k_st, k_sh, v.data_ptr(), v_st, v_sh, _ROW[q.dtype], t, *seqs, int(first), *turn, _stream(gpu))
+        nat.call("rh3_kv_write_rope", cache._ref, args, _stream(gpu))
     return out
 
 
@@ -243,7 +251,8 @@ def kv_read(cache, table, lens, cu=None, rows=None, dtype=torch.bfloat16, out=No
         if dtype not in _ROW:
             raise TypeError(f"kv_read: bf16, fp16 or fp32 values, got {dtype}")
         alloc = torch.empty if cu is None else torch.zeros      # rows that no sequence has are not written
-        out = alloc((2, n, cache.heads, cache.dim), dtype=dtype, device=cache.device).unbind(0)
+        out = alloc((2, n, cache.heads, cache.dim), dtype=dtype, device=cache.device)
+        out = out[0], out[1]
     k, v = out
     _rows_call("kv_read", "rh3_kv_read", ("out[0]", "out[1]"), cache, k, v, table, lens, cu)
     return k, v

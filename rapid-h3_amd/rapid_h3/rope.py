@@ -8,6 +8,7 @@ the first rot channels become (a cos - b sin, b cos + a sin) in fp32, with the c
 64 bits, so far positions keep their angle) times `factor`, each rounded to fp32 once; one rounding to the rows' type at the end.
 """
 import math
+import struct
 
 import torch
 
@@ -15,6 +16,8 @@ from . import _native as nat
 from ._rows import _ROW, _on, _stream
 
 LAYOUTS = ("half", "interleaved")
+_TURN = "3qdqd3q"                                # rh3_turn
+_ARGS = struct.Struct("=18q" + _TURN)            # rh3_rope_args
 
 
 class Rotary:
@@ -76,45 +79,48 @@ def rotary(rot, layout="half", device="cuda", **how):
 
 
 def _turn(name, rotary, q_weight, k_weight, eps, dim, dtype, gpu):
-    """The entry points' arguments for a Rotary and a norm: freq, rot, interleaved, factor, norm, eps, the weights, their width."""
+    """rh3_turn of a Rotary and a norm: freq, rot, interleaved, factor, norm, eps, the weights, their width."""
+    if eps is None:
+        if rotary is None:
+            raise ValueError(f"{name}: neither a rotary nor eps: nothing to do")
+        if q_weight is not None or k_weight is not None:
+            raise ValueError(f"{name}: weights without eps (eps=None is no norm)")
     if rotary is not None and (rotary.gpu != gpu or rotary.rot > dim):
         raise RuntimeError(f"{name}: rotary must be on the rows' GPU and turn at most {dim} channels, got {rotary.rot}")
-    wide = None
-    for w in (q_weight, k_weight):
-        if w is None:
-            continue
-        if eps is None:
-            raise ValueError(f"{name}: weights without eps (eps=None is no norm)")
-        if w.shape != (dim,) or w.dtype not in (dtype, torch.float32) or w.stride(0) != 1 or w.get_device() != gpu:
-            raise RuntimeError(f"{name}: norm weights must be contiguous [{dim}] of the rows' type or fp32, on their GPU")
-        if wide is not None and wide != (w.dtype == torch.float32):
-            raise RuntimeError(f"{name}: the norm weights must be of one type")
-        wide = w.dtype == torch.float32
-    if rotary is None and eps is None:
-        raise ValueError(f"{name}: neither a rotary nor eps: nothing to do")
-    return (*(rotary._args if rotary is not None else (None, 0, False, 1.0)), eps is not None, 0.0 if eps is None else float(eps),
-            nat.ptr(q_weight), nat.ptr(k_weight), bool(wide))
+    wide, at = None, [0, 0]
+    for i, w in enumerate((q_weight, k_weight)):
+        if w is not None:
+            t = w.dtype
+            if w.shape != (dim,) or (t != dtype and t != torch.float32) or not w.is_contiguous() or w.get_device() != gpu:
+                raise RuntimeError(f"{name}: norm weights must be contiguous [{dim}] of the rows' type or fp32, on their GPU")
+            if wide is not None and wide != (t == torch.float32):
+                raise RuntimeError(f"{name}: the norm weights must be of one type")
+            wide, at[i] = t == torch.float32, w.data_ptr()
+    freq, rot, interleaved, factor = (0, 0, False, 1.0) if rotary is None else rotary._args
+    return freq, rot, interleaved, factor, eps is not None, 0.0 if eps is None else eps, at[0], at[1], bool(wide)
 
 
-def _heads(name, what, x, like=None):
-    """Strides of rows [rows, heads, dim]; 0 for an axis of length 1."""
-    if x.ndim != 3 or x.shape[2] not in (64, 128) or x.stride(2) != 1 or x.dtype not in _ROW:
-        raise RuntimeError(f"{name}: {what} must be [rows, heads, 64 or 128] bf16, fp16 or fp32 with a contiguous last dim, got {x.dtype} "
+def _rows_of(name, what, x):
+    """rh3_head_rows of rows [rows, heads, dim] (strides 0 for axes of length 1), and their sizes."""
+    if x.ndim != 3 or x.dtype not in _ROW or not x.is_cuda:
+        raise RuntimeError(f"{name}: {what} must be [rows, heads, 64 or 128] bf16, fp16 or fp32 on a GPU (no CPU path), got {x.dtype} "
                            f"{tuple(x.shape)}")
-    if like is not None and (x.shape[0] != like.shape[0] or x.shape[2] != like.shape[2] or x.dtype != like.dtype or x.get_device() != like.get_device()):
-        raise RuntimeError(f"{name}: {what} must be of q's rows, dim, type and GPU")
-    if not x.is_cuda:
-        raise RuntimeError(f"{name}: {what} must be on a GPU (no CPU path)")
-    st, sh, _ = x.stride()
-    return st if x.shape[0] > 1 else 0, sh if x.shape[1] > 1 else 0
+    t, h, d = x.shape
+    st, sh, sd = x.stride()
+    if sd != 1 or (d != 128 and d != 64):
+        raise RuntimeError(f"{name}: {what} must be [rows, heads, 64 or 128] with a contiguous last dim, got {(t, h, d)}")
+    return (x.data_ptr(), st if t > 1 else 0, sh if h > 1 else 0), t, h, d
 
 
-def _result(name, what, x, out):
+def _result(name, what, x, t, h, d, out):
+    """A new result like rows x, or `out`, checked; and its rh3_head_rows."""
     if out is None:
-        return torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    if out.shape != x.shape or out.dtype != x.dtype or out.stride(2) != 1 or out.get_device() != x.get_device():
-        raise RuntimeError(f"{name}: out for {what} must be like it, with a contiguous last dim")
-    return out
+        out = torch.empty_strided((t, h, d), (h * d, d, 1), dtype=x.dtype, device=x.device)
+        return out, (out.data_ptr(), h * d, d)
+    rows, to, ho, do = _rows_of(name, f"out for {what}", out)
+    if (to, ho, do) != (t, h, d) or out.dtype != x.dtype or out.get_device() != x.get_device():
+        raise RuntimeError(f"{name}: out for {what} must be like it")
+    return out, rows
 
 
 def qk_norm_rope(q, k, positions, rotary, q_weight=None, k_weight=None, eps=None, out=None):
@@ -122,20 +128,24 @@ def qk_norm_rope(q, k, positions, rotary, q_weight=None, k_weight=None, eps=None
     (bf16, fp16 or fp32, strided ok; k may be None) at positions [rows] int32 -> new tensors like them, or `out`, a pair. out may lie
     exactly over q and k."""
     name = "qk_norm_rope"
-    q_st, q_sh = _heads(name, "q", q)
-    gpu = q.get_device()
-    t, hq, dim = q.shape
-    turn = _turn(name, rotary, q_weight, k_weight, eps, dim, q.dtype, gpu)
-    if rotary is not None and (positions.dtype != torch.int32 or positions.shape != (t,) or not positions.is_contiguous() or positions.get_device() != gpu):
-        raise RuntimeError(f"{name}: positions must be contiguous int32 [{t}] on the rows' GPU")
+    qr, t, hq, dim = _rows_of(name, "q", q)
+    dtype, gpu = q.dtype, q.get_device()
+    at = 0
+    if rotary is not None:
+        if positions.dtype != torch.int32 or positions.shape != (t,) or not positions.is_contiguous() or positions.get_device() != gpu:
+            raise RuntimeError(f"{name}: positions must be contiguous int32 [{t}] on the rows' GPU")
+        at = positions.data_ptr()
+    turn = _turn(name, rotary, q_weight, k_weight, eps, dim, dtype, gpu)
     qo, ko = (None, None) if out is None else out
-    qo = _result(name, "q", q, qo)
-    keys = (None, 0, 0, None, 0, 0, 0)
+    qo, qor = _result(name, "q", q, t, hq, dim, qo)
+    kr = kor = (0, 0, 0)
+    hk = 0
     if k is not None:
-        k_st, k_sh = _heads(name, "k", k, q)
-        ko = _result(name, "k", k, ko)
-        keys = (k.data_ptr(), k_st, k_sh, ko.data_ptr(), *_heads(name, "out for k", ko), k.shape[1])
+        kr, tk, hk, dk = _rows_of(name, "k", k)
+        if tk != t or dk != dim or k.dtype != dtype or k.get_device() != gpu:
+            raise RuntimeError(f"{name}: k must be of q's rows, dim, type and GPU")
+        ko, kor = _result(name, "k", k, t, hk, dim, ko)
+    args = _ARGS.pack(*qr, *qor, *kr, *kor, hq, hk, t, dim, _ROW[dtype], at, *turn)
     with _on(gpu):
-        nat.call("rh3_qk_norm_rope", q.data_ptr(), q_st, q_sh, qo.data_ptr(), *_heads(name, "out for q", qo), hq, *keys, t, dim, _ROW[q.dtype],
-                 None if rotary is None else positions.data_ptr(), *turn, _stream(gpu))
+        nat.call("rh3_qk_norm_rope", args, _stream(gpu))
     return qo, ko if k is not None else None
