@@ -98,28 +98,6 @@ __device__ __forceinline__ float inverse_rms(const float* x, double eps) {
 }
 
 template <int DT>
-struct Raw {
-  uint4 w[DT == RH3_DTYPE_F32 ? 2 : 1];
-};
-template <int DT>
-__device__ __forceinline__ Raw<DT> load_raw(const void* p, int64_t at) {
-  Raw<DT> r;
-  const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p) + at * (DT == RH3_DTYPE_F32 ? 4 : 2));
-  r.w[0] = src[0];
-  if constexpr (DT == RH3_DTYPE_F32) r.w[1] = src[1];
-  return r;
-}
-template <int DT>
-__device__ __forceinline__ void values_of(const Raw<DT>& r, float* x) {
-  if constexpr (DT == RH3_DTYPE_F32) {
-    const uint32_t w[8] = {r.w[0].x, r.w[0].y, r.w[0].z, r.w[0].w, r.w[1].x, r.w[1].y, r.w[1].z, r.w[1].w};
-#pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = __uint_as_float(w[e]);
-  } else {
-    row8<DT>(r.w[0], x);
-  }
-}
-template <int DT>
 __device__ __forceinline__ void weights8(const Turn& t, const void* w, int at, float* x) {
   if (!w) {
 #pragma unroll
