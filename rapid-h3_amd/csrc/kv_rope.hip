@@ -11,8 +11,8 @@
 //
 // Bound by memory. A workgroup takes 4 tokens (few rows: 1), makes their cosines and sines in LDS, one angle to a thread, and walks
 // the heads, 16 rows of 128 at a time (64: 32); a row is 8 channels in each of dim / 8 lanes, which keep their token and so the
-// cosines and sines of their channels in registers. The other channels of a lane's pairs, where they lie rot / 2 apart, are loaded
-// a second time (from L1) and normed again, which needs no exchange between lanes.
+// cosines and sines of their channels in registers. The 8 are 4 and the 4 that they turn with, so no lane needs another's; keys on
+// their way into a cache are 8 neighbours, as their codes lie.
 #include "kv_rows.hpp"
 
 namespace rh3 {
@@ -34,7 +34,7 @@ struct RopeArgs {
   Turn t;
   rh3_head_rows q, k, v;             // v: not of FMT NONE
   rh3_head_rows qo, ko;              // ko: of FMT NONE
-  int q_heads, k_heads, rows, log2tt;
+  int q_heads, k_heads, rows, log2tt, once;
   int first;                         // added to the positions of the cache's rows
   const int32_t* positions;          // FMT NONE
   Cache c;
@@ -97,15 +97,71 @@ __device__ __forceinline__ float inverse_rms(const float* x, double eps) {
   return static_cast<float>(y);
 }
 
+// 4 channels of a row as they lie
 template <int DT>
-__device__ __forceinline__ void weights8(const Turn& t, const void* w, int at, float* x) {
-  if (!w) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = 1.0f;
-  } else if (t.wide) {
-    load_row8<RH3_DTYPE_F32>(w, at, x);
+struct Raw4 {
+  uint32_t w[DT == RH3_DTYPE_F32 ? 4 : 2];
+};
+template <int DT>
+__device__ __forceinline__ Raw4<DT> load_raw4(const void* p, int64_t at, bool once) {
+  Raw4<DT> r;
+  if constexpr (DT == RH3_DTYPE_F32) {
+    const u32x4_t* src = reinterpret_cast<const u32x4_t*>(static_cast<const float*>(p) + at);
+    const u32x4_t x = once ? __builtin_nontemporal_load(src) : *src;
+    r.w[0] = x[0]; r.w[1] = x[1]; r.w[2] = x[2]; r.w[3] = x[3];
   } else {
-    load_row8<DT>(w, at, x);
+    const u32x2_t* src = reinterpret_cast<const u32x2_t*>(static_cast<const uint16_t*>(p) + at);
+    const u32x2_t x = once ? __builtin_nontemporal_load(src) : *src;
+    r.w[0] = x[0]; r.w[1] = x[1];
+  }
+  return r;
+}
+template <int DT>
+__device__ __forceinline__ void values_of(const Raw4<DT>& r, float* x) {
+  if constexpr (DT == RH3_DTYPE_F32) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = __uint_as_float(r.w[e]);
+  } else if constexpr (DT == RH3_DTYPE_BF16) {
+#pragma unroll
+    for (int e = 0; e < 4; e += 2) {
+      x[e] = __uint_as_float(r.w[e / 2] << 16);
+      x[e + 1] = __uint_as_float(r.w[e / 2] & 0xffff0000u);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; e += 2) {
+      const h2_t h = __builtin_bit_cast(h2_t, r.w[e / 2]);
+      x[e] = static_cast<float>(h[0]);
+      x[e + 1] = static_cast<float>(h[1]);
+    }
+  }
+}
+template <int DT>
+__device__ __forceinline__ void store4(void* p, int64_t at, const float* x, bool once) {
+  if constexpr (DT == RH3_DTYPE_F32) {
+    const u32x4_t r = {__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3])};
+    u32x4_t* to = reinterpret_cast<u32x4_t*>(static_cast<float*>(p) + at);
+    if (once) __builtin_nontemporal_store(r, to);
+    else *to = r;
+  } else {
+    const u32x2_t r = DT == RH3_DTYPE_BF16 ? u32x2_t{pack_bf2(x[0], x[1]), pack_bf2(x[2], x[3])} : u32x2_t{pack_h2(x[0], x[1]), pack_h2(x[2], x[3])};
+    u32x2_t* to = reinterpret_cast<u32x2_t*>(static_cast<uint16_t*>(p) + at);
+    if (once) __builtin_nontemporal_store(r, to);
+    else *to = r;
+  }
+}
+template <int DT, int N>
+__device__ __forceinline__ void weights_of(const Turn& t, const void* w, int at, float* x) {
+#pragma unroll
+  for (int i = 0; i < N; i += 4) {
+    if (!w) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[i + e] = 1.0f;
+    } else if (t.wide) {
+      values_of<RH3_DTYPE_F32>(load_raw4<RH3_DTYPE_F32>(w, at + i, false), x + i);
+    } else {
+      values_of<DT>(load_raw4<DT>(w, at + i, false), x + i);
+    }
   }
 }
 // rounded to the rows' type
@@ -128,106 +184,166 @@ __global__ void __launch_bounds__(NT) rope_kernel(RopeArgs a) {
   const int tt = 1 << a.log2tt, heads_at_once = SLOTS >> a.log2tt;
   const int tok = slot & (tt - 1), row = (blockIdx.x << a.log2tt) + tok, hs = slot >> a.log2tt;
   const Turn& t = a.t;
-  const int half = t.rot >> 1, c0 = 8 * l;
-  const bool turned = c0 < t.rot;
-  // the other half's channels of the lane's pairs
-  const int p0 = t.interleaved || !turned ? c0 : c0 < half ? c0 + half : c0 - half;
+  const int half = t.rot >> 1;
+  // two pieces of 4 channels that hold whole pairs: 4 l and its partners, or 8 neighbours
+  const bool split = !t.interleaved && l < half / 4;
+  const int c0 = split ? 4 * l : 8 * l, c1 = split ? half + 4 * l : c0 + 4;
+  const bool turned = split || (t.interleaved && c0 < t.rot);
 
   Place place{0, 0, 0, true, false};
   if constexpr (FMT != NONE) place = place_of<FMT, D>(a.s, a.c, row);
   const bool mine = row < a.rows && place.mine;
+  // groups of heads that go at once: the queries', then the keys'
   const int q_groups = (a.q_heads + heads_at_once - 1) / heads_at_once, k_groups = (a.k_heads + heads_at_once - 1) / heads_at_once;
+  const int plain = FMT == NONE ? q_groups + k_groups : q_groups;   // those whose rows go out as rows
   int g = blockIdx.y;
-  auto load = [&](int g, Raw<DT>& own, Raw<DT>& other) __attribute__((always_inline)) {
+  auto load = [&](int g, Raw4<DT>& r0, Raw4<DT>& r1) __attribute__((always_inline)) {
     const bool key = g >= q_groups;
     const int h = (key ? g - q_groups : g) * heads_at_once + hs;
-    if (mine && g < q_groups + k_groups && h < (key ? a.k_heads : a.q_heads)) {
+    if (mine && g < plain && h < (key ? a.k_heads : a.q_heads)) {
       const rh3_head_rows& r = key ? a.k : a.q;
-      own = load_raw<DT>(r.x, row * r.st + h * r.sh + c0);
-      other = load_raw<DT>(r.x, row * r.st + h * r.sh + p0);
+      const int64_t at = row * r.st + h * r.sh;
+      r0 = load_raw4<DT>(r.x, at + c0, a.once);
+      r1 = load_raw4<DT>(r.x, at + c1, a.once);
     }
   };
-  Raw<DT> own{}, other{};
-  load(g, own, other);
+  Raw4<DT> raw0{}, raw1{};
+  load(g, raw0, raw1);
 
   if (half) {
-    for (int i = threadIdx.x; i < half << a.log2tt; i += NT) {
-      const int r = i / half, f = i - r * half;
-      const int at = (blockIdx.x << a.log2tt) + r;
-      int pos = 0;
-      if constexpr (FMT == NONE) {
-        if (at < a.rows) pos = a.positions[at];
-        turns[r][f] = cos_sin(static_cast<double>(pos) * t.freq[f], t.factor);
+    if constexpr (FMT == NONE) {
+      for (int i = threadIdx.x; i < half << a.log2tt; i += NT) {
+        const int r = i / half, f = i - r * half, at = (blockIdx.x << a.log2tt) + r;
+        turns[r][f] = cos_sin(static_cast<double>(at < a.rows ? a.positions[at] : 0) * t.freq[f], t.factor);
       }
-    }
-    if constexpr (FMT != NONE) {
-      // a token's position is known to its own lanes: LPR of them and, with other heads of it, those of other slots
+    } else {
+      // a token's position is known to its own lanes, those of all its heads
       const double pos = static_cast<double>(static_cast<int64_t>(place.pos) + a.first);
       for (int f = hs * LPR + l; f < half; f += heads_at_once * LPR) turns[tok][f] = cos_sin(pos * t.freq[f], t.factor);
     }
     __syncthreads();
   }
-  float cs[8], sn[8];
+  {
+    float cs[4], sn[4];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    cs[e] = 1.0f;
-    sn[e] = 0.0f;
+    for (int e = 0; e < 4; ++e) {
+      const float2 v = turned ? turns[tok][4 * l + e] : make_float2(1.0f, 0.0f);
+      cs[e] = v.x;
+      sn[e] = v.y;
+    }
+    float w0[4], w1[4];
+    bool loaded_q = false, loaded_k = false;
+    for (; g < plain; g += gridDim.y) {
+      const bool key = g >= q_groups;
+      const int h = (key ? g - q_groups : g) * heads_at_once + hs;
+      const bool here = mine && h < (key ? a.k_heads : a.q_heads);
+      Raw4<DT> next0{}, next1{};
+      load(g + gridDim.y, next0, next1);
+      if (t.norm && !(key ? loaded_k : loaded_q)) {
+        weights_of<DT, 4>(t, key ? t.kw : t.qw, c0, w0);
+        weights_of<DT, 4>(t, key ? t.kw : t.qw, c1, w1);
+        loaded_q = !key;
+        loaded_k = key;
+      }
+      if (here) {   // whole rows of lanes
+        float x[8];
+        values_of<DT>(raw0, x);
+        values_of<DT>(raw1, x + 4);
+        if (t.norm) {
+          const float r = inverse_rms<D>(x, t.eps);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            x[e] = (x[e] * r) * w0[e];
+            x[4 + e] = (x[4 + e] * r) * w1[e];
+          }
+        }
+        if (turned) {
+          float y[8];
+          if (t.interleaved) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              y[2 * e] = x[2 * e] * cs[e] - x[2 * e + 1] * sn[e];
+              y[2 * e + 1] = x[2 * e + 1] * cs[e] + x[2 * e] * sn[e];
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              y[e] = x[e] * cs[e] - x[4 + e] * sn[e];
+              y[4 + e] = x[4 + e] * cs[e] + x[e] * sn[e];
+            }
+          }
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[e] = y[e];
+        }
+        const rh3_head_rows& o = key ? a.ko : a.qo;
+        const int64_t at = row * o.st + h * o.sh;
+        store4<DT>(o.x, at + c0, x, a.once);
+        store4<DT>(o.x, at + c1, x + 4, a.once);
+      }
+      raw0 = next0;
+      raw1 = next1;
+    }
   }
-  if (turned) {
+  if constexpr (FMT != NONE) {
+    // Keys and values on their way into the cache: a lane has 8 neighbours, as the codes are kept. The other channels of its pairs,
+    // where they lie rot / 2 apart, are loaded a second time (from L1) and normed again.
+    const int own = 8 * l;
+    const bool turned = own < t.rot;
+    const int other = t.interleaved || !turned ? own : own < half ? own + half : own - half;
+    auto load_kv = [&](int g, Raw<DT>& k, Raw<DT>& p, Raw<DT>& v) __attribute__((always_inline)) {
+      const int h = (g - q_groups) * heads_at_once + hs;
+      if (place.there && h < a.k_heads) {
+        const int64_t at = row * a.k.st + h * a.k.sh;
+        k = load_raw<DT>(a.k.x, at + own);
+        p = load_raw<DT>(a.k.x, at + other);
+        v = load_raw<DT>(a.v.x, row * a.v.st + h * a.v.sh + own);
+      }
+    };
+    Raw<DT> rk{}, rp{}, rv{};
+    if (g < q_groups + k_groups) load_kv(g, rk, rp, rv);
+    float cs[8], sn[8], w[8], wo[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const float2 v = turns[tok][t.interleaved ? (c0 + e) >> 1 : (c0 < half ? c0 : c0 - half) + e];
+      const float2 v = turned ? turns[tok][t.interleaved ? (own + e) >> 1 : (own < half ? own : own - half) + e] : make_float2(1.0f, 0.0f);
       cs[e] = v.x;
-      sn[e] = (t.interleaved ? (e & 1) == 0 : c0 < half) ? -v.y : v.y;
+      sn[e] = (t.interleaved ? (e & 1) == 0 : own < half) ? -v.y : v.y;
     }
-  }
-  float w[8], wo[8];
-  bool loaded_q = false, loaded_k = false;
-  for (; g < q_groups + k_groups; g += gridDim.y) {
-    const bool key = g >= q_groups;
-    const int h = (key ? g - q_groups : g) * heads_at_once + hs;
-    const bool here = mine && h < (key ? a.k_heads : a.q_heads);
-    Raw<DT> next_own{}, next_other{};
-    load(g + gridDim.y, next_own, next_other);
-    if (t.norm && !(key ? loaded_k : loaded_q)) {
-      weights8<DT>(t, key ? t.kw : t.qw, c0, w);
-      weights8<DT>(t, key ? t.kw : t.qw, p0, wo);
-      loaded_q = !key;
-      loaded_k = key;
+    if (t.norm && g < q_groups + k_groups) {
+      weights_of<DT, 8>(t, t.kw, own, w);
+      weights_of<DT, 8>(t, t.kw, other, wo);
     }
-    if (here) {   // whole rows of lanes
-      float x[8], o[8];
-      values_of<DT>(own, x);
-      values_of<DT>(other, o);
-      if (t.norm) {
-        const float r = inverse_rms<D>(x, t.eps);
+    for (; g < q_groups + k_groups; g += gridDim.y) {
+      const int h = (g - q_groups) * heads_at_once + hs;
+      Raw<DT> nk{}, np{}, nv{};
+      load_kv(g + gridDim.y, nk, np, nv);
+      if (place.there && h < a.k_heads) {   // whole rows of lanes
+        float x[8], o[8], y[8];
+        values_of<DT>(rk, x);
+        values_of<DT>(rp, o);
+        values_of<DT>(rv, y);
+        if (t.norm) {
+          const float r = inverse_rms<D>(x, t.eps);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          x[e] = (x[e] * r) * w[e];
-          o[e] = (o[e] * r) * wo[e];
+          for (int e = 0; e < 8; ++e) {
+            x[e] = (x[e] * r) * w[e];
+            o[e] = (o[e] * r) * wo[e];
+          }
         }
-      }
-      if (turned) {
-        if (t.interleaved) {
+        if (turned) {
+          if (t.interleaved) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) o[e] = x[e ^ 1];
+            for (int e = 0; e < 8; ++e) o[e] = x[e ^ 1];
+          }
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[e] = x[e] * cs[e] + o[e] * sn[e];
         }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = x[e] * cs[e] + o[e] * sn[e];
-      }
-      if (!key) {
-        store_row8<DT>(a.qo.x, row * a.qo.st + h * a.qo.sh + c0, x);
-      } else if constexpr (FMT == NONE) {
-        store_row8<DT>(a.ko.x, row * a.ko.st + h * a.ko.sh + c0, x);
-      } else if (place.there) {
-        float y[8];
-        values_of<DT>(load_raw<DT>(a.v.x, row * a.v.st + h * a.v.sh + c0), y);
         rounded8<DT>(x);
         put<FMT, D>(a.c, place, h, l, x, y);
       }
+      rk = nk;
+      rp = np;
+      rv = nv;
     }
-    own = next_own;
-    other = next_other;
   }
 }
 
@@ -263,6 +379,7 @@ template <int FMT, int D>
 int launch_rope(const char* name, RopeArgs& a, int64_t dtype, hipStream_t st) {
   const int64_t cus = device_cus() > 0 ? device_cus() : 256;
   a.log2tt = a.rows < 4 * cus ? 0 : 2;
+  a.once = static_cast<int64_t>(a.rows) * (a.q_heads + a.k_heads) * D * (dtype == RH3_DTYPE_F32 ? 4 : 2) > LAST_CACHE;
   const int at_once = NT / (D / 8) >> a.log2tt;
   const int64_t gx = (static_cast<int64_t>(a.rows) + (1 << a.log2tt) - 1) >> a.log2tt;
   const int64_t groups = (a.q_heads + at_once - 1) / at_once + (a.k_heads + at_once - 1) / at_once;
