@@ -17,7 +17,7 @@ namespace rh3 {
 namespace kv {
 namespace {
 
-constexpr int NT = 1024, WAVES = NT / 64, ROW_NT = 256;
+constexpr int ROW_NT = 256;
 constexpr int NEAR = 2048;             // sequences whose sums are kept in LDS
 constexpr int MOST = 1 << 30;          // positions of a sequence
 
@@ -52,32 +52,55 @@ __device__ __forceinline__ int search(const Array at, int n, int v) {
   return lo;
 }
 
+// the same for N values side by side, whose loads do not wait for each other
+template <int N, typename Array>
+__device__ __forceinline__ void search(const Array at, int n, const int (&v)[N], int (&lo)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) lo[i] = 0;
+  while (n > 1) {   // halves of one size for all: the second may begin inside the first
+    const int half = n >> 1;
+#pragma unroll
+    for (int i = 0; i < N; ++i) lo[i] = at[lo[i] + half] <= v[i] ? lo[i] + half : lo[i];
+    n -= half;
+  }
+}
+
 __device__ __forceinline__ int pages_for(const PagesArgs& a, int positions) {
   return min((positions + (1 << a.log2page) - 1) >> a.log2page, a.width);
 }
 
-// sum of v over the threads before this one, and of all
-template <typename T>
-__device__ __forceinline__ T scan(T v, T* waves, T& all) {
+// sums over the threads before this one, in place, and over all; one barrier before the next call's may begin
+struct Counts {
+  int back, taken;
+  int64_t rows;
+};
+template <int WAVES>
+__device__ __forceinline__ Counts scan(Counts& v, Counts (&waves)[WAVES]) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  T s = v;
+  Counts s = v;
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) {
-    const T up = __shfl_up(s, d);
-    if (lane >= d) s += up;
+    const Counts up{__shfl_up(s.back, d), __shfl_up(s.taken, d), __shfl_up(s.rows, d)};
+    if (lane >= d) {
+      s.back += up.back;
+      s.taken += up.taken;
+      s.rows += up.rows;
+    }
   }
   if (lane == 63) waves[wave] = s;
   __syncthreads();
-  T before = 0, total = 0;
+  // the waves' sums, one to a lane, and theirs up to each
+  Counts w = lane < WAVES ? waves[lane] : Counts{0, 0, 0};
+  const Counts own = waves[wave];
 #pragma unroll
-  for (int w = 0; w < WAVES; ++w) {
-    const T x = waves[w];
-    before += w < wave ? x : 0;
-    total += x;
+  for (int d = 1; d < WAVES; d <<= 1) {
+    const Counts up{__shfl_up(w.back, d), __shfl_up(w.taken, d), __shfl_up(w.rows, d)};
+    if (lane >= d) w = Counts{w.back + up.back, w.taken + up.taken, w.rows + up.rows};
   }
-  __syncthreads();
-  all = total;
-  return before + s - v;
+  auto at = [&](int l) { return Counts{__shfl(w.back, l), __shfl(w.taken, l), __shfl(w.rows, l)}; };
+  const Counts to = at(wave);
+  v = Counts{to.back - own.back + s.back - v.back, to.taken - own.taken + s.taken - v.taken, to.rows - own.rows + s.rows - v.rows};
+  return at(WAVES - 1);
 }
 
 // page i of those taken: sequence s, with `first` the number taken before it and p0 its first entry that is filled
@@ -104,88 +127,114 @@ __device__ __forceinline__ void row(const PagesArgs& a, const Cu cu, const Array
   if (page >= 0) slot = (static_cast<int64_t>(page) << a.log2page) + (pos & ((1 << a.log2page) - 1));
 }
 
+template <int NT>
 __global__ void __launch_bounds__(NT) plan_kernel(PagesArgs a) {
+  constexpr int WAVES = NT / 64;
   __shared__ int near_back[NEAR + 1], near_taken[NEAR + 1], near_cu[NEAR + 1];
-  __shared__ int waves[WAVES];
-  __shared__ int64_t waves64[WAVES];
+  __shared__ Counts counts[2][WAVES];   // two in turn, so that one barrier to a turn is enough
+  constexpr int EACH = 8;
+  __shared__ int valid[2][EACH * WAVES];
   const int tid = threadIdx.x;
   const bool near = a.batch <= NEAR;
   const int held0 = min(max(a.state[0], 0), a.pages);
-  int back = 0, taken = 0;
-  int64_t rows = 0;
-  for (int at = 0; at < a.batch; at += NT) {
+  Counts sum{0, 0, 0};
+  for (int at = 0, turn = 0; at < a.batch; at += NT, turn ^= 1) {
     const int b = at + tid;
-    int start = 0, end = 0, more = 0, gone = 0;
+    int start = 0, end = 0;
+    Counts mine{0, 0, 0};
     if (b < a.batch) {
-      const int len = min(max(a.lens[b], 0), MOST);
-      more = min(max(a.more[b], 0), MOST);
+      const int len = min(max(a.lens[b], 0), MOST), more = min(max(a.more[b], 0), MOST);
       const bool over = a.done && a.done[b];
-      gone = over ? pages_for(a, len) : 0;
       start = over ? 0 : len;
       end = min(start + more, MOST);
+      mine = Counts{over ? pages_for(a, len) : 0, max(pages_for(a, end) - pages_for(a, start), 0), more};
     }
-    const int need = max(pages_for(a, end) - pages_for(a, start), 0);
-    int all_back, all_taken;
-    int64_t all_rows;
-    const int x = back + scan(gone, waves, all_back), y = taken + scan(need, waves, all_taken);
-    const int64_t z = rows + scan(static_cast<int64_t>(more), waves64, all_rows);
+    const Counts all = scan(mine, counts[turn]);
     if (b < a.batch) {
-      const int c = static_cast<int>(min(z, static_cast<int64_t>(INT32_MAX)));
+      const int back = sum.back + mine.back, taken = sum.taken + mine.taken;
+      const int cu = static_cast<int>(min(sum.rows + mine.rows, static_cast<int64_t>(INT32_MAX)));
       a.lens[b] = end;
-      a.cu[b] = c;
+      a.cu[b] = cu;
       a.start[b] = start;
-      a.taken[b] = y;
       if (near) {
-        near_back[b] = x;
-        near_taken[b] = y;
-        near_cu[b] = c;
+        near_back[b] = back;
+        near_taken[b] = taken;
+        near_cu[b] = cu;
       } else {
-        a.back[b] = x;
+        a.back[b] = back;
       }
+      if (!near || !a.alone) a.taken[b] = taken;
     }
-    back += all_back;
-    taken += all_taken;
-    rows += all_rows;
+    sum = Counts{sum.back + all.back, sum.taken + all.taken, sum.rows + all.rows};
   }
+  const int back = sum.back, taken = sum.taken;
   if (tid == 0) {
-    const int c = static_cast<int>(min(rows, static_cast<int64_t>(INT32_MAX)));
-    a.cu[a.batch] = c;
+    const int cu = static_cast<int>(min(sum.rows, static_cast<int64_t>(INT32_MAX)));
+    a.cu[a.batch] = cu;
     a.taken[a.batch] = taken;
     if (near) {
       near_back[a.batch] = back;
       near_taken[a.batch] = taken;
-      near_cu[a.batch] = c;
+      near_cu[a.batch] = cu;
     } else {
       a.back[a.batch] = back;
     }
   }
   __syncthreads();
 
+  // what comes back: EACH entries to a thread, NT apart, so that neighbours' lie side by side. An entry's place on the list is counted
+  // over those before it: of earlier EACH, of earlier waves, of earlier lanes.
   int held = held0;
-  constexpr int EACH = 4;
-  for (int at = 0; at < back; at += NT * EACH) {
-    int entry[EACH], n = 0;
+  const int lane = tid & 63, wave = tid >> 6;
+  for (int at = 0, turn = 0; at < back; at += NT * EACH, turn ^= 1) {
+    int f[EACH], s[EACH], entry[EACH];
+    uint64_t there[EACH];
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) f[i] = min(at + NT * i + tid, back - 1);
+    near ? search(near_back, a.batch, f, s) : search(a.back, a.batch, f, s);
 #pragma unroll
     for (int i = 0; i < EACH; ++i) {
-      const int f = at + EACH * tid + i;
+      int32_t* e = a.table + s[i] * a.table_stride + (f[i] - (near ? near_back[s[i]] : a.back[s[i]]));
       entry[i] = -1;
-      if (f < back) {
-        const int s = near ? search(near_back, a.batch, f) : search(a.back, a.batch, f);
-        int32_t* e = a.table + s * a.table_stride + (f - (near ? near_back[s] : a.back[s]));
+      if (at + NT * i + tid < back) {
         entry[i] = *e;
         *e = -1;
       }
-      if (entry[i] < 0 || entry[i] >= a.pages) entry[i] = -1;
-      n += entry[i] >= 0;
     }
-    int all;
-    int to = held + scan(n, waves, all);
 #pragma unroll
-    for (int i = 0; i < EACH; ++i)
-      if (entry[i] >= 0) {
-        if (to < a.pages) a.free[to] = entry[i];
-        ++to;
-      }
+    for (int i = 0; i < EACH; ++i) {
+      there[i] = __builtin_amdgcn_ballot_w64(entry[i] >= 0 && entry[i] < a.pages);
+      if (lane == 0) valid[turn][i * WAVES + wave] = __popcll(there[i]);
+    }
+    __syncthreads();
+    // counts in order, PER to a lane, and their sums up to each
+    constexpr int PER = (EACH * WAVES + 63) / 64;
+    int n[PER], sum = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      n[i] = PER * lane + i < EACH * WAVES ? valid[turn][PER * lane + i] : 0;
+      sum += n[i];
+    }
+    int upto = sum;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int up = __shfl_up(upto, d);
+      if (lane >= d) upto += up;
+    }
+    const int all = __shfl(upto, 63);
+    int before[EACH];
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+      const int at = i * WAVES + wave, l = at / PER;
+      before[i] = __shfl(upto - sum, l);
+#pragma unroll
+      for (int j = 0; j + 1 < PER; ++j) before[i] += j < at % PER ? __shfl(n[j], l) : 0;
+    }
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+      const int to = held + before[i] + static_cast<int>(__popcll(there[i] & ((uint64_t{1} << lane) - 1)));
+      if ((there[i] >> lane & 1) && to < a.pages) a.free[to] = entry[i];
+    }
     held = min(held + all, a.pages);
   }
   if (tid == 0) {
@@ -276,8 +325,10 @@ extern "C" int rh3_kv_extend(const rh3_kv_extend_args* x, hipStream_t stream) {
   a.width = static_cast<int>(width);
   a.batch = static_cast<int>(batch);
   a.rows = static_cast<int>(rows);
-  a.alone = rows <= 4 * NT && batch <= NEAR;
-  hipLaunchKernelGGL(plan_kernel, dim3(1), dim3(NT), 0, stream, a);
+  // 1,024 threads for as long as one workgroup is enough for all, 256 where they would idle (each barrier is for all of them)
+  a.alone = rows <= 4096 && batch <= NEAR;
+  if (rows <= 1024 && batch <= 256) hipLaunchKernelGGL(plan_kernel<256>, dim3(1), dim3(256), 0, stream, a);
+  else hipLaunchKernelGGL(plan_kernel<1024>, dim3(1), dim3(1024), 0, stream, a);
   if (const int e = launch_status(name)) return e;
   if (a.alone) return RH3_OK;
   const int64_t all = rows + rows / page + batch, most = 8 * static_cast<int64_t>(device_cus() > 0 ? device_cus() : 256);
