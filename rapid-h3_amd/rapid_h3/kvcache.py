@@ -45,10 +45,10 @@ class KVCache:
     """The pages of one layer: k, v [P, heads, page, dim] int8 or float8_e4m3fn codes, k_scale, v_scale [P, heads, page]
     fp32 (page 16 to 256, a power of two; dim 64 or 128; views of larger buffers whose pages and heads lie apart are fine,
     k like v and k_scale like v_scale). 4-bit codes: k, v [P, heads, page, dim / 2] float4_e2m1fn_x2 or uint8, two codes to a byte, the
-    lower channel in the low half; k_scale, v_scale [P, heads, page, dim / 32] float8_e8m0fnu or uint8, e + 127. Where a position holds something, no code is NaN and a scale is finite and not
-    negative, or NaN for a row that is (as kv_write leaves them); of 4-bit codes, a scale byte is at most 252, or 255 in all of
-    k_scale's at a position whose key or value is not finite (NaN in both). The tensors are kept and used as they are; the attributes
-    cannot be changed."""
+    lower channel in the low half; k_scale, v_scale [P, heads, page, dim / 32] float8_e8m0fnu or uint8, e + 127. Where a position
+    holds something, no code is NaN and a scale is finite and not negative, or NaN for a row that is (as kv_write leaves them); of
+    4-bit codes, a scale byte is at most 252, or 255 in all of k_scale's at a position whose key or value is not finite (NaN in both).
+    The tensors are kept and used as they are; the attributes cannot be changed."""
 
     __slots__ = ("k", "v", "k_scale", "v_scale", "pages", "heads", "page", "dim", "device", "gpu", "_desc", "_ref")
 
@@ -155,6 +155,8 @@ def kv_extend(pool, table, lens, new, rows, done=None):
     if rows < 0:
         raise ValueError(f"{name}: {rows} rows")
     dev = table.device
+    if b == 0:
+        return torch.zeros(1, dtype=torch.int32, device=dev), *(torch.full((rows,), -1, dtype=t, device=dev) for t in (torch.int32, torch.int64))
     cu = torch.empty(b + 1, dtype=torch.int32, device=dev)
     positions = torch.empty(rows, dtype=torch.int32, device=dev)
     # the slots, with the workspace of 3 (b + 1) words behind them (16-byte aligned)

@@ -110,6 +110,14 @@ def test_no_rows(dev):
     assert cu.tolist() == [0, 0, 0] and positions.numel() == slots.numel() == 0 and pool.state.tolist() == [4, 0]
 
 
+def test_empty_batch(dev):
+    pool = kv.kv_pages(4, 16, dev)
+    none = torch.empty(0, dtype=torch.int32, device=dev)
+    cu, positions, slots = kv.kv_extend(pool, none.view(0, 3), none, none, 5)
+    assert cu.tolist() == [0] and positions.tolist() == slots.tolist() == [-1] * 5 and slots.dtype == torch.int64
+    assert pool.state.tolist() == [4, 0]
+
+
 def test_captured(dev):
     """A captured step goes on from what it finds on every replay."""
     pages, page, b, w = 60, 16, 6, 8

@@ -224,8 +224,6 @@ def test_rope_oracles_agree():
             a, b = (f(x, pos, freq, layout, 1.25, None, eps) for f in (orope.turned, orope.turned64))
             assert ((a.double() - b).abs() <= 1e-6 * (1 + b.abs())).all()
         y = orope.turned64(x, pos, freq, layout, 1.0, None, None)
-        for z in (x, y):
-            u, w, _ = orope._pairs(z.double(), 24, layout)
-            length = torch.hypot(u, w) if z is x else (torch.hypot(u, w) - length).abs().max()
-        assert length < 1e-12
+        before, after = (torch.hypot(*orope._pairs(z.double(), 24, layout)[:2]) for z in (x, y))
+        assert (before - after).abs().max() < 1e-12
         assert torch.equal(orope.turned(x, pos * 0, freq, layout, 1.0, None, None), x)
