@@ -198,15 +198,28 @@ struct Plan {
 // call, token / chunk, 8 K/V heads of 128, rows of a K/V head): 1 sequence of 16,384 keys: 32 rows 24 / 39, 96 41 / 49, 128 45 / 53,
 // 192 58 / 47, 256 67 / 53; 16 of 4,096: 32 50 / 66, 48 68 / 71, 64 82 / 73, 96 121 / 80; 4 of 65,536: 32 140 / 188, 48 285 / 197;
 // 4 of 1,024: 16 16 / 37, 256 24 / 49. Heads of 64: 1 of 65,536: 128 60 / 70, 192 81 / 80, 256 103 / 87; 4: 96 150 / 158, 128 186 / 169.
-Plan plan_of(int fmt, int64_t rows, int64_t batch, bool even, int64_t group, int64_t heads, int64_t dim, int64_t cap, bool keep, int form) {
+// In 4 bits (us a call, token / chunk, the same sizes, whole calls; fp16 in brackets, whose queries and probabilities are two terms):
+// 4 of 65,536: 16 rows 58 / 147, 32 76 / 151, 48 129 / 154 (140 / 208), 96 190 / 159 (209 / 226), 128 229 / 168 (259 / 243); 64 of
+// 2,048: 32 41 / 84, 64 71 / 83 (79 / 119), 96 102 / 86 (110 / 124); 1 of 16,384: 128 36 / 43. Heads of 64: 4 of 65,536: 32 57 / 105,
+// 64 96 / 107, 96 133 / 108; 64 of 2,048: 64 52 / 61, 96 75 / 62. As mb counts 8-bit codes.
+struct Cost {
+  double token, chunk, begin;    // rates of a pass over 16 or 32 rows, over 128, and what the chunk kernel takes longer beside them
+};
+Cost cost_of(int fmt, bool fine, int64_t dim) {
+  if (fmt != FP4) return Cost{6.8, 3.0, 34.0};
+  if (dim == 128) return Cost{9.8, fine ? 3.2 : 4.8, 14.0};
+  return Cost{7.0, fine ? 2.8 : 3.5, 9.0};
+}
+Plan plan_of(int fmt, bool fine, int64_t rows, int64_t batch, bool even, int64_t group, int64_t heads, int64_t dim, int64_t cap, bool keep, int form) {
   const int64_t cus = device_cus() > 0 ? device_cus() : 256;
   const int64_t mean = (rows * group + batch - 1) / batch;    // query rows of a sequence's K/V head
-  const int small = fmt != FP4 && dim == 64 && mean > 16 ? 32 : 16;
+  const int small = (fmt == FP4 || dim == 64) && mean > 16 ? 32 : 16;
   const double mb = 2e-6 * static_cast<double>(dim + 4) * static_cast<double>(batch * heads) * static_cast<double>(cap);
+  const Cost c = cost_of(fmt, fine, dim);
   Plan p{};
-  p.chunk = form != RH3_KV_BY_SIZE ? form == RH3_KV_CHUNK : static_cast<double>((mean + small - 1) / small) * mb / 6.8 > 34.0 + static_cast<double>((mean + 127) / 128) * mb / 3.0;
+  p.chunk = form != RH3_KV_BY_SIZE ? form == RH3_KV_CHUNK : static_cast<double>((mean + small - 1) / small) * mb / c.token > c.begin + static_cast<double>((mean + 127) / 128) * mb / c.chunk;
   p.rows = !p.chunk ? small : mean <= 128 ? 128 : 256;
-  p.wgs = static_cast<int>(p.rows == 256 ? cus : fmt == FP4 && !p.chunk ? 3 * cus : 2 * cus);
+  p.wgs = static_cast<int>(p.rows == 256 ? cus : p.rows == 16 && fmt == FP4 ? 3 * cus : 2 * cus);
   p.items = !keep ? 0 : heads * (even ? batch * ((rows / batch * group + p.rows - 1) / p.rows) : rows * group / p.rows + batch);
   p.slots = 2 * static_cast<int64_t>(p.wgs) + p.items;
   return p;
@@ -218,12 +231,12 @@ struct Call {
   bool joined;            // the prefix is a sequence of the one launch
   int64_t bytes;
 };
-Call call_of(int fmt, int64_t rows, int64_t q_heads, int64_t heads, int64_t dim, int64_t cap, int64_t batch, bool even, int64_t prefix_len, int form) {
+Call call_of(int fmt, bool fine, int64_t rows, int64_t q_heads, int64_t heads, int64_t dim, int64_t cap, int64_t batch, bool even, int64_t prefix_len, int form) {
   Call c{};
   const int64_t group = q_heads / heads;
-  c.own = plan_of(fmt, rows, batch, even, group, heads, dim, cap, prefix_len > 0, form);
+  c.own = plan_of(fmt, fine, rows, batch, even, group, heads, dim, cap, prefix_len > 0, form);
   if (prefix_len > 0) {
-    c.prefix = plan_of(fmt, rows, 1, true, group, heads, dim, prefix_len, true, form);
+    c.prefix = plan_of(fmt, fine, rows, 1, true, group, heads, dim, prefix_len, true, form);
     c.joined = c.own.chunk == c.prefix.chunk;   // the prefix's rows then go by the sequences' tiles
     if (c.joined) {
       const int64_t items = heads * ((rows * group + c.own.rows - 1) / c.own.rows);
@@ -238,7 +251,7 @@ Call call_of(int fmt, int64_t rows, int64_t q_heads, int64_t heads, int64_t dim,
 }
 
 void launch(const AttnArgs& a, const Plan& p, int fmt, int dim, hipStream_t st) {
-  if (fmt == FP4) p.chunk ? launch_chunk4(a, dim, p.rows, st) : launch_token4(a, dim, st);
+  if (fmt == FP4) p.chunk ? launch_chunk4(a, dim, p.rows, st) : launch_token4(a, dim, p.rows, st);
   else if (p.chunk) launch_chunk(a, fmt, dim, p.rows, st);
   else launch_token(a, fmt, dim, p.rows, st);
 }
@@ -255,10 +268,14 @@ extern "C" int64_t rh3_kv_attention_workspace_bytes(int64_t q_heads, int64_t hea
   if (heads < 1 || heads > 65535 || q_heads < heads || q_heads % heads || rows < 1 || rows > MAX_ROWS || q_heads / heads > MAX_ROWS / rows ||
       batch < 1 || batch > 65536 || capacity < 1 || capacity > MAX_ROWS || prefix_len < 0 || prefix_len > MAX_ROWS || (dim != 64 && dim != 128))
     return 0;
-  // enough for a cache of either width of codes
-  const int64_t eight = call_of(INT8, rows, q_heads, heads, dim, capacity, batch, even != 0, prefix_len, form).bytes;
-  const int64_t four = call_of(FP4, rows, q_heads, heads, dim, capacity, batch, even != 0, prefix_len, form).bytes;
-  return eight > four ? eight : four;
+  // enough for a cache of either width of codes, and queries of either type
+  int64_t most = 0;
+  for (const int fmt : {INT8, FP4})
+    for (const bool fine : {false, true}) {
+      const int64_t n = call_of(fmt, fine, rows, q_heads, heads, dim, capacity, batch, even != 0, prefix_len, form).bytes;
+      most = n > most ? n : most;
+    }
+  return most;
 }
 
 extern "C" int rh3_kv_attention(const rh3_kv_cache* cache, const void* q, int64_t q_st, int64_t q_sh, int64_t q_heads, int dtype,
@@ -284,7 +301,7 @@ extern "C" int rh3_kv_attention(const rh3_kv_cache* cache, const void* q, int64_
               static_cast<long long>(prefix_len));
   RH3_REQUIRE(form >= RH3_KV_BY_SIZE && form <= RH3_KV_CHUNK, "kv_attention: form %d", form);
   const int dim = static_cast<int>(cache->dim), fmt = static_cast<int>(cache->format);
-  const Call call = call_of(fmt, rows, q_heads, a.c.heads, dim, width * cache->page, batch, cu == nullptr, prefix_len, form);
+  const Call call = call_of(fmt, dtype == RH3_DTYPE_F16, rows, q_heads, a.c.heads, dim, width * cache->page, batch, cu == nullptr, prefix_len, form);
   RH3_REQUIRE(workspace && aligned16(workspace) && workspace_bytes >= call.bytes,
               "kv_attention: workspace of %lld bytes needed, %lld given", static_cast<long long>(call.bytes), static_cast<long long>(workspace_bytes));
   // Parts that a row may have: the workgroups over the least count of items, no more than the keys make. Measured (kernel us, by

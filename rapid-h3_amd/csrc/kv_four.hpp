@@ -76,7 +76,7 @@ __device__ __forceinline__ float reference_over(float top) { return top + OVER; 
 constexpr float PART_UP = 0x1p24f;
 
 // host: launches of the two kernels for their checked arguments
-void launch_token4(const AttnArgs& a, int dim, hipStream_t st);
+void launch_token4(const AttnArgs& a, int dim, int rows, hipStream_t st);
 void launch_chunk4(const AttnArgs& a, int dim, int rows, hipStream_t st);
 
 }  // namespace kv

@@ -14,7 +14,7 @@ namespace rh3 {
 namespace kv {
 namespace {
 
-constexpr int WAVES = 4, NT = WAVES * 64, R = 16;
+constexpr int WAVES = 4, NT = WAVES * 64;
 
 template <int D>
 struct Tile {
@@ -129,75 +129,85 @@ __device__ __forceinline__ void exchange(const uint2 (&v)[D / 64], uint32_t (&w)
   }
 }
 
-// one wave's running state for 16 query rows (row l % 16)
-template <int D>
+// one wave's running state for MT x 16 query rows (row l % 16 of each)
+template <int D, int MT>
 struct State {
-  f4_t o[D / 16];   // o[i][r]: channel channel_of(4 (l / 16) + r) + i
-  float ref, sum;
+  f4_t o[MT][D / 16];   // o[m][i][r]: channel channel_of(4 (l / 16) + r) + i
+  float ref[MT], sum[MT];
 };
 
 // One tile. FINE: fp16 queries, in two terms. The wave's next tile (nt, pages pn) is loaded into the same registers, its keys as soon
 // as these are used, its values as soon as theirs are. (The last turn loads its own tile again: loads that are only sometimes there
 // would be waited for at once.)
-template <int D, bool FINE, bool SMALL>
-__device__ __forceinline__ void compute(const AttnArgs& a, Tile<D>& t, int tile, const Pages<SMALL>& pg, const b8_t (&q)[D / 32],
-                                        const b8_t (&ql)[D / 32], int lim, int low, int len, const uint8_t* const (&head)[4], int nt, const Pages<SMALL>& pn, State<D>& st) {
+template <int D, int MT, bool FINE, bool SMALL>
+__device__ __forceinline__ void compute(const AttnArgs& a, Tile<D>& t, int tile, const Pages<SMALL>& pg, const b8_t (&q)[MT][D / 32],
+                                        const b8_t (&ql)[MT][D / 32], const int (&lim)[MT], int low, int len, const uint8_t* const (&head)[4], int nt,
+                                        const Pages<SMALL>& pn, State<D, MT>& st) {
   const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
   const int kb = tile * TOKEN_KEYS;
   // low: keys that every row sees
   const bool edge = kb + TOKEN_KEYS > low || pg.of(0) < 0 || pg.of(1) < 0;
-  f4_t acc[2];
+  f4_t acc[MT][2];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    acc[h] = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int m = 0; m < MT; ++m) acc[m][h] = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
     const float s = __uint_as_float(t.ks[h] << 23);
 #pragma unroll
     for (int c = 0; c < D / 32; ++c) {
       const b8_t k = values4(t.k[h][c], s);
-      acc[h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, q[c], acc[h], 0, 0, 0);
-      if constexpr (FINE) acc[h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, ql[c], acc[h], 0, 0, 0);
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        acc[m][h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, q[m][c], acc[m][h], 0, 0, 0);
+        if constexpr (FINE) acc[m][h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, ql[m][c], acc[m][h], 0, 0, 0);
+      }
     }
   }
   load_keys<D, SMALL>(a, head, nt, pn, t);
   auto key = [&](int j) { return kb + 16 * (j >> 2) + 4 * g + (j & 3); };
   auto hidden = [&](int j, int end) { return key(j) >= end || pg.of(j >> 2) < 0; };
-  // scores less the reference, which is finite: before a row's first key it is the lowest number
-  float y[8];
+  b8_t p[MT], rest[MT];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) y[j] = fmaf(acc[j >> 2][j & 3], a.scale_log2, -st.ref);
-  if (edge) {
+  for (int m = 0; m < MT; ++m) {
+    // scores less the reference, which is finite: before a row's first key it is the lowest number
+    float y[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) y[j] = hidden(j, lim) ? -INFINITY : y[j];
-  }
-  float top = y[0];
+    for (int j = 0; j < 8; ++j) y[j] = fmaf(acc[m][j >> 2][j & 3], a.scale_log2, -st.ref[m]);
+    if (edge) {
 #pragma unroll
-  for (int j = 1; j < 8; ++j) top = fmaxf(top, y[j]);
-  if (__builtin_amdgcn_ballot_w64(top > STALE)) {
-    float n = -INFINITY;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      y[j] = edge && hidden(j, lim) ? -INFINITY : acc[j >> 2][j & 3] * a.scale_log2;
-      n = fmaxf(n, y[j]);
+      for (int j = 0; j < 8; ++j) y[j] = hidden(j, lim[m]) ? -INFINITY : y[j];
     }
-    n = across_max<true>(n);
-    const float to = n - st.ref > STALE ? reference_over(n) : st.ref;
-    const float f = __builtin_amdgcn_exp2f(st.ref - to);
-    st.ref = to;
-    st.sum *= f;
+    float top = y[0];
 #pragma unroll
-    for (int i = 0; i < D / 16; ++i) st.o[i] *= f;
+    for (int j = 1; j < 8; ++j) top = fmaxf(top, y[j]);
+    if (__builtin_amdgcn_ballot_w64(top > STALE)) {
+      float n = -INFINITY;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) y[j] -= to;
+      for (int j = 0; j < 8; ++j) {
+        y[j] = edge && hidden(j, lim[m]) ? -INFINITY : acc[m][j >> 2][j & 3] * a.scale_log2;
+        n = fmaxf(n, y[j]);
+      }
+      n = across_max<true>(n);
+      const float to = n - st.ref[m] > STALE ? reference_over(n) : st.ref[m];
+      const float f = __builtin_amdgcn_exp2f(st.ref[m] - to);
+      st.ref[m] = to;
+      st.sum[m] *= f;
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) st.o[m][i] *= f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) y[j] -= to;
+    }
+    uint32_t hi[4], lo[4];
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) {
+      const float e0 = __builtin_amdgcn_exp2f(y[j]), e1 = __builtin_amdgcn_exp2f(y[j + 1]);
+      st.sum[m] += e0 + e1;
+      hi[j / 2] = pack_bf2(e0, e1);
+      lo[j / 2] = pack_bf2(e0 - __uint_as_float(hi[j / 2] << 16), e1 - __uint_as_float(hi[j / 2] & 0xffff0000u));
+    }
+    p[m] = bf16x8(hi[0], hi[1], hi[2], hi[3]);
+    rest[m] = bf16x8(lo[0], lo[1], lo[2], lo[3]);
   }
-  uint32_t hi[4], lo[4];
-#pragma unroll
-  for (int j = 0; j < 8; j += 2) {
-    const float e0 = __builtin_amdgcn_exp2f(y[j]), e1 = __builtin_amdgcn_exp2f(y[j + 1]);
-    st.sum += e0 + e1;
-    hi[j / 2] = pack_bf2(e0, e1);
-    lo[j / 2] = pack_bf2(e0 - __uint_as_float(hi[j / 2] << 16), e1 - __uint_as_float(hi[j / 2] & 0xffff0000u));
-  }
-  const b8_t p = bf16x8(hi[0], hi[1], hi[2], hi[3]), rest = bf16x8(lo[0], lo[1], lo[2], lo[3]);
 
   // the scale byte of the lane's group to where a float's exponent is; what lies beside it is not looked at
   const int group = channel_of<D>(l16) / GROUP4;
@@ -234,8 +244,11 @@ __device__ __forceinline__ void compute(const AttnArgs& a, Tile<D>& t, int tile,
       const uint32_t sel = e ? 0x07060302u : 0x05040100u;
       const b8_t x = bf16x8(__builtin_amdgcn_perm(w[1], w[0], sel), __builtin_amdgcn_perm(w[3], w[2], sel),
                             __builtin_amdgcn_perm(w[5], w[4], sel), __builtin_amdgcn_perm(w[7], w[6], sel));
-      st.o[2 * c + e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, p, st.o[2 * c + e], 0, 0, 0);
-      st.o[2 * c + e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, rest, st.o[2 * c + e], 0, 0, 0);
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        st.o[m][2 * c + e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, p[m], st.o[m][2 * c + e], 0, 0, 0);
+        st.o[m][2 * c + e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, rest[m], st.o[m][2 * c + e], 0, 0, 0);
+      }
     }
   };
   load_values<D, SMALL>(a, head, nt, pn, t);
@@ -299,9 +312,9 @@ struct Listed {
   }
 };
 
-template <int D, bool FINE, bool SMALL>
-__global__ void __launch_bounds__(NT, 3) token_kernel(AttnArgs a) {
-  constexpr int PAD = D + 4;
+template <int D, int MT, bool FINE, bool SMALL>
+__global__ void __launch_bounds__(NT, MT == 1 ? 3 : 2) token_kernel(AttnArgs a) {
+  constexpr int R = 16 * MT, PAD = D + 4;
   const Tiling TILING = tiling(false, R);
   __shared__ float so[WAVES][R][PAD];
   __shared__ float sm[WAVES][R], sl[WAVES][R];
@@ -339,13 +352,17 @@ __global__ void __launch_bounds__(NT, 3) token_kernel(AttnArgs a) {
     // query rows: lane l holds row l % 16, channels (dim / 4) (l / 16) + 8 c + 0 .. 7 in step c
     int t = t0 + wave;
     Pages<SMALL> pg = pages_of<SMALL>(a, row, width, t), pn = pages_of<SMALL>(a, row, width, t + WAVES);
-    const int mine = rt * R + l16, rr = mine < rows ? mine : 0;
-    const int tok = rr / a.group, hd = kvh * a.group + rr - tok * a.group;
-    uint4 raw[D / 32];
-    const uint16_t* src = static_cast<const uint16_t*>(a.q) + (sq.first + tok) * a.q_st + hd * a.q_sh + (D / 4) * g;
+    uint4 raw[MT][D / 32];
+    int lim[MT];
 #pragma unroll
-    for (int c = 0; c < D / 32; ++c) raw[c] = *reinterpret_cast<const uint4*>(src + 8 * c);
-    const int lim = causal ? min(sq.len, sq.pos + tok + 1) : sq.len;
+    for (int m = 0; m < MT; ++m) {
+      const int mine = rt * R + 16 * m + l16, rr = mine < rows ? mine : 0;
+      const int tok = rr / a.group, hd = kvh * a.group + rr - tok * a.group;
+      const uint16_t* src = static_cast<const uint16_t*>(a.q) + (sq.first + tok) * a.q_st + hd * a.q_sh + (D / 4) * g;
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c) raw[m][c] = *reinterpret_cast<const uint4*>(src + 8 * c);
+      lim[m] = causal ? min(sq.len, sq.pos + tok + 1) : sq.len;
+    }
     // the first keys and values are on their way while the query rows come in
     Tile<D> tile;
     const int64_t codes = kvh * a.c.head_stride, scales = kvh * a.c.shead_stride;
@@ -355,35 +372,44 @@ __global__ void __launch_bounds__(NT, 3) token_kernel(AttnArgs a) {
       load_keys<D, SMALL>(a, head, t, pg, tile);
       load_values<D, SMALL>(a, head, t, pg, tile);
     }
-    b8_t q[D / 32], ql[D / 32];
+    b8_t q[MT][D / 32], ql[MT][D / 32];
 #pragma unroll
-    for (int c = 0; c < D / 32; ++c) query8<FINE>(mine < rows ? raw[c] : make_uint4(0, 0, 0, 0), q[c], ql[c]);
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c) query8<FINE>(rt * R + 16 * m + l16 < rows ? raw[m][c] : make_uint4(0, 0, 0, 0), q[m][c], ql[m][c]);
     const int low = causal ? min(sq.len, sq.pos + scalar((rt * R) / a.group) + 1) : sq.len;
 
-    State<D> st;
-    st.ref = NO_REF;
-    st.sum = 0.0f;
+    State<D, MT> st;
 #pragma unroll
-    for (int i = 0; i < D / 16; ++i) st.o[i] = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int m = 0; m < MT; ++m) {
+      st.ref[m] = NO_REF;
+      st.sum[m] = 0.0f;
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) st.o[m][i] = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    }
     while (t < t1) {
       const Pages<SMALL> p2 = pages_of<SMALL>(a, row, width, t + 2 * WAVES);
       const bool more = t + WAVES < t1;
-      compute<D, FINE, SMALL>(a, tile, t, pg, q, ql, lim, low, sq.len, head, more ? t + WAVES : t, more ? pn : pg, st);
+      compute<D, MT, FINE, SMALL>(a, tile, t, pg, q, ql, lim, low, sq.len, head, more ? t + WAVES : t, more ? pn : pg, st);
       pg = pn;
       pn = p2;
       t += WAVES;
     }
     // join the waves
-    const float mysum = across_sum<true>(st.sum);
-    if (g == 0) {
-      sm[wave][l16] = st.ref;
-      sl[wave][l16] = mysum;
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      const float sum = across_sum<true>(st.sum[m]);
+      if (g == 0) {
+        sm[wave][16 * m + l16] = st.ref[m];
+        sl[wave][16 * m + l16] = sum;
+      }
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int i = 0; i < D / 16; i += 4)
+          *reinterpret_cast<float4*>(&so[wave][16 * m + l16][channel_of<D>(4 * g + r) + i]) =
+              make_float4(st.o[m][i][r], st.o[m][i + 1][r], st.o[m][i + 2][r], st.o[m][i + 3][r]);
     }
-#pragma unroll
-    for (int r = 0; r < 4; ++r)
-#pragma unroll
-      for (int i = 0; i < D / 16; i += 4)
-        *reinterpret_cast<float4*>(&so[wave][l16][channel_of<D>(4 * g + r) + i]) = make_float4(st.o[i][r], st.o[i + 1][r], st.o[i + 2][r], st.o[i + 3][r]);
     __syncthreads();
     const bool whole = t0 == 0 && u1 == sw.span;
     constexpr int TPR = NT / R, EPT = D / TPR;   // threads to a row, channels to a thread
@@ -429,11 +455,18 @@ __global__ void __launch_bounds__(NT, 3) token_kernel(AttnArgs a) {
 
 }  // namespace
 
-void launch_token4(const AttnArgs& a, int dim, hipStream_t st) {
+void launch_token4(const AttnArgs& a, int dim, int rows, hipStream_t st) {
   auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(a.wgs)), dim3(NT), 0, st, a); };
-  auto by = [&](auto small, auto large) { a.c.log2page == 4 ? go(small) : go(large); };
-  if (dim == 128) a.fp16 ? by(token_kernel<128, true, true>, token_kernel<128, true, false>) : by(token_kernel<128, false, true>, token_kernel<128, false, false>);
-  else a.fp16 ? by(token_kernel<64, true, true>, token_kernel<64, true, false>) : by(token_kernel<64, false, true>, token_kernel<64, false, false>);
+  auto by_page = [&](auto small, auto large) { a.c.log2page == 4 ? go(small) : go(large); };
+  auto by_type = [&](auto D, auto MT) {
+    constexpr int d = decltype(D)::value, m = decltype(MT)::value;
+    if (a.fp16) by_page(token_kernel<d, m, true, true>, token_kernel<d, m, true, false>);
+    else by_page(token_kernel<d, m, false, true>, token_kernel<d, m, false, false>);
+  };
+  using One = std::integral_constant<int, 1>;
+  using Two = std::integral_constant<int, 2>;
+  if (dim == 128) rows == 16 ? by_type(std::integral_constant<int, 128>(), One()) : by_type(std::integral_constant<int, 128>(), Two());
+  else rows == 16 ? by_type(std::integral_constant<int, 64>(), One()) : by_type(std::integral_constant<int, 64>(), Two());
 }
 
 }  // namespace kv
