@@ -1,16 +1,17 @@
-// Writing rows of keys and values into a paged cache as INT8 or e4m3 codes with one fp32 scale per row and head, and reading
-// them back.
+// Writing rows of keys and values into a paged cache as INT8 or e4m3 codes with one fp32 scale per row and head, or as 4-bit codes
+// with a power of two to 32 channels, and reading them back.
 //
 // s = max(amax / QMAX, 1e-12) (QMAX 127 or 448), code = round to nearest even of the fp32 quotient x / s: the rule of the row
 // quantizers, over the 64 or 128 values of one head. A row that holds an infinity or a NaN gets s = NaN and codes 0: it reads
-// back as NaN and every attention row that sees it is NaN, while no code of the cache is ever a NaN.
+// back as NaN and every attention row that sees it is NaN, while no code of the cache is ever a NaN. (4 bits: kv_four.hpp.)
 //
-// Both are bound by memory. A row of a head is 8 values in each of dim / 8 lanes (16-byte loads of 16-bit rows, 8 bytes of codes);
-// a workgroup takes 256 / (dim / 8) consecutive rows of one head after another, so that the codes it writes (a page holds a
-// head's positions back to back) and its scales are whole lines, while each read of a row is dim consecutive values.
-// Measured, K and V of 22,332 rows x 56 heads of 128, bf16 and e4m3 (0.97 GB each way; a large copy moves 4.8 TB/s): written in
-// 237 us (4.1 TB/s, the vector units 55 % busy), read back in 184 us (5.3 TB/s); 8 x 7,919 rows x 16 heads int8 (0.79 GB)
-// read back in 160 to 187 us. 16 rows of 8 heads: 3.9 and 2.8 us, the length of a few dependent loads.
+// Both are bound by memory. A row of a head is 8 values in each of dim / 8 lanes (16-byte loads of 16-bit rows, 8 or 4 bytes of
+// codes); a workgroup takes 256 / (dim / 8) consecutive rows of one head after another, so that the codes it writes (a page holds a
+// head's positions back to back) and its scales are whole lines, while each read of a row is dim consecutive values. Rows of more
+// than the last cache's 256 MB are streamed past it (in 4 bits read back 178 -> 127 us: the codes stay in it; written 167 -> 160).
+// Measured, K and V of 22,332 rows x 56 heads of 128, bf16 (a large copy moves 5.1 TB/s): 4 bits (0.81 GB each way) written in 160 us
+// (5.1 TB/s), read back in 126 (6.4); e4m3 (0.97 GB) written in 220 us (4.4), read back in 190 (5.1); 8 x 7,919 rows x 16 heads
+// int8 (0.79 GB) read back in 166 us. 16 rows of 8 heads: 3.9 and 2.8 us, the length of a few dependent loads.
 #include "kv_rows.hpp"
 
 namespace rh3 {

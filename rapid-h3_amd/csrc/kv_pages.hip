@@ -8,9 +8,10 @@
 // All of it is prefix sums over the sequences and searches in them, so the result is the same in every run.
 //
 // Bound by latency: a step moves 9 bytes a sequence, 12 a row and 8 a page. The sums need one workgroup: it makes them, walks the
-// pages that come back (4 entries to a thread at a time, in order) and, of small calls, does the rest too; of large ones a second
+// pages that come back (8 entries to a thread at a time, in order) and, of small calls, does the rest too; of large ones a second
 // launch spreads the pages taken and the rows over the chip. A page that is taken is looked up in the list, not in the table, which
-// the same launch is writing.
+// the same launch is writing. Measured: 16 sequences, a row each, 5.8 us; 700 sequences, 9,000 pages back, 8,000 taken, 130,000
+// rows 10.9 + 4 to 5.5 us (with each entry's search on its own 15.4 + 5.3).
 #include "kv_common.hpp"
 
 namespace rh3 {
