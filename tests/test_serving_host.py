@@ -41,7 +41,8 @@ def _write_rope(desc=None, **kw):
     d = dict(zip(WRITE, (FAKE, 1024, 128, FAKE, 1024, 128, FAKE, 512, 128, FAKE, 512, 128, 8, 1, 6, FAKE, 8, 8, FAKE, 0, 2, 0, FAKE, 128, 0, 1.0, 1,
                          1e-6, FAKE, FAKE, 0)))
     d.update(kw)
-    return nat.lib().rh3_kv_write_rope(ctypes.addressof(desc or _desc()), kv._WRITE_ROPE.pack(*d.values()), None)
+    desc = desc or _desc()                      # held until the call returns
+    return nat.lib().rh3_kv_write_rope(ctypes.addressof(desc), kv._WRITE_ROPE.pack(*d.values()), None)
 
 
 EXTEND = "free pages state page table table_stride width lens more done batch cu positions slots rows ws n".split()
