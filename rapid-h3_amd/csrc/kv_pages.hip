@@ -125,7 +125,7 @@ __device__ __forceinline__ void row(const PagesArgs& a, const Cu cu, const Array
   const int p = pos >> a.log2page, p0 = pages_for(a, start);
   if (p >= a.width) return;
   const int page = p < p0 ? a.table[s * a.table_stride + p] : taken_page(a, held, taken[s] + p - p0);
-  if (page >= 0) slot = (static_cast<int64_t>(page) << a.log2page) + (pos & ((1 << a.log2page) - 1));
+  if (page >= 0 && page < a.pages) slot = (static_cast<int64_t>(page) << a.log2page) + (pos & ((1 << a.log2page) - 1));
 }
 
 template <int NT>

@@ -103,6 +103,19 @@ def test_bad_contents_stay_inside(dev):
     assert all((whole[a:z] == 99).all() for a, z in ((0, 4), (10, 12), (14, 20), (32, 40), (44, 64)))
 
 
+def test_slots_of_no_page(dev):
+    """Entries of the table and of the pool that are no pages are places to none: slots stay inside the cache."""
+    page = 16
+    pool = kv.KVPages(_i32([9, 8, 4, 2], dev), _i32([3, 0], dev), page)      # taken: 4, 8, 9
+    table, lens = _i32([[3, 4, -1, -1], [1, -1, -1, -1], [7, -1, -1, -1]], dev), _i32([20, 16, 2], dev)
+    cu, positions, slots = kv.kv_extend(pool, table, lens, _i32([20, 20, 2], dev), 43)
+    # sequence 0: positions 20 to 31 in page 4, which is none, 32 to 39 in the pool's 4, none; 1: in 8 and 9, none; 2: in 7, none
+    assert positions.tolist() == [*range(20, 40), *range(16, 36), 2, 3, -1] and slots.tolist() == [-1] * 43
+    lens.copy_(_i32([3, 16, 2], dev))
+    _, _, slots = kv.kv_extend(pool, table, lens, _i32([2, 0, 0], dev), 2)
+    assert slots.tolist() == [3 * page + 3, 3 * page + 4]
+
+
 def test_no_rows(dev):
     pool = kv.kv_pages(4, 16, dev)
     table, lens = torch.full((2, 2), -1, dtype=torch.int32, device=dev), torch.zeros(2, dtype=torch.int32, device=dev)
@@ -202,3 +215,52 @@ def test_a_served_batch(dev, fmt, graphs):
         tol = 2.0 ** -8 * 1.01 * ref.abs() + (weight + torch.expm1(2 * err)[..., None]) * mag * 1.05 + 1e-30
         assert ((out[:t].double() - ref).abs() <= tol).all()
         assert ((lse[:t].double() - rl).abs() <= err + 2.0 ** -22 * rl.abs() + 2.0 ** -20).all()
+
+
+def test_two_graphs_and_a_stream_of_its_own(dev):
+    """Steps of two batches, captured each in a graph of one memory pool, replayed in turn on a stream that is not theirs, with eager
+    steps of a third between: every one as if it were alone."""
+    hq, hkv, dim, page, room, b = 8, 2, 64, 16, 40, 3
+    turn = rope.rotary(dim, "interleaved", dev)
+
+    class Batch:
+        def __init__(self, seed):
+            g = torch.Generator().manual_seed(seed)
+            self.cache, self.pool = kv.kv_cache(40, hkv, page, dim, torch.float4_e2m1fn_x2, dev), kv.kv_pages(40, page, dev)
+            self.table, self.lens = torch.full((b, 8), -1, dtype=torch.int32, device=dev), torch.zeros(b, dtype=torch.int32, device=dev)
+            self.new = torch.zeros(b, dtype=torch.int32, device=dev)
+            self.rows = [torch.randn(room, h, dim, generator=g).to(torch.bfloat16).to(dev) for h in (hq, hkv, hkv)]
+
+        def step(self):
+            cu, positions, slots = kv.kv_extend(self.pool, self.table, self.lens, self.new, room)
+            q = kv.kv_write_rope(self.cache, *self.rows, self.table, self.lens, cu, turn)
+            return positions, slots, q, kv.kv_attention(q, self.cache, self.table, self.lens, cu)
+    counts = [[9, 30, 1], [1, 1, 1], [0, 17, 2], [1, 1, 1]]
+    want = {}
+    for seed in range(3):
+        x = Batch(seed)
+        for i, n in enumerate(counts):
+            x.new.copy_(_i32(n, dev))
+            want[seed, i] = [t.clone() for t in x.step()]
+    torch.cuda.synchronize()
+
+    batches, graphs, outs = [Batch(seed) for seed in range(3)], [], []
+    for x in batches[:2]:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, pool=graphs[0].pool() if graphs else None):
+            outs.append(x.step())
+        graphs.append(graph)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for i, n in enumerate(counts):
+            for seed, x in enumerate(batches):
+                x.new.copy_(_i32(n, dev))
+                if seed < 2:
+                    graphs[seed].replay()
+                    got = outs[seed]
+                else:
+                    got = x.step()
+                side.synchronize()
+                for t, w in zip(got, want[seed, i]):
+                    assert torch.equal(t, w), (seed, i)
