@@ -569,3 +569,27 @@ def test_bytes_and_named_types(dev):
     args = (_i32([[1]], dev), _i32([4], dev))
     kv.kv_write(d, x, x, *args)
     assert torch.equal(kv.kv_read(c, *args, rows=4)[0], ok.values4(*ok.quantise4(x)).to(BF))
+
+
+@pytest.mark.parametrize("fmt", [torch.int8, torch.float8_e4m3fn, torch.float4_e2m1fn_x2])
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_rows_beyond_the_last_cache(dev, fmt, dtype):
+    """Calls of so many rows that they are streamed leave what calls of parts of them leave, bit for bit."""
+    n, heads, dim, page = 9001, 64, 128, 64
+    pages = -(-n // page)
+    g = torch.Generator(device=dev).manual_seed(5)
+    k, v = (torch.randn(n, heads, dim, generator=g, device=dev).to(dtype) for _ in range(2))
+    table = torch.randperm(pages, generator=torch.Generator().manual_seed(6)).to(torch.int32).to(dev)[None]
+    one, parts = (kv.kv_cache(pages, heads, page, dim, fmt, dev) for _ in range(2))
+    kv.kv_write(one, k, v, table, _i32([n], dev))
+    step = 1000                          # 65 MB of 32-bit K and V
+    for at in range(0, n, step):
+        end = min(at + step, n)
+        kv.kv_write(parts, k[at:end], v[at:end], table, _i32([end], dev))
+    for x, y in zip((one.k, one.v, one.k_scale, one.v_scale), (parts.k, parts.v, parts.k_scale, parts.v_scale)):
+        assert torch.equal(x.view(torch.uint8), y.view(torch.uint8))
+    rk, rv = kv.kv_read(one, table, _i32([n], dev), rows=n, dtype=dtype)
+    for at in range(0, n, step):
+        end = min(at + step, n)
+        pk, pv = kv.kv_read(parts, table, _i32([end], dev), rows=end - at, dtype=dtype)
+        assert torch.equal(rk[at:end], pk) and torch.equal(rv[at:end], pv)

@@ -226,3 +226,28 @@ def test_bad_contents_stay_inside(dev):
         kv.kv_write_rope(c, q, k, v, _i32(table, dev), _i32(lens, dev), None if cu is None else _i32(cu, dev), rotary=turn)
     torch.cuda.synchronize()
     assert not c.k.any() and not c.k_scale.any()
+
+
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_rows_beyond_the_last_cache(dev, dtype, layout):
+    """Calls of so many rows that they are streamed leave what calls of parts of them leave, bit for bit."""
+    n, hq, hkv, dim, page = 9001, 96, 32, 128, 64
+    g = torch.Generator(device=dev).manual_seed(5)
+    q, k, v = (torch.randn(n, h, dim, generator=g, device=dev).to(dtype) for h in (hq, hkv, hkv))
+    turn = rope.rotary(96, layout, dev)
+    weight = (1 + 0.1 * torch.randn(dim, generator=g, device=dev)).to(dtype)
+    positions = torch.arange(n, dtype=torch.int32, device=dev)
+    gq, gk = rope.qk_norm_rope(q, k, positions, turn, weight, weight, 1e-6)
+    pages = -(-n // page)
+    table = torch.arange(pages, dtype=torch.int32, device=dev)[None]
+    cache, parts = (kv.kv_cache(pages, hkv, page, dim, FMT[2], dev) for _ in range(2))
+    wq = kv.kv_write_rope(cache, q, k, v, table, _i32([n], dev), None, turn, weight, weight, 1e-6)
+    assert torch.equal(wq, gq)
+    for at in range(0, n, 500):
+        end = min(at + 500, n)
+        pq, pk = rope.qk_norm_rope(q[at:end], k[at:end], positions[at:end].clone(), turn, weight, weight, 1e-6)
+        assert torch.equal(gq[at:end], pq) and torch.equal(gk[at:end], pk)
+        kv.kv_write(parts, pk, v[at:end], table, _i32([end], dev))
+    for x, y in zip((cache.k, cache.v, cache.k_scale, cache.v_scale), (parts.k, parts.v, parts.k_scale, parts.v_scale)):
+        assert torch.equal(x.view(torch.uint8), y.view(torch.uint8))
