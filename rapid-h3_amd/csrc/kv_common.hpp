@@ -51,7 +51,8 @@ struct Seq {
 constexpr int64_t MAX_ROWS = int64_t{1} << 30;   // of a call, and positions of a table
 
 RH3_HD int clamped(int v, int lo, int hi) { return v < lo ? lo : v > hi ? hi : v; }
-RH3_HD Seq seq_at(const Seqs& s, int b) {
+// row0: the position that row 0 of the call would have in the sequence, not clamped as `pos` is (to what the table can hold)
+RH3_HD Seq seq_at(const Seqs& s, int b, int64_t& row0) {
   Seq r;
   int64_t end;
   if (s.cu) {
@@ -64,15 +65,20 @@ RH3_HD Seq seq_at(const Seqs& s, int b) {
     end = r.first + r.n;
   }
   const int64_t len = s.lens[b], pos = len - end + r.first;
+  row0 = len - end;
   r.len = clamped(static_cast<int>(len), 0, s.cap);
   r.pos = static_cast<int>(pos < -MAX_ROWS ? -MAX_ROWS : pos > s.cap ? s.cap : pos);
   return r;
+}
+RH3_HD Seq seq_at(const Seqs& s, int b) {
+  int64_t row0;
+  return seq_at(s, b, row0);
 }
 
 // The sequence of a row: the last b with cu[b] <= row, by a search over LANES (8, 16 or 64) lanes that hold the same
 // row, or -1 for a row that no sequence has (behind the last one, or in a cu that does not rise).
 template <int LANES>
-__device__ __forceinline__ int seq_of_row(const Seqs& s, int row, Seq& q) {
+__device__ __forceinline__ int seq_of_row(const Seqs& s, int row, Seq& q, int64_t& row0) {
   int b;
   if (!s.cu) {
     b = row / s.per;
@@ -92,8 +98,13 @@ __device__ __forceinline__ int seq_of_row(const Seqs& s, int row, Seq& q) {
     }
     b = lo;
   }
-  q = seq_at(s, b);
+  q = seq_at(s, b, row0);
   return row >= q.first && row < q.first + q.n ? b : -1;
+}
+template <int LANES>
+__device__ __forceinline__ int seq_of_row(const Seqs& s, int row, Seq& q) {
+  int64_t row0;
+  return seq_of_row<LANES>(s, row, q, row0);
 }
 
 // page of a position of sequence b (pos < cap), or -1

@@ -222,7 +222,7 @@ __global__ void __launch_bounds__(NT) rope_kernel(RopeArgs a) {
       }
     } else {
       // a token's position is known to its own lanes, those of all its heads
-      const double pos = static_cast<double>(static_cast<int64_t>(place.pos) + a.first);
+      const double pos = static_cast<double>(place.pos + a.first);
       for (int f = hs * LPR + l; f < half; f += heads_at_once * LPR) turns[tok][f] = cos_sin(pos * t.freq[f], t.factor);
     }
     __syncthreads();

@@ -13,21 +13,22 @@ constexpr int NT = 256;
 // (no sequence has the row, its position is before the first or past the table, its page is absent). `mine`: a sequence has the row.
 struct Place {
   int64_t code, scale;
-  int pos;          // of a row that is `mine`
+  int64_t pos;      // of a row that is `mine`, wherever that is: a sequence's rows have their positions past the table's end too
   bool mine, there;
 };
 template <int FMT, int D>
 __device__ __forceinline__ Place place_of(const Seqs& s, const Cache& c, int row) {
   Place p{0, 0, 0, false, false};
   Seq q;
-  const int b = seq_of_row<D / 8 == 16 ? 16 : 8>(s, min(row, s.rows - 1), q);
+  int64_t row0;
+  const int b = seq_of_row<D / 8 == 16 ? 16 : 8>(s, min(row, s.rows - 1), q, row0);
   if (b < 0 || row >= s.rows) return p;
   p.mine = true;
-  p.pos = q.pos + (row - q.first);
+  p.pos = row0 + row;
   if (p.pos < 0 || p.pos >= s.cap) return p;
-  const int pg = page_of(s, c, b, p.pos);
+  const int pos = static_cast<int>(p.pos), pg = page_of(s, c, b, pos);
   if (pg < 0) return p;
-  const int off = p.pos & ((1 << c.log2page) - 1);
+  const int off = pos & ((1 << c.log2page) - 1);
   p.code = pg * c.page_stride + off * (FMT == FP4 ? D / 2 : D);
   p.scale = pg * c.spage_stride + off * (FMT == FP4 ? D / GROUP4 : 1);
   p.there = true;

@@ -175,6 +175,36 @@ def test_write_rope_is_both(dev, fmt, dtype, hq, hkv, dim, page, lens, new, rot,
     assert torch.equal(x[mine], wq[mine]) and torch.equal(x[~mine], q[~mine])
 
 
+@pytest.mark.parametrize("fmt", FMT)
+@pytest.mark.parametrize("ragged", [False, True])
+@pytest.mark.parametrize("first", [0, 777])
+def test_rows_past_the_table_turn_by_their_positions(dev, fmt, ragged, first):
+    """Sequences that have outgrown their tables: rows that begin behind the last page, or in it and go on behind it, are written
+    nowhere, and their queries turn by the positions that kv_extend gives them, however the rows are split over calls."""
+    hq, hkv, dim, page = 4, 2, 64, 16
+    had, new = ([95, 10, 3, 1 << 29], [5, 10, 4, 3]) if ragged else ([95, 10, 3, 1 << 29], [4] * 4)
+    b, t = len(new), sum(new)
+    pool = kv.kv_pages(8, page, dev)
+    table, lens = _i32([[p] for p in range(b)], dev), _i32(had, dev)
+    cu, positions, slots = kv.kv_extend(pool, table, lens, _i32(new, dev), t)
+    assert positions.tolist() == [p for n, m in zip(had, new) for p in range(n, n + m)]
+    q, k, v = _rows(t, [hq, hkv, hkv], dim, BF, 5, dev)
+    turn = rope.rotary(dim, "half", dev)
+    one, two, parts = (kv.kv_cache(8, hkv, page, dim, fmt, dev) for _ in range(3))
+    got = kv.kv_write_rope(one, q, k, v, table, lens, cu if ragged else None, turn, eps=1e-6, first=first)
+    wq, wk = rope.qk_norm_rope(q, k, positions + first, turn, eps=1e-6)
+    assert torch.equal(got, wq)
+    kv.kv_write(two, wk, v, table, lens, cu if ragged else None)
+    bounds = cu.tolist()
+    for i, n in enumerate(had):                  # one row to a call
+        for j in range(new[i]):
+            r = bounds[i] + j
+            x = kv.kv_write_rope(parts, q[r:r + 1], k[r:r + 1], v[r:r + 1], table[i:i + 1], _i32([n + j + 1], dev), None, turn, eps=1e-6, first=first)
+            assert torch.equal(x, wq[r:r + 1]), (i, j)
+    for x, y, z in zip(*((c.k, c.v, c.k_scale, c.v_scale) for c in (one, two, parts))):
+        assert torch.equal(x.view(torch.uint8), y.view(torch.uint8)) and torch.equal(x.view(torch.uint8), z.view(torch.uint8))
+
+
 def test_captured(dev):
     """A captured call follows new rows, positions, lengths and tables on every replay, beside another on its own stream."""
     steps = []
