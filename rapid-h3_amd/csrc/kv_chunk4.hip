@@ -304,7 +304,7 @@ __global__ void __launch_bounds__(WAVES * 64, 2) chunk_kernel(AttnArgs a) {
         top = fmaxf(top, y[i]);
       }
       top = across_max<false>(top);
-      const float to = top - ref > STALE ? reference_over(top) : ref;
+      const float to = next_reference(ref, top, across_sum<false>(sum));
       const float f = __builtin_amdgcn_exp2f(ref - to);
       ref = to;
       sum *= f;
@@ -373,6 +373,8 @@ __global__ void __launch_bounds__(WAVES * 64, 2) chunk_kernel(AttnArgs a) {
         staged_v = staged_k = odd = made = false;
         there = all_there(++s);
         if (s >= t1) break;
+        // now and then: 8 steps bring a lane's sum 2^-8 further at most
+        if ((s & 7) == 0 && __builtin_amdgcn_ballot_w64(sum > SUM_MOST)) break;
       }
       if (s >= t1) break;
       const int b = s & 1;

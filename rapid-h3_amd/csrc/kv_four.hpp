@@ -65,13 +65,22 @@ __device__ __forceinline__ void query8(const uint4 raw, b8_t& hi, b8_t& lo) {
 }
 
 // Probabilities are 2^(score - reference), base 2, with the reference OVER over the row's running maximum, moved where a score comes
-// to more than 2^-STALE: with bf16's exponents their size costs nothing, and sums of 2^24 keys' values stay in fp32 up to the
-// largest value there is, while values down to 2^-94 keep their bits. (From 2^28 on, a score's last place is more than OVER: the
-// reference is then the maximum itself, or the next number.)
+// to less than -STALE under it: with bf16's exponents their size costs nothing. Of equal scores 2^16 make a lane's sum, of scores that
+// rose just so far that the reference stayed 2^4; at SUM_MOST it moves up by LATER. So a row's sum over the 16 lanes that share it in
+// a workgroup is under 0.1, its values' sum, not yet divided, under 0.1 of the largest of them, and fp32 holds both, and the join of all
+// workgroups' times PART, up to the largest value there is (1.5 * 2^127) for any number of keys. Values down to 2^-94 keep their bits
+// (2^-82 after one LATER). (From 2^28 on, a score's last place is more than OVER: the reference is then the maximum itself, or the next
+// number, and does not move for a sum's sake.)
 constexpr float OVER = 24.0f;
 constexpr float STALE = -12.0f;
+constexpr float SUM_MOST = 0x1p-8f;
+constexpr float LATER = 12.0f;
 constexpr float NO_REF = -0x1.fffffep127f;   // reference of a row that has seen no key: any score moves it
 __device__ __forceinline__ float reference_over(float top) { return top + OVER; }
+// a row's reference for keys whose largest score is `top`; sum: of its probabilities so far, over all lanes
+__device__ __forceinline__ float next_reference(float ref, float top, float sum) {
+  return top - ref > STALE ? reference_over(top) : sum > SUM_MOST ? ref + LATER : ref;
+}
 // parts are kept against a reference 2^24 lower (their sums times PART, as the join takes them)
 constexpr float PART_UP = 0x1p24f;
 

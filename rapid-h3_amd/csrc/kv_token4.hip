@@ -184,9 +184,9 @@ __device__ __forceinline__ void compute(const AttnArgs& a, Tile<D>& t, int tile,
 #pragma unroll
       for (int j = 0; j < 8; ++j) y[j] = hidden(j, lim[m]) ? -INFINITY : y[j];
     }
-    float top = y[0];
+    float top = st.sum[m] + (STALE - SUM_MOST);   // over STALE where the sum is over SUM_MOST
 #pragma unroll
-    for (int j = 1; j < 8; ++j) top = fmaxf(top, y[j]);
+    for (int j = 0; j < 8; ++j) top = fmaxf(top, y[j]);
     if (__builtin_amdgcn_ballot_w64(top > STALE)) {
       float n = -INFINITY;
 #pragma unroll
@@ -195,7 +195,7 @@ __device__ __forceinline__ void compute(const AttnArgs& a, Tile<D>& t, int tile,
         n = fmaxf(n, y[j]);
       }
       n = across_max<true>(n);
-      const float to = n - st.ref[m] > STALE ? reference_over(n) : st.ref[m];
+      const float to = next_reference(st.ref[m], n, across_sum<true>(st.sum[m]));
       const float f = __builtin_amdgcn_exp2f(st.ref[m] - to);
       st.ref[m] = to;
       st.sum[m] *= f;

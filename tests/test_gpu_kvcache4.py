@@ -406,6 +406,34 @@ def test_value_magnitudes(dev, form, rows, n, prefix_len, size):
 
 @pytest.mark.parametrize("dim", [64, 128])
 @pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("rise,low", [(11, 128), (0, 0)])
+def test_sums_of_the_largest_values(dev, dim, form, rise, low):
+    """Very many keys on one wave, all of the same weight but a first stretch `rise` (base 2) below, with the largest values that the
+    format holds: their sums, not yet divided, stay finite. So many sequences that a workgroup has all keys of one; they share pages."""
+    b, heads, page, n = 96, 8, 64, (1 << 15) + 128
+    pages = -(-n // page)
+    c = kv.kv_cache(pages, heads, page, dim, FP4, dev)
+    codes, scales = ok.quantise4(torch.full((dim,), 6 * 2.0 ** 125))
+    c.v.view(torch.uint8)[:] = codes.to(dev)
+    c.v_scale.view(torch.uint8)[:] = scales.to(dev)
+    key = torch.zeros(dim)
+    key[0] = 6.0
+    codes, scales = ok.quantise4(key)
+    c.k.view(torch.uint8)[low // page:] = codes.to(dev)
+    c.k_scale.view(torch.uint8)[:] = scales.to(dev)
+    q = torch.zeros(b, heads, dim, dtype=BF, device=dev)
+    q[..., 0] = 1.0
+    table = torch.arange(pages, dtype=torch.int32, device=dev).expand(b, pages).contiguous()
+    scale = rise * math.log(2) / 6.0
+    out, lse = kv.kv_attention(q, c, table, _i32([n] * b, dev), scale=scale, lse=True, form=form)
+    ref = torch.full((b, heads, dim), 6 * 2.0 ** 125, dtype=torch.float64, device=dev)
+    err = torch.full((b, heads), 2.0 ** -20, dtype=torch.float64, device=dev)   # a score is one product, scaled and less a reference: 3 roundings
+    _check(out, ref, ref, err, form, n)
+    _check_lse(lse, torch.full_like(err, math.log(low + (n - low) * 2.0 ** rise)), err)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("form", FORMS)
 @pytest.mark.parametrize("rows,prefix_len", [(3, 0), (90, 0), (90, 300)])
 def test_fp16_results_are_rounded_once(dev, dim, form, rows, prefix_len):
     """fp16 results differ from float64 by little more than their own rounding."""
