@@ -2,6 +2,7 @@
 (kvcache.kv_write_rope), on the GPU against the plain restatement and float64."""
 import math
 
+import numpy as np
 import pytest
 import torch
 
@@ -203,6 +204,41 @@ def test_rows_past_the_table_turn_by_their_positions(dev, fmt, ragged, first):
             assert torch.equal(x, wq[r:r + 1]), (i, j)
     for x, y, z in zip(*((c.k, c.v, c.k_scale, c.v_scale) for c in (one, two, parts))):
         assert torch.equal(x.view(torch.uint8), y.view(torch.uint8)) and torch.equal(x.view(torch.uint8), z.view(torch.uint8))
+
+
+def _rows_at_a_border(n, dim, eps, seed):
+    """fp32 rows whose inverse root mean square lies at the middle of two fp32 numbers, as near as their squares' sum in 64 bits can tell:
+    three channels are chosen for it, each taking what the one before it left."""
+    r = np.random.default_rng(seed)
+    x = r.standard_normal((n, dim)).astype(np.float32)
+    for row in x:
+        last = r.choice(dim, 3, replace=False)
+        row[last] = 0.0
+        rest = (row.astype(np.longdouble) ** 2).sum()
+        near = np.float32(1 / np.sqrt((rest + 1 + r.random()) / dim + eps))
+        middle = np.longdouble(near) + np.longdouble(np.spacing(near)) / 2
+        left = dim * (1 / middle ** 2 - np.longdouble(eps)) - rest
+        for i in last:
+            y = np.float32(np.sqrt(left))
+            row[i] = y if np.longdouble(y) ** 2 <= left else np.nextafter(y, np.float32(0))
+            left -= np.longdouble(row[i]) ** 2
+    return torch.from_numpy(x)
+
+
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+@pytest.mark.parametrize("dim,rot", [(128, 128), (128, 96), (64, 64), (64, 16), (128, 0)])
+def test_write_rope_is_both_where_the_norm_is_at_a_border(dev, dim, rot, layout):
+    """The same bits also of fp32 rows whose norm would be rounded to another number if its squares were summed in another order."""
+    n, heads, page = 300, 3, 64
+    k = _rows_at_a_border(n * heads, dim, 1e-6, 1).view(n, heads, dim).to(dev)
+    turn = rope.rotary(rot, layout, dev) if rot else None
+    table, lens = _i32([range(5)], dev), _i32([n], dev)
+    one, two = (kv.kv_cache(5, heads, page, dim, FMT[0], dev) for _ in range(2))
+    pos = torch.arange(n, dtype=torch.int32, device=dev)
+    kv.kv_write_rope(one, k, k, k, table, lens, None, turn, eps=1e-6)
+    kv.kv_write(two, rope.qk_norm_rope(k, None, pos, turn, eps=1e-6)[0], k, table, lens)
+    for x, y in zip((one.k, one.v, one.k_scale, one.v_scale), (two.k, two.v, two.k_scale, two.v_scale)):
+        assert torch.equal(x, y)
 
 
 def test_captured(dev):
