@@ -26,6 +26,10 @@ namespace {
 
 constexpr int KT = CHUNK_KEYS;
 constexpr float SUM_STALE = 0x1p-12f;        // up to this sum of a half's probabilities none of them is over 2^STALE
+// Past it one of 16 is over 2^(STALE - 4): the plain path moves the reference from a little under that on, so that the next halves of
+// scores like these pass (with STALE itself, scores 9 to 12 over a share's first ones go both paths half after half until their sum
+// moves it; before it did, to the end: 488 us for 266)
+constexpr float SLOW_STALE = STALE - 5.0f;
 
 // 16-byte pieces of the LDS rows. Each row has one piece more than it needs, so that 16 rows' pieces of one number lie in all 16
 // parts of the banks, and every read of a tile is one lane address with an immediate offset.
@@ -304,7 +308,7 @@ __global__ void __launch_bounds__(WAVES * 64, 2) chunk_kernel(AttnArgs a) {
         top = fmaxf(top, y[i]);
       }
       top = across_max<false>(top);
-      const float to = next_reference(ref, top, across_sum<false>(sum));
+      const float to = next_reference(ref, top, across_sum<false>(sum), SLOW_STALE);
       const float f = __builtin_amdgcn_exp2f(ref - to);
       ref = to;
       sum *= f;

@@ -78,8 +78,8 @@ constexpr float LATER = 12.0f;
 constexpr float NO_REF = -0x1.fffffep127f;   // reference of a row that has seen no key: any score moves it
 __device__ __forceinline__ float reference_over(float top) { return top + OVER; }
 // a row's reference for keys whose largest score is `top`; sum: of its probabilities so far, over all lanes
-__device__ __forceinline__ float next_reference(float ref, float top, float sum) {
-  return top - ref > STALE ? reference_over(top) : sum > SUM_MOST ? ref + LATER : ref;
+__device__ __forceinline__ float next_reference(float ref, float top, float sum, float stale = STALE) {
+  return top - ref > stale ? reference_over(top) : sum > SUM_MOST ? ref + LATER : ref;
 }
 // parts are kept against a reference 2^24 lower (their sums times PART, as the join takes them)
 constexpr float PART_UP = 0x1p24f;

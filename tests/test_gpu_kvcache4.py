@@ -354,6 +354,43 @@ def test_rising_scores(dev, dim, form, rows, gap):
     _check_lse(lse, rl, err)
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("rows", [2, 100, 600])
+@pytest.mark.parametrize("gap", [5, 7, 8, 9, 11, 12])
+def test_scores_that_rise_a_little(dev, dim, form, rows, gap):
+    """Rises about as far as a reference stays where it is."""
+    test_rising_scores(dev, dim, form, rows, gap)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_time_of_scores_that_rise_a_little(dev, dim):
+    """Keys that score 10 (base 2) over a share's first ones move the reference once, as such do that score 20 over: the same time, where
+    doing every half's softmax again took 1.8 to 1.9 times as long. So many sequences that a workgroup has all keys of one."""
+    b, rows, heads, page, n = 256, 128, 2, 64, 8192
+    c = _pool(dev, n // page, heads, page, dim, 3)
+    for t in (c.k, c.k_scale):
+        t.view(torch.uint8).zero_()
+    key = torch.zeros(dim)
+    key[0] = 6.0
+    codes, scales = ok.quantise4(key)
+    c.k.view(torch.uint8)[1:], c.k_scale.view(torch.uint8)[1:] = codes.to(dev), scales.to(dev)
+    q = torch.zeros(b * rows, heads, dim, dtype=BF, device=dev)
+    q[..., 0] = 1.0
+    args = (torch.arange(n // page, dtype=torch.int32, device=dev).expand(b, -1).contiguous(), _i32([n] * b, dev))
+    best = {10: math.inf, 20: math.inf}
+    for _ in range(8):
+        for gap in best:
+            a, z = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+            a.record()
+            for _ in range(4):
+                kv.kv_attention(q, c, *args, causal=False, scale=gap * math.log(2) / 6, form="chunk")
+            z.record()
+            z.synchronize()
+            best[gap] = min(best[gap], a.elapsed_time(z))
+    assert best[10] < 1.4 * best[20], best
+
+
 @pytest.mark.parametrize("form", FORMS)
 @pytest.mark.parametrize("rows", [1, 90])
 @pytest.mark.parametrize("dtype", [BF, HF])
