@@ -491,11 +491,14 @@ typedef struct rh3_kv_cache {
 
 /* The page tables of a batch from one step to the next. A pool: free_pages [pages], of which the first state[0] are free, taken and
  * given back at the end; state[1]: how many pages this call lacked. In the order of the sequences: the pages of those with done[b] != 0
- * (done NULL: none) go back, in the order of the table, which then holds -1; each sequence's length becomes (done ? 0 : lens[b]) +
- * more[b], and the entries of its row of the table that this adds (as far as width) are the next pages off the list, -1 where it is
- * empty. cu [batch + 1]: where each one's new rows begin; of each of `rows` (a capacity) its position in its sequence and its slot, page *
- * page size + offset; slots -1 where it has no place, both -1 behind cu[batch]. Negative lens and more count as 0; a length is at most
- * 2^30. batch * width at most 2^30. Everything is device memory; nothing is read back. The workspace holds sums for a call. */
+ * (done NULL: none) go back, in the order of the table, which then holds -1; a negative more[b] takes rows back: the length falls by
+ * them, not under 0, and the pages that then hold no position of the sequence go back too. Each sequence's length becomes (done ? 0 :
+ * lens[b]) + more[b], and the entries of its row of the table that this adds (as far as width) are the next pages off the list, -1
+ * where it is empty (the same rows taken back, and the step can be made again when there are pages). cu [batch + 1]: where each one's
+ * new rows begin; of each of `rows` (a capacity) its position in its sequence and its slot, page * page size + offset; slots -1 where
+ * it has no place, both -1 behind cu[batch]. Lengths are shortened by done and more alone: the pages behind a length that the caller
+ * lowers itself are in no list any more. Negative lens count as 0; a length is at most 2^30. batch * width at most 2^30. Everything is
+ * device memory; nothing is read back. The workspace holds sums for a call. */
 int64_t rh3_kv_extend_workspace_bytes(int64_t batch);
 typedef struct rh3_kv_extend_args {
   int32_t* free_pages;

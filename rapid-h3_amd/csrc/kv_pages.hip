@@ -1,10 +1,12 @@
-// The page tables of a batch from one step to the next, kept on the GPU: sequences that have ended give their pages back, every
-// sequence takes the pages that its new rows need, and of each new row the position and the slot in the cache are written down.
+// The page tables of a batch from one step to the next, kept on the GPU: sequences that have ended give their pages back, those that
+// take rows back (drafts that were not accepted, a step for which there were too few pages) the pages behind them, every sequence
+// takes the pages that its new rows need, and of each new row the position and the slot in the cache are written down.
 //
 // A pool is a list of free pages, taken and given back at its end, and how many there are. In the order of the sequences, and of each
-// one's table: the pages of those that have ended go on the list, then those that the others need come off it. With start = 0 for a
-// sequence that has ended and its length else, end = start + its new rows, P positions to a page: the entries
-// [ceil(start / P), ceil(end / P)) of its row of the table are the next pages off the list, as far as the row and the list reach.
+// one's table: the pages that come back go on the list, then those that are needed come off it. With start = 0 for a sequence that has
+// ended, its length less the rows it takes back else, end = start + its new rows, P positions to a page: the entries
+// [ceil(start / P), ceil(length / P)) of its row of the table come back, the entries [ceil(start / P), ceil(end / P)) are then the next
+// pages off the list, as far as the row and the list reach.
 // All of it is prefix sums over the sequences and searches in them, so the result is the same in every run.
 //
 // Bound by latency: a step moves 9 bytes a sequence, 12 a row and 8 a page. The sums need one workgroup: it makes them, walks the
@@ -132,6 +134,7 @@ template <int NT>
 __global__ void __launch_bounds__(NT) plan_kernel(PagesArgs a) {
   constexpr int WAVES = NT / 64;
   __shared__ int near_back[NEAR + 1], near_taken[NEAR + 1], near_cu[NEAR + 1];
+  __shared__ int near_entry[NEAR];      // the first entry that comes back, less those of the sequences before
   __shared__ Counts counts[2][WAVES];   // two in turn, so that one barrier to a turn is enough
   constexpr int EACH = 8;
   __shared__ int valid[2][EACH * WAVES];
@@ -144,11 +147,11 @@ __global__ void __launch_bounds__(NT) plan_kernel(PagesArgs a) {
     int start = 0, end = 0;
     Counts mine{0, 0, 0};
     if (b < a.batch) {
-      const int len = min(max(a.lens[b], 0), MOST), more = min(max(a.more[b], 0), MOST);
+      const int len = min(max(a.lens[b], 0), MOST), more = min(max(a.more[b], -MOST), MOST);
       const bool over = a.done && a.done[b];
-      start = over ? 0 : len;
-      end = min(start + more, MOST);
-      mine = Counts{over ? pages_for(a, len) : 0, max(pages_for(a, end) - pages_for(a, start), 0), more};
+      start = over ? 0 : max(len + min(more, 0), 0);
+      end = min(start + max(more, 0), MOST);
+      mine = Counts{pages_for(a, len) - pages_for(a, start), pages_for(a, end) - pages_for(a, start), max(more, 0)};
     }
     const Counts all = scan(mine, counts[turn]);
     if (b < a.batch) {
@@ -159,6 +162,7 @@ __global__ void __launch_bounds__(NT) plan_kernel(PagesArgs a) {
       a.start[b] = start;
       if (near) {
         near_back[b] = back;
+        near_entry[b] = pages_for(a, start) - back;
         near_taken[b] = taken;
         near_cu[b] = cu;
       } else {
@@ -195,7 +199,7 @@ __global__ void __launch_bounds__(NT) plan_kernel(PagesArgs a) {
     near ? search(near_back, a.batch, f, s) : search(a.back, a.batch, f, s);
 #pragma unroll
     for (int i = 0; i < EACH; ++i) {
-      int32_t* e = a.table + s[i] * a.table_stride + (f[i] - (near ? near_back[s[i]] : a.back[s[i]]));
+      int32_t* e = a.table + s[i] * a.table_stride + (f[i] + (near ? near_entry[s[i]] : pages_for(a, a.start[s[i]]) - a.back[s[i]]));
       entry[i] = -1;
       if (at + NT * i + tid < back) {
         entry[i] = *e;

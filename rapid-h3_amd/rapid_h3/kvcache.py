@@ -137,8 +137,10 @@ def kv_pages(pages, page=64, device="cuda"):
 def kv_extend(pool, table, lens, new, rows, done=None):
     """A step's page table, made on the GPU: sequences with done [B] (bool) give their pages back to the pool and begin again at
     length 0; lens grows by new [B] int32, the rows that each sequence gets in this step; the pages that takes are put into table
-    [B, W] (entries past W are left out; -1 where the pool is empty: pool.state[1] says how many those are). table and lens change in
-    place. -> cu [B + 1], positions [rows] int32 and slots [rows] int64 of the new rows, packed sequence by sequence: the position in the
+    [B, W] (entries past W are left out; -1 where the pool is empty: pool.state[1] says how many those are). A negative new takes that many
+    rows back (drafts that were not accepted, a step that lacked pages): the pages behind what is left go back to the pool. That and
+    done are the ways to shorten a sequence: pages behind a length that a program lowers itself are lost to the pool. table and lens
+    change in place. -> cu [B + 1], positions [rows] int32 and slots [rows] int64 of the new rows, packed sequence by sequence: the position in the
     sequence, and page * pool.page + offset, where k.transpose(1, 2) of the cache has it (-1: nowhere). rows: how many the call has room
     for; behind the last row both are -1. cu, lens and table are what the other calls take."""
     name = "kv_extend"

@@ -85,6 +85,70 @@ def test_steps(dev, pages, page, b, w, most, seed):
         assert (wide[:, w:] == -7).all()
 
 
+class Cut(Lists):
+    """Lists whose sequences also take rows back (a negative number of new ones)."""
+
+    def extend(self, new, rows, done):
+        page, cut = self.page, [not d and m < 0 for m, d in zip(new, done)]
+        for b, row in enumerate(self.table):     # what comes back of all sequences, in their order, before anything is taken
+            n = self.lens[b]
+            keep = 0 if done[b] else max(n + new[b], 0) if cut[b] else n
+            for i in range(-(-keep // page), min(-(-n // page), len(row))):
+                if 0 <= row[i] < len(self.free) and self.held < len(self.free):
+                    self.free[self.held] = row[i]
+                    self.held += 1
+                row[i] = -1
+            self.lens[b] = keep
+        return super().extend([max(m, 0) for m in new], rows, [False] * len(new))
+
+
+@pytest.mark.parametrize("pages,page,b,w,most,seed", [
+    (5, 16, 1, 3, 20, 0),
+    (40, 64, 7, 9, 130, 1),
+    (300, 16, 64, 12, 60, 2),
+    (4000, 32, 1500, 40, 300, 3),
+    (9000, 16, 3000, 9, 40, 4),
+    (2000, 256, 30, 80, 9000, 5),
+])
+def test_rows_taken_back(dev, pages, page, b, w, most, seed):
+    """Steps in which some sequences grow, others lose their last rows, some more than they have, some end: no page is lost."""
+    r = random.Random(seed)
+    pool, lists = kv.kv_pages(pages, page, dev), Cut(pages, page, b, w)
+    table, lens = torch.full((b, w), -1, dtype=torch.int32, device=dev), torch.zeros(b, dtype=torch.int32, device=dev)
+    for step in range(6):
+        new = [r.choice((0, 1, r.randint(0, most), -1, -r.randint(0, most), -r.randint(0, 3 * most))) if step else r.randint(0, most) for _ in range(b)]
+        done = [r.random() < 0.1 for _ in range(b)] if step else [False] * b
+        rows = sum(max(m, 0) for m in new) + 2
+        got = kv.kv_extend(pool, table, lens, _i32(new, dev), rows, torch.tensor(done, device=dev) if step else None)
+        for x, y in zip(got, lists.extend(new, rows, done)):
+            assert x.tolist() == y, step
+        _same(pool, table, lens, lists)
+        owned = table[table >= 0].tolist()
+        assert sorted(owned + pool.free[:int(pool.state[0])].tolist()) == list(range(pages)), step
+
+
+def test_drafts_and_a_pool_that_runs_out(dev):
+    """Drafts that are not accepted go back with their pages, step after step; a step that lacked pages is undone and made again when
+    another sequence has ended; the smallest number takes back everything."""
+    page, pages = 16, 6
+    pool = kv.kv_pages(pages, page, dev)
+    table, lens = torch.full((2, 5), -1, dtype=torch.int32, device=dev), torch.zeros(2, dtype=torch.int32, device=dev)
+    kv.kv_extend(pool, table, lens, _i32([15, 10], dev), 25)
+    for _ in range(20):                          # four drafts each, of which one or none is kept
+        kv.kv_extend(pool, table, lens, _i32([20, 4], dev), 24)
+        kv.kv_extend(pool, table, lens, _i32([-20, -4], dev), 0)
+    assert pool.state.tolist() == [4, 0] and lens.tolist() == [15, 10] and (table[:, 1:] == -1).all()
+    before = table.tolist()
+    kv.kv_extend(pool, table, lens, _i32([50, 40], dev), 90)
+    assert pool.state.tolist() == [0, 3]
+    kv.kv_extend(pool, table, lens, _i32([-50, -40], dev), 0)
+    assert pool.state.tolist() == [4, 0] and lens.tolist() == [15, 10] and table.tolist() == before
+    _, positions, slots = kv.kv_extend(pool, table, lens, _i32([50, 0], dev), 50, torch.tensor([False, True], device=dev))
+    assert pool.state.tolist() == [1, 0] and positions.tolist() == list(range(15, 65)) and (slots >= 0).all()
+    cu, _, _ = kv.kv_extend(pool, table, lens, _i32([-2 ** 31, 3], dev), 3)
+    assert cu.tolist() == [0, 0, 3] and lens.tolist() == [0, 3] and pool.state.tolist() == [5, 0] and (table[0] == -1).all()
+
+
 def test_bad_contents_stay_inside(dev):
     """Counts beyond the list, negative lengths and rows, entries that are no pages, pages given back twice."""
     b, w, pages, page = 4, 3, 6, 16
