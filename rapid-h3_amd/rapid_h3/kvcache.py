@@ -158,6 +158,7 @@ def kv_extend(pool, table, lens, new, rows, done=None):
         raise ValueError(f"{name}: {rows} rows")
     dev = table.device
     if b == 0:
+        pool.state[1:].zero_()
         return torch.zeros(1, dtype=torch.int32, device=dev), *(torch.full((rows,), -1, dtype=t, device=dev) for t in (torch.int32, torch.int64))
     cu = torch.empty(b + 1, dtype=torch.int32, device=dev)
     positions = torch.empty(rows, dtype=torch.int32, device=dev)

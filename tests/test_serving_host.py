@@ -181,6 +181,15 @@ def test_wrappers_refuse(monkeypatch):
                          x[..., :64], x[..., :64], x[..., :64], table, n, rotary=rope.Rotary(rope.frequencies(128)[0]))
 
 
+def test_extend_of_an_empty_batch_lacks_no_pages(monkeypatch):
+    """pool.state[1] is of the last call, also where that had no sequences."""
+    monkeypatch.setattr(torch.Tensor, "is_cuda", True)
+    pool = kv.KVPages(torch.arange(4, dtype=torch.int32), torch.tensor([3, 7], dtype=torch.int32), 16)
+    none = torch.empty(0, dtype=torch.int32)
+    kv.kv_extend(pool, none.view(0, 3), none, none, 2)
+    assert pool.state.tolist() == [3, 0]
+
+
 def test_frequencies():
     f, one = rope.frequencies(128)
     assert one == 1.0 and f.dtype == torch.float64 and torch.equal(f, 10000.0 ** (-torch.arange(64, dtype=torch.float64) / 64))
