@@ -35,6 +35,8 @@ extern "C" {
 #define RH3_KV_BY_SIZE 0
 #define RH3_KV_TOKEN 1
 #define RH3_KV_CHUNK 2
+/* added to the form in rh3_kv_attention_workspace_bytes: for calls with caches of this format and queries of this type alone */
+#define RH3_KV_SIZE_OF(format, dtype) (16 * ((format) + 1) + 256 * ((dtype) + 1))
 
 /* Message of the last failed call on this thread ("" if none). */
 const char* rh3_last_error(void);
@@ -583,7 +585,8 @@ int rh3_kv_write_rope(const rh3_kv_cache* cache, const rh3_kv_rope_args* args, h
  * stands for the lengths, which only the device knows.
  * The workspace (capacity: width * page; even: 1 where cu is NULL) holds the parts of rows whose keys several workgroups share;
  * how keys are split depends on the sizes, lengths and the CU count, and with it the last bits of the result; the same call
- * gives the same bits. The size is 0 for sizes that attention refuses or that leave nothing to do. */
+ * gives the same bits. The size is 0 for sizes that attention refuses or that leave nothing to do; for form alone it is enough for caches
+ * of all formats and queries of both types, for form + RH3_KV_SIZE_OF(format, dtype) for those. */
 int64_t rh3_kv_attention_workspace_bytes(int64_t q_heads, int64_t heads, int64_t dim, int64_t rows, int64_t capacity,
                                          int64_t batch, int even, int64_t prefix_len, int form);
 int rh3_kv_attention(const rh3_kv_cache* cache, const void* q, int64_t q_st, int64_t q_sh, int64_t q_heads, int dtype,

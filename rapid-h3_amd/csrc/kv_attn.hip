@@ -268,11 +268,13 @@ extern "C" int64_t rh3_kv_attention_workspace_bytes(int64_t q_heads, int64_t hea
   if (heads < 1 || heads > 65535 || q_heads < heads || q_heads % heads || rows < 1 || rows > MAX_ROWS || q_heads / heads > MAX_ROWS / rows ||
       batch < 1 || batch > 65536 || capacity < 1 || capacity > MAX_ROWS || prefix_len < 0 || prefix_len > MAX_ROWS || (dim != 64 && dim != 128))
     return 0;
-  // enough for a cache of either width of codes, and queries of either type
+  // RH3_KV_SIZE_OF: the cache's format and the queries' type, or neither
+  const int of = form & ~15, kernel = form & 15;
   int64_t most = 0;
-  for (const int fmt : {INT8, FP4})
-    for (const bool fine : {false, true}) {
-      const int64_t n = call_of(fmt, fine, rows, q_heads, heads, dim, capacity, batch, even != 0, prefix_len, form).bytes;
+  for (const int fmt : {INT8, E4M3, FP4})
+    for (const int dtype : {RH3_DTYPE_BF16, RH3_DTYPE_F16}) {
+      if (of && of != RH3_KV_SIZE_OF(fmt, dtype)) continue;
+      const int64_t n = call_of(fmt, dtype == RH3_DTYPE_F16, rows, q_heads, heads, dim, capacity, batch, even != 0, prefix_len, kernel).bytes;
       most = n > most ? n : most;
     }
   return most;

@@ -103,6 +103,10 @@ RH3_KV_E4M3 = 1
 RH3_KV_FP4 = 4
 RH3_KV_BY_SIZE, RH3_KV_TOKEN, RH3_KV_CHUNK = 0, 1, 2
 
+
+def RH3_KV_SIZE_OF(fmt, dtype):
+    return 16 * (fmt + 1) + 256 * (dtype + 1)
+
 _lib = None
 _FN = {}   # entry point name -> bound function, filled by lib()
 

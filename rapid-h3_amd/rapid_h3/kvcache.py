@@ -50,7 +50,7 @@ class KVCache:
     4-bit codes, a scale byte is at most 252, or 255 in all of k_scale's at a position whose key or value is not finite (NaN in both).
     The tensors are kept and used as they are; the attributes cannot be changed."""
 
-    __slots__ = ("k", "v", "k_scale", "v_scale", "pages", "heads", "page", "dim", "device", "gpu", "_desc", "_ref")
+    __slots__ = ("k", "v", "k_scale", "v_scale", "pages", "heads", "page", "dim", "device", "gpu", "_sizes", "_desc", "_ref")
 
     def __init__(self, k, v, k_scale, v_scale):
         if k.ndim != 4 or v.shape != k.shape or any(_st(v, i) != _st(k, i) for i in range(4)):
@@ -78,9 +78,10 @@ class KVCache:
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.pages, self.heads, self.page, self.dim, self.device = p, h, n, dim, k.device
         self.gpu = k.get_device()
+        fmt = nat.RH3_KV_FP4 if four else nat.RH3_KV_INT8 if k.dtype == torch.int8 else nat.RH3_KV_E4M3
+        self._sizes = {t: nat.RH3_KV_SIZE_OF(fmt, t) for t in (nat.RH3_DTYPE_BF16, nat.RH3_DTYPE_F16)}
         self._desc = nat.KvCacheDesc(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), _st(k, 0), _st(k, 1),
-                                     _st(k_scale, 0), _st(k_scale, 1), p, h, n, dim,
-                                     nat.RH3_KV_FP4 if four else nat.RH3_KV_INT8 if k.dtype == torch.int8 else nat.RH3_KV_E4M3)
+                                     _st(k_scale, 0), _st(k_scale, 1), p, h, n, dim, fmt)
         self._ref = ctypes.addressof(self._desc)
 
     def __setattr__(self, name, value):
@@ -299,7 +300,9 @@ def _attention(name, q, cache, prefix, prefix_len, table, lens, cu, causal, scal
         q_sh = o_sh = 0
     sums = alloc((t, hq), dtype=torch.float32, device=dev) if lse else None
     with _on(gpu):
-        n = _workspace_bytes(gpu, hq, cache.heads, d, t, seqs[2] * cache.page, seqs[5], cu is None, prefix_len, f)
+        # (of a cache that says nothing of its format: enough for any)
+        n = _workspace_bytes(gpu, hq, cache.heads, d, t, seqs[2] * cache.page, seqs[5], cu is None, prefix_len,
+                             f + getattr(cache, "_sizes", {}).get(dt, 0))
         ws = torch.empty(n, dtype=torch.uint8, device=dev)
         nat.call("rh3_kv_attention", cache._ref, q.data_ptr(), q_st, q_sh, hq, dt, t, *seqs, causal, d ** -0.5 if scale is None else scale,
                  out.data_ptr(), o_st, o_sh, None if sums is None else sums.data_ptr(), None if prefix is None else prefix.data_ptr(),

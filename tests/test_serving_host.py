@@ -1,5 +1,6 @@
 """CPU tests of the serving step's entry points (rh3_kv_extend, rh3_qk_norm_rope, rh3_kv_write_rope, the 4-bit cache): what they
 refuse, with which message, before touching the device; the frequencies; the oracles' own properties."""
+import contextlib
 import ctypes
 import math
 
@@ -188,6 +189,39 @@ def test_extend_of_an_empty_batch_lacks_no_pages(monkeypatch):
     none = torch.empty(0, dtype=torch.int32)
     kv.kv_extend(pool, none.view(0, 3), none, none, 2)
     assert pool.state.tolist() == [3, 0]
+
+
+def test_workspace_is_of_the_caches_format(monkeypatch):
+    """A call allocates what its own format and query type need: caches of 8-bit codes nothing for the 4-bit kernels' plans. Without them the
+    size is enough for all."""
+    size, of = nat.lib().rh3_kv_attention_workspace_bytes, nat.RH3_KV_SIZE_OF
+    formats, types = (nat.RH3_KV_INT8, nat.RH3_KV_E4M3, nat.RH3_KV_FP4), (nat.RH3_DTYPE_BF16, nat.RH3_DTYPE_F16)
+    for hq, heads, dim, rows, cap, batch, prefix in ((32, 8, 128, 1, 16384, 1, 0), (32, 8, 128, 128, 4096, 16, 0), (28, 4, 64, 512, 65536, 4, 0),
+                                                     (32, 8, 128, 384, 65536, 4, 0), (56, 8, 128, 120, 640, 40, 24001)):
+        for form in (nat.RH3_KV_BY_SIZE, nat.RH3_KV_TOKEN, nat.RH3_KV_CHUNK):
+            n = {(f, t): size(hq, heads, dim, rows, cap, batch, 1, prefix, form + of(f, t)) for f in formats for t in types}
+            assert max(n.values()) == size(hq, heads, dim, rows, cap, batch, 1, prefix, form) > 0
+            assert len({n[f, t] for f in formats[:2] for t in types}) == 1
+    # one token: slots for the parts of two workgroups to a CU, or three
+    a, b = (size(32, 8, 128, 1, 16384, 1, 1, 0, of(f, types[0])) for f in (nat.RH3_KV_INT8, nat.RH3_KV_FP4))
+    assert 3 * a == 2 * b and a % (2 * 2 * 16 * (128 + 2) * 4) == 0
+    assert size(32, 8, 128, 1, 16384, 1, 1, 0, of(3, types[0])) == 0
+
+    given = []
+    monkeypatch.setattr(torch.Tensor, "is_cuda", True)
+    monkeypatch.setattr(kv, "_on", lambda gpu: contextlib.nullcontext())
+    monkeypatch.setattr(kv, "_stream", lambda gpu: None)
+    monkeypatch.setattr(nat, "call", lambda name, *args: given.append(args[-2]))
+    codes, scales = torch.zeros((4, 2, 64, 128), dtype=torch.int8), torch.zeros((4, 2, 64))
+    byte, four = torch.zeros((4, 2, 64, 64), dtype=torch.uint8), torch.zeros((4, 2, 64, 4), dtype=torch.uint8)
+    table, lens = torch.zeros((3, 2), dtype=torch.int32), torch.ones(3, dtype=torch.int32)
+    kv._workspace_bytes.cache_clear()
+    for dtype, t in ((torch.bfloat16, types[0]), (torch.float16, types[1])):
+        q = torch.zeros((3, 8, 128), dtype=dtype)
+        for args, f in (((codes, codes, scales, scales), formats[0]), ((codes.view(kv.FP8),) * 2 + (scales, scales), formats[1]), ((byte, byte, four, four), formats[2])):
+            kv.kv_attention(q, kv.KVCache(*args), table, lens)
+            assert given[-1] == size(8, 2, 128, 3, 128, 3, 1, 0, of(f, t))
+    kv._workspace_bytes.cache_clear()
 
 
 def test_frequencies():
