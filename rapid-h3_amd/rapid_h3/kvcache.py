@@ -25,10 +25,11 @@ from . import rope
 from ._rows import _ROW, _on, _stream
 
 FP8 = torch.float8_e4m3fn
-FP4 = torch.float4_e2m1fn_x2          # two codes to a byte
+FP4 = getattr(torch, "float4_e2m1fn_x2", None)        # two codes to a byte (a torch without the type: bytes)
+_E8M0 = getattr(torch, "float8_e8m0fnu", torch.uint8)
 GROUP4 = 32                           # channels of a 4-bit row that share a scale
 _BYTES = (torch.uint8, FP4)
-_SCALE4 = (torch.uint8, torch.float8_e8m0fnu)
+_SCALE4 = (torch.uint8, _E8M0)
 _FORM = {None: nat.RH3_KV_BY_SIZE, "token": nat.RH3_KV_TOKEN, "chunk": nat.RH3_KV_CHUNK}
 
 
@@ -92,14 +93,14 @@ class KVCache:
 
 def kv_cache(pages, heads, page=64, dim=128, dtype=torch.int8, device="cuda"):
     """A new cache of zeros: dtype int8, float8_e4m3fn or float4_e2m1fn_x2."""
-    four = dtype == FP4
+    four = FP4 is not None and dtype == FP4
 
     def codes():
         return torch.zeros((pages, heads, page, dim // 2 if four else dim), dtype=torch.uint8, device=device).view(dtype)
 
     def scales():
         if four:
-            return torch.zeros((pages, heads, page, dim // GROUP4), dtype=torch.uint8, device=device).view(torch.float8_e8m0fnu)
+            return torch.zeros((pages, heads, page, dim // GROUP4), dtype=torch.uint8, device=device).view(_E8M0)
         return torch.zeros((pages, heads, page), dtype=torch.float32, device=device)
     return KVCache(codes(), codes(), scales(), scales())
 

@@ -3,6 +3,9 @@ refuse, with which message, before touching the device; the frequencies; the ora
 import contextlib
 import ctypes
 import math
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -222,6 +225,16 @@ def test_workspace_is_of_the_caches_format(monkeypatch):
             kv.kv_attention(q, kv.KVCache(*args), table, lens)
             assert given[-1] == size(8, 2, 128, 3, 128, 3, 1, 0, of(f, t))
     kv._workspace_bytes.cache_clear()
+
+
+def test_a_torch_without_the_four_bit_types():
+    """8-bit caches, and 4-bit ones of bytes, need no torch that names the 4-bit and exponent types."""
+    code = ("import torch; del torch.float4_e2m1fn_x2, torch.float8_e8m0fnu; from rapid_h3 import kvcache as kv; torch.Tensor.is_cuda = True; "
+            "assert kv.kv_cache(2, 1, device='cpu').dim == 128 and kv.kv_cache(2, 1, dtype=kv.FP8, device='cpu').dim == 128; "
+            "x, s = torch.zeros((2, 1, 16, 32), dtype=torch.uint8), torch.zeros((2, 1, 16, 2), dtype=torch.uint8); assert kv.KVCache(x, x, s, s).dim == 64")
+    path = os.pathsep.join([os.path.dirname(os.path.dirname(kv.__file__)), os.environ.get("PYTHONPATH", "")])
+    r = subprocess.run([sys.executable, "-c", code], env={**os.environ, "PYTHONPATH": path}, capture_output=True, text=True, timeout=110)
+    assert r.returncode == 0, r.stderr
 
 
 def test_frequencies():
