@@ -106,9 +106,10 @@ __device__ __forceinline__ Counts scan(Counts& v, Counts (&waves)[WAVES]) {
   return at(WAVES - 1);
 }
 
-// page i of those taken: sequence s, with `first` the number taken before it and p0 its first entry that is filled
+// page i of those taken, off the end of a list of `held`; -1 where it is empty
 __device__ __forceinline__ int taken_page(const PagesArgs& a, int held, int i) { return i < held ? a.free[held - 1 - i] : -1; }
 
+// ... into its place in the table
 template <typename Array>
 __device__ __forceinline__ void take(const PagesArgs& a, const Array taken, int held, int i) {
   const int s = search(taken, a.batch, i);
@@ -116,6 +117,7 @@ __device__ __forceinline__ void take(const PagesArgs& a, const Array taken, int 
   a.table[s * a.table_stride + p0 + i - taken[s]] = taken_page(a, held, i);
 }
 
+// position and slot of row r
 template <typename Cu, typename Array>
 __device__ __forceinline__ void row(const PagesArgs& a, const Cu cu, const Array taken, int held, int r, int& pos, int64_t& slot) {
   pos = -1;
@@ -133,13 +135,14 @@ __device__ __forceinline__ void row(const PagesArgs& a, const Cu cu, const Array
 template <int NT>
 __global__ void __launch_bounds__(NT) plan_kernel(PagesArgs a) {
   constexpr int WAVES = NT / 64;
+  constexpr bool FEW = NT == 256;      // calls that are near and alone
   __shared__ int near_back[NEAR + 1], near_taken[NEAR + 1], near_cu[NEAR + 1];
   __shared__ int near_entry[NEAR];      // the first entry that comes back, less those of the sequences before
   __shared__ Counts counts[2][WAVES];   // two in turn, so that one barrier to a turn is enough
   constexpr int EACH = 8;
   __shared__ int valid[2][EACH * WAVES];
   const int tid = threadIdx.x;
-  const bool near = a.batch <= NEAR;
+  const bool near = FEW || a.batch <= NEAR, alone = FEW || a.alone;
   const int held0 = min(max(a.state[0], 0), a.pages);
   Counts sum{0, 0, 0};
   for (int at = 0, turn = 0; at < a.batch; at += NT, turn ^= 1) {
@@ -168,7 +171,7 @@ __global__ void __launch_bounds__(NT) plan_kernel(PagesArgs a) {
       } else {
         a.back[b] = back;
       }
-      if (!near || !a.alone) a.taken[b] = taken;
+      if (!alone) a.taken[b] = taken;
     }
     sum = Counts{sum.back + all.back, sum.taken + all.taken, sum.rows + all.rows};
   }
@@ -247,14 +250,13 @@ __global__ void __launch_bounds__(NT) plan_kernel(PagesArgs a) {
     a.state[1] = max(taken - held, 0);
     a.start[a.batch] = held;           // for the second launch
   }
-  if (!a.alone) return;
+  if (!alone) return;                  // (alone: few sequences, whose sums are near)
   __syncthreads();
-  for (int i = tid; i < taken; i += NT) near ? take(a, near_taken, held, i) : take(a, a.taken, held, i);
+  for (int i = tid; i < taken; i += NT) take(a, near_taken, held, i);
   for (int r = tid; r < a.rows; r += NT) {
     int pos;
     int64_t slot;
-    if (near) row(a, near_cu, near_taken, held, r, pos, slot);
-    else row(a, a.cu, a.taken, held, r, pos, slot);
+    row(a, near_cu, near_taken, held, r, pos, slot);
     a.positions[r] = pos;
     a.slots[r] = slot;
   }
