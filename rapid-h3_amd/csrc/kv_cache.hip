@@ -7,11 +7,11 @@
 //
 // Both are bound by memory. A row of a head is 8 values in each of dim / 8 lanes (16-byte loads of 16-bit rows, 8 or 4 bytes of
 // codes); a workgroup takes 256 / (dim / 8) consecutive rows of one head after another, so that the codes it writes (a page holds a
-// head's positions back to back) and its scales are whole lines, while each read of a row is dim consecutive values. Rows of more
-// than the last cache's 256 MB are streamed past it (in 4 bits read back 178 -> 127 us: the codes stay in it; written 167 -> 160).
+// head's positions back to back) and its scales are whole lines, while each read of a row is dim consecutive values. 16-bit rows of more
+// than the last cache's 256 MB are streamed past it: read back always, written where their codes fit it (launch_rows).
 // Measured, K and V of 22,332 rows x 56 heads of 128, bf16 (a large copy moves 5.1 TB/s): 4 bits (0.81 GB each way) written in 160 us
-// (5.1 TB/s), read back in 126 (6.4); e4m3 (0.97 GB) written in 220 us (4.4), read back in 190 (5.1); 8 x 7,919 rows x 16 heads
-// int8 (0.79 GB) read back in 166 us. 16 rows of 8 heads: 3.9 and 2.8 us, the length of a few dependent loads.
+// (5.1 TB/s), read back in 126 (6.4); e4m3 (0.97 GB) written in 207 us (4.7), read back in 191 (5.1); 8 x 7,919 rows x 16 heads
+// int8 (0.79 GB) written in 150, read back in 158 us. 16 rows of 8 heads: 3.9 and 2.8 us, the length of a few dependent loads.
 #include "kv_rows.hpp"
 
 namespace rh3 {
@@ -88,20 +88,27 @@ __global__ void __launch_bounds__(NT) read_kernel(Cache c, Seqs s, void* __restr
         values<FMT>(*reinterpret_cast<const uint2*>(c.v + code), c.vs[scale], y);
       }
     }
-    if (once) {
-      store_row8_once<DT>(k, row * k_st + h * k_sh + 8 * l, x);
-      store_row8_once<DT>(v, row * v_st + h * v_sh + 8 * l, y);
-    } else {
-      store_row8<DT>(k, row * k_st + h * k_sh + 8 * l, x);
-      store_row8<DT>(v, row * v_st + h * v_sh + 8 * l, y);
-    }
+    auto store = [&](void* to, int64_t at, const float* values) {
+      if constexpr (DT != RH3_DTYPE_F32) {
+        if (once) return store_row8_once<DT>(to, at, values);
+      }
+      store_row8<DT>(to, at, values);
+    };
+    store(k, row * k_st + h * k_sh + 8 * l, x);
+    store(v, row * v_st + h * v_sh + 8 * l, y);
   }
 }
 
 template <bool WRITE, int FMT, int D>
 void launch_rows(int dtype, dim3 g, hipStream_t st, const Cache& c, const Seqs& s, void* k, int64_t k_st, int64_t k_sh, void* v,
                  int64_t v_st, int64_t v_sh) {
-  const bool once = 2 * static_cast<int64_t>(s.rows) * c.heads * D * (dtype == RH3_DTYPE_F32 ? 4 : 2) > LAST_CACHE;
+  // Streaming rows past the last cache, us without and with. Read back, so that the codes stay in it: 22,332 x 56 x 128 bf16 in 4 bits 172
+  // and 126, int8 204 and 192, 90,000 x 56 790 and 781, a reader of the rows behind it counted too 367 and 363. Written, so that the
+  // codes are all that is kept: 4 bits (160 MB of codes) 170 and 160, int8 18,000 x 56 (258 MB) 170 and 160; codes that do not fit
+  // gain nothing by it: int8 22,332 x 56 (320 MB) 208 and 224, 4 bits 45,000 x 56 (323 MB) 345 and 372. fp32 rows, of which a lane's
+  // two halves go one by one, lose: 12,000 x 56 written 188 and 220, read back 240 and 314.
+  const int64_t values = 2 * static_cast<int64_t>(s.rows) * c.heads * D, codes = FMT == FP4 ? values / 2 : values;
+  const bool once = dtype != RH3_DTYPE_F32 && 2 * values > LAST_CACHE && (!WRITE || codes <= LAST_CACHE);
   auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, g, dim3(NT), 0, st, c, s, k, k_st, k_sh, v, v_st, v_sh, once); };
   if constexpr (WRITE) {
     if (dtype == RH3_DTYPE_BF16) go(write_kernel<FMT, D, RH3_DTYPE_BF16>);

@@ -102,25 +102,25 @@ template <int DT>
 struct Raw {
   uint4 w[DT == RH3_DTYPE_F32 ? 2 : 1];
 };
-// once: rows that together are more than the last cache holds, which are best kept out of it
+// once: 16-bit rows that are best kept out of the last cache
 template <int DT>
 __device__ __forceinline__ Raw<DT> load_raw(const void* p, int64_t at, bool once = false) {
   Raw<DT> r;
   const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p) + at * (DT == RH3_DTYPE_F32 ? 4 : 2));
-#pragma unroll
-  for (int i = 0; i < (DT == RH3_DTYPE_F32 ? 2 : 1); ++i) r.w[i] = once ? ld_stream16(src + i) : src[i];
+  if constexpr (DT == RH3_DTYPE_F32) {
+    r.w[0] = src[0];
+    r.w[1] = src[1];
+  } else {
+    r.w[0] = once ? ld_stream16(src) : src[0];
+  }
   return r;
 }
-template <int DT>
+template <int DT>   // bf16 or fp16
 __device__ __forceinline__ void store_row8_once(void* p, int64_t at, const float* v) {
-  uint4 r[DT == RH3_DTYPE_F32 ? 2 : 1];
-  store_row8<DT>(r, 0, v);
-  uint4* to = reinterpret_cast<uint4*>(static_cast<uint8_t*>(p) + at * (DT == RH3_DTYPE_F32 ? 4 : 2));
-#pragma unroll
-  for (int i = 0; i < (DT == RH3_DTYPE_F32 ? 2 : 1); ++i) {
-    const u32x4_t t = {r[i].x, r[i].y, r[i].z, r[i].w};
-    __builtin_nontemporal_store(t, reinterpret_cast<u32x4_t*>(to + i));
-  }
+  uint4 r;
+  store_row8<DT>(&r, 0, v);
+  const u32x4_t t = {r.x, r.y, r.z, r.w};
+  __builtin_nontemporal_store(t, reinterpret_cast<u32x4_t*>(static_cast<uint16_t*>(p) + at));
 }
 constexpr int64_t LAST_CACHE = int64_t{256} << 20;
 template <int DT>
@@ -135,8 +135,8 @@ __device__ __forceinline__ void values_of(const Raw<DT>& r, float* x) {
 }
 
 // Workgroups for `rows` rows: along x the rows, along y as many heads side by side as it takes for 8 workgroups to a CU, or 32 where
-// that leaves a workgroup 8 heads (22,332 rows x 56 heads in 4 bits: written in 177 and 171 us, read in 192 and 178; 24,009 x 8:
-// 28.2 and 29.8, 24.9 and 24.1); the other heads are the workgroup's loop, which resolves a row's page once for all of them.
+// that leaves a workgroup 8 heads (22,332 rows x 56 heads in int8: written in 218 and 208 us, read in 202 and 193; in 4 bits 157
+// and 159, 128 and 127; 24,009 x 8: 28.2 and 29.8, 24.9 and 24.1); the other heads are the workgroup's loop, which resolves a row's page once for all of them.
 inline dim3 grid_of(int64_t rows, int heads, int dim) {
   const int64_t gx = (rows + NT / (dim / 8) - 1) / (NT / (dim / 8));
   const int64_t cus = device_cus() > 0 ? device_cus() : 256;
