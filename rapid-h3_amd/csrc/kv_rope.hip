@@ -13,7 +13,8 @@
 // the heads, 16 rows of 128 at a time (64: 32); a row is 8 channels in each of dim / 8 lanes, which keep their token and so the
 // cosines and sines of their channels in registers. The 8 are 4 and the 4 that they turn with, so no lane needs another's (8
 // neighbours, and their partners loaded and normed a second time: 305 us for the next line's 272, the vector units 71 % busy); keys
-// on their way into a cache are 8 neighbours, as their codes lie. Rows of more than the last cache holds are streamed past it.
+// on their way into a cache are 8 neighbours, as their codes lie. (Rows of more than the last cache holds streamed past it take the
+// same time, 16 and 32 bits, alone, with a reader behind them and on their way into a cache.)
 // Measured: 22,332 rows x 112 heads of 128, bf16, 96 channels turned, normed (1.28 GB) 272 us, 4.7 TB/s (a large copy moves 5.1), the
 // vector units 64 % busy; 24,009 rows x 56 query heads and 8 K/V heads, fp16, 64 channels turned, into an int8 cache (0.84 GB) 190 us,
 // 4.4 TB/s. 8 rows x 40 heads 4.4 us, 24 x 48 into a 4-bit cache 5.2: a few dependent loads, the cosines and a barrier.
@@ -38,7 +39,7 @@ struct RopeArgs {
   Turn t;
   rh3_head_rows q, k, v;             // v: not of FMT NONE
   rh3_head_rows qo, ko;              // ko: of FMT NONE
-  int q_heads, k_heads, rows, log2tt, once;
+  int q_heads, k_heads, rows, log2tt;
   int first;                         // added to the positions of the cache's rows
   const int32_t* positions;          // FMT NONE
   Cache c;
@@ -110,15 +111,13 @@ struct Raw4 {
   uint32_t w[DT == RH3_DTYPE_F32 ? 4 : 2];
 };
 template <int DT>
-__device__ __forceinline__ Raw4<DT> load_raw4(const void* p, int64_t at, bool once) {
+__device__ __forceinline__ Raw4<DT> load_raw4(const void* p, int64_t at) {
   Raw4<DT> r;
   if constexpr (DT == RH3_DTYPE_F32) {
-    const u32x4_t* src = reinterpret_cast<const u32x4_t*>(static_cast<const float*>(p) + at);
-    const u32x4_t x = once ? __builtin_nontemporal_load(src) : *src;
+    const u32x4_t x = *reinterpret_cast<const u32x4_t*>(static_cast<const float*>(p) + at);
     r.w[0] = x[0]; r.w[1] = x[1]; r.w[2] = x[2]; r.w[3] = x[3];
   } else {
-    const u32x2_t* src = reinterpret_cast<const u32x2_t*>(static_cast<const uint16_t*>(p) + at);
-    const u32x2_t x = once ? __builtin_nontemporal_load(src) : *src;
+    const u32x2_t x = *reinterpret_cast<const u32x2_t*>(static_cast<const uint16_t*>(p) + at);
     r.w[0] = x[0]; r.w[1] = x[1];
   }
   return r;
@@ -144,17 +143,13 @@ __device__ __forceinline__ void values_of(const Raw4<DT>& r, float* x) {
   }
 }
 template <int DT>
-__device__ __forceinline__ void store4(void* p, int64_t at, const float* x, bool once) {
+__device__ __forceinline__ void store4(void* p, int64_t at, const float* x) {
   if constexpr (DT == RH3_DTYPE_F32) {
     const u32x4_t r = {__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3])};
-    u32x4_t* to = reinterpret_cast<u32x4_t*>(static_cast<float*>(p) + at);
-    if (once) __builtin_nontemporal_store(r, to);
-    else *to = r;
+    *reinterpret_cast<u32x4_t*>(static_cast<float*>(p) + at) = r;
   } else {
     const u32x2_t r = DT == RH3_DTYPE_BF16 ? u32x2_t{pack_bf2(x[0], x[1]), pack_bf2(x[2], x[3])} : u32x2_t{pack_h2(x[0], x[1]), pack_h2(x[2], x[3])};
-    u32x2_t* to = reinterpret_cast<u32x2_t*>(static_cast<uint16_t*>(p) + at);
-    if (once) __builtin_nontemporal_store(r, to);
-    else *to = r;
+    *reinterpret_cast<u32x2_t*>(static_cast<uint16_t*>(p) + at) = r;
   }
 }
 template <int DT, int N>
@@ -165,9 +160,9 @@ __device__ __forceinline__ void weights_of(const Turn& t, const void* w, int at,
 #pragma unroll
       for (int e = 0; e < 4; ++e) x[i + e] = 1.0f;
     } else if (t.wide) {
-      values_of<RH3_DTYPE_F32>(load_raw4<RH3_DTYPE_F32>(w, at + i, false), x + i);
+      values_of<RH3_DTYPE_F32>(load_raw4<RH3_DTYPE_F32>(w, at + i), x + i);
     } else {
-      values_of<DT>(load_raw4<DT>(w, at + i, false), x + i);
+      values_of<DT>(load_raw4<DT>(w, at + i), x + i);
     }
   }
 }
@@ -211,8 +206,8 @@ __global__ void __launch_bounds__(NT, FMT == NONE || DT == RH3_DTYPE_F32 ? 4 : 5
     if (mine && g < plain && h < (key ? a.k_heads : a.q_heads)) {
       const rh3_head_rows& r = key ? a.k : a.q;
       const int64_t at = row * r.st + h * r.sh;
-      r0 = load_raw4<DT>(r.x, at + c0, a.once);
-      r1 = load_raw4<DT>(r.x, at + c1, a.once);
+      r0 = load_raw4<DT>(r.x, at + c0);
+      r1 = load_raw4<DT>(r.x, at + c1);
     }
   };
   Raw4<DT> raw0{}, raw1{};
@@ -285,8 +280,8 @@ __global__ void __launch_bounds__(NT, FMT == NONE || DT == RH3_DTYPE_F32 ? 4 : 5
         }
         const rh3_head_rows& o = key ? a.ko : a.qo;
         const int64_t at = row * o.st + h * o.sh;
-        store4<DT>(o.x, at + c0, x, a.once);
-        store4<DT>(o.x, at + c1, x + 4, a.once);
+        store4<DT>(o.x, at + c0, x);
+        store4<DT>(o.x, at + c1, x + 4);
       }
       raw0 = next0;
       raw1 = next1;
@@ -402,7 +397,6 @@ template <int FMT, int D>
 int launch_rope(const char* name, RopeArgs& a, int64_t dtype, hipStream_t st) {
   const int64_t cus = device_cus() > 0 ? device_cus() : 256;
   a.log2tt = a.rows < 4 * cus ? 0 : 2;
-  a.once = static_cast<int64_t>(a.rows) * (a.q_heads + a.k_heads) * D * (dtype == RH3_DTYPE_F32 ? 4 : 2) > LAST_CACHE;
   const int at_once = NT / (D / 8) >> a.log2tt;
   const int64_t gx = (static_cast<int64_t>(a.rows) + (1 << a.log2tt) - 1) >> a.log2tt;
   const int64_t groups = (a.q_heads + at_once - 1) / at_once + (a.k_heads + at_once - 1) / at_once;
