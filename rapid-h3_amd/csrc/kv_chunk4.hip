@@ -16,8 +16,9 @@
 // The keys are taken by halves of 32: while one half's softmax runs, so do the MFMAs of the next half's scores and of the half
 // before's values. Where keys are masked, a page is absent or a reference has to move, a plain path does the half.
 // Vector work per score: one fma (softmax scale and reference at once), the exponential, the sum and half a conversion.
-// Roundings: the probability to bf16, 2^-8 relative at most, as a bf16 result's own. FINE, for fp16 results: the queries, which
-// bf16 does not hold, and the probabilities in two terms each (2^-16).
+// Roundings: the probability to bf16, 2^-8 relative at most, as a bf16 result's own: on random rows a result is off by 2.34e-3 (relative
+// to all values' norm) for the 1.66e-3 of its own rounding alone. Two terms, which leave 1.66e-3, are a half more matrix work: the first
+// size took 668 us for 480. FINE, for fp16 results: the queries, which bf16 does not hold, and the probabilities in two terms each (2^-16).
 #include "kv_four.hpp"
 
 namespace rh3 {

@@ -12,8 +12,8 @@
 // Bound by latency: a step moves 9 bytes a sequence, 12 a row and 8 a page. The sums need one workgroup: it makes them, walks the
 // pages that come back (8 entries to a thread at a time, in order) and, of small calls, does the rest too; of large ones a second
 // launch spreads the pages taken and the rows over the chip. A page that is taken is looked up in the list, not in the table, which
-// the same launch is writing. Measured: 16 sequences, a row each, 5.8 us; 700 sequences, 9,000 pages back, 8,000 taken, 130,000
-// rows 10.9 + 4 to 5.5 us (with each entry's search on its own 15.4 + 5.3).
+// the same launch is writing. Measured: 16 sequences, a row each, 5.6 us; 700 sequences, 7,698 pages back, 10,112 taken, 161,371
+// rows 10.8 + 5.3 us (with each entry's search on its own 15.4 + 5.3), of which the pages that come back are 6.5.
 #include "kv_common.hpp"
 
 namespace rh3 {

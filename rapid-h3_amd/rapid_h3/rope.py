@@ -1,7 +1,7 @@
 """Position rotations of queries and keys, and their RMS norm for each head in the same pass (librh3: rh3_qk_norm_rope), for rows at
 any positions: heads of 64 or 128 channels, as many query heads as there are, rotated whole or in part. With the write into a
-key / value cache in the same pass: kvcache.kv_write_rope. (attention.rms_rope_ is the DiT block's form: a table of bf16 coefficients
-for tokens 0 .. S, the norm's result rounded in between.)
+key / value cache in the same pass: kvcache.kv_write_rope. A row has one position. (attention.rms_rope_ is the DiT block's form: a table
+of bf16 coefficients for tokens 0 .. S, which may turn by positions on several axes, the norm's result rounded in between.)
 
 Of a row x of a head: y = (x * r) * w with r = 1 / sqrt(mean x^2 + eps), made in 64 bits and rounded to fp32 once; then pairs (a, b) of
 the first rot channels become (a cos - b sin, b cos + a sin) in fp32, with the cosine and sine of position * freq[i] (a product in
@@ -52,7 +52,8 @@ def frequencies(rot, base=10000.0, scaling=None, stretch=1.0, original=None, low
       "linear"  all divided by stretch (positions squeezed together)
       "base"    base * stretch ** (rot / (rot - 2)): the lowest frequency is divided by stretch, the highest stays
       "parts"   by how often a frequency turns within the original length: over `high` times it stays, under `low` it is divided by
-                stretch, a straight line in between; factor 0.1 ln(stretch) + 1"""
+                stretch, a straight line in between; factor 0.1 ln(stretch) + 1. (The line is over the number of turns. Models that draw
+                it over the channel's number, or have another factor or none, give Rotary their own frequencies and factor.)"""
     if rot < 4 or rot % 2:
         raise ValueError(f"frequencies: rot {rot} (an even number from 4 on)")
     if scaling not in (None, "linear", "base", "parts"):
