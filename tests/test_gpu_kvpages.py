@@ -149,6 +149,67 @@ def test_drafts_and_a_pool_that_runs_out(dev):
     assert cu.tolist() == [0, 0, 3] and lens.tolist() == [0, 3] and pool.state.tolist() == [5, 0] and (table[0] == -1).all()
 
 
+def test_captured_steps_that_take_rows_back(dev):
+    """A captured step takes rows back on the replays whose numbers say so."""
+    pages, page, b, w, rows = 60, 16, 6, 8, 250
+    pool, lists = kv.kv_pages(pages, page, dev), Cut(pages, page, b, w)
+    table, lens = torch.full((b, w), -1, dtype=torch.int32, device=dev), torch.zeros(b, dtype=torch.int32, device=dev)
+    new, done = torch.zeros(b, dtype=torch.int32, device=dev), torch.zeros(b, dtype=torch.bool, device=dev)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = kv.kv_extend(pool, table, lens, new, rows, done)
+    r = random.Random(8)
+    for replay in range(8):
+        n, d = [r.randint(-20 if replay else 0, 40) for _ in range(b)], [replay > 2 and r.random() < 0.2 for _ in range(b)]
+        new.copy_(_i32(n, dev))
+        done.copy_(torch.tensor(d, device=dev))
+        graph.replay()
+        torch.cuda.synchronize()
+        for x, y in zip(got, lists.extend(n, rows, d)):
+            assert x.tolist() == y, replay
+        _same(pool, table, lens, lists)
+
+
+@pytest.mark.parametrize("fmt", [torch.int8, torch.float4_e2m1fn_x2])
+def test_drafts_that_are_not_accepted_leave_nothing(dev, fmt):
+    """A batch whose every step writes and attends three drafted rows to each sequence, of which one to three are kept: what the kept rows gave,
+    and what a step over the whole history then gives, are the bits of a batch that never drafted."""
+    b, hq, hkv, dim, page, pages, w, steps = 3, 4, 2, 64, 16, 24, 6, 12
+    turn = rope.rotary(dim, "half", dev)
+    r = random.Random(5)
+    kept = [[r.randint(1, 3) for _ in range(b)] for _ in range(steps)]
+    kept[0] = [3, 3, 3]
+    g = torch.Generator().manual_seed(6)
+    most = 3 * steps
+    whole = [torch.randn(b, most, h, dim, generator=g).to(torch.bfloat16).to(dev) for h in (hq, hkv, hkv)]
+    other = [torch.randn(b, 3, h, dim, generator=g).to(torch.bfloat16).to(dev) for h in (hq, hkv, hkv)]    # of drafts that are wrong
+
+    def run(drafts):
+        cache, pool = kv.kv_cache(pages, hkv, page, dim, fmt, dev), kv.kv_pages(pages, page, dev)
+        table, lens = torch.full((b, w), -1, dtype=torch.int32, device=dev), torch.zeros(b, dtype=torch.int32, device=dev)
+        at, outs = [0] * b, []
+        for keep in kept:
+            n = [3] * b if drafts else keep
+            q, k, v = (torch.cat([torch.cat([x[i, at[i]:at[i] + keep[i]], y[i, keep[i]:n[i]]]) for i in range(b)]) for x, y in zip(whole, other))
+            cu, _, slots = kv.kv_extend(pool, table, lens, _i32(n, dev), sum(n))
+            assert (slots >= 0).all()
+            out = kv.kv_attention(kv.kv_write_rope(cache, q, k, v, table, lens, cu, turn), cache, table, lens, cu, form="token")
+            first = cu.tolist()
+            outs += [out[first[i]:first[i] + keep[i]] for i in range(b)]
+            if drafts:
+                kv.kv_extend(pool, table, lens, _i32([a - c for a, c in zip(keep, n)], dev), 0)
+            at = [a + c for a, c in zip(at, keep)]
+            assert lens.tolist() == at and int(pool.state[0]) == pages - sum(-(-a // page) for a in at)
+        q = torch.cat([whole[0][i, :1] for i in range(b)])
+        return outs, kv.kv_attention(q, cache, table, lens, form="token")
+    (a, last_a), (c, last_c) = run(True), run(False)
+    assert torch.equal(last_a, last_c)
+    for x, y in zip(a, c):
+        # other rows beside a row may change its last bits: on either side the result's rounding, 2^-8 of it, and one of each weight to f16
+        # or finer, 2^-11 of the largest value
+        assert ((x.double() - y.double()).abs() <= 2.0 ** -7 * y.double().abs() + 2.0 ** -10 * float(whole[2].abs().max())).all()
+
+
 def test_bad_contents_stay_inside(dev):
     """Counts beyond the list, negative lengths and rows, entries that are no pages, pages given back twice."""
     b, w, pages, page = 4, 3, 6, 16
