@@ -69,8 +69,8 @@ __device__ __forceinline__ void query8(const uint4 raw, b8_t& hi, b8_t& lo) {
 // rose just so far that the reference stayed 2^4; at SUM_MOST it moves up by LATER. So a row's sum over the 16 lanes that share it in
 // a workgroup is under 0.1, its values' sum, not yet divided, under 0.1 of the largest of them, and fp32 holds both, and the join of all
 // workgroups' times PART, up to the largest value there is (1.5 * 2^127) for any number of keys. Values down to 2^-94 keep their bits
-// (2^-82 after one LATER: 2^17 equal scores and more). (From 2^28 on, a score's last place is more than OVER: the reference is then the maximum itself, or the next
-// number, and does not move for a sum's sake.)
+// (2^-82 after one LATER: 2^17 equal scores and more). (From 2^28 on, a score's last place is more than OVER: the reference is then
+// the maximum itself, or the next number, and does not move for a sum's sake.)
 constexpr float OVER = 24.0f;
 constexpr float STALE = -12.0f;
 constexpr float SUM_MOST = 0x1p-8f;

@@ -136,7 +136,8 @@ __device__ __forceinline__ void values_of(const Raw<DT>& r, float* x) {
 
 // Workgroups for `rows` rows: along x the rows, along y as many heads side by side as it takes for 8 workgroups to a CU, or 32 where
 // that leaves a workgroup 8 heads (22,332 rows x 56 heads in int8: written in 218 and 208 us, read in 202 and 193; in 4 bits 157
-// and 159, 128 and 127; 24,009 x 8: 28.2 and 29.8, 24.9 and 24.1); the other heads are the workgroup's loop, which resolves a row's page once for all of them.
+// and 159, 128 and 127; 24,009 x 8: 28.2 and 29.8, 24.9 and 24.1); the other heads are the workgroup's loop, which resolves a row's
+// page once for all of them.
 inline dim3 grid_of(int64_t rows, int heads, int dim) {
   const int64_t gx = (rows + NT / (dim / 8) - 1) / (NT / (dim / 8));
   const int64_t cus = device_cus() > 0 ? device_cus() : 256;
